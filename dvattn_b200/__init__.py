@@ -4,7 +4,9 @@ Importing the package loads ``dvatt.abi3.so``, which registers the reference's
 ``torch.ops.libdvatt`` schemas (``dvattn_paged_sdpa``, ``dvattn_varlen_paged_sdpa``,
 ``dvattn_rope``, ``dvattn_varlen_rope``, ``dvattn_sdpa``, ``dvattn_fused``) plus the B200
 additions (``dvattn_paged_sdpa_ex``, ``dvattn_varlen_paged_sdpa_ex``, ``dvattn_lse_merge``,
-``dvattn_paged_append``, ``dvattn_build_views`` and the ``*_rope`` attention variants).  There is no CPU fallback: if the native libraries are missing,
+``dvattn_paged_append``, ``dvattn_build_views``, the ``*_rope`` attention variants, the draft-tree
+``dvattn_tree_sdpa`` / ``dvattn_tree_append`` and the bounded-cache ``dvattn_paged_mass`` /
+``dvattn_paged_evict``).  There is no CPU fallback: if the native libraries are missing,
 the import fails.
 """
 from __future__ import annotations
@@ -34,10 +36,14 @@ from .api import (  # noqa: E402
     dvattn_fused,
     dvattn_lse_merge,
     dvattn_paged_append,
+    dvattn_paged_evict,
+    dvattn_paged_mass,
     dvattn_paged_sdpa,
     dvattn_paged_sdpa_rope,
     dvattn_rope,
     dvattn_sdpa,
+    dvattn_tree_append,
+    dvattn_tree_sdpa,
     dvattn_varlen_paged_sdpa,
     dvattn_varlen_paged_sdpa_rope,
     dvattn_varlen_rope,
@@ -50,10 +56,14 @@ __all__ = [
     "dvattn_fused",
     "dvattn_lse_merge",
     "dvattn_paged_append",
+    "dvattn_paged_evict",
+    "dvattn_paged_mass",
     "dvattn_paged_sdpa",
     "dvattn_paged_sdpa_rope",
     "dvattn_rope",
     "dvattn_sdpa",
+    "dvattn_tree_append",
+    "dvattn_tree_sdpa",
     "dvattn_varlen_paged_sdpa",
     "dvattn_varlen_paged_sdpa_rope",
     "dvattn_varlen_rope",

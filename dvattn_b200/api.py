@@ -150,6 +150,70 @@ def dvattn_paged_append(k_cache: torch.Tensor, v_cache: torch.Tensor, keys: torc
     _ops.dvattn_paged_append(k_cache, v_cache, keys, values, cosines, sines, block_tables, positions, counts)
 
 
+def dvattn_tree_sdpa(queries: torch.Tensor, parents: torch.Tensor, locations: torch.Tensor, cosines: torch.Tensor,
+                     sines: torch.Tensor, fragment_lengths: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     block_tables: torch.Tensor, draft_keys: torch.Tensor, draft_values: torch.Tensor, scale: float,
+                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A tree of S drafted tokens per sequence attends over the paged multi-turn cache and
+    over itself, in one pass over the cache.  queries [W,Hq,S,E] and draft_keys /
+    draft_values [W,Hkv,S,E] (keys unrotated); parents [W,S] i32: the index of each token's
+    parent among the S (before it), -1 for a child of the cached context, -2 for no token
+    (padding; gets zeros).  locations [F,W,S] i32: the last cached key of each turn that the
+    token sees (not its own position); cos/sin [F,W,S,R] f32 rotate its query for each turn,
+    those of the last turn its key as well.  -> out [W,Hq,S,E]; ``lse`` ([W,Hq,S] f32) is an
+    optional extra output.  The cache is not written (``dvattn_tree_append`` does that for
+    the accepted tokens)."""
+    if out is None:
+        out = torch.empty(queries.shape[:3] + (v_cache.size(3),), dtype=queries.dtype, device=queries.device)
+    _ops.dvattn_tree_sdpa(out, lse, scale, parents, locations, queries, cosines, sines, fragment_lengths, k_cache,
+                          v_cache, block_tables, draft_keys, draft_values)
+    return out
+
+
+def dvattn_tree_append(k_cache: torch.Tensor, v_cache: torch.Tensor, draft_keys: torch.Tensor,
+                       draft_values: torch.Tensor, cosines: torch.Tensor, sines: torch.Tensor,
+                       block_tables: torch.Tensor, positions: torch.Tensor, accepted: torch.Tensor,
+                       counts: Optional[torch.Tensor] = None) -> None:
+    """Write the accepted tokens of a drafted tree into the paged cache: for i < counts[w]
+    (None: all) drafted token accepted[w, i] of sequence w goes to logical position
+    positions[w] + i, its key rotated with cos/sin [W,S,R] f32 (the last turn's angles of
+    ``dvattn_tree_sdpa``) as ``dvattn_paged_append`` rotates.  draft_keys / draft_values
+    [W,Hkv,S,E], accepted [W,A] i32, positions and counts [W] i32."""
+    _ops.dvattn_tree_append(k_cache, v_cache, draft_keys, draft_values, cosines, sines, block_tables, positions,
+                            accepted, counts)
+
+
+def dvattn_paged_mass(mass: torch.Tensor, queries: torch.Tensor, lse: torch.Tensor, locations: torch.Tensor,
+                      cosines: torch.Tensor, sines: torch.Tensor, fragment_lengths: torch.Tensor,
+                      k_cache: torch.Tensor, block_tables: torch.Tensor, scale: float) -> torch.Tensor:
+    """Add the attention weight that every cached key received from the queries to ``mass``
+    [W,Hkv,N] f32 (by logical position; in place): mass[w,h,p] += sum over the queries and
+    the query heads of h of exp(scale * q.k_p - lse).  queries, locations and cos/sin as in
+    the attention call that returned ``lse`` [W,Hq,S] f32; a query whose lse is -inf (a token
+    that is not there, or one that was rejected) adds nothing."""
+    _ops.dvattn_paged_mass(mass, scale, locations, queries, lse, cosines, sines, fragment_lengths, k_cache,
+                           block_tables)
+    return mass
+
+
+def dvattn_paged_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor, block_tables: torch.Tensor,
+                       starts: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor, sink: int = 0, recent: int = 0,
+                       mass_out: Optional[torch.Tensor] = None, source: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Keep keep[w] of the lengths[w] tokens at logical positions starts[w] + i of every
+    sequence (i32 [W] each): per KV head the first ``sink``, the last ``recent``, then those of
+    largest ``mass`` [W,Hkv,N] (NaN last, equal ones by position).  Survivors in front of
+    keep[w] stay, the freed positions there are filled by the survivors behind, in order;
+    their K and V rows move with them, and keys carry their own rotation, so attention over
+    the kept positions follows.  Returns ``mass_out`` (default: ``mass``, in place), moved
+    alike, 0 where keys left; ``source`` ([W,Hkv,N] i32, optional) gets the position that
+    each position's key came from, -1 where keys left.  The pages of the range must belong to
+    sequence w alone."""
+    if mass_out is None:
+        mass_out = mass
+    _ops.dvattn_paged_evict(k_cache, v_cache, mass, mass_out, source, block_tables, starts, lengths, keep, sink, recent)
+    return mass_out
+
+
 def dvattn_rope(queries: torch.Tensor, cosines: torch.Tensor, sines: torch.Tensor, out=None) -> torch.Tensor:
     """Same signature as python/dvattn/attention.py:68-72: out [F,W,Hq,S,E]."""
     if out is None:

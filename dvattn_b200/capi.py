@@ -65,6 +65,13 @@ EXPORTS = [
     "dvattn_paged_sdpa_rope",
     "dvattn_varlen_paged_sdpa_rope_workspace_size",
     "dvattn_varlen_paged_sdpa_rope",
+    "dvattn_tree_sdpa_workspace_size",
+    "dvattn_tree_sdpa",
+    "dvattn_tree_append",
+    "dvattn_paged_mass_workspace_size",
+    "dvattn_paged_mass",
+    "dvattn_paged_evict_workspace_size",
+    "dvattn_paged_evict",
 ]
 
 _vp = ctypes.c_void_p
@@ -112,6 +119,36 @@ class ViewsArgs(ctypes.Structure):
 class RotaryArgs(ctypes.Structure):
     _fields_ = [("rope_base", ctypes.c_float), ("attention_scaling", ctypes.c_float), ("round_dtype", _i),
                 ("inv_freq", _vp)]
+
+
+class TreeArgs(ctypes.Structure):
+    _fields_ = [("dtype", _i), ("F", _i), ("W", _i), ("Hq", _i), ("Hkv", _i), ("E", _i), ("Ev", _i), ("S", _i),
+                ("R", _i), ("block_size", _i), ("max_blocks_per_seq", _i), ("num_blocks", ctypes.c_longlong),
+                ("scale", ctypes.c_float), ("out", _vp), ("queries", _vp), ("parents", _vp), ("cosines", _vp),
+                ("sines", _vp), ("locations", _vp), ("fragment_lengths", _vp), ("k_cache", _vp), ("v_cache", _vp),
+                ("block_tables", _vp), ("draft_keys", _vp), ("draft_values", _vp), ("lse_out", _vp)]
+
+
+class TreeAppendArgs(ctypes.Structure):
+    _fields_ = [("dtype", _i), ("W", _i), ("Hkv", _i), ("E", _i), ("Ev", _i), ("S", _i), ("A", _i), ("R", _i),
+                ("block_size", _i), ("max_blocks_per_seq", _i), ("num_blocks", ctypes.c_longlong),
+                ("k_cache", _vp), ("v_cache", _vp), ("draft_keys", _vp), ("draft_values", _vp), ("cosines", _vp),
+                ("sines", _vp), ("block_tables", _vp), ("positions", _vp), ("accepted", _vp), ("counts", _vp)]
+
+
+class MassArgs(ctypes.Structure):
+    _fields_ = [("dtype", _i), ("F", _i), ("W", _i), ("Hq", _i), ("Hkv", _i), ("E", _i), ("S", _i), ("R", _i),
+                ("block_size", _i), ("max_blocks_per_seq", _i), ("num_blocks", ctypes.c_longlong),
+                ("positions", ctypes.c_longlong), ("scale", ctypes.c_float), ("mass", _vp), ("queries", _vp),
+                ("lse", _vp), ("cosines", _vp), ("sines", _vp), ("locations", _vp), ("fragment_lengths", _vp),
+                ("k_cache", _vp), ("block_tables", _vp)]
+
+
+class EvictArgs(ctypes.Structure):
+    _fields_ = [("dtype", _i), ("W", _i), ("Hkv", _i), ("E", _i), ("Ev", _i), ("block_size", _i),
+                ("max_blocks_per_seq", _i), ("sink", _i), ("recent", _i), ("num_blocks", ctypes.c_longlong),
+                ("positions", ctypes.c_longlong), ("k_cache", _vp), ("v_cache", _vp), ("mass", _vp), ("mass_out", _vp),
+                ("source", _vp), ("block_tables", _vp), ("starts", _vp), ("lengths", _vp), ("keep", _vp)]
 
 
 _lib: Optional[ctypes.CDLL] = None
@@ -185,6 +222,12 @@ def lib() -> ctypes.CDLL:
                                                     ctypes.c_size_t, _vp]
         L.dvattn_build_views.restype = _i
         L.dvattn_build_views.argtypes = [ctypes.POINTER(ViewsArgs), _vp]
+        for name, args in (("dvattn_tree_sdpa", TreeArgs), ("dvattn_paged_mass", MassArgs), ("dvattn_paged_evict", EvictArgs)):
+            size, call = getattr(L, name + "_workspace_size"), getattr(L, name)
+            size.restype, size.argtypes = ctypes.c_size_t, [ctypes.POINTER(args)]
+            call.restype, call.argtypes = _i, [ctypes.POINTER(args), _vp, ctypes.c_size_t, _vp]
+        L.dvattn_tree_append.restype = _i
+        L.dvattn_tree_append.argtypes = [ctypes.POINTER(TreeAppendArgs), _vp]
         _lib = L
     return _lib
 
@@ -555,3 +598,62 @@ def varlen_paged_sdpa_rope(out, scale, locations, queries, fragment_lengths, k_c
     if st != DVATTN_OK:
         raise DvattnError(st, "dvattn_varlen_paged_sdpa_rope")
     return out
+
+
+def _with_workspace(name, args, device, workspace=None):
+    """Call a (args, workspace, bytes, stream) entry point on the current stream; the
+    workspace used is returned (its error word: workspace_status)."""
+    if workspace is None:
+        n = getattr(lib(), name + "_workspace_size")(ctypes.byref(args))
+        workspace = torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+    st = getattr(lib(), name)(ctypes.byref(args), workspace.data_ptr(), workspace.numel(), _stream(None))
+    if st != DVATTN_OK:
+        raise DvattnError(st, name)
+    return workspace
+
+
+def tree_sdpa(out, scale, parents, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, block_tables,
+              draft_keys, draft_values, lse=None, workspace=None):
+    """dvattn_tree_sdpa through the C ABI; returns the workspace."""
+    W, Hq, S, E = queries.shape
+    a = TreeArgs(_DTYPE.get(out.dtype, -1), locations.size(0), W, Hq, k_cache.size(2), E, v_cache.size(3), S,
+                 cosines.size(3), k_cache.size(1), block_tables.size(1), k_cache.size(0), float(scale), out.data_ptr(),
+                 queries.data_ptr(), parents.data_ptr(), _ptr(cosines), _ptr(sines), locations.data_ptr(),
+                 fragment_lengths.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
+                 draft_keys.data_ptr(), draft_values.data_ptr(), _ptr(lse))
+    return _with_workspace("dvattn_tree_sdpa", a, out.device, workspace)
+
+
+def tree_append(k_cache, v_cache, draft_keys, draft_values, cosines, sines, block_tables, positions, accepted,
+                counts=None):
+    """dvattn_tree_append through the C ABI."""
+    W, Hkv, S, E = draft_keys.shape
+    a = TreeAppendArgs(_DTYPE.get(k_cache.dtype, -1), W, Hkv, E, draft_values.size(3), S, accepted.size(1),
+                       cosines.size(2), k_cache.size(1), block_tables.size(1), k_cache.size(0), k_cache.data_ptr(),
+                       v_cache.data_ptr(), draft_keys.data_ptr(), draft_values.data_ptr(), _ptr(cosines), _ptr(sines),
+                       block_tables.data_ptr(), positions.data_ptr(), accepted.data_ptr(), _ptr(counts))
+    st = lib().dvattn_tree_append(ctypes.byref(a), _stream(None))
+    if st != DVATTN_OK:
+        raise DvattnError(st, "dvattn_tree_append")
+
+
+def paged_mass(mass, scale, locations, queries, lse, cosines, sines, fragment_lengths, k_cache, block_tables,
+               workspace=None):
+    """dvattn_paged_mass through the C ABI; returns the workspace."""
+    W, Hq, S, E = queries.shape
+    a = MassArgs(_DTYPE.get(queries.dtype, -1), locations.size(0), W, Hq, k_cache.size(2), E, S, cosines.size(3),
+                 k_cache.size(1), block_tables.size(1), k_cache.size(0), mass.size(2), float(scale), mass.data_ptr(),
+                 queries.data_ptr(), lse.data_ptr(), _ptr(cosines), _ptr(sines), locations.data_ptr(),
+                 fragment_lengths.data_ptr(), k_cache.data_ptr(), block_tables.data_ptr())
+    return _with_workspace("dvattn_paged_mass", a, mass.device, workspace)
+
+
+def paged_evict(k_cache, v_cache, mass, block_tables, starts, lengths, keep, sink=0, recent=0, mass_out=None,
+                source=None, workspace=None):
+    """dvattn_paged_evict through the C ABI (mass_out None: in place); returns the workspace."""
+    W, Hkv, N = mass.shape
+    a = EvictArgs(_DTYPE.get(k_cache.dtype, -1), W, Hkv, k_cache.size(3), v_cache.size(3), k_cache.size(1),
+                  block_tables.size(1), sink, recent, k_cache.size(0), N, k_cache.data_ptr(), v_cache.data_ptr(),
+                  mass.data_ptr(), (mass if mass_out is None else mass_out).data_ptr(), _ptr(source),
+                  block_tables.data_ptr(), starts.data_ptr(), lengths.data_ptr(), keep.data_ptr())
+    return _with_workspace("dvattn_paged_evict", a, mass.device, workspace)

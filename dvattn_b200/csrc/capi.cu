@@ -78,6 +78,28 @@ int dvattn_paged_append(const dvattn_append_args* args, dvattn_stream_t stream) 
     return dvb::paged_append_launch(args, reinterpret_cast<cudaStream_t>(stream));
 }
 
+size_t dvattn_tree_sdpa_workspace_size(const dvattn_tree_args* args) { return dvb::tree_workspace_size(args); }
+
+int dvattn_tree_sdpa(const dvattn_tree_args* args, void* workspace, size_t workspace_bytes, dvattn_stream_t stream) {
+    return dvb::tree_launch(args, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int dvattn_tree_append(const dvattn_tree_append_args* args, dvattn_stream_t stream) {
+    return dvb::tree_append_launch(args, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t dvattn_paged_mass_workspace_size(const dvattn_mass_args* args) { return dvb::mass_workspace_size(args); }
+
+int dvattn_paged_mass(const dvattn_mass_args* args, void* workspace, size_t workspace_bytes, dvattn_stream_t stream) {
+    return dvb::mass_launch(args, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t dvattn_paged_evict_workspace_size(const dvattn_evict_args* args) { return dvb::evict_workspace_size(args); }
+
+int dvattn_paged_evict(const dvattn_evict_args* args, void* workspace, size_t workspace_bytes, dvattn_stream_t stream) {
+    return dvb::evict_launch(args, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
 size_t dvattn_sdpa_workspace_size(const dvattn_sdpa_args* args) { return dvb::sdpa_workspace_size(args); }
 
 int dvattn_sdpa(const dvattn_sdpa_args* args, void* workspace, size_t workspace_bytes, dvattn_stream_t stream) {

@@ -27,6 +27,16 @@ int varlen_rope_attn_launch(const dvattn_varlen_args* a, const dvattn_rotary_arg
                             cudaStream_t stream);
 // paged KV append with fused K rotation (append.cu)
 int paged_append_launch(const dvattn_append_args* a, cudaStream_t stream);
+// the accepted tokens of a drafted tree appended (append.cu)
+int tree_append_launch(const dvattn_tree_append_args* a, cudaStream_t stream);
+// attention of a drafted tree (tree.cu)
+size_t tree_workspace_size(const dvattn_tree_args* a);
+int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaStream_t stream);
+// accumulated attention weight of the cached keys (mass.cu), eviction by it (evict.cu)
+size_t mass_workspace_size(const dvattn_mass_args* a);
+int mass_launch(const dvattn_mass_args* a, void* workspace, size_t wbytes, cudaStream_t stream);
+size_t evict_workspace_size(const dvattn_evict_args* a);
+int evict_launch(const dvattn_evict_args* a, void* workspace, size_t wbytes, cudaStream_t stream);
 // contiguous fragments (the dvattn_sdpa op)
 size_t sdpa_workspace_size(const dvattn_sdpa_args* a);
 int sdpa_launch(const dvattn_sdpa_args* a, void* workspace, size_t wbytes, cudaStream_t stream);

@@ -1,0 +1,300 @@
+// Accumulated attention weight: how much of the softmax every cached key received.
+//
+//   mass[w, h, off_f + l] += sum over the query heads g of KV head h and the queries s of
+//   exp(scale * q_f[w, g, s] . k_l - lse[w, g, s])   for the keys that (w, s) sees,
+//
+// with the log-sum-exp that the attention call of the same queries returned.  A query whose
+// lse is -inf (it saw nothing, or the caller takes it out) gives no weight.  Every key's sum
+// is formed by one thread block in a fixed order, so results repeat bit by bit.
+//
+// Two launches: mass_prep_kernel (rotated queries of every turn, spans), then the kernel
+// that streams the keys once.
+#include "turns.cuh"
+
+#include <cstdio>
+#include <cstdlib>
+
+namespace dvb {
+
+struct MassParams : TurnSplit {
+    int Hq, Hkv, G, S, R, rows;  // rows = S * G queries of a KV head: row r = (query r / G, head r % G)
+    long long N;                 // positions of a mass row
+    float scale_log2;
+    float* mass;
+    const float* lse;
+    const void* q;
+    const float* cos;
+    const float* sin;
+    const void* k;
+    // workspace
+    int* header;  // [3] error word (kErrorWordOffset)
+    void* qr;     // [F][W][Hkv][rows][E] T, queries rotated for the turn
+    float* lse2;  // [W][Hkv][rows] lse in log2 units; +inf: no weight
+};
+
+// ---- prep: block (w, 16-row tile of a KV head, turn) -----------------------------------
+constexpr int kPrepRows = 16;
+
+template <class T>
+__global__ void __launch_bounds__(128) mass_prep_kernel(MassParams p, int E) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x, f = blockIdx.z, w = blockIdx.x;
+    const int tiles = (p.rows + kPrepRows - 1) / kPrepRows;
+    const int h = blockIdx.y / tiles, r0 = (blockIdx.y - h * tiles) * kPrepRows, r1 = min(r0 + kPrepRows, p.rows);
+    if (f == 0 && blockIdx.y == 0) {
+        if (w == 0 && tid < 4) p.header[tid] = 0;
+        __shared__ int red[4];
+        long long off = 0;
+        int nw = 0;
+        for (int t = 0; t < p.F; ++t) {
+            const int Lt = __ldg(p.L + t);
+            int v = 0;
+            for (int s = tid; s < p.S; s += 128) v = max(v, turn_seen(Lt, __ldg(p.loc + ((size_t)t * p.W + w) * p.S + s), off, p.cap));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+            if ((tid & 31) == 0) red[tid >> 5] = v;
+            __syncthreads();
+            v = max(max(red[0], red[1]), max(red[2], red[3]));
+            __syncthreads();
+            if (tid == 0) p.span[(size_t)w * p.F + t] = v;
+            nw += (v + p.kt - 1) / p.kt;
+            off += Lt > 0 ? Lt : 0;
+        }
+        if (tid == 0) p.nwin[w] = nw;
+    }
+    const int half = p.R >> 1;
+    for (int r = r0 + (tid >> 5); r < r1; r += 4) {  // a warp per row
+        const int s = r / p.G, hq = h * p.G + (r - s * p.G);
+        const size_t qrow = ((size_t)w * p.Hq + hq) * p.S + s;
+        if (f == 0 && (tid & 31) == 0) {
+            const float x = __ldg(p.lse + qrow);
+            p.lse2[((size_t)w * p.Hkv + h) * p.rows + r] = x == neg_inf() ? -neg_inf() : x * kLog2e;
+        }
+        const T* x = static_cast<const T*>(p.q) + qrow * E;
+        T* y = static_cast<T*>(p.qr) + ((((size_t)f * p.W + w) * p.Hkv + h) * p.rows + r) * E;
+        const size_t cs = (((size_t)f * p.W + w) * p.S + s) * p.R;
+        for (int e = tid & 31; e < E; e += 32) {
+            if (e >= p.R) {
+                y[e] = x[e];
+            } else {
+                const int j = e < half ? e : e - half;
+                const float a = Elem<T>::to_f(x[e]), b = Elem<T>::to_f(e < half ? x[e + half] : x[e - half]);
+                y[e] = Elem<T>::from_f(__fadd_rn(__fmul_rn(a, __ldg(p.cos + cs + j)), __fmul_rn(e < half ? -b : b, __ldg(p.sin + cs + j))));
+            }
+        }
+    }
+}
+
+// ---- CUDA-core kernel: 32 keys x 32 rows per step, 8 warps of 4 rows, a lane per key ----
+template <class T, int E>
+__global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
+    constexpr int KT = 32, MT = 32, ROW = E * (int)sizeof(T) + 16, CH = E * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T);
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint8_t* sQ = smem;                                              // [MT] rows
+    uint8_t* sK = smem + MT * ROW;                                   // [KT] rows
+    float* red = reinterpret_cast<float*>(sK + KT * ROW);            // [8][KT]
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
+    SplitWalk walk;
+    {
+        const long long total = split_total(p, lane);
+        walk.u = split_bound(total, g, p.groups);
+        walk.u1 = split_bound(total, g + 1, p.groups);
+        split_locate(p, lane, walk.u, walk.w, walk.base);
+    }
+    SplitPiece pc;
+    while (walk.next(p, pc)) {
+        SplitWin win;
+        win.start();
+        for (int i = pc.i0; i < pc.i1; ++i) {
+            win.seek(p, pc.w, i);
+            for (int c = tid; c < KT * CH; c += 256) {
+                const int r = c / CH, ch = c - r * CH;
+                const T* kp = nullptr;
+                if (r < win.n) {
+                    const int pos = (int)(win.off + win.k0 + r);
+                    const int page = __ldg(p.bt + (size_t)pc.w * p.maxb + pos / p.BS);
+                    if (page >= 0 && page < p.NB)
+                        kp = static_cast<const T*>(p.k) + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E + ch * PER;
+                }
+                cp_async16_zfill(smem_u32(sK + r * ROW + ch * 16), kp ? kp : static_cast<const T*>(p.k), kp ? 16 : 0);
+            }
+            cp_async_commit();
+            const T* qr = static_cast<const T*>(p.qr) + (((size_t)win.f * p.W + pc.w) * p.Hkv + h) * p.rows * E;
+            const float* lse2 = p.lse2 + ((size_t)pc.w * p.Hkv + h) * p.rows;
+            const int Lf = __ldg(p.L + win.f);
+            float acc = 0.f;
+            for (int r0 = 0; r0 < p.rows; r0 += MT) {
+                for (int c = tid; c < MT * CH; c += 256) {
+                    const int r = c / CH, ch = c - r * CH;
+                    const bool in = r0 + r < p.rows;
+                    cp_async16_zfill(smem_u32(sQ + r * ROW + ch * 16), qr + (size_t)(in ? r0 + r : 0) * E + ch * PER, in ? 16 : 0);
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                __syncthreads();
+                float sc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+                for (int ch = 0; ch < CH; ++ch) {
+                    const T* kc = reinterpret_cast<const T*>(sK + lane * ROW + ch * 16);
+                    float kv[PER];
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) kv[e] = Elem<T>::to_f(kc[e]);
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        const T* qc = reinterpret_cast<const T*>(sQ + (wid * 4 + a) * ROW + ch * 16);
+#pragma unroll
+                        for (int e = 0; e < PER; ++e) sc[a] = fmaf(Elem<T>::to_f(qc[e]), kv[e], sc[a]);
+                    }
+                }
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const int r = r0 + wid * 4 + a;
+                    if (r >= p.rows) continue;
+                    const float l2 = __ldcg(lse2 + r);
+                    const int lim = turn_seen(Lf, __ldg(p.loc + ((size_t)win.f * p.W + pc.w) * p.S + r / p.G), win.off, p.cap);
+                    if (l2 != -neg_inf() && lane < win.n && win.k0 + lane < lim) acc += fast_exp2(sc[a] * p.scale_log2 - l2);
+                }
+                __syncthreads();
+            }
+            red[wid * KT + lane] = acc;
+            __syncthreads();
+            if (wid == 0 && lane < win.n) {
+                const long long pos = win.off + win.k0 + lane;
+                if (pos < p.N) {
+                    float sum = red[lane];
+#pragma unroll
+                    for (int x = 1; x < 8; ++x) sum += red[x * KT + lane];
+                    p.mass[((size_t)pc.w * p.Hkv + h) * p.N + pos] += sum;
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+struct MassKernel {
+    const void* fn;
+    int threads, kt;
+    size_t smem;
+};
+template <class T, int E> static MassKernel mass_simt() {
+    return MassKernel{(const void*)&mass_simt_kernel<T, E>, 256, 32, (size_t)64 * (E * sizeof(T) + 16) + 8 * 32 * 4};
+}
+template <class T> static MassKernel mass_pick_e(int E) {
+    return E == 64 ? mass_simt<T, 64>() : E == 128 ? mass_simt<T, 128>() : mass_simt<T, 256>();
+}
+static MassKernel mass_pick(const dvattn_mass_args* a) {
+    return a->dtype == DVATTN_FLOAT32 ? mass_pick_e<float>(a->E)
+         : a->dtype == DVATTN_FLOAT16 ? mass_pick_e<__half>(a->E) : mass_pick_e<__nv_bfloat16>(a->E);
+}
+
+static int mass_validate(const dvattn_mass_args* a) {
+    if (!a) return DVATTN_ERR_INVALID_ARGUMENT;
+    dvattn_paged_args v{};  // the shape rules of the paged attention
+    v.dtype = a->dtype; v.F = a->F; v.W = a->W; v.Hq = a->Hq; v.Hkv = a->Hkv; v.E = a->E; v.Ev = a->E; v.S = a->S;
+    v.R = a->R; v.block_size = a->block_size; v.max_blocks_per_seq = a->max_blocks_per_seq; v.num_blocks = a->num_blocks;
+    const int st = decode_validate(&v);
+    if (st != DVATTN_OK) return st;
+    if (a->positions < 0) return DVATTN_ERR_INVALID_ARGUMENT;
+    // grid limits of the prep kernel: turns are its z, row tiles of the KV heads its y
+    const long long rows = (long long)a->S * (a->Hq / a->Hkv);
+    if (a->F > 65535 || (rows + kPrepRows - 1) / kPrepRows * a->Hkv > 65535) return DVATTN_ERR_UNSUPPORTED;
+    return DVATTN_OK;
+}
+static bool mass_nothing(const dvattn_mass_args* a) {
+    return (long long)a->W * a->S == 0 || a->Hq == 0 || a->F == 0 || a->positions == 0 || a->num_blocks <= 0 || a->max_blocks_per_seq == 0;
+}
+
+struct MassLayout {
+    size_t nwin, span, qr, lse2, total;
+    int groups;
+};
+static int mass_layout(const dvattn_mass_args* a, const MassKernel& k, MassLayout& L) {
+    int dev = 0, sms = 0, occ = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+        cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k.fn, k.threads, k.smem) != cudaSuccess || occ < 1)
+        return DVATTN_ERR_CUDA;
+    L.groups = sms * occ / a->Hkv;
+    if (L.groups < 1) L.groups = 1;
+    const size_t esz = a->dtype == DVATTN_FLOAT32 ? 4 : 2, rows = (size_t)a->S * (a->Hq / a->Hkv);
+    size_t at = 256;
+    auto take = [&](size_t bytes) {
+        const size_t r = at;
+        at += (bytes + 255) / 256 * 256;
+        return r;
+    };
+    L.nwin = take(4 * (size_t)a->W);
+    L.span = take(4 * (size_t)a->W * a->F);
+    L.qr = take(esz * (size_t)a->F * a->W * a->Hkv * rows * a->E);
+    L.lse2 = take(4 * (size_t)a->W * a->Hkv * rows);
+    L.total = at;
+    return DVATTN_OK;
+}
+
+size_t mass_workspace_size(const dvattn_mass_args* a) {
+    if (mass_validate(a) != DVATTN_OK || mass_nothing(a)) return 0;
+    MassLayout L;
+    return mass_layout(a, mass_pick(a), L) == DVATTN_OK ? L.total : 0;
+}
+
+int mass_launch(const dvattn_mass_args* a, void* workspace, size_t wbytes, cudaStream_t stream) {
+    int st = mass_validate(a);
+    if (st != DVATTN_OK) return st;
+    if (mass_nothing(a)) return DVATTN_OK;
+    if (!a->mass || !a->queries || !a->lse || !a->locations || !a->fragment_lengths || !a->k_cache || !a->block_tables ||
+        (a->R > 0 && (!a->cosines || !a->sines)))
+        return DVATTN_ERR_INVALID_ARGUMENT;
+    if ((reinterpret_cast<uintptr_t>(a->queries) & 15) || (reinterpret_cast<uintptr_t>(a->k_cache) & 15)) return DVATTN_ERR_INVALID_ARGUMENT;
+    const MassKernel k = mass_pick(a);
+    MassLayout L;
+    if ((st = mass_layout(a, k, L)) != DVATTN_OK) return st;
+    if (!workspace || wbytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return DVATTN_ERR_WORKSPACE;
+    char* ws = static_cast<char*>(workspace);
+    MassParams p{};
+    p.F = a->F; p.W = a->W; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.S = a->S; p.R = a->R;
+    p.rows = p.S * p.G;
+    p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
+    const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
+    p.cap = cap > 0x7fffffffLL ? 0x7fffffff : (int)cap;
+    p.tail = 0; p.kt = k.kt; p.nt = 1; p.groups = L.groups;
+    p.N = a->positions;
+    p.scale_log2 = a->scale * kLog2e;
+    p.mass = a->mass; p.lse = a->lse; p.q = a->queries; p.cos = a->cosines; p.sin = a->sines; p.k = a->k_cache;
+    p.loc = a->locations; p.L = a->fragment_lengths; p.bt = a->block_tables;
+    p.header = reinterpret_cast<int*>(ws);
+    p.nwin = reinterpret_cast<int*>(ws + L.nwin);
+    p.span = reinterpret_cast<int*>(ws + L.span);
+    p.qr = ws + L.qr;
+    p.lse2 = reinterpret_cast<float*>(ws + L.lse2);
+    const void* prep = a->dtype == DVATTN_FLOAT32   ? (const void*)&mass_prep_kernel<float>
+                       : a->dtype == DVATTN_FLOAT16 ? (const void*)&mass_prep_kernel<__half> : (const void*)&mass_prep_kernel<__nv_bfloat16>;
+    int E = a->E;
+    void* pargs[] = {&p, &E};
+    const unsigned tiles = (unsigned)((p.rows + kPrepRows - 1) / kPrepRows * a->Hkv);
+    cudaError_t e = cudaLaunchKernel(prep, dim3(a->W, tiles, a->F), dim3(128), pargs, 0, stream);
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        cfg.stream = stream;
+        cfg.gridDim = dim3((unsigned)(L.groups * a->Hkv));
+        cfg.blockDim = dim3(k.threads);
+        cfg.dynamicSmemBytes = k.smem;
+        void* args[] = {&p};
+        e = cudaLaunchKernelExC(&cfg, k.fn, args);
+    }
+    if (e != cudaSuccess) {
+        if (getenv("DVATTN_DEBUG")) fprintf(stderr, "dvattn mass launch: %s\n", cudaGetErrorString(e));
+        return DVATTN_ERR_CUDA;
+    }
+    return cudaGetLastError() == cudaSuccess ? DVATTN_OK : DVATTN_ERR_CUDA;
+}
+
+}  // namespace dvb

@@ -506,6 +506,248 @@ void dvattn_paged_append_op(at::Tensor& k_cache, at::Tensor& v_cache, const at::
 }
 
 // ---------------------------------------------------------------------------------
+// dvattn_tree_sdpa / dvattn_tree_append (B200 additions): a tree of drafted tokens attends
+// over the paged cache and itself; its accepted tokens enter the pages
+// ---------------------------------------------------------------------------------
+template <class Args>
+void run_with_workspace(const at::Tensor& out, const Args& a, size_t (*size)(const Args*),
+                        int (*call)(const Args*, void*, size_t, dvattn_stream_t), const char* name, bool has_status) {
+    int st = call(&a, nullptr, 0, cur_stream(out));  // validation only when nothing to do
+    if (st == DVATTN_ERR_WORKSPACE) {
+        const size_t wsb = size(&a);
+        TORCH_CHECK(wsb > 0, name, ": could not size the workspace");
+        at::Tensor ws = at::empty({(int64_t)wsb}, out.options().dtype(at::kByte));
+        st = call(&a, ws.data_ptr(), wsb, cur_stream(out));
+        check_status(st, name);
+        if (has_status) check_call_status(ws, cur_stream(out), name);
+    }
+    check_status(st, name);
+}
+
+void dvattn_tree_sdpa_op(at::Tensor& out, const c10::optional<at::Tensor>& lse, double scale, const at::Tensor& parents,
+                         const at::Tensor& locations, const at::Tensor& queries, const at::Tensor& cosines,
+                         const at::Tensor& sines, const at::Tensor& fragment_lengths, const at::Tensor& k_cache,
+                         const at::Tensor& v_cache, const at::Tensor& block_tables, const at::Tensor& draft_keys,
+                         const at::Tensor& draft_values) {
+    const c10::cuda::CUDAGuard guard(out.device());
+    const int dt = dtype_code(out);
+    TORCH_CHECK(out.dim() == 4 && parents.dim() == 2 && locations.dim() == 3 && queries.dim() == 4 && cosines.dim() == 4 &&
+                    sines.dim() == 4 && fragment_lengths.dim() == 1 && k_cache.dim() == 4 && v_cache.dim() == 4 &&
+                    block_tables.dim() == 2 && draft_keys.dim() == 4 && draft_values.dim() == 4,
+                "dvattn_tree_sdpa: wrong tensor ranks");
+    for (const at::Tensor* t : {&queries, &k_cache, &v_cache, &draft_keys, &draft_values})
+        TORCH_CHECK(t->scalar_type() == out.scalar_type(),
+                    "dvattn_tree_sdpa: queries, caches and drafted keys/values must have the output dtype");
+    TORCH_CHECK(cosines.scalar_type() == at::kFloat && sines.scalar_type() == at::kFloat,
+                "dvattn_tree_sdpa: cosines/sines must be float32");
+    check_i32(parents, "parents");
+    check_i32(locations, "locations");
+    check_i32(fragment_lengths, "fragment_lengths");
+    check_i32(block_tables, "block_tables");
+    check_all(out, {Named{&out, "output"}, Named{&parents, "parents"}, Named{&locations, "locations"},
+                    Named{&queries, "queries"}, Named{&cosines, "cosines"}, Named{&sines, "sines"},
+                    Named{&fragment_lengths, "fragment_lengths"}, Named{&k_cache, "k_cache"}, Named{&v_cache, "v_cache"},
+                    Named{&block_tables, "block_tables"}, Named{&draft_keys, "draft_keys"},
+                    Named{&draft_values, "draft_values"}});
+    const int W = queries.size(0), Hq = queries.size(1), S = queries.size(2), E = queries.size(3);
+    const int F = locations.size(0), Hkv = k_cache.size(2), Ev = v_cache.size(3);
+    TORCH_CHECK(out.size(0) == W && out.size(1) == Hq && out.size(2) == S && out.size(3) == Ev,
+                "dvattn_tree_sdpa: output must be [W, Hq, S, Ev]");
+    TORCH_CHECK(parents.size(0) == W && parents.size(1) == S, "dvattn_tree_sdpa: parents must be [W, S]");
+    TORCH_CHECK(locations.size(1) == W && locations.size(2) == S, "dvattn_tree_sdpa: locations must be [F, W, S]");
+    TORCH_CHECK(cosines.size(0) == F && cosines.size(1) == W && cosines.size(2) == S && sines.sizes() == cosines.sizes(),
+                "dvattn_tree_sdpa: cosines/sines must be [F, W, S, R]");
+    TORCH_CHECK(fragment_lengths.size(0) == F, "dvattn_tree_sdpa: fragment_lengths must be [F]");
+    TORCH_CHECK(k_cache.size(3) == E, "dvattn_tree_sdpa: k_cache must be [NB, BS, Hkv, E]");
+    TORCH_CHECK(v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1) && v_cache.size(2) == Hkv,
+                "dvattn_tree_sdpa: v_cache must be [NB, BS, Hkv, Ev]");
+    TORCH_CHECK(block_tables.size(0) == W, "dvattn_tree_sdpa: block_tables must be [W, max_blocks]");
+    TORCH_CHECK(draft_keys.size(0) == W && draft_keys.size(1) == Hkv && draft_keys.size(2) == S && draft_keys.size(3) == E,
+                "dvattn_tree_sdpa: draft_keys must be [W, Hkv, S, E]");
+    TORCH_CHECK(draft_values.size(0) == W && draft_values.size(1) == Hkv && draft_values.size(2) == S && draft_values.size(3) == Ev,
+                "dvattn_tree_sdpa: draft_values must be [W, Hkv, S, Ev]");
+    dvattn_tree_args a{};
+    a.dtype = dt;
+    a.F = F; a.W = W; a.Hq = Hq; a.Hkv = Hkv; a.E = E; a.Ev = Ev; a.S = S; a.R = cosines.size(3);
+    a.block_size = k_cache.size(1);
+    a.max_blocks_per_seq = block_tables.size(1);
+    a.num_blocks = k_cache.size(0);
+    a.scale = static_cast<float>(scale);
+    a.out = out.data_ptr();
+    a.queries = queries.const_data_ptr();
+    a.parents = parents.const_data_ptr<int>();
+    a.cosines = cosines.const_data_ptr<float>();
+    a.sines = sines.const_data_ptr<float>();
+    a.locations = locations.const_data_ptr<int>();
+    a.fragment_lengths = fragment_lengths.const_data_ptr<int>();
+    a.k_cache = k_cache.const_data_ptr();
+    a.v_cache = v_cache.const_data_ptr();
+    a.block_tables = block_tables.const_data_ptr<int>();
+    a.draft_keys = draft_keys.const_data_ptr();
+    a.draft_values = draft_values.const_data_ptr();
+    if (lse.has_value()) {
+        check_cuda_tensor(*lse, "lse", out);
+        TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->numel() == (int64_t)W * Hq * S, "dvattn_tree_sdpa: lse must be f32 [W, Hq, S]");
+        a.lse_out = lse->data_ptr<float>();
+    }
+    run_with_workspace(out, a, dvattn_tree_sdpa_workspace_size, dvattn_tree_sdpa, "dvattn_tree_sdpa", true);
+}
+
+void dvattn_tree_append_op(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& draft_keys,
+                           const at::Tensor& draft_values, const at::Tensor& cosines, const at::Tensor& sines,
+                           const at::Tensor& block_tables, const at::Tensor& positions, const at::Tensor& accepted,
+                           const c10::optional<at::Tensor>& counts) {
+    const c10::cuda::CUDAGuard guard(k_cache.device());
+    const int dt = dtype_code(k_cache);
+    TORCH_CHECK(k_cache.dim() == 4 && v_cache.dim() == 4 && draft_keys.dim() == 4 && draft_values.dim() == 4 &&
+                    cosines.dim() == 3 && sines.dim() == 3 && block_tables.dim() == 2 && positions.dim() == 1 && accepted.dim() == 2,
+                "dvattn_tree_append: wrong tensor ranks");
+    for (const at::Tensor* t : {(const at::Tensor*)&v_cache, &draft_keys, &draft_values})
+        TORCH_CHECK(t->scalar_type() == k_cache.scalar_type(), "dvattn_tree_append: caches and drafted tokens must share the dtype");
+    TORCH_CHECK(cosines.scalar_type() == at::kFloat && sines.scalar_type() == at::kFloat,
+                "dvattn_tree_append: cosines/sines must be float32");
+    check_i32(block_tables, "block_tables");
+    check_i32(positions, "positions");
+    check_i32(accepted, "accepted");
+    check_all(k_cache, {Named{&k_cache, "k_cache"}, Named{&v_cache, "v_cache"}, Named{&draft_keys, "draft_keys"},
+                        Named{&draft_values, "draft_values"}, Named{&cosines, "cosines"}, Named{&sines, "sines"},
+                        Named{&block_tables, "block_tables"}, Named{&positions, "positions"}, Named{&accepted, "accepted"}});
+    const int W = draft_keys.size(0), Hkv = draft_keys.size(1), S = draft_keys.size(2), E = draft_keys.size(3);
+    const int Ev = draft_values.size(3), R = cosines.size(2);
+    TORCH_CHECK(draft_values.size(0) == W && draft_values.size(1) == Hkv && draft_values.size(2) == S,
+                "dvattn_tree_append: draft_values must be [W, Hkv, S, Ev]");
+    TORCH_CHECK(k_cache.size(2) == Hkv && k_cache.size(3) == E, "dvattn_tree_append: k_cache must be [NB, BS, Hkv, E]");
+    TORCH_CHECK(v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1) && v_cache.size(2) == Hkv &&
+                    v_cache.size(3) == Ev, "dvattn_tree_append: v_cache must be [NB, BS, Hkv, Ev]");
+    TORCH_CHECK(cosines.size(0) == W && cosines.size(1) == S && sines.sizes() == cosines.sizes(),
+                "dvattn_tree_append: cosines/sines must be [W, S, R]");
+    TORCH_CHECK(block_tables.size(0) == W && positions.size(0) == W && accepted.size(0) == W,
+                "dvattn_tree_append: block_tables [W, max_blocks], positions [W], accepted [W, A]");
+    dvattn_tree_append_args a{};
+    a.dtype = dt;
+    a.W = W; a.Hkv = Hkv; a.E = E; a.Ev = Ev; a.S = S; a.A = accepted.size(1); a.R = R;
+    a.block_size = k_cache.size(1);
+    a.max_blocks_per_seq = block_tables.size(1);
+    a.num_blocks = k_cache.size(0);
+    a.k_cache = k_cache.data_ptr();
+    a.v_cache = v_cache.data_ptr();
+    a.draft_keys = draft_keys.const_data_ptr();
+    a.draft_values = draft_values.const_data_ptr();
+    a.cosines = cosines.const_data_ptr<float>();
+    a.sines = sines.const_data_ptr<float>();
+    a.block_tables = block_tables.const_data_ptr<int>();
+    a.positions = positions.const_data_ptr<int>();
+    a.accepted = accepted.const_data_ptr<int>();
+    if (counts.has_value()) {
+        check_cuda_tensor(*counts, "counts", k_cache);
+        check_i32(*counts, "counts");
+        TORCH_CHECK(counts->numel() == W, "dvattn_tree_append: counts must be [W]");
+        a.counts = counts->const_data_ptr<int>();
+    }
+    check_status(dvattn_tree_append(&a, cur_stream(k_cache)), "dvattn_tree_append");
+}
+
+// ---------------------------------------------------------------------------------
+// dvattn_paged_mass / dvattn_paged_evict (B200 additions): accumulated attention weight of
+// the cached keys, eviction of the least attended ones
+// ---------------------------------------------------------------------------------
+void dvattn_paged_mass_op(at::Tensor& mass, double scale, const at::Tensor& locations, const at::Tensor& queries,
+                          const at::Tensor& lse, const at::Tensor& cosines, const at::Tensor& sines,
+                          const at::Tensor& fragment_lengths, const at::Tensor& k_cache, const at::Tensor& block_tables) {
+    const c10::cuda::CUDAGuard guard(mass.device());
+    const int dt = dtype_code(queries);
+    TORCH_CHECK(mass.dim() == 3 && locations.dim() == 3 && queries.dim() == 4 && lse.dim() == 3 && cosines.dim() == 4 &&
+                    sines.dim() == 4 && fragment_lengths.dim() == 1 && k_cache.dim() == 4 && block_tables.dim() == 2,
+                "dvattn_paged_mass: wrong tensor ranks");
+    TORCH_CHECK(k_cache.scalar_type() == queries.scalar_type(), "dvattn_paged_mass: k_cache must have the dtype of the queries");
+    for (const at::Tensor* t : {(const at::Tensor*)&mass, &lse, &cosines, &sines})
+        TORCH_CHECK(t->scalar_type() == at::kFloat, "dvattn_paged_mass: mass, lse and cosines/sines must be float32");
+    check_i32(locations, "locations");
+    check_i32(fragment_lengths, "fragment_lengths");
+    check_i32(block_tables, "block_tables");
+    check_all(mass, {Named{&mass, "mass"}, Named{&locations, "locations"}, Named{&queries, "queries"}, Named{&lse, "lse"},
+                     Named{&cosines, "cosines"}, Named{&sines, "sines"}, Named{&fragment_lengths, "fragment_lengths"},
+                     Named{&k_cache, "k_cache"}, Named{&block_tables, "block_tables"}});
+    const int W = queries.size(0), Hq = queries.size(1), S = queries.size(2), E = queries.size(3);
+    const int F = locations.size(0), Hkv = k_cache.size(2);
+    TORCH_CHECK(mass.size(0) == W && mass.size(1) == Hkv, "dvattn_paged_mass: mass must be [W, Hkv, N]");
+    TORCH_CHECK(locations.size(1) == W && locations.size(2) == S, "dvattn_paged_mass: locations must be [F, W, S]");
+    TORCH_CHECK(lse.size(0) == W && lse.size(1) == Hq && lse.size(2) == S, "dvattn_paged_mass: lse must be [W, Hq, S]");
+    TORCH_CHECK(cosines.size(0) == F && cosines.size(1) == W && cosines.size(2) == S && sines.sizes() == cosines.sizes(),
+                "dvattn_paged_mass: cosines/sines must be [F, W, S, R]");
+    TORCH_CHECK(fragment_lengths.size(0) == F, "dvattn_paged_mass: fragment_lengths must be [F]");
+    TORCH_CHECK(k_cache.size(3) == E, "dvattn_paged_mass: k_cache must be [NB, BS, Hkv, E]");
+    TORCH_CHECK(block_tables.size(0) == W, "dvattn_paged_mass: block_tables must be [W, max_blocks]");
+    dvattn_mass_args a{};
+    a.dtype = dt;
+    a.F = F; a.W = W; a.Hq = Hq; a.Hkv = Hkv; a.E = E; a.S = S; a.R = cosines.size(3);
+    a.block_size = k_cache.size(1);
+    a.max_blocks_per_seq = block_tables.size(1);
+    a.num_blocks = k_cache.size(0);
+    a.positions = mass.size(2);
+    a.scale = static_cast<float>(scale);
+    a.mass = mass.data_ptr<float>();
+    a.queries = queries.const_data_ptr();
+    a.lse = lse.const_data_ptr<float>();
+    a.cosines = cosines.const_data_ptr<float>();
+    a.sines = sines.const_data_ptr<float>();
+    a.locations = locations.const_data_ptr<int>();
+    a.fragment_lengths = fragment_lengths.const_data_ptr<int>();
+    a.k_cache = k_cache.const_data_ptr();
+    a.block_tables = block_tables.const_data_ptr<int>();
+    run_with_workspace(mass, a, dvattn_paged_mass_workspace_size, dvattn_paged_mass, "dvattn_paged_mass", true);
+}
+
+void dvattn_paged_evict_op(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& mass, at::Tensor& mass_out,
+                           const c10::optional<at::Tensor>& source, const at::Tensor& block_tables, const at::Tensor& starts,
+                           const at::Tensor& lengths, const at::Tensor& keep, int64_t sink, int64_t recent) {
+    const c10::cuda::CUDAGuard guard(k_cache.device());
+    const int dt = dtype_code(k_cache);
+    TORCH_CHECK(k_cache.dim() == 4 && v_cache.dim() == 4 && mass.dim() == 3 && mass_out.dim() == 3 && block_tables.dim() == 2 &&
+                    starts.dim() == 1 && lengths.dim() == 1 && keep.dim() == 1,
+                "dvattn_paged_evict: wrong tensor ranks");
+    TORCH_CHECK(v_cache.scalar_type() == k_cache.scalar_type(), "dvattn_paged_evict: the caches must share the dtype");
+    TORCH_CHECK(mass.scalar_type() == at::kFloat && mass_out.scalar_type() == at::kFloat, "dvattn_paged_evict: mass must be float32");
+    check_i32(block_tables, "block_tables");
+    check_i32(starts, "starts");
+    check_i32(lengths, "lengths");
+    check_i32(keep, "keep");
+    check_all(k_cache, {Named{&k_cache, "k_cache"}, Named{&v_cache, "v_cache"}, Named{&mass, "mass"}, Named{&mass_out, "mass_out"},
+                        Named{&block_tables, "block_tables"}, Named{&starts, "starts"}, Named{&lengths, "lengths"}, Named{&keep, "keep"}});
+    const int W = block_tables.size(0), Hkv = k_cache.size(2);
+    TORCH_CHECK(mass.size(0) == W && mass.size(1) == Hkv && mass_out.sizes() == mass.sizes(),
+                "dvattn_paged_evict: mass and mass_out must be [W, Hkv, N]");
+    TORCH_CHECK(v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1) && v_cache.size(2) == Hkv,
+                "dvattn_paged_evict: v_cache must be [NB, BS, Hkv, Ev]");
+    TORCH_CHECK(starts.size(0) == W && lengths.size(0) == W && keep.size(0) == W,
+                "dvattn_paged_evict: starts, lengths and keep must be [W]");
+    TORCH_CHECK(sink >= 0 && sink <= INT32_MAX && recent >= 0 && recent <= INT32_MAX, "dvattn_paged_evict: sink and recent must be >= 0");
+    dvattn_evict_args a{};
+    a.dtype = dt;
+    a.W = W; a.Hkv = Hkv; a.E = k_cache.size(3); a.Ev = v_cache.size(3);
+    a.block_size = k_cache.size(1);
+    a.max_blocks_per_seq = block_tables.size(1);
+    a.sink = static_cast<int>(sink); a.recent = static_cast<int>(recent);
+    a.num_blocks = k_cache.size(0);
+    a.positions = mass.size(2);
+    a.k_cache = k_cache.data_ptr();
+    a.v_cache = v_cache.data_ptr();
+    a.mass = mass.const_data_ptr<float>();
+    a.mass_out = mass_out.data_ptr<float>();
+    if (source.has_value()) {
+        check_cuda_tensor(*source, "source", k_cache);
+        check_i32(*source, "source");
+        TORCH_CHECK(source->sizes() == mass.sizes(), "dvattn_paged_evict: source must be i32 [W, Hkv, N]");
+        a.source = source->data_ptr<int>();
+    }
+    a.block_tables = block_tables.const_data_ptr<int>();
+    a.starts = starts.const_data_ptr<int>();
+    a.lengths = lengths.const_data_ptr<int>();
+    a.keep = keep.const_data_ptr<int>();
+    run_with_workspace(k_cache, a, dvattn_paged_evict_workspace_size, dvattn_paged_evict, "dvattn_paged_evict", false);
+}
+
+// ---------------------------------------------------------------------------------
 // dvattn_sdpa / dvattn_fused: contiguous per-turn fragments (src/binding.cu:79-149,
 // 356-372).  key_fragments[f] is [Hkv, L_f, E] or [B, Hkv, L_f, E] with B = 1 (one
 // fragment shared by the W workers) or B = W; queries are [F, W, Hq, S, E], rotated.
@@ -631,6 +873,17 @@ TORCH_LIBRARY(libdvatt, m) {
           "Tensor seg_order, Tensor? inv_freq, float rope_base, float attention_scaling, int round_dtype) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
     m.def("dvattn_paged_append(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor keys, Tensor values, Tensor cosines, "
           "Tensor sines, Tensor block_tables, Tensor positions, Tensor? counts) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("dvattn_tree_sdpa(Tensor(a!) output, Tensor(b!)? lse, float scale, Tensor parents, Tensor locations, "
+          "Tensor queries, Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor v_cache, "
+          "Tensor block_tables, Tensor draft_keys, Tensor draft_values) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("dvattn_tree_append(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor draft_keys, Tensor draft_values, "
+          "Tensor cosines, Tensor sines, Tensor block_tables, Tensor positions, Tensor accepted, Tensor? counts) -> ()",
+          tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("dvattn_paged_mass(Tensor(a!) mass, float scale, Tensor locations, Tensor queries, Tensor lse, Tensor cosines, "
+          "Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor block_tables) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("dvattn_paged_evict(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor mass, Tensor(c!) mass_out, "
+          "Tensor(d!)? source, Tensor block_tables, Tensor starts, Tensor lengths, Tensor keep, int sink, int recent) -> ()",
+          tags, torch::_RegisterOrVerify::REGISTER);
 }
 
 TORCH_LIBRARY_IMPL(libdvatt, CUDA, m) {
@@ -647,4 +900,8 @@ TORCH_LIBRARY_IMPL(libdvatt, CUDA, m) {
     m.impl("dvattn_build_views", dvattn_build_views_op);
     m.impl("dvattn_paged_sdpa_rope", dvattn_paged_sdpa_rope_op);
     m.impl("dvattn_varlen_paged_sdpa_rope", dvattn_varlen_paged_sdpa_rope_op);
+    m.impl("dvattn_tree_sdpa", dvattn_tree_sdpa_op);
+    m.impl("dvattn_tree_append", dvattn_tree_append_op);
+    m.impl("dvattn_paged_mass", dvattn_paged_mass_op);
+    m.impl("dvattn_paged_evict", dvattn_paged_evict_op);
 }

@@ -1,0 +1,520 @@
+// Attention of a tree of drafted tokens over the paged multi-turn cache, verified in one
+// pass (tree.cuh: the items; turns.cuh: the work split).
+//
+//   out[w, h, s] = sum_j softmax_j(scale * q . k_j) v_j  over the cached keys that
+//   (w, s) sees in every turn (q rotated for that turn) and the drafted keys of s's
+//   ancestors and of s itself (q and key rotated with their own angles in the last turn).
+//
+// Three launches: tree_prep_kernel (ancestor sets, visible spans, rotated drafted keys),
+// the attention kernel, and tree_merge_kernel, each a programmatic dependent of the one
+// before it.  The running maximum and sum, the scores and the output accumulate in 32 bits.
+#include "tree.cuh"
+
+#include <cstdio>
+#include <cstdlib>
+
+namespace dvb {
+
+// ---- prep: one block per (sequence, KV head) -----------------------------------------
+// The rotation is apply_rotary_pos_emb's with separate roundings of the two products and
+// of the sum, then one rounding to T, so a drafted key has the bits that the paged append
+// writes for it.
+template <class T>
+__global__ void __launch_bounds__(128) tree_prep_kernel(TreeParams p, int E) {
+    extern __shared__ int par[];  // [S]
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int w = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+    if (h == 0) {
+        if (w == 0 && tid < 4) p.header[tid] = 0;
+        for (int j = tid; j < p.S; j += 128) par[j] = __ldg(p.parents + (size_t)w * p.S + j);
+        __syncthreads();
+        // a token is there if its line of parents, each before its child, ends at -1
+        for (int j = tid; j < p.S; j += 128) {
+            int c = j;
+            while (c >= 0 && par[c] < c && par[c] >= -1) c = par[c];
+            const bool there = c == -1;
+            uint32_t* a = p.anc + ((size_t)w * p.S + j) * p.SW;
+            c = there ? j : -1;
+            for (int word = p.SW - 1; word >= 0; --word) {
+                uint32_t bits = 0;
+                while (c >= 32 * word) {  // c < 32 * (word + 1) here: parents come before
+                    bits |= 1u << (c & 31);
+                    c = par[c];
+                    if (c < 0) break;
+                }
+                a[word] = bits;
+            }
+        }
+        __shared__ int red[4];
+        __syncthreads();  // the block's own global writes are visible to it after this
+        long long off = 0;
+        int nw = 0;
+        for (int f = 0; f < p.F; ++f) {
+            const int Lf = __ldg(p.L + f);
+            int v = 0;
+            for (int s = tid; s < p.S; s += 128)
+                if (p.anc[((size_t)w * p.S + s) * p.SW + (s >> 5)] >> (s & 31) & 1u)
+                    v = max(v, turn_seen(Lf, __ldg(p.loc + ((size_t)f * p.W + w) * p.S + s), off, p.cap));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+            if ((tid & 31) == 0) red[tid >> 5] = v;
+            __syncthreads();
+            v = max(max(red[0], red[1]), max(red[2], red[3]));
+            __syncthreads();
+            if (tid == 0) p.span[(size_t)w * p.F + f] = v;
+            nw += (v + p.kt - 1) / p.kt;
+            off += Lf > 0 ? Lf : 0;
+        }
+        if (tid == 0) p.nwin[w] = nw + (p.S + p.kt - 1) / p.kt;
+    }
+    const int half = p.R >> 1;
+    const T* x = static_cast<const T*>(p.dk) + ((size_t)w * p.Hkv + h) * p.S * E;
+    T* y = static_cast<T*>(p.dkr) + ((size_t)w * p.Hkv + h) * p.S * E;
+    const size_t cs = ((size_t)(p.F - 1) * p.W + w) * p.S;
+    for (int i = tid; i < p.S * E; i += 128) {
+        const int s = i / E, e = i - s * E;
+        if (e >= p.R) {
+            y[i] = x[i];
+        } else {
+            const int j = e < half ? e : e - half;
+            const float c = __ldg(p.cos + (cs + s) * p.R + j), sn = __ldg(p.sin + (cs + s) * p.R + j);
+            const float a = Elem<T>::to_f(x[i]), b = Elem<T>::to_f(e < half ? x[i + half] : x[i - half]);
+            y[i] = Elem<T>::from_f(__fadd_rn(__fmul_rn(a, c), __fmul_rn(e < half ? -b : b, sn)));
+        }
+    }
+}
+
+// ---- CUDA-core attention --------------------------------------------------------------
+// 32 rows x 32 keys per step, 8 warps of 4 rows.  Scores: a lane per key, q rows broadcast
+// from shared memory; output: a lane per E / 32 columns.  K and V tiles are double-buffered
+// with cp.async (zero-filled where a key is not seen, so what lies there never matters).
+template <class T, int E> struct SimtCfg {
+    static constexpr int KT = 32, MI = 32, THREADS = 256;
+    static constexpr int ROW = E * (int)sizeof(T) + 16;  // padded row, bytes
+    static constexpr size_t SMEM = (size_t)MI * (E + 4) * 4 + 4 * (size_t)KT * ROW + (size_t)MI * (KT + 4) * 4;
+};
+
+// key (f, l) of KV head h: its address, or null where there is none to read
+template <class T>
+__device__ __forceinline__ const T* tree_row(const TreeParams& p, const void* cache, const void* draft, int E, int w, int h,
+                                             const SplitWin& win, int l) {
+    if (win.f == p.F) {
+        // a drafted token that is not there is read as zeros
+        if (!(__ldcg(p.anc + ((size_t)w * p.S + l) * p.SW + (l >> 5)) >> (l & 31) & 1u)) return nullptr;
+        return static_cast<const T*>(draft) + (((size_t)w * p.Hkv + h) * p.S + l) * E;
+    }
+    const int pos = (int)(win.off + l);
+    const int page = __ldg(p.bt + (size_t)w * p.maxb + pos / p.BS);
+    if (page < 0 || page >= p.NB) return nullptr;
+    return static_cast<const T*>(cache) + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E;
+}
+
+template <class T, int N>
+__device__ __forceinline__ void load_n(const void* src, float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = Elem<T>::to_f(static_cast<const T*>(src)[i]);
+}
+
+template <class T, int E>
+__global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeParams p) {
+    using C = SimtCfg<T, E>;
+    constexpr int KT = C::KT, MI = C::MI, ROW = C::ROW, CH = E * (int)sizeof(T) / 16, VC = E / 32;
+    constexpr int PER = 16 / (int)sizeof(T);
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* sQ = reinterpret_cast<float*>(smem);                        // [MI][E + 4]
+    uint8_t* sK = smem + (size_t)MI * (E + 4) * 4;                     // [2][KT] rows
+    uint8_t* sV = sK + 2 * KT * ROW;                                   // [2][KT] rows
+    float* sP = reinterpret_cast<float*>(sV + 2 * KT * ROW);           // [MI][KT + 4]
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
+    SplitWalk walk;
+    {
+        const long long total = split_total(p, lane);
+        walk.u = split_bound(total, g, p.groups);
+        walk.u1 = split_bound(total, g + 1, p.groups);
+        split_locate(p, lane, walk.u, walk.w, walk.base);
+    }
+    const int rows = p.S * p.G;
+    SplitPiece pc;
+    while (walk.next(p, pc)) {
+        SplitWin ld, win;
+        ld.start();
+        win.start();
+        auto load = [&](int i, int st) {
+            ld.seek(p, pc.w, i);
+            for (int c = tid; c < KT * CH; c += C::THREADS) {
+                const int r = c / CH, ch = c - r * CH;
+                const T* kp = nullptr;
+                const T* vp = nullptr;
+                if (r < ld.n) {
+                    kp = tree_row<T>(p, p.k, p.dkr, E, pc.w, h, ld, ld.k0 + r);
+                    vp = tree_row<T>(p, p.v, p.dv, E, pc.w, h, ld, ld.k0 + r);
+                }
+                cp_async16_zfill(smem_u32(sK + (st * KT + r) * ROW + ch * 16), kp ? kp + ch * PER : static_cast<const T*>(p.k), kp ? 16 : 0);
+                cp_async16_zfill(smem_u32(sV + (st * KT + r) * ROW + ch * 16), vp ? vp + ch * PER : static_cast<const T*>(p.v), vp ? 16 : 0);
+            }
+            cp_async_commit();
+        };
+        float m[4], l[4], o[4][VC];
+        int lim[4], tok[4];  // the rows' tokens and the keys they see in the window's turn
+        uint32_t there = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            m[i] = neg_inf();
+            l[i] = 0.f;
+            const int r = pc.t * MI + wid * 4 + i;
+            tok[i] = r < rows ? r / p.G : -1;
+            if (tok[i] >= 0 && (__ldcg(p.anc + ((size_t)pc.w * p.S + tok[i]) * p.SW + (tok[i] >> 5)) >> (tok[i] & 31) & 1u)) there |= 1u << i;
+#pragma unroll
+            for (int c = 0; c < VC; ++c) o[i][c] = 0.f;
+        }
+        int turn = -1;
+        load(pc.i0, 0);
+        for (int i = pc.i0; i < pc.i1; ++i) {
+            const int st = (i - pc.i0) & 1;
+            if (i + 1 < pc.i1) {
+                load(i + 1, st ^ 1);
+                cp_async_wait<1>();
+            } else {
+                cp_async_wait<0>();
+            }
+            win.seek(p, pc.w, i);
+            const int qt = win.f < p.F ? win.f : p.F - 1;  // the turn whose rotation q takes
+            if (qt != turn) {
+                turn = qt;
+                for (int c = tid; c < MI * E; c += C::THREADS) {
+                    const int r = c / E, e = c - r * E, rr = pc.t * MI + r;
+                    float x = 0.f;
+                    if (rr < rows) {
+                        const int s = rr / p.G, hq = h * p.G + (rr - s * p.G), half = p.R >> 1;
+                        const T* q = static_cast<const T*>(p.q) + (((size_t)pc.w * p.Hq + hq) * p.S + s) * E;
+                        x = Elem<T>::to_f(q[e]);
+                        if (e < p.R) {
+                            const size_t cs = (((size_t)qt * p.W + pc.w) * p.S + s) * p.R + (e < half ? e : e - half);
+                            const float b = Elem<T>::to_f(e < half ? q[e + half] : q[e - half]);
+                            x = __fadd_rn(__fmul_rn(x, __ldg(p.cos + cs)), __fmul_rn(e < half ? -b : b, __ldg(p.sin + cs)));
+                            x = Elem<T>::to_f(Elem<T>::from_f(x));
+                        }
+                    }
+                    sQ[r * (E + 4) + e] = x;
+                }
+            }
+            if (win.f < p.F)
+#pragma unroll
+                for (int a = 0; a < 4; ++a)
+                    lim[a] = there >> a & 1u ? turn_seen(__ldg(p.L + win.f), __ldg(p.loc + ((size_t)win.f * p.W + pc.w) * p.S + tok[a]), win.off, p.cap) : 0;
+            __syncthreads();
+            // scores of this warp's 4 rows and the lane's key
+            float sc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int ch = 0; ch < CH; ++ch) {
+                float kv[PER];
+                load_n<T, PER>(sK + (st * KT + lane) * ROW + ch * 16, kv);
+#pragma unroll
+                for (int a = 0; a < 4; ++a)
+#pragma unroll
+                    for (int e = 0; e < PER; e += 4) {
+                        const float4 q4 = *reinterpret_cast<const float4*>(sQ + (wid * 4 + a) * (E + 4) + ch * PER + e);
+                        sc[a] = fmaf(q4.x, kv[e], sc[a]);
+                        sc[a] = fmaf(q4.y, kv[e + 1], sc[a]);
+                        sc[a] = fmaf(q4.z, kv[e + 2], sc[a]);
+                        sc[a] = fmaf(q4.w, kv[e + 3], sc[a]);
+                    }
+            }
+            const int key = win.k0 + lane;
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                bool sees = false;
+                if (lane < win.n && (there >> a & 1u))
+                    sees = win.f < p.F ? key < lim[a]
+                                       : (__ldcg(p.anc + ((size_t)pc.w * p.S + tok[a]) * p.SW + (key >> 5)) >> (key & 31) & 1u) != 0;
+                const float x = sees ? sc[a] * p.scale_log2 : neg_inf();
+                float mx = x;
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                mx = fmaxf(mx, m[a]);
+                const float mu = mx == neg_inf() ? 0.f : mx;
+                const float e = fast_exp2(x - mu), alpha = fast_exp2(m[a] - mu);
+                float sum = e;
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                l[a] = l[a] * alpha + sum;
+                m[a] = mx;
+                sP[(wid * 4 + a) * (KT + 4) + lane] = e;
+#pragma unroll
+                for (int c = 0; c < VC; ++c) o[a][c] *= alpha;
+            }
+            __syncwarp();
+#pragma unroll 2
+            for (int k4 = 0; k4 < KT; k4 += 4) {
+                float pr[4][4];
+#pragma unroll
+                for (int a = 0; a < 4; ++a)
+                    *reinterpret_cast<float4*>(pr[a]) = *reinterpret_cast<const float4*>(sP + (wid * 4 + a) * (KT + 4) + k4);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float vv[VC];
+                    load_n<T, VC>(sV + (st * KT + k4 + u) * ROW + lane * VC * (int)sizeof(T), vv);
+#pragma unroll
+                    for (int a = 0; a < 4; ++a)
+#pragma unroll
+                        for (int c = 0; c < VC; ++c) o[a][c] = fmaf(pr[a][u], vv[c], o[a][c]);
+                }
+            }
+            __syncthreads();
+        }
+        // the piece's result
+        const bool whole = pc.whole();
+        const size_t slot = (size_t)blockIdx.x * 2 + pc.slot();
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            if (tok[a] < 0) continue;
+            const float inv = l[a] > 0.f ? 1.f / l[a] : l[a] == 0.f ? 0.f : l[a];
+            const float lse2 = l[a] == 0.f ? neg_inf() : m[a] + log2f(l[a]);
+            const int r = wid * 4 + a, hq = h * p.G + (pc.t * MI + r - tok[a] * p.G);
+            const size_t orow = ((size_t)pc.w * p.Hq + hq) * p.S + tok[a];
+            if (whole) {
+#pragma unroll
+                for (int c = 0; c < VC; ++c) static_cast<T*>(p.out)[orow * E + lane * VC + c] = Elem<T>::from_f(o[a][c] * inv);
+                if (p.lse_out && lane == 0) p.lse_out[orow] = lse2 * kLn2;
+            } else {
+#pragma unroll
+                for (int c = 0; c < VC; ++c) p.part_o[(slot * MI + r) * E + lane * VC + c] = o[a][c] * inv;
+                if (lane == 0) p.part_lse[slot * MI + r] = lse2;
+            }
+        }
+    }
+}
+
+// ---- merge ----------------------------------------------------------------------------
+// Rows of items that more than one group worked on: the log-sum-exp combination of their
+// partials, in group order.  E / 4 threads per row.  A call whose error word is set gets
+// NaN in every output.
+template <class T, int E>
+__global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
+    constexpr int TPR = E / 4, RPB = 256 / TPR;  // threads per row, rows per block
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int item = blockIdx.x, h = item % p.Hkv, t = item / p.Hkv % p.nt, w = item / p.Hkv / p.nt;
+    const int i = blockIdx.y * RPB + tid / TPR, e = tid % TPR * 4;
+    const int r = t * p.mi + i;
+    const bool row_ok = i < p.mi && r < p.S * p.G;
+    const int s = row_ok ? r / p.G : 0, hq = h * p.G + (row_ok ? r - s * p.G : 0);
+    const size_t orow = ((size_t)w * p.Hq + hq) * p.S + s;
+    T* op = static_cast<T*>(p.out) + orow * E + e;
+    if (__ldcg(p.header + 3) != 0) {
+        const float nan = __int_as_float(0x7fc00000);
+        if (row_ok) {
+            store_quad<T>(op, nan, nan, nan, nan);
+            if (p.lse_out && e == 0) p.lse_out[orow] = nan;
+        }
+        return;
+    }
+    // the groups that hold the item's first and last window
+    long long total = 0, before = 0;
+    for (int x = lane; x < p.W; x += 32) {
+        const int n = __ldcg(p.nwin + x);
+        total += n;
+        if (x < w) before += n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    total *= p.nt;
+    const int nw = __ldcg(p.nwin + w);
+    const long long us = before * p.nt + (long long)t * nw, ue = us + nw - 1;
+    auto group_of = [&](long long u) {
+        int g = (int)(u * p.groups / total);
+        while (g > 0 && split_bound(total, g, p.groups) > u) --g;
+        while (g + 1 < p.groups && split_bound(total, g + 1, p.groups) <= u) ++g;
+        return g;
+    };
+    const int g0 = group_of(us), g1 = group_of(ue);
+    if (g0 == g1 || !row_ok) return;
+    auto slot_of = [&](int g) { return ((size_t)g * p.Hkv + h) * 2 + (g == g0 ? 1 : 0); };
+    auto empty = [&](int g) { return split_bound(total, g, p.groups) == split_bound(total, g + 1, p.groups); };
+    float mx = neg_inf();
+    bool bad = false;  // a partial of NaN: fmaxf drops it, the result must not
+    for (int g = g0; g <= g1; ++g) {
+        if (empty(g)) continue;
+        const float x = __ldcg(p.part_lse + slot_of(g) * p.mi + i);
+        mx = fmaxf(mx, x);
+        bad |= x != x;
+    }
+    float den = 0.f, a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+    if (mx != neg_inf()) {
+        for (int g = g0; g <= g1; ++g) {
+            if (empty(g)) continue;
+            const size_t sl = slot_of(g) * p.mi + i;
+            const float x = __ldcg(p.part_lse + sl);
+            if (x == neg_inf()) continue;
+            const float wgt = fast_exp2(x - mx);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + sl * E + e));
+            den += wgt;
+            a0 = fmaf(wgt, v.x, a0);
+            a1 = fmaf(wgt, v.y, a1);
+            a2 = fmaf(wgt, v.z, a2);
+            a3 = fmaf(wgt, v.w, a3);
+        }
+    }
+    float inv = den > 0.f ? 1.f / den : 0.f;
+    if (bad) inv = __int_as_float(0x7fc00000);
+    store_quad<T>(op, a0 * inv, a1 * inv, a2 * inv, a3 * inv);
+    if (p.lse_out && e == 0) p.lse_out[orow] = bad ? inv : den > 0.f ? (mx + log2f(den)) * kLn2 : neg_inf();
+}
+
+// ---------------------------------------------------------------------------------------
+constexpr int kTreeMaxTokens = 1024;
+
+template <class T, int E> static TreeKernel simt_kernel() {
+    TreeKernel k{};
+    k.fn = (const void*)&tree_simt_kernel<T, E>;
+    k.threads = SimtCfg<T, E>::THREADS;
+    k.kt = SimtCfg<T, E>::KT;
+    k.mi = SimtCfg<T, E>::MI;
+    k.smem = SimtCfg<T, E>::SMEM;
+    return k;
+}
+template <class T> static TreeKernel tree_pick_e(int E) {
+    return E == 64 ? simt_kernel<T, 64>() : E == 128 ? simt_kernel<T, 128>() : simt_kernel<T, 256>();
+}
+static TreeKernel tree_pick(const dvattn_tree_args* a) {
+    return a->dtype == DVATTN_FLOAT32 ? tree_pick_e<float>(a->E)
+         : a->dtype == DVATTN_FLOAT16 ? tree_pick_e<__half>(a->E) : tree_pick_e<__nv_bfloat16>(a->E);
+}
+
+static int tree_validate(const dvattn_tree_args* a) {
+    if (!a) return DVATTN_ERR_INVALID_ARGUMENT;
+    dvattn_paged_args v{};  // the shape rules of the paged attention
+    v.dtype = a->dtype; v.F = a->F; v.W = a->W; v.Hq = a->Hq; v.Hkv = a->Hkv; v.E = a->E; v.Ev = a->Ev; v.S = a->S;
+    v.R = a->R; v.block_size = a->block_size; v.max_blocks_per_seq = a->max_blocks_per_seq; v.num_blocks = a->num_blocks;
+    const int st = decode_validate(&v);
+    if (st != DVATTN_OK) return st;
+    if (a->F < 1) return DVATTN_ERR_INVALID_ARGUMENT;  // the drafted tokens belong to the last turn
+    if (a->S > kTreeMaxTokens) return DVATTN_ERR_UNSUPPORTED;
+    // grid limits: sequences are the prep grid's x, heads its y; items are the merge grid's x
+    const long long rows = (long long)a->S * (a->Hq / a->Hkv);
+    if (a->Hkv > 65535 || (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
+    return DVATTN_OK;
+}
+
+struct TreeLayout {
+    size_t nwin, span, anc, dkr, po, pl, total;
+    int groups, sw, nt;
+};
+
+static int tree_layout(const dvattn_tree_args* a, const TreeKernel& k, TreeLayout& L) {
+    int dev = 0, sms = 0, occ = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return DVATTN_ERR_CUDA;
+    if (cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem) != cudaSuccess) return DVATTN_ERR_CUDA;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k.fn, k.threads, k.smem) != cudaSuccess || occ < 1)
+        return DVATTN_ERR_CUDA;
+    L.groups = sms * occ / a->Hkv;
+    if (L.groups < 1) L.groups = 1;
+    L.sw = (a->S + 127) / 128 * 4;
+    L.nt = (int)(((long long)a->S * (a->Hq / a->Hkv) + k.mi - 1) / k.mi);
+    const size_t ctas = (size_t)L.groups * a->Hkv, esz = a->dtype == DVATTN_FLOAT32 ? 4 : 2;
+    size_t at = 256;
+    auto take = [&](size_t bytes) {
+        const size_t r = at;
+        at += (bytes + 255) / 256 * 256;
+        return r;
+    };
+    L.nwin = take(4 * (size_t)a->W);
+    L.span = take(4 * (size_t)a->W * a->F);
+    L.anc = take(4 * (size_t)a->W * a->S * L.sw);
+    L.dkr = take(esz * (size_t)a->W * a->Hkv * a->S * a->E);
+    L.po = take(4 * ctas * 2 * k.mi * a->E);
+    L.pl = take(4 * ctas * 2 * k.mi);
+    L.total = at;
+    return DVATTN_OK;
+}
+
+size_t tree_workspace_size(const dvattn_tree_args* a) {
+    if (tree_validate(a) != DVATTN_OK || (long long)a->W * a->S == 0 || a->Hq == 0) return 0;
+    TreeLayout L;
+    return tree_layout(a, tree_pick(a), L) == DVATTN_OK ? L.total : 0;
+}
+
+static bool aligned16(const void* x) { return !(reinterpret_cast<uintptr_t>(x) & 15); }
+
+template <class T> static const void* merge_fn(int E) {
+    return E == 64 ? (const void*)&tree_merge_kernel<T, 64> : E == 128 ? (const void*)&tree_merge_kernel<T, 128>
+                                                                      : (const void*)&tree_merge_kernel<T, 256>;
+}
+
+int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaStream_t stream) {
+    int st = tree_validate(a);
+    if (st != DVATTN_OK) return st;
+    if ((long long)a->W * a->S == 0 || a->Hq == 0) return DVATTN_OK;
+    if (!a->out || !a->queries || !a->parents || !a->locations || !a->fragment_lengths || !a->draft_keys || !a->draft_values ||
+        (a->R > 0 && (!a->cosines || !a->sines)))
+        return DVATTN_ERR_INVALID_ARGUMENT;
+    if (a->max_blocks_per_seq > 0 && a->num_blocks > 0 && (!a->k_cache || !a->v_cache || !a->block_tables))
+        return DVATTN_ERR_INVALID_ARGUMENT;
+    for (const void* x : {a->queries, a->k_cache, a->v_cache, a->draft_keys, a->draft_values, (const void*)a->out})
+        if (!aligned16(x)) return DVATTN_ERR_INVALID_ARGUMENT;
+    const TreeKernel k = tree_pick(a);
+    TreeLayout L;
+    if ((st = tree_layout(a, k, L)) != DVATTN_OK) return st;
+    if (!workspace || wbytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return DVATTN_ERR_WORKSPACE;
+    char* ws = static_cast<char*>(workspace);
+    TreeParams p{};
+    p.F = a->F; p.W = a->W; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.S = a->S; p.R = a->R;
+    p.tail = a->S; p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
+    const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
+    p.cap = a->num_blocks <= 0 ? 0 : cap > 0x7fffffffLL ? 0x7fffffff : (int)cap;
+    p.SW = L.sw; p.kt = k.kt; p.mi = k.mi; p.nt = L.nt; p.groups = L.groups;
+    p.scale_log2 = a->scale * kLog2e;
+    p.out = a->out; p.lse_out = a->lse_out; p.q = a->queries; p.cos = a->cosines; p.sin = a->sines;
+    p.loc = a->locations; p.L = a->fragment_lengths; p.parents = a->parents;
+    p.k = a->k_cache ? a->k_cache : a->draft_keys; p.v = a->v_cache ? a->v_cache : a->draft_values;
+    p.bt = a->block_tables; p.dk = a->draft_keys; p.dv = a->draft_values;
+    p.header = reinterpret_cast<int*>(ws);
+    p.nwin = reinterpret_cast<int*>(ws + L.nwin);
+    p.span = reinterpret_cast<int*>(ws + L.span);
+    p.anc = reinterpret_cast<uint32_t*>(ws + L.anc);
+    p.dkr = ws + L.dkr;
+    p.part_o = reinterpret_cast<float*>(ws + L.po);
+    p.part_lse = reinterpret_cast<float*>(ws + L.pl);
+
+    const void* prep = a->dtype == DVATTN_FLOAT32   ? (const void*)&tree_prep_kernel<float>
+                       : a->dtype == DVATTN_FLOAT16 ? (const void*)&tree_prep_kernel<__half> : (const void*)&tree_prep_kernel<__nv_bfloat16>;
+    const void* merge = a->dtype == DVATTN_FLOAT32   ? merge_fn<float>(a->E)
+                        : a->dtype == DVATTN_FLOAT16 ? merge_fn<__half>(a->E) : merge_fn<__nv_bfloat16>(a->E);
+    int E = a->E;
+    void* pargs[] = {&p, &E};
+    if (cudaLaunchKernel(prep, dim3(a->W, a->Hkv), dim3(128), pargs, sizeof(int) * (size_t)a->S, stream) != cudaSuccess)
+        return DVATTN_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.stream = stream;
+    cfg.gridDim = dim3((unsigned)(L.groups * a->Hkv));
+    cfg.blockDim = dim3(k.threads);
+    cfg.dynamicSmemBytes = k.smem;
+    void* args[] = {&p};
+    cudaError_t e = cudaLaunchKernelExC(&cfg, k.fn, args);
+    if (e == cudaSuccess) {
+        const int rpb = 256 / (a->E / 4), rows_max = L.nt > 1 ? k.mi : a->S * p.G;
+        cfg.gridDim = dim3((unsigned)((long long)a->W * L.nt * a->Hkv), (unsigned)((rows_max + rpb - 1) / rpb));
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        e = cudaLaunchKernelExC(&cfg, merge, args);
+    }
+    if (e != cudaSuccess) {
+        if (getenv("DVATTN_DEBUG")) fprintf(stderr, "dvattn tree launch: %s\n", cudaGetErrorString(e));
+        return DVATTN_ERR_CUDA;
+    }
+    return cudaGetLastError() == cudaSuccess ? DVATTN_OK : DVATTN_ERR_CUDA;
+}
+
+}  // namespace dvb

@@ -1,0 +1,47 @@
+// What the draft-tree attention kernels share: the call's parameters.
+//
+// A call attends, for every sequence w, the S tokens of a drafted tree over the sequence's
+// cached turns and over the tree itself: token s sees the cached keys its locations let it
+// see and the drafted keys of its ancestors (and its own).  All S * G query rows of a KV
+// head (row r = token r / G, head r % G of the group) read the same keys, so an item is
+// (w, row tile of `mi` rows, KV head), and its windows (turns.cuh) end with the drafted
+// keys.  A CTA's range that starts or ends inside an item leaves a partial result (two slots
+// per CTA: 0 for the piece that continues an item, 1 for the piece that starts one), merged
+// by tree_merge_kernel.
+#pragma once
+
+#include "turns.cuh"
+
+namespace dvb {
+
+struct TreeParams : TurnSplit {
+    int Hq, Hkv, G, S, R;
+    int SW;  // 32-bit words of a token's ancestor set, a multiple of 4
+    int mi;  // rows per item
+    float scale_log2;
+    void* out;
+    float* lse_out;
+    const void* q;
+    const float* cos;
+    const float* sin;
+    const int* parents;
+    const void* k;
+    const void* v;
+    const void* dk;
+    const void* dv;
+    // workspace
+    int* header;      // [3] error word (kErrorWordOffset)
+    uint32_t* anc;    // [W][S][SW] ancestor sets; a token that is not there has an empty one
+    void* dkr;        // [W][Hkv][S][E] T, drafted keys rotated
+    float* part_o;    // [CTAs][2][mi][E] normalised partial outputs
+    float* part_lse;  // [CTAs][2][mi] log2 sums, -inf: nothing seen
+};
+
+// An attention kernel and its launch shape.
+struct TreeKernel {
+    const void* fn;
+    int threads, kt, mi;
+    size_t smem;
+};
+
+}  // namespace dvb

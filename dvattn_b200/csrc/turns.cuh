@@ -1,0 +1,127 @@
+// Work split over the cached turns of a batch, shared by the kernels in which all query rows
+// of a sequence's KV head read the same keys (tree.cu, tree_tc.cu, mass.cu).
+//
+// A sequence's keys are cut into windows of `kt` keys: each turn's visible keys (the union
+// over the queries) from the turn's first key on, then `tail` keys that lie outside the
+// cache (the drafted tokens of a tree; 0 where there are none).  The windows of all
+// (sequence, row tile) pairs, one after the other, are cut into `groups` ranges of equal
+// length.  A group is Hkv CTAs that walk the same range, one KV head each, so the heads of a
+// token (contiguous in a page) are read at about the same time.
+#pragma once
+
+#include "decode.cuh"
+
+namespace dvb {
+
+struct TurnSplit {
+    int F, W, BS, maxb, cap, tail;
+    int kt, nt, groups;  // keys per window, row tiles per sequence, CTA groups
+    long long NB;
+    const int* loc;
+    const int* L;
+    const int* bt;
+    int* nwin;  // workspace: [W] windows of a sequence's row tile
+    int* span;  // workspace: [W][F] keys of the turn that some query of the sequence sees
+};
+
+// Keys of a turn that a query with location `loc` sees, the turn starting at logical
+// position `off`: l <= loc, l < L and off + l < cap.
+__device__ __forceinline__ int turn_seen(int L, int loc, long long off, int cap) {
+    if (loc < 0 || L <= 0 || off >= cap) return 0;
+    const int v = loc >= L ? L : loc + 1;
+    const long long room = cap - off;
+    return v < room ? v : (int)room;
+}
+
+__device__ __forceinline__ long long split_bound(long long total, int g, int groups) { return total * g / groups; }
+
+// Totals and the position of unit `at` among the windows, by one whole warp (every lane
+// returns the same values): `w` the sequence, `base` the first unit of its windows.
+__device__ __forceinline__ long long split_total(const TurnSplit& p, int lane) {
+    long long t = 0;
+    for (int w = lane; w < p.W; w += 32) t += __ldcg(p.nwin + w);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    return t * p.nt;
+}
+__device__ __forceinline__ void split_locate(const TurnSplit& p, int lane, long long at, int& w, long long& base) {
+    long long acc = 0;
+    for (int w0 = 0; w0 < p.W; w0 += 32) {
+        const long long mine = w0 + lane < p.W ? (long long)__ldcg(p.nwin + w0 + lane) * p.nt : 0;
+        long long incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, mine > 0 && at >= acc + incl - mine && at < acc + incl);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            w = w0 + src;
+            base = acc + __shfl_sync(0xffffffffu, incl - mine, src);
+            return;
+        }
+        acc += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    w = p.W;
+    base = acc;
+}
+
+// A piece of a CTA's range: windows [i0, i1) of the nw windows of item (w, t, h).
+struct SplitPiece {
+    int w, t, i0, i1, nw;
+    __device__ __forceinline__ bool whole() const { return i0 == 0 && i1 == nw; }
+    __device__ __forceinline__ int slot() const { return i0 == 0 ? 1 : 0; }
+};
+// Walks a range [u, u1) of units; every role of a CTA walks it for itself.
+struct SplitWalk {
+    long long u, u1, base;
+    int w;
+    __device__ __forceinline__ bool next(const TurnSplit& p, SplitPiece& pc) {
+        while (u < u1 && w < p.W) {
+            const int nw = __ldcg(p.nwin + w);
+            const long long end = base + (long long)nw * p.nt;
+            if (u >= end) {
+                base = end;
+                ++w;
+                continue;
+            }
+            const long long local = u - base;
+            pc.w = w;
+            pc.nw = nw;
+            pc.t = (int)(local / nw);
+            pc.i0 = (int)(local - (long long)pc.t * nw);
+            const long long left = u1 - u;
+            pc.i1 = left < nw - pc.i0 ? pc.i0 + (int)left : nw;
+            u += pc.i1 - pc.i0;
+            return true;
+        }
+        return false;
+    }
+};
+
+// The turn and the keys of window i of a sequence: keys [k0, k0 + n) of turn f, or of the
+// tail where f == F.  `f`, `first` (the turn's first window) and `off` carry over
+// between calls with increasing i; start with f = first = off = 0.
+struct SplitWin {
+    int f, first, k0, n;
+    long long off;
+    __device__ __forceinline__ void start() { f = 0, first = 0, off = 0; }
+    __device__ __forceinline__ void seek(const TurnSplit& p, int w, int i) {
+        for (; f < p.F; ++f) {
+            const int sp = __ldcg(p.span + (size_t)w * p.F + f), nf = (sp + p.kt - 1) / p.kt;
+            if (i < first + nf) {
+                k0 = (i - first) * p.kt;
+                n = min(p.kt, sp - k0);
+                return;
+            }
+            first += nf;
+            const int Lf = __ldg(p.L + f);
+            off += Lf > 0 ? Lf : 0;
+        }
+        k0 = (i - first) * p.kt;
+        n = min(p.kt, p.tail - k0);
+    }
+};
+
+}  // namespace dvb

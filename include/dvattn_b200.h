@@ -174,6 +174,118 @@ typedef struct dvattn_rotary_args {
     const float* inv_freq;        /* [R/2] f32 or null (1 / rope_base^(2j/R) on device)  */
 } dvattn_rotary_args;
 
+/*
+ * Arguments of one draft-tree attention call: the S drafted tokens of every sequence attend
+ * over its cached turns and over the tree.  parents[w][s] is the index of token s's parent
+ * among the S (it comes before s), -1 for a child of the cached context, anything else
+ * (below -1, or not before s) for a token that is not there; the descendants of such a token
+ * are not there either.  Token s sees the cached keys l <= locations[f,w,s] of every turn
+ * (locations: the last cached key it sees, not its own position) and the drafted keys of its
+ * ancestors and itself.  cosines/sines[f,w,s] rotate its query for turn f; those of the last
+ * turn rotate its key as well.  A token that is not there gets zeros (lse: -inf).
+ */
+typedef struct dvattn_tree_args {
+    int dtype;
+    int F, W, Hq, Hkv, E, Ev, S;  /* F >= 1; S <= 1024                                   */
+    int R;                        /* rotary dim = cosines.size(3)                        */
+    int block_size;
+    int max_blocks_per_seq;
+    long long num_blocks;
+    float scale;
+    void* out;                    /* [W,Hq,S,Ev] T                                       */
+    const void* queries;          /* [W,Hq,S,E] T, unrotated                             */
+    const int* parents;           /* [W,S] i32                                           */
+    const float* cosines;         /* [F,W,S,R] f32 (the first R/2 entries are read)      */
+    const float* sines;
+    const int* locations;         /* [F,W,S] i32                                         */
+    const int* fragment_lengths;  /* [F] i32                                             */
+    const void* k_cache;          /* [NB,BS,Hkv,E] T                                     */
+    const void* v_cache;          /* [NB,BS,Hkv,Ev] T                                    */
+    const int* block_tables;      /* [W,max_blocks] i32                                  */
+    const void* draft_keys;       /* [W,Hkv,S,E] T, unrotated                            */
+    const void* draft_values;     /* [W,Hkv,S,Ev] T                                      */
+    float* lse_out;               /* optional [W,Hq,S] natural-log LSE of scale*q.k      */
+} dvattn_tree_args;
+
+/*
+ * Arguments of the append of a drafted tree's accepted tokens: entry i < counts[w] of
+ * sequence w writes the key (rotated as in dvattn_paged_append) and value of drafted token
+ * accepted[w][i] at logical position positions[w] + i.
+ */
+typedef struct dvattn_tree_append_args {
+    int dtype;
+    int W, Hkv, E, Ev;
+    int S;                        /* drafted tokens per sequence                         */
+    int A;                        /* entries of `accepted` per sequence                  */
+    int R;
+    int block_size;
+    int max_blocks_per_seq;
+    long long num_blocks;
+    void* k_cache;                /* [NB,BS,Hkv,E] T, written                            */
+    void* v_cache;                /* [NB,BS,Hkv,Ev] T, written                           */
+    const void* draft_keys;       /* [W,Hkv,S,E] T, unrotated                            */
+    const void* draft_values;     /* [W,Hkv,S,Ev] T                                      */
+    const float* cosines;         /* [W,S,R] f32, full width (both halves read)          */
+    const float* sines;
+    const int* block_tables;      /* [W,max_blocks] i32                                  */
+    const int* positions;         /* [W] i32                                             */
+    const int* accepted;          /* [W,A] i32; entries outside [0,S) are skipped        */
+    const int* counts;            /* [W] i32 or null (all A)                             */
+} dvattn_tree_append_args;
+
+/*
+ * Arguments of the accumulation of attention weight: mass[w,h,p] grows by the softmax weight
+ * that the key at logical position p of sequence w and KV head h received from the queries
+ * [W,Hq,S,E] of one attention call, whose lse is given.  A query whose lse is -inf adds
+ * nothing.  Positions at and past `positions` are not accumulated.
+ */
+typedef struct dvattn_mass_args {
+    int dtype;
+    int F, W, Hq, Hkv, E, S, R;
+    int block_size;
+    int max_blocks_per_seq;
+    long long num_blocks;
+    long long positions;          /* mass.size(2)                                        */
+    float scale;
+    float* mass;                  /* [W,Hkv,positions] f32, added to                     */
+    const void* queries;          /* [W,Hq,S,E] T, unrotated                             */
+    const float* lse;             /* [W,Hq,S] f32, natural log                           */
+    const float* cosines;         /* [F,W,S,R] f32 (the first R/2 entries are read)      */
+    const float* sines;
+    const int* locations;         /* [F,W,S] i32                                         */
+    const int* fragment_lengths;  /* [F] i32                                             */
+    const void* k_cache;          /* [NB,BS,Hkv,E] T                                     */
+    const int* block_tables;      /* [W,max_blocks] i32                                  */
+} dvattn_mass_args;
+
+/*
+ * Arguments of the eviction of the least attended keys.  Of the lengths[w] tokens at logical
+ * positions starts[w] + i, every KV head keeps keep[w] of its own: the first `sink`, the last
+ * `recent`, then those of largest mass (NaN after everything else; equal ones by position).
+ * Survivors in front of keep[w] stay in place, the i-th freed position there is filled by the
+ * i-th survivor behind it.  The range's pages belong to sequence w alone.
+ */
+typedef struct dvattn_evict_args {
+    int dtype;
+    int W, Hkv, E, Ev;
+    int block_size;
+    int max_blocks_per_seq;
+    int sink, recent;
+    long long num_blocks;
+    long long positions;          /* mass.size(2); the range is cut off there            */
+    void* k_cache;                /* [NB,BS,Hkv,E] T, rows moved                         */
+    void* v_cache;                /* [NB,BS,Hkv,Ev] T, rows moved                        */
+    const float* mass;            /* [W,Hkv,positions] f32                               */
+    float* mass_out;              /* [W,Hkv,positions] f32: the mass of the key now at each
+                                     position, 0 where keys left; may be `mass` itself   */
+    int* source;                  /* optional [W,Hkv,positions] i32: the position that each
+                                     position's key came from, -1 where keys left        */
+    const int* block_tables;      /* [W,max_blocks] i32                                  */
+    const int* starts;            /* [W] i32                                             */
+    const int* lengths;           /* [W] i32                                             */
+    const int* keep;              /* [W] i32                                             */
+} dvattn_evict_args;
+
 /* ABI version of this header (bumped on any layout change of the structs above). */
 int dvattn_abi_version(void);
 
@@ -307,6 +419,25 @@ int dvattn_paged_sdpa_rope(const dvattn_paged_args* args, const dvattn_rotary_ar
 size_t dvattn_varlen_paged_sdpa_rope_workspace_size(const dvattn_varlen_args* args, const dvattn_rotary_args* rotary);
 int dvattn_varlen_paged_sdpa_rope(const dvattn_varlen_args* args, const dvattn_rotary_args* rotary, void* workspace,
                                   size_t workspace_bytes, dvattn_stream_t stream);
+
+/*
+ * Attention of a drafted tree over the paged cache and itself (speculative decoding: all
+ * drafted tokens verified in one pass that reads the cache once).  The cache is not written:
+ * the accepted tokens enter it with dvattn_tree_append, rejected ones leave no trace.  No
+ * counterpart in the reference.  Workspace and status as for dvattn_paged_sdpa.
+ */
+size_t dvattn_tree_sdpa_workspace_size(const dvattn_tree_args* args);
+int dvattn_tree_sdpa(const dvattn_tree_args* args, void* workspace, size_t workspace_bytes, dvattn_stream_t stream);
+int dvattn_tree_append(const dvattn_tree_append_args* args, dvattn_stream_t stream);
+
+/*
+ * A bounded cache: dvattn_paged_mass adds up the attention weight of every cached key,
+ * dvattn_paged_evict lets the least attended ones go.  No counterpart in the reference.
+ */
+size_t dvattn_paged_mass_workspace_size(const dvattn_mass_args* args);
+int dvattn_paged_mass(const dvattn_mass_args* args, void* workspace, size_t workspace_bytes, dvattn_stream_t stream);
+size_t dvattn_paged_evict_workspace_size(const dvattn_evict_args* args);
+int dvattn_paged_evict(const dvattn_evict_args* args, void* workspace, size_t workspace_bytes, dvattn_stream_t stream);
 
 /*
  * Standalone query rotation, schema `dvattn_rope` (src/binding.cu:41-77, src/rope.cuh:2-65):
