@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(256, APPEND_MINB) paged_append_kernel(AppendPa
     }
 }
 
-// `accepted`: null for the plain append, else [W][m] (tree_append_launch).
-static int append_launch(const dvattn_append_args* a, const int* accepted, int m, cudaStream_t stream) {
+// The plain append, or with `tree` that of a drafted tree's accepted tokens, [W][m].
+static int append_launch(const dvattn_append_args* a, bool tree, const int* accepted, int m, cudaStream_t stream) {
     if (a->dtype < 0 || a->dtype > 2) return DVATTN_ERR_UNSUPPORTED;
     if (a->W < 0 || a->n < 0 || a->Hkv <= 0 || a->E <= 0 || a->Ev <= 0 || a->R < 0 || a->R > a->E || (a->R & 1) ||
         a->block_size <= 0 || a->max_blocks_per_seq < 0 || a->num_blocks < 0)
@@ -190,7 +190,7 @@ static int append_launch(const dvattn_append_args* a, const int* accepted, int m
     if ((long long)a->W * a->n >= (1LL << 31) || (long long)a->W * m >= (1LL << 31) || (long long)a->max_blocks_per_seq * a->block_size >= (1LL << 31))
         return DVATTN_ERR_UNSUPPORTED;
     if (!a->k_cache || !a->v_cache || !a->keys || !a->values || !a->block_tables || !a->positions ||
-        (a->R > 0 && (!a->cosines || !a->sines)))
+        (a->R > 0 && (!a->cosines || !a->sines)) || (tree && !accepted))
         return DVATTN_ERR_INVALID_ARGUMENT;
     for (const void* q : {(const void*)a->k_cache, (const void*)a->v_cache, a->keys, a->values})
         if (reinterpret_cast<uintptr_t>(q) & 15) return DVATTN_ERR_INVALID_ARGUMENT;
@@ -221,7 +221,7 @@ static int append_launch(const dvattn_append_args* a, const int* accepted, int m
 
 int paged_append_launch(const dvattn_append_args* a, cudaStream_t stream) {
     if (!a) return DVATTN_ERR_INVALID_ARGUMENT;
-    return append_launch(a, nullptr, a->n, stream);
+    return append_launch(a, false, nullptr, a->n, stream);
 }
 
 int tree_append_launch(const dvattn_tree_append_args* t, cudaStream_t stream) {
@@ -232,8 +232,7 @@ int tree_append_launch(const dvattn_tree_append_args* t, cudaStream_t stream) {
     a.k_cache = t->k_cache; a.v_cache = t->v_cache; a.keys = t->draft_keys; a.values = t->draft_values;
     a.cosines = t->cosines; a.sines = t->sines; a.block_tables = t->block_tables; a.positions = t->positions;
     a.counts = t->counts;
-    if ((long long)t->W * t->S > 0 && t->A > 0 && !t->accepted) return DVATTN_ERR_INVALID_ARGUMENT;
-    return append_launch(&a, t->accepted, t->A, stream);
+    return append_launch(&a, true, t->accepted, t->A, stream);
 }
 
 }  // namespace dvb

@@ -59,7 +59,7 @@ def test_validation(name, make, kw, status):
 
 
 @pytest.mark.parametrize("kw,status", [(dict(dtype=9), UNSUPPORTED), (dict(A=-1), INVALID), (dict(S=-1), INVALID), (dict(R=33), INVALID),
-                                       (dict(E=4), UNSUPPORTED), (dict(), INVALID)])
+                                       (dict(E=36), UNSUPPORTED), (dict(), INVALID)])
 def test_append_validation(kw, status):
     assert LIB.dvattn_tree_append(ctypes.byref(append(**kw)), None) == status
 
