@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
     SplitPiece pc;
     while (walk.next(p, pc)) {
         SplitWin win;
-        win.start();
+        win.start(p, pc.w);
         for (int i = pc.i0; i < pc.i1; ++i) {
             win.seek(p, pc.w, i);
             for (int c = tid; c < KT * CH; c += 256) {

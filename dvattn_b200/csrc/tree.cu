@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
     SplitPiece pc;
     while (walk.next(p, pc)) {
         SplitWin ld, win;
-        ld.start();
-        win.start();
+        ld.start(p, pc.w);
+        win.start(p, pc.w);
         auto load = [&](int i, int st) {
             ld.seek(p, pc.w, i);
             for (int c = tid; c < KT * CH; c += C::THREADS) {
@@ -379,12 +379,18 @@ template <class T, int E> static TreeKernel simt_kernel() {
     k.smem = SimtCfg<T, E>::SMEM;
     return k;
 }
-template <class T> static TreeKernel tree_pick_e(int E) {
-    return E == 64 ? simt_kernel<T, 64>() : E == 128 ? simt_kernel<T, 128>() : simt_kernel<T, 256>();
-}
 static TreeKernel tree_pick(const dvattn_tree_args* a) {
-    return a->dtype == DVATTN_FLOAT32 ? tree_pick_e<float>(a->E)
-         : a->dtype == DVATTN_FLOAT16 ? tree_pick_e<__half>(a->E) : tree_pick_e<__nv_bfloat16>(a->E);
+    if (a->dtype != DVATTN_FLOAT32) return tree_tc_pick(a->dtype, a->E, a->S * (a->Hq / a->Hkv));
+    return a->E == 64 ? simt_kernel<float, 64>() : a->E == 128 ? simt_kernel<float, 128>() : simt_kernel<float, 256>();
+}
+
+// DVATTN_TEST_STALL_TILE=<i>: tests only (see the decode launcher); read once per process.
+static int tree_stall_hook() {
+    static const int t = [] {
+        const char* e = getenv("DVATTN_TEST_STALL_TILE");
+        return e && *e ? atoi(e) : -1;
+    }();
+    return t;
 }
 
 static int tree_validate(const dvattn_tree_args* a) {
@@ -475,6 +481,7 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     p.loc = a->locations; p.L = a->fragment_lengths; p.parents = a->parents;
     p.k = a->k_cache ? a->k_cache : a->draft_keys; p.v = a->v_cache ? a->v_cache : a->draft_values;
     p.bt = a->block_tables; p.dk = a->draft_keys; p.dv = a->draft_values;
+    p.stall_tile = tree_stall_hook();
     p.header = reinterpret_cast<int*>(ws);
     p.nwin = reinterpret_cast<int*>(ws + L.nwin);
     p.span = reinterpret_cast<int*>(ws + L.span);

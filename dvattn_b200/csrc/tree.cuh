@@ -18,6 +18,7 @@ struct TreeParams : TurnSplit {
     int Hq, Hkv, G, S, R;
     int SW;  // 32-bit words of a token's ancestor set, a multiple of 4
     int mi;  // rows per item
+    int stall_tile;  // test hook (DVATTN_TEST_STALL_TILE), -1: off
     float scale_log2;
     void* out;
     float* lse_out;
@@ -43,5 +44,7 @@ struct TreeKernel {
     int threads, kt, mi;
     size_t smem;
 };
+// the 16-bit kernel on the 5th-generation tensor cores (tree_tc.cu)
+TreeKernel tree_tc_pick(int dtype, int E, int rows);
 
 }  // namespace dvb

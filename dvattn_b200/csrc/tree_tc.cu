@@ -1,0 +1,555 @@
+// Draft-tree attention on the 5th-generation tensor cores (tcgen05 + TMEM), 16-bit types.
+//
+// A CTA walks a range of key windows (turns.cuh).  Jobs: a job is S = Q K^T of one 128-row
+// query tile and one window, its softmax, and O += P V.  Job j uses score buffer j & 1 of
+// TMEM, and the tensor core issues S(j + 1) before PV(j), so it works for one job while the
+// other's softmax runs.  What job j is depends on the rows of a KV head:
+//   more than 128 rows: two row tiles share every window; j & 1 is the tile;
+//   up to 128 rows:     one tile; the windows alternate between two independent halves, each
+//                       with its own running maximum, sum and O, joined at the end of a piece
+//                       (one tile's chain softmax -> PV -> next S would not keep up with HBM);
+//   head dim 256:       one tile and one O (256 columns); only the score buffers alternate.
+// Warps: 4 per softmax group (a thread owns one query row = one TMEM lane), one MMA issuer,
+// one K and one V producer.  Producers gather rows with cp.async (any page size; rows that
+// nobody sees are zero-filled, so what lies there never matters) into swizzled rings.
+//
+// Every wait is bounded; one that gives up sets the call's error word, ends the CTA with
+// nothing in flight, and tree_merge_kernel writes NaN to all outputs of the call.
+#include "tcgen05.cuh"
+#include "tree.cuh"
+
+namespace dvb {
+
+template <int E> struct TcCfg {
+    static constexpr int KT = E == 256 ? 64 : 128;  // keys per window
+    static constexpr int NG = E == 256 ? 1 : 2;     // softmax groups (and O accumulators)
+    static constexpr int NP = E / 64;               // 64-column panels
+    static constexpr int QPANEL = 128 * 128, KPANEL = KT * 128, QTILE = NP * QPANEL, KTILE = NP * KPANEL;
+    static constexpr int NT = (4 * NG + 3) * 32;
+    static constexpr int WARP_MMA = 4 * NG, WARP_K = 4 * NG + 1, WARP_V = 4 * NG + 2;
+    static constexpr int RING = E == 64 ? 4 : 3;    // most stages of a ring
+    // tiles of 32 KB (16 KB at E = 64): Q, the K ring, the V ring
+    static constexpr int K_STAGES = E == 64 ? 4 : E == 256 ? 2 : 3;
+    __host__ __device__ static constexpr int v_stages(bool two) { return E == 64 ? 4 : E == 256 ? 3 : two ? 2 : 3; }
+    __host__ __device__ static constexpr int q_bytes(bool two) { return two ? 2 * QTILE : QTILE; }
+    static constexpr int OFF_BAR = E == 64 ? 2 * QTILE + 8 * KTILE : 7 * 32768;
+    static constexpr int OFF_MISC = OFF_BAR + 32 * 8;
+    static constexpr int OFF_ML = OFF_MISC + 64;    // [2][128] (maximum, sum)
+    static constexpr int SMEM = OFF_ML + 2 * 128 * 8;
+    static_assert(SMEM <= 232448, "more shared memory than a CTA may use");
+};
+
+template <class T, int E>
+__global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p) {
+    using C = TcCfg<E>;
+    constexpr int KT = C::KT, NG = C::NG;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    const uint32_t s0 = smem_u32(smem);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const bool bf16 = Elem<T>::dtype == DVATTN_BFLOAT16;
+    const bool two = p.mi == 256;
+    const int VS = C::v_stages(two);
+    const uint32_t off_k = C::q_bytes(two), off_v = off_k + C::K_STAGES * C::KTILE;
+    const uint32_t bar = s0 + C::OFF_BAR;
+    const uint32_t k_full = bar, k_empty = bar + 32, v_full = bar + 64, v_empty = bar + 96;
+    const uint32_t s_full = bar + 128, p_full = bar + 144, q_ready = bar + 160, o_done = bar + 176, epi1 = bar + 184, epi2 = bar + 192;
+    volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
+    if (tid == 0) {
+        for (int s = 0; s < C::RING; ++s) {
+            mbar_init(k_full + 8 * s, 32);
+            mbar_init(k_empty + 8 * s, 1);
+            mbar_init(v_full + 8 * s, 32);
+            mbar_init(v_empty + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(s_full + 8 * s, 1);
+            mbar_init(p_full + 8 * s, 128);
+            mbar_init(q_ready + 8 * s, two ? 128 : 128 * NG);
+        }
+        mbar_init(o_done, 1);
+        mbar_init(epi1, 128 * NG);
+        mbar_init(epi2, 128 * NG);
+        *s_abort = 0;
+        fence_mbar_init();
+    }
+    // TMEM columns: scores (P over them) at 0 and KT, O at 256 and 384
+    if (wid == C::WARP_MMA) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(s0 + C::OFF_MISC) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + C::OFF_MISC);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
+    SplitWalk walk;
+    {
+        const long long total = split_total(p, lane);
+        walk.u = split_bound(total, g, p.groups);
+        walk.u1 = split_bound(total, g + 1, p.groups);
+        split_locate(p, lane, walk.u, walk.w, walk.base);
+    }
+    SplitPiece pc;
+    SplitWin win;
+    // a whole warp waits, and gives up as a whole
+    auto wait = [&](uint32_t b, int phase) { return __all_sync(0xffffffffu, mbar_wait(b, phase & 1)); };
+    auto wait_lazy = [&](uint32_t b, int phase) { return __all_sync(0xffffffffu, mbar_wait_lazy(b, phase & 1)); };
+    auto give_up = [&](int bit) {
+        if (lane == 0) {
+            *s_abort = 1;
+            atomicOr(p.header + 3, bit);
+        }
+    };
+
+    if (wid == C::WARP_K || wid == C::WARP_V) {
+        // ================================ producers ================================
+        const bool is_k = wid == C::WARP_K;
+        const int stages = is_k ? C::K_STAGES : VS;
+        const uint32_t full = is_k ? k_full : v_full, empty = is_k ? k_empty : v_empty, ring = s0 + (is_k ? off_k : off_v);
+        const T* cache = static_cast<const T*>(is_k ? p.k : p.v);
+        const T* draft = static_cast<const T*>(is_k ? p.dkr : p.dv);
+        constexpr int NR = KT / 32;      // rows of a window whose addresses a lane finds
+        constexpr int CH = E / 8;        // 16-byte chunks of a row
+        constexpr int RPI = 32 / CH;     // rows per copy instruction
+        const T* next[NR];               // rows lane + 32 k of the next window, null: zeros
+        auto find = [&](int i) {
+            win.seek(p, pc.w, i);
+#pragma unroll
+            for (int k = 0; k < NR; ++k) {
+                const int r = lane + 32 * k, l = win.k0 + r;
+                next[k] = nullptr;
+                if (r >= win.n) continue;
+                if (win.f == p.F) {
+                    if (__ldcg(p.anc + ((size_t)pc.w * p.S + l) * p.SW + (l >> 5)) >> (l & 31) & 1u)
+                        next[k] = draft + (((size_t)pc.w * p.Hkv + h) * p.S + l) * E;
+                } else {
+                    const int pos = (int)win.off + l;
+                    const int page = __ldg(p.bt + (size_t)pc.w * p.maxb + pos / p.BS);
+                    if (page >= 0 && page < p.NB) next[k] = cache + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E;
+                }
+            }
+        };
+        int iw = 0, signalled = 0;  // windows requested, windows handed over
+        auto hand_over = [&](int upto) {  // their copies have landed
+            fence_proxy_async_smem();
+            // test hook: CTA 0's K windows from stall_tile on never arrive
+            if (is_k && blockIdx.x == 0 && p.stall_tile >= 0) upto = min(upto, p.stall_tile);
+            for (; signalled < upto; ++signalled) mbar_arrive(full + 8 * (signalled % stages));
+        };
+        bool ok = true;
+        while (ok && walk.next(p, pc)) {
+            win.start(p, pc.w);
+            find(pc.i0);
+            for (int i = pc.i0; i < pc.i1; ++i, ++iw) {
+                const int st = iw % stages;
+                if (iw >= stages) {
+                    const int ph = iw / stages - 1;
+                    if (!__all_sync(0xffffffffu, mbar_try_wait(empty + 8 * st, ph & 1))) {
+                        // about to wait: hand over what is under way first
+                        cp_async_wait<0>();
+                        hand_over(iw);
+                        if (*s_abort || !wait_lazy(empty + 8 * st, ph)) {
+                            ok = false;
+                            break;
+                        }
+                    }
+                }
+                const T* row[NR];
+#pragma unroll
+                for (int k = 0; k < NR; ++k) row[k] = next[k];
+                if (i + 1 < pc.i1) find(i + 1);
+                const uint32_t dst = ring + (uint32_t)(st * C::KTILE);
+                const int ch = lane % CH;
+#pragma unroll
+                for (int k = 0; k < NR; ++k) {
+                    const unsigned long long mine = reinterpret_cast<unsigned long long>(row[k]);
+#pragma unroll 4
+                    for (int x = 0; x < CH; ++x) {
+                        const int rl = x * RPI + lane / CH, r = 32 * k + rl;
+                        const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, mine, rl));
+                        cp_async16_zfill(dst + (uint32_t)((ch >> 3) * C::KPANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
+                                         src ? src + ch * 8 : cache, src ? 16 : 0);
+                    }
+                }
+                cp_async_commit();
+                cp_async_wait<1>();
+                hand_over(iw);
+            }
+        }
+        cp_async_wait<0>();
+        if (ok) hand_over(iw);
+        else give_up(1);
+    } else if (wid == C::WARP_MMA) {
+        // =================================== MMA ===================================
+        const uint32_t id_s = idesc(bf16, 128, KT, false), id_o = idesc(bf16, 128, E, true);
+        const uint64_t dq0 = sdesc(s0, 16, 1024), dk0 = sdesc(s0 + off_k, 16, 1024), dv0 = sdesc(s0 + off_v, C::KPANEL, 1024);
+        int j = 0, iw = 0, epoch = 0, piece = 0;
+        bool ok = true;
+        // PV of job jj over V window vw; `first`: the first of its O in this piece
+        auto issue_pv = [&](int jj, int vw, bool first, bool last_use) {
+            const int b = jj & 1, vs = vw % VS;
+            if (!wait_lazy(v_full + 8 * vs, vw / VS) || !wait(p_full + 8 * b, jj >> 1)) return false;
+            tc_fence_after();
+            if (lane == 0) {
+                const uint64_t b0 = dv0 + (uint64_t)((vs * C::KTILE) >> 4);
+                const uint32_t d = tmem + 256 + (NG == 2 ? 128 * b : 0), a = tmem + KT * b;
+#pragma unroll
+                for (int kk = 0; kk < KT / 16; ++kk) umma_ts(d, a + 8 * kk, b0 + (uint64_t)((kk * 16 * 128) >> 4), id_o, !first || kk > 0);
+                if (last_use) umma_commit(v_empty + 8 * vs);
+            }
+            __syncwarp();
+            return true;
+        };
+        while (ok && walk.next(p, pc)) {
+            win.start(p, pc.w);
+            const int jp = j, wp = iw;  // the piece's first job and window
+            int turn = -1;
+            for (int i = pc.i0; ok && i < pc.i1; ++i, ++iw) {
+                win.seek(p, pc.w, i);
+                const int qt = min(win.f, p.F - 1), ks = iw % C::K_STAGES;
+                if (!wait_lazy(k_full + 8 * ks, iw / C::K_STAGES)) {
+                    ok = false;
+                    break;
+                }
+                for (int t = 0; t < (two ? 2 : 1); ++t, ++j) {
+                    if (qt != turn && !wait_lazy(q_ready + 8 * t, epoch)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint64_t a0 = dq0 + (uint64_t)((t * C::QTILE) >> 4), b0 = dk0 + (uint64_t)((ks * C::KTILE) >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < E / 16; ++kk)
+                            umma(tmem + KT * (j & 1), a0 + (uint64_t)(((kk >> 2) * C::QPANEL + (kk & 3) * 32) >> 4),
+                                 b0 + (uint64_t)(((kk >> 2) * C::KPANEL + (kk & 3) * 32) >> 4), id_s, kk > 0);
+                        umma_commit(s_full + 8 * (j & 1));
+                        if (!two || t == 1) umma_commit(k_empty + 8 * ks);
+                    }
+                    __syncwarp();
+                    if (j > jp) {  // the job before this one
+                        const int jj = j - 1 - jp;
+                        if (!issue_pv(j - 1, wp + (two ? jj >> 1 : jj), jj < (NG == 2 ? 2 : 1), !two || (jj & 1))) {
+                            ok = false;
+                            break;
+                        }
+                    }
+                }
+                if (qt != turn) ++epoch, turn = qt;
+            }
+            if (ok) {
+                const int jj = j - 1 - jp;
+                ok = issue_pv(j - 1, wp + (two ? jj >> 1 : jj), jj < (NG == 2 ? 2 : 1), true);
+            }
+            if (ok) {
+                if (lane == 0) umma_commit(o_done);
+                __syncwarp();
+                ++piece;
+            }
+        }
+        if (!ok) {
+            give_up(2);
+            // all issued MMAs have completed before TMEM is released
+            if (lane == 0) umma_commit(o_done);
+            __syncwarp();
+            mbar_wait(o_done, piece & 1);
+        }
+    } else {
+        // ================================= softmax =================================
+        const int grp = wid >> 2, r = (wid & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((wid & 3) * 32) << 16;
+        const uint32_t tO = tmem + lanes + 256 + 128 * grp;
+        const int tile = two ? grp : 0;  // the query tile this thread's row lies in
+        float2* sML = reinterpret_cast<float2*>(smem + C::OFF_ML);
+        const int rows = p.S * p.G, half = p.R >> 1;
+        int j = 0, iw = 0, piece = 0;
+        bool ok = true;
+        while (ok && walk.next(p, pc)) {
+            win.start(p, pc.w);
+            const int row = pc.t * p.mi + tile * 128 + r;
+            const int tok = row < rows ? row / p.G : 0, hq = h * p.G + (row < rows ? row - tok * p.G : 0);
+            const uint32_t* anc = p.anc + ((size_t)pc.w * p.S + tok) * p.SW;
+            const bool there = row < rows && (__ldcg(anc + (tok >> 5)) >> (tok & 31) & 1u);
+            const bool live = __any_sync(0xffffffffu, there);  // the warp has a row to compute
+            const size_t orow = ((size_t)pc.w * p.Hq + hq) * p.S + tok;
+            float m = neg_inf(), l = 0.f;
+            const int jp = j;
+            int turn = -1, lim = 0, lim_f = -1, mine = 0;
+            for (int i = pc.i0; ok && i < pc.i1; ++i, ++iw) {
+                win.seek(p, pc.w, i);
+                const int qt = min(win.f, p.F - 1);
+                if (qt != turn) {
+                    // ---- this row's q, rotated for the turn, into the A tile ----
+                    // every S that reads the tile's old contents has completed
+                    if (j > jp && !(two ? wait(s_full + 8 * grp, (j - 2 + grp) >> 1)
+                                        : wait(s_full + 8 * ((j - 1) & 1), (j - 1) >> 1) && (j < 2 || wait(s_full + 8 * (j & 1), (j - 2) >> 1)))) {
+                        ok = false;
+                        break;
+                    }
+                    turn = qt;
+                    const T* q = static_cast<const T*>(p.q) + orow * E;
+                    const size_t cs = (((size_t)qt * p.W + pc.w) * p.S + tok) * p.R;
+                    const uint32_t qt0 = (uint32_t)(tile * C::QTILE + r * 128);
+                    auto slot = [&](int c) { return reinterpret_cast<uint4*>(smem + qt0 + (c >> 3) * C::QPANEL + (((c & 7) ^ (r & 7)) << 4)); };
+                    // with one tile the two groups share the row: chunk pairs by parity
+                    const int c0 = two ? 0 : grp, step = two ? 1 : NG;
+                    if (!there) {
+                        for (int c = c0; c < E / 8; c += step) *slot(c) = make_uint4(0u, 0u, 0u, 0u);
+                    } else if (half % 8 == 0) {
+                        const int nh = half / 8;
+                        for (int c = c0; c < nh; c += step) {
+                            const uint4 xv = __ldg(reinterpret_cast<const uint4*>(q + c * 8)), yv = __ldg(reinterpret_cast<const uint4*>(q + (c + nh) * 8));
+                            const T* x = reinterpret_cast<const T*>(&xv);
+                            const T* y = reinterpret_cast<const T*>(&yv);
+                            uint32_t lo[4], hi[4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                float a[2], b[2];
+#pragma unroll
+                                for (int v = 0; v < 2; ++v) {
+                                    const float cv = __ldg(p.cos + cs + c * 8 + 2 * u + v), sv = __ldg(p.sin + cs + c * 8 + 2 * u + v);
+                                    const float xf = Elem<T>::to_f(x[2 * u + v]), yf = Elem<T>::to_f(y[2 * u + v]);
+                                    a[v] = __fsub_rn(__fmul_rn(xf, cv), __fmul_rn(yf, sv));
+                                    b[v] = __fadd_rn(__fmul_rn(yf, cv), __fmul_rn(xf, sv));
+                                }
+                                lo[u] = Elem<T>::pack2(a[0], a[1]);
+                                hi[u] = Elem<T>::pack2(b[0], b[1]);
+                            }
+                            *slot(c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            *slot(c + nh) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        }
+                        for (int c = 2 * nh + c0; c < E / 8; c += step) *slot(c) = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
+                    } else {  // a rotary half that ends inside a chunk: element by element
+                        for (int c = c0; c < E / 8; c += step) {
+                            alignas(16) T o[8];
+                            for (int u = 0; u < 8; ++u) {
+                                const int e = c * 8 + u;
+                                o[u] = q[e];
+                                if (e < p.R) {
+                                    const int x = e < half ? e : e - half;
+                                    const float a = Elem<T>::to_f(q[e]), b = Elem<T>::to_f(e < half ? q[e + half] : q[e - half]);
+                                    o[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(a, __ldg(p.cos + cs + x)), __fmul_rn(e < half ? -b : b, __ldg(p.sin + cs + x))));
+                                }
+                            }
+                            *slot(c) = *reinterpret_cast<const uint4*>(o);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    mbar_arrive(q_ready + 8 * tile);
+                }
+                if (win.f < p.F && win.f != lim_f) {
+                    lim_f = win.f;
+                    lim = there ? turn_seen(__ldg(p.L + win.f), __ldg(p.loc + ((size_t)win.f * p.W + pc.w) * p.S + tok), win.off, p.cap) : 0;
+                }
+                // ---- this group's job of the window, if it has one ----
+                const int job = two ? j + grp : j;
+                j += two ? 2 : 1;
+                if (NG == 2 && !two && (job & 1) != grp) continue;
+                const int b = job & 1;
+                const uint32_t tS = tmem + lanes + KT * b;
+                if (!wait(s_full + 8 * b, job >> 1)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                if (live) {
+                    float sv[KT];
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) tmem_ld32(tS + 32 * c, *reinterpret_cast<float(*)[32]>(sv + 32 * c));
+                    tmem_wait_ld();
+                    reg_fence<KT>(sv);
+                    // the maximum is taken before scaling and masked scores are -inf: a scale that is
+                    // not positive goes into the scores first
+                    const float sl2 = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+                    if (p.scale_log2 <= 0.f)
+#pragma unroll
+                        for (int c = 0; c < KT; ++c) sv[c] = p.scale_log2 == 0.f ? 0.f : -sv[c];
+                    uint32_t see[KT / 32];
+                    bool every = true;
+#pragma unroll
+                    for (int x = 0; x < KT / 32; ++x) {
+                        if (win.f < p.F) {
+                            const int d = lim - win.k0 - 32 * x;
+                            see[x] = d >= 32 ? 0xffffffffu : d <= 0 ? 0u : (1u << d) - 1;
+                        } else {
+                            see[x] = there ? __ldcg(anc + (win.k0 >> 5) + x) : 0u;
+                        }
+                        every = every && see[x] == 0xffffffffu;
+                    }
+                    if (!__all_sync(0xffffffffu, every)) {
+#pragma unroll
+                        for (int c = 0; c < KT; ++c)
+                            if (!(see[c >> 5] >> (c & 31) & 1u)) sv[c] = neg_inf();
+                    }
+                    float mx[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) mx[u] = sv[u];
+#pragma unroll
+                    for (int c = 8; c < KT; c += 16)
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) mx[u] = fmax3(mx[u], sv[c + u], sv[c + 8 + u < KT ? c + 8 + u : c + u]);
+                    const float mxs = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * sl2;
+                    // the reference point moves only when the maximum grows by more than 8 (a
+                    // factor 256 in the exponentials); the result is exact either way
+                    const float mnew = mxs > m + 8.f ? mxs : m;
+                    const float alpha = mnew == m ? 1.f : ex2(m - mnew);
+                    const float mu = mnew == neg_inf() ? 0.f : mnew;
+                    const uint64_t sc2 = f2u(sl2, sl2), nmu2 = f2u(-mu, -mu);
+                    uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            float x0, x1;
+                            u2f(ffma2(f2u(sv[32 * c + 2 * u], sv[32 * c + 2 * u + 1]), sc2, nmu2), x0, x1);
+                            const float e0 = ex2(x0), e1 = ex2(x1);
+                            ps2[u & 3] = fadd2(ps2[u & 3], f2u(e0, e1));
+                            pk[u] = Elem<T>::pack2(e0, e1);
+                        }
+                        tmem_st16(tS + 16 * c, pk);
+                    }
+                    float a0, a1;
+                    u2f(fadd2(fadd2(ps2[0], ps2[1]), fadd2(ps2[2], ps2[3])), a0, a1);
+                    l = l * alpha + (a0 + a1);
+                    m = mnew;
+                    if (mine > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                        // O holds the PV of this group's earlier jobs.  With two groups they completed
+                        // before this S was signalled (S(j) is issued after PV(j - 2)); with one, the
+                        // last of them is PV(j - 1), whose completion frees its V window.
+                        if (NG == 1 && !wait(v_empty + 8 * ((iw - 1) % VS), (iw - 1) / VS)) {
+                            ok = false;
+                            break;
+                        }
+                        if (NG == 1) tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < E / 32; ++c) {
+                            float ov[32];
+                            tmem_ld32(tO + 32 * c, ov);
+                            tmem_wait_ld();
+                            reg_fence<32>(ov);
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) ov[u] *= alpha;
+                            tmem_st32(tO + 32 * c, ov);
+                        }
+                    }
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                mbar_arrive(p_full + 8 * b);
+                ++mine;
+            }
+            if (!ok) break;
+            // ---- the piece's result ----
+            if (!wait(o_done, piece)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const bool join = NG == 2 && !two;
+            float w0 = 1.f, w1 = 0.f;
+            bool other = false;  // O of the other group has jobs in it
+            if (join) {
+                sML[grp * 128 + r] = make_float2(m, l);
+                mbar_arrive(epi1);
+                if (!wait(epi1, piece)) {
+                    ok = false;
+                    break;
+                }
+                const float2 a = sML[r], b = sML[128 + r];
+                m = fmaxf(a.x, b.x);
+                const float mu = m == neg_inf() ? 0.f : m;
+                w0 = a.x == neg_inf() && a.y == 0.f ? 0.f : ex2(a.x - mu);
+                w1 = b.x == neg_inf() && b.y == 0.f ? 0.f : ex2(b.x - mu);
+                l = a.y * w0 + b.y * w1;
+                // first the accumulator of the piece's first job, which always has one
+                other = j - jp > 1;
+                if (jp & 1) {
+                    const float x = w0;
+                    w0 = w1, w1 = x;
+                }
+            }
+            const bool whole = pc.whole();
+            const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+            const float lse2 = l == 0.f ? neg_inf() : m + log2f(l);
+            const size_t prow = ((size_t)blockIdx.x * 2 + pc.slot()) * p.mi + tile * 128 + r;
+            const uint32_t ta = join ? tmem + lanes + 256 + 128 * (jp & 1) : tO, tb = tmem + lanes + 256 + 128 * (~jp & 1);
+            const int cb = join ? grp * (E / 64) : 0, ce = join ? cb + E / 64 : E / 32;  // this thread's 32-column blocks
+            if (live) {
+#pragma unroll 1
+                for (int c = cb; c < ce; ++c) {
+                    float ov[32];
+                    tmem_ld32(ta + 32 * c, ov);
+                    tmem_wait_ld();
+                    reg_fence<32>(ov);
+#pragma unroll
+                    for (int u = 0; u < 32; ++u) ov[u] *= w0 * inv;
+                    if (other) {
+                        float o2[32];
+                        tmem_ld32(tb + 32 * c, o2);
+                        tmem_wait_ld();
+                        reg_fence<32>(o2);
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) ov[u] += o2[u] * (w1 * inv);
+                    }
+                    if (l == 0.f)
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) ov[u] = 0.f;
+                    if (row < rows) {
+                        if (whole) {
+                            T* op = static_cast<T*>(p.out) + orow * E + 32 * c;
+#pragma unroll
+                            for (int u = 0; u < 32; u += 8)
+                                *reinterpret_cast<uint4*>(op + u) = make_uint4(Elem<T>::pack2(ov[u], ov[u + 1]), Elem<T>::pack2(ov[u + 2], ov[u + 3]),
+                                                                               Elem<T>::pack2(ov[u + 4], ov[u + 5]), Elem<T>::pack2(ov[u + 6], ov[u + 7]));
+                        } else {
+                            float* op = p.part_o + prow * E + 32 * c;
+#pragma unroll
+                            for (int u = 0; u < 32; u += 4) *reinterpret_cast<float4*>(op + u) = make_float4(ov[u], ov[u + 1], ov[u + 2], ov[u + 3]);
+                        }
+                    }
+                }
+            } else if (row < rows) {  // a warp without a token that is there
+                for (int e = 32 * cb; e < 32 * ce; e += 4) {
+                    if (whole) *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + orow * E + e) = make_uint2(0u, 0u);
+                    else *reinterpret_cast<float4*>(p.part_o + prow * E + e) = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            }
+            if (row < rows && (!join || grp == 0)) {
+                if (!whole) p.part_lse[prow] = lse2;
+                else if (p.lse_out) p.lse_out[orow] = lse2 * kLn2;
+            }
+            if (join) {
+                // both groups have read both accumulators before the next piece's PV writes them
+                tc_fence_before();
+                mbar_arrive(epi2);
+                if (!wait(epi2, piece)) {
+                    ok = false;
+                    break;
+                }
+            }
+            ++piece;
+        }
+        if (!ok) give_up(8);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (wid == C::WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <class T, int E> static TreeKernel tc_kernel(int rows) {
+    // one row tile up to 128 rows and at head dim 256, else two
+    return TreeKernel{(const void*)&tree_tc_kernel<T, E>, TcCfg<E>::NT, TcCfg<E>::KT, rows > 128 && E != 256 ? 256 : 128, TcCfg<E>::SMEM};
+}
+template <class T> static TreeKernel tc_pick(int E, int rows) {
+    return E == 64 ? tc_kernel<T, 64>(rows) : E == 128 ? tc_kernel<T, 128>(rows) : tc_kernel<T, 256>(rows);
+}
+TreeKernel tree_tc_pick(int dtype, int E, int rows) {
+    return dtype == DVATTN_FLOAT16 ? tc_pick<__half>(E, rows) : tc_pick<__nv_bfloat16>(E, rows);
+}
+
+}  // namespace dvb

@@ -101,26 +101,28 @@ struct SplitWalk {
 };
 
 // The turn and the keys of window i of a sequence: keys [k0, k0 + n) of turn f, or of the
-// tail where f == F.  `f`, `first` (the turn's first window) and `off` carry over
-// between calls with increasing i; start with f = first = off = 0.
+// tail where f == F.  Windows are sought in increasing order; `start` begins a sequence.
 struct SplitWin {
-    int f, first, k0, n;
-    long long off;
-    __device__ __forceinline__ void start() { f = 0, first = 0, off = 0; }
+    int f, first, nf, sp, k0, n;  // turn, its first window, its windows, its seen keys
+    long long off;                // the turn's first logical position
+    __device__ __forceinline__ void enter(const TurnSplit& p, int w) {
+        sp = f < p.F ? __ldcg(p.span + (size_t)w * p.F + f) : p.tail;
+        nf = f < p.F ? (sp + p.kt - 1) / p.kt : 0x7fffffff - first;
+    }
+    __device__ __forceinline__ void start(const TurnSplit& p, int w) {
+        f = 0, first = 0, off = 0;
+        enter(p, w);
+    }
     __device__ __forceinline__ void seek(const TurnSplit& p, int w, int i) {
-        for (; f < p.F; ++f) {
-            const int sp = __ldcg(p.span + (size_t)w * p.F + f), nf = (sp + p.kt - 1) / p.kt;
-            if (i < first + nf) {
-                k0 = (i - first) * p.kt;
-                n = min(p.kt, sp - k0);
-                return;
-            }
-            first += nf;
+        while (i >= first + nf) {
             const int Lf = __ldg(p.L + f);
             off += Lf > 0 ? Lf : 0;
+            first += nf;
+            ++f;
+            enter(p, w);
         }
         k0 = (i - first) * p.kt;
-        n = min(p.kt, p.tail - k0);
+        n = min(p.kt, sp - k0);
     }
 };
 
