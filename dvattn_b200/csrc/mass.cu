@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(128) mass_prep_kernel(MassParams p, int E) {
             v = max(max(red[0], red[1]), max(red[2], red[3]));
             __syncthreads();
             if (tid == 0) p.span[(size_t)w * p.F + t] = v;
-            nw += (v + p.kt - 1) / p.kt;
+            nw += turn_windows(p, v, off);
             off += Lt > 0 ? Lt : 0;
         }
         if (tid == 0) p.nwin[w] = nw;
@@ -260,7 +260,7 @@ int mass_launch(const dvattn_mass_args* a, void* workspace, size_t wbytes, cudaS
     p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
     const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
     p.cap = cap > 0x7fffffffLL ? 0x7fffffff : (int)cap;
-    p.tail = 0; p.kt = k.kt; p.nt = 1; p.groups = L.groups;
+    p.tail = 0; p.align = 1; p.kt = k.kt; p.nt = 1; p.groups = L.groups;
     p.N = a->positions;
     p.scale_log2 = a->scale * kLog2e;
     p.mass = a->mass; p.lse = a->lse; p.q = a->queries; p.cos = a->cosines; p.sin = a->sines; p.k = a->k_cache;

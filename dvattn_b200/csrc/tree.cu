@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(128) tree_prep_kernel(TreeParams p, int E) {
             v = max(max(red[0], red[1]), max(red[2], red[3]));
             __syncthreads();
             if (tid == 0) p.span[(size_t)w * p.F + f] = v;
-            nw += (v + p.kt - 1) / p.kt;
+            nw += turn_windows(p, v, off);
             off += Lf > 0 ? Lf : 0;
         }
         if (tid == 0) p.nwin[w] = nw + (p.S + p.kt - 1) / p.kt;
@@ -490,6 +490,9 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     p.part_o = reinterpret_cast<float*>(ws + L.po);
     p.part_lse = reinterpret_cast<float*>(ws + L.pl);
 
+    alignas(64) TreeMaps maps;
+    p.align = 1;
+    if (a->dtype != DVATTN_FLOAT32 && !tree_tc_maps(p, a->dtype, a->E, maps)) return DVATTN_ERR_CUDA;
     const void* prep = a->dtype == DVATTN_FLOAT32   ? (const void*)&tree_prep_kernel<float>
                        : a->dtype == DVATTN_FLOAT16 ? (const void*)&tree_prep_kernel<__half> : (const void*)&tree_prep_kernel<__nv_bfloat16>;
     const void* merge = a->dtype == DVATTN_FLOAT32   ? merge_fn<float>(a->E)
@@ -508,7 +511,7 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     cfg.gridDim = dim3((unsigned)(L.groups * a->Hkv));
     cfg.blockDim = dim3(k.threads);
     cfg.dynamicSmemBytes = k.smem;
-    void* args[] = {&p};
+    void* args[] = {&p, &maps};  // the CUDA-core and merge kernels take the first only
     cudaError_t e = cudaLaunchKernelExC(&cfg, k.fn, args);
     if (e == cudaSuccess) {
         const int rpb = 256 / (a->E / 4), rows_max = L.nt > 1 ? k.mi : a->S * p.G;

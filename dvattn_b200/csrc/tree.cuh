@@ -10,6 +10,8 @@
 // by tree_merge_kernel.
 #pragma once
 
+#include <cuda.h>
+
 #include "turns.cuh"
 
 namespace dvb {
@@ -18,6 +20,7 @@ struct TreeParams : TurnSplit {
     int Hq, Hkv, G, S, R;
     int SW;  // 32-bit words of a token's ancestor set, a multiple of 4
     int mi;  // rows per item
+    int box;  // rows of a TMA box (pages and windows are whole numbers of boxes); 0: rows are gathered
     int stall_tile;  // test hook (DVATTN_TEST_STALL_TILE), -1: off
     float scale_log2;
     void* out;
@@ -44,7 +47,12 @@ struct TreeKernel {
     int threads, kt, mi;
     size_t smem;
 };
-// the 16-bit kernel on the 5th-generation tensor cores (tree_tc.cu)
+// the 16-bit kernel on the 5th-generation tensor cores (tree_tc.cu), and its tensor maps
+struct TreeMaps {
+    CUtensorMap k, v, dk, dv;
+};
 TreeKernel tree_tc_pick(int dtype, int E, int rows);
+// Sets p.box and p.align and fills the maps the kernel then uses; false: a CUDA error.
+bool tree_tc_maps(TreeParams& p, int dtype, int E, TreeMaps& maps);
 
 }  // namespace dvb

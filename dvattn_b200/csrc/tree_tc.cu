@@ -10,12 +10,15 @@
 //                       (one tile's chain softmax -> PV -> next S would not keep up with HBM);
 //   head dim 256:       one tile and one O (256 columns); only the score buffers alternate.
 // Warps: 4 per softmax group (a thread owns one query row = one TMEM lane), one MMA issuer,
-// one K and one V producer.  Producers gather rows with cp.async (any page size; rows that
-// nobody sees are zero-filled, so what lies there never matters) into swizzled rings.
+// one K and one V producer.  Producers fill swizzled rings with TMA boxes where pages and
+// windows are whole numbers of boxes of 8 or more rows (page sizes that are multiples of 8),
+// else they gather rows with cp.async.  What lies in rows that nobody sees never matters:
+// their scores are masked, and their V rows are zeroed before PV (0 * NaN is NaN).
 //
 // Every wait is bounded; one that gives up sets the call's error word, ends the CTA with
 // nothing in flight, and tree_merge_kernel writes NaN to all outputs of the call.
 #include "tcgen05.cuh"
+#include "tma_host.cuh"
 #include "tree.cuh"
 
 namespace dvb {
@@ -40,7 +43,7 @@ template <int E> struct TcCfg {
 };
 
 template <class T, int E>
-__global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p) {
+__global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, const __grid_constant__ TreeMaps maps) {
     using C = TcCfg<E>;
     constexpr int KT = C::KT, NG = C::NG;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -57,9 +60,9 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p) 
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
     if (tid == 0) {
         for (int s = 0; s < C::RING; ++s) {
-            mbar_init(k_full + 8 * s, 32);
+            mbar_init(k_full + 8 * s, p.box ? 1 : 32);
             mbar_init(k_empty + 8 * s, 1);
-            mbar_init(v_full + 8 * s, 32);
+            mbar_init(v_full + 8 * s, p.box ? 1 : 32);
             mbar_init(v_empty + 8 * s, 1);
         }
         for (int s = 0; s < 2; ++s) {
@@ -104,8 +107,67 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p) 
         }
     };
 
-    if (wid == C::WARP_K || wid == C::WARP_V) {
-        // ================================ producers ================================
+    if ((wid == C::WARP_K || wid == C::WARP_V) && p.box) {
+        // ============================== TMA producers ==============================
+        const bool is_k = wid == C::WARP_K;
+        const int stages = is_k ? C::K_STAGES : VS;
+        const uint32_t full = is_k ? k_full : v_full, empty = is_k ? k_empty : v_empty, ring = s0 + (is_k ? off_k : off_v);
+        const CUtensorMap* cache = is_k ? &maps.k : &maps.v;
+        const CUtensorMap* draft = is_k ? &maps.dk : &maps.dv;
+        if (lane == 0) {
+            prefetch_tmap(cache);
+            prefetch_tmap(draft);
+        }
+        // the rotated drafted keys were written by the kernel before, with ordinary stores
+        asm volatile("fence.proxy.async;" ::: "memory");
+        const int boxes = KT / p.box, absent = -2 * p.BS;  // a coordinate that loads zeros
+        int next = 0;  // first token of the lane's box of the next window
+        auto find = [&](int i) {
+            win.seek(p, pc.w, i);
+            next = absent;
+            if (win.f == p.F) {
+                next = (pc.w * p.Hkv + h) * p.S + win.k0;
+            } else if (lane < boxes) {
+                const int l = win.k0 + lane * p.box, pos = (int)win.off + l;
+                if (l + p.box > 0 && l < win.sp) {
+                    const int page = __ldg(p.bt + (size_t)pc.w * p.maxb + pos / p.BS);
+                    if (page >= 0 && page < p.NB) next = page * p.BS + pos % p.BS;
+                }
+            }
+        };
+        const bool stall = is_k && blockIdx.x == 0;  // test hook: this window never lands
+        int iw = 0;
+        bool ok = true;
+        while (ok && walk.next(p, pc)) {
+            win.start(p, pc.w);
+            find(pc.i0);
+            for (int i = pc.i0; i < pc.i1; ++i, ++iw) {
+                const int st = iw % stages;
+                if (iw >= stages && (*s_abort || !wait_lazy(empty + 8 * st, iw / stages - 1))) {
+                    ok = false;
+                    break;
+                }
+                const int z = next;
+                const bool tail = win.f == p.F;
+                if (i + 1 < pc.i1) find(i + 1);
+                if (stall && iw == p.stall_tile) continue;
+                if (lane == 0) mbar_expect_tx(full + 8 * st, (uint32_t)C::KTILE);
+                __syncwarp();
+                const uint32_t dst = ring + (uint32_t)(st * C::KTILE);
+                if (tail ? lane == 0 : lane < boxes)
+#pragma unroll
+                    for (int x = 0; x < C::NP; ++x)
+                        tma_load_3d(dst + (uint32_t)(x * C::KPANEL + lane * p.box * 128), tail ? draft : cache, x * 64, tail ? 0 : h, z, full + 8 * st);
+            }
+        }
+        if (!ok) {
+            give_up(1);
+            // the windows already requested land before the CTA can exit (bounded waits)
+            for (int x = max(0, iw - stages); x < iw; ++x)
+                if (!(stall && x == p.stall_tile)) mbar_wait(full + 8 * (x % stages), (x / stages) & 1);
+        }
+    } else if (wid == C::WARP_K || wid == C::WARP_V) {
+        // ============================= gather producers ============================
         const bool is_k = wid == C::WARP_K;
         const int stages = is_k ? C::K_STAGES : VS;
         const uint32_t full = is_k ? k_full : v_full, empty = is_k ? k_empty : v_empty, ring = s0 + (is_k ? off_k : off_v);
@@ -372,8 +434,9 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p) 
 #pragma unroll
                     for (int x = 0; x < KT / 32; ++x) {
                         if (win.f < p.F) {
-                            const int d = lim - win.k0 - 32 * x;
+                            const int d = lim - win.k0 - 32 * x, e = -win.k0 - 32 * x;  // columns in front of d, not of e
                             see[x] = d >= 32 ? 0xffffffffu : d <= 0 ? 0u : (1u << d) - 1;
+                            see[x] &= e <= 0 ? 0xffffffffu : e >= 32 ? 0u : 0xffffffffu << e;
                         } else {
                             see[x] = there ? __ldcg(anc + (win.k0 >> 5) + x) : 0u;
                         }
@@ -437,6 +500,24 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p) 
                         }
                     }
                     tmem_wait_st();
+                }
+                if (p.box && (!two || grp == 0) && (win.f == p.F || win.k0 < 0 || win.n < KT)) {
+                    // V rows of this window that nobody sees: P is 0 there
+                    if (!wait(v_full + 8 * (iw % VS), iw / VS)) {
+                        ok = false;
+                        break;
+                    }
+                    const int key = win.k0 + r;
+                    bool seen = r < win.n && key >= 0;
+                    if (seen && win.f == p.F) seen = __ldcg(p.anc + ((size_t)pc.w * p.S + key) * p.SW + (key >> 5)) >> (key & 31) & 1u;
+                    if (r < KT && !seen) {
+                        uint8_t* v = smem + off_v + (iw % VS) * C::KTILE + r * 128;
+#pragma unroll
+                        for (int x = 0; x < C::NP; ++x)
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + x * C::KPANEL + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async_smem();
                 }
                 tc_fence_before();
                 mbar_arrive(p_full + 8 * b);
@@ -550,6 +631,21 @@ template <class T> static TreeKernel tc_pick(int E, int rows) {
 }
 TreeKernel tree_tc_pick(int dtype, int E, int rows) {
     return dtype == DVATTN_FLOAT16 ? tc_pick<__half>(E, rows) : tc_pick<__nv_bfloat16>(E, rows);
+}
+
+bool tree_tc_maps(TreeParams& p, int dtype, int E, TreeMaps& m) {
+    const int kt = p.kt;
+    int b = kt;  // the largest power of two that divides the page size, at most a window
+    while (p.BS % b) b >>= 1;
+    const long long tokens = p.NB * p.BS, drafts = (long long)p.W * p.Hkv * p.S;
+    p.box = 0;
+    p.align = 1;
+    // 8 rows are what the 128-byte swizzle repeats over; coordinates are 32-bit
+    if (b < 8 || p.cap == 0 || tokens > 0x7fffffffLL - 2 * (long long)p.BS || drafts > 0x7fffffffLL - kt) return true;
+    p.box = b;
+    p.align = b;
+    return encode_cache_map(&m.k, p.k, dtype, E, p.Hkv, tokens, b) && encode_cache_map(&m.v, p.v, dtype, E, p.Hkv, tokens, b) &&
+           encode_cache_map(&m.dk, p.dkr, dtype, E, 1, drafts, kt) && encode_cache_map(&m.dv, p.dv, dtype, E, 1, drafts, kt);
 }
 
 }  // namespace dvb

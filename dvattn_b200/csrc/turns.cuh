@@ -2,7 +2,8 @@
 // of a sequence's KV head read the same keys (tree.cu, tree_tc.cu, mass.cu).
 //
 // A sequence's keys are cut into windows of `kt` keys: each turn's visible keys (the union
-// over the queries) from the turn's first key on, then `tail` keys that lie outside the
+// over the queries) from the turn's first key on (or from up to `align` - 1 positions before
+// it, so that windows begin on a multiple of `align`), then `tail` keys that lie outside the
 // cache (the drafted tokens of a tree; 0 where there are none).  The windows of all
 // (sequence, row tile) pairs, one after the other, are cut into `groups` ranges of equal
 // length.  A group is Hkv CTAs that walk the same range, one KV head each, so the heads of a
@@ -16,6 +17,7 @@ namespace dvb {
 struct TurnSplit {
     int F, W, BS, maxb, cap, tail;
     int kt, nt, groups;  // keys per window, row tiles per sequence, CTA groups
+    int align;           // windows over the cache begin on logical positions that are multiples of it
     long long NB;
     const int* loc;
     const int* L;
@@ -31,6 +33,11 @@ __device__ __forceinline__ int turn_seen(int L, int loc, long long off, int cap)
     const int v = loc >= L ? L : loc + 1;
     const long long room = cap - off;
     return v < room ? v : (int)room;
+}
+
+// Windows of a turn of which `seen` keys are seen.
+__device__ __forceinline__ int turn_windows(const TurnSplit& p, int seen, long long off) {
+    return seen > 0 ? ((int)(off % p.align) + seen + p.kt - 1) / p.kt : 0;
 }
 
 __device__ __forceinline__ long long split_bound(long long total, int g, int groups) { return total * g / groups; }
@@ -100,14 +107,16 @@ struct SplitWalk {
     }
 };
 
-// The turn and the keys of window i of a sequence: keys [k0, k0 + n) of turn f, or of the
-// tail where f == F.  Windows are sought in increasing order; `start` begins a sequence.
+// The turn and the keys of window i of a sequence: column c of the window is key k0 + c of
+// turn f (of the tail where f == F), for c < n and k0 + c >= 0.  Windows are sought in
+// increasing order; `start` begins a sequence.
 struct SplitWin {
-    int f, first, nf, sp, k0, n;  // turn, its first window, its windows, its seen keys
+    int f, first, nf, sp, lead, k0, n;  // turn, its first window, its windows, its seen keys
     long long off;                // the turn's first logical position
     __device__ __forceinline__ void enter(const TurnSplit& p, int w) {
         sp = f < p.F ? __ldcg(p.span + (size_t)w * p.F + f) : p.tail;
-        nf = f < p.F ? (sp + p.kt - 1) / p.kt : 0x7fffffff - first;
+        lead = f < p.F ? (int)(off % p.align) : 0;
+        nf = f < p.F ? turn_windows(p, sp, off) : 0x7fffffff - first;
     }
     __device__ __forceinline__ void start(const TurnSplit& p, int w) {
         f = 0, first = 0, off = 0;
@@ -121,7 +130,7 @@ struct SplitWin {
             ++f;
             enter(p, w);
         }
-        k0 = (i - first) * p.kt;
+        k0 = (i - first) * p.kt - lead;
         n = min(p.kt, sp - k0);
     }
 };
