@@ -98,9 +98,9 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
     const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
     SplitWalk walk;
     {
-        const long long total = split_total(p, lane);
-        walk.u = split_bound(total, g, p.groups);
-        walk.u1 = split_bound(total, g + 1, p.groups);
+        const SplitRange range(split_total(p, lane), p.groups);
+        walk.u = range.begin(g);
+        walk.u1 = range.begin(g + 1);
         split_locate(p, lane, walk.u, walk.w, walk.base);
     }
     SplitPiece pc;

@@ -15,16 +15,21 @@
 
 namespace dvb {
 
-// ---- prep: one block per (sequence, KV head) -----------------------------------------
-// The rotation is apply_rotary_pos_emb's with separate roundings of the two products and
-// of the sum, then one rounding to T, so a drafted key has the bits that the paged append
-// writes for it.
+// ---- prep ---------------------------------------------------------------------------
+// Block (w, 0) finds sequence w's ancestor sets and spans; the others rotate its drafted
+// keys, a warp per (token, KV head) row.  The rotation is apply_rotary_pos_emb's with
+// separate roundings of the two products and of the sum, then one rounding to T, so a
+// drafted key has the bits that the paged append writes for it.
+constexpr int kPrepRows = 8;  // rows of a rotating block (of 4 warps)
+
 template <class T>
 __global__ void __launch_bounds__(128) tree_prep_kernel(TreeParams p, int E) {
-    extern __shared__ int par[];  // [S]
+    extern __shared__ int par[];  // [S] parents, then [S] whether a token is there
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int w = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-    if (h == 0) {
+    const int w = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    if (blockIdx.y == 0) {
+        __shared__ int red[4];
+        int* there = par + p.S;
         if (w == 0 && tid < 4) p.header[tid] = 0;
         for (int j = tid; j < p.S; j += 128) par[j] = __ldg(p.parents + (size_t)w * p.S + j);
         __syncthreads();
@@ -32,9 +37,9 @@ __global__ void __launch_bounds__(128) tree_prep_kernel(TreeParams p, int E) {
         for (int j = tid; j < p.S; j += 128) {
             int c = j;
             while (c >= 0 && par[c] < c && par[c] >= -1) c = par[c];
-            const bool there = c == -1;
+            there[j] = c == -1;
             uint32_t* a = p.anc + ((size_t)w * p.S + j) * p.SW;
-            c = there ? j : -1;
+            c = c == -1 ? j : -1;
             for (int word = p.SW - 1; word >= 0; --word) {
                 uint32_t bits = 0;
                 while (c >= 32 * word) {  // c < 32 * (word + 1) here: parents come before
@@ -45,19 +50,18 @@ __global__ void __launch_bounds__(128) tree_prep_kernel(TreeParams p, int E) {
                 a[word] = bits;
             }
         }
-        __shared__ int red[4];
-        __syncthreads();  // the block's own global writes are visible to it after this
+        __syncthreads();
         long long off = 0;
         int nw = 0;
         for (int f = 0; f < p.F; ++f) {
             const int Lf = __ldg(p.L + f);
             int v = 0;
-            for (int s = tid; s < p.S; s += 128)
-                if (p.anc[((size_t)w * p.S + s) * p.SW + (s >> 5)] >> (s & 31) & 1u)
-                    v = max(v, turn_seen(Lf, __ldg(p.loc + ((size_t)f * p.W + w) * p.S + s), off, p.cap));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-            if ((tid & 31) == 0) red[tid >> 5] = v;
+            for (int s = tid; s < p.S; s += 128) {
+                const int n = turn_seen(Lf, __ldg(p.loc + ((size_t)f * p.W + w) * p.S + s), off, p.cap);
+                if (there[s]) v = max(v, n);
+            }
+            v = __reduce_max_sync(0xffffffffu, v);
+            if (lane == 0) red[wid] = v;
             __syncthreads();
             v = max(max(red[0], red[1]), max(red[2], red[3]));
             __syncthreads();
@@ -66,20 +70,23 @@ __global__ void __launch_bounds__(128) tree_prep_kernel(TreeParams p, int E) {
             off += Lf > 0 ? Lf : 0;
         }
         if (tid == 0) p.nwin[w] = nw + (p.S + p.kt - 1) / p.kt;
+        return;
     }
-    const int half = p.R >> 1;
-    const T* x = static_cast<const T*>(p.dk) + ((size_t)w * p.Hkv + h) * p.S * E;
-    T* y = static_cast<T*>(p.dkr) + ((size_t)w * p.Hkv + h) * p.S * E;
-    const size_t cs = ((size_t)(p.F - 1) * p.W + w) * p.S;
-    for (int i = tid; i < p.S * E; i += 128) {
-        const int s = i / E, e = i - s * E;
-        if (e >= p.R) {
-            y[i] = x[i];
-        } else {
-            const int j = e < half ? e : e - half;
-            const float c = __ldg(p.cos + (cs + s) * p.R + j), sn = __ldg(p.sin + (cs + s) * p.R + j);
-            const float a = Elem<T>::to_f(x[i]), b = Elem<T>::to_f(e < half ? x[i + half] : x[i - half]);
-            y[i] = Elem<T>::from_f(__fadd_rn(__fmul_rn(a, c), __fmul_rn(e < half ? -b : b, sn)));
+    const int half = p.R >> 1, rows = p.Hkv * p.S, r0 = (blockIdx.y - 1) * kPrepRows;
+    for (int r = r0 + wid; r < min(r0 + kPrepRows, rows); r += 4) {
+        const int s = r % p.S;
+        const size_t at = ((size_t)w * rows + r) * E, cs = (((size_t)(p.F - 1) * p.W + w) * p.S + s) * p.R;
+        const T* x = static_cast<const T*>(p.dk) + at;
+        T* y = static_cast<T*>(p.dkr) + at;
+        for (int e = lane; e < E; e += 32) {
+            if (e >= p.R) {
+                y[e] = x[e];
+            } else {
+                const int j = e < half ? e : e - half;
+                const float c = __ldg(p.cos + cs + j), sn = __ldg(p.sin + cs + j);
+                const float a = Elem<T>::to_f(x[e]), b = Elem<T>::to_f(e < half ? x[e + half] : x[e - half]);
+                y[e] = Elem<T>::from_f(__fadd_rn(__fmul_rn(a, c), __fmul_rn(e < half ? -b : b, sn)));
+            }
         }
     }
 }
@@ -131,9 +138,9 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
     const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
     SplitWalk walk;
     {
-        const long long total = split_total(p, lane);
-        walk.u = split_bound(total, g, p.groups);
-        walk.u1 = split_bound(total, g + 1, p.groups);
+        const SplitRange range(split_total(p, lane), p.groups);
+        walk.u = range.begin(g);
+        walk.u1 = range.begin(g + 1);
         split_locate(p, lane, walk.u, walk.w, walk.base);
     }
     const int rows = p.S * p.G;
@@ -290,13 +297,14 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
 
 // ---- merge ----------------------------------------------------------------------------
 // Rows of items that more than one group worked on: the log-sum-exp combination of their
-// partials, in group order.  E / 4 threads per row.  A call whose error word is set gets
-// NaN in every output.
+// partials, in group order.  E / 4 lanes per row; up to a segment of lanes at a time look at
+// the partials' sums, one each, then all partials' columns are read with their loads in
+// flight.  A call whose error word is set gets NaN in every output.
 template <class T, int E>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
-    constexpr int TPR = E / 4, RPB = 256 / TPR;  // threads per row, rows per block
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int tid = threadIdx.x, lane = tid & 31;
+    constexpr int TPR = E / 4, RPB = 256 / TPR;     // threads per row, rows per block
+    constexpr int SEG = TPR < 32 ? TPR : 32;        // lanes that work on one row together
+    const int tid = threadIdx.x, lane = tid & 31, sl = tid % SEG;
     const int item = blockIdx.x, h = item % p.Hkv, t = item / p.Hkv % p.nt, w = item / p.Hkv / p.nt;
     const int i = blockIdx.y * RPB + tid / TPR, e = tid % TPR * 4;
     const int r = t * p.mi + i;
@@ -304,8 +312,9 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
     const int s = row_ok ? r / p.G : 0, hq = h * p.G + (row_ok ? r - s * p.G : 0);
     const size_t orow = ((size_t)w * p.Hq + hq) * p.S + s;
     T* op = static_cast<T*>(p.out) + orow * E + e;
+    const float nan = __int_as_float(0x7fc00000);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (__ldcg(p.header + 3) != 0) {
-        const float nan = __int_as_float(0x7fc00000);
         if (row_ok) {
             store_quad<T>(op, nan, nan, nan, nan);
             if (p.lse_out && e == 0) p.lse_out[orow] = nan;
@@ -324,47 +333,44 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
         total += __shfl_xor_sync(0xffffffffu, total, o);
         before += __shfl_xor_sync(0xffffffffu, before, o);
     }
-    total *= p.nt;
     const int nw = __ldcg(p.nwin + w);
-    const long long us = before * p.nt + (long long)t * nw, ue = us + nw - 1;
-    auto group_of = [&](long long u) {
-        int g = (int)(u * p.groups / total);
-        while (g > 0 && split_bound(total, g, p.groups) > u) --g;
-        while (g + 1 < p.groups && split_bound(total, g + 1, p.groups) <= u) ++g;
-        return g;
-    };
-    const int g0 = group_of(us), g1 = group_of(ue);
-    if (g0 == g1 || !row_ok) return;
-    auto slot_of = [&](int g) { return ((size_t)g * p.Hkv + h) * 2 + (g == g0 ? 1 : 0); };
-    auto empty = [&](int g) { return split_bound(total, g, p.groups) == split_bound(total, g + 1, p.groups); };
-    float mx = neg_inf();
-    bool bad = false;  // a partial of NaN: fmaxf drops it, the result must not
-    for (int g = g0; g <= g1; ++g) {
-        if (empty(g)) continue;
-        const float x = __ldcg(p.part_lse + slot_of(g) * p.mi + i);
-        mx = fmaxf(mx, x);
-        bad |= x != x;
-    }
-    float den = 0.f, a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-    if (mx != neg_inf()) {
-        for (int g = g0; g <= g1; ++g) {
-            if (empty(g)) continue;
-            const size_t sl = slot_of(g) * p.mi + i;
-            const float x = __ldcg(p.part_lse + sl);
-            if (x == neg_inf()) continue;
-            const float wgt = fast_exp2(x - mx);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + sl * E + e));
-            den += wgt;
-            a0 = fmaf(wgt, v.x, a0);
-            a1 = fmaf(wgt, v.y, a1);
-            a2 = fmaf(wgt, v.z, a2);
-            a3 = fmaf(wgt, v.w, a3);
+    const SplitRange range(total * p.nt, p.groups);
+    const long long us = before * p.nt + (long long)t * nw;
+    const int g0 = range.group_of(us), g1 = range.group_of(us + nw - 1);
+    if (g0 == g1) return;
+    auto slot_of = [&](int g) { return (((size_t)g * p.Hkv + h) * 2 + (g == g0 ? 1 : 0)) * p.mi + (row_ok ? i : 0); };
+    float m = neg_inf(), den = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int gb = g0; gb <= g1; gb += SEG) {
+        const int n = min(SEG, g1 - gb + 1);
+        const float x = sl < n ? __ldcg(p.part_lse + slot_of(gb + sl)) : neg_inf();
+        float mx = x;
+        bool bad = x != x;  // fmaxf drops a NaN, the result must not
+#pragma unroll
+        for (int o = SEG / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        mx = fmaxf(mx, m);
+        const float mu = mx == neg_inf() ? 0.f : mx;
+        const float wgt = bad ? nan : fast_exp2(x - mu), alpha = fast_exp2(m - mu);
+        m = mx;
+        den *= alpha;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) a[c] *= alpha;
+#pragma unroll 8
+        for (int y = 0; y < n; ++y) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot_of(gb + y) * E + e));
+            const float f = __shfl_sync(0xffffffffu, wgt, y, SEG);
+            den += f;
+            if (f != 0.f) {  // an empty part adds nothing
+                a[0] = fmaf(f, v.x, a[0]);
+                a[1] = fmaf(f, v.y, a[1]);
+                a[2] = fmaf(f, v.z, a[2]);
+                a[3] = fmaf(f, v.w, a[3]);
+            }
         }
     }
-    float inv = den > 0.f ? 1.f / den : 0.f;
-    if (bad) inv = __int_as_float(0x7fc00000);
-    store_quad<T>(op, a0 * inv, a1 * inv, a2 * inv, a3 * inv);
-    if (p.lse_out && e == 0) p.lse_out[orow] = bad ? inv : den > 0.f ? (mx + log2f(den)) * kLn2 : neg_inf();
+    if (!row_ok) return;
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    store_quad<T>(op, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+    if (p.lse_out && e == 0) p.lse_out[orow] = den == 0.f ? neg_inf() : (m + log2f(den)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -402,9 +408,9 @@ static int tree_validate(const dvattn_tree_args* a) {
     if (st != DVATTN_OK) return st;
     if (a->F < 1) return DVATTN_ERR_INVALID_ARGUMENT;  // the drafted tokens belong to the last turn
     if (a->S > kTreeMaxTokens) return DVATTN_ERR_UNSUPPORTED;
-    // grid limits: sequences are the prep grid's x, heads its y; items are the merge grid's x
+    // grid limits: sequences are the prep grid's x, row blocks its y; items are the merge grid's x
     const long long rows = (long long)a->S * (a->Hq / a->Hkv);
-    if (a->Hkv > 65535 || (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
+    if ((long long)a->Hkv * a->S > 65534LL * kPrepRows || (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
     return DVATTN_OK;
 }
 
@@ -499,7 +505,8 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
                         : a->dtype == DVATTN_FLOAT16 ? merge_fn<__half>(a->E) : merge_fn<__nv_bfloat16>(a->E);
     int E = a->E;
     void* pargs[] = {&p, &E};
-    if (cudaLaunchKernel(prep, dim3(a->W, a->Hkv), dim3(128), pargs, sizeof(int) * (size_t)a->S, stream) != cudaSuccess)
+    if (cudaLaunchKernel(prep, dim3(a->W, 1 + (a->Hkv * a->S + kPrepRows - 1) / kPrepRows), dim3(128), pargs,
+                         2 * sizeof(int) * (size_t)a->S, stream) != cudaSuccess)
         return DVATTN_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];

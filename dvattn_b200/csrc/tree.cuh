@@ -21,6 +21,7 @@ struct TreeParams : TurnSplit {
     int SW;  // 32-bit words of a token's ancestor set, a multiple of 4
     int mi;  // rows per item
     int box;  // rows of a TMA box (pages and windows are whole numbers of boxes); 0: rows are gathered
+    int rot_vec;     // rotary halves are whole 16-byte chunks, cos/sin rows 16-byte aligned
     int stall_tile;  // test hook (DVATTN_TEST_STALL_TILE), -1: off
     float scale_log2;
     void* out;

@@ -90,9 +90,9 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
     const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
     SplitWalk walk;
     {
-        const long long total = split_total(p, lane);
-        walk.u = split_bound(total, g, p.groups);
-        walk.u1 = split_bound(total, g + 1, p.groups);
+        const SplitRange range(split_total(p, lane), p.groups);
+        walk.u = range.begin(g);
+        walk.u1 = range.begin(g + 1);
         split_locate(p, lane, walk.u, walk.w, walk.base);
     }
     SplitPiece pc;
@@ -135,12 +135,24 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                 }
             }
         };
+        // the queries of a piece are on their way to L2 before the softmax threads ask for them
+        auto prefetch_q = [&] {
+            const int rows = p.S * p.G;
+            for (int x = lane; x < p.mi * (E / 64); x += 32) {
+                const int row = pc.t * p.mi + x / (E / 64);
+                if (row >= rows) break;
+                const int s = row / p.G;
+                const T* q = static_cast<const T*>(p.q) + (((size_t)pc.w * p.Hq + h * p.G + row - s * p.G) * p.S + s) * E + x % (E / 64) * 64;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+            }
+        };
         const bool stall = is_k && blockIdx.x == 0;  // test hook: this window never lands
         int iw = 0;
         bool ok = true;
         while (ok && walk.next(p, pc)) {
             win.start(p, pc.w);
             find(pc.i0);
+            if (!is_k) prefetch_q();
             for (int i = pc.i0; i < pc.i1; ++i, ++iw) {
                 const int st = iw % stages;
                 if (iw >= stages && (*s_abort || !wait_lazy(empty + 8 * st, iw / stages - 1))) {
@@ -246,79 +258,67 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         else give_up(1);
     } else if (wid == C::WARP_MMA) {
         // =================================== MMA ===================================
+        // one thread: its waits, issues and commits are on every job's path
         const uint32_t id_s = idesc(bf16, 128, KT, false), id_o = idesc(bf16, 128, E, true);
         const uint64_t dq0 = sdesc(s0, 16, 1024), dk0 = sdesc(s0 + off_k, 16, 1024), dv0 = sdesc(s0 + off_v, C::KPANEL, 1024);
-        int j = 0, iw = 0, epoch = 0, piece = 0;
-        bool ok = true;
-        // PV of job jj over V window vw; `first`: the first of its O in this piece
-        auto issue_pv = [&](int jj, int vw, bool first, bool last_use) {
-            const int b = jj & 1, vs = vw % VS;
-            if (!wait_lazy(v_full + 8 * vs, vw / VS) || !wait(p_full + 8 * b, jj >> 1)) return false;
-            tc_fence_after();
-            if (lane == 0) {
+        if (lane == 0) {
+            int j = 0, ks = 0, kp = 0, vs = 0, vp = 0, epoch = 0, piece = 0;
+            bool ok = true;
+            // PV of job jj, the n-th of its piece, over the V window at hand; `last`: its last use
+            auto issue_pv = [&](int jj, int n, bool last) {
+                const int b = jj & 1;
+                if (!mbar_wait(v_full + 8 * vs, vp) || !mbar_wait(p_full + 8 * b, (jj >> 1) & 1)) return false;
+                tc_fence_after();
                 const uint64_t b0 = dv0 + (uint64_t)((vs * C::KTILE) >> 4);
                 const uint32_t d = tmem + 256 + (NG == 2 ? 128 * b : 0), a = tmem + KT * b;
+                const uint32_t acc = n >= NG;  // the first PV of an O in a piece overwrites it
 #pragma unroll
-                for (int kk = 0; kk < KT / 16; ++kk) umma_ts(d, a + 8 * kk, b0 + (uint64_t)((kk * 16 * 128) >> 4), id_o, !first || kk > 0);
-                if (last_use) umma_commit(v_empty + 8 * vs);
-            }
-            __syncwarp();
-            return true;
-        };
-        while (ok && walk.next(p, pc)) {
-            win.start(p, pc.w);
-            const int jp = j, wp = iw;  // the piece's first job and window
-            int turn = -1;
-            for (int i = pc.i0; ok && i < pc.i1; ++i, ++iw) {
-                win.seek(p, pc.w, i);
-                const int qt = min(win.f, p.F - 1), ks = iw % C::K_STAGES;
-                if (!wait_lazy(k_full + 8 * ks, iw / C::K_STAGES)) {
-                    ok = false;
-                    break;
+                for (int kk = 0; kk < KT / 16; ++kk) umma_ts(d, a + 8 * kk, b0 + (uint64_t)((kk * 16 * 128) >> 4), id_o, kk > 0 ? 1u : acc);
+                if (last) {
+                    umma_commit(v_empty + 8 * vs);
+                    if (++vs == VS) vs = 0, vp ^= 1;
                 }
-                for (int t = 0; t < (two ? 2 : 1); ++t, ++j) {
-                    if (qt != turn && !wait_lazy(q_ready + 8 * t, epoch)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    if (lane == 0) {
+                return true;
+            };
+            while (ok && walk.next(p, pc)) {
+                win.start(p, pc.w);
+                int n = 0, turn = -1;  // jobs of the piece issued, the turn q is rotated for
+                for (int i = pc.i0; ok && i < pc.i1; ++i) {
+                    win.seek(p, pc.w, i);
+                    const int qt = min(win.f, p.F - 1);
+                    if (!mbar_wait(k_full + 8 * ks, kp)) ok = false;
+                    for (int t = 0; ok && t < (two ? 2 : 1); ++t, ++j, ++n) {
+                        if (qt != turn && !mbar_wait(q_ready + 8 * t, epoch & 1)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
                         const uint64_t a0 = dq0 + (uint64_t)((t * C::QTILE) >> 4), b0 = dk0 + (uint64_t)((ks * C::KTILE) >> 4);
 #pragma unroll
                         for (int kk = 0; kk < E / 16; ++kk)
                             umma(tmem + KT * (j & 1), a0 + (uint64_t)(((kk >> 2) * C::QPANEL + (kk & 3) * 32) >> 4),
-                                 b0 + (uint64_t)(((kk >> 2) * C::KPANEL + (kk & 3) * 32) >> 4), id_s, kk > 0);
+                                 b0 + (uint64_t)(((kk >> 2) * C::KPANEL + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
                         umma_commit(s_full + 8 * (j & 1));
                         if (!two || t == 1) umma_commit(k_empty + 8 * ks);
+                        if (n > 0 && !issue_pv(j - 1, n - 1, !two || t == 0)) ok = false;
                     }
-                    __syncwarp();
-                    if (j > jp) {  // the job before this one
-                        const int jj = j - 1 - jp;
-                        if (!issue_pv(j - 1, wp + (two ? jj >> 1 : jj), jj < (NG == 2 ? 2 : 1), !two || (jj & 1))) {
-                            ok = false;
-                            break;
-                        }
-                    }
+                    if (++ks == C::K_STAGES) ks = 0, kp ^= 1;
+                    if (qt != turn) ++epoch, turn = qt;
                 }
-                if (qt != turn) ++epoch, turn = qt;
+                if (ok) ok = issue_pv(j - 1, n - 1, true);
+                if (ok) {
+                    umma_commit(o_done);
+                    ++piece;
+                }
             }
-            if (ok) {
-                const int jj = j - 1 - jp;
-                ok = issue_pv(j - 1, wp + (two ? jj >> 1 : jj), jj < (NG == 2 ? 2 : 1), true);
-            }
-            if (ok) {
-                if (lane == 0) umma_commit(o_done);
-                __syncwarp();
-                ++piece;
+            if (!ok) {
+                give_up(2);
+                // all issued MMAs have completed before TMEM is released
+                umma_commit(o_done);
+                mbar_wait(o_done, piece & 1);
             }
         }
-        if (!ok) {
-            give_up(2);
-            // all issued MMAs have completed before TMEM is released
-            if (lane == 0) umma_commit(o_done);
-            __syncwarp();
-            mbar_wait(o_done, piece & 1);
-        }
+        __syncwarp();
     } else {
         // ================================= softmax =================================
         const int grp = wid >> 2, r = (wid & 3) * 32 + lane;
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             const int row = pc.t * p.mi + tile * 128 + r;
             const int tok = row < rows ? row / p.G : 0, hq = h * p.G + (row < rows ? row - tok * p.G : 0);
             const uint32_t* anc = p.anc + ((size_t)pc.w * p.S + tok) * p.SW;
-            const bool there = row < rows && (__ldcg(anc + (tok >> 5)) >> (tok & 31) & 1u);
+            const bool there = row < rows && (__ldg(anc + (tok >> 5)) >> (tok & 31) & 1u);
             const bool live = __any_sync(0xffffffffu, there);  // the warp has a row to compute
             const size_t orow = ((size_t)pc.w * p.Hq + hq) * p.S + tok;
             float m = neg_inf(), l = 0.f;
@@ -360,31 +360,50 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                     const int c0 = two ? 0 : grp, step = two ? 1 : NG;
                     if (!there) {
                         for (int c = c0; c < E / 8; c += step) *slot(c) = make_uint4(0u, 0u, 0u, 0u);
-                    } else if (half % 8 == 0) {
+                    } else if (p.rot_vec) {
+                        // chunk pairs two at a time, all their loads in flight together
                         const int nh = half / 8;
-                        for (int c = c0; c < nh; c += step) {
-                            const uint4 xv = __ldg(reinterpret_cast<const uint4*>(q + c * 8)), yv = __ldg(reinterpret_cast<const uint4*>(q + (c + nh) * 8));
-                            const T* x = reinterpret_cast<const T*>(&xv);
-                            const T* y = reinterpret_cast<const T*>(&yv);
-                            uint32_t lo[4], hi[4];
+                        for (int c = c0; c < nh; c += 2 * step) {
+                            uint4 xv[2], yv[2];
+                            float4 cv[2][2], sv[2][2];
 #pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                float a[2], b[2];
+                            for (int z = 0; z < 2; ++z) {
+                                const int cc = min(c + z * step, nh - 1);
+                                xv[z] = __ldg(reinterpret_cast<const uint4*>(q + cc * 8));
+                                yv[z] = __ldg(reinterpret_cast<const uint4*>(q + (cc + nh) * 8));
 #pragma unroll
-                                for (int v = 0; v < 2; ++v) {
-                                    const float cv = __ldg(p.cos + cs + c * 8 + 2 * u + v), sv = __ldg(p.sin + cs + c * 8 + 2 * u + v);
-                                    const float xf = Elem<T>::to_f(x[2 * u + v]), yf = Elem<T>::to_f(y[2 * u + v]);
-                                    a[v] = __fsub_rn(__fmul_rn(xf, cv), __fmul_rn(yf, sv));
-                                    b[v] = __fadd_rn(__fmul_rn(yf, cv), __fmul_rn(xf, sv));
+                                for (int u = 0; u < 2; ++u) {
+                                    cv[z][u] = __ldg(reinterpret_cast<const float4*>(p.cos + cs + cc * 8 + 4 * u));
+                                    sv[z][u] = __ldg(reinterpret_cast<const float4*>(p.sin + cs + cc * 8 + 4 * u));
                                 }
-                                lo[u] = Elem<T>::pack2(a[0], a[1]);
-                                hi[u] = Elem<T>::pack2(b[0], b[1]);
                             }
-                            *slot(c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                            *slot(c + nh) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+#pragma unroll
+                            for (int z = 0; z < 2; ++z) {
+                                const int cc = min(c + z * step, nh - 1);  // the last pair twice where the count is odd
+                                const T* x = reinterpret_cast<const T*>(&xv[z]);
+                                const T* y = reinterpret_cast<const T*>(&yv[z]);
+                                const float* cf = reinterpret_cast<const float*>(cv[z]);
+                                const float* sf = reinterpret_cast<const float*>(sv[z]);
+                                uint32_t lo[4], hi[4];
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) {
+                                    float a[2], b[2];
+#pragma unroll
+                                    for (int v = 0; v < 2; ++v) {
+                                        const float xf = Elem<T>::to_f(x[2 * u + v]), yf = Elem<T>::to_f(y[2 * u + v]);
+                                        a[v] = __fsub_rn(__fmul_rn(xf, cf[2 * u + v]), __fmul_rn(yf, sf[2 * u + v]));
+                                        b[v] = __fadd_rn(__fmul_rn(yf, cf[2 * u + v]), __fmul_rn(xf, sf[2 * u + v]));
+                                    }
+                                    lo[u] = Elem<T>::pack2(a[0], a[1]);
+                                    hi[u] = Elem<T>::pack2(b[0], b[1]);
+                                }
+                                *slot(cc) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                                *slot(cc + nh) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            }
                         }
+#pragma unroll 4
                         for (int c = 2 * nh + c0; c < E / 8; c += step) *slot(c) = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
-                    } else {  // a rotary half that ends inside a chunk: element by element
+                    } else {  // a rotary half that ends inside a chunk, unaligned tables: element by element
                         for (int c = c0; c < E / 8; c += step) {
                             alignas(16) T o[8];
                             for (int u = 0; u < 8; ++u) {
@@ -429,23 +448,21 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                     if (p.scale_log2 <= 0.f)
 #pragma unroll
                         for (int c = 0; c < KT; ++c) sv[c] = p.scale_log2 == 0.f ? 0.f : -sv[c];
-                    uint32_t see[KT / 32];
-                    bool every = true;
+                    if (win.f == p.F || !__all_sync(0xffffffffu, win.k0 >= 0 && lim - win.k0 >= KT)) {
 #pragma unroll
-                    for (int x = 0; x < KT / 32; ++x) {
-                        if (win.f < p.F) {
-                            const int d = lim - win.k0 - 32 * x, e = -win.k0 - 32 * x;  // columns in front of d, not of e
-                            see[x] = d >= 32 ? 0xffffffffu : d <= 0 ? 0u : (1u << d) - 1;
-                            see[x] &= e <= 0 ? 0xffffffffu : e >= 32 ? 0u : 0xffffffffu << e;
-                        } else {
-                            see[x] = there ? __ldcg(anc + (win.k0 >> 5) + x) : 0u;
+                        for (int x = 0; x < KT / 32; ++x) {
+                            uint32_t see;
+                            if (win.f < p.F) {
+                                const int d = lim - win.k0 - 32 * x, e = -win.k0 - 32 * x;  // columns in front of d, not of e
+                                see = d >= 32 ? 0xffffffffu : d <= 0 ? 0u : (1u << d) - 1;
+                                see &= e <= 0 ? 0xffffffffu : e >= 32 ? 0u : 0xffffffffu << e;
+                            } else {
+                                see = there ? __ldg(anc + (win.k0 >> 5) + x) : 0u;
+                            }
+#pragma unroll
+                            for (int c = 0; c < 32; ++c)
+                                if (!(see >> c & 1u)) sv[32 * x + c] = neg_inf();
                         }
-                        every = every && see[x] == 0xffffffffu;
-                    }
-                    if (!__all_sync(0xffffffffu, every)) {
-#pragma unroll
-                        for (int c = 0; c < KT; ++c)
-                            if (!(see[c >> 5] >> (c & 31) & 1u)) sv[c] = neg_inf();
                     }
                     float mx[8];
 #pragma unroll
@@ -509,7 +526,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                     }
                     const int key = win.k0 + r;
                     bool seen = r < win.n && key >= 0;
-                    if (seen && win.f == p.F) seen = __ldcg(p.anc + ((size_t)pc.w * p.S + key) * p.SW + (key >> 5)) >> (key & 31) & 1u;
+                    if (seen && win.f == p.F) seen = __ldg(p.anc + ((size_t)pc.w * p.S + key) * p.SW + (key >> 5)) >> (key & 31) & 1u;
                     if (r < KT && !seen) {
                         uint8_t* v = smem + off_v + (iw % VS) * C::KTILE + r * 128;
 #pragma unroll
@@ -638,6 +655,7 @@ bool tree_tc_maps(TreeParams& p, int dtype, int E, TreeMaps& m) {
     int b = kt;  // the largest power of two that divides the page size, at most a window
     while (p.BS % b) b >>= 1;
     const long long tokens = p.NB * p.BS, drafts = (long long)p.W * p.Hkv * p.S;
+    p.rot_vec = p.R % 16 == 0 && !((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15);
     p.box = 0;
     p.align = 1;
     // 8 rows are what the 128-byte swizzle repeats over; coordinates are 32-bit

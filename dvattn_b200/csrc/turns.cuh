@@ -40,7 +40,28 @@ __device__ __forceinline__ int turn_windows(const TurnSplit& p, int seen, long l
     return seen > 0 ? ((int)(off % p.align) + seen + p.kt - 1) / p.kt : 0;
 }
 
-__device__ __forceinline__ long long split_bound(long long total, int g, int groups) { return total * g / groups; }
+// The split of `total` windows over the groups: the first total % groups of them take one
+// window more than the others.
+struct SplitRange {
+    long long q, r;  // windows of a group, groups with one more
+    __device__ __forceinline__ SplitRange(long long total, int groups) {
+        if (total <= 0x7fffffffLL) {
+            const unsigned t = (unsigned)total, n = (unsigned)groups;
+            q = t / n;
+            r = t % n;
+        } else {
+            q = total / groups;
+            r = total % groups;
+        }
+    }
+    __device__ __forceinline__ long long begin(int g) const { return g * q + (g < r ? g : r); }
+    // the group of window u < total; the groups between two windows' are never empty
+    __device__ __forceinline__ int group_of(long long u) const {
+        const long long more = r * (q + 1);
+        if (u < more) return (int)(u <= 0x7fffffffLL && q < 0x7fffffffLL ? (unsigned)u / (unsigned)(q + 1) : u / (q + 1));
+        return (int)(r + (u - more <= 0x7fffffffLL && q <= 0x7fffffffLL ? (unsigned)(u - more) / (unsigned)q : (u - more) / q));
+    }
+};
 
 // Totals and the position of unit `at` among the windows, by one whole warp (every lane
 // returns the same values): `w` the sequence, `base` the first unit of its windows.
