@@ -97,12 +97,7 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
     SplitWalk walk;
-    {
-        const SplitRange range(split_total(p, lane), p.groups);
-        walk.u = range.begin(g);
-        walk.u1 = range.begin(g + 1);
-        split_locate(p, lane, walk.u, walk.w, walk.base);
-    }
+    walk.place(p, lane, g);
     SplitPiece pc;
     while (walk.next(p, pc)) {
         SplitWin win;

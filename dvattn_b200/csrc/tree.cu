@@ -137,12 +137,7 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
     SplitWalk walk;
-    {
-        const SplitRange range(split_total(p, lane), p.groups);
-        walk.u = range.begin(g);
-        walk.u1 = range.begin(g + 1);
-        split_locate(p, lane, walk.u, walk.w, walk.base);
-    }
+    walk.place(p, lane, g);
     const int rows = p.S * p.G;
     SplitPiece pc;
     while (walk.next(p, pc)) {
@@ -410,7 +405,7 @@ static int tree_validate(const dvattn_tree_args* a) {
     if (a->S > kTreeMaxTokens) return DVATTN_ERR_UNSUPPORTED;
     // grid limits: sequences are the prep grid's x, row blocks its y; items are the merge grid's x
     const long long rows = (long long)a->S * (a->Hq / a->Hkv);
-    if ((long long)a->Hkv * a->S > 65534LL * kPrepRows || (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
+    if ((long long)a->W * a->Hq * a->S > 0x7fffffffLL || (long long)a->Hkv * a->S > 65534LL * kPrepRows || (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
     return DVATTN_OK;
 }
 

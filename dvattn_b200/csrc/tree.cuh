@@ -22,6 +22,7 @@ struct TreeParams : TurnSplit {
     int mi;  // rows per item
     int box;  // rows of a TMA box (pages and windows are whole numbers of boxes); 0: rows are gathered
     int rot_vec;     // rotary halves are whole 16-byte chunks, cos/sin rows 16-byte aligned
+    int out_sectors; // the output is 32-byte aligned
     int stall_tile;  // test hook (DVATTN_TEST_STALL_TILE), -1: off
     float scale_log2;
     void* out;

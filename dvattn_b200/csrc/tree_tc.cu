@@ -28,7 +28,11 @@ template <int E> struct TcCfg {
     static constexpr int NG = E == 256 ? 1 : 2;     // softmax groups (and O accumulators)
     static constexpr int NP = E / 64;               // 64-column panels
     static constexpr int QPANEL = 128 * 128, KPANEL = KT * 128, QTILE = NP * QPANEL, KTILE = NP * KPANEL;
-    static constexpr int NT = (4 * NG + 3) * 32;
+    static constexpr int NT = (4 * NG + 4) * 32;    // the last warpgroup: MMA, K, V, one idle warp
+    // Registers: two softmax warpgroups with a row of 128 scores each do not fit in the 168 of an
+    // even share (they spilled, the batched decode took 206 us instead of @); 384 x 168 =
+    // 256 x 208 + 128 x 88.  With one softmax warpgroup every thread may have 255.
+    static constexpr bool SPLIT_REGS = NG == 2;
     static constexpr int WARP_MMA = 4 * NG, WARP_K = 4 * NG + 1, WARP_V = 4 * NG + 2;
     static constexpr int RING = E == 64 ? 4 : 3;    // most stages of a ring
     // tiles of 32 KB (16 KB at E = 64): Q, the K ring, the V ring
@@ -41,6 +45,13 @@ template <int E> struct TcCfg {
     static constexpr int SMEM = OFF_ML + 2 * 128 * 8;
     static_assert(SMEM <= 232448, "more shared memory than a CTA may use");
 };
+
+// 32 bytes in one store (the address a multiple of 32).
+__device__ __forceinline__ void store_sector(void* dst, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 
 template <class T, int E>
 __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, const __grid_constant__ TreeMaps maps) {
@@ -89,12 +100,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
 
     const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
     SplitWalk walk;
-    {
-        const SplitRange range(split_total(p, lane), p.groups);
-        walk.u = range.begin(g);
-        walk.u1 = range.begin(g + 1);
-        split_locate(p, lane, walk.u, walk.w, walk.base);
-    }
+    walk.place(p, lane, g);
     SplitPiece pc;
     SplitWin win;
     // a whole warp waits, and gives up as a whole
@@ -107,6 +113,8 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         }
     };
 
+    if (wid >= C::WARP_MMA) {
+        if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if ((wid == C::WARP_K || wid == C::WARP_V) && p.box) {
         // ============================== TMA producers ==============================
         const bool is_k = wid == C::WARP_K;
@@ -319,118 +327,233 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             }
         }
         __syncwarp();
+    }
     } else {
         // ================================= softmax =================================
+        if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int grp = wid >> 2, r = (wid & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((wid & 3) * 32) << 16;
         const uint32_t tO = tmem + lanes + 256 + 128 * grp;
         const int tile = two ? grp : 0;  // the query tile this thread's row lies in
+        const bool join = NG == 2 && !two;
         float2* sML = reinterpret_cast<float2*>(smem + C::OFF_ML);
         const int rows = p.S * p.G, half = p.R >> 1;
-        int j = 0, iw = 0, piece = 0;
-        bool ok = true;
-        while (ok && walk.next(p, pc)) {
-            win.start(p, pc.w);
+        int j = 0, iw = 0, piece = 0, turn = -1;
+        // ---- this thread's row of the piece at hand ----
+        int tok = 0, orow = 0;  // token, output row
+        bool in = false, there = false, live = false;  // a row; its token is there; the warp has such a row
+        auto enter = [&] {
             const int row = pc.t * p.mi + tile * 128 + r;
-            const int tok = row < rows ? row / p.G : 0, hq = h * p.G + (row < rows ? row - tok * p.G : 0);
-            const uint32_t* anc = p.anc + ((size_t)pc.w * p.S + tok) * p.SW;
-            const bool there = row < rows && (__ldg(anc + (tok >> 5)) >> (tok & 31) & 1u);
-            const bool live = __any_sync(0xffffffffu, there);  // the warp has a row to compute
-            const size_t orow = ((size_t)pc.w * p.Hq + hq) * p.S + tok;
-            float m = neg_inf(), l = 0.f;
-            const int jp = j;
-            int turn = -1, lim = 0, lim_f = -1, mine = 0;
-            for (int i = pc.i0; ok && i < pc.i1; ++i, ++iw) {
+            in = row < rows;
+            tok = in ? row / p.G : 0;
+            orow = (pc.w * p.Hq + h * p.G + (in ? row - tok * p.G : 0)) * p.S + tok;
+            there = in && (__ldcg(p.anc + ((size_t)pc.w * p.S + tok) * p.SW + (tok >> 5)) >> (tok & 31) & 1u);
+            live = __any_sync(0xffffffffu, there);
+            win.start(p, pc.w);
+            turn = -1;
+        };
+        // The row's q, rotated for turn qt, into the A tile, once every S that reads the tile's
+        // old contents has completed.  With one tile the groups share the row, chunk pairs by parity.
+        auto rotate = [&](int qt) {
+            if (two ? j > 0 && !wait(s_full + 8 * grp, (j - 2 + grp) >> 1)
+                    : (j > 0 && !wait(s_full + 8 * ((j - 1) & 1), (j - 1) >> 1)) || (j > 1 && !wait(s_full + 8 * (j & 1), (j - 2) >> 1)))
+                return false;
+            turn = qt;
+            const T* q = static_cast<const T*>(p.q) + (size_t)orow * E;
+            const size_t cs = (((size_t)qt * p.W + pc.w) * p.S + tok) * p.R;
+            const uint32_t qt0 = (uint32_t)(tile * C::QTILE + r * 128);
+            auto slot = [&](int c) { return reinterpret_cast<uint4*>(smem + qt0 + (c >> 3) * C::QPANEL + (((c & 7) ^ (r & 7)) << 4)); };
+            const int c0 = two ? 0 : grp, step = two ? 1 : NG;
+            if (!there) {
+                for (int c = c0; c < E / 8; c += step) *slot(c) = make_uint4(0u, 0u, 0u, 0u);
+            } else if (p.rot_vec) {
+                // chunk pairs two at a time, all their loads in flight together
+                const int nh = half / 8;
+                for (int c = c0; c < nh; c += 2 * step) {
+                    uint4 xv[2], yv[2];
+                    float4 cv[2][2], sv[2][2];
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const int cc = min(c + z * step, nh - 1);
+                        xv[z] = __ldg(reinterpret_cast<const uint4*>(q + cc * 8));
+                        yv[z] = __ldg(reinterpret_cast<const uint4*>(q + (cc + nh) * 8));
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            cv[z][u] = __ldg(reinterpret_cast<const float4*>(p.cos + cs + cc * 8 + 4 * u));
+                            sv[z][u] = __ldg(reinterpret_cast<const float4*>(p.sin + cs + cc * 8 + 4 * u));
+                        }
+                    }
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const int cc = min(c + z * step, nh - 1);  // the last pair twice where the count is odd
+                        const T* x = reinterpret_cast<const T*>(&xv[z]);
+                        const T* y = reinterpret_cast<const T*>(&yv[z]);
+                        const float* cf = reinterpret_cast<const float*>(cv[z]);
+                        const float* sf = reinterpret_cast<const float*>(sv[z]);
+                        uint32_t lo[4], hi[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            float a[2], b[2];
+#pragma unroll
+                            for (int v = 0; v < 2; ++v) {
+                                const float xf = Elem<T>::to_f(x[2 * u + v]), yf = Elem<T>::to_f(y[2 * u + v]);
+                                a[v] = __fsub_rn(__fmul_rn(xf, cf[2 * u + v]), __fmul_rn(yf, sf[2 * u + v]));
+                                b[v] = __fadd_rn(__fmul_rn(yf, cf[2 * u + v]), __fmul_rn(xf, sf[2 * u + v]));
+                            }
+                            lo[u] = Elem<T>::pack2(a[0], a[1]);
+                            hi[u] = Elem<T>::pack2(b[0], b[1]);
+                        }
+                        *slot(cc) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        *slot(cc + nh) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    }
+                }
+#pragma unroll 4
+                for (int c = 2 * nh + c0; c < E / 8; c += step) *slot(c) = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
+            } else {  // a rotary half that ends inside a chunk, unaligned tables: element by element
+                for (int c = c0; c < E / 8; c += step) {
+                    alignas(16) T o[8];
+                    for (int u = 0; u < 8; ++u) {
+                        const int e = c * 8 + u;
+                        o[u] = q[e];
+                        if (e < p.R) {
+                            const int x = e < half ? e : e - half;
+                            const float a = Elem<T>::to_f(q[e]), b = Elem<T>::to_f(e < half ? q[e + half] : q[e - half]);
+                            o[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(a, __ldg(p.cos + cs + x)), __fmul_rn(e < half ? -b : b, __ldg(p.sin + cs + x))));
+                        }
+                    }
+                    *slot(c) = *reinterpret_cast<const uint4*>(o);
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(q_ready + 8 * tile);
+            return true;
+        };
+        // One turn of a piece after the other.  A finished piece's result is written after the
+        // next piece's q has gone into the tile, so that its first S runs meanwhile.  What the
+        // inner loop over the windows does not need is kept out of it: a row of 128 scores leaves
+        // few registers.
+        float m = neg_inf(), l = 0.f;  // running maximum (log2 units, stepped) and sum
+        int jp = 0, mine = 0, i = 0;
+        bool pending = false, whole = false, was_in = false, was_live = false;
+        int was_row = 0, jobs = 0;
+        size_t prow = 0;
+        bool have = walk.next(p, pc), ok = true;
+        if (have) {
+            enter();
+            i = pc.i0;
+        }
+        while (have || pending) {
+            if (have) {
                 win.seek(p, pc.w, i);
                 const int qt = min(win.f, p.F - 1);
-                if (qt != turn) {
-                    // ---- this row's q, rotated for the turn, into the A tile ----
-                    // every S that reads the tile's old contents has completed
-                    if (j > jp && !(two ? wait(s_full + 8 * grp, (j - 2 + grp) >> 1)
-                                        : wait(s_full + 8 * ((j - 1) & 1), (j - 1) >> 1) && (j < 2 || wait(s_full + 8 * (j & 1), (j - 2) >> 1)))) {
-                        ok = false;
-                        break;
+                if (qt != turn && !(ok = rotate(qt))) break;
+            }
+            if (pending) {
+                // ---- the piece's result ----
+                if (!(ok = wait(o_done, piece))) break;
+                tc_fence_after();
+                float w0 = 1.f, w1 = 0.f;
+                bool other = false;  // O of the other group has jobs in it
+                if (join) {
+                    sML[grp * 128 + r] = make_float2(m, l);
+                    mbar_arrive(epi1);
+                    if (!(ok = wait(epi1, piece))) break;
+                    const float2 a = sML[r], b = sML[128 + r];
+                    m = fmaxf(a.x, b.x);
+                    const float mu = m == neg_inf() ? 0.f : m;
+                    w0 = a.x == neg_inf() && a.y == 0.f ? 0.f : ex2(a.x - mu);
+                    w1 = b.x == neg_inf() && b.y == 0.f ? 0.f : ex2(b.x - mu);
+                    l = a.y * w0 + b.y * w1;
+                    // first the accumulator of the piece's first job, which always has one
+                    other = jobs > 1;
+                    if (jp & 1) {
+                        const float x = w0;
+                        w0 = w1, w1 = x;
                     }
-                    turn = qt;
-                    const T* q = static_cast<const T*>(p.q) + orow * E;
-                    const size_t cs = (((size_t)qt * p.W + pc.w) * p.S + tok) * p.R;
-                    const uint32_t qt0 = (uint32_t)(tile * C::QTILE + r * 128);
-                    auto slot = [&](int c) { return reinterpret_cast<uint4*>(smem + qt0 + (c >> 3) * C::QPANEL + (((c & 7) ^ (r & 7)) << 4)); };
-                    // with one tile the two groups share the row: chunk pairs by parity
-                    const int c0 = two ? 0 : grp, step = two ? 1 : NG;
-                    if (!there) {
-                        for (int c = c0; c < E / 8; c += step) *slot(c) = make_uint4(0u, 0u, 0u, 0u);
-                    } else if (p.rot_vec) {
-                        // chunk pairs two at a time, all their loads in flight together
-                        const int nh = half / 8;
-                        for (int c = c0; c < nh; c += 2 * step) {
-                            uint4 xv[2], yv[2];
-                            float4 cv[2][2], sv[2][2];
+                }
+                const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+                const float lse2 = l == 0.f ? neg_inf() : m + log2f(l);
+                const uint32_t ta = join ? tmem + lanes + 256 + 128 * (jp & 1) : tO, tb = tmem + lanes + 256 + 128 * (~jp & 1);
+                const int cb = join ? grp * (E / 64) : 0, ce = join ? cb + E / 64 : E / 32;  // this thread's 32-column blocks
+#pragma unroll 1
+                for (int c = cb; c < ce; ++c) {
+                    float ov[32];
+                    if (was_live) {
+                        tmem_ld32(ta + 32 * c, ov);
+                        tmem_wait_ld();
+                        reg_fence<32>(ov);
 #pragma unroll
-                            for (int z = 0; z < 2; ++z) {
-                                const int cc = min(c + z * step, nh - 1);
-                                xv[z] = __ldg(reinterpret_cast<const uint4*>(q + cc * 8));
-                                yv[z] = __ldg(reinterpret_cast<const uint4*>(q + (cc + nh) * 8));
+                        for (int u = 0; u < 32; ++u) ov[u] *= w0 * inv;
+                        if (other) {
+                            float o2[32];
+                            tmem_ld32(tb + 32 * c, o2);
+                            tmem_wait_ld();
+                            reg_fence<32>(o2);
 #pragma unroll
-                                for (int u = 0; u < 2; ++u) {
-                                    cv[z][u] = __ldg(reinterpret_cast<const float4*>(p.cos + cs + cc * 8 + 4 * u));
-                                    sv[z][u] = __ldg(reinterpret_cast<const float4*>(p.sin + cs + cc * 8 + 4 * u));
-                                }
-                            }
-#pragma unroll
-                            for (int z = 0; z < 2; ++z) {
-                                const int cc = min(c + z * step, nh - 1);  // the last pair twice where the count is odd
-                                const T* x = reinterpret_cast<const T*>(&xv[z]);
-                                const T* y = reinterpret_cast<const T*>(&yv[z]);
-                                const float* cf = reinterpret_cast<const float*>(cv[z]);
-                                const float* sf = reinterpret_cast<const float*>(sv[z]);
-                                uint32_t lo[4], hi[4];
-#pragma unroll
-                                for (int u = 0; u < 4; ++u) {
-                                    float a[2], b[2];
-#pragma unroll
-                                    for (int v = 0; v < 2; ++v) {
-                                        const float xf = Elem<T>::to_f(x[2 * u + v]), yf = Elem<T>::to_f(y[2 * u + v]);
-                                        a[v] = __fsub_rn(__fmul_rn(xf, cf[2 * u + v]), __fmul_rn(yf, sf[2 * u + v]));
-                                        b[v] = __fadd_rn(__fmul_rn(yf, cf[2 * u + v]), __fmul_rn(xf, sf[2 * u + v]));
-                                    }
-                                    lo[u] = Elem<T>::pack2(a[0], a[1]);
-                                    hi[u] = Elem<T>::pack2(b[0], b[1]);
-                                }
-                                *slot(cc) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                                *slot(cc + nh) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                            }
-                        }
-#pragma unroll 4
-                        for (int c = 2 * nh + c0; c < E / 8; c += step) *slot(c) = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
-                    } else {  // a rotary half that ends inside a chunk, unaligned tables: element by element
-                        for (int c = c0; c < E / 8; c += step) {
-                            alignas(16) T o[8];
-                            for (int u = 0; u < 8; ++u) {
-                                const int e = c * 8 + u;
-                                o[u] = q[e];
-                                if (e < p.R) {
-                                    const int x = e < half ? e : e - half;
-                                    const float a = Elem<T>::to_f(q[e]), b = Elem<T>::to_f(e < half ? q[e + half] : q[e - half]);
-                                    o[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(a, __ldg(p.cos + cs + x)), __fmul_rn(e < half ? -b : b, __ldg(p.sin + cs + x))));
-                                }
-                            }
-                            *slot(c) = *reinterpret_cast<const uint4*>(o);
+                            for (int u = 0; u < 32; ++u) ov[u] += o2[u] * (w1 * inv);
                         }
                     }
-                    fence_proxy_async_smem();
-                    mbar_arrive(q_ready + 8 * tile);
+                    if (l == 0.f)  // a token that is not there, a piece without a key that it sees
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) ov[u] = 0.f;
+                    if (was_in) {
+                        // a thread writes whole 32-byte sectors of its row
+                        uint32_t x[32];
+                        if (whole) {
+                            T* op = static_cast<T*>(p.out) + (size_t)was_row * E + 32 * c;
+#pragma unroll
+                            for (int u = 0; u < 16; ++u) x[u] = Elem<T>::pack2(ov[2 * u], ov[2 * u + 1]);
+                            if (p.out_sectors) {
+#pragma unroll
+                                for (int u = 0; u < 2; ++u) store_sector(op + 16 * u, x + 8 * u);
+                            } else {
+#pragma unroll
+                                for (int u = 0; u < 4; ++u)
+                                    *reinterpret_cast<uint4*>(op + 8 * u) = make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) x[u] = __float_as_uint(ov[u]);
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) store_sector(p.part_o + prow * E + 32 * c + 8 * u, x + 8 * u);
+                        }
+                    }
                 }
-                if (win.f < p.F && win.f != lim_f) {
-                    lim_f = win.f;
-                    lim = there ? turn_seen(__ldg(p.L + win.f), __ldg(p.loc + ((size_t)win.f * p.W + pc.w) * p.S + tok), win.off, p.cap) : 0;
+                if (was_in && (!join || grp == 0)) {
+                    if (!whole) p.part_lse[prow] = lse2;
+                    else if (p.lse_out) p.lse_out[was_row] = lse2 * kLn2;
                 }
-                // ---- this group's job of the window, if it has one ----
-                const int job = two ? j + grp : j;
-                j += two ? 2 : 1;
-                if (NG == 2 && !two && (job & 1) != grp) continue;
-                const int b = job & 1;
+                if (join) {
+                    // both groups have read both accumulators before the next piece's PV writes them
+                    tc_fence_before();
+                    mbar_arrive(epi2);
+                    if (!(ok = wait(epi2, piece))) break;
+                }
+                pending = false;
+                ++piece;
+                m = neg_inf(), l = 0.f;
+                jp = j, mine = 0;
+                if (!have) break;
+            }
+            const bool tail = win.f == p.F;
+            const int lim = !there || tail ? 0
+                            : turn_seen(__ldg(p.L + win.f), __ldg(p.loc + ((size_t)win.f * p.W + pc.w) * p.S + tok), win.off, p.cap);
+            // ---- this group's jobs of the turn's windows ----
+            const int nx = min(pc.i1, win.first + win.nf) - i, k00 = win.k0, sp = win.sp;
+            for (int x0 = join ? (grp - j) & 1 : 0; x0 < nx; x0 += join ? 2 : 1) {
+                const int job = two ? j + 2 * x0 + grp : j + x0, b = job & 1;
+                const int k0 = k00 + x0 * KT, n = min(KT, sp - k0);
                 const uint32_t tS = tmem + lanes + KT * b;
+                // drafted keys: the row's ancestors among them, and whether the thread's V row counts
+                uint32_t anc[KT / 32];
+                bool v_seen = r < n && k0 + r >= 0;
+                if (tail) {
+                    const uint32_t* words = p.anc + (size_t)pc.w * p.S * p.SW;
+                    const int key = k0 + r;
+#pragma unroll
+                    for (int x = 0; x < KT / 32; ++x) anc[x] = there ? __ldcg(words + (size_t)tok * p.SW + (k0 >> 5) + x) : 0u;
+                    if (v_seen) v_seen = __ldcg(words + (size_t)key * p.SW + (key >> 5)) >> (key & 31) & 1u;
+                }
                 if (!wait(s_full + 8 * b, job >> 1)) {
                     ok = false;
                     break;
@@ -448,16 +571,16 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                     if (p.scale_log2 <= 0.f)
 #pragma unroll
                         for (int c = 0; c < KT; ++c) sv[c] = p.scale_log2 == 0.f ? 0.f : -sv[c];
-                    if (win.f == p.F || !__all_sync(0xffffffffu, win.k0 >= 0 && lim - win.k0 >= KT)) {
+                    if (tail || !__all_sync(0xffffffffu, k0 >= 0 && lim - k0 >= KT)) {
 #pragma unroll
                         for (int x = 0; x < KT / 32; ++x) {
                             uint32_t see;
-                            if (win.f < p.F) {
-                                const int d = lim - win.k0 - 32 * x, e = -win.k0 - 32 * x;  // columns in front of d, not of e
+                            if (tail) {
+                                see = anc[x];
+                            } else {
+                                const int d = lim - k0 - 32 * x, e = -k0 - 32 * x;  // columns in front of d, not of e
                                 see = d >= 32 ? 0xffffffffu : d <= 0 ? 0u : (1u << d) - 1;
                                 see &= e <= 0 ? 0xffffffffu : e >= 32 ? 0u : 0xffffffffu << e;
-                            } else {
-                                see = there ? __ldg(anc + (win.k0 >> 5) + x) : 0u;
                             }
 #pragma unroll
                             for (int c = 0; c < 32; ++c)
@@ -500,7 +623,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                         // O holds the PV of this group's earlier jobs.  With two groups they completed
                         // before this S was signalled (S(j) is issued after PV(j - 2)); with one, the
                         // last of them is PV(j - 1), whose completion frees its V window.
-                        if (NG == 1 && !wait(v_empty + 8 * ((iw - 1) % VS), (iw - 1) / VS)) {
+                        if (NG == 1 && !wait(v_empty + 8 * ((iw + x0 - 1) % VS), (iw + x0 - 1) / VS)) {
                             ok = false;
                             break;
                         }
@@ -518,17 +641,14 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                     }
                     tmem_wait_st();
                 }
-                if (p.box && (!two || grp == 0) && (win.f == p.F || win.k0 < 0 || win.n < KT)) {
+                if (p.box && (!two || grp == 0) && (tail || k0 < 0 || n < KT)) {
                     // V rows of this window that nobody sees: P is 0 there
-                    if (!wait(v_full + 8 * (iw % VS), iw / VS)) {
+                    if (!wait(v_full + 8 * ((iw + x0) % VS), (iw + x0) / VS)) {
                         ok = false;
                         break;
                     }
-                    const int key = win.k0 + r;
-                    bool seen = r < win.n && key >= 0;
-                    if (seen && win.f == p.F) seen = __ldg(p.anc + ((size_t)pc.w * p.S + key) * p.SW + (key >> 5)) >> (key & 31) & 1u;
-                    if (r < KT && !seen) {
-                        uint8_t* v = smem + off_v + (iw % VS) * C::KTILE + r * 128;
+                    if (r < KT && !v_seen) {
+                        uint8_t* v = smem + off_v + ((iw + x0) % VS) * C::KTILE + r * 128;
 #pragma unroll
                         for (int x = 0; x < C::NP; ++x)
 #pragma unroll
@@ -541,95 +661,19 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                 ++mine;
             }
             if (!ok) break;
-            // ---- the piece's result ----
-            if (!wait(o_done, piece)) {
-                ok = false;
-                break;
-            }
-            tc_fence_after();
-            const bool join = NG == 2 && !two;
-            float w0 = 1.f, w1 = 0.f;
-            bool other = false;  // O of the other group has jobs in it
-            if (join) {
-                sML[grp * 128 + r] = make_float2(m, l);
-                mbar_arrive(epi1);
-                if (!wait(epi1, piece)) {
-                    ok = false;
-                    break;
-                }
-                const float2 a = sML[r], b = sML[128 + r];
-                m = fmaxf(a.x, b.x);
-                const float mu = m == neg_inf() ? 0.f : m;
-                w0 = a.x == neg_inf() && a.y == 0.f ? 0.f : ex2(a.x - mu);
-                w1 = b.x == neg_inf() && b.y == 0.f ? 0.f : ex2(b.x - mu);
-                l = a.y * w0 + b.y * w1;
-                // first the accumulator of the piece's first job, which always has one
-                other = j - jp > 1;
-                if (jp & 1) {
-                    const float x = w0;
-                    w0 = w1, w1 = x;
+            j += two ? 2 * nx : nx;
+            iw += nx;
+            i += nx;
+            if (i == pc.i1) {
+                pending = true;
+                whole = pc.whole(), was_in = in, was_live = live, was_row = orow, jobs = j - jp;
+                prow = ((size_t)blockIdx.x * 2 + pc.slot()) * p.mi + tile * 128 + r;
+                have = walk.next(p, pc);
+                if (have) {
+                    enter();
+                    i = pc.i0;
                 }
             }
-            const bool whole = pc.whole();
-            const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-            const float lse2 = l == 0.f ? neg_inf() : m + log2f(l);
-            const size_t prow = ((size_t)blockIdx.x * 2 + pc.slot()) * p.mi + tile * 128 + r;
-            const uint32_t ta = join ? tmem + lanes + 256 + 128 * (jp & 1) : tO, tb = tmem + lanes + 256 + 128 * (~jp & 1);
-            const int cb = join ? grp * (E / 64) : 0, ce = join ? cb + E / 64 : E / 32;  // this thread's 32-column blocks
-            if (live) {
-#pragma unroll 1
-                for (int c = cb; c < ce; ++c) {
-                    float ov[32];
-                    tmem_ld32(ta + 32 * c, ov);
-                    tmem_wait_ld();
-                    reg_fence<32>(ov);
-#pragma unroll
-                    for (int u = 0; u < 32; ++u) ov[u] *= w0 * inv;
-                    if (other) {
-                        float o2[32];
-                        tmem_ld32(tb + 32 * c, o2);
-                        tmem_wait_ld();
-                        reg_fence<32>(o2);
-#pragma unroll
-                        for (int u = 0; u < 32; ++u) ov[u] += o2[u] * (w1 * inv);
-                    }
-                    if (l == 0.f)
-#pragma unroll
-                        for (int u = 0; u < 32; ++u) ov[u] = 0.f;
-                    if (row < rows) {
-                        if (whole) {
-                            T* op = static_cast<T*>(p.out) + orow * E + 32 * c;
-#pragma unroll
-                            for (int u = 0; u < 32; u += 8)
-                                *reinterpret_cast<uint4*>(op + u) = make_uint4(Elem<T>::pack2(ov[u], ov[u + 1]), Elem<T>::pack2(ov[u + 2], ov[u + 3]),
-                                                                               Elem<T>::pack2(ov[u + 4], ov[u + 5]), Elem<T>::pack2(ov[u + 6], ov[u + 7]));
-                        } else {
-                            float* op = p.part_o + prow * E + 32 * c;
-#pragma unroll
-                            for (int u = 0; u < 32; u += 4) *reinterpret_cast<float4*>(op + u) = make_float4(ov[u], ov[u + 1], ov[u + 2], ov[u + 3]);
-                        }
-                    }
-                }
-            } else if (row < rows) {  // a warp without a token that is there
-                for (int e = 32 * cb; e < 32 * ce; e += 4) {
-                    if (whole) *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + orow * E + e) = make_uint2(0u, 0u);
-                    else *reinterpret_cast<float4*>(p.part_o + prow * E + e) = make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-            }
-            if (row < rows && (!join || grp == 0)) {
-                if (!whole) p.part_lse[prow] = lse2;
-                else if (p.lse_out) p.lse_out[orow] = lse2 * kLn2;
-            }
-            if (join) {
-                // both groups have read both accumulators before the next piece's PV writes them
-                tc_fence_before();
-                mbar_arrive(epi2);
-                if (!wait(epi2, piece)) {
-                    ok = false;
-                    break;
-                }
-            }
-            ++piece;
         }
         if (!ok) give_up(8);
     }
@@ -656,6 +700,7 @@ bool tree_tc_maps(TreeParams& p, int dtype, int E, TreeMaps& m) {
     while (p.BS % b) b >>= 1;
     const long long tokens = p.NB * p.BS, drafts = (long long)p.W * p.Hkv * p.S;
     p.rot_vec = p.R % 16 == 0 && !((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15);
+    p.out_sectors = !(reinterpret_cast<uintptr_t>(p.out) & 31);
     p.box = 0;
     p.align = 1;
     // 8 rows are what the 128-byte swizzle repeats over; coordinates are 32-bit

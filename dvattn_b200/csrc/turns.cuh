@@ -63,38 +63,6 @@ struct SplitRange {
     }
 };
 
-// Totals and the position of unit `at` among the windows, by one whole warp (every lane
-// returns the same values): `w` the sequence, `base` the first unit of its windows.
-__device__ __forceinline__ long long split_total(const TurnSplit& p, int lane) {
-    long long t = 0;
-    for (int w = lane; w < p.W; w += 32) t += __ldcg(p.nwin + w);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    return t * p.nt;
-}
-__device__ __forceinline__ void split_locate(const TurnSplit& p, int lane, long long at, int& w, long long& base) {
-    long long acc = 0;
-    for (int w0 = 0; w0 < p.W; w0 += 32) {
-        const long long mine = w0 + lane < p.W ? (long long)__ldcg(p.nwin + w0 + lane) * p.nt : 0;
-        long long incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += up;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, mine > 0 && at >= acc + incl - mine && at < acc + incl);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            w = w0 + src;
-            base = acc + __shfl_sync(0xffffffffu, incl - mine, src);
-            return;
-        }
-        acc += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    w = p.W;
-    base = acc;
-}
-
 // A piece of a CTA's range: windows [i0, i1) of the nw windows of item (w, t, h).
 struct SplitPiece {
     int w, t, i0, i1, nw;
@@ -103,22 +71,69 @@ struct SplitPiece {
 };
 // Walks a range [u, u1) of units; every role of a CTA walks it for itself.
 struct SplitWalk {
-    long long u, u1, base;
-    int w;
+    long long u, u1, base;  // next unit, end, first unit of sequence w's windows
+    int w, nw;              // sequence, its windows per row tile
+    // The range of group g, by one whole warp (every lane ends with the same values).  The
+    // window counts of up to 256 sequences are loaded at once: one round trip to L2.
+    __device__ __forceinline__ void place(const TurnSplit& p, int lane, int g) {
+        constexpr int N = 8;
+        int v[N];
+        long long total = 0;
+        for (int w0 = 0; w0 < p.W; w0 += 32 * N) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int x = w0 + 32 * k + lane;
+                v[k] = x < p.W ? __ldcg(p.nwin + x) : 0;
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) total += v[k];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        const SplitRange range(total * p.nt, p.groups);
+        u = range.begin(g);
+        u1 = range.begin(g + 1);
+        base = 0;
+        w = p.W;
+        nw = 0;
+        for (int w0 = 0; w0 < p.W; w0 += 32 * N) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int x = w0 + 32 * k + lane;
+                if (p.W > 32 * N) v[k] = x < p.W ? __ldcg(p.nwin + x) : 0;
+                int incl = v[k];
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += up;
+                }
+                const long long end = base + (long long)incl * p.nt;
+                const unsigned hit = __ballot_sync(0xffffffffu, v[k] > 0 && u < end);
+                if (hit) {
+                    const int src = __ffs(hit) - 1;
+                    w = w0 + 32 * k + src;
+                    nw = __shfl_sync(0xffffffffu, v[k], src);
+                    base = __shfl_sync(0xffffffffu, end, src) - (long long)nw * p.nt;
+                    return;
+                }
+                base = __shfl_sync(0xffffffffu, end, 31);
+            }
+        }
+    }
     __device__ __forceinline__ bool next(const TurnSplit& p, SplitPiece& pc) {
         while (u < u1 && w < p.W) {
-            const int nw = __ldcg(p.nwin + w);
             const long long end = base + (long long)nw * p.nt;
             if (u >= end) {
                 base = end;
                 ++w;
+                if (w < p.W) nw = __ldcg(p.nwin + w);
                 continue;
             }
-            const long long local = u - base;
+            const int local = (int)(u - base);
             pc.w = w;
             pc.nw = nw;
-            pc.t = (int)(local / nw);
-            pc.i0 = (int)(local - (long long)pc.t * nw);
+            pc.t = p.nt == 1 ? 0 : local / nw;
+            pc.i0 = local - pc.t * nw;
             const long long left = u1 - u;
             pc.i1 = left < nw - pc.i0 ? pc.i0 + (int)left : nw;
             u += pc.i1 - pc.i0;
