@@ -18,6 +18,7 @@ namespace dvb {
 
 struct MassParams : TurnSplit {
     int Hq, Hkv, G, S, R, rows;  // rows = S * G queries of a KV head: row r = (query r / G, head r % G)
+    int rot_vec;                 // rotary halves are whole 16-byte chunks, cos/sin rows 16-byte aligned
     long long N;                 // positions of a mass row
     float scale_log2;
     float* mass;
@@ -56,13 +57,13 @@ __global__ void __launch_bounds__(128) mass_prep_kernel(MassParams p, int E) {
             __syncthreads();
             v = max(max(red[0], red[1]), max(red[2], red[3]));
             __syncthreads();
-            if (tid == 0) p.span[(size_t)w * p.F + t] = v;
-            nw += turn_windows(p, v, off);
+            const int first = v > 0 ? (int)off : 0;
+            if (tid == 0) p.span[(size_t)w * p.F + t] = make_int2(v, first);
+            nw += turn_windows(p, v, first);
             off += Lt > 0 ? Lt : 0;
         }
         if (tid == 0) p.nwin[w] = nw;
     }
-    const int half = p.R >> 1;
     for (int r = r0 + (tid >> 5); r < r1; r += 4) {  // a warp per row
         const int s = r / p.G, hq = h * p.G + (r - s * p.G);
         const size_t qrow = ((size_t)w * p.Hq + hq) * p.S + s;
@@ -70,18 +71,9 @@ __global__ void __launch_bounds__(128) mass_prep_kernel(MassParams p, int E) {
             const float x = __ldg(p.lse + qrow);
             p.lse2[((size_t)w * p.Hkv + h) * p.rows + r] = x == neg_inf() ? -neg_inf() : x * kLog2e;
         }
-        const T* x = static_cast<const T*>(p.q) + qrow * E;
-        T* y = static_cast<T*>(p.qr) + ((((size_t)f * p.W + w) * p.Hkv + h) * p.rows + r) * E;
         const size_t cs = (((size_t)f * p.W + w) * p.S + s) * p.R;
-        for (int e = tid & 31; e < E; e += 32) {
-            if (e >= p.R) {
-                y[e] = x[e];
-            } else {
-                const int j = e < half ? e : e - half;
-                const float a = Elem<T>::to_f(x[e]), b = Elem<T>::to_f(e < half ? x[e + half] : x[e - half]);
-                y[e] = Elem<T>::from_f(__fadd_rn(__fmul_rn(a, __ldg(p.cos + cs + j)), __fmul_rn(e < half ? -b : b, __ldg(p.sin + cs + j))));
-            }
-        }
+        rotate_row<T>(static_cast<const T*>(p.q) + qrow * E, static_cast<T*>(p.qr) + ((((size_t)f * p.W + w) * p.Hkv + h) * p.rows + r) * E,
+                      p.cos + cs, p.sin + cs, E, p.R, p.rot_vec, tid & 31, 32);
     }
 }
 
@@ -108,7 +100,7 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
                 const int r = c / CH, ch = c - r * CH;
                 const T* kp = nullptr;
                 if (r < win.n) {
-                    const int pos = (int)(win.off + win.k0 + r);
+                    const int pos = win.off + win.k0 + r;
                     const int page = __ldg(p.bt + (size_t)pc.w * p.maxb + pos / p.BS);
                     if (page >= 0 && page < p.NB)
                         kp = static_cast<const T*>(p.k) + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E + ch * PER;
@@ -156,7 +148,7 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
             red[wid * KT + lane] = acc;
             __syncthreads();
             if (wid == 0 && lane < win.n) {
-                const long long pos = win.off + win.k0 + lane;
+                const long long pos = (long long)win.off + win.k0 + lane;
                 if (pos < p.N) {
                     float sum = red[lane];
 #pragma unroll
@@ -223,7 +215,7 @@ static int mass_layout(const dvattn_mass_args* a, const MassKernel& k, MassLayou
         return r;
     };
     L.nwin = take(4 * (size_t)a->W);
-    L.span = take(4 * (size_t)a->W * a->F);
+    L.span = take(8 * (size_t)a->W * a->F);
     L.qr = take(esz * (size_t)a->F * a->W * a->Hkv * rows * a->E);
     L.lse2 = take(4 * (size_t)a->W * a->Hkv * rows);
     L.total = at;
@@ -252,6 +244,7 @@ int mass_launch(const dvattn_mass_args* a, void* workspace, size_t wbytes, cudaS
     MassParams p{};
     p.F = a->F; p.W = a->W; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.S = a->S; p.R = a->R;
     p.rows = p.S * p.G;
+    p.rot_vec = rotate_vec(a->R, a->cosines, a->sines);
     p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
     const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
     p.cap = cap > 0x7fffffffLL ? 0x7fffffff : (int)cap;
@@ -262,7 +255,7 @@ int mass_launch(const dvattn_mass_args* a, void* workspace, size_t wbytes, cudaS
     p.loc = a->locations; p.L = a->fragment_lengths; p.bt = a->block_tables;
     p.header = reinterpret_cast<int*>(ws);
     p.nwin = reinterpret_cast<int*>(ws + L.nwin);
-    p.span = reinterpret_cast<int*>(ws + L.span);
+    p.span = reinterpret_cast<int2*>(ws + L.span);
     p.qr = ws + L.qr;
     p.lse2 = reinterpret_cast<float*>(ws + L.lse2);
     const void* prep = a->dtype == DVATTN_FLOAT32   ? (const void*)&mass_prep_kernel<float>

@@ -16,30 +16,34 @@
 namespace dvb {
 
 // ---- prep ---------------------------------------------------------------------------
-// Block (w, 0) finds sequence w's ancestor sets and spans; the others rotate its drafted
-// keys, a warp per (token, KV head) row.  The rotation is apply_rotary_pos_emb's with
-// separate roundings of the two products and of the sum, then one rounding to T, so a
-// drafted key has the bits that the paged append writes for it.
-constexpr int kPrepRows = 8;  // rows of a rotating block (of 4 warps)
+// Block (w, 0) finds sequence w's ancestor sets, what each token sees of each turn and the
+// spans; the others rotate its queries for every turn and its drafted keys, once for all the
+// CTAs that read them.  Reads and writes (F + 1 parts of Hkv rows) a few percent of a call's
+// bytes; done by the attention kernel's own threads, the rotation stood between two pieces of
+// its work for 5 us and more.
+constexpr int kPrepRows = 32;  // rows of a rotating block
 
 template <class T>
-__global__ void __launch_bounds__(128) tree_prep_kernel(TreeParams p, int E) {
+__global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
     extern __shared__ int par[];  // [S] parents, then [S] whether a token is there
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int w = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    int* there = par + p.S;
+    for (int j = tid; j < p.S; j += 256) par[j] = __ldg(p.parents + (size_t)w * p.S + j);
+    __syncthreads();
+    // a token is there if its line of parents, each before its child, ends at -1
+    for (int j = tid; j < p.S; j += 256) {
+        int c = j;
+        while (c >= 0 && par[c] < c && par[c] >= -1) c = par[c];
+        there[j] = c == -1;
+    }
+    __syncthreads();
     if (blockIdx.y == 0) {
-        __shared__ int red[4];
-        int* there = par + p.S;
+        __shared__ int red[8];
         if (w == 0 && tid < 4) p.header[tid] = 0;
-        for (int j = tid; j < p.S; j += 128) par[j] = __ldg(p.parents + (size_t)w * p.S + j);
-        __syncthreads();
-        // a token is there if its line of parents, each before its child, ends at -1
-        for (int j = tid; j < p.S; j += 128) {
-            int c = j;
-            while (c >= 0 && par[c] < c && par[c] >= -1) c = par[c];
-            there[j] = c == -1;
+        for (int j = tid; j < p.S; j += 256) {
             uint32_t* a = p.anc + ((size_t)w * p.S + j) * p.SW;
-            c = c == -1 ? j : -1;
+            int c = there[j] ? j : -1;
             for (int word = p.SW - 1; word >= 0; --word) {
                 uint32_t bits = 0;
                 while (c >= 32 * word) {  // c < 32 * (word + 1) here: parents come before
@@ -50,43 +54,54 @@ __global__ void __launch_bounds__(128) tree_prep_kernel(TreeParams p, int E) {
                 a[word] = bits;
             }
         }
-        __syncthreads();
         long long off = 0;
         int nw = 0;
         for (int f = 0; f < p.F; ++f) {
             const int Lf = __ldg(p.L + f);
             int v = 0;
-            for (int s = tid; s < p.S; s += 128) {
-                const int n = turn_seen(Lf, __ldg(p.loc + ((size_t)f * p.W + w) * p.S + s), off, p.cap);
-                if (there[s]) v = max(v, n);
+            for (int s = tid; s < p.S; s += 256) {
+                const size_t at = ((size_t)f * p.W + w) * p.S + s;
+                const int n = there[s] ? turn_seen(Lf, __ldg(p.loc + at), off, p.cap) : 0;
+                p.lim[at] = n;
+                v = max(v, n);
             }
             v = __reduce_max_sync(0xffffffffu, v);
             if (lane == 0) red[wid] = v;
             __syncthreads();
-            v = max(max(red[0], red[1]), max(red[2], red[3]));
+            v = 0;
+            for (int x = 0; x < 8; ++x) v = max(v, red[x]);
             __syncthreads();
-            if (tid == 0) p.span[(size_t)w * p.F + f] = v;
-            nw += turn_windows(p, v, off);
+            const int first = v > 0 ? (int)off : 0;  // below cap where a key is seen
+            if (tid == 0) p.span[(size_t)w * p.F + f] = make_int2(v, first);
+            nw += turn_windows(p, v, first);
             off += Lf > 0 ? Lf : 0;
         }
         if (tid == 0) p.nwin[w] = nw + (p.S + p.kt - 1) / p.kt;
         return;
     }
-    const int half = p.R >> 1, rows = p.Hkv * p.S, r0 = (blockIdx.y - 1) * kPrepRows;
-    for (int r = r0 + wid; r < min(r0 + kPrepRows, rows); r += 4) {
-        const int s = r % p.S;
-        const size_t at = ((size_t)w * rows + r) * E, cs = (((size_t)(p.F - 1) * p.W + w) * p.S + s) * p.R;
-        const T* x = static_cast<const T*>(p.dk) + at;
-        T* y = static_cast<T*>(p.dkr) + at;
-        for (int e = lane; e < E; e += 32) {
-            if (e >= p.R) {
-                y[e] = x[e];
-            } else {
-                const int j = e < half ? e : e - half;
-                const float c = __ldg(p.cos + cs + j), sn = __ldg(p.sin + cs + j);
-                const float a = Elem<T>::to_f(x[e]), b = Elem<T>::to_f(e < half ? x[e + half] : x[e - half]);
-                y[e] = Elem<T>::from_f(__fadd_rn(__fmul_rn(a, c), __fmul_rn(e < half ? -b : b, sn)));
-            }
+    // rows: the drafted keys [Hkv][S], then the queries [F][Hkv][rows]
+    const int keys = p.Hkv * p.S, all = keys + p.F * p.Hkv * p.rows, r0 = (blockIdx.y - 1) * kPrepRows;
+    const int lanes = min(32, E * (int)sizeof(T) / 16), per = 32 / lanes;
+    for (int x = r0 + wid * per + lane / lanes; x < min(r0 + kPrepRows, all); x += 8 * per) {
+        const T* src;
+        T* dst;
+        int f = p.F - 1, s;
+        if (x < keys) {
+            s = x % p.S;
+            src = static_cast<const T*>(p.dk) + ((size_t)w * keys + x) * E;
+            dst = static_cast<T*>(p.dkr) + ((size_t)w * keys + x) * E;
+        } else {
+            const int y = x - keys, h = y / p.rows % p.Hkv, r = y % p.rows;
+            f = y / p.rows / p.Hkv;
+            s = r / p.G;
+            src = static_cast<const T*>(p.q) + (((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s) * E;
+            dst = static_cast<T*>(p.qr) + ((((size_t)f * p.W + w) * p.Hkv + h) * p.rows + r) * E;
+        }
+        const size_t cs = (((size_t)f * p.W + w) * p.S + s) * p.R;
+        if (there[s]) {
+            rotate_row<T>(src, dst, p.cos + cs, p.sin + cs, E, p.R, p.rot_vec, lane % lanes, lanes);
+        } else {
+            for (int c = lane % lanes; c < E * (int)sizeof(T) / 16; c += lanes) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0u, 0u, 0u, 0u);
         }
     }
 }
@@ -110,7 +125,7 @@ __device__ __forceinline__ const T* tree_row(const TreeParams& p, const void* ca
         if (!(__ldcg(p.anc + ((size_t)w * p.S + l) * p.SW + (l >> 5)) >> (l & 31) & 1u)) return nullptr;
         return static_cast<const T*>(draft) + (((size_t)w * p.Hkv + h) * p.S + l) * E;
     }
-    const int pos = (int)(win.off + l);
+    const int pos = win.off + l;
     const int page = __ldg(p.bt + (size_t)w * p.maxb + pos / p.BS);
     if (page < 0 || page >= p.NB) return nullptr;
     return static_cast<const T*>(cache) + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E;
@@ -138,7 +153,7 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
     const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
     SplitWalk walk;
     walk.place(p, lane, g);
-    const int rows = p.S * p.G;
+    const int rows = p.rows;
     SplitPiece pc;
     while (walk.next(p, pc)) {
         SplitWin ld, win;
@@ -186,27 +201,16 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
             const int qt = win.f < p.F ? win.f : p.F - 1;  // the turn whose rotation q takes
             if (qt != turn) {
                 turn = qt;
+                const T* qr = static_cast<const T*>(p.qr) + (((size_t)qt * p.W + pc.w) * p.Hkv + h) * p.rows * E;
                 for (int c = tid; c < MI * E; c += C::THREADS) {
                     const int r = c / E, e = c - r * E, rr = pc.t * MI + r;
-                    float x = 0.f;
-                    if (rr < rows) {
-                        const int s = rr / p.G, hq = h * p.G + (rr - s * p.G), half = p.R >> 1;
-                        const T* q = static_cast<const T*>(p.q) + (((size_t)pc.w * p.Hq + hq) * p.S + s) * E;
-                        x = Elem<T>::to_f(q[e]);
-                        if (e < p.R) {
-                            const size_t cs = (((size_t)qt * p.W + pc.w) * p.S + s) * p.R + (e < half ? e : e - half);
-                            const float b = Elem<T>::to_f(e < half ? q[e + half] : q[e - half]);
-                            x = __fadd_rn(__fmul_rn(x, __ldg(p.cos + cs)), __fmul_rn(e < half ? -b : b, __ldg(p.sin + cs)));
-                            x = Elem<T>::to_f(Elem<T>::from_f(x));
-                        }
-                    }
-                    sQ[r * (E + 4) + e] = x;
+                    sQ[r * (E + 4) + e] = rr < p.rows ? Elem<T>::to_f(__ldcg(qr + (size_t)rr * E + e)) : 0.f;
                 }
             }
             if (win.f < p.F)
 #pragma unroll
                 for (int a = 0; a < 4; ++a)
-                    lim[a] = there >> a & 1u ? turn_seen(__ldg(p.L + win.f), __ldg(p.loc + ((size_t)win.f * p.W + pc.w) * p.S + tok[a]), win.off, p.cap) : 0;
+                    lim[a] = there >> a & 1u ? __ldcg(p.lim + ((size_t)win.f * p.W + pc.w) * p.S + tok[a]) : 0;
             __syncthreads();
             // scores of this warp's 4 rows and the lane's key
             float sc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -405,12 +409,12 @@ static int tree_validate(const dvattn_tree_args* a) {
     if (a->S > kTreeMaxTokens) return DVATTN_ERR_UNSUPPORTED;
     // grid limits: sequences are the prep grid's x, row blocks its y; items are the merge grid's x
     const long long rows = (long long)a->S * (a->Hq / a->Hkv);
-    if ((long long)a->W * a->Hq * a->S > 0x7fffffffLL || (long long)a->Hkv * a->S > 65534LL * kPrepRows || (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
+    if ((long long)a->F * a->W * a->Hq * a->S > 0x7fffffffLL || ((long long)a->F * a->Hq + a->Hkv) * a->S > 65534LL * kPrepRows || (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
     return DVATTN_OK;
 }
 
 struct TreeLayout {
-    size_t nwin, span, anc, dkr, po, pl, total;
+    size_t nwin, span, anc, lim, dkr, qr, po, pl, total;
     int groups, sw, nt;
 };
 
@@ -433,8 +437,10 @@ static int tree_layout(const dvattn_tree_args* a, const TreeKernel& k, TreeLayou
         return r;
     };
     L.nwin = take(4 * (size_t)a->W);
-    L.span = take(4 * (size_t)a->W * a->F);
+    L.span = take(8 * (size_t)a->W * a->F);
     L.anc = take(4 * (size_t)a->W * a->S * L.sw);
+    L.lim = take(4 * (size_t)a->F * a->W * a->S);
+    L.qr = take(esz * (size_t)a->F * a->W * a->Hq * a->S * a->E);
     L.dkr = take(esz * (size_t)a->W * a->Hkv * a->S * a->E);
     L.po = take(4 * ctas * 2 * k.mi * a->E);
     L.pl = take(4 * ctas * 2 * k.mi);
@@ -473,6 +479,8 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     char* ws = static_cast<char*>(workspace);
     TreeParams p{};
     p.F = a->F; p.W = a->W; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.S = a->S; p.R = a->R;
+    p.rows = p.S * p.G;
+    p.rot_vec = rotate_vec(a->R, a->cosines, a->sines);
     p.tail = a->S; p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
     const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
     p.cap = a->num_blocks <= 0 ? 0 : cap > 0x7fffffffLL ? 0x7fffffff : (int)cap;
@@ -485,7 +493,9 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     p.stall_tile = tree_stall_hook();
     p.header = reinterpret_cast<int*>(ws);
     p.nwin = reinterpret_cast<int*>(ws + L.nwin);
-    p.span = reinterpret_cast<int*>(ws + L.span);
+    p.span = reinterpret_cast<int2*>(ws + L.span);
+    p.lim = reinterpret_cast<int*>(ws + L.lim);
+    p.qr = ws + L.qr;
     p.anc = reinterpret_cast<uint32_t*>(ws + L.anc);
     p.dkr = ws + L.dkr;
     p.part_o = reinterpret_cast<float*>(ws + L.po);
@@ -500,7 +510,7 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
                         : a->dtype == DVATTN_FLOAT16 ? merge_fn<__half>(a->E) : merge_fn<__nv_bfloat16>(a->E);
     int E = a->E;
     void* pargs[] = {&p, &E};
-    if (cudaLaunchKernel(prep, dim3(a->W, 1 + (a->Hkv * a->S + kPrepRows - 1) / kPrepRows), dim3(128), pargs,
+    if (cudaLaunchKernel(prep, dim3(a->W, 1 + (a->Hkv * a->S + a->F * a->Hq * a->S + kPrepRows - 1) / kPrepRows), dim3(256), pargs,
                          2 * sizeof(int) * (size_t)a->S, stream) != cudaSuccess)
         return DVATTN_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};

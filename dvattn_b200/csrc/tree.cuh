@@ -22,6 +22,7 @@ struct TreeParams : TurnSplit {
     int mi;  // rows per item
     int box;  // rows of a TMA box (pages and windows are whole numbers of boxes); 0: rows are gathered
     int rot_vec;     // rotary halves are whole 16-byte chunks, cos/sin rows 16-byte aligned
+    int rows;        // S * G query rows of a KV head
     int out_sectors; // the output is 32-byte aligned
     int stall_tile;  // test hook (DVATTN_TEST_STALL_TILE), -1: off
     float scale_log2;
@@ -38,7 +39,9 @@ struct TreeParams : TurnSplit {
     // workspace
     int* header;      // [3] error word (kErrorWordOffset)
     uint32_t* anc;    // [W][S][SW] ancestor sets; a token that is not there has an empty one
+    int* lim;         // [F][W][S] keys of the turn that the token sees; 0: it is not there
     void* dkr;        // [W][Hkv][S][E] T, drafted keys rotated
+    void* qr;         // [F][W][Hkv][rows][E] T, queries rotated for the turn, zeros where the token is not there
     float* part_o;    // [CTAs][2][mi][E] normalised partial outputs
     float* part_lse;  // [CTAs][2][mi] log2 sums, -inf: nothing seen
 };
@@ -51,7 +54,7 @@ struct TreeKernel {
 };
 // the 16-bit kernel on the 5th-generation tensor cores (tree_tc.cu), and its tensor maps
 struct TreeMaps {
-    CUtensorMap k, v, dk, dv;
+    CUtensorMap q, k, v, dk, dv;
 };
 TreeKernel tree_tc_pick(int dtype, int E, int rows);
 // Sets p.box and p.align and fills the maps the kernel then uses; false: a CUDA error.

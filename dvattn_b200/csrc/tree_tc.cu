@@ -28,18 +28,22 @@ template <int E> struct TcCfg {
     static constexpr int NG = E == 256 ? 1 : 2;     // softmax groups (and O accumulators)
     static constexpr int NP = E / 64;               // 64-column panels
     static constexpr int QPANEL = 128 * 128, KPANEL = KT * 128, QTILE = NP * QPANEL, KTILE = NP * KPANEL;
-    static constexpr int NT = (4 * NG + 4) * 32;    // the last warpgroup: MMA, K, V, one idle warp
+    static constexpr int NT = (4 * NG + 4) * 32;    // the last warpgroup: MMA, K, V, Q
     // Registers: two softmax warpgroups with a row of 128 scores each do not fit in the 168 of an
     // even share (they spilled, the batched decode took 206 us instead of @); 384 x 168 =
     // 256 x 208 + 128 x 88.  With one softmax warpgroup every thread may have 255.
     static constexpr bool SPLIT_REGS = NG == 2;
-    static constexpr int WARP_MMA = 4 * NG, WARP_K = 4 * NG + 1, WARP_V = 4 * NG + 2;
+    static constexpr int WARP_MMA = 4 * NG, WARP_K = 4 * NG + 1, WARP_V = 4 * NG + 2, WARP_Q = 4 * NG + 3;
     static constexpr int RING = E == 64 ? 4 : 3;    // most stages of a ring
-    // tiles of 32 KB (16 KB at E = 64): Q, the K ring, the V ring
+    // tiles of 32 KB (16 KB at E = 64): Q (room for two sets of one tile, so that the next turn's
+    // or piece's is there in time; with two tiles at E = 128, and at E = 256, one set), the K
+    // ring, the V ring
     static constexpr int K_STAGES = E == 64 ? 4 : E == 256 ? 2 : 3;
-    __host__ __device__ static constexpr int v_stages(bool two) { return E == 64 ? 4 : E == 256 ? 3 : two ? 2 : 3; }
-    __host__ __device__ static constexpr int q_bytes(bool two) { return two ? 2 * QTILE : QTILE; }
-    static constexpr int OFF_BAR = E == 64 ? 2 * QTILE + 8 * KTILE : 7 * 32768;
+    static constexpr int VS = E == 64 ? 4 : E == 256 ? 3 : 2;
+    __host__ __device__ static constexpr int q_sets(bool two) { return E == 64 ? 2 : E == 256 || two ? 1 : 2; }
+    static constexpr int OFF_K = E == 64 ? 4 * QTILE : E == 256 ? QTILE : 2 * QTILE;
+    static constexpr int OFF_V = OFF_K + K_STAGES * KTILE;
+    static constexpr int OFF_BAR = OFF_V + VS * KTILE;
     static constexpr int OFF_MISC = OFF_BAR + 32 * 8;
     static constexpr int OFF_ML = OFF_MISC + 64;    // [2][128] (maximum, sum)
     static constexpr int SMEM = OFF_ML + 2 * 128 * 8;
@@ -63,11 +67,12 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const bool bf16 = Elem<T>::dtype == DVATTN_BFLOAT16;
     const bool two = p.mi == 256;
-    const int VS = C::v_stages(two);
-    const uint32_t off_k = C::q_bytes(two), off_v = off_k + C::K_STAGES * C::KTILE;
+    constexpr int VS = C::VS;
+    constexpr uint32_t off_k = C::OFF_K, off_v = C::OFF_V;
+    const int q_sets = C::q_sets(two), q_set_bytes = two ? 2 * C::QTILE : C::QTILE;
     const uint32_t bar = s0 + C::OFF_BAR;
     const uint32_t k_full = bar, k_empty = bar + 32, v_full = bar + 64, v_empty = bar + 96;
-    const uint32_t s_full = bar + 128, p_full = bar + 144, q_ready = bar + 160, o_done = bar + 176, epi1 = bar + 184, epi2 = bar + 192;
+    const uint32_t s_full = bar + 128, p_full = bar + 144, q_full = bar + 160, q_empty = bar + 176, o_done = bar + 192, epi1 = bar + 200, epi2 = bar + 208;
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
     if (tid == 0) {
         for (int s = 0; s < C::RING; ++s) {
@@ -79,7 +84,8 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         for (int s = 0; s < 2; ++s) {
             mbar_init(s_full + 8 * s, 1);
             mbar_init(p_full + 8 * s, 128);
-            mbar_init(q_ready + 8 * s, two ? 128 : 128 * NG);
+            mbar_init(q_full + 8 * s, 1);
+            mbar_init(q_empty + 8 * s, 1);
         }
         mbar_init(o_done, 1);
         mbar_init(epi1, 128 * NG);
@@ -136,22 +142,11 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             if (win.f == p.F) {
                 next = (pc.w * p.Hkv + h) * p.S + win.k0;
             } else if (lane < boxes) {
-                const int l = win.k0 + lane * p.box, pos = (int)win.off + l;
+                const int l = win.k0 + lane * p.box, pos = win.off + l;
                 if (l + p.box > 0 && l < win.sp) {
                     const int page = __ldg(p.bt + (size_t)pc.w * p.maxb + pos / p.BS);
                     if (page >= 0 && page < p.NB) next = page * p.BS + pos % p.BS;
                 }
-            }
-        };
-        // the queries of a piece are on their way to L2 before the softmax threads ask for them
-        auto prefetch_q = [&] {
-            const int rows = p.S * p.G;
-            for (int x = lane; x < p.mi * (E / 64); x += 32) {
-                const int row = pc.t * p.mi + x / (E / 64);
-                if (row >= rows) break;
-                const int s = row / p.G;
-                const T* q = static_cast<const T*>(p.q) + (((size_t)pc.w * p.Hq + h * p.G + row - s * p.G) * p.S + s) * E + x % (E / 64) * 64;
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
             }
         };
         const bool stall = is_k && blockIdx.x == 0;  // test hook: this window never lands
@@ -160,7 +155,6 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         while (ok && walk.next(p, pc)) {
             win.start(p, pc.w);
             find(pc.i0);
-            if (!is_k) prefetch_q();
             for (int i = pc.i0; i < pc.i1; ++i, ++iw) {
                 const int st = iw % stages;
                 if (iw >= stages && (*s_abort || !wait_lazy(empty + 8 * st, iw / stages - 1))) {
@@ -208,7 +202,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                     if (__ldcg(p.anc + ((size_t)pc.w * p.S + l) * p.SW + (l >> 5)) >> (l & 31) & 1u)
                         next[k] = draft + (((size_t)pc.w * p.Hkv + h) * p.S + l) * E;
                 } else {
-                    const int pos = (int)win.off + l;
+                    const int pos = win.off + l;
                     const int page = __ldg(p.bt + (size_t)pc.w * p.maxb + pos / p.BS);
                     if (page >= 0 && page < p.NB) next[k] = cache + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E;
                 }
@@ -264,13 +258,47 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         cp_async_wait<0>();
         if (ok) hand_over(iw);
         else give_up(1);
+    } else if (wid == C::WARP_Q) {
+        // =================================== Q ====================================
+        // a piece's tiles, again for each turn (the drafted keys keep the last turn's)
+        asm volatile("fence.proxy.async;" ::: "memory");  // written by the kernel before, with ordinary stores
+        int epoch = 0;
+        bool ok = true;
+        while (ok && walk.next(p, pc)) {
+            win.start(p, pc.w);
+            int turn = -1;
+            for (int i = pc.i0; i < pc.i1; i += win.run(pc, i)) {
+                win.seek(p, pc.w, i);
+                const int qt = min(win.f, p.F - 1), set = epoch % q_sets;
+                if (qt == turn) continue;
+                if (epoch >= q_sets && (*s_abort || !wait_lazy(q_empty + 8 * set, epoch / q_sets - 1))) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) {
+                    mbar_expect_tx(q_full + 8 * set, (uint32_t)q_set_bytes);
+                    const int z = ((qt * p.W + pc.w) * p.Hkv + h) * p.rows + pc.t * p.mi;
+                    for (int t = 0; t < (two ? 2 : 1); ++t)
+#pragma unroll
+                        for (int x = 0; x < C::NP; ++x)
+                            tma_load_3d(s0 + (uint32_t)(set * q_set_bytes + t * C::QTILE + x * C::QPANEL), &maps.q, x * 64, 0, z + 128 * t, q_full + 8 * set);
+                }
+                __syncwarp();
+                turn = qt;
+                ++epoch;
+            }
+        }
+        if (!ok) {
+            give_up(1);
+            for (int x = max(0, epoch - q_sets); x < epoch; ++x) mbar_wait(q_full + 8 * (x % q_sets), (x / q_sets) & 1);
+        }
     } else if (wid == C::WARP_MMA) {
         // =================================== MMA ===================================
         // one thread: its waits, issues and commits are on every job's path
         const uint32_t id_s = idesc(bf16, 128, KT, false), id_o = idesc(bf16, 128, E, true);
         const uint64_t dq0 = sdesc(s0, 16, 1024), dk0 = sdesc(s0 + off_k, 16, 1024), dv0 = sdesc(s0 + off_v, C::KPANEL, 1024);
         if (lane == 0) {
-            int j = 0, ks = 0, kp = 0, vs = 0, vp = 0, epoch = 0, piece = 0;
+            int j = 0, ks = 0, kp = 0, vs = 0, vp = 0, qs = 0, qp = 0, piece = 0;
             bool ok = true;
             // PV of job jj, the n-th of its piece, over the V window at hand; `last`: its last use
             auto issue_pv = [&](int jj, int n, bool last) {
@@ -291,27 +319,34 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             while (ok && walk.next(p, pc)) {
                 win.start(p, pc.w);
                 int n = 0, turn = -1;  // jobs of the piece issued, the turn q is rotated for
-                for (int i = pc.i0; ok && i < pc.i1; ++i) {
+                for (int i = pc.i0; ok && i < pc.i1;) {
                     win.seek(p, pc.w, i);
-                    const int qt = min(win.f, p.F - 1);
-                    if (!mbar_wait(k_full + 8 * ks, kp)) ok = false;
-                    for (int t = 0; ok && t < (two ? 2 : 1); ++t, ++j, ++n) {
-                        if (qt != turn && !mbar_wait(q_ready + 8 * t, epoch & 1)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint64_t a0 = dq0 + (uint64_t)((t * C::QTILE) >> 4), b0 = dk0 + (uint64_t)((ks * C::KTILE) >> 4);
-#pragma unroll
-                        for (int kk = 0; kk < E / 16; ++kk)
-                            umma(tmem + KT * (j & 1), a0 + (uint64_t)(((kk >> 2) * C::QPANEL + (kk & 3) * 32) >> 4),
-                                 b0 + (uint64_t)(((kk >> 2) * C::KPANEL + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
-                        umma_commit(s_full + 8 * (j & 1));
-                        if (!two || t == 1) umma_commit(k_empty + 8 * ks);
-                        if (n > 0 && !issue_pv(j - 1, n - 1, !two || t == 0)) ok = false;
+                    const int qt = min(win.f, p.F - 1), end = i + win.run(pc, i);
+                    const bool last_of_q = end == pc.i1 || qt != p.F - 1;  // the next run has another q
+                    if (qt != turn) {
+                        if (!mbar_wait(q_full + 8 * qs, qp)) ok = false;
+                        turn = qt;
                     }
-                    if (++ks == C::K_STAGES) ks = 0, kp ^= 1;
-                    if (qt != turn) ++epoch, turn = qt;
+                    const uint64_t qd = dq0 + (uint64_t)((qs * q_set_bytes) >> 4);
+                    for (; ok && i < end; ++i) {
+                        if (!mbar_wait(k_full + 8 * ks, kp)) ok = false;
+                        for (int t = 0; ok && t < (two ? 2 : 1); ++t, ++j, ++n) {
+                            tc_fence_after();
+                            const uint64_t a0 = qd + (uint64_t)((t * C::QTILE) >> 4), b0 = dk0 + (uint64_t)((ks * C::KTILE) >> 4);
+#pragma unroll
+                            for (int kk = 0; kk < E / 16; ++kk)
+                                umma(tmem + KT * (j & 1), a0 + (uint64_t)(((kk >> 2) * C::QPANEL + (kk & 3) * 32) >> 4),
+                                     b0 + (uint64_t)(((kk >> 2) * C::KPANEL + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
+                            umma_commit(s_full + 8 * (j & 1));
+                            if (!two || t == 1) {
+                                umma_commit(k_empty + 8 * ks);
+                                if (last_of_q && i + 1 == end) umma_commit(q_empty + 8 * qs);
+                            }
+                            if (n > 0 && !issue_pv(j - 1, n - 1, !two || t == 0)) ok = false;
+                        }
+                        if (++ks == C::K_STAGES) ks = 0, kp ^= 1;
+                    }
+                    if (last_of_q && ++qs == q_sets) qs = 0, qp ^= 1;
                 }
                 if (ok) ok = issue_pv(j - 1, n - 1, true);
                 if (ok) {
@@ -337,103 +372,23 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         const int tile = two ? grp : 0;  // the query tile this thread's row lies in
         const bool join = NG == 2 && !two;
         float2* sML = reinterpret_cast<float2*>(smem + C::OFF_ML);
-        const int rows = p.S * p.G, half = p.R >> 1;
-        int j = 0, iw = 0, piece = 0, turn = -1;
+        int j = 0, iw = 0, piece = 0;
         // ---- this thread's row of the piece at hand ----
-        int tok = 0, orow = 0;  // token, output row
-        bool in = false, there = false, live = false;  // a row; its token is there; the warp has such a row
+        int tok = 0, orow = 0;         // token, output row
+        bool in = false, live = false;  // it is one; the warp has one
         auto enter = [&] {
             const int row = pc.t * p.mi + tile * 128 + r;
-            in = row < rows;
+            in = row < p.rows;
             tok = in ? row / p.G : 0;
             orow = (pc.w * p.Hq + h * p.G + (in ? row - tok * p.G : 0)) * p.S + tok;
-            there = in && (__ldcg(p.anc + ((size_t)pc.w * p.S + tok) * p.SW + (tok >> 5)) >> (tok & 31) & 1u);
-            live = __any_sync(0xffffffffu, there);
+            live = __any_sync(0xffffffffu, in);
             win.start(p, pc.w);
-            turn = -1;
         };
-        // The row's q, rotated for turn qt, into the A tile, once every S that reads the tile's
-        // old contents has completed.  With one tile the groups share the row, chunk pairs by parity.
-        auto rotate = [&](int qt) {
-            if (two ? j > 0 && !wait(s_full + 8 * grp, (j - 2 + grp) >> 1)
-                    : (j > 0 && !wait(s_full + 8 * ((j - 1) & 1), (j - 1) >> 1)) || (j > 1 && !wait(s_full + 8 * (j & 1), (j - 2) >> 1)))
-                return false;
-            turn = qt;
-            const T* q = static_cast<const T*>(p.q) + (size_t)orow * E;
-            const size_t cs = (((size_t)qt * p.W + pc.w) * p.S + tok) * p.R;
-            const uint32_t qt0 = (uint32_t)(tile * C::QTILE + r * 128);
-            auto slot = [&](int c) { return reinterpret_cast<uint4*>(smem + qt0 + (c >> 3) * C::QPANEL + (((c & 7) ^ (r & 7)) << 4)); };
-            const int c0 = two ? 0 : grp, step = two ? 1 : NG;
-            if (!there) {
-                for (int c = c0; c < E / 8; c += step) *slot(c) = make_uint4(0u, 0u, 0u, 0u);
-            } else if (p.rot_vec) {
-                // chunk pairs two at a time, all their loads in flight together
-                const int nh = half / 8;
-                for (int c = c0; c < nh; c += 2 * step) {
-                    uint4 xv[2], yv[2];
-                    float4 cv[2][2], sv[2][2];
-#pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        const int cc = min(c + z * step, nh - 1);
-                        xv[z] = __ldg(reinterpret_cast<const uint4*>(q + cc * 8));
-                        yv[z] = __ldg(reinterpret_cast<const uint4*>(q + (cc + nh) * 8));
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            cv[z][u] = __ldg(reinterpret_cast<const float4*>(p.cos + cs + cc * 8 + 4 * u));
-                            sv[z][u] = __ldg(reinterpret_cast<const float4*>(p.sin + cs + cc * 8 + 4 * u));
-                        }
-                    }
-#pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        const int cc = min(c + z * step, nh - 1);  // the last pair twice where the count is odd
-                        const T* x = reinterpret_cast<const T*>(&xv[z]);
-                        const T* y = reinterpret_cast<const T*>(&yv[z]);
-                        const float* cf = reinterpret_cast<const float*>(cv[z]);
-                        const float* sf = reinterpret_cast<const float*>(sv[z]);
-                        uint32_t lo[4], hi[4];
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            float a[2], b[2];
-#pragma unroll
-                            for (int v = 0; v < 2; ++v) {
-                                const float xf = Elem<T>::to_f(x[2 * u + v]), yf = Elem<T>::to_f(y[2 * u + v]);
-                                a[v] = __fsub_rn(__fmul_rn(xf, cf[2 * u + v]), __fmul_rn(yf, sf[2 * u + v]));
-                                b[v] = __fadd_rn(__fmul_rn(yf, cf[2 * u + v]), __fmul_rn(xf, sf[2 * u + v]));
-                            }
-                            lo[u] = Elem<T>::pack2(a[0], a[1]);
-                            hi[u] = Elem<T>::pack2(b[0], b[1]);
-                        }
-                        *slot(cc) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        *slot(cc + nh) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    }
-                }
-#pragma unroll 4
-                for (int c = 2 * nh + c0; c < E / 8; c += step) *slot(c) = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
-            } else {  // a rotary half that ends inside a chunk, unaligned tables: element by element
-                for (int c = c0; c < E / 8; c += step) {
-                    alignas(16) T o[8];
-                    for (int u = 0; u < 8; ++u) {
-                        const int e = c * 8 + u;
-                        o[u] = q[e];
-                        if (e < p.R) {
-                            const int x = e < half ? e : e - half;
-                            const float a = Elem<T>::to_f(q[e]), b = Elem<T>::to_f(e < half ? q[e + half] : q[e - half]);
-                            o[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(a, __ldg(p.cos + cs + x)), __fmul_rn(e < half ? -b : b, __ldg(p.sin + cs + x))));
-                        }
-                    }
-                    *slot(c) = *reinterpret_cast<const uint4*>(o);
-                }
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(q_ready + 8 * tile);
-            return true;
-        };
-        // One turn of a piece after the other.  A finished piece's result is written after the
-        // next piece's q has gone into the tile, so that its first S runs meanwhile.  What the
-        // inner loop over the windows does not need is kept out of it: a row of 128 scores leaves
-        // few registers.
+        // One turn of a piece after the other; a finished piece's result is written once what the
+        // next one needs is on its way.  What the inner loop over the windows does not need is
+        // kept out of it: a row of 128 scores leaves few registers.
         float m = neg_inf(), l = 0.f;  // running maximum (log2 units, stepped) and sum
-        int jp = 0, mine = 0, i = 0;
+        int jp = 0, mine = 0, i = 0, lim = 0;
         bool pending = false, whole = false, was_in = false, was_live = false;
         int was_row = 0, jobs = 0;
         size_t prow = 0;
@@ -445,8 +400,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         while (have || pending) {
             if (have) {
                 win.seek(p, pc.w, i);
-                const int qt = min(win.f, p.F - 1);
-                if (qt != turn && !(ok = rotate(qt))) break;
+                if (in && win.f < p.F) lim = __ldcg(p.lim + ((size_t)win.f * p.W + pc.w) * p.S + tok);
             }
             if (pending) {
                 // ---- the piece's result ----
@@ -536,10 +490,9 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                 if (!have) break;
             }
             const bool tail = win.f == p.F;
-            const int lim = !there || tail ? 0
-                            : turn_seen(__ldg(p.L + win.f), __ldg(p.loc + ((size_t)win.f * p.W + pc.w) * p.S + tok), win.off, p.cap);
+            if (!in || tail) lim = 0;
             // ---- this group's jobs of the turn's windows ----
-            const int nx = min(pc.i1, win.first + win.nf) - i, k00 = win.k0, sp = win.sp;
+            const int nx = win.run(pc, i), k00 = win.k0, sp = win.sp;
             for (int x0 = join ? (grp - j) & 1 : 0; x0 < nx; x0 += join ? 2 : 1) {
                 const int job = two ? j + 2 * x0 + grp : j + x0, b = job & 1;
                 const int k0 = k00 + x0 * KT, n = min(KT, sp - k0);
@@ -551,7 +504,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                     const uint32_t* words = p.anc + (size_t)pc.w * p.S * p.SW;
                     const int key = k0 + r;
 #pragma unroll
-                    for (int x = 0; x < KT / 32; ++x) anc[x] = there ? __ldcg(words + (size_t)tok * p.SW + (k0 >> 5) + x) : 0u;
+                    for (int x = 0; x < KT / 32; ++x) anc[x] = in ? __ldcg(words + (size_t)tok * p.SW + (k0 >> 5) + x) : 0u;
                     if (v_seen) v_seen = __ldcg(words + (size_t)key * p.SW + (key >> 5)) >> (key & 31) & 1u;
                 }
                 if (!wait(s_full + 8 * b, job >> 1)) {
@@ -699,10 +652,10 @@ bool tree_tc_maps(TreeParams& p, int dtype, int E, TreeMaps& m) {
     int b = kt;  // the largest power of two that divides the page size, at most a window
     while (p.BS % b) b >>= 1;
     const long long tokens = p.NB * p.BS, drafts = (long long)p.W * p.Hkv * p.S;
-    p.rot_vec = p.R % 16 == 0 && !((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15);
     p.out_sectors = !(reinterpret_cast<uintptr_t>(p.out) & 31);
     p.box = 0;
     p.align = 1;
+    if (!encode_cache_map(&m.q, p.qr, dtype, E, 1, (long long)p.F * p.W * p.Hq * p.S, 128)) return false;
     // 8 rows are what the 128-byte swizzle repeats over; coordinates are 32-bit
     if (b < 8 || p.cap == 0 || tokens > 0x7fffffffLL - 2 * (long long)p.BS || drafts > 0x7fffffffLL - kt) return true;
     p.box = b;

@@ -23,7 +23,7 @@ struct TurnSplit {
     const int* L;
     const int* bt;
     int* nwin;  // workspace: [W] windows of a sequence's row tile
-    int* span;  // workspace: [W][F] keys of the turn that some query of the sequence sees
+    int2* span;  // workspace: [W][F] {keys of the turn that some query of the sequence sees, its first position}
 };
 
 // Keys of a turn that a query with location `loc` sees, the turn starting at logical
@@ -35,9 +35,9 @@ __device__ __forceinline__ int turn_seen(int L, int loc, long long off, int cap)
     return v < room ? v : (int)room;
 }
 
-// Windows of a turn of which `seen` keys are seen.
-__device__ __forceinline__ int turn_windows(const TurnSplit& p, int seen, long long off) {
-    return seen > 0 ? ((int)(off % p.align) + seen + p.kt - 1) / p.kt : 0;
+// Windows of a turn of which `seen` keys are seen (`align` is a power of two).
+__device__ __forceinline__ int turn_windows(const TurnSplit& p, int seen, int off) {
+    return seen > 0 ? ((off & (p.align - 1)) + seen + p.kt - 1) / p.kt : 0;
 }
 
 // The split of `total` windows over the groups: the first total % groups of them take one
@@ -147,28 +147,79 @@ struct SplitWalk {
 // turn f (of the tail where f == F), for c < n and k0 + c >= 0.  Windows are sought in
 // increasing order; `start` begins a sequence.
 struct SplitWin {
-    int f, first, nf, sp, lead, k0, n;  // turn, its first window, its windows, its seen keys
-    long long off;                // the turn's first logical position
-    __device__ __forceinline__ void enter(const TurnSplit& p, int w) {
-        sp = f < p.F ? __ldcg(p.span + (size_t)w * p.F + f) : p.tail;
-        lead = f < p.F ? (int)(off % p.align) : 0;
+    int f, first, nf, sp, off, k0, n;  // turn, its first window, its windows, seen keys and first position
+    int2 ahead;                        // the next turn's, loaded a turn early
+    __device__ __forceinline__ int2 load(const TurnSplit& p, int w, int f_) const {
+        return f_ < p.F ? __ldcg(p.span + (size_t)w * p.F + f_) : make_int2(p.tail, 0);
+    }
+    __device__ __forceinline__ void enter(const TurnSplit& p, int w, int2 x) {
+        ahead = load(p, w, f + 1);
+        sp = x.x;
+        off = x.y;
         nf = f < p.F ? turn_windows(p, sp, off) : 0x7fffffff - first;
     }
     __device__ __forceinline__ void start(const TurnSplit& p, int w) {
-        f = 0, first = 0, off = 0;
-        enter(p, w);
+        f = 0, first = 0;
+        enter(p, w, load(p, w, 0));
     }
     __device__ __forceinline__ void seek(const TurnSplit& p, int w, int i) {
         while (i >= first + nf) {
-            const int Lf = __ldg(p.L + f);
-            off += Lf > 0 ? Lf : 0;
             first += nf;
             ++f;
-            enter(p, w);
+            enter(p, w, ahead);
         }
-        k0 = (i - first) * p.kt - lead;
+        k0 = (i - first) * p.kt - (off & (p.align - 1));
         n = min(p.kt, sp - k0);
     }
+    // windows from i on that belong to the same turn of the piece
+    __device__ __forceinline__ int run(const SplitPiece& pc, int i) const { return min(pc.i1, first + nf) - i; }
 };
+
+// One row of E elements rotated by apply_rotary_pos_emb: o[e] = x[e] c[e] - x[e + R/2] s[e],
+// o[e + R/2] = x[e + R/2] c[e] + x[e] s[e] for e < R/2 (the first half of the cos/sin row),
+// separate roundings of the products and of the sum, one rounding to T: the bits of the paged
+// append.  `LANES` lanes of a warp work on the row, lane `l` on 16-byte chunks l, l + LANES...
+template <class T>
+__device__ __forceinline__ void rotate_row(const T* x, T* y, const float* cos, const float* sin, int E, int R, bool vec, int l, int lanes) {
+    constexpr int PER = 16 / (int)sizeof(T);
+    const int half = R >> 1;
+    for (int c = l; c < E / PER; c += lanes) {
+        const int e0 = c * PER;
+        alignas(16) T a[PER], b[PER];
+        *reinterpret_cast<uint4*>(a) = __ldg(reinterpret_cast<const uint4*>(x + e0));
+        if (e0 >= R) {
+            *reinterpret_cast<uint4*>(y + e0) = *reinterpret_cast<const uint4*>(a);
+        } else if (vec) {  // rotary halves are whole chunks, cos/sin rows 16-byte aligned
+            const bool lo = e0 < half;
+            const int j = lo ? e0 : e0 - half;
+            *reinterpret_cast<uint4*>(b) = __ldg(reinterpret_cast<const uint4*>(x + (lo ? e0 + half : e0 - half)));
+            float cs[PER], sn[PER];
+#pragma unroll
+            for (int u = 0; u < PER; u += 4) {
+                *reinterpret_cast<float4*>(cs + u) = __ldg(reinterpret_cast<const float4*>(cos + j + u));
+                *reinterpret_cast<float4*>(sn + u) = __ldg(reinterpret_cast<const float4*>(sin + j + u));
+            }
+#pragma unroll
+            for (int u = 0; u < PER; ++u) {
+                const float v = Elem<T>::to_f(b[u]);
+                a[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(Elem<T>::to_f(a[u]), cs[u]), __fmul_rn(lo ? -v : v, sn[u])));
+            }
+            *reinterpret_cast<uint4*>(y + e0) = *reinterpret_cast<const uint4*>(a);
+        } else {
+            for (int u = 0; u < PER; ++u) {
+                const int e = e0 + u;
+                if (e < R) {
+                    const int j = e < half ? e : e - half;
+                    const float v = Elem<T>::to_f(e < half ? x[e + half] : x[e - half]);
+                    a[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(Elem<T>::to_f(x[e]), __ldg(cos + j)), __fmul_rn(e < half ? -v : v, __ldg(sin + j))));
+                }
+            }
+            *reinterpret_cast<uint4*>(y + e0) = *reinterpret_cast<const uint4*>(a);
+        }
+    }
+}
+inline bool rotate_vec(int R, const float* cos, const float* sin) {
+    return R % 16 == 0 && !((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15);
+}
 
 }  // namespace dvb
