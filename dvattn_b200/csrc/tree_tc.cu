@@ -9,8 +9,8 @@
 //                       with its own running maximum, sum and O, joined at the end of a piece
 //                       (one tile's chain softmax -> PV -> next S would not keep up with HBM);
 //   head dim 256:       one tile and one O (256 columns); only the score buffers alternate.
-// Warps: 4 per softmax group (a thread owns one query row = one TMEM lane), one MMA issuer,
-// one K and one V producer.  Producers fill swizzled rings with TMA boxes where pages and
+// Warps: 4 per softmax group (a thread owns one query row = one TMEM lane), one that walks the
+// range (split_schedule), one MMA issuer, one K (and Q) and one V producer.  Producers fill swizzled rings with TMA boxes where pages and
 // windows are whole numbers of boxes of 8 or more rows (page sizes that are multiples of 8),
 // else they gather rows with cp.async.  What lies in rows that nobody sees never matters:
 // their scores are masked, and their V rows are zeroed before PV (0 * NaN is NaN).
@@ -28,12 +28,12 @@ template <int E> struct TcCfg {
     static constexpr int NG = E == 256 ? 1 : 2;     // softmax groups (and O accumulators)
     static constexpr int NP = E / 64;               // 64-column panels
     static constexpr int QPANEL = 128 * 128, KPANEL = KT * 128, QTILE = NP * QPANEL, KTILE = NP * KPANEL;
-    static constexpr int NT = (4 * NG + 4) * 32;    // the last warpgroup: MMA, K, V, Q
+    static constexpr int NT = (4 * NG + 4) * 32;    // the last warpgroup: MMA, K, V, the walk
     // Registers: two softmax warpgroups with a row of 128 scores each do not fit in the 168 of an
     // even share (they spilled, the batched decode took 206 us instead of @); 384 x 168 =
     // 256 x 208 + 128 x 88.  With one softmax warpgroup every thread may have 255.
     static constexpr bool SPLIT_REGS = NG == 2;
-    static constexpr int WARP_MMA = 4 * NG, WARP_K = 4 * NG + 1, WARP_V = 4 * NG + 2, WARP_Q = 4 * NG + 3;
+    static constexpr int WARP_MMA = 4 * NG, WARP_K = 4 * NG + 1, WARP_V = 4 * NG + 2, WARP_WALK = 4 * NG + 3;
     static constexpr int RING = E == 64 ? 4 : 3;    // most stages of a ring
     // tiles of 32 KB (16 KB at E = 64): Q (room for two sets of one tile, so that the next turn's
     // or piece's is there in time; with two tiles at E = 128, and at E = 256, one set), the K
@@ -44,8 +44,9 @@ template <int E> struct TcCfg {
     static constexpr int OFF_K = E == 64 ? 4 * QTILE : E == 256 ? QTILE : 2 * QTILE;
     static constexpr int OFF_V = OFF_K + K_STAGES * KTILE;
     static constexpr int OFF_BAR = OFF_V + VS * KTILE;
-    static constexpr int OFF_MISC = OFF_BAR + 32 * 8;
-    static constexpr int OFF_ML = OFF_MISC + 64;    // [2][128] (maximum, sum)
+    static constexpr int OFF_MISC = OFF_BAR + 48 * 8;
+    static constexpr int OFF_RUN = OFF_MISC + 32;
+    static constexpr int OFF_ML = OFF_RUN + RUN_RING * (int)sizeof(SplitRun);  // [2][128] (maximum, sum)
     static constexpr int SMEM = OFF_ML + 2 * 128 * 8;
     static_assert(SMEM <= 232448, "more shared memory than a CTA may use");
 };
@@ -73,6 +74,8 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
     const uint32_t bar = s0 + C::OFF_BAR;
     const uint32_t k_full = bar, k_empty = bar + 32, v_full = bar + 64, v_empty = bar + 96;
     const uint32_t s_full = bar + 128, p_full = bar + 144, q_full = bar + 160, q_empty = bar + 176, o_done = bar + 192, epi1 = bar + 200, epi2 = bar + 208;
+    const uint32_t run_full = bar + 216, run_empty = run_full + 8 * RUN_RING;
+    SplitRun* runs = reinterpret_cast<SplitRun*>(smem + C::OFF_RUN);
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
     if (tid == 0) {
         for (int s = 0; s < C::RING; ++s) {
@@ -86,6 +89,10 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             mbar_init(p_full + 8 * s, 128);
             mbar_init(q_full + 8 * s, 1);
             mbar_init(q_empty + 8 * s, 1);
+        }
+        for (int s = 0; s < RUN_RING; ++s) {
+            mbar_init(run_full + 8 * s, 1);
+            mbar_init(run_empty + 8 * s, 3 + 4 * NG);  // MMA, K, V, the softmax warps
         }
         mbar_init(o_done, 1);
         mbar_init(epi1, 128 * NG);
@@ -105,13 +112,19 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
-    SplitWalk walk;
-    walk.place(p, lane, g);
-    SplitPiece pc;
-    SplitWin win;
     // a whole warp waits, and gives up as a whole
     auto wait = [&](uint32_t b, int phase) { return __all_sync(0xffffffffu, mbar_wait(b, phase & 1)); };
     auto wait_lazy = [&](uint32_t b, int phase) { return __all_sync(0xffffffffu, mbar_wait_lazy(b, phase & 1)); };
+    // the n-th run, by a whole warp or by the one thread of its role
+    auto take_run = [&](int n, SplitRun& run, bool warp) {
+        const uint32_t f = run_full + 8 * (n % RUN_RING);
+        const bool got = mbar_wait(f, (n / RUN_RING) & 1);
+        if (warp ? !__all_sync(0xffffffffu, got) : !got) return false;
+        run = runs[n % RUN_RING];
+        if (warp) __syncwarp();
+        if (!warp || lane == 0) mbar_arrive(run_empty + 8 * (n % RUN_RING));
+        return true;
+    };
     auto give_up = [&](int bit) {
         if (lane == 0) {
             *s_abort = 1;
@@ -119,6 +132,22 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         }
     };
 
+    // A piece's query tiles, again for each turn (the drafted keys keep the last turn's); by the
+    // K producer.  false: a wait gave up, nothing was requested.
+    auto load_q = [&](const SplitRun& run, int epoch) {
+        const int set = epoch % q_sets;
+        if (epoch >= q_sets && (*s_abort || !wait(q_empty + 8 * set, epoch / q_sets - 1))) return false;
+        if (lane == 0) {
+            mbar_expect_tx(q_full + 8 * set, (uint32_t)q_set_bytes);
+            const int z = ((min(run.f, p.F - 1) * p.W + run.w) * p.Hkv + h) * p.rows + run.t * p.mi;
+            for (int t = 0; t < (two ? 2 : 1); ++t)
+#pragma unroll
+                for (int x = 0; x < C::NP; ++x)
+                    tma_load_3d(s0 + (uint32_t)(set * q_set_bytes + t * C::QTILE + x * C::QPANEL), &maps.q, x * 64, 0, z + 128 * t, q_full + 8 * set);
+        }
+        __syncwarp();
+        return true;
+    };
     if (wid >= C::WARP_MMA) {
         if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if ((wid == C::WARP_K || wid == C::WARP_V) && p.box) {
@@ -135,50 +164,57 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         // the rotated drafted keys were written by the kernel before, with ordinary stores
         asm volatile("fence.proxy.async;" ::: "memory");
         const int boxes = KT / p.box, absent = -2 * p.BS;  // a coordinate that loads zeros
-        int next = 0;  // first token of the lane's box of the next window
-        auto find = [&](int i) {
-            win.seek(p, pc.w, i);
+        SplitRun run;
+        int nr = 0, x = 0, next = 0;  // runs taken, window of the run, first token of the lane's box of that window
+        auto find = [&] {
+            const int k0 = run.k0 + x * KT;
             next = absent;
-            if (win.f == p.F) {
-                next = (pc.w * p.Hkv + h) * p.S + win.k0;
+            if (run.f == p.F) {
+                next = (run.w * p.Hkv + h) * p.S + k0;
             } else if (lane < boxes) {
-                const int l = win.k0 + lane * p.box, pos = win.off + l;
-                if (l + p.box > 0 && l < win.sp) {
-                    const int page = __ldg(p.bt + (size_t)pc.w * p.maxb + pos / p.BS);
+                const int l = k0 + lane * p.box, pos = run.off + l;
+                if (l + p.box > 0 && l < run.sp) {
+                    const int page = __ldg(p.bt + (size_t)run.w * p.maxb + pos / p.BS);
                     if (page >= 0 && page < p.NB) next = page * p.BS + pos % p.BS;
                 }
             }
         };
         const bool stall = is_k && blockIdx.x == 0;  // test hook: this window never lands
-        int iw = 0;
-        bool ok = true;
-        while (ok && walk.next(p, pc)) {
-            win.start(p, pc.w);
-            find(pc.i0);
-            for (int i = pc.i0; i < pc.i1; ++i, ++iw) {
-                const int st = iw % stages;
-                if (iw >= stages && (*s_abort || !wait_lazy(empty + 8 * st, iw / stages - 1))) {
-                    ok = false;
-                    break;
-                }
-                const int z = next;
-                const bool tail = win.f == p.F;
-                if (i + 1 < pc.i1) find(i + 1);
-                if (stall && iw == p.stall_tile) continue;
+        int iw = 0, epoch = 0;
+        bool ok = take_run(nr++, run, true);
+        if (ok && run.n) find();
+        while (ok && run.n) {
+            const int st = iw % stages;
+            if (iw >= stages && (*s_abort || !wait(empty + 8 * st, iw / stages - 1))) {
+                ok = false;
+                break;
+            }
+            const int z = next;
+            const bool tail = run.f == p.F;
+            if (!(stall && iw == p.stall_tile)) {
                 if (lane == 0) mbar_expect_tx(full + 8 * st, (uint32_t)C::KTILE);
                 __syncwarp();
                 const uint32_t dst = ring + (uint32_t)(st * C::KTILE);
                 if (tail ? lane == 0 : lane < boxes)
 #pragma unroll
-                    for (int x = 0; x < C::NP; ++x)
-                        tma_load_3d(dst + (uint32_t)(x * C::KPANEL + lane * p.box * 128), tail ? draft : cache, x * 64, tail ? 0 : h, z, full + 8 * st);
+                    for (int y = 0; y < C::NP; ++y)
+                        tma_load_3d(dst + (uint32_t)(y * C::KPANEL + lane * p.box * 128), tail ? draft : cache, y * 64, tail ? 0 : h, z, full + 8 * st);
             }
+            ++iw;
+            if (is_k && x == 0 && (run.how & RUN_Q_NEW) && !(ok = load_q(run, epoch++))) break;
+            if (++x == run.n) {
+                x = 0;
+                if (!(ok = take_run(nr++, run, true))) break;
+            }
+            if (run.n) find();
         }
         if (!ok) {
             give_up(1);
-            // the windows already requested land before the CTA can exit (bounded waits)
-            for (int x = max(0, iw - stages); x < iw; ++x)
-                if (!(stall && x == p.stall_tile)) mbar_wait(full + 8 * (x % stages), (x / stages) & 1);
+            // the loads already requested land before the CTA can exit (bounded waits)
+            for (int y = max(0, iw - stages); y < iw; ++y)
+                if (!(stall && y == p.stall_tile)) mbar_wait(full + 8 * (y % stages), (y / stages) & 1);
+            if (is_k)
+                for (int y = max(0, epoch - q_sets); y < epoch; ++y) mbar_wait(q_full + 8 * (y % q_sets), (y / q_sets) & 1);
         }
     } else if (wid == C::WARP_K || wid == C::WARP_V) {
         // ============================= gather producers ============================
@@ -190,108 +226,90 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         constexpr int NR = KT / 32;      // rows of a window whose addresses a lane finds
         constexpr int CH = E / 8;        // 16-byte chunks of a row
         constexpr int RPI = 32 / CH;     // rows per copy instruction
-        const T* next[NR];               // rows lane + 32 k of the next window, null: zeros
-        auto find = [&](int i) {
-            win.seek(p, pc.w, i);
+        const T* next[NR];               // rows lane + 32 k of the window to be requested, null: zeros
+        SplitRun run;
+        int nr = 0, x = 0;
+        auto find = [&] {
+            const int k0 = run.k0 + x * KT;
 #pragma unroll
             for (int k = 0; k < NR; ++k) {
-                const int r = lane + 32 * k, l = win.k0 + r;
+                const int l = k0 + lane + 32 * k;
                 next[k] = nullptr;
-                if (r >= win.n) continue;
-                if (win.f == p.F) {
-                    if (__ldcg(p.anc + ((size_t)pc.w * p.S + l) * p.SW + (l >> 5)) >> (l & 31) & 1u)
-                        next[k] = draft + (((size_t)pc.w * p.Hkv + h) * p.S + l) * E;
+                if (l >= run.sp) continue;
+                if (run.f == p.F) {
+                    if (__ldcg(p.anc + ((size_t)run.w * p.S + l) * p.SW + (l >> 5)) >> (l & 31) & 1u)
+                        next[k] = draft + (((size_t)run.w * p.Hkv + h) * p.S + l) * E;
                 } else {
-                    const int pos = win.off + l;
-                    const int page = __ldg(p.bt + (size_t)pc.w * p.maxb + pos / p.BS);
+                    const int pos = run.off + l;
+                    const int page = __ldg(p.bt + (size_t)run.w * p.maxb + pos / p.BS);
                     if (page >= 0 && page < p.NB) next[k] = cache + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E;
                 }
             }
         };
-        int iw = 0, signalled = 0;  // windows requested, windows handed over
-        auto hand_over = [&](int upto) {  // their copies have landed
+        int iw = 0, signalled = 0, epoch = 0;  // windows requested, windows handed over
+        auto hand_over = [&](int upto) {       // their copies have landed
             fence_proxy_async_smem();
             // test hook: CTA 0's K windows from stall_tile on never arrive
             if (is_k && blockIdx.x == 0 && p.stall_tile >= 0) upto = min(upto, p.stall_tile);
             for (; signalled < upto; ++signalled) mbar_arrive(full + 8 * (signalled % stages));
         };
-        bool ok = true;
-        while (ok && walk.next(p, pc)) {
-            win.start(p, pc.w);
-            find(pc.i0);
-            for (int i = pc.i0; i < pc.i1; ++i, ++iw) {
-                const int st = iw % stages;
-                if (iw >= stages) {
-                    const int ph = iw / stages - 1;
-                    if (!__all_sync(0xffffffffu, mbar_try_wait(empty + 8 * st, ph & 1))) {
-                        // about to wait: hand over what is under way first
-                        cp_async_wait<0>();
-                        hand_over(iw);
-                        if (*s_abort || !wait_lazy(empty + 8 * st, ph)) {
-                            ok = false;
-                            break;
-                        }
+        if (is_k) asm volatile("fence.proxy.async;" ::: "memory");  // the queries: ordinary stores of the kernel before
+        bool ok = take_run(nr++, run, true);
+        if (ok && run.n) find();
+        while (ok && run.n) {
+            const int st = iw % stages;
+            if (iw >= stages) {
+                const int ph = iw / stages - 1;
+                if (!__all_sync(0xffffffffu, mbar_try_wait(empty + 8 * st, ph & 1))) {
+                    // about to wait: hand over what is under way first
+                    cp_async_wait<0>();
+                    hand_over(iw);
+                    if (*s_abort || !wait(empty + 8 * st, ph)) {
+                        ok = false;
+                        break;
                     }
                 }
-                const T* row[NR];
-#pragma unroll
-                for (int k = 0; k < NR; ++k) row[k] = next[k];
-                if (i + 1 < pc.i1) find(i + 1);
-                const uint32_t dst = ring + (uint32_t)(st * C::KTILE);
-                const int ch = lane % CH;
-#pragma unroll
-                for (int k = 0; k < NR; ++k) {
-                    const unsigned long long mine = reinterpret_cast<unsigned long long>(row[k]);
-#pragma unroll 4
-                    for (int x = 0; x < CH; ++x) {
-                        const int rl = x * RPI + lane / CH, r = 32 * k + rl;
-                        const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, mine, rl));
-                        cp_async16_zfill(dst + (uint32_t)((ch >> 3) * C::KPANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
-                                         src ? src + ch * 8 : cache, src ? 16 : 0);
-                    }
-                }
-                cp_async_commit();
-                cp_async_wait<1>();
-                hand_over(iw);
             }
+            const uint32_t dst = ring + (uint32_t)(st * C::KTILE);
+            const int ch = lane % CH;
+#pragma unroll
+            for (int k = 0; k < NR; ++k) {
+                const unsigned long long mine = reinterpret_cast<unsigned long long>(next[k]);
+#pragma unroll 4
+                for (int y = 0; y < CH; ++y) {
+                    const int rl = y * RPI + lane / CH, r = 32 * k + rl;
+                    const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, mine, rl));
+                    cp_async16_zfill(dst + (uint32_t)((ch >> 3) * C::KPANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
+                                     src ? src + ch * 8 : cache, src ? 16 : 0);
+                }
+            }
+            cp_async_commit();
+            cp_async_wait<1>();
+            hand_over(iw);
+            ++iw;
+            if (is_k && x == 0 && (run.how & RUN_Q_NEW)) {
+                if (epoch >= q_sets) {  // load_q may wait
+                    cp_async_wait<0>();
+                    hand_over(iw);
+                }
+                if (!(ok = load_q(run, epoch++))) break;
+            }
+            if (++x == run.n) {
+                x = 0;
+                if (!(ok = take_run(nr++, run, true))) break;
+            }
+            if (run.n) find();
         }
         cp_async_wait<0>();
-        if (ok) hand_over(iw);
-        else give_up(1);
-    } else if (wid == C::WARP_Q) {
-        // =================================== Q ====================================
-        // a piece's tiles, again for each turn (the drafted keys keep the last turn's)
-        asm volatile("fence.proxy.async;" ::: "memory");  // written by the kernel before, with ordinary stores
-        int epoch = 0;
-        bool ok = true;
-        while (ok && walk.next(p, pc)) {
-            win.start(p, pc.w);
-            int turn = -1;
-            for (int i = pc.i0; i < pc.i1; i += win.run(pc, i)) {
-                win.seek(p, pc.w, i);
-                const int qt = min(win.f, p.F - 1), set = epoch % q_sets;
-                if (qt == turn) continue;
-                if (epoch >= q_sets && (*s_abort || !wait_lazy(q_empty + 8 * set, epoch / q_sets - 1))) {
-                    ok = false;
-                    break;
-                }
-                if (lane == 0) {
-                    mbar_expect_tx(q_full + 8 * set, (uint32_t)q_set_bytes);
-                    const int z = ((qt * p.W + pc.w) * p.Hkv + h) * p.rows + pc.t * p.mi;
-                    for (int t = 0; t < (two ? 2 : 1); ++t)
-#pragma unroll
-                        for (int x = 0; x < C::NP; ++x)
-                            tma_load_3d(s0 + (uint32_t)(set * q_set_bytes + t * C::QTILE + x * C::QPANEL), &maps.q, x * 64, 0, z + 128 * t, q_full + 8 * set);
-                }
-                __syncwarp();
-                turn = qt;
-                ++epoch;
-            }
-        }
-        if (!ok) {
+        if (ok) {
+            hand_over(iw);
+        } else {
             give_up(1);
-            for (int x = max(0, epoch - q_sets); x < epoch; ++x) mbar_wait(q_full + 8 * (x % q_sets), (x / q_sets) & 1);
+            if (is_k)
+                for (int y = max(0, epoch - q_sets); y < epoch; ++y) mbar_wait(q_full + 8 * (y % q_sets), (y / q_sets) & 1);
         }
+    } else if (wid == C::WARP_WALK) {
+        if (!split_schedule(p, lane, g, runs, run_full, run_empty, [&] { return *s_abort != 0; })) give_up(1);
     } else if (wid == C::WARP_MMA) {
         // =================================== MMA ===================================
         // one thread: its waits, issues and commits are on every job's path
@@ -316,40 +334,34 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                 }
                 return true;
             };
-            while (ok && walk.next(p, pc)) {
-                win.start(p, pc.w);
-                int n = 0, turn = -1;  // jobs of the piece issued, the turn q is rotated for
-                for (int i = pc.i0; ok && i < pc.i1;) {
-                    win.seek(p, pc.w, i);
-                    const int qt = min(win.f, p.F - 1), end = i + win.run(pc, i);
-                    const bool last_of_q = end == pc.i1 || qt != p.F - 1;  // the next run has another q
-                    if (qt != turn) {
-                        if (!mbar_wait(q_full + 8 * qs, qp)) ok = false;
-                        turn = qt;
-                    }
-                    const uint64_t qd = dq0 + (uint64_t)((qs * q_set_bytes) >> 4);
-                    for (; ok && i < end; ++i) {
-                        if (!mbar_wait(k_full + 8 * ks, kp)) ok = false;
-                        for (int t = 0; ok && t < (two ? 2 : 1); ++t, ++j, ++n) {
-                            tc_fence_after();
-                            const uint64_t a0 = qd + (uint64_t)((t * C::QTILE) >> 4), b0 = dk0 + (uint64_t)((ks * C::KTILE) >> 4);
+            SplitRun run;
+            int nr = 0, n = 0;  // runs taken, jobs of the piece issued
+            while ((ok = take_run(nr++, run, false)) && run.n) {
+                if (run.how & RUN_FIRST) n = 0;
+                if ((run.how & RUN_Q_NEW) && !(ok = mbar_wait(q_full + 8 * qs, qp))) break;
+                const uint64_t qd = dq0 + (uint64_t)((qs * q_set_bytes) >> 4);
+                for (int x = 0; ok && x < run.n; ++x) {
+                    if (!(ok = mbar_wait(k_full + 8 * ks, kp))) break;
+                    for (int t = 0; ok && t < (two ? 2 : 1); ++t, ++j, ++n) {
+                        tc_fence_after();
+                        const uint64_t a0 = qd + (uint64_t)((t * C::QTILE) >> 4), b0 = dk0 + (uint64_t)((ks * C::KTILE) >> 4);
 #pragma unroll
-                            for (int kk = 0; kk < E / 16; ++kk)
-                                umma(tmem + KT * (j & 1), a0 + (uint64_t)(((kk >> 2) * C::QPANEL + (kk & 3) * 32) >> 4),
-                                     b0 + (uint64_t)(((kk >> 2) * C::KPANEL + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
-                            umma_commit(s_full + 8 * (j & 1));
-                            if (!two || t == 1) {
-                                umma_commit(k_empty + 8 * ks);
-                                if (last_of_q && i + 1 == end) umma_commit(q_empty + 8 * qs);
-                            }
-                            if (n > 0 && !issue_pv(j - 1, n - 1, !two || t == 0)) ok = false;
+                        for (int kk = 0; kk < E / 16; ++kk)
+                            umma(tmem + KT * (j & 1), a0 + (uint64_t)(((kk >> 2) * C::QPANEL + (kk & 3) * 32) >> 4),
+                                 b0 + (uint64_t)(((kk >> 2) * C::KPANEL + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
+                        umma_commit(s_full + 8 * (j & 1));
+                        if (!two || t == 1) {
+                            umma_commit(k_empty + 8 * ks);
+                            if ((run.how & RUN_Q_END) && x + 1 == run.n) umma_commit(q_empty + 8 * qs);
                         }
-                        if (++ks == C::K_STAGES) ks = 0, kp ^= 1;
+                        if (n > 0) ok = issue_pv(j - 1, n - 1, !two || t == 0);
                     }
-                    if (last_of_q && ++qs == q_sets) qs = 0, qp ^= 1;
+                    if (++ks == C::K_STAGES) ks = 0, kp ^= 1;
                 }
-                if (ok) ok = issue_pv(j - 1, n - 1, true);
-                if (ok) {
+                if (!ok) break;
+                if ((run.how & RUN_Q_END) && ++qs == q_sets) qs = 0, qp ^= 1;
+                if (run.how & RUN_LAST) {
+                    if (!(ok = issue_pv(j - 1, n - 1, true))) break;
                     umma_commit(o_done);
                     ++piece;
                 }
@@ -373,35 +385,27 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         const bool join = NG == 2 && !two;
         float2* sML = reinterpret_cast<float2*>(smem + C::OFF_ML);
         int j = 0, iw = 0, piece = 0;
-        // ---- this thread's row of the piece at hand ----
-        int tok = 0, orow = 0;         // token, output row
+        int tok = 0, orow = 0;          // this thread's row of the piece at hand: token, output row
         bool in = false, live = false;  // it is one; the warp has one
-        auto enter = [&] {
-            const int row = pc.t * p.mi + tile * 128 + r;
-            in = row < p.rows;
-            tok = in ? row / p.G : 0;
-            orow = (pc.w * p.Hq + h * p.G + (in ? row - tok * p.G : 0)) * p.S + tok;
-            live = __any_sync(0xffffffffu, in);
-            win.start(p, pc.w);
-        };
-        // One turn of a piece after the other; a finished piece's result is written once what the
-        // next one needs is on its way.  What the inner loop over the windows does not need is
-        // kept out of it: a row of 128 scores leaves few registers.
+        // One run after the other; a finished piece's result is written once the next run's limit
+        // is on its way.
         float m = neg_inf(), l = 0.f;  // running maximum (log2 units, stepped) and sum
-        int jp = 0, mine = 0, i = 0, lim = 0;
+        int jp = 0, mine = 0, nr = 0, jobs = 0, was_row = 0;
         bool pending = false, whole = false, was_in = false, was_live = false;
-        int was_row = 0, jobs = 0;
         size_t prow = 0;
-        bool have = walk.next(p, pc), ok = true;
-        if (have) {
-            enter();
-            i = pc.i0;
-        }
-        while (have || pending) {
-            if (have) {
-                win.seek(p, pc.w, i);
-                if (in && win.f < p.F) lim = __ldcg(p.lim + ((size_t)win.f * p.W + pc.w) * p.S + tok);
+        SplitRun run;
+        bool ok;
+        while ((ok = take_run(nr++, run, true))) {
+            if (run.how & RUN_FIRST) {
+                const int row = run.t * p.mi + tile * 128 + r;
+                in = row < p.rows;
+                tok = in ? row / p.G : 0;
+                orow = (run.w * p.Hq + h * p.G + (in ? row - tok * p.G : 0)) * p.S + tok;
+                live = __any_sync(0xffffffffu, in);
             }
+            const bool tail = run.f == p.F;
+            int lim = 0;  // keys of the turn that the row sees
+            if (run.n && in && !tail) lim = __ldcg(p.lim + ((size_t)run.f * p.W + run.w) * p.S + tok);
             if (pending) {
                 // ---- the piece's result ----
                 if (!(ok = wait(o_done, piece))) break;
@@ -487,21 +491,18 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                 ++piece;
                 m = neg_inf(), l = 0.f;
                 jp = j, mine = 0;
-                if (!have) break;
             }
-            const bool tail = win.f == p.F;
-            if (!in || tail) lim = 0;
-            // ---- this group's jobs of the turn's windows ----
-            const int nx = win.run(pc, i), k00 = win.k0, sp = win.sp;
-            for (int x0 = join ? (grp - j) & 1 : 0; x0 < nx; x0 += join ? 2 : 1) {
+            if (!run.n) break;
+            // ---- this group's jobs of the run's windows ----
+            for (int x0 = join ? (grp - j) & 1 : 0; x0 < run.n; x0 += join ? 2 : 1) {
                 const int job = two ? j + 2 * x0 + grp : j + x0, b = job & 1;
-                const int k0 = k00 + x0 * KT, n = min(KT, sp - k0);
+                const int k0 = run.k0 + x0 * KT, n = min(KT, run.sp - k0);
                 const uint32_t tS = tmem + lanes + KT * b;
                 // drafted keys: the row's ancestors among them, and whether the thread's V row counts
                 uint32_t anc[KT / 32];
                 bool v_seen = r < n && k0 + r >= 0;
                 if (tail) {
-                    const uint32_t* words = p.anc + (size_t)pc.w * p.S * p.SW;
+                    const uint32_t* words = p.anc + (size_t)run.w * p.S * p.SW;
                     const int key = k0 + r;
 #pragma unroll
                     for (int x = 0; x < KT / 32; ++x) anc[x] = in ? __ldcg(words + (size_t)tok * p.SW + (k0 >> 5) + x) : 0u;
@@ -614,18 +615,12 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                 ++mine;
             }
             if (!ok) break;
-            j += two ? 2 * nx : nx;
-            iw += nx;
-            i += nx;
-            if (i == pc.i1) {
+            j += two ? 2 * run.n : run.n;
+            iw += run.n;
+            if (run.how & RUN_LAST) {
                 pending = true;
-                whole = pc.whole(), was_in = in, was_live = live, was_row = orow, jobs = j - jp;
-                prow = ((size_t)blockIdx.x * 2 + pc.slot()) * p.mi + tile * 128 + r;
-                have = walk.next(p, pc);
-                if (have) {
-                    enter();
-                    i = pc.i0;
-                }
+                whole = run.how & RUN_WHOLE, was_in = in, was_live = live, was_row = orow, jobs = j - jp;
+                prow = ((size_t)blockIdx.x * 2 + (run.how & RUN_BEGIN ? 1 : 0)) * p.mi + tile * 128 + r;
             }
         }
         if (!ok) give_up(8);

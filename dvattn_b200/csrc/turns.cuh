@@ -10,6 +10,7 @@
 // token (contiguous in a page) are read at about the same time.
 #pragma once
 
+#include "tcgen05.cuh"
 #include "decode.cuh"
 
 namespace dvb {
@@ -174,6 +175,57 @@ struct SplitWin {
     // windows from i on that belong to the same turn of the piece
     __device__ __forceinline__ int run(const SplitPiece& pc, int i) const { return min(pc.i1, first + nf) - i; }
 };
+
+// A run: consecutive windows of one turn of a piece.  In the warp-specialised kernels one warp
+// walks the CTA's range and hands the runs to the others through a ring in shared memory, a few
+// ahead, so that none of them keeps the walk's state or waits for its loads.
+struct alignas(16) SplitRun {
+    int w, t, f, off;    // sequence, row tile, turn (F: the tail), the turn's first position
+    int k0, sp, n, how;  // first key of the first window, seen keys, windows (0: the end), RUN_* bits
+};
+constexpr int RUN_FIRST = 1, RUN_LAST = 2;   // of its piece
+constexpr int RUN_WHOLE = 4, RUN_BEGIN = 8;  // the piece is a whole item; it begins one (SplitPiece::slot)
+constexpr int RUN_Q_NEW = 16, RUN_Q_END = 32;  // q rotated for another turn than before; the next run's will be
+constexpr int RUN_RING = 8;
+
+// The walking warp: `full` and `empty` are RUN_RING mbarriers each (one arrival; one per
+// consumer).  false: a wait gave up.
+template <class Stop>
+__device__ __forceinline__ bool split_schedule(const TurnSplit& p, int lane, int g, SplitRun* ring, uint32_t full, uint32_t empty, Stop stopped) {
+    SplitWalk walk;
+    walk.place(p, lane, g);
+    SplitPiece pc;
+    SplitWin win;
+    int n = 0;
+    auto push = [&](const SplitRun& r) {
+        const int s = n % RUN_RING;
+        if (n >= RUN_RING && (stopped() || !__all_sync(0xffffffffu, mbar_wait_lazy(empty + 8 * s, (n / RUN_RING - 1) & 1)))) return false;
+        if (lane == 0) {
+            ring[s] = r;
+            mbar_arrive(full + 8 * s);
+        }
+        __syncwarp();
+        ++n;
+        return true;
+    };
+    while (walk.next(p, pc)) {
+        win.start(p, pc.w);
+        int turn = -1;
+        for (int i = pc.i0; i < pc.i1;) {
+            win.seek(p, pc.w, i);
+            const int nx = win.run(pc, i), qt = min(win.f, p.F - 1);
+            SplitRun r;
+            r.w = pc.w, r.t = pc.t, r.f = win.f, r.off = win.off, r.k0 = win.k0, r.sp = win.sp, r.n = nx;
+            r.how = (i == pc.i0 ? RUN_FIRST : 0) | (i + nx == pc.i1 ? RUN_LAST : 0) | (pc.whole() ? RUN_WHOLE : 0) | (pc.slot() ? RUN_BEGIN : 0) |
+                    (qt != turn ? RUN_Q_NEW : 0) | (i + nx == pc.i1 || qt != p.F - 1 ? RUN_Q_END : 0);
+            if (!push(r)) return false;
+            turn = qt;
+            i += nx;
+        }
+    }
+    SplitRun end{};
+    return push(end);
+}
 
 // One row of E elements rotated by apply_rotary_pos_emb: o[e] = x[e] c[e] - x[e + R/2] s[e],
 // o[e + R/2] = x[e + R/2] c[e] + x[e] s[e] for e < R/2 (the first half of the cos/sin row),
