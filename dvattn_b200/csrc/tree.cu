@@ -28,22 +28,19 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
     extern __shared__ int par[];  // [S] parents, then [S] whether a token is there
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int w = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    int* there = par + p.S;
-    for (int j = tid; j < p.S; j += 256) par[j] = __ldg(p.parents + (size_t)w * p.S + j);
-    __syncthreads();
-    // a token is there if its line of parents, each before its child, ends at -1
-    for (int j = tid; j < p.S; j += 256) {
-        int c = j;
-        while (c >= 0 && par[c] < c && par[c] >= -1) c = par[c];
-        there[j] = c == -1;
-    }
-    __syncthreads();
     if (blockIdx.y == 0) {
-        __shared__ int red[8];
+        __shared__ int part[8];
+        int* there = par + p.S;
         if (w == 0 && tid < 4) p.header[tid] = 0;
+        for (int j = tid; j < p.S; j += 256) par[j] = __ldg(p.parents + (size_t)w * p.S + j);
+        __syncthreads();
+        // a token is there if its line of parents, each before its child, ends at -1
         for (int j = tid; j < p.S; j += 256) {
+            int c = j;
+            while (c >= 0 && par[c] < c && par[c] >= -1) c = par[c];
+            there[j] = c == -1;
             uint32_t* a = p.anc + ((size_t)w * p.S + j) * p.SW;
-            int c = there[j] ? j : -1;
+            c = c == -1 ? j : -1;
             for (int word = p.SW - 1; word >= 0; --word) {
                 uint32_t bits = 0;
                 while (c >= 32 * word) {  // c < 32 * (word + 1) here: parents come before
@@ -54,29 +51,31 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
                 a[word] = bits;
             }
         }
+        __syncthreads();
+        // a warp per turn
         long long off = 0;
-        int nw = 0;
-        for (int f = 0; f < p.F; ++f) {
+        int nw = 0, at = 0;  // `off`: the first position of turn `at`
+        for (int f = wid; f < p.F; f += 8) {
+            for (; at < f; ++at) off += max(__ldg(p.L + at), 0);
             const int Lf = __ldg(p.L + f);
             int v = 0;
-            for (int s = tid; s < p.S; s += 256) {
-                const size_t at = ((size_t)f * p.W + w) * p.S + s;
-                const int n = there[s] ? turn_seen(Lf, __ldg(p.loc + at), off, p.cap) : 0;
-                p.lim[at] = n;
+            for (int s = lane; s < p.S; s += 32) {
+                const size_t x = ((size_t)f * p.W + w) * p.S + s;
+                const int n = there[s] ? turn_seen(Lf, __ldg(p.loc + x), off, p.cap) : 0;
+                p.lim[x] = n;
                 v = max(v, n);
             }
             v = __reduce_max_sync(0xffffffffu, v);
-            if (lane == 0) red[wid] = v;
-            __syncthreads();
-            v = 0;
-            for (int x = 0; x < 8; ++x) v = max(v, red[x]);
-            __syncthreads();
             const int first = v > 0 ? (int)off : 0;  // below cap where a key is seen
-            if (tid == 0) p.span[(size_t)w * p.F + f] = make_int2(v, first);
+            if (lane == 0) p.span[(size_t)w * p.F + f] = make_int2(v, first);
             nw += turn_windows(p, v, first);
-            off += Lf > 0 ? Lf : 0;
         }
-        if (tid == 0) p.nwin[w] = nw + (p.S + p.kt - 1) / p.kt;
+        if (lane == 0) part[wid] = nw;
+        __syncthreads();
+        if (tid == 0) {
+            for (int x = 1; x < 8; ++x) nw += part[x];
+            p.nwin[w] = nw + (p.S + p.kt - 1) / p.kt;
+        }
         return;
     }
     // rows: the drafted keys [Hkv][S], then the queries [F][Hkv][rows]
@@ -98,11 +97,7 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
             dst = static_cast<T*>(p.qr) + ((((size_t)f * p.W + w) * p.Hkv + h) * p.rows + r) * E;
         }
         const size_t cs = (((size_t)f * p.W + w) * p.S + s) * p.R;
-        if (there[s]) {
-            rotate_row<T>(src, dst, p.cos + cs, p.sin + cs, E, p.R, p.rot_vec, lane % lanes, lanes);
-        } else {
-            for (int c = lane % lanes; c < E * (int)sizeof(T) / 16; c += lanes) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0u, 0u, 0u, 0u);
-        }
+        rotate_row<T>(src, dst, p.cos + cs, p.sin + cs, E, p.R, p.rot_vec, lane % lanes, lanes);
     }
 }
 
@@ -148,8 +143,8 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
     uint8_t* sV = sK + 2 * KT * ROW;                                   // [2][KT] rows
     float* sP = reinterpret_cast<float*>(sV + 2 * KT * ROW);           // [MI][KT + 4]
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // see tree_tc_kernel
     const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
     SplitWalk walk;
     walk.place(p, lane, g);
@@ -296,30 +291,18 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
 
 // ---- merge ----------------------------------------------------------------------------
 // Rows of items that more than one group worked on: the log-sum-exp combination of their
-// partials, in group order.  E / 4 lanes per row; up to a segment of lanes at a time look at
-// the partials' sums, one each, then all partials' columns are read with their loads in
-// flight.  A call whose error word is set gets NaN in every output.
+// partials, in group order.  E / 4 lanes per row, two rows each.  Everything but the partials
+// is known before the attention kernel ends (the prep kernel has ended when this one is
+// launched); after the wait the sums and columns of up to kMergeAhead partials are read in one
+// round trip.  A call whose error word is set gets NaN in every output.
+constexpr int kMergeAhead = 4;
+
 template <class T, int E>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
-    constexpr int TPR = E / 4, RPB = 256 / TPR;     // threads per row, rows per block
-    constexpr int SEG = TPR < 32 ? TPR : 32;        // lanes that work on one row together
-    const int tid = threadIdx.x, lane = tid & 31, sl = tid % SEG;
+    constexpr int TPR = E / 4, RPB = 256 / TPR;  // threads per row, rows per block
+    const int tid = threadIdx.x, lane = tid & 31;
     const int item = blockIdx.x, h = item % p.Hkv, t = item / p.Hkv % p.nt, w = item / p.Hkv / p.nt;
-    const int i = blockIdx.y * RPB + tid / TPR, e = tid % TPR * 4;
-    const int r = t * p.mi + i;
-    const bool row_ok = i < p.mi && r < p.S * p.G;
-    const int s = row_ok ? r / p.G : 0, hq = h * p.G + (row_ok ? r - s * p.G : 0);
-    const size_t orow = ((size_t)w * p.Hq + hq) * p.S + s;
-    T* op = static_cast<T*>(p.out) + orow * E + e;
     const float nan = __int_as_float(0x7fc00000);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (__ldcg(p.header + 3) != 0) {
-        if (row_ok) {
-            store_quad<T>(op, nan, nan, nan, nan);
-            if (p.lse_out && e == 0) p.lse_out[orow] = nan;
-        }
-        return;
-    }
     // the groups that hold the item's first and last window
     long long total = 0, before = 0;
     for (int x = lane; x < p.W; x += 32) {
@@ -336,40 +319,60 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
     const SplitRange range(total * p.nt, p.groups);
     const long long us = before * p.nt + (long long)t * nw;
     const int g0 = range.group_of(us), g1 = range.group_of(us + nw - 1);
-    if (g0 == g1) return;
-    auto slot_of = [&](int g) { return (((size_t)g * p.Hkv + h) * 2 + (g == g0 ? 1 : 0)) * p.mi + (row_ok ? i : 0); };
-    float m = neg_inf(), den = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int gb = g0; gb <= g1; gb += SEG) {
-        const int n = min(SEG, g1 - gb + 1);
-        const float x = sl < n ? __ldcg(p.part_lse + slot_of(gb + sl)) : neg_inf();
-        float mx = x;
-        bool bad = x != x;  // fmaxf drops a NaN, the result must not
+    const int e = tid % TPR * 4;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const bool failed = __ldcg(p.header + 3) != 0;
+    if (g0 == g1 && !failed) return;
+    for (int i = blockIdx.y * RPB + tid / TPR; i < p.mi; i += gridDim.y * RPB) {
+        const int r = t * p.mi + i;
+        if (r >= p.rows) break;
+        const int s = r / p.G, hq = h * p.G + r - s * p.G;
+        const size_t orow = ((size_t)w * p.Hq + hq) * p.S + s;
+        T* op = static_cast<T*>(p.out) + orow * E + e;
+        if (failed) {
+            store_quad<T>(op, nan, nan, nan, nan);
+            if (p.lse_out && e == 0) p.lse_out[orow] = nan;
+            continue;
+        }
+        float m = neg_inf(), den = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int g = g0; g <= g1; g += kMergeAhead) {
+            float x[kMergeAhead];
+            float4 v[kMergeAhead];
 #pragma unroll
-        for (int o = SEG / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        mx = fmaxf(mx, m);
-        const float mu = mx == neg_inf() ? 0.f : mx;
-        const float wgt = bad ? nan : fast_exp2(x - mu), alpha = fast_exp2(m - mu);
-        m = mx;
-        den *= alpha;
+            for (int k = 0; k < kMergeAhead; ++k) {
+                const int gg = min(g + k, g1);
+                const size_t at = (((size_t)gg * p.Hkv + h) * 2 + (gg == g0 ? 1 : 0)) * p.mi + i;
+                x[k] = __ldcg(p.part_lse + at);
+                v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * E + e));
+                if (g + k > g1) x[k] = neg_inf();
+            }
+            float mx = m;
+            bool bad = false;  // fmaxf drops a NaN, the result must not
 #pragma unroll
-        for (int c = 0; c < 4; ++c) a[c] *= alpha;
-#pragma unroll 8
-        for (int y = 0; y < n; ++y) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot_of(gb + y) * E + e));
-            const float f = __shfl_sync(0xffffffffu, wgt, y, SEG);
-            den += f;
-            if (f != 0.f) {  // an empty part adds nothing
-                a[0] = fmaf(f, v.x, a[0]);
-                a[1] = fmaf(f, v.y, a[1]);
-                a[2] = fmaf(f, v.z, a[2]);
-                a[3] = fmaf(f, v.w, a[3]);
+            for (int k = 0; k < kMergeAhead; ++k) {
+                mx = fmaxf(mx, x[k]);
+                bad |= x[k] != x[k];
+            }
+            const float mu = mx == neg_inf() ? 0.f : mx, alpha = fast_exp2(m - mu);
+            m = mx;
+            den = bad ? nan : den * alpha;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) a[c] *= alpha;
+#pragma unroll
+            for (int k = 0; k < kMergeAhead; ++k) {
+                if (x[k] == neg_inf()) continue;  // an empty part adds nothing
+                const float f = fast_exp2(x[k] - mu);
+                den += f;
+                a[0] = fmaf(f, v[k].x, a[0]);
+                a[1] = fmaf(f, v[k].y, a[1]);
+                a[2] = fmaf(f, v[k].z, a[2]);
+                a[3] = fmaf(f, v[k].w, a[3]);
             }
         }
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        store_quad<T>(op, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+        if (p.lse_out && e == 0) p.lse_out[orow] = den == 0.f ? neg_inf() : (m + log2f(den)) * kLn2;
     }
-    if (!row_ok) return;
-    const float inv = den == 0.f ? 0.f : 1.f / den;
-    store_quad<T>(op, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
-    if (p.lse_out && e == 0) p.lse_out[orow] = den == 0.f ? neg_inf() : (m + log2f(den)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -382,6 +385,7 @@ template <class T, int E> static TreeKernel simt_kernel() {
     k.kt = SimtCfg<T, E>::KT;
     k.mi = SimtCfg<T, E>::MI;
     k.smem = SimtCfg<T, E>::SMEM;
+    k.ctas = E == 256 ? 1 : E == 128 ? 2 : 4;  // by their shared memory: 170, 90, 49 KB
     return k;
 }
 static TreeKernel tree_pick(const dvattn_tree_args* a) {
@@ -419,13 +423,13 @@ struct TreeLayout {
 };
 
 static int tree_layout(const dvattn_tree_args* a, const TreeKernel& k, TreeLayout& L) {
-    int dev = 0, sms = 0, occ = 0;
+    int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return DVATTN_ERR_CUDA;
-    if (cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem) != cudaSuccess) return DVATTN_ERR_CUDA;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k.fn, k.threads, k.smem) != cudaSuccess || occ < 1)
+    if (cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem) != cudaSuccess ||
+        cudaFuncSetAttribute(k.fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
         return DVATTN_ERR_CUDA;
-    L.groups = sms * occ / a->Hkv;
+    L.groups = sms * k.ctas / a->Hkv;
     if (L.groups < 1) L.groups = 1;
     L.sw = (a->S + 127) / 128 * 4;
     L.nt = (int)(((long long)a->S * (a->Hq / a->Hkv) + k.mi - 1) / k.mi);
@@ -527,7 +531,7 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     cudaError_t e = cudaLaunchKernelExC(&cfg, k.fn, args);
     if (e == cudaSuccess) {
         const int rpb = 256 / (a->E / 4), rows_max = L.nt > 1 ? k.mi : a->S * p.G;
-        cfg.gridDim = dim3((unsigned)((long long)a->W * L.nt * a->Hkv), (unsigned)((rows_max + rpb - 1) / rpb));
+        cfg.gridDim = dim3((unsigned)((long long)a->W * L.nt * a->Hkv), (unsigned)((rows_max + 2 * rpb - 1) / (2 * rpb)));
         cfg.blockDim = dim3(256);
         cfg.dynamicSmemBytes = 0;
         e = cudaLaunchKernelExC(&cfg, merge, args);

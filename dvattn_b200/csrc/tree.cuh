@@ -41,7 +41,7 @@ struct TreeParams : TurnSplit {
     uint32_t* anc;    // [W][S][SW] ancestor sets; a token that is not there has an empty one
     int* lim;         // [F][W][S] keys of the turn that the token sees; 0: it is not there
     void* dkr;        // [W][Hkv][S][E] T, drafted keys rotated
-    void* qr;         // [F][W][Hkv][rows][E] T, queries rotated for the turn, zeros where the token is not there
+    void* qr;         // [F][W][Hkv][rows][E] T, queries rotated for the turn
     float* part_o;    // [CTAs][2][mi][E] normalised partial outputs
     float* part_lse;  // [CTAs][2][mi] log2 sums, -inf: nothing seen
 };
@@ -50,6 +50,7 @@ struct TreeParams : TurnSplit {
 struct TreeKernel {
     const void* fn;
     int threads, kt, mi;
+    int ctas;  // per SM
     size_t smem;
 };
 // the 16-bit kernel on the 5th-generation tensor cores (tree_tc.cu), and its tensor maps

@@ -3,12 +3,12 @@
 // A CTA walks a range of key windows (turns.cuh).  Jobs: a job is S = Q K^T of one 128-row
 // query tile and one window, its softmax, and O += P V.  Job j uses score buffer j & 1 of
 // TMEM, and the tensor core issues S(j + 1) before PV(j), so it works for one job while the
-// other's softmax runs.  What job j is depends on the rows of a KV head:
-//   more than 128 rows: two row tiles share every window; j & 1 is the tile;
-//   up to 128 rows:     one tile; the windows alternate between two independent halves, each
-//                       with its own running maximum, sum and O, joined at the end of a piece
-//                       (one tile's chain softmax -> PV -> next S would not keep up with HBM);
-//   head dim 256:       one tile and one O (256 columns); only the score buffers alternate.
+// other's softmax runs.  Two forms, by the rows S * G of a KV head:
+//   more than 128 rows (head dims 64, 128): bound by the softmax-PV-S chain.  Two row tiles
+//     share every 128-key window; j & 1 is the tile, each with its own softmax warpgroup.
+//   up to 128 rows, and head dim 256: bound by HBM.  One tile, 64-key windows, one softmax
+//     warpgroup, half an SM (head dim 256: a whole one): what the beginning and end of a
+//     piece cost one CTA is hidden behind the other's stream.
 // Warps: 4 per softmax group (a thread owns one query row = one TMEM lane), one that walks the
 // range (split_schedule), one MMA issuer, one K (and Q) and one V producer.  Producers fill swizzled rings with TMA boxes where pages and
 // windows are whole numbers of boxes of 8 or more rows (page sizes that are multiples of 8),
@@ -23,32 +23,30 @@
 
 namespace dvb {
 
-template <int E> struct TcCfg {
-    static constexpr int KT = E == 256 ? 64 : 128;  // keys per window
-    static constexpr int NG = E == 256 ? 1 : 2;     // softmax groups (and O accumulators)
+template <int E, bool TWO> struct TcCfg {
+    static constexpr int KT = TWO ? 128 : 64;       // keys per window
+    static constexpr int NG = TWO ? 2 : 1;          // row tiles, softmax warpgroups, O accumulators
+    static constexpr int CTAS = TWO || E == 256 ? 1 : 2;  // per SM
     static constexpr int NP = E / 64;               // 64-column panels
     static constexpr int QPANEL = 128 * 128, KPANEL = KT * 128, QTILE = NP * QPANEL, KTILE = NP * KPANEL;
     static constexpr int NT = (4 * NG + 4) * 32;    // the last warpgroup: MMA, K, V, the walk
-    // Registers: two softmax warpgroups with a row of 128 scores each do not fit in the 168 of an
-    // even share (they spilled, the batched decode took 206 us instead of @); 384 x 168 =
-    // 256 x 208 + 128 x 88.  With one softmax warpgroup every thread may have 255.
-    static constexpr bool SPLIT_REGS = NG == 2;
     static constexpr int WARP_MMA = 4 * NG, WARP_K = 4 * NG + 1, WARP_V = 4 * NG + 2, WARP_WALK = 4 * NG + 3;
-    static constexpr int RING = E == 64 ? 4 : 3;    // most stages of a ring
-    // tiles of 32 KB (16 KB at E = 64): Q (room for two sets of one tile, so that the next turn's
-    // or piece's is there in time; with two tiles at E = 128, and at E = 256, one set), the K
-    // ring, the V ring
-    static constexpr int K_STAGES = E == 64 ? 4 : E == 256 ? 2 : 3;
-    static constexpr int VS = E == 64 ? 4 : E == 256 ? 3 : 2;
-    __host__ __device__ static constexpr int q_sets(bool two) { return E == 64 ? 2 : E == 256 || two ? 1 : 2; }
-    static constexpr int OFF_K = E == 64 ? 4 * QTILE : E == 256 ? QTILE : 2 * QTILE;
-    static constexpr int OFF_V = OFF_K + K_STAGES * KTILE;
-    static constexpr int OFF_BAR = OFF_V + VS * KTILE;
+    // Registers of a softmax thread and of the others, out of an even share of 168 (two tiles,
+    // 384 threads) or 128 (256 threads, two CTAs): 256 * 208 + 128 * 88 = 384 * 168 and
+    // 128 * 168 + 128 * 88 = 256 * 128.  A row of 128 scores does not fit in 168 (the batched
+    // decode took 206 us instead of 139 when it spilled).  0: every thread may have 255.
+    static constexpr int REGS = TWO ? 208 : E == 256 ? 0 : 168;
+    // Shared memory: sets of Q tiles (a second one lets the next turn's or piece's arrive while
+    // the last one is in use), the K ring, the V ring.
+    static constexpr int Q_SETS = E == 64 ? 2 : 1, K_STAGES = E == 64 ? 4 : E == 256 ? 2 : 3, VS = E == 64 ? 4 : E == 256 ? 3 : 2;
+    static constexpr int Q_SET = NG * QTILE;
+    static constexpr int OFF_K = Q_SETS * Q_SET, OFF_V = OFF_K + K_STAGES * KTILE, OFF_BAR = OFF_V + VS * KTILE;
     static constexpr int OFF_MISC = OFF_BAR + 48 * 8;
     static constexpr int OFF_RUN = OFF_MISC + 32;
-    static constexpr int OFF_ML = OFF_RUN + RUN_RING * (int)sizeof(SplitRun);  // [2][128] (maximum, sum)
-    static constexpr int SMEM = OFF_ML + 2 * 128 * 8;
-    static_assert(SMEM <= 232448, "more shared memory than a CTA may use");
+    static constexpr int SMEM = OFF_RUN + RUN_RING * (int)sizeof(SplitRun);
+    static_assert(SMEM <= (CTAS == 2 ? 115712 : 232448), "more shared memory than a CTA may use");
+    // TMEM columns: scores (P over them) at 0 and KT, O
+    static constexpr int COLS = CTAS == 2 ? 256 : 512, TM_O = CTAS == 2 ? 128 : 256;
 };
 
 // 32 bytes in one store (the address a multiple of 32).
@@ -58,27 +56,27 @@ __device__ __forceinline__ void store_sector(void* dst, const uint32_t* v) {
                  : "memory");
 }
 
-template <class T, int E>
-__global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, const __grid_constant__ TreeMaps maps) {
-    using C = TcCfg<E>;
-    constexpr int KT = C::KT, NG = C::NG;
+template <class T, int E, bool TWO>
+__global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_tc_kernel(TreeParams p, const __grid_constant__ TreeMaps maps) {
+    using C = TcCfg<E, TWO>;
+    constexpr int KT = C::KT, NG = C::NG, VS = C::VS;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const uint32_t s0 = smem_u32(smem);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (s0 & 1023) {  // the swizzle's period
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (tid == 0) atomicOr(p.header + 3, 4);
+        return;
+    }
     const bool bf16 = Elem<T>::dtype == DVATTN_BFLOAT16;
-    const bool two = p.mi == 256;
-    constexpr int VS = C::VS;
-    constexpr uint32_t off_k = C::OFF_K, off_v = C::OFF_V;
-    const int q_sets = C::q_sets(two), q_set_bytes = two ? 2 * C::QTILE : C::QTILE;
     const uint32_t bar = s0 + C::OFF_BAR;
     const uint32_t k_full = bar, k_empty = bar + 32, v_full = bar + 64, v_empty = bar + 96;
-    const uint32_t s_full = bar + 128, p_full = bar + 144, q_full = bar + 160, q_empty = bar + 176, o_done = bar + 192, epi1 = bar + 200, epi2 = bar + 208;
-    const uint32_t run_full = bar + 216, run_empty = run_full + 8 * RUN_RING;
+    const uint32_t s_full = bar + 128, p_full = bar + 144, q_full = bar + 160, q_empty = bar + 176, o_done = bar + 192;
+    const uint32_t run_full = bar + 200, run_empty = run_full + 8 * RUN_RING;
     SplitRun* runs = reinterpret_cast<SplitRun*>(smem + C::OFF_RUN);
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
     if (tid == 0) {
-        for (int s = 0; s < C::RING; ++s) {
+        for (int s = 0; s < 4; ++s) {
             mbar_init(k_full + 8 * s, p.box ? 1 : 32);
             mbar_init(k_empty + 8 * s, 1);
             mbar_init(v_full + 8 * s, p.box ? 1 : 32);
@@ -95,14 +93,11 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             mbar_init(run_empty + 8 * s, 3 + 4 * NG);  // MMA, K, V, the softmax warps
         }
         mbar_init(o_done, 1);
-        mbar_init(epi1, 128 * NG);
-        mbar_init(epi2, 128 * NG);
         *s_abort = 0;
         fence_mbar_init();
     }
-    // TMEM columns: scores (P over them) at 0 and KT, O at 256 and 384
     if (wid == C::WARP_MMA) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(s0 + C::OFF_MISC) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s0 + C::OFF_MISC), "n"(C::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -110,19 +105,18 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + C::OFF_MISC);
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    // the merge may be launched now: it reads the prep kernel's results without waiting
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int g = blockIdx.x / p.Hkv, h = blockIdx.x - g * p.Hkv;
     // a whole warp waits, and gives up as a whole
     auto wait = [&](uint32_t b, int phase) { return __all_sync(0xffffffffu, mbar_wait(b, phase & 1)); };
     auto wait_lazy = [&](uint32_t b, int phase) { return __all_sync(0xffffffffu, mbar_wait_lazy(b, phase & 1)); };
-    // the n-th run, by a whole warp or by the one thread of its role
-    auto take_run = [&](int n, SplitRun& run, bool warp) {
-        const uint32_t f = run_full + 8 * (n % RUN_RING);
-        const bool got = mbar_wait(f, (n / RUN_RING) & 1);
-        if (warp ? !__all_sync(0xffffffffu, got) : !got) return false;
+    auto take_run = [&](int n, SplitRun& run) {  // the n-th run, by a whole warp
+        if (!wait(run_full + 8 * (n % RUN_RING), n / RUN_RING)) return false;
         run = runs[n % RUN_RING];
-        if (warp) __syncwarp();
-        if (!warp || lane == 0) mbar_arrive(run_empty + 8 * (n % RUN_RING));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(run_empty + 8 * (n % RUN_RING));
         return true;
     };
     auto give_up = [&](int bit) {
@@ -135,26 +129,26 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
     // A piece's query tiles, again for each turn (the drafted keys keep the last turn's); by the
     // K producer.  false: a wait gave up, nothing was requested.
     auto load_q = [&](const SplitRun& run, int epoch) {
-        const int set = epoch % q_sets;
-        if (epoch >= q_sets && (*s_abort || !wait(q_empty + 8 * set, epoch / q_sets - 1))) return false;
+        const int set = epoch % C::Q_SETS;
+        if (epoch >= C::Q_SETS && (*s_abort || !wait(q_empty + 8 * set, epoch / C::Q_SETS - 1))) return false;
         if (lane == 0) {
-            mbar_expect_tx(q_full + 8 * set, (uint32_t)q_set_bytes);
+            mbar_expect_tx(q_full + 8 * set, (uint32_t)C::Q_SET);
             const int z = ((min(run.f, p.F - 1) * p.W + run.w) * p.Hkv + h) * p.rows + run.t * p.mi;
-            for (int t = 0; t < (two ? 2 : 1); ++t)
+            for (int t = 0; t < NG; ++t)
 #pragma unroll
                 for (int x = 0; x < C::NP; ++x)
-                    tma_load_3d(s0 + (uint32_t)(set * q_set_bytes + t * C::QTILE + x * C::QPANEL), &maps.q, x * 64, 0, z + 128 * t, q_full + 8 * set);
+                    tma_load_3d(s0 + (uint32_t)(set * C::Q_SET + t * C::QTILE + x * C::QPANEL), &maps.q, x * 64, 0, z + 128 * t, q_full + 8 * set);
         }
         __syncwarp();
         return true;
     };
     if (wid >= C::WARP_MMA) {
-        if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if constexpr (C::REGS > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if ((wid == C::WARP_K || wid == C::WARP_V) && p.box) {
         // ============================== TMA producers ==============================
         const bool is_k = wid == C::WARP_K;
         const int stages = is_k ? C::K_STAGES : VS;
-        const uint32_t full = is_k ? k_full : v_full, empty = is_k ? k_empty : v_empty, ring = s0 + (is_k ? off_k : off_v);
+        const uint32_t full = is_k ? k_full : v_full, empty = is_k ? k_empty : v_empty, ring = s0 + (is_k ? C::OFF_K : C::OFF_V);
         const CUtensorMap* cache = is_k ? &maps.k : &maps.v;
         const CUtensorMap* draft = is_k ? &maps.dk : &maps.dv;
         if (lane == 0) {
@@ -181,7 +175,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         };
         const bool stall = is_k && blockIdx.x == 0;  // test hook: this window never lands
         int iw = 0, epoch = 0;
-        bool ok = take_run(nr++, run, true);
+        bool ok = take_run(nr++, run);
         if (ok && run.n) find();
         while (ok && run.n) {
             const int st = iw % stages;
@@ -204,7 +198,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             if (is_k && x == 0 && (run.how & RUN_Q_NEW) && !(ok = load_q(run, epoch++))) break;
             if (++x == run.n) {
                 x = 0;
-                if (!(ok = take_run(nr++, run, true))) break;
+                if (!(ok = take_run(nr++, run))) break;
             }
             if (run.n) find();
         }
@@ -214,13 +208,13 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             for (int y = max(0, iw - stages); y < iw; ++y)
                 if (!(stall && y == p.stall_tile)) mbar_wait(full + 8 * (y % stages), (y / stages) & 1);
             if (is_k)
-                for (int y = max(0, epoch - q_sets); y < epoch; ++y) mbar_wait(q_full + 8 * (y % q_sets), (y / q_sets) & 1);
+                for (int y = max(0, epoch - C::Q_SETS); y < epoch; ++y) mbar_wait(q_full + 8 * (y % C::Q_SETS), (y / C::Q_SETS) & 1);
         }
     } else if (wid == C::WARP_K || wid == C::WARP_V) {
         // ============================= gather producers ============================
         const bool is_k = wid == C::WARP_K;
         const int stages = is_k ? C::K_STAGES : VS;
-        const uint32_t full = is_k ? k_full : v_full, empty = is_k ? k_empty : v_empty, ring = s0 + (is_k ? off_k : off_v);
+        const uint32_t full = is_k ? k_full : v_full, empty = is_k ? k_empty : v_empty, ring = s0 + (is_k ? C::OFF_K : C::OFF_V);
         const T* cache = static_cast<const T*>(is_k ? p.k : p.v);
         const T* draft = static_cast<const T*>(is_k ? p.dkr : p.dv);
         constexpr int NR = KT / 32;      // rows of a window whose addresses a lane finds
@@ -254,7 +248,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             for (; signalled < upto; ++signalled) mbar_arrive(full + 8 * (signalled % stages));
         };
         if (is_k) asm volatile("fence.proxy.async;" ::: "memory");  // the queries: ordinary stores of the kernel before
-        bool ok = take_run(nr++, run, true);
+        bool ok = take_run(nr++, run);
         if (ok && run.n) find();
         while (ok && run.n) {
             const int st = iw % stages;
@@ -288,7 +282,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             hand_over(iw);
             ++iw;
             if (is_k && x == 0 && (run.how & RUN_Q_NEW)) {
-                if (epoch >= q_sets) {  // load_q may wait
+                if (epoch >= C::Q_SETS) {  // load_q may wait
                     cp_async_wait<0>();
                     hand_over(iw);
                 }
@@ -296,7 +290,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
             }
             if (++x == run.n) {
                 x = 0;
-                if (!(ok = take_run(nr++, run, true))) break;
+                if (!(ok = take_run(nr++, run))) break;
             }
             if (run.n) find();
         }
@@ -306,98 +300,94 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
         } else {
             give_up(1);
             if (is_k)
-                for (int y = max(0, epoch - q_sets); y < epoch; ++y) mbar_wait(q_full + 8 * (y % q_sets), (y / q_sets) & 1);
+                for (int y = max(0, epoch - C::Q_SETS); y < epoch; ++y) mbar_wait(q_full + 8 * (y % C::Q_SETS), (y / C::Q_SETS) & 1);
         }
     } else if (wid == C::WARP_WALK) {
         if (!split_schedule(p, lane, g, runs, run_full, run_empty, [&] { return *s_abort != 0; })) give_up(1);
     } else if (wid == C::WARP_MMA) {
         // =================================== MMA ===================================
-        // one thread: its waits, issues and commits are on every job's path
+        // (the whole warp converged: umma_warp)
         const uint32_t id_s = idesc(bf16, 128, KT, false), id_o = idesc(bf16, 128, E, true);
-        const uint64_t dq0 = sdesc(s0, 16, 1024), dk0 = sdesc(s0 + off_k, 16, 1024), dv0 = sdesc(s0 + off_v, C::KPANEL, 1024);
-        if (lane == 0) {
+        const uint64_t dq0 = sdesc(s0, 16, 1024), dk0 = sdesc(s0 + C::OFF_K, 16, 1024), dv0 = sdesc(s0 + C::OFF_V, C::KPANEL, 1024);
+        {
             int j = 0, ks = 0, kp = 0, vs = 0, vp = 0, qs = 0, qp = 0, piece = 0;
             bool ok = true;
             // PV of job jj, the n-th of its piece, over the V window at hand; `last`: its last use
             auto issue_pv = [&](int jj, int n, bool last) {
                 const int b = jj & 1;
-                if (!mbar_wait(v_full + 8 * vs, vp) || !mbar_wait(p_full + 8 * b, (jj >> 1) & 1)) return false;
+                if (!wait(v_full + 8 * vs, vp) || !wait(p_full + 8 * b, jj >> 1)) return false;
                 tc_fence_after();
                 const uint64_t b0 = dv0 + (uint64_t)((vs * C::KTILE) >> 4);
-                const uint32_t d = tmem + 256 + (NG == 2 ? 128 * b : 0), a = tmem + KT * b;
+                const uint32_t d = tmem + C::TM_O + (TWO ? 128 * b : 0), a = tmem + KT * b;
                 const uint32_t acc = n >= NG;  // the first PV of an O in a piece overwrites it
 #pragma unroll
-                for (int kk = 0; kk < KT / 16; ++kk) umma_ts(d, a + 8 * kk, b0 + (uint64_t)((kk * 16 * 128) >> 4), id_o, kk > 0 ? 1u : acc);
+                for (int kk = 0; kk < KT / 16; ++kk) umma_ts_warp(d, a + 8 * kk, b0 + (uint64_t)((kk * 16 * 128) >> 4), id_o, kk > 0 ? 1u : acc);
                 if (last) {
-                    umma_commit(v_empty + 8 * vs);
+                    umma_commit_warp(v_empty + 8 * vs);
                     if (++vs == VS) vs = 0, vp ^= 1;
                 }
                 return true;
             };
             SplitRun run;
             int nr = 0, n = 0;  // runs taken, jobs of the piece issued
-            while ((ok = take_run(nr++, run, false)) && run.n) {
+            while ((ok = take_run(nr++, run)) && run.n) {
                 if (run.how & RUN_FIRST) n = 0;
-                if ((run.how & RUN_Q_NEW) && !(ok = mbar_wait(q_full + 8 * qs, qp))) break;
-                const uint64_t qd = dq0 + (uint64_t)((qs * q_set_bytes) >> 4);
+                if ((run.how & RUN_Q_NEW) && !(ok = wait(q_full + 8 * qs, qp))) break;
+                const uint64_t qd = dq0 + (uint64_t)((qs * C::Q_SET) >> 4);
                 for (int x = 0; ok && x < run.n; ++x) {
-                    if (!(ok = mbar_wait(k_full + 8 * ks, kp))) break;
-                    for (int t = 0; ok && t < (two ? 2 : 1); ++t, ++j, ++n) {
+                    if (!(ok = wait(k_full + 8 * ks, kp))) break;
+                    for (int t = 0; ok && t < NG; ++t, ++j, ++n) {
                         tc_fence_after();
                         const uint64_t a0 = qd + (uint64_t)((t * C::QTILE) >> 4), b0 = dk0 + (uint64_t)((ks * C::KTILE) >> 4);
 #pragma unroll
                         for (int kk = 0; kk < E / 16; ++kk)
-                            umma(tmem + KT * (j & 1), a0 + (uint64_t)(((kk >> 2) * C::QPANEL + (kk & 3) * 32) >> 4),
+                            umma_warp(tmem + KT * (j & 1), a0 + (uint64_t)(((kk >> 2) * C::QPANEL + (kk & 3) * 32) >> 4),
                                  b0 + (uint64_t)(((kk >> 2) * C::KPANEL + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
-                        umma_commit(s_full + 8 * (j & 1));
-                        if (!two || t == 1) {
-                            umma_commit(k_empty + 8 * ks);
-                            if ((run.how & RUN_Q_END) && x + 1 == run.n) umma_commit(q_empty + 8 * qs);
+                        umma_commit_warp(s_full + 8 * (j & 1));
+                        if (t == NG - 1) {
+                            umma_commit_warp(k_empty + 8 * ks);
+                            if ((run.how & RUN_Q_END) && x + 1 == run.n) umma_commit_warp(q_empty + 8 * qs);
                         }
-                        if (n > 0) ok = issue_pv(j - 1, n - 1, !two || t == 0);
+                        if (n > 0) ok = issue_pv(j - 1, n - 1, !TWO || t == 0);
                     }
                     if (++ks == C::K_STAGES) ks = 0, kp ^= 1;
                 }
                 if (!ok) break;
-                if ((run.how & RUN_Q_END) && ++qs == q_sets) qs = 0, qp ^= 1;
+                if ((run.how & RUN_Q_END) && ++qs == C::Q_SETS) qs = 0, qp ^= 1;
                 if (run.how & RUN_LAST) {
                     if (!(ok = issue_pv(j - 1, n - 1, true))) break;
-                    umma_commit(o_done);
+                    umma_commit_warp(o_done);
                     ++piece;
                 }
             }
             if (!ok) {
                 give_up(2);
                 // all issued MMAs have completed before TMEM is released
-                umma_commit(o_done);
+                umma_commit_warp(o_done);
                 mbar_wait(o_done, piece & 1);
             }
         }
-        __syncwarp();
     }
     } else {
         // ================================= softmax =================================
-        if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        if constexpr (C::REGS > 0) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS));
         const int grp = wid >> 2, r = (wid & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((wid & 3) * 32) << 16;
-        const uint32_t tO = tmem + lanes + 256 + 128 * grp;
-        const int tile = two ? grp : 0;  // the query tile this thread's row lies in
-        const bool join = NG == 2 && !two;
-        float2* sML = reinterpret_cast<float2*>(smem + C::OFF_ML);
+        const uint32_t tO = tmem + lanes + C::TM_O + 128 * grp;
         int j = 0, iw = 0, piece = 0;
         int tok = 0, orow = 0;          // this thread's row of the piece at hand: token, output row
         bool in = false, live = false;  // it is one; the warp has one
         // One run after the other; a finished piece's result is written once the next run's limit
         // is on its way.
         float m = neg_inf(), l = 0.f;  // running maximum (log2 units, stepped) and sum
-        int jp = 0, mine = 0, nr = 0, jobs = 0, was_row = 0;
+        int mine = 0, nr = 0, was_row = 0;  // jobs of the piece done, runs taken
         bool pending = false, whole = false, was_in = false, was_live = false;
         size_t prow = 0;
         SplitRun run;
         bool ok;
-        while ((ok = take_run(nr++, run, true))) {
+        while ((ok = take_run(nr++, run))) {
             if (run.how & RUN_FIRST) {
-                const int row = run.t * p.mi + tile * 128 + r;
+                const int row = run.t * p.mi + grp * 128 + r;
                 in = row < p.rows;
                 tok = in ? row / p.G : 0;
                 orow = (run.w * p.Hq + h * p.G + (in ? row - tok * p.G : 0)) * p.S + tok;
@@ -410,46 +400,17 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                 // ---- the piece's result ----
                 if (!(ok = wait(o_done, piece))) break;
                 tc_fence_after();
-                float w0 = 1.f, w1 = 0.f;
-                bool other = false;  // O of the other group has jobs in it
-                if (join) {
-                    sML[grp * 128 + r] = make_float2(m, l);
-                    mbar_arrive(epi1);
-                    if (!(ok = wait(epi1, piece))) break;
-                    const float2 a = sML[r], b = sML[128 + r];
-                    m = fmaxf(a.x, b.x);
-                    const float mu = m == neg_inf() ? 0.f : m;
-                    w0 = a.x == neg_inf() && a.y == 0.f ? 0.f : ex2(a.x - mu);
-                    w1 = b.x == neg_inf() && b.y == 0.f ? 0.f : ex2(b.x - mu);
-                    l = a.y * w0 + b.y * w1;
-                    // first the accumulator of the piece's first job, which always has one
-                    other = jobs > 1;
-                    if (jp & 1) {
-                        const float x = w0;
-                        w0 = w1, w1 = x;
-                    }
-                }
                 const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
                 const float lse2 = l == 0.f ? neg_inf() : m + log2f(l);
-                const uint32_t ta = join ? tmem + lanes + 256 + 128 * (jp & 1) : tO, tb = tmem + lanes + 256 + 128 * (~jp & 1);
-                const int cb = join ? grp * (E / 64) : 0, ce = join ? cb + E / 64 : E / 32;  // this thread's 32-column blocks
 #pragma unroll 1
-                for (int c = cb; c < ce; ++c) {
+                for (int c = 0; c < E / 32; ++c) {
                     float ov[32];
                     if (was_live) {
-                        tmem_ld32(ta + 32 * c, ov);
+                        tmem_ld32(tO + 32 * c, ov);
                         tmem_wait_ld();
                         reg_fence<32>(ov);
 #pragma unroll
-                        for (int u = 0; u < 32; ++u) ov[u] *= w0 * inv;
-                        if (other) {
-                            float o2[32];
-                            tmem_ld32(tb + 32 * c, o2);
-                            tmem_wait_ld();
-                            reg_fence<32>(o2);
-#pragma unroll
-                            for (int u = 0; u < 32; ++u) ov[u] += o2[u] * (w1 * inv);
-                        }
+                        for (int u = 0; u < 32; ++u) ov[u] *= inv;
                     }
                     if (l == 0.f)  // a token that is not there, a piece without a key that it sees
 #pragma unroll
@@ -477,25 +438,19 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                         }
                     }
                 }
-                if (was_in && (!join || grp == 0)) {
+                if (was_in) {
                     if (!whole) p.part_lse[prow] = lse2;
                     else if (p.lse_out) p.lse_out[was_row] = lse2 * kLn2;
-                }
-                if (join) {
-                    // both groups have read both accumulators before the next piece's PV writes them
-                    tc_fence_before();
-                    mbar_arrive(epi2);
-                    if (!(ok = wait(epi2, piece))) break;
                 }
                 pending = false;
                 ++piece;
                 m = neg_inf(), l = 0.f;
-                jp = j, mine = 0;
+                mine = 0;
             }
             if (!run.n) break;
             // ---- this group's jobs of the run's windows ----
-            for (int x0 = join ? (grp - j) & 1 : 0; x0 < run.n; x0 += join ? 2 : 1) {
-                const int job = two ? j + 2 * x0 + grp : j + x0, b = job & 1;
+            for (int x0 = 0; x0 < run.n; ++x0) {
+                const int job = j + NG * x0 + grp, b = job & 1;
                 const int k0 = run.k0 + x0 * KT, n = min(KT, run.sp - k0);
                 const uint32_t tS = tmem + lanes + KT * b;
                 // drafted keys: the row's ancestors among them, and whether the thread's V row counts
@@ -574,7 +529,7 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                     l = l * alpha + (a0 + a1);
                     m = mnew;
                     if (mine > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-                        // O holds the PV of this group's earlier jobs.  With two groups they completed
+                        // O holds the PV of this tile's earlier jobs.  With two tiles they completed
                         // before this S was signalled (S(j) is issued after PV(j - 2)); with one, the
                         // last of them is PV(j - 1), whose completion frees its V window.
                         if (NG == 1 && !wait(v_empty + 8 * ((iw + x0 - 1) % VS), (iw + x0 - 1) / VS)) {
@@ -595,14 +550,14 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                     }
                     tmem_wait_st();
                 }
-                if (p.box && (!two || grp == 0) && (tail || k0 < 0 || n < KT)) {
+                if (p.box && grp == 0 && (tail || k0 < 0 || n < KT)) {
                     // V rows of this window that nobody sees: P is 0 there
                     if (!wait(v_full + 8 * ((iw + x0) % VS), (iw + x0) / VS)) {
                         ok = false;
                         break;
                     }
                     if (r < KT && !v_seen) {
-                        uint8_t* v = smem + off_v + ((iw + x0) % VS) * C::KTILE + r * 128;
+                        uint8_t* v = smem + C::OFF_V + ((iw + x0) % VS) * C::KTILE + r * 128;
 #pragma unroll
                         for (int x = 0; x < C::NP; ++x)
 #pragma unroll
@@ -615,12 +570,12 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
                 ++mine;
             }
             if (!ok) break;
-            j += two ? 2 * run.n : run.n;
+            j += NG * run.n;
             iw += run.n;
             if (run.how & RUN_LAST) {
                 pending = true;
-                whole = run.how & RUN_WHOLE, was_in = in, was_live = live, was_row = orow, jobs = j - jp;
-                prow = ((size_t)blockIdx.x * 2 + (run.how & RUN_BEGIN ? 1 : 0)) * p.mi + tile * 128 + r;
+                whole = run.how & RUN_WHOLE, was_in = in, was_live = live, was_row = orow;
+                prow = ((size_t)blockIdx.x * 2 + (run.how & RUN_BEGIN ? 1 : 0)) * p.mi + grp * 128 + r;
             }
         }
         if (!ok) give_up(8);
@@ -628,15 +583,17 @@ __global__ void __launch_bounds__(TcCfg<E>::NT, 1) tree_tc_kernel(TreeParams p, 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (wid == C::WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (wid == C::WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::COLS) : "memory");
 }
 
-template <class T, int E> static TreeKernel tc_kernel(int rows) {
-    // one row tile up to 128 rows and at head dim 256, else two
-    return TreeKernel{(const void*)&tree_tc_kernel<T, E>, TcCfg<E>::NT, TcCfg<E>::KT, rows > 128 && E != 256 ? 256 : 128, TcCfg<E>::SMEM};
+template <class T, int E, bool TWO> static TreeKernel tc_kernel() {
+    using C = TcCfg<E, TWO>;
+    return TreeKernel{(const void*)&tree_tc_kernel<T, E, TWO>, C::NT, C::KT, 128 * C::NG, C::CTAS, (size_t)C::SMEM};
 }
 template <class T> static TreeKernel tc_pick(int E, int rows) {
-    return E == 64 ? tc_kernel<T, 64>(rows) : E == 128 ? tc_kernel<T, 128>(rows) : tc_kernel<T, 256>(rows);
+    if (E == 256) return tc_kernel<T, 256, false>();
+    if (rows > 128) return E == 64 ? tc_kernel<T, 64, true>() : tc_kernel<T, 128, true>();
+    return E == 64 ? tc_kernel<T, 64, false>() : tc_kernel<T, 128, false>();
 }
 TreeKernel tree_tc_pick(int dtype, int E, int rows) {
     return dtype == DVATTN_FLOAT16 ? tc_pick<__half>(E, rows) : tc_pick<__nv_bfloat16>(E, rows);
