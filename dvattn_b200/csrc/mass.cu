@@ -64,16 +64,29 @@ __global__ void __launch_bounds__(128) mass_prep_kernel(MassParams p, int E) {
         }
         if (tid == 0) p.nwin[w] = nw;
     }
-    for (int r = r0 + (tid >> 5); r < r1; r += 4) {  // a warp per row
-        const int s = r / p.G, hq = h * p.G + (r - s * p.G);
-        const size_t qrow = ((size_t)w * p.Hq + hq) * p.S + s;
-        if (f == 0 && (tid & 31) == 0) {
-            const float x = __ldg(p.lse + qrow);
+    if (f == 0)
+        for (int r = r0 + tid; r < r1; r += 128) {
+            const int s = r / p.G;
+            const float x = __ldg(p.lse + ((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s);
             p.lse2[((size_t)w * p.Hkv + h) * p.rows + r] = x == neg_inf() ? -neg_inf() : x * kLog2e;
         }
-        const size_t cs = (((size_t)f * p.W + w) * p.S + s) * p.R;
-        rotate_row<T>(static_cast<const T*>(p.q) + qrow * E, static_cast<T*>(p.qr) + ((((size_t)f * p.W + w) * p.Hkv + h) * p.rows + r) * E,
-                      p.cos + cs, p.sin + cs, E, p.R, p.rot_vec, tid & 31, 32);
+    constexpr int AHEAD = 2;  // chunks a thread has in flight
+    const int per = E * (int)sizeof(T) / 16;
+    for (int c0 = r0 * per + tid; c0 < r1 * per; c0 += 128 * AHEAD) {
+        RotateChunk<T> ch[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int c = c0 + 128 * k;
+            if (c >= r1 * per) break;
+            const int r = c / per, s = r / p.G;
+            const size_t cs = (((size_t)f * p.W + w) * p.S + s) * p.R;
+            ch[k].load(static_cast<const T*>(p.q) + (((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s) * E,
+                       static_cast<T*>(p.qr) + ((((size_t)f * p.W + w) * p.Hkv + h) * p.rows + r) * E, p.cos + cs, p.sin + cs,
+                       (c - r * per) * RotateChunk<T>::PER, p.R, p.rot_vec);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (c0 + 128 * k < r1 * per) ch[k].store(p.R, p.rot_vec);
     }
 }
 

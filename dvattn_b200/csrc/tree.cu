@@ -21,7 +21,7 @@ namespace dvb {
 // CTAs that read them.  Reads and writes (F + 1 parts of Hkv rows) a few percent of a call's
 // bytes; done by the attention kernel's own threads, the rotation stood between two pieces of
 // its work for 5 us and more.
-constexpr int kPrepRows = 32;  // rows of a rotating block
+constexpr int kPrepChunks = 512;  // 16-byte chunks of a rotating block, two a thread
 
 template <class T>
 __global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
@@ -78,10 +78,15 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
         }
         return;
     }
-    // rows: the drafted keys [Hkv][S], then the queries [F][Hkv][rows]
-    const int keys = p.Hkv * p.S, all = keys + p.F * p.Hkv * p.rows, r0 = (blockIdx.y - 1) * kPrepRows;
-    const int lanes = min(32, E * (int)sizeof(T) / 16), per = 32 / lanes;
-    for (int x = r0 + wid * per + lane / lanes; x < min(r0 + kPrepRows, all); x += 8 * per) {
+    // chunks of rows: the drafted keys [Hkv][S], then the queries [F][Hkv][rows]
+    const int keys = p.Hkv * p.S, per = E * (int)sizeof(T) / 16, all = (keys + p.F * p.Hkv * p.rows) * per;
+    const int first = (blockIdx.y - 1) * kPrepChunks;
+    RotateChunk<T> ch[kPrepChunks / 256];
+#pragma unroll
+    for (int k = 0; k < kPrepChunks / 256; ++k) {
+        const int c = first + 256 * k + tid;
+        if (c >= all) break;
+        const int x = c / per, e0 = (c - x * per) * RotateChunk<T>::PER;
         const T* src;
         T* dst;
         int f = p.F - 1, s;
@@ -97,8 +102,11 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
             dst = static_cast<T*>(p.qr) + ((((size_t)f * p.W + w) * p.Hkv + h) * p.rows + r) * E;
         }
         const size_t cs = (((size_t)f * p.W + w) * p.S + s) * p.R;
-        rotate_row<T>(src, dst, p.cos + cs, p.sin + cs, E, p.R, p.rot_vec, lane % lanes, lanes);
+        ch[k].load(src, dst, p.cos + cs, p.sin + cs, e0, p.R, p.rot_vec);
     }
+#pragma unroll
+    for (int k = 0; k < kPrepChunks / 256; ++k)
+        if (first + 256 * k + tid < all) ch[k].store(p.R, p.rot_vec);
 }
 
 // ---- CUDA-core attention --------------------------------------------------------------
@@ -402,6 +410,11 @@ static int tree_stall_hook() {
     return t;
 }
 
+// 16-byte chunks of a sequence's drafted keys and of its queries for every turn.
+static long long tree_prep_chunks(const dvattn_tree_args* a) {
+    return ((long long)a->F * a->Hq + a->Hkv) * a->S * (a->E * (a->dtype == DVATTN_FLOAT32 ? 4 : 2) / 16);
+}
+
 static int tree_validate(const dvattn_tree_args* a) {
     if (!a) return DVATTN_ERR_INVALID_ARGUMENT;
     dvattn_paged_args v{};  // the shape rules of the paged attention
@@ -413,7 +426,7 @@ static int tree_validate(const dvattn_tree_args* a) {
     if (a->S > kTreeMaxTokens) return DVATTN_ERR_UNSUPPORTED;
     // grid limits: sequences are the prep grid's x, row blocks its y; items are the merge grid's x
     const long long rows = (long long)a->S * (a->Hq / a->Hkv);
-    if ((long long)a->F * a->W * a->Hq * a->S > 0x7fffffffLL || ((long long)a->F * a->Hq + a->Hkv) * a->S > 65534LL * kPrepRows || (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
+    if ((long long)a->F * a->W * a->Hq * a->S > 0x7fffffffLL || tree_prep_chunks(a) > 65534LL * kPrepChunks || (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
     return DVATTN_OK;
 }
 
@@ -514,7 +527,8 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
                         : a->dtype == DVATTN_FLOAT16 ? merge_fn<__half>(a->E) : merge_fn<__nv_bfloat16>(a->E);
     int E = a->E;
     void* pargs[] = {&p, &E};
-    if (cudaLaunchKernel(prep, dim3(a->W, 1 + (a->Hkv * a->S + a->F * a->Hq * a->S + kPrepRows - 1) / kPrepRows), dim3(256), pargs,
+    const long long chunks = tree_prep_chunks(a);
+    if (cudaLaunchKernel(prep, dim3(a->W, 1 + (unsigned)((chunks + kPrepChunks - 1) / kPrepChunks)), dim3(256), pargs,
                          2 * sizeof(int) * (size_t)a->S, stream) != cudaSuccess)
         return DVATTN_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};

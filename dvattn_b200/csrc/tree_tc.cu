@@ -173,6 +173,9 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
                 }
             }
         };
+        // keys and values that one row tile reads are read once: they leave L2 first, the partial
+        // results stay for the merge
+        const uint64_t policy = p.nt == 1 ? l2_evict_first() : l2_evict_normal();
         const bool stall = is_k && blockIdx.x == 0;  // test hook: this window never lands
         int iw = 0, epoch = 0;
         bool ok = take_run(nr++, run);
@@ -192,7 +195,8 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
                 if (tail ? lane == 0 : lane < boxes)
 #pragma unroll
                     for (int y = 0; y < C::NP; ++y)
-                        tma_load_3d(dst + (uint32_t)(y * C::KPANEL + lane * p.box * 128), tail ? draft : cache, y * 64, tail ? 0 : h, z, full + 8 * st);
+                        tma_load_3d_hint(dst + (uint32_t)(y * C::KPANEL + lane * p.box * 128), tail ? draft : cache, y * 64, tail ? 0 : h, z,
+                                         full + 8 * st, policy);
             }
             ++iw;
             if (is_k && x == 0 && (run.how & RUN_Q_NEW) && !(ok = load_q(run, epoch++))) break;

@@ -227,49 +227,55 @@ __device__ __forceinline__ bool split_schedule(const TurnSplit& p, int lane, int
     return push(end);
 }
 
-// One row of E elements rotated by apply_rotary_pos_emb: o[e] = x[e] c[e] - x[e + R/2] s[e],
-// o[e + R/2] = x[e + R/2] c[e] + x[e] s[e] for e < R/2 (the first half of the cos/sin row),
-// separate roundings of the products and of the sum, one rounding to T: the bits of the paged
-// append.  `LANES` lanes of a warp work on the row, lane `l` on 16-byte chunks l, l + LANES...
-template <class T>
-__device__ __forceinline__ void rotate_row(const T* x, T* y, const float* cos, const float* sin, int E, int R, bool vec, int l, int lanes) {
-    constexpr int PER = 16 / (int)sizeof(T);
-    const int half = R >> 1;
-    for (int c = l; c < E / PER; c += lanes) {
-        const int e0 = c * PER;
-        alignas(16) T a[PER], b[PER];
-        *reinterpret_cast<uint4*>(a) = __ldg(reinterpret_cast<const uint4*>(x + e0));
-        if (e0 >= R) {
-            *reinterpret_cast<uint4*>(y + e0) = *reinterpret_cast<const uint4*>(a);
-        } else if (vec) {  // rotary halves are whole chunks, cos/sin rows 16-byte aligned
-            const bool lo = e0 < half;
-            const int j = lo ? e0 : e0 - half;
-            *reinterpret_cast<uint4*>(b) = __ldg(reinterpret_cast<const uint4*>(x + (lo ? e0 + half : e0 - half)));
-            float cs[PER], sn[PER];
+// A 16-byte chunk (elements e0...) of a row rotated by apply_rotary_pos_emb: o[e] = x[e] c[e] -
+// x[e + R/2] s[e], o[e + R/2] = x[e + R/2] c[e] + x[e] s[e] for e < R/2 (the first half of the
+// cos/sin row), separate roundings of the products and of the sum, one rounding to T: the bits
+// of the paged append.  load() issues the chunk's reads, store() computes and writes, so that a
+// thread can have several chunks in flight.
+template <class T> struct RotateChunk {
+    static constexpr int PER = 16 / (int)sizeof(T);
+    uint4 a, b;
+    float4 c[PER / 4], s[PER / 4];
+    const T* x;
+    T* y;
+    const float *cos, *sin;
+    int e0;
+    __device__ __forceinline__ void load(const T* x_, T* y_, const float* cos_, const float* sin_, int e0_, int R, bool vec) {
+        x = x_, y = y_, cos = cos_, sin = sin_, e0 = e0_;
+        a = __ldg(reinterpret_cast<const uint4*>(x + e0));
+        if (e0 < R && vec) {  // rotary halves are whole chunks, cos/sin rows 16-byte aligned
+            const int half = R >> 1, j = e0 < half ? e0 : e0 - half;
+            b = __ldg(reinterpret_cast<const uint4*>(x + (e0 < half ? e0 + half : j)));
 #pragma unroll
-            for (int u = 0; u < PER; u += 4) {
-                *reinterpret_cast<float4*>(cs + u) = __ldg(reinterpret_cast<const float4*>(cos + j + u));
-                *reinterpret_cast<float4*>(sn + u) = __ldg(reinterpret_cast<const float4*>(sin + j + u));
+            for (int u = 0; u < PER / 4; ++u) {
+                c[u] = __ldg(reinterpret_cast<const float4*>(cos + j) + u);
+                s[u] = __ldg(reinterpret_cast<const float4*>(sin + j) + u);
             }
-#pragma unroll
-            for (int u = 0; u < PER; ++u) {
-                const float v = Elem<T>::to_f(b[u]);
-                a[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(Elem<T>::to_f(a[u]), cs[u]), __fmul_rn(lo ? -v : v, sn[u])));
-            }
-            *reinterpret_cast<uint4*>(y + e0) = *reinterpret_cast<const uint4*>(a);
-        } else {
-            for (int u = 0; u < PER; ++u) {
-                const int e = e0 + u;
-                if (e < R) {
-                    const int j = e < half ? e : e - half;
-                    const float v = Elem<T>::to_f(e < half ? x[e + half] : x[e - half]);
-                    a[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(Elem<T>::to_f(x[e]), __ldg(cos + j)), __fmul_rn(e < half ? -v : v, __ldg(sin + j))));
-                }
-            }
-            *reinterpret_cast<uint4*>(y + e0) = *reinterpret_cast<const uint4*>(a);
         }
     }
-}
+    __device__ __forceinline__ void store(int R, bool vec) {
+        const int half = R >> 1;
+        alignas(16) T o[PER];
+        *reinterpret_cast<uint4*>(o) = a;
+        if (e0 < R && vec) {
+            const T* bt = reinterpret_cast<const T*>(&b);
+            const float* cf = reinterpret_cast<const float*>(c);
+            const float* sf = reinterpret_cast<const float*>(s);
+#pragma unroll
+            for (int u = 0; u < PER; ++u) {
+                const float v = Elem<T>::to_f(bt[u]);
+                o[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(Elem<T>::to_f(o[u]), cf[u]), __fmul_rn(e0 < half ? -v : v, sf[u])));
+            }
+        } else if (e0 < R) {  // element by element
+            for (int u = 0; u < PER && e0 + u < R; ++u) {
+                const int e = e0 + u, j = e < half ? e : e - half;
+                const float v = Elem<T>::to_f(e < half ? x[e + half] : x[j]);
+                o[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(Elem<T>::to_f(x[e]), __ldg(cos + j)), __fmul_rn(e < half ? -v : v, __ldg(sin + j))));
+            }
+        }
+        *reinterpret_cast<uint4*>(y + e0) = *reinterpret_cast<const uint4*>(o);
+    }
+};
 inline bool rotate_vec(int R, const float* cos, const float* sin) {
     return R % 16 == 0 && !((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15);
 }
