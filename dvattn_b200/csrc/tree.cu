@@ -26,6 +26,7 @@ constexpr int kPrepChunks = 512;  // 16-byte chunks of a rotating block, two a t
 template <class T>
 __global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
     extern __shared__ int par[];  // [S] parents, then [S] whether a token is there
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // a programmatic dependent of whatever is before it
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int w = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     if (blockIdx.y == 0) {
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
 // is known before the attention kernel ends (the prep kernel has ended when this one is
 // launched); after the wait the sums and columns of up to kMergeAhead partials are read in one
 // round trip.  A call whose error word is set gets NaN in every output.
-constexpr int kMergeAhead = 4;
+constexpr int kMergeAhead = 8;
 
 template <class T, int E>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
         before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     const int nw = __ldcg(p.nwin + w);
-    const SplitRange range(total * p.nt, p.groups);
+    const SplitRange range(total * p.nt, p);
     const long long us = before * p.nt + (long long)t * nw;
     const int g0 = range.group_of(us), g1 = range.group_of(us + nw - 1);
     const int e = tid % TPR * 4;
@@ -348,11 +349,14 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
             float4 v[kMergeAhead];
 #pragma unroll
             for (int k = 0; k < kMergeAhead; ++k) {
-                const int gg = min(g + k, g1);
+                const int gg = g + k;
                 const size_t at = (((size_t)gg * p.Hkv + h) * 2 + (gg == g0 ? 1 : 0)) * p.mi + i;
-                x[k] = __ldcg(p.part_lse + at);
-                v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * E + e));
-                if (g + k > g1) x[k] = neg_inf();
+                x[k] = neg_inf();
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (g + k <= g1) {
+                    x[k] = __ldcg(p.part_lse + at);
+                    v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * E + e));
+                }
             }
             float mx = m;
             bool bad = false;  // fmaxf drops a NaN, the result must not
@@ -393,6 +397,7 @@ template <class T, int E> static TreeKernel simt_kernel() {
     k.kt = SimtCfg<T, E>::KT;
     k.mi = SimtCfg<T, E>::MI;
     k.smem = SimtCfg<T, E>::SMEM;
+    k.least = 1;  // 1024 keys, 4 tokens: 29 us, with 2 and 4 windows 33 and 45: a window takes it 4 us
     k.ctas = E == 256 ? 1 : E == 128 ? 2 : 4;  // by their shared memory: 170, 90, 49 KB
     return k;
 }
@@ -501,7 +506,7 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     p.tail = a->S; p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
     const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
     p.cap = a->num_blocks <= 0 ? 0 : cap > 0x7fffffffLL ? 0x7fffffff : (int)cap;
-    p.SW = L.sw; p.kt = k.kt; p.mi = k.mi; p.nt = L.nt; p.groups = L.groups;
+    p.SW = L.sw; p.kt = k.kt; p.mi = k.mi; p.nt = L.nt; p.groups = L.groups; p.least = k.least;
     p.scale_log2 = a->scale * kLog2e;
     p.out = a->out; p.lse_out = a->lse_out; p.q = a->queries; p.cos = a->cosines; p.sin = a->sines;
     p.loc = a->locations; p.L = a->fragment_lengths; p.parents = a->parents;
@@ -528,9 +533,6 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     int E = a->E;
     void* pargs[] = {&p, &E};
     const long long chunks = tree_prep_chunks(a);
-    if (cudaLaunchKernel(prep, dim3(a->W, 1 + (unsigned)((chunks + kPrepChunks - 1) / kPrepChunks)), dim3(256), pargs,
-                         2 * sizeof(int) * (size_t)a->S, stream) != cudaSuccess)
-        return DVATTN_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -538,11 +540,15 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     cfg.stream = stream;
+    cfg.gridDim = dim3(a->W, 1 + (unsigned)((chunks + kPrepChunks - 1) / kPrepChunks));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 2 * sizeof(int) * (size_t)a->S;
+    cudaError_t e = cudaLaunchKernelExC(&cfg, prep, pargs);
     cfg.gridDim = dim3((unsigned)(L.groups * a->Hkv));
     cfg.blockDim = dim3(k.threads);
     cfg.dynamicSmemBytes = k.smem;
     void* args[] = {&p, &maps};  // the CUDA-core and merge kernels take the first only
-    cudaError_t e = cudaLaunchKernelExC(&cfg, k.fn, args);
+    if (e == cudaSuccess) e = cudaLaunchKernelExC(&cfg, k.fn, args);
     if (e == cudaSuccess) {
         const int rpb = 256 / (a->E / 4), rows_max = L.nt > 1 ? k.mi : a->S * p.G;
         cfg.gridDim = dim3((unsigned)((long long)a->W * L.nt * a->Hkv), (unsigned)((rows_max + 2 * rpb - 1) / (2 * rpb)));

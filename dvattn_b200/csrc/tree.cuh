@@ -50,7 +50,8 @@ struct TreeParams : TurnSplit {
 struct TreeKernel {
     const void* fn;
     int threads, kt, mi;
-    int ctas;  // per SM
+    int ctas;   // per SM
+    int least;  // windows a CTA group has at least
     size_t smem;
 };
 // the 16-bit kernel on the 5th-generation tensor cores (tree_tc.cu), and its tensor maps

@@ -20,6 +20,7 @@
 #include "tcgen05.cuh"
 #include "tma_host.cuh"
 #include "tree.cuh"
+#include "windows.cuh"
 
 namespace dvb {
 
@@ -144,166 +145,23 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
     };
     if (wid >= C::WARP_MMA) {
         if constexpr (C::REGS > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if ((wid == C::WARP_K || wid == C::WARP_V) && p.box) {
-        // ============================== TMA producers ==============================
+    if (wid == C::WARP_K || wid == C::WARP_V) {
         const bool is_k = wid == C::WARP_K;
-        const int stages = is_k ? C::K_STAGES : VS;
-        const uint32_t full = is_k ? k_full : v_full, empty = is_k ? k_empty : v_empty, ring = s0 + (is_k ? C::OFF_K : C::OFF_V);
-        const CUtensorMap* cache = is_k ? &maps.k : &maps.v;
-        const CUtensorMap* draft = is_k ? &maps.dk : &maps.dv;
-        if (lane == 0) {
-            prefetch_tmap(cache);
-            prefetch_tmap(draft);
-        }
-        // the rotated drafted keys were written by the kernel before, with ordinary stores
-        asm volatile("fence.proxy.async;" ::: "memory");
-        const int boxes = KT / p.box, absent = -2 * p.BS;  // a coordinate that loads zeros
-        SplitRun run;
-        int nr = 0, x = 0, next = 0;  // runs taken, window of the run, first token of the lane's box of that window
-        auto find = [&] {
-            const int k0 = run.k0 + x * KT;
-            next = absent;
-            if (run.f == p.F) {
-                next = (run.w * p.Hkv + h) * p.S + k0;
-            } else if (lane < boxes) {
-                const int l = k0 + lane * p.box, pos = run.off + l;
-                if (l + p.box > 0 && l < run.sp) {
-                    const int page = __ldg(p.bt + (size_t)run.w * p.maxb + pos / p.BS);
-                    if (page >= 0 && page < p.NB) next = page * p.BS + pos % p.BS;
-                }
-            }
-        };
+        WindowSource src;
+        src.cache = is_k ? p.k : p.v, src.tail = is_k ? p.dkr : p.dv;
+        src.map = is_k ? &maps.k : &maps.v, src.tail_map = is_k ? &maps.dk : &maps.dv;
+        src.h = h, src.Hkv = p.Hkv, src.box = p.box, src.anc = p.anc, src.SW = p.SW;
         // keys and values that one row tile reads are read once: they leave L2 first, the partial
         // results stay for the merge
-        const uint64_t policy = p.nt == 1 ? l2_evict_first() : l2_evict_normal();
-        const bool stall = is_k && blockIdx.x == 0;  // test hook: this window never lands
-        int iw = 0, epoch = 0;
-        bool ok = take_run(nr++, run);
-        if (ok && run.n) find();
-        while (ok && run.n) {
-            const int st = iw % stages;
-            if (iw >= stages && (*s_abort || !wait(empty + 8 * st, iw / stages - 1))) {
-                ok = false;
-                break;
-            }
-            const int z = next;
-            const bool tail = run.f == p.F;
-            if (!(stall && iw == p.stall_tile)) {
-                if (lane == 0) mbar_expect_tx(full + 8 * st, (uint32_t)C::KTILE);
-                __syncwarp();
-                const uint32_t dst = ring + (uint32_t)(st * C::KTILE);
-                if (tail ? lane == 0 : lane < boxes)
-#pragma unroll
-                    for (int y = 0; y < C::NP; ++y)
-                        tma_load_3d_hint(dst + (uint32_t)(y * C::KPANEL + lane * p.box * 128), tail ? draft : cache, y * 64, tail ? 0 : h, z,
-                                         full + 8 * st, policy);
-            }
-            ++iw;
-            if (is_k && x == 0 && (run.how & RUN_Q_NEW) && !(ok = load_q(run, epoch++))) break;
-            if (++x == run.n) {
-                x = 0;
-                if (!(ok = take_run(nr++, run))) break;
-            }
-            if (run.n) find();
-        }
+        src.policy = p.nt == 1 ? l2_evict_first() : l2_evict_normal();
+        src.stall = is_k && blockIdx.x == 0 ? p.stall_tile : -1;
+        int epoch = 0;
+        const bool ok = produce_windows<T, E, KT>(
+            p, src, is_k ? C::K_STAGES : VS, s0 + (is_k ? C::OFF_K : C::OFF_V), is_k ? k_full : v_full, is_k ? k_empty : v_empty, take_run, wait,
+            [&] { return *s_abort != 0; }, [&](const SplitRun& run) { return !is_k || !(run.how & RUN_Q_NEW) || load_q(run, epoch++); });
         if (!ok) {
             give_up(1);
-            // the loads already requested land before the CTA can exit (bounded waits)
-            for (int y = max(0, iw - stages); y < iw; ++y)
-                if (!(stall && y == p.stall_tile)) mbar_wait(full + 8 * (y % stages), (y / stages) & 1);
-            if (is_k)
-                for (int y = max(0, epoch - C::Q_SETS); y < epoch; ++y) mbar_wait(q_full + 8 * (y % C::Q_SETS), (y / C::Q_SETS) & 1);
-        }
-    } else if (wid == C::WARP_K || wid == C::WARP_V) {
-        // ============================= gather producers ============================
-        const bool is_k = wid == C::WARP_K;
-        const int stages = is_k ? C::K_STAGES : VS;
-        const uint32_t full = is_k ? k_full : v_full, empty = is_k ? k_empty : v_empty, ring = s0 + (is_k ? C::OFF_K : C::OFF_V);
-        const T* cache = static_cast<const T*>(is_k ? p.k : p.v);
-        const T* draft = static_cast<const T*>(is_k ? p.dkr : p.dv);
-        constexpr int NR = KT / 32;      // rows of a window whose addresses a lane finds
-        constexpr int CH = E / 8;        // 16-byte chunks of a row
-        constexpr int RPI = 32 / CH;     // rows per copy instruction
-        const T* next[NR];               // rows lane + 32 k of the window to be requested, null: zeros
-        SplitRun run;
-        int nr = 0, x = 0;
-        auto find = [&] {
-            const int k0 = run.k0 + x * KT;
-#pragma unroll
-            for (int k = 0; k < NR; ++k) {
-                const int l = k0 + lane + 32 * k;
-                next[k] = nullptr;
-                if (l >= run.sp) continue;
-                if (run.f == p.F) {
-                    if (__ldcg(p.anc + ((size_t)run.w * p.S + l) * p.SW + (l >> 5)) >> (l & 31) & 1u)
-                        next[k] = draft + (((size_t)run.w * p.Hkv + h) * p.S + l) * E;
-                } else {
-                    const int pos = run.off + l;
-                    const int page = __ldg(p.bt + (size_t)run.w * p.maxb + pos / p.BS);
-                    if (page >= 0 && page < p.NB) next[k] = cache + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E;
-                }
-            }
-        };
-        int iw = 0, signalled = 0, epoch = 0;  // windows requested, windows handed over
-        auto hand_over = [&](int upto) {       // their copies have landed
-            fence_proxy_async_smem();
-            // test hook: CTA 0's K windows from stall_tile on never arrive
-            if (is_k && blockIdx.x == 0 && p.stall_tile >= 0) upto = min(upto, p.stall_tile);
-            for (; signalled < upto; ++signalled) mbar_arrive(full + 8 * (signalled % stages));
-        };
-        if (is_k) asm volatile("fence.proxy.async;" ::: "memory");  // the queries: ordinary stores of the kernel before
-        bool ok = take_run(nr++, run);
-        if (ok && run.n) find();
-        while (ok && run.n) {
-            const int st = iw % stages;
-            if (iw >= stages) {
-                const int ph = iw / stages - 1;
-                if (!__all_sync(0xffffffffu, mbar_try_wait(empty + 8 * st, ph & 1))) {
-                    // about to wait: hand over what is under way first
-                    cp_async_wait<0>();
-                    hand_over(iw);
-                    if (*s_abort || !wait(empty + 8 * st, ph)) {
-                        ok = false;
-                        break;
-                    }
-                }
-            }
-            const uint32_t dst = ring + (uint32_t)(st * C::KTILE);
-            const int ch = lane % CH;
-#pragma unroll
-            for (int k = 0; k < NR; ++k) {
-                const unsigned long long mine = reinterpret_cast<unsigned long long>(next[k]);
-#pragma unroll 4
-                for (int y = 0; y < CH; ++y) {
-                    const int rl = y * RPI + lane / CH, r = 32 * k + rl;
-                    const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, mine, rl));
-                    cp_async16_zfill(dst + (uint32_t)((ch >> 3) * C::KPANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
-                                     src ? src + ch * 8 : cache, src ? 16 : 0);
-                }
-            }
-            cp_async_commit();
-            cp_async_wait<1>();
-            hand_over(iw);
-            ++iw;
-            if (is_k && x == 0 && (run.how & RUN_Q_NEW)) {
-                if (epoch >= C::Q_SETS) {  // load_q may wait
-                    cp_async_wait<0>();
-                    hand_over(iw);
-                }
-                if (!(ok = load_q(run, epoch++))) break;
-            }
-            if (++x == run.n) {
-                x = 0;
-                if (!(ok = take_run(nr++, run))) break;
-            }
-            if (run.n) find();
-        }
-        cp_async_wait<0>();
-        if (ok) {
-            hand_over(iw);
-        } else {
-            give_up(1);
-            if (is_k)
+            if (is_k)  // what load_q requested lands before the CTA can exit, too
                 for (int y = max(0, epoch - C::Q_SETS); y < epoch; ++y) mbar_wait(q_full + 8 * (y % C::Q_SETS), (y / C::Q_SETS) & 1);
         }
     } else if (wid == C::WARP_WALK) {
@@ -592,7 +450,10 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
 
 template <class T, int E, bool TWO> static TreeKernel tc_kernel() {
     using C = TcCfg<E, TWO>;
-    return TreeKernel{(const void*)&tree_tc_kernel<T, E, TWO>, C::NT, C::KT, 128 * C::NG, C::CTAS, (size_t)C::SMEM};
+    // One sequence of 16384 keys, 128 rows: 30 us with at least 8 windows a group, 45 and 49 with 4
+    // and 1 (the merge reads that many more partials); two tiles, 4 x 4096 keys: 43 us with at
+    // least 4, 51 with 8.
+    return TreeKernel{(const void*)&tree_tc_kernel<T, E, TWO>, C::NT, C::KT, 128 * C::NG, C::CTAS, TWO ? 4 : 8, (size_t)C::SMEM};
 }
 template <class T> static TreeKernel tc_pick(int E, int rows) {
     if (E == 256) return tc_kernel<T, 256, false>();

@@ -18,6 +18,7 @@ namespace dvb {
 struct TurnSplit {
     int F, W, BS, maxb, cap, tail;
     int kt, nt, groups;  // keys per window, row tiles per sequence, CTA groups
+    int least;           // windows a group has at least, where there are that many
     int align;           // windows over the cache begin on logical positions that are multiples of it
     long long NB;
     const int* loc;
@@ -41,11 +42,15 @@ __device__ __forceinline__ int turn_windows(const TurnSplit& p, int seen, int of
     return seen > 0 ? ((off & (p.align - 1)) + seen + p.kt - 1) / p.kt : 0;
 }
 
-// The split of `total` windows over the groups: the first total % groups of them take one
-// window more than the others.
+// The split of `total` windows over the groups that get any (every one at least p.least, so that
+// short calls do not fall into more partial results than the merge is quick with): the first
+// total % groups of them take one window more than the others.
 struct SplitRange {
     long long q, r;  // windows of a group, groups with one more
-    __device__ __forceinline__ SplitRange(long long total, int groups) {
+    int groups;
+    __device__ __forceinline__ SplitRange(long long total, const TurnSplit& p) {
+        const long long most = total / p.least;
+        groups = most < p.groups ? (most > 0 ? (int)most : 1) : p.groups;
         if (total <= 0x7fffffffLL) {
             const unsigned t = (unsigned)total, n = (unsigned)groups;
             q = t / n;
@@ -55,7 +60,10 @@ struct SplitRange {
             r = total % groups;
         }
     }
-    __device__ __forceinline__ long long begin(int g) const { return g * q + (g < r ? g : r); }
+    __device__ __forceinline__ long long begin(int g) const {
+        if (g > groups) g = groups;
+        return g * q + (g < r ? g : r);
+    }
     // the group of window u < total; the groups between two windows' are never empty
     __device__ __forceinline__ int group_of(long long u) const {
         const long long more = r * (q + 1);
@@ -91,7 +99,7 @@ struct SplitWalk {
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        const SplitRange range(total * p.nt, p.groups);
+        const SplitRange range(total * p.nt, p);
         u = range.begin(g);
         u1 = range.begin(g + 1);
         base = 0;

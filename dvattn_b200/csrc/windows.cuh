@@ -1,0 +1,167 @@
+// The producer warp of the tensor-core kernels over the paged turns (tree_tc.cu, mass_tc.cu):
+// fills a ring of swizzled [KT rows][E] tiles with the windows of the CTA's runs.
+//
+// Where pages and windows are whole numbers of boxes of 8 or more rows (page sizes that are
+// multiples of 8), by TMA, one box per lane and 64-column panel; a box that holds no seen key
+// loads zeros, other rows that nobody sees load what lies there.  Else rows are gathered with
+// cp.async, and rows that nobody sees are zeros.
+#pragma once
+
+#include "tma_host.cuh"
+#include "turns.cuh"
+
+namespace dvb {
+
+struct WindowSource {
+    const void* cache;            // [NB][BS][Hkv][E]
+    const void* tail;             // [W][Hkv][tail][E], or null where the split has no tail
+    const CUtensorMap* map;
+    const CUtensorMap* tail_map;
+    const uint32_t* anc;          // [W][tail][SW]: a tail row without its own bit is not there
+    int SW, h, Hkv;
+    int box;                      // rows of a TMA box, 0: gathered
+    int stall;                    // test hook: this window never arrives; -1: off
+    uint64_t policy;              // L2
+};
+
+// `take_run(n, run)`, `wait(barrier, phase)`: as a whole warp, false when they give up.
+// `opened(run)` is called once the first window of a run has been requested.  false: a wait gave
+// up; everything that was requested has landed.
+template <class T, int E, int KT, class Take, class Wait, class Stop, class Opened>
+__device__ __forceinline__ bool produce_windows(const TurnSplit& p, const WindowSource& s, int stages, uint32_t ring, uint32_t full, uint32_t empty,
+                                                Take take_run, Wait wait, Stop stopped, Opened opened) {
+    constexpr int NP = E / 64, KPANEL = KT * 128, KTILE = NP * KPANEL;
+    const int lane = threadIdx.x & 31;
+    const int h = s.h, Hkv = s.Hkv;
+    // what the kernel before wrote with ordinary stores is read by TMA
+    asm volatile("fence.proxy.async;" ::: "memory");
+    SplitRun run;
+    int nr = 0, x = 0, iw = 0;  // runs taken, window of the run, windows requested
+    bool ok = take_run(nr++, run);
+    if (s.box) {
+        if (lane == 0) {
+            prefetch_tmap(s.map);
+            if (s.tail) prefetch_tmap(s.tail_map);
+        }
+        const int boxes = KT / s.box, absent = -2 * p.BS;  // a coordinate that loads zeros
+        int next = 0;  // first token of the lane's box of the window to be requested
+        auto find = [&] {
+            const int k0 = run.k0 + x * KT;
+            next = absent;
+            if (run.f == p.F) {
+                next = (run.w * Hkv + h) * p.tail + k0;
+            } else if (lane < boxes) {
+                const int l = k0 + lane * s.box, pos = run.off + l;
+                if (l + s.box > 0 && l < run.sp) {
+                    const int page = __ldg(p.bt + (size_t)run.w * p.maxb + pos / p.BS);
+                    if (page >= 0 && page < p.NB) next = page * p.BS + pos % p.BS;
+                }
+            }
+        };
+        if (ok && run.n) find();
+        while (ok && run.n) {
+            const int st = iw % stages;
+            if (iw >= stages && (stopped() || !wait(empty + 8 * st, iw / stages - 1))) {
+                ok = false;
+                break;
+            }
+            const int z = next;
+            const bool tail = run.f == p.F;
+            if (iw != s.stall) {
+                if (lane == 0) mbar_expect_tx(full + 8 * st, (uint32_t)KTILE);
+                __syncwarp();
+                const uint32_t dst = ring + (uint32_t)(st * KTILE);
+                if (tail ? lane == 0 : lane < boxes)
+#pragma unroll
+                    for (int y = 0; y < NP; ++y)
+                        tma_load_3d_hint(dst + (uint32_t)(y * KPANEL + lane * s.box * 128), tail ? s.tail_map : s.map, y * 64, tail ? 0 : h, z,
+                                         full + 8 * st, s.policy);
+            }
+            ++iw;
+            if (x == 0 && !(ok = opened(run))) break;
+            if (++x == run.n) {
+                x = 0;
+                if (!(ok = take_run(nr++, run))) break;
+            }
+            if (run.n) find();
+        }
+        if (!ok)  // bounded waits
+            for (int y = max(0, iw - stages); y < iw; ++y)
+                if (y != s.stall) mbar_wait(full + 8 * (y % stages), (y / stages) & 1);
+        return ok;
+    }
+    const T* cache = static_cast<const T*>(s.cache);
+    const T* draft = static_cast<const T*>(s.tail);
+    constexpr int NR = KT / 32;  // rows of a window whose addresses a lane finds
+    constexpr int CH = E / 8;    // 16-byte chunks of a row
+    constexpr int RPI = 32 / CH; // rows per copy instruction
+    const T* next[NR];           // rows lane + 32 k of the window to be requested, null: zeros
+    auto find = [&] {
+        const int k0 = run.k0 + x * KT;
+#pragma unroll
+        for (int k = 0; k < NR; ++k) {
+            const int l = k0 + lane + 32 * k;
+            next[k] = nullptr;
+            if (l >= run.sp) continue;
+            if (run.f == p.F) {
+                if (__ldcg(s.anc + ((size_t)run.w * p.tail + l) * s.SW + (l >> 5)) >> (l & 31) & 1u)
+                    next[k] = draft + (((size_t)run.w * Hkv + h) * p.tail + l) * E;
+            } else {
+                const int pos = run.off + l;
+                const int page = __ldg(p.bt + (size_t)run.w * p.maxb + pos / p.BS);
+                if (page >= 0 && page < p.NB) next[k] = cache + (((size_t)page * p.BS + pos % p.BS) * Hkv + h) * E;
+            }
+        }
+    };
+    int signalled = 0;                // windows handed over
+    auto hand_over = [&](int upto) {  // their copies have landed
+        fence_proxy_async_smem();
+        for (; signalled < upto; ++signalled)
+            if (signalled != s.stall) mbar_arrive(full + 8 * (signalled % stages));
+    };
+    if (ok && run.n) find();
+    while (ok && run.n) {
+        const int st = iw % stages;
+        if (iw >= stages && !__all_sync(0xffffffffu, mbar_try_wait(empty + 8 * st, (iw / stages - 1) & 1))) {
+            // about to wait: hand over what is under way first
+            cp_async_wait<0>();
+            hand_over(iw);
+            if (stopped() || !wait(empty + 8 * st, iw / stages - 1)) {
+                ok = false;
+                break;
+            }
+        }
+        const uint32_t dst = ring + (uint32_t)(st * KTILE);
+        const int ch = lane % CH;
+#pragma unroll
+        for (int k = 0; k < NR; ++k) {
+            const unsigned long long mine = reinterpret_cast<unsigned long long>(next[k]);
+#pragma unroll 4
+            for (int y = 0; y < CH; ++y) {
+                const int rl = y * RPI + lane / CH, r = 32 * k + rl;
+                const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, mine, rl));
+                cp_async16_zfill(dst + (uint32_t)((ch >> 3) * KPANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4)), src ? src + ch * 8 : cache,
+                                 src ? 16 : 0);
+            }
+        }
+        cp_async_commit();
+        cp_async_wait<1>();
+        hand_over(iw);
+        ++iw;
+        if (x == 0) {
+            cp_async_wait<0>();  // opened() may wait
+            hand_over(iw);
+            if (!(ok = opened(run))) break;
+        }
+        if (++x == run.n) {
+            x = 0;
+            if (!(ok = take_run(nr++, run))) break;
+        }
+        if (run.n) find();
+    }
+    cp_async_wait<0>();
+    if (ok) hand_over(iw);
+    return ok;
+}
+
+}  // namespace dvb
