@@ -218,6 +218,12 @@ __device__ __forceinline__ void tma_load_3d_hint(uint32_t dst, const void* map, 
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
         : "memory");
 }
+// Untiled bulk copy: both addresses 16-byte aligned, `bytes` a multiple of 16.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, int bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+                 "r"(bar)
+                 : "memory");
+}
 __device__ __forceinline__ void prefetch_tmap(const void* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }

@@ -9,90 +9,100 @@
 //
 // Two launches: mass_prep_kernel (rotated queries of every turn, spans), then the kernel
 // that streams the keys once.
-#include "turns.cuh"
+#include "mass.cuh"
 
 #include <cstdio>
 #include <cstdlib>
 
 namespace dvb {
 
-struct MassParams : TurnSplit {
-    int Hq, Hkv, G, S, R, rows;  // rows = S * G queries of a KV head: row r = (query r / G, head r % G)
-    int rot_vec;                 // rotary halves are whole 16-byte chunks, cos/sin rows 16-byte aligned
-    long long N;                 // positions of a mass row
-    float scale_log2;
-    float* mass;
-    const float* lse;
-    const void* q;
-    const float* cos;
-    const float* sin;
-    const void* k;
-    // workspace
-    int* header;  // [3] error word (kErrorWordOffset)
-    void* qr;     // [F][W][Hkv][rows][E] T, queries rotated for the turn
-    float* lse2;  // [W][Hkv][rows] lse in log2 units; +inf: no weight
-};
-
 // ---- prep: block (w, 16-row tile of a KV head, turn) -----------------------------------
+// The queries rotated for every turn, once for all the CTAs that read them; what each row and
+// every row sees of the turn; the spans.
 constexpr int kPrepRows = 16;
 
 template <class T>
 __global__ void __launch_bounds__(128) mass_prep_kernel(MassParams p, int E) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // a programmatic dependent of whatever is before it
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int tid = threadIdx.x, f = blockIdx.z, w = blockIdx.x;
-    const int tiles = (p.rows + kPrepRows - 1) / kPrepRows;
-    const int h = blockIdx.y / tiles, r0 = (blockIdx.y - h * tiles) * kPrepRows, r1 = min(r0 + kPrepRows, p.rows);
-    if (f == 0 && blockIdx.y == 0) {
+    const int tid = threadIdx.x, lane = tid & 31, f = blockIdx.z, w = blockIdx.x;
+    const int tiles = p.rows_pad / kPrepRows;
+    const int h = blockIdx.y / tiles, r0 = (blockIdx.y - h * tiles) * kPrepRows;
+    auto row_lse = [&](int r) { return r < p.rows ? __ldg(p.lse + ((size_t)w * p.Hq + h * p.G + r % p.G) * p.S + r / p.G) : neg_inf(); };
+    long long off = 0;
+    for (int t = 0; t < f; ++t) off += max(__ldg(p.L + t), 0);
+    const int Lf = __ldg(p.L + f);
+    const size_t fw = (size_t)f * p.W + w, fwh = fw * p.Hkv + h;
+    auto seen = [&](int s) { return turn_seen(Lf, __ldg(p.loc + fw * p.S + s), off, p.cap); };
+    __shared__ int red[4];
+    if (r0 == 0) {  // this (turn, sequence, head): what every row sees that gives weight
+        int least = 0x7fffffff;
+        for (int r = tid; r < p.rows; r += 128)
+            if (row_lse(r) != neg_inf()) least = min(least, seen(r / p.G));
+        least = __reduce_min_sync(0xffffffffu, least);
+        if (lane == 0) red[tid >> 5] = least;
+        __syncthreads();
+        least = min(min(red[0], red[1]), min(red[2], red[3]));
+        if (tid == 0) p.all[fwh] = least == 0x7fffffff ? 0 : least;
+        __syncthreads();
+    }
+    if (blockIdx.y == 0 && f == 0) {
         if (w == 0 && tid < 4) p.header[tid] = 0;
-        __shared__ int red[4];
-        long long off = 0;
+        long long at = 0;
         int nw = 0;
         for (int t = 0; t < p.F; ++t) {
             const int Lt = __ldg(p.L + t);
             int v = 0;
-            for (int s = tid; s < p.S; s += 128) v = max(v, turn_seen(Lt, __ldg(p.loc + ((size_t)t * p.W + w) * p.S + s), off, p.cap));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-            if ((tid & 31) == 0) red[tid >> 5] = v;
+            for (int s = tid; s < p.S; s += 128) v = max(v, turn_seen(Lt, __ldg(p.loc + ((size_t)t * p.W + w) * p.S + s), at, p.cap));
+            v = __reduce_max_sync(0xffffffffu, v);
+            if (lane == 0) red[tid >> 5] = v;
             __syncthreads();
             v = max(max(red[0], red[1]), max(red[2], red[3]));
             __syncthreads();
-            const int first = v > 0 ? (int)off : 0;
+            const int first = v > 0 ? (int)at : 0;
             if (tid == 0) p.span[(size_t)w * p.F + t] = make_int2(v, first);
             nw += turn_windows(p, v, first);
-            off += Lt > 0 ? Lt : 0;
+            at += max(Lt, 0);
         }
         if (tid == 0) p.nwin[w] = nw;
     }
-    if (f == 0)
-        for (int r = r0 + tid; r < r1; r += 128) {
-            const int s = r / p.G;
-            const float x = __ldg(p.lse + ((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s);
-            p.lse2[((size_t)w * p.Hkv + h) * p.rows + r] = x == neg_inf() ? -neg_inf() : x * kLog2e;
-        }
+    if (tid < kPrepRows) {
+        const int r = r0 + tid;
+        const float x = row_lse(r);
+        const size_t wh = (size_t)w * p.Hkv + h;
+        if (f == 0) p.nlse[wh * p.rows_pad + r] = x == neg_inf() ? neg_inf() : -x * kLog2e;
+        p.lim[fwh * p.rows_pad + r] = x == neg_inf() ? 0 : seen(r / p.G);
+    }
     constexpr int AHEAD = 2;  // chunks a thread has in flight
-    const int per = E * (int)sizeof(T) / 16;
-    for (int c0 = r0 * per + tid; c0 < r1 * per; c0 += 128 * AHEAD) {
+    const int per = E * (int)sizeof(T) / 16, n = kPrepRows * per;
+    for (int c0 = tid; c0 < n; c0 += 128 * AHEAD) {
         RotateChunk<T> ch[AHEAD];
+        bool counts[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             const int c = c0 + 128 * k;
-            if (c >= r1 * per) break;
-            const int r = c / per, s = r / p.G;
-            const size_t cs = (((size_t)f * p.W + w) * p.S + s) * p.R;
-            ch[k].load(static_cast<const T*>(p.q) + (((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s) * E,
-                       static_cast<T*>(p.qr) + ((((size_t)f * p.W + w) * p.Hkv + h) * p.rows + r) * E, p.cos + cs, p.sin + cs,
-                       (c - r * per) * RotateChunk<T>::PER, p.R, p.rot_vec);
+            counts[k] = false;
+            if (c >= n) break;
+            const int r = r0 + c / per, s = r / p.G, e0 = c % per * RotateChunk<T>::PER;
+            T* dst = static_cast<T*>(p.qr) + (fwh * p.rows_pad + r) * E;
+            counts[k] = row_lse(r) != neg_inf();
+            if (counts[k])
+                ch[k].load(static_cast<const T*>(p.q) + (((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s) * E, dst,
+                           p.cos + (fw * p.S + s) * p.R, p.sin + (fw * p.S + s) * p.R, e0, p.R, p.rot_vec);
+            else
+                *reinterpret_cast<uint4*>(dst + e0) = make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
-            if (c0 + 128 * k < r1 * per) ch[k].store(p.R, p.rot_vec);
+            if (counts[k]) ch[k].store(p.R, p.rot_vec);
     }
 }
 
 // ---- CUDA-core kernel: 32 keys x 32 rows per step, 8 warps of 4 rows, a lane per key ----
-template <class T, int E>
+// (f32; the 16-bit types run on mass_tc_kernel)
+template <int E>
 __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
+    using T = float;
     constexpr int KT = 32, MT = 32, ROW = E * (int)sizeof(T) + 16, CH = E * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T);
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* sQ = smem;                                              // [MT] rows
@@ -121,9 +131,9 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
                 cp_async16_zfill(smem_u32(sK + r * ROW + ch * 16), kp ? kp : static_cast<const T*>(p.k), kp ? 16 : 0);
             }
             cp_async_commit();
-            const T* qr = static_cast<const T*>(p.qr) + (((size_t)win.f * p.W + pc.w) * p.Hkv + h) * p.rows * E;
-            const float* lse2 = p.lse2 + ((size_t)pc.w * p.Hkv + h) * p.rows;
-            const int Lf = __ldg(p.L + win.f);
+            const T* qr = static_cast<const T*>(p.qr) + (((size_t)win.f * p.W + pc.w) * p.Hkv + h) * p.rows_pad * E;
+            const float* nlse = p.nlse + ((size_t)pc.w * p.Hkv + h) * p.rows_pad;
+            const int* lim = p.lim + (((size_t)win.f * p.W + pc.w) * p.Hkv + h) * p.rows_pad;
             float acc = 0.f;
             for (int r0 = 0; r0 < p.rows; r0 += MT) {
                 for (int c = tid; c < MT * CH; c += 256) {
@@ -152,9 +162,7 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
                 for (int a = 0; a < 4; ++a) {
                     const int r = r0 + wid * 4 + a;
                     if (r >= p.rows) continue;
-                    const float l2 = __ldcg(lse2 + r);
-                    const int lim = turn_seen(Lf, __ldg(p.loc + ((size_t)win.f * p.W + pc.w) * p.S + r / p.G), win.off, p.cap);
-                    if (l2 != -neg_inf() && lane < win.n && win.k0 + lane < lim) acc += fast_exp2(sc[a] * p.scale_log2 - l2);
+                    if (lane < win.n && win.k0 + lane < __ldcg(lim + r)) acc += fast_exp2(fmaf(sc[a], p.scale_log2, __ldcg(nlse + r)));
                 }
                 __syncthreads();
             }
@@ -175,21 +183,24 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
 }
 
 // ---------------------------------------------------------------------------------------
-struct MassKernel {
-    const void* fn;
-    int threads, kt;
-    size_t smem;
-};
-template <class T, int E> static MassKernel mass_simt() {
-    return MassKernel{(const void*)&mass_simt_kernel<T, E>, 256, 32, (size_t)64 * (E * sizeof(T) + 16) + 8 * 32 * 4};
-}
-template <class T> static MassKernel mass_pick_e(int E) {
-    return E == 64 ? mass_simt<T, 64>() : E == 128 ? mass_simt<T, 128>() : mass_simt<T, 256>();
+template <int E> static MassKernel mass_simt() {
+    const size_t smem = (size_t)64 * (E * 4 + 16) + 8 * 32 * 4;
+    return MassKernel{(const void*)&mass_simt_kernel<E>, 256, 32, E == 64 ? 8 : E == 128 ? 6 : 3, 1 << 30, smem};
 }
 static MassKernel mass_pick(const dvattn_mass_args* a) {
-    return a->dtype == DVATTN_FLOAT32 ? mass_pick_e<float>(a->E)
-         : a->dtype == DVATTN_FLOAT16 ? mass_pick_e<__half>(a->E) : mass_pick_e<__nv_bfloat16>(a->E);
+    if (a->dtype != DVATTN_FLOAT32) return mass_tc_pick(a->dtype, a->E, a->S * (a->Hq / a->Hkv));
+    return a->E == 64 ? mass_simt<64>() : a->E == 128 ? mass_simt<128>() : mass_simt<256>();
 }
+
+// DVATTN_TEST_STALL_TILE=<i>: tests only (see the decode launcher); read once per process.
+static int mass_stall_hook() {
+    static const int t = [] {
+        const char* e = getenv("DVATTN_TEST_STALL_TILE");
+        return e && *e ? atoi(e) : -1;
+    }();
+    return t;
+}
+static long long mass_rows_pad(const dvattn_mass_args* a) { return ((long long)a->S * (a->Hq / a->Hkv) + kPrepRows - 1) / kPrepRows * kPrepRows; }
 
 static int mass_validate(const dvattn_mass_args* a) {
     if (!a) return DVATTN_ERR_INVALID_ARGUMENT;
@@ -199,9 +210,9 @@ static int mass_validate(const dvattn_mass_args* a) {
     const int st = decode_validate(&v);
     if (st != DVATTN_OK) return st;
     if (a->positions < 0) return DVATTN_ERR_INVALID_ARGUMENT;
-    // grid limits of the prep kernel: turns are its z, row tiles of the KV heads its y
-    const long long rows = (long long)a->S * (a->Hq / a->Hkv);
-    if (a->F > 65535 || (rows + kPrepRows - 1) / kPrepRows * a->Hkv > 65535) return DVATTN_ERR_UNSUPPORTED;
+    // grid limits of the prep kernel: turns are its z, row tiles of the KV heads its y; 32-bit rows
+    if (a->F > 65535 || mass_rows_pad(a) / kPrepRows * a->Hkv > 65535 || (double)a->F * a->W * a->Hkv * mass_rows_pad(a) > 0x7fffffffLL - 128)
+        return DVATTN_ERR_UNSUPPORTED;
     return DVATTN_OK;
 }
 static bool mass_nothing(const dvattn_mass_args* a) {
@@ -209,18 +220,17 @@ static bool mass_nothing(const dvattn_mass_args* a) {
 }
 
 struct MassLayout {
-    size_t nwin, span, qr, lse2, total;
+    size_t nwin, span, qr, nlse, lim, all, total;
     int groups;
 };
 static int mass_layout(const dvattn_mass_args* a, const MassKernel& k, MassLayout& L) {
-    int dev = 0, sms = 0, occ = 0;
+    int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k.fn, k.threads, k.smem) != cudaSuccess || occ < 1)
+        cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem) != cudaSuccess)
         return DVATTN_ERR_CUDA;
-    L.groups = sms * occ / a->Hkv;
+    L.groups = sms * k.ctas / a->Hkv;
     if (L.groups < 1) L.groups = 1;
-    const size_t esz = a->dtype == DVATTN_FLOAT32 ? 4 : 2, rows = (size_t)a->S * (a->Hq / a->Hkv);
+    const size_t esz = a->dtype == DVATTN_FLOAT32 ? 4 : 2, rows = (size_t)mass_rows_pad(a), wh = (size_t)a->W * a->Hkv;
     size_t at = 256;
     auto take = [&](size_t bytes) {
         const size_t r = at;
@@ -229,8 +239,10 @@ static int mass_layout(const dvattn_mass_args* a, const MassKernel& k, MassLayou
     };
     L.nwin = take(4 * (size_t)a->W);
     L.span = take(8 * (size_t)a->W * a->F);
-    L.qr = take(esz * (size_t)a->F * a->W * a->Hkv * rows * a->E);
-    L.lse2 = take(4 * (size_t)a->W * a->Hkv * rows);
+    L.qr = take(esz * a->F * wh * rows * a->E);
+    L.nlse = take(4 * wh * rows);
+    L.lim = take(4 * a->F * wh * rows);
+    L.all = take(4 * a->F * wh);
     L.total = at;
     return DVATTN_OK;
 }
@@ -257,6 +269,9 @@ int mass_launch(const dvattn_mass_args* a, void* workspace, size_t wbytes, cudaS
     MassParams p{};
     p.F = a->F; p.W = a->W; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.S = a->S; p.R = a->R;
     p.rows = p.S * p.G;
+    p.rows_pad = (int)mass_rows_pad(a);
+    p.passes = (p.rows_pad + k.pass_rows - 1) / k.pass_rows;
+    p.stall_tile = mass_stall_hook();
     p.rot_vec = rotate_vec(a->R, a->cosines, a->sines);
     p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
     const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
@@ -270,25 +285,30 @@ int mass_launch(const dvattn_mass_args* a, void* workspace, size_t wbytes, cudaS
     p.nwin = reinterpret_cast<int*>(ws + L.nwin);
     p.span = reinterpret_cast<int2*>(ws + L.span);
     p.qr = ws + L.qr;
-    p.lse2 = reinterpret_cast<float*>(ws + L.lse2);
+    p.nlse = reinterpret_cast<float*>(ws + L.nlse);
+    p.lim = reinterpret_cast<int*>(ws + L.lim);
+    p.all = reinterpret_cast<int*>(ws + L.all);
+    alignas(64) MassMaps maps;
+    if (a->dtype != DVATTN_FLOAT32 && !mass_tc_maps(p, a->dtype, a->E, maps)) return DVATTN_ERR_CUDA;
     const void* prep = a->dtype == DVATTN_FLOAT32   ? (const void*)&mass_prep_kernel<float>
                        : a->dtype == DVATTN_FLOAT16 ? (const void*)&mass_prep_kernel<__half> : (const void*)&mass_prep_kernel<__nv_bfloat16>;
     int E = a->E;
     void* pargs[] = {&p, &E};
-    const unsigned tiles = (unsigned)((p.rows + kPrepRows - 1) / kPrepRows * a->Hkv);
-    cudaError_t e = cudaLaunchKernel(prep, dim3(a->W, tiles, a->F), dim3(128), pargs, 0, stream);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.stream = stream;
+    cfg.gridDim = dim3(a->W, (unsigned)(p.rows_pad / kPrepRows * a->Hkv), a->F);
+    cfg.blockDim = dim3(128);
+    cudaError_t e = cudaLaunchKernelExC(&cfg, prep, pargs);
     if (e == cudaSuccess) {
-        cudaLaunchConfig_t cfg = {};
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        cfg.stream = stream;
         cfg.gridDim = dim3((unsigned)(L.groups * a->Hkv));
         cfg.blockDim = dim3(k.threads);
         cfg.dynamicSmemBytes = k.smem;
-        void* args[] = {&p};
+        void* args[] = {&p, &maps};  // the CUDA-core kernel takes the first only
         e = cudaLaunchKernelExC(&cfg, k.fn, args);
     }
     if (e != cudaSuccess) {

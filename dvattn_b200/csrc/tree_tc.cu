@@ -465,20 +465,14 @@ TreeKernel tree_tc_pick(int dtype, int E, int rows) {
 }
 
 bool tree_tc_maps(TreeParams& p, int dtype, int E, TreeMaps& m) {
-    const int kt = p.kt;
-    int b = kt;  // the largest power of two that divides the page size, at most a window
-    while (p.BS % b) b >>= 1;
     const long long tokens = p.NB * p.BS, drafts = (long long)p.W * p.Hkv * p.S;
     p.out_sectors = !(reinterpret_cast<uintptr_t>(p.out) & 31);
-    p.box = 0;
-    p.align = 1;
     if (!encode_cache_map(&m.q, p.qr, dtype, E, 1, (long long)p.F * p.W * p.Hq * p.S, 128)) return false;
-    // 8 rows are what the 128-byte swizzle repeats over; coordinates are 32-bit
-    if (b < 8 || p.cap == 0 || tokens > 0x7fffffffLL - 2 * (long long)p.BS || drafts > 0x7fffffffLL - kt) return true;
-    p.box = b;
-    p.align = b;
-    return encode_cache_map(&m.k, p.k, dtype, E, p.Hkv, tokens, b) && encode_cache_map(&m.v, p.v, dtype, E, p.Hkv, tokens, b) &&
-           encode_cache_map(&m.dk, p.dkr, dtype, E, 1, drafts, kt) && encode_cache_map(&m.dv, p.dv, dtype, E, 1, drafts, kt);
+    p.box = p.cap > 0 && drafts <= 0x7fffffffLL - p.kt ? window_box(p.BS, p.kt, p.NB) : 0;
+    p.align = p.box ? p.box : 1;
+    if (!p.box) return true;
+    return encode_cache_map(&m.k, p.k, dtype, E, p.Hkv, tokens, p.box) && encode_cache_map(&m.v, p.v, dtype, E, p.Hkv, tokens, p.box) &&
+           encode_cache_map(&m.dk, p.dkr, dtype, E, 1, drafts, p.kt) && encode_cache_map(&m.dv, p.dv, dtype, E, 1, drafts, p.kt);
 }
 
 }  // namespace dvb

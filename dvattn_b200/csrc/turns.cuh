@@ -188,7 +188,7 @@ struct SplitWin {
 // walks the CTA's range and hands the runs to the others through a ring in shared memory, a few
 // ahead, so that none of them keeps the walk's state or waits for its loads.
 struct alignas(16) SplitRun {
-    int w, t, f, off;    // sequence, row tile, turn (F: the tail), the turn's first position
+    int w, t, f, off;    // sequence, row tile (or pass), turn (F: the tail), the turn's first position
     int k0, sp, n, how;  // first key of the first window, seen keys, windows (0: the end), RUN_* bits
 };
 constexpr int RUN_FIRST = 1, RUN_LAST = 2;   // of its piece
@@ -196,10 +196,12 @@ constexpr int RUN_WHOLE = 4, RUN_BEGIN = 8;  // the piece is a whole item; it be
 constexpr int RUN_Q_NEW = 16, RUN_Q_END = 32;  // q rotated for another turn than before; the next run's will be
 constexpr int RUN_RING = 8;
 
-// The walking warp: `full` and `empty` are RUN_RING mbarriers each (one arrival; one per
+// The walking warp.  passes > 1: every run that many times, t = 0, 1, ..., each with its own q
+// (the split then has one row tile).  `full` and `empty` are RUN_RING mbarriers each (one arrival; one per
 // consumer).  false: a wait gave up.
 template <class Stop>
-__device__ __forceinline__ bool split_schedule(const TurnSplit& p, int lane, int g, SplitRun* ring, uint32_t full, uint32_t empty, Stop stopped) {
+__device__ __forceinline__ bool split_schedule(const TurnSplit& p, int lane, int g, SplitRun* ring, uint32_t full, uint32_t empty, Stop stopped,
+                                               int passes = 1) {
     SplitWalk walk;
     walk.place(p, lane, g);
     SplitPiece pc;
@@ -226,7 +228,10 @@ __device__ __forceinline__ bool split_schedule(const TurnSplit& p, int lane, int
             r.w = pc.w, r.t = pc.t, r.f = win.f, r.off = win.off, r.k0 = win.k0, r.sp = win.sp, r.n = nx;
             r.how = (i == pc.i0 ? RUN_FIRST : 0) | (i + nx == pc.i1 ? RUN_LAST : 0) | (pc.whole() ? RUN_WHOLE : 0) | (pc.slot() ? RUN_BEGIN : 0) |
                     (qt != turn ? RUN_Q_NEW : 0) | (i + nx == pc.i1 || qt != p.F - 1 ? RUN_Q_END : 0);
-            if (!push(r)) return false;
+            for (int pass = 0; pass < passes; ++pass) {
+                if (passes > 1) r.t = pass, r.how |= RUN_Q_NEW | RUN_Q_END;
+                if (!push(r)) return false;
+            }
             turn = qt;
             i += nx;
         }

@@ -12,6 +12,15 @@
 
 namespace dvb {
 
+// Rows of a TMA box: the largest power of two that divides the page size, at most a window; 0
+// where it is below the 8 rows that the 128-byte swizzle repeats over, or a coordinate might not
+// fit in 32 bits.
+inline int window_box(int BS, int kt, long long NB) {
+    int b = kt;
+    while (BS % b) b >>= 1;
+    return b < 8 || NB * BS > 0x7fffffffLL - 2 * (long long)BS ? 0 : b;
+}
+
 struct WindowSource {
     const void* cache;            // [NB][BS][Hkv][E]
     const void* tail;             // [W][Hkv][tail][E], or null where the split has no tail
