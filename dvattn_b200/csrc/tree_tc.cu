@@ -150,13 +150,13 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
         WindowSource src;
         src.cache = is_k ? p.k : p.v, src.tail = is_k ? p.dkr : p.dv;
         src.map = is_k ? &maps.k : &maps.v, src.tail_map = is_k ? &maps.dk : &maps.dv;
-        src.h = h, src.Hkv = p.Hkv, src.box = p.box, src.anc = p.anc, src.SW = p.SW;
+        src.h = h, src.Hkv = p.Hkv, src.box = p.box, src.me = 0, src.of = 1, src.anc = p.anc, src.SW = p.SW;
         // keys and values that one row tile reads are read once: they leave L2 first, the partial
         // results stay for the merge
         src.policy = p.nt == 1 ? l2_evict_first() : l2_evict_normal();
         src.stall = is_k && blockIdx.x == 0 ? p.stall_tile : -1;
         int epoch = 0;
-        const bool ok = produce_windows<T, E, KT>(
+        const bool ok = produce_windows<T, E, KT, 1>(
             p, src, is_k ? C::K_STAGES : VS, s0 + (is_k ? C::OFF_K : C::OFF_V), is_k ? k_full : v_full, is_k ? k_empty : v_empty, take_run, wait,
             [&] { return *s_abort != 0; }, [&](const SplitRun& run) { return !is_k || !(run.how & RUN_Q_NEW) || load_q(run, epoch++); });
         if (!ok) {

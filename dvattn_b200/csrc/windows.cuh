@@ -29,24 +29,53 @@ struct WindowSource {
     const uint32_t* anc;          // [W][tail][SW]: a tail row without its own bit is not there
     int SW, h, Hkv;
     int box;                      // rows of a TMA box, 0: gathered
+    int me, of;                   // this warp requests the windows me, me + of, ... of every run
     int stall;                    // test hook: this window never arrives; -1: off
     uint64_t policy;              // L2
 };
 
 // `take_run(n, run)`, `wait(barrier, phase)`: as a whole warp, false when they give up.
-// `opened(run)` is called once the first window of a run has been requested.  false: a wait gave
-// up; everything that was requested has landed.
-template <class T, int E, int KT, class Take, class Wait, class Stop, class Opened>
+// `opened(run)` is called at the beginning of a run, after its first window has been requested
+// where that is this warp's.  false: a wait gave up; everything that was requested has landed.
+// PARTS: a window comes as that many tiles of E / PARTS columns, one after the other, each in a
+// stage of its own.
+//
+// The ring belongs to this warp and one consumer, so both see every phase of its barriers: a
+// parity cannot be taken for the one two phases before.
+//
+// A warp takes about 75 cycles to issue a box.  With pages of 16 keys that is 1200 cycles for a
+// window of 128 keys of one tensor, as long as HBM takes to bring it; hence `of`.
+template <class T, int E, int KT, int PARTS, class Take, class Wait, class Stop, class Opened>
 __device__ __forceinline__ bool produce_windows(const TurnSplit& p, const WindowSource& s, int stages, uint32_t ring, uint32_t full, uint32_t empty,
                                                 Take take_run, Wait wait, Stop stopped, Opened opened) {
-    constexpr int NP = E / 64, KPANEL = KT * 128, KTILE = NP * KPANEL;
+    constexpr int NP = E / 64 / PARTS, KPANEL = KT * 128, KTILE = NP * KPANEL;  // of a part
     const int lane = threadIdx.x & 31;
     const int h = s.h, Hkv = s.Hkv;
     // what the kernel before wrote with ordinary stores is read by TMA
     asm volatile("fence.proxy.async;" ::: "memory");
     SplitRun run;
-    int nr = 0, x = 0, iw = 0;  // runs taken, window of the run, windows requested
+    int nr = 0, x = s.me, iw = 0;  // runs taken, window of the run, tiles requested
+    bool fresh = true;             // the run has not been opened
     bool ok = take_run(nr++, run);
+    // after a window (or none) of this warp: opens the run, goes on to the next window
+    auto advance = [&](bool requested) {
+        if (fresh && run.n) {
+            fresh = false;
+            if (!opened(run)) return false;
+        }
+        if (requested) x += s.of;
+        while (run.n && x >= run.n) {
+            x = s.me;
+            if (!take_run(nr++, run)) return false;
+            if (run.n && x >= run.n) {  // a run without a window of this warp
+                if (!opened(run)) return false;
+                continue;
+            }
+            fresh = true;
+        }
+        return true;
+    };
+    if (ok && run.n && x >= run.n) ok = advance(false);
     if (s.box) {
         if (lane == 0) {
             prefetch_tmap(s.map);
@@ -69,29 +98,25 @@ __device__ __forceinline__ bool produce_windows(const TurnSplit& p, const Window
         };
         if (ok && run.n) find();
         while (ok && run.n) {
-            const int st = iw % stages;
-            if (iw >= stages && (stopped() || !wait(empty + 8 * st, iw / stages - 1))) {
-                ok = false;
-                break;
-            }
             const int z = next;
             const bool tail = run.f == p.F;
-            if (iw != s.stall) {
+            for (int part = 0; part < PARTS; ++part, ++iw) {
+                const int st = iw % stages;
+                if (iw >= stages && (stopped() || !wait(empty + 8 * st, iw / stages - 1))) {
+                    ok = false;
+                    break;
+                }
+                if (iw == s.stall) continue;
                 if (lane == 0) mbar_expect_tx(full + 8 * st, (uint32_t)KTILE);
                 __syncwarp();
                 const uint32_t dst = ring + (uint32_t)(st * KTILE);
                 if (tail ? lane == 0 : lane < boxes)
 #pragma unroll
                     for (int y = 0; y < NP; ++y)
-                        tma_load_3d_hint(dst + (uint32_t)(y * KPANEL + lane * s.box * 128), tail ? s.tail_map : s.map, y * 64, tail ? 0 : h, z,
-                                         full + 8 * st, s.policy);
+                        tma_load_3d_hint(dst + (uint32_t)(y * KPANEL + lane * s.box * 128), tail ? s.tail_map : s.map, (part * NP + y) * 64,
+                                         tail ? 0 : h, z, full + 8 * st, s.policy);
             }
-            ++iw;
-            if (x == 0 && !(ok = opened(run))) break;
-            if (++x == run.n) {
-                x = 0;
-                if (!(ok = take_run(nr++, run))) break;
-            }
+            if (!ok || !(ok = advance(true))) break;
             if (run.n) find();
         }
         if (!ok)  // bounded waits
@@ -101,10 +126,10 @@ __device__ __forceinline__ bool produce_windows(const TurnSplit& p, const Window
     }
     const T* cache = static_cast<const T*>(s.cache);
     const T* draft = static_cast<const T*>(s.tail);
-    constexpr int NR = KT / 32;  // rows of a window whose addresses a lane finds
-    constexpr int CH = E / 8;    // 16-byte chunks of a row
-    constexpr int RPI = 32 / CH; // rows per copy instruction
-    const T* next[NR];           // rows lane + 32 k of the window to be requested, null: zeros
+    constexpr int NR = KT / 32;          // rows of a window whose addresses a lane finds
+    constexpr int CH = E / 8 / PARTS;    // 16-byte chunks of a row of a part
+    constexpr int RPI = 32 / CH;         // rows per copy instruction
+    const T* next[NR];                   // rows lane + 32 k of the window to be requested, null: zeros
     auto find = [&] {
         const int k0 = run.k0 + x * KT;
 #pragma unroll
@@ -122,7 +147,7 @@ __device__ __forceinline__ bool produce_windows(const TurnSplit& p, const Window
             }
         }
     };
-    int signalled = 0;                // windows handed over
+    int signalled = 0;                // tiles handed over
     auto hand_over = [&](int upto) {  // their copies have landed
         fence_proxy_async_smem();
         for (; signalled < upto; ++signalled)
@@ -130,42 +155,40 @@ __device__ __forceinline__ bool produce_windows(const TurnSplit& p, const Window
     };
     if (ok && run.n) find();
     while (ok && run.n) {
-        const int st = iw % stages;
-        if (iw >= stages && !__all_sync(0xffffffffu, mbar_try_wait(empty + 8 * st, (iw / stages - 1) & 1))) {
-            // about to wait: hand over what is under way first
+        for (int part = 0; part < PARTS; ++part, ++iw) {
+            const int st = iw % stages;
+            if (iw >= stages && !__all_sync(0xffffffffu, mbar_try_wait(empty + 8 * st, (iw / stages - 1) & 1))) {
+                // about to wait: hand over what is under way first
+                cp_async_wait<0>();
+                hand_over(iw);
+                if (stopped() || !wait(empty + 8 * st, iw / stages - 1)) {
+                    ok = false;
+                    break;
+                }
+            }
+            const uint32_t dst = ring + (uint32_t)(st * KTILE);
+            const int ch = lane % CH;
+#pragma unroll
+            for (int k = 0; k < NR; ++k) {
+                const unsigned long long row = reinterpret_cast<unsigned long long>(next[k]);
+#pragma unroll 4
+                for (int y = 0; y < CH; ++y) {
+                    const int rl = y * RPI + lane / CH, r = 32 * k + rl;
+                    const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, row, rl));
+                    cp_async16_zfill(dst + (uint32_t)((ch >> 3) * KPANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
+                                     src ? src + (part * CH + ch) * 8 : cache, src ? 16 : 0);
+                }
+            }
+            cp_async_commit();
+            cp_async_wait<1>();
+            hand_over(iw);
+        }
+        if (!ok) break;
+        if (fresh || x + s.of >= run.n) {  // advance() may wait
             cp_async_wait<0>();
             hand_over(iw);
-            if (stopped() || !wait(empty + 8 * st, iw / stages - 1)) {
-                ok = false;
-                break;
-            }
         }
-        const uint32_t dst = ring + (uint32_t)(st * KTILE);
-        const int ch = lane % CH;
-#pragma unroll
-        for (int k = 0; k < NR; ++k) {
-            const unsigned long long mine = reinterpret_cast<unsigned long long>(next[k]);
-#pragma unroll 4
-            for (int y = 0; y < CH; ++y) {
-                const int rl = y * RPI + lane / CH, r = 32 * k + rl;
-                const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, mine, rl));
-                cp_async16_zfill(dst + (uint32_t)((ch >> 3) * KPANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4)), src ? src + ch * 8 : cache,
-                                 src ? 16 : 0);
-            }
-        }
-        cp_async_commit();
-        cp_async_wait<1>();
-        hand_over(iw);
-        ++iw;
-        if (x == 0) {
-            cp_async_wait<0>();  // opened() may wait
-            hand_over(iw);
-            if (!(ok = opened(run))) break;
-        }
-        if (++x == run.n) {
-            x = 0;
-            if (!(ok = take_run(nr++, run))) break;
-        }
+        if (!(ok = advance(true))) break;
         if (run.n) find();
     }
     cp_async_wait<0>();
