@@ -13,10 +13,6 @@
 // and o[e+R/2] = x[e+R/2]*c[e+R/2] + x[e]*s[e+R/2] (full-width cos/sin rows, both
 // halves read), dims e >= R copied; f32 math, one rounding to T.
 //
-// With `accepted` (dvattn_tree_append) the new tokens are nodes of a drafted tree: worker w's
-// entry i takes token accepted[w][i] of the n drafted ones and goes to position pos[w] + i,
-// for i < counts[w].
-//
 // A warp per new token, a lane per 16-byte chunk of its K / V rows: a K chunk in the
 // first rotary half also reads its partner chunk R/2 further, and vice versa.  HBM-bound.
 #include "decode.cuh"
@@ -25,7 +21,6 @@ namespace dvb {
 
 struct AppendParams {
     int W, Hkv, E, Ev, n, R, BS, maxb;
-    int m;    // entries per worker: n, or the width of `accepted`
     int vec;  // 1: R/2 a multiple of the chunk width (or R = 0) and cos/sin 16-byte aligned
     long long NB;
     void* k_cache;
@@ -37,7 +32,6 @@ struct AppendParams {
     const int* bt;
     const int* pos;
     const int* cnt;
-    const int* acc;  // [W][m] token of each entry, or null: the last cnt of the n tokens
 };
 
 template <class T>
@@ -67,29 +61,21 @@ __global__ void __launch_bounds__(256, APPEND_MINB) paged_append_kernel(AppendPa
     const int per_tok = p.Hkv * (ck + cv);
     const int lane = threadIdx.x & 31;
     // 32-bit token / position arithmetic: the launch checks W*n and maxb*BS < 2^31
-    const int ntok = p.W * p.m;
+    const int ntok = p.W * p.n;
     const int nwarp = gridDim.x * (blockDim.x >> 5);
     for (int wt = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); wt < ntok; wt += nwarp) {
-        const int w = wt / p.m, i = wt - w * p.m;
-        const int cnt = p.cnt ? __ldg(p.cnt + w) : p.m;
-        int t = i, at = i;  // the token, and its place after the worker's position
-        if (p.acc) {
-            if (i >= cnt) continue;
-            t = __ldg(p.acc + wt);
-            if (t < 0 || t >= p.n) continue;
-        } else {
-            const int first = p.n - (cnt < p.n ? (cnt > 0 ? cnt : 0) : p.n);
-            if (t < first) continue;  // left padding: only the last cnt tokens are new
-            at = t - first;
-        }
-        const long long lp64 = (long long)__ldg(p.pos + w) + at;
+        const int w = wt / p.n, t = wt - w * p.n;
+        const int cnt = p.cnt ? __ldg(p.cnt + w) : p.n;
+        const int first = p.n - (cnt < p.n ? (cnt > 0 ? cnt : 0) : p.n);
+        if (t < first) continue;  // left padding: only the last cnt tokens are new
+        const long long lp64 = (long long)__ldg(p.pos + w) + (t - first);
         if (lp64 < 0 || lp64 >= (long long)p.maxb * p.BS) continue;
         const int lp = (int)lp64;
         const int pg = lp / p.BS;
         const int page = __ldg(p.bt + (size_t)w * p.maxb + pg);
         const bool page_ok = page >= 0 && page < p.NB;  // checked before any store
         const long long slot = (long long)page * p.BS + (lp - pg * p.BS);
-        const size_t crow = ((size_t)w * p.n + t) * p.R;
+        const size_t crow = (size_t)wt * p.R;
         if (p.vec) {
             // every chunk lies inside one rotary half (or past R): a lane issues all the
             // 16-byte loads of its APPEND_UNROLL chunks, in flight with the block-table
@@ -178,19 +164,19 @@ __global__ void __launch_bounds__(256, APPEND_MINB) paged_append_kernel(AppendPa
     }
 }
 
-// The plain append, or with `tree` that of a drafted tree's accepted tokens, [W][m].
-static int append_launch(const dvattn_append_args* a, bool tree, const int* accepted, int m, cudaStream_t stream) {
+int paged_append_launch(const dvattn_append_args* a, cudaStream_t stream) {
+    if (!a) return DVATTN_ERR_INVALID_ARGUMENT;
     if (a->dtype < 0 || a->dtype > 2) return DVATTN_ERR_UNSUPPORTED;
     if (a->W < 0 || a->n < 0 || a->Hkv <= 0 || a->E <= 0 || a->Ev <= 0 || a->R < 0 || a->R > a->E || (a->R & 1) ||
         a->block_size <= 0 || a->max_blocks_per_seq < 0 || a->num_blocks < 0)
         return DVATTN_ERR_INVALID_ARGUMENT;
     const int esz = a->dtype == DVATTN_FLOAT32 ? 4 : 2;
     if ((a->E * esz) % 16 || (a->Ev * esz) % 16) return DVATTN_ERR_UNSUPPORTED;
-    if ((long long)a->W * a->n == 0 || m == 0) return DVATTN_OK;
-    if ((long long)a->W * a->n >= (1LL << 31) || (long long)a->W * m >= (1LL << 31) || (long long)a->max_blocks_per_seq * a->block_size >= (1LL << 31))
+    if ((long long)a->W * a->n == 0) return DVATTN_OK;
+    if ((long long)a->W * a->n >= (1LL << 31) || (long long)a->max_blocks_per_seq * a->block_size >= (1LL << 31))
         return DVATTN_ERR_UNSUPPORTED;
     if (!a->k_cache || !a->v_cache || !a->keys || !a->values || !a->block_tables || !a->positions ||
-        (a->R > 0 && (!a->cosines || !a->sines)) || (tree && !accepted))
+        (a->R > 0 && (!a->cosines || !a->sines)))
         return DVATTN_ERR_INVALID_ARGUMENT;
     for (const void* q : {(const void*)a->k_cache, (const void*)a->v_cache, a->keys, a->values})
         if (reinterpret_cast<uintptr_t>(q) & 15) return DVATTN_ERR_INVALID_ARGUMENT;
@@ -199,7 +185,6 @@ static int append_launch(const dvattn_append_args* a, bool tree, const int* acce
     p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
     p.k_cache = a->k_cache; p.v_cache = a->v_cache; p.keys = a->keys; p.values = a->values;
     p.cos = a->cosines; p.sin = a->sines; p.bt = a->block_tables; p.pos = a->positions; p.cnt = a->counts;
-    p.m = m; p.acc = accepted;
     {
         const int per = 16 / esz;
         p.vec = ((a->R >> 1) % per) == 0 && !(reinterpret_cast<uintptr_t>(a->cosines) & 15) &&
@@ -208,7 +193,7 @@ static int append_launch(const dvattn_append_args* a, bool tree, const int* acce
     int sms = 148;
     int dev = 0;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const long long want = ((long long)a->W * m + 7) / 8;  // 8 warps (tokens) per block
+    const long long want = ((long long)a->W * a->n + 7) / 8;  // 8 warps (tokens) per block
     const long long cap = (long long)sms * APPEND_MINB;  // one wave of resident blocks
     const int grid = (int)(want < cap ? want : cap);
     switch (a->dtype) {
@@ -217,22 +202,6 @@ static int append_launch(const dvattn_append_args* a, bool tree, const int* acce
         default: paged_append_kernel<float><<<grid, 256, 0, stream>>>(p); break;
     }
     return cudaGetLastError() == cudaSuccess ? DVATTN_OK : DVATTN_ERR_CUDA;
-}
-
-int paged_append_launch(const dvattn_append_args* a, cudaStream_t stream) {
-    if (!a) return DVATTN_ERR_INVALID_ARGUMENT;
-    return append_launch(a, false, nullptr, a->n, stream);
-}
-
-int tree_append_launch(const dvattn_tree_append_args* t, cudaStream_t stream) {
-    if (!t || t->A < 0) return DVATTN_ERR_INVALID_ARGUMENT;
-    dvattn_append_args a{};
-    a.dtype = t->dtype; a.W = t->W; a.Hkv = t->Hkv; a.E = t->E; a.Ev = t->Ev; a.n = t->S; a.R = t->R;
-    a.block_size = t->block_size; a.max_blocks_per_seq = t->max_blocks_per_seq; a.num_blocks = t->num_blocks;
-    a.k_cache = t->k_cache; a.v_cache = t->v_cache; a.keys = t->draft_keys; a.values = t->draft_values;
-    a.cosines = t->cosines; a.sines = t->sines; a.block_tables = t->block_tables; a.positions = t->positions;
-    a.counts = t->counts;
-    return append_launch(&a, true, t->accepted, t->A, stream);
 }
 
 }  // namespace dvb
