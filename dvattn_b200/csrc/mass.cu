@@ -102,8 +102,7 @@ __global__ void __launch_bounds__(128) mass_prep_kernel(MassParams p, int E) {
 // (f32; the 16-bit types run on mass_tc_kernel)
 template <int E>
 __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
-    using T = float;
-    constexpr int KT = 32, MT = 32, ROW = E * (int)sizeof(T) + 16, CH = E * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T);
+    constexpr int KT = 32, MT = 32, ROW = E * 4 + 16, CH = E / 4;
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* sQ = smem;                                              // [MT] rows
     uint8_t* sK = smem + MT * ROW;                                   // [KT] rows
@@ -121,17 +120,17 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
             win.seek(p, pc.w, i);
             for (int c = tid; c < KT * CH; c += 256) {
                 const int r = c / CH, ch = c - r * CH;
-                const T* kp = nullptr;
+                const float* kp = nullptr;
                 if (r < win.n) {
                     const int pos = win.off + win.k0 + r;
                     const int page = __ldg(p.bt + (size_t)pc.w * p.maxb + pos / p.BS);
                     if (page >= 0 && page < p.NB)
-                        kp = static_cast<const T*>(p.k) + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E + ch * PER;
+                        kp = static_cast<const float*>(p.k) + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E + ch * 4;
                 }
-                cp_async16_zfill(smem_u32(sK + r * ROW + ch * 16), kp ? kp : static_cast<const T*>(p.k), kp ? 16 : 0);
+                cp_async16_zfill(smem_u32(sK + r * ROW + ch * 16), kp ? kp : static_cast<const float*>(p.k), kp ? 16 : 0);
             }
             cp_async_commit();
-            const T* qr = static_cast<const T*>(p.qr) + (((size_t)win.f * p.W + pc.w) * p.Hkv + h) * p.rows_pad * E;
+            const float* qr = static_cast<const float*>(p.qr) + (((size_t)win.f * p.W + pc.w) * p.Hkv + h) * p.rows_pad * E;
             const float* nlse = p.nlse + ((size_t)pc.w * p.Hkv + h) * p.rows_pad;
             const int* lim = p.lim + (((size_t)win.f * p.W + pc.w) * p.Hkv + h) * p.rows_pad;
             float acc = 0.f;
@@ -139,7 +138,7 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
                 for (int c = tid; c < MT * CH; c += 256) {
                     const int r = c / CH, ch = c - r * CH;
                     const bool in = r0 + r < p.rows;
-                    cp_async16_zfill(smem_u32(sQ + r * ROW + ch * 16), qr + (size_t)(in ? r0 + r : 0) * E + ch * PER, in ? 16 : 0);
+                    cp_async16_zfill(smem_u32(sQ + r * ROW + ch * 16), qr + (size_t)(in ? r0 + r : 0) * E + ch * 4, in ? 16 : 0);
                 }
                 cp_async_commit();
                 cp_async_wait<0>();
@@ -147,15 +146,14 @@ __global__ void __launch_bounds__(256) mass_simt_kernel(MassParams p) {
                 float sc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
                 for (int ch = 0; ch < CH; ++ch) {
-                    const T* kc = reinterpret_cast<const T*>(sK + lane * ROW + ch * 16);
-                    float kv[PER];
-#pragma unroll
-                    for (int e = 0; e < PER; ++e) kv[e] = Elem<T>::to_f(kc[e]);
+                    const float4 k4 = *reinterpret_cast<const float4*>(sK + lane * ROW + ch * 16);
 #pragma unroll
                     for (int a = 0; a < 4; ++a) {
-                        const T* qc = reinterpret_cast<const T*>(sQ + (wid * 4 + a) * ROW + ch * 16);
-#pragma unroll
-                        for (int e = 0; e < PER; ++e) sc[a] = fmaf(Elem<T>::to_f(qc[e]), kv[e], sc[a]);
+                        const float4 q4 = *reinterpret_cast<const float4*>(sQ + (wid * 4 + a) * ROW + ch * 16);
+                        sc[a] = fmaf(q4.x, k4.x, sc[a]);
+                        sc[a] = fmaf(q4.y, k4.y, sc[a]);
+                        sc[a] = fmaf(q4.z, k4.z, sc[a]);
+                        sc[a] = fmaf(q4.w, k4.w, sc[a]);
                     }
                 }
 #pragma unroll

@@ -110,42 +110,46 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
         if (first + 256 * k + tid < all) ch[k].store(p.R, p.rot_vec);
 }
 
-// ---- CUDA-core attention --------------------------------------------------------------
+// ---- CUDA-core attention, 32-bit types -----------------------------------------------------
 // 32 rows x 32 keys per step, 8 warps of 4 rows.  Scores: a lane per key, q rows broadcast
 // from shared memory; output: a lane per E / 32 columns.  K and V tiles are double-buffered
 // with cp.async (zero-filled where a key is not seen, so what lies there never matters).
-template <class T, int E> struct SimtCfg {
+template <int E> struct SimtCfg {
     static constexpr int KT = 32, MI = 32, THREADS = 256;
-    static constexpr int ROW = E * (int)sizeof(T) + 16;  // padded row, bytes
+    static constexpr int ROW = E * 4 + 16;  // padded row, bytes
     static constexpr size_t SMEM = (size_t)MI * (E + 4) * 4 + 4 * (size_t)KT * ROW + (size_t)MI * (KT + 4) * 4;
 };
 
 // key (f, l) of KV head h: its address, or null where there is none to read
-template <class T>
-__device__ __forceinline__ const T* tree_row(const TreeParams& p, const void* cache, const void* draft, int E, int w, int h,
-                                             const SplitWin& win, int l) {
+__device__ __forceinline__ const float* tree_row(const TreeParams& p, const void* cache, const void* draft, int E, int w, int h,
+                                                 const SplitWin& win, int l) {
     if (win.f == p.F) {
         // a drafted token that is not there is read as zeros
         if (!(__ldcg(p.anc + ((size_t)w * p.S + l) * p.SW + (l >> 5)) >> (l & 31) & 1u)) return nullptr;
-        return static_cast<const T*>(draft) + (((size_t)w * p.Hkv + h) * p.S + l) * E;
+        return static_cast<const float*>(draft) + (((size_t)w * p.Hkv + h) * p.S + l) * E;
     }
     const int pos = win.off + l;
     const int page = __ldg(p.bt + (size_t)w * p.maxb + pos / p.BS);
     if (page < 0 || page >= p.NB) return nullptr;
-    return static_cast<const T*>(cache) + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E;
+    return static_cast<const float*>(cache) + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E;
 }
 
-template <class T, int N>
-__device__ __forceinline__ void load_n(const void* src, float (&v)[N]) {
+template <int N> __device__ __forceinline__ void load_n(const float* src, float (&v)[N]) {  // N * 4 bytes aligned, up to 16
+    if constexpr (N == 2) {
+        const float2 x = *reinterpret_cast<const float2*>(src);
+        v[0] = x.x, v[1] = x.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = Elem<T>::to_f(static_cast<const T*>(src)[i]);
+        for (int i = 0; i < N; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(src + i);
+            v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+        }
+    }
 }
 
-template <class T, int E>
-__global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeParams p) {
-    using C = SimtCfg<T, E>;
-    constexpr int KT = C::KT, MI = C::MI, ROW = C::ROW, CH = E * (int)sizeof(T) / 16, VC = E / 32;
-    constexpr int PER = 16 / (int)sizeof(T);
+template <int E> __global__ void __launch_bounds__(SimtCfg<E>::THREADS) tree_simt_kernel(TreeParams p) {
+    using C = SimtCfg<E>;
+    constexpr int KT = C::KT, MI = C::MI, ROW = C::ROW, CH = E / 4, VC = E / 32;
     extern __shared__ __align__(16) uint8_t smem[];
     float* sQ = reinterpret_cast<float*>(smem);                        // [MI][E + 4]
     uint8_t* sK = smem + (size_t)MI * (E + 4) * 4;                     // [2][KT] rows
@@ -167,14 +171,14 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
             ld.seek(p, pc.w, i);
             for (int c = tid; c < KT * CH; c += C::THREADS) {
                 const int r = c / CH, ch = c - r * CH;
-                const T* kp = nullptr;
-                const T* vp = nullptr;
+                const float* kp = nullptr;
+                const float* vp = nullptr;
                 if (r < ld.n) {
-                    kp = tree_row<T>(p, p.k, p.dkr, E, pc.w, h, ld, ld.k0 + r);
-                    vp = tree_row<T>(p, p.v, p.dv, E, pc.w, h, ld, ld.k0 + r);
+                    kp = tree_row(p, p.k, p.dkr, E, pc.w, h, ld, ld.k0 + r);
+                    vp = tree_row(p, p.v, p.dv, E, pc.w, h, ld, ld.k0 + r);
                 }
-                cp_async16_zfill(smem_u32(sK + (st * KT + r) * ROW + ch * 16), kp ? kp + ch * PER : static_cast<const T*>(p.k), kp ? 16 : 0);
-                cp_async16_zfill(smem_u32(sV + (st * KT + r) * ROW + ch * 16), vp ? vp + ch * PER : static_cast<const T*>(p.v), vp ? 16 : 0);
+                cp_async16_zfill(smem_u32(sK + (st * KT + r) * ROW + ch * 16), kp ? kp + ch * 4 : static_cast<const float*>(p.k), kp ? 16 : 0);
+                cp_async16_zfill(smem_u32(sV + (st * KT + r) * ROW + ch * 16), vp ? vp + ch * 4 : static_cast<const float*>(p.v), vp ? 16 : 0);
             }
             cp_async_commit();
         };
@@ -205,10 +209,10 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
             const int qt = win.f < p.F ? win.f : p.F - 1;  // the turn whose rotation q takes
             if (qt != turn) {
                 turn = qt;
-                const T* qr = static_cast<const T*>(p.qr) + (((size_t)qt * p.W + pc.w) * p.Hkv + h) * p.rows * E;
+                const float* qr = static_cast<const float*>(p.qr) + (((size_t)qt * p.W + pc.w) * p.Hkv + h) * p.rows * E;
                 for (int c = tid; c < MI * E; c += C::THREADS) {
                     const int r = c / E, e = c - r * E, rr = pc.t * MI + r;
-                    sQ[r * (E + 4) + e] = rr < p.rows ? Elem<T>::to_f(__ldcg(qr + (size_t)rr * E + e)) : 0.f;
+                    sQ[r * (E + 4) + e] = rr < p.rows ? __ldcg(qr + (size_t)rr * E + e) : 0.f;
                 }
             }
             if (win.f < p.F)
@@ -220,18 +224,16 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
             float sc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
             for (int ch = 0; ch < CH; ++ch) {
-                float kv[PER];
-                load_n<T, PER>(sK + (st * KT + lane) * ROW + ch * 16, kv);
+                float kv[4];
+                load_n(reinterpret_cast<const float*>(sK + (st * KT + lane) * ROW + ch * 16), kv);
 #pragma unroll
-                for (int a = 0; a < 4; ++a)
-#pragma unroll
-                    for (int e = 0; e < PER; e += 4) {
-                        const float4 q4 = *reinterpret_cast<const float4*>(sQ + (wid * 4 + a) * (E + 4) + ch * PER + e);
-                        sc[a] = fmaf(q4.x, kv[e], sc[a]);
-                        sc[a] = fmaf(q4.y, kv[e + 1], sc[a]);
-                        sc[a] = fmaf(q4.z, kv[e + 2], sc[a]);
-                        sc[a] = fmaf(q4.w, kv[e + 3], sc[a]);
-                    }
+                for (int a = 0; a < 4; ++a) {
+                    const float4 q4 = *reinterpret_cast<const float4*>(sQ + (wid * 4 + a) * (E + 4) + ch * 4);
+                    sc[a] = fmaf(q4.x, kv[0], sc[a]);
+                    sc[a] = fmaf(q4.y, kv[1], sc[a]);
+                    sc[a] = fmaf(q4.z, kv[2], sc[a]);
+                    sc[a] = fmaf(q4.w, kv[3], sc[a]);
+                }
             }
             const int key = win.k0 + lane;
 #pragma unroll
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     float vv[VC];
-                    load_n<T, VC>(sV + (st * KT + k4 + u) * ROW + lane * VC * (int)sizeof(T), vv);
+                    load_n(reinterpret_cast<const float*>(sV + (st * KT + k4 + u) * ROW) + lane * VC, vv);
 #pragma unroll
                     for (int a = 0; a < 4; ++a)
 #pragma unroll
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(SimtCfg<T, E>::THREADS) tree_simt_kernel(TreeP
             const size_t orow = ((size_t)pc.w * p.Hq + hq) * p.S + tok[a];
             if (whole) {
 #pragma unroll
-                for (int c = 0; c < VC; ++c) static_cast<T*>(p.out)[orow * E + lane * VC + c] = Elem<T>::from_f(o[a][c] * inv);
+                for (int c = 0; c < VC; ++c) static_cast<float*>(p.out)[orow * E + lane * VC + c] = o[a][c] * inv;
                 if (p.lse_out && lane == 0) p.lse_out[orow] = lse2 * kLn2;
             } else {
 #pragma unroll
@@ -390,20 +392,20 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
 // ---------------------------------------------------------------------------------------
 constexpr int kTreeMaxTokens = 1024;
 
-template <class T, int E> static TreeKernel simt_kernel() {
+template <int E> static TreeKernel simt_kernel() {
     TreeKernel k{};
-    k.fn = (const void*)&tree_simt_kernel<T, E>;
-    k.threads = SimtCfg<T, E>::THREADS;
-    k.kt = SimtCfg<T, E>::KT;
-    k.mi = SimtCfg<T, E>::MI;
-    k.smem = SimtCfg<T, E>::SMEM;
+    k.fn = (const void*)&tree_simt_kernel<E>;
+    k.threads = SimtCfg<E>::THREADS;
+    k.kt = SimtCfg<E>::KT;
+    k.mi = SimtCfg<E>::MI;
+    k.smem = SimtCfg<E>::SMEM;
     k.least = 1;  // 1024 keys, 4 tokens: 29 us, with 2 and 4 windows 33 and 45: a window takes it 4 us
     k.ctas = E == 256 ? 1 : E == 128 ? 2 : 4;  // by their shared memory: 170, 90, 49 KB
     return k;
 }
 static TreeKernel tree_pick(const dvattn_tree_args* a) {
     if (a->dtype != DVATTN_FLOAT32) return tree_tc_pick(a->dtype, a->E, a->S * (a->Hq / a->Hkv));
-    return a->E == 64 ? simt_kernel<float, 64>() : a->E == 128 ? simt_kernel<float, 128>() : simt_kernel<float, 256>();
+    return a->E == 64 ? simt_kernel<64>() : a->E == 128 ? simt_kernel<128>() : simt_kernel<256>();
 }
 
 // DVATTN_TEST_STALL_TILE=<i>: tests only (see the decode launcher); read once per process.
@@ -431,7 +433,9 @@ static int tree_validate(const dvattn_tree_args* a) {
     if (a->S > kTreeMaxTokens) return DVATTN_ERR_UNSUPPORTED;
     // grid limits: sequences are the prep grid's x, row blocks its y; items are the merge grid's x
     const long long rows = (long long)a->S * (a->Hq / a->Hkv);
-    if ((long long)a->F * a->W * a->Hq * a->S > 0x7fffffffLL || tree_prep_chunks(a) > 65534LL * kPrepChunks || (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
+    if ((long long)a->F * a->W * a->Hq * a->S > 0x7fffffffLL || tree_prep_chunks(a) > 65534LL * kPrepChunks ||
+        (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL)
+        return DVATTN_ERR_UNSUPPORTED;
     return DVATTN_OK;
 }
 
