@@ -13,8 +13,12 @@
 // are, the CTA runs its windows again for each pass of rows.  Every wait is bounded (see
 // tree_tc.cu); a call that gave up leaves the error word set, its sums unfinished.
 //
-// Bound: few rows (a decode step) HBM, 128 keys x E x 2 bytes a window; many rows the exponentials,
-// 16 a clock and SM, at 128 x E x 2 flops each.
+// Bound: few rows, HBM: a decode step of 32 sequences, 154 MB, takes 35 us, 68% of its copy rate (88%
+// with 128 sequences).  Many rows, the sums: 496 rows over 4 x 26000 keys take 176 us; the SFU,
+// 16 exponentials a clock and SM, is busy for two thirds of the time, the tensor core for a
+// third.  Twice the warps for the sums (177 us), a share of the exponentials as polynomials on
+// the FMA pipe (an eighth 178 us, a quarter 185), and score buffers that are given back as soon as
+// they are read (182) do not help; two scores' loads in flight across jobs cost registers (245).
 #include <type_traits>
 
 #include "mass.cuh"
@@ -22,14 +26,13 @@
 
 namespace dvb {
 
-template <int E, bool BIG> struct MassCfg {
-    static constexpr int KT = 128, NP = E / 64;
-    // rows of a pass: query tile sets of 8 to 64 KB next to the groups' K rings
-    static constexpr int ROWS = BIG ? (E == 64 ? 512 : E == 128 ? 256 : 128) : 64;
-    static constexpr int Q_SETS = BIG || E == 256 ? 1 : 2;
+// ROWS: query rows of a pass, a tile set of 8 to 128 KB next to the groups' K rings.
+template <int E, int ROWS_> struct MassCfg {
+    static constexpr int KT = 128, NP = E / 64, ROWS = ROWS_;
+    static constexpr int Q_SETS = ROWS > 64 || E == 256 ? 1 : 2;
     static constexpr int PARTS = E == 256 ? 2 : 1;  // a K window of head dim 256 comes in two tiles
     static constexpr int QPANEL = ROWS * 128, KPANEL = KT * 128, QTILE = NP * QPANEL, KTILE = NP / PARTS * KPANEL;
-    static constexpr int K_STAGES = E == 64 ? 4 : BIG ? 2 : 3;  // of a group
+    static constexpr int K_STAGES = E == 64 ? 4 : QTILE > 65536 ? 1 : QTILE > 32768 ? 2 : 3;  // of a group
     static constexpr int ROWDATA = 2 * ROWS * 4;  // nlse, lim
     static constexpr int OFF_K = Q_SETS * QTILE, OFF_ROW = OFF_K + 2 * K_STAGES * KTILE, OFF_BAR = OFF_ROW + Q_SETS * ROWDATA;
     static constexpr int OFF_MISC = OFF_BAR + 48 * 8, OFF_RUN = OFF_MISC + 32, SMEM = OFF_RUN + RUN_RING * (int)sizeof(SplitRun);
@@ -37,9 +40,9 @@ template <int E, bool BIG> struct MassCfg {
     static_assert(SMEM <= 232448, "more shared memory than a CTA may use");
 };
 
-template <class T, int E, bool BIG>
-__global__ void __launch_bounds__(MassCfg<E, BIG>::NT, 1) mass_tc_kernel(MassParams p, const __grid_constant__ MassMaps maps) {
-    using C = MassCfg<E, BIG>;
+template <class T, int E, int ROWS>
+__global__ void __launch_bounds__(MassCfg<E, ROWS>::NT, 1) mass_tc_kernel(MassParams p, const __grid_constant__ MassMaps maps) {
+    using C = MassCfg<E, ROWS>;
     constexpr int KT = C::KT, KS = E / 16 / C::PARTS;  // MMA steps of a tile
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -277,15 +280,17 @@ __global__ void __launch_bounds__(MassCfg<E, BIG>::NT, 1) mass_tc_kernel(MassPar
     if (wid == C::WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-template <class T, int E, bool BIG> static MassKernel mass_tc() {
-    using C = MassCfg<E, BIG>;
-    return MassKernel{(const void*)&mass_tc_kernel<T, E, BIG>, C::NT, C::KT, 1, C::ROWS, (size_t)C::SMEM};
+template <class T, int E, int ROWS> static MassKernel mass_tc() {
+    using C = MassCfg<E, ROWS>;
+    return MassKernel{(const void*)&mass_tc_kernel<T, E, ROWS>, C::NT, C::KT, 1, C::ROWS, (size_t)C::SMEM};
 }
 template <class T> static MassKernel mass_tc_e(int E, int rows) {
-    // the smaller query tiles leave more of the shared memory to the K ring
-    if (E == 64) return rows <= MassCfg<64, false>::ROWS ? mass_tc<T, 64, false>() : mass_tc<T, 64, true>();
-    if (E == 128) return rows <= MassCfg<128, false>::ROWS ? mass_tc<T, 128, false>() : mass_tc<T, 128, true>();
-    return rows <= MassCfg<256, false>::ROWS ? mass_tc<T, 256, false>() : mass_tc<T, 256, true>();
+    // The smaller query tiles leave more of the shared memory to the K rings, the larger ones run the
+    // windows fewer times: head dim 128, 128 rows 57 us with tiles of 256 rows and 61 with 512, 496
+    // rows 186 and 176.
+    if (E == 64) return rows <= 64 ? mass_tc<T, 64, 64>() : mass_tc<T, 64, 512>();
+    if (E == 128) return rows <= 64 ? mass_tc<T, 128, 64>() : rows <= 256 ? mass_tc<T, 128, 256>() : mass_tc<T, 128, 512>();
+    return rows <= 64 ? mass_tc<T, 256, 64>() : mass_tc<T, 256, 128>();
 }
 MassKernel mass_tc_pick(int dtype, int E, int rows) { return dtype == DVATTN_FLOAT16 ? mass_tc_e<__half>(E, rows) : mass_tc_e<__nv_bfloat16>(E, rows); }
 

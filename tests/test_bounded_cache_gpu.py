@@ -113,6 +113,16 @@ def test_mass_repeats_streams_and_c_abi():
     assert torch.equal(a, b) and torch.equal(a, d) and torch.equal(a, m)
 
 
+@pytest.mark.parametrize("E", [64, 128, 256])
+@pytest.mark.parametrize("S", [5, 8, 9, 17, 33, 35, 67])
+def test_mass_repeats_with_row_passes(E, S):
+    """Rows of one and several passes, with an odd number of row tiles: a key's sum has one order."""
+    c = make([[2500, 1100], [40, 1700]], S, 16, 1, E, 64, 16, F16, seed=S)
+    a = add_mass(c)
+    assert all(torch.equal(a, add_mass(c)) for _ in range(3))
+    check(c)
+
+
 def test_mass_of_a_decode_sums_to_the_queries():
     """With the lse of the attention call itself, the weights of every query add up to one."""
     c = wl.make_paged([[500, 77], [64, 300]], 32, 2, 128, 64, 16, BF16, seed=4, device=DEV)
