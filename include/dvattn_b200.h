@@ -272,7 +272,7 @@ typedef struct dvattn_evict_args {
     int max_blocks_per_seq;
     int sink, recent;
     long long num_blocks;
-    long long positions;          /* mass.size(2); the range is cut off there            */
+    long long positions;          /* mass.size(2) <= 0x7fff0000; the range is cut off there */
     void* k_cache;                /* [NB,BS,Hkv,E] T, rows moved                         */
     void* v_cache;                /* [NB,BS,Hkv,Ev] T, rows moved                        */
     const float* mass;            /* [W,Hkv,positions] f32                               */
@@ -345,13 +345,14 @@ int dvattn_paged_sdpa_noalloc(const dvattn_paged_args* args, dvattn_stream_t str
 
 /*
  * Error word of the last attention call that used `workspace` (dvattn_paged_sdpa,
- * dvattn_varlen_paged_sdpa, dvattn_sdpa and their *_rope / *_phase forms), or, with
- * workspace == NULL, of the last dvattn_paged_sdpa_noalloc call on the current device.
- * Waits for `stream` (call it after the attention call, before the next call on the same
+ * dvattn_varlen_paged_sdpa, dvattn_sdpa and their *_rope / *_phase forms, dvattn_tree_sdpa,
+ * dvattn_paged_mass), or, with workspace == NULL, of the last dvattn_paged_sdpa_noalloc call
+ * on the current device.  Waits for `stream` (call it after the attention call, before the next call on the same
  * workspace).  *error_word == 0: the call completed.  Nonzero: a bounded wait inside a
  * kernel gave up (~2 s; bit 1 loader, bit 2 / 8 compute warps, bit 4 bad shared-memory
- * alignment) and that call's outputs are invalid; the paged decode writes NaN to all of
- * them, the tensor-core prefill to the rows of the items that gave up.  The reference
+ * alignment) and that call's outputs are invalid; the paged decode and the draft-tree
+ * attention write NaN to all of them, the tensor-core prefill to the rows of the items that
+ * gave up, dvattn_paged_mass leaves its sums unfinished.  The reference
  * reports kernel failures as a RuntimeError from C10_CUDA_CHECK (src/binding.cu:200,
  * src/cuda_check.cuh:16-29); its kernels have no waits that can give up.
  */
