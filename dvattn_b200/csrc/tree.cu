@@ -19,12 +19,12 @@ namespace dvb {
 // Block (w, 0) finds sequence w's ancestor sets, what each token sees of each turn and the
 // spans; the others rotate its queries for every turn and its drafted keys, once for all the
 // CTAs that read them.  Reads and writes (F + 1 parts of Hkv rows) a few percent of a call's
-// bytes; done by the attention kernel's own threads, the rotation stood between two pieces of
-// its work for 5 us and more.
-constexpr int kPrepChunks = 512;  // 16-byte chunks of a rotating block, two a thread
+// bytes, 6 us for one turn and one more per turn; done by the attention kernel's own threads, the
+// rotation stood between two pieces of its work for 5 us and more.
+constexpr int kPrepChunks = 256;  // 16-byte chunks of a rotating block
 
 template <class T>
-__global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
+__global__ void __launch_bounds__(256, 4) tree_prep_kernel(TreeParams p, int E) {
     extern __shared__ int par[];  // [S] parents, then [S] whether a token is there
     asm volatile("griddepcontrol.wait;" ::: "memory");  // a programmatic dependent of whatever is before it
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -79,35 +79,26 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(TreeParams p, int E) {
         }
         return;
     }
-    // chunks of rows: the drafted keys [Hkv][S], then the queries [F][Hkv][rows]
-    const int keys = p.Hkv * p.S, per = E * (int)sizeof(T) / 16, all = (keys + p.F * p.Hkv * p.rows) * per;
-    const int first = (blockIdx.y - 1) * kPrepChunks;
-    RotateChunk<T> ch[kPrepChunks / 256];
-#pragma unroll
-    for (int k = 0; k < kPrepChunks / 256; ++k) {
-        const int c = first + 256 * k + tid;
-        if (c >= all) break;
-        const int x = c / per, e0 = (c - x * per) * RotateChunk<T>::PER;
-        const T* src;
-        T* dst;
-        int f = p.F - 1, s;
-        if (x < keys) {
-            s = x % p.S;
-            src = static_cast<const T*>(p.dk) + ((size_t)w * keys + x) * E;
-            dst = static_cast<T*>(p.dkr) + ((size_t)w * keys + x) * E;
-        } else {
-            const int y = x - keys, h = y / p.rows % p.Hkv, r = y % p.rows;
-            f = y / p.rows / p.Hkv;
-            s = r / p.G;
-            src = static_cast<const T*>(p.q) + (((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s) * E;
-            dst = static_cast<T*>(p.qr) + ((((size_t)f * p.W + w) * p.Hkv + h) * p.rows + r) * E;
-        }
-        const size_t cs = (((size_t)f * p.W + w) * p.S + s) * p.R;
-        ch[k].load(src, dst, p.cos + cs, p.sin + cs, e0, p.R, p.rot_vec);
+    // a chunk a thread: of the drafted keys [Hkv][S], for the last turn, or of the queries
+    // [Hkv][rows], for every turn
+    const int keys = p.Hkv * p.S, per = E * (int)sizeof(T) / 16, all = (keys + p.Hkv * p.rows) * per;
+    const int c = (blockIdx.y - 1) * kPrepChunks + tid;
+    if (c >= all) return;
+    const int x = c / per, e0 = (c - x * per) * RotateChunk<T>::PER;
+    const bool key = x < keys;
+    const int y = x - keys, h = y / p.rows, r = y - h * p.rows, s = key ? x % p.S : r / p.G;
+    const T* src = key ? static_cast<const T*>(p.dk) + ((size_t)w * keys + x) * E
+                       : static_cast<const T*>(p.q) + (((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s) * E;
+    T* dst = key ? static_cast<T*>(p.dkr) + ((size_t)w * keys + x) * E : static_cast<T*>(p.qr) + (((size_t)w * p.Hkv + h) * p.rows + r) * E;
+    RotateChunk<T> ch;
+    ch.load_row(src, e0, p.R, p.rot_vec);
+    int f = key ? p.F - 1 : 0;
+    for (size_t angle = (((size_t)f * p.W + w) * p.S + s) * p.R; f < p.F; ++f) {
+        ch.load_angles(dst, p.cos + angle, p.sin + angle, p.R, p.rot_vec);
+        ch.store(p.R, p.rot_vec);
+        dst += (size_t)p.W * p.Hkv * p.rows * E;
+        angle += (size_t)p.W * p.S * p.R;
     }
-#pragma unroll
-    for (int k = 0; k < kPrepChunks / 256; ++k)
-        if (first + 256 * k + tid < all) ch[k].store(p.R, p.rot_vec);
 }
 
 // ---- CUDA-core attention, 32-bit types -----------------------------------------------------
@@ -305,8 +296,10 @@ template <int E> __global__ void __launch_bounds__(SimtCfg<E>::THREADS) tree_sim
 // partials, in group order.  E / 4 lanes per row, two rows each.  Everything but the partials
 // is known before the attention kernel ends (the prep kernel has ended when this one is
 // launched); after the wait the sums and columns of up to kMergeAhead partials are read in one
-// round trip.  A call whose error word is set gets NaN in every output.
-constexpr int kMergeAhead = 8;
+// round trip.  Four at a time leave 48 registers and more resident blocks: 32 sequences 89 us, with
+// eight (66 registers) 94; one sequence in 33 parts 30 and 29.  A call whose error word is set gets
+// NaN in every output.
+constexpr int kMergeAhead = 4;
 
 template <class T, int E>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
@@ -417,9 +410,9 @@ static int tree_stall_hook() {
     return t;
 }
 
-// 16-byte chunks of a sequence's drafted keys and of its queries for every turn.
+// 16-byte chunks of a sequence's drafted keys and of its queries.
 static long long tree_prep_chunks(const dvattn_tree_args* a) {
-    return ((long long)a->F * a->Hq + a->Hkv) * a->S * (a->E * (a->dtype == DVATTN_FLOAT32 ? 4 : 2) / 16);
+    return ((long long)a->Hq + a->Hkv) * a->S * (a->E * (a->dtype == DVATTN_FLOAT32 ? 4 : 2) / 16);
 }
 
 static int tree_validate(const dvattn_tree_args* a) {

@@ -16,10 +16,10 @@
 // rows that nobody sees never matters: their scores are masked, and their V rows are zeroed
 // before PV (0 * NaN is NaN).
 //
-// Measured with prep and merge: 32 sequences of two turns, 64/4 heads, 8 tokens, 337 MB: 94 us, 55%
+// Measured with prep and merge: 32 sequences of two turns, 64/4 heads, 8 tokens, 337 MB: 89 us, 59%
 // of HBM's copy rate (203 with one CTA per SM, rows gathered and rotated by its own threads); the
 // stream alone reaches 89% with 128 rows, 98% with 32.  4 sequences of up to 131072 keys, 128/8
-// heads, 16 tokens (two tiles): 583 us, 658 TFLOP/s, 4325 cycles per 128-key window at the 1.5 GHz
+// heads, 16 tokens (two tiles): 572 us, 671 TFLOP/s, 4325 cycles per 128-key window at the 1.5 GHz
 // that the power limit leaves; tensor core and SFU are each busy for a third of the time.
 //
 // Every wait is bounded; one that gives up sets the call's error word, ends the CTA with
@@ -380,6 +380,8 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
                     const float mu = mnew == neg_inf() ? 0.f : mnew;
                     const uint64_t sc2 = f2u(sl2, sl2), nmu2 = f2u(-mu, -mu);
                     uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
+                    // P is rounded to T, the tensor core's operand next to V (half an ulp of T a
+                    // weight, as in the paged decode); the sum is of the unrounded weights
 #pragma unroll
                     for (int c = 0; c < KT / 32; ++c) {
                         uint32_t pk[16];

@@ -244,7 +244,7 @@ __device__ __forceinline__ bool split_schedule(const TurnSplit& p, int lane, int
 // x[e + R/2] s[e], o[e + R/2] = x[e + R/2] c[e] + x[e] s[e] for e < R/2 (the first half of the
 // cos/sin row), separate roundings of the products and of the sum, one rounding to T: the bits
 // of the paged append.  load() issues the chunk's reads, store() computes and writes, so that a
-// thread can have several chunks in flight.
+// thread can have several chunks in flight; load_angles() begins another rotation of the same row.
 template <class T> struct RotateChunk {
     static constexpr int PER = 16 / (int)sizeof(T);
     uint4 a, b;
@@ -254,11 +254,19 @@ template <class T> struct RotateChunk {
     const float *cos, *sin;
     int e0;
     __device__ __forceinline__ void load(const T* x_, T* y_, const float* cos_, const float* sin_, int e0_, int R, bool vec) {
-        x = x_, y = y_, cos = cos_, sin = sin_, e0 = e0_;
+        load_row(x_, e0_, R, vec);
+        load_angles(y_, cos_, sin_, R, vec);
+    }
+    __device__ __forceinline__ void load_row(const T* x_, int e0_, int R, bool vec) {
+        x = x_, e0 = e0_;
         a = __ldg(reinterpret_cast<const uint4*>(x + e0));
-        if (e0 < R && vec) {  // rotary halves are whole chunks, cos/sin rows 16-byte aligned
+        // vec: rotary halves are whole chunks, cos/sin rows 16-byte aligned
+        if (e0 < R && vec) b = __ldg(reinterpret_cast<const uint4*>(x + (e0 < R >> 1 ? e0 + (R >> 1) : e0 - (R >> 1))));
+    }
+    __device__ __forceinline__ void load_angles(T* y_, const float* cos_, const float* sin_, int R, bool vec) {
+        y = y_, cos = cos_, sin = sin_;
+        if (e0 < R && vec) {
             const int half = R >> 1, j = e0 < half ? e0 : e0 - half;
-            b = __ldg(reinterpret_cast<const uint4*>(x + (e0 < half ? e0 + half : j)));
 #pragma unroll
             for (int u = 0; u < PER / 4; ++u) {
                 c[u] = __ldg(reinterpret_cast<const float4*>(cos + j) + u);
