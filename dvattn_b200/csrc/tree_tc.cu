@@ -57,6 +57,14 @@ template <int E, bool TWO> struct TcCfg {
     static constexpr int COLS = CTAS == 2 ? 256 : 512, TM_O = CTAS == 2 ? 128 : 256;
 };
 
+// How far (log2) the softmax's reference point lies below the maximum it was taken from.  fp16 is
+// normal down to 2^-14 and zero below 2^-25: weights relative to the maximum itself lose their bits
+// 10 nats under it and are gone at 17, where a long context still has thousands of keys, while the
+// sum counts them.  With the maximum 8 above the reference at most, 2^15 is the largest weight, and a
+// weight is rounded by half an ulp or by 2^-32 of the row's largest one, whichever is more.
+template <class T> constexpr float kRefBelow = 0.f;  // bf16 has the range of the sums
+template <> constexpr float kRefBelow<__half> = 7.f;
+
 // 32 bytes in one store (the address a multiple of 32).
 __device__ __forceinline__ void store_sector(void* dst, const uint32_t* v) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
@@ -372,7 +380,7 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
                     for (int c = 8; c < KT; c += 16)
 #pragma unroll
                         for (int u = 0; u < 8; ++u) mx[u] = fmax3(mx[u], sv[c + u], sv[c + 8 + u < KT ? c + 8 + u : c + u]);
-                    const float mxs = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * sl2;
+                    const float mxs = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * sl2 - kRefBelow<T>;
                     // the reference point moves only when the maximum grows by more than 8 (a
                     // factor 256 in the exponentials); the result is exact either way
                     const float mnew = mxs > m + 8.f ? mxs : m;
@@ -381,7 +389,7 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
                     const uint64_t sc2 = f2u(sl2, sl2), nmu2 = f2u(-mu, -mu);
                     uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
                     // P is rounded to T, the tensor core's operand next to V (half an ulp of T a
-                    // weight, as in the paged decode); the sum is of the unrounded weights
+                    // weight, and see kRefBelow); the sum is of the unrounded weights
 #pragma unroll
                     for (int c = 0; c < KT / 32; ++c) {
                         uint32_t pk[16];

@@ -187,6 +187,37 @@ def test_large_scores(dtype):
     check(c, "negative scale")
 
 
+@pytest.mark.parametrize("nats", [15.0, 16.0, 17.0, 18.03])
+@pytest.mark.parametrize("E,S,G", [(64, 1, 4), (128, 1, 4), (256, 1, 4), (64, 33, 4), (128, 33, 4)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_one_key_far_above_many(dtype, E, S, G, nats):
+    """A key whose value is zero, and thousands of keys that far below it whose values have one sign: their
+    weights are small for the type, their sum is the result.  Many sequences share the pages, so that a
+    sequence's keys are one block's work."""
+    W, n, BS = 300, 20000, 64
+    pages = -(-n // BS)
+    g = torch.Generator().manual_seed(E + S)
+    kc = torch.zeros((pages, BS, 1, E), dtype=dtype)
+    vc = (0.5 + torch.rand((pages, BS, 1, E), generator=g)).to(dtype)
+    dv = (0.5 + torch.rand((1, 1, S, E), generator=g)).to(dtype)
+    kc[0, 0, 0, 0], vc[0, 0] = nats, 0
+    q = torch.zeros((W, G, S, E), dtype=dtype)
+    q[..., 0] = 1
+    none = torch.zeros((1, W, S, 0))
+    c = dict(q=q, parents=torch.full((W, S), -1, dtype=torch.int32), loc=torch.full((1, W, S), n - 1, dtype=torch.int32), cos=none, sin=none,
+             L=torch.tensor([n], dtype=torch.int32), kc=kc, vc=vc, bt=torch.arange(pages, dtype=torch.int32).repeat(W, 1), scale=1.0,
+             dk=torch.zeros((W, 1, S, E), dtype=dtype), dv=dv.repeat(W, 1, 1, 1))
+    out, lse = call(on_gpu(c))
+    top = math.exp(float(kc[0, 0, 0, 0]))
+    total = top + n  # the dominant key, n - 1 others and the token itself
+    ref = (vc.reshape(-1, E)[:n].double().sum(0) + dv[0, 0].double()) / total  # [S, E]
+    bound = plain64.out_bound(c, ref, ref, n + 1)
+    if dtype == F16:  # a weight's rounding is at most 2^-32 of the largest weight where fp16 is subnormal
+        bound = bound + n * 2.0 ** -32 * 1.5
+    assert bool(((out.double().cpu() - ref).abs() <= bound).all())
+    assert bool(((lse.double().cpu() - math.log(total)).abs() <= plain64.lse_bound(c, torch.tensor(math.log(total)).double(), n + 1)).all())
+
+
 def test_equal_to_a_causal_decode_of_the_appended_chain():
     """A chain of drafts gives what the paged decode gives once the chain is in the cache."""
     S = 5
