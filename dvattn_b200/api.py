@@ -160,7 +160,7 @@ def dvattn_tree_sdpa(queries: torch.Tensor, parents: torch.Tensor, locations: to
     parent among the S (before it), -1 for a child of the cached context, -2 for no token
     (padding; gets zeros).  locations [F,W,S] i32: the last cached key of each turn that the
     token sees (not its own position); cos/sin [F,W,S,R] f32 rotate its query for each turn,
-    those of the last turn its key as well.  -> out [W,Hq,S,E]; ``lse`` ([W,Hq,S] f32) is an
+    those of the last turn its key as ``dvattn_tree_append`` does.  -> out [W,Hq,S,E]; ``lse`` ([W,Hq,S] f32) is an
     optional extra output.  The cache is not written (``dvattn_tree_append`` does that for
     the accepted tokens)."""
     if out is None:

@@ -3,7 +3,8 @@
 //
 //   out[w, h, s] = sum_j softmax_j(scale * q . k_j) v_j  over the cached keys that
 //   (w, s) sees in every turn (q rotated for that turn) and the drafted keys of s's
-//   ancestors and of s itself (q and key rotated with their own angles in the last turn).
+//   ancestors and of s itself (q and key rotated with their own angles in the last turn, the key
+//   as tree_append.cu writes it).
 //
 // Three launches: tree_prep_kernel (ancestor sets, visible spans, rotated drafted keys),
 // the attention kernel, and tree_merge_kernel, each a programmatic dependent of the one
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(256, 4) tree_prep_kernel(TreeParams p, int E) 
                        : static_cast<const T*>(p.q) + (((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s) * E;
     T* dst = key ? static_cast<T*>(p.dkr) + ((size_t)w * keys + x) * E : static_cast<T*>(p.qr) + (((size_t)w * p.Hkv + h) * p.rows + r) * E;
     RotateChunk<T> ch;
-    ch.load_row(src, e0, p.R, p.rot_vec);
+    ch.load_row(src, e0, p.R, p.rot_vec, key);
     int f = key ? p.F - 1 : 0;
     for (size_t angle = (((size_t)f * p.W + w) * p.S + s) * p.R; f < p.F; ++f) {
         ch.load_angles(dst, p.cos + angle, p.sin + angle, p.R, p.rot_vec);

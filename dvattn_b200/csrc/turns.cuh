@@ -241,9 +241,10 @@ __device__ __forceinline__ bool split_schedule(const TurnSplit& p, int lane, int
 }
 
 // A 16-byte chunk (elements e0...) of a row rotated by apply_rotary_pos_emb: o[e] = x[e] c[e] -
-// x[e + R/2] s[e], o[e + R/2] = x[e + R/2] c[e] + x[e] s[e] for e < R/2 (the first half of the
-// cos/sin row), separate roundings of the products and of the sum, one rounding to T: the bits
-// of the paged append.  load() issues the chunk's reads, store() computes and writes, so that a
+// x[e + R/2] s[e], o[e + R/2] = x[e + R/2] c[y] + x[e] s[y] for e < R/2, separate roundings of the
+// products and of the sum, one rounding to T.  Queries take y = e (the first half of the cos/sin
+// row, as in the paged attention), keys y = e + R/2 (`full`: the whole row; the bits of the
+// paged append).  load() issues the chunk's reads, store() computes and writes, so that a
 // thread can have several chunks in flight; load_angles() begins another rotation of the same row.
 template <class T> struct RotateChunk {
     static constexpr int PER = 16 / (int)sizeof(T);
@@ -253,12 +254,13 @@ template <class T> struct RotateChunk {
     T* y;
     const float *cos, *sin;
     int e0;
+    int back;  // the angle of element e >= R/2 is entry e - back
     __device__ __forceinline__ void load(const T* x_, T* y_, const float* cos_, const float* sin_, int e0_, int R, bool vec) {
         load_row(x_, e0_, R, vec);
         load_angles(y_, cos_, sin_, R, vec);
     }
-    __device__ __forceinline__ void load_row(const T* x_, int e0_, int R, bool vec) {
-        x = x_, e0 = e0_;
+    __device__ __forceinline__ void load_row(const T* x_, int e0_, int R, bool vec, bool full = false) {
+        x = x_, e0 = e0_, back = full ? 0 : R >> 1;
         a = __ldg(reinterpret_cast<const uint4*>(x + e0));
         // vec: rotary halves are whole chunks, cos/sin rows 16-byte aligned
         if (e0 < R && vec) b = __ldg(reinterpret_cast<const uint4*>(x + (e0 < R >> 1 ? e0 + (R >> 1) : e0 - (R >> 1))));
@@ -266,7 +268,7 @@ template <class T> struct RotateChunk {
     __device__ __forceinline__ void load_angles(T* y_, const float* cos_, const float* sin_, int R, bool vec) {
         y = y_, cos = cos_, sin = sin_;
         if (e0 < R && vec) {
-            const int half = R >> 1, j = e0 < half ? e0 : e0 - half;
+            const int j = e0 < R >> 1 ? e0 : e0 - back;
 #pragma unroll
             for (int u = 0; u < PER / 4; ++u) {
                 c[u] = __ldg(reinterpret_cast<const float4*>(cos + j) + u);
@@ -289,8 +291,8 @@ template <class T> struct RotateChunk {
             }
         } else if (e0 < R) {  // element by element
             for (int u = 0; u < PER && e0 + u < R; ++u) {
-                const int e = e0 + u, j = e < half ? e : e - half;
-                const float v = Elem<T>::to_f(e < half ? x[e + half] : x[j]);
+                const int e = e0 + u, j = e < half ? e : e - back;
+                const float v = Elem<T>::to_f(e < half ? x[e + half] : x[e - half]);
                 o[u] = Elem<T>::from_f(__fadd_rn(__fmul_rn(Elem<T>::to_f(x[e]), __ldg(cos + j)), __fmul_rn(e < half ? -v : v, __ldg(sin + j))));
             }
         }

@@ -195,7 +195,8 @@ typedef struct dvattn_tree_args {
     void* out;                    /* [W,Hq,S,Ev] T                                       */
     const void* queries;          /* [W,Hq,S,E] T, unrotated                             */
     const int* parents;           /* [W,S] i32                                           */
-    const float* cosines;         /* [F,W,S,R] f32 (the first R/2 entries are read)      */
+    const float* cosines;         /* [F,W,S,R] f32: the first R/2 entries turn a query, all of
+                                     the last turn's a drafted key, as in dvattn_tree_append */
     const float* sines;
     const int* locations;         /* [F,W,S] i32                                         */
     const int* fragment_lengths;  /* [F] i32                                             */

@@ -246,6 +246,38 @@ def test_equal_to_a_causal_decode_of_the_appended_chain():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R", [24, 64])
+def test_drafted_keys_are_those_that_the_append_writes(dtype, R):
+    """cos/sin rows whose halves differ: a drafted key is turned by both, like the key that goes into the cache."""
+    S = 6
+    c = make([[90], [31]], S, 8, 2, 128, R, 16, dtype, seed=15, parents=[[-1, 0, 0, 1, 1, 2]] * 2)
+    g = torch.Generator().manual_seed(15)
+    c["cos"][..., R // 2:], c["sin"][..., R // 2:] = torch.rand((2,) + c["cos"][..., R // 2:].shape, generator=g)
+    out, lse = call(on_gpu(c))
+    cos, sin = c["cos"][0][:, None], c["sin"][0][:, None]
+    k, h = c["dk"].double(), R // 2
+    turned = k.clone()
+    turned[..., :h] = k[..., :h] * cos[..., :h].double() - k[..., h:R] * sin[..., :h].double()
+    turned[..., h:R] = k[..., h:R] * cos[..., h:].double() + k[..., :h] * sin[..., h:].double()
+    turned = turned.to(dtype).double()
+    sees = plain64.ancestors(c["parents"][0].tolist())
+    for w, n in enumerate((90, 31)):
+        for kv in range(2):
+            q = plain64.rotate(c["q"][w, 4 * kv:4 * kv + 4], c["cos"][0, w], c["sin"][0, w])
+            cached = plain64.scores(c, w, kv)[0][1]
+            z = torch.cat([cached, (c["scale"] * q @ turned[w, kv].T).masked_fill(~sees, -math.inf)], -1)
+            v = torch.cat([plain64.key_rows(c["vc"], c["bt"][w], 0, cached.size(-1), kv), c["dv"][w, kv].double()])
+            p = z.softmax(-1)
+            v = torch.where((p > 0).flatten(0, 1).any(0)[:, None], v, torch.zeros((), dtype=torch.float64))
+            got, got_lse = (t[w, 4 * kv:4 * kv + 4].double().cpu() for t in (out, lse))
+            # the rotated keys' own rounding: in 64 bits here, of 32-bit products there: an ulp of T of the
+            # rare element that lies between two, on a row of E elements
+            s = plain64.UNIT[dtype] * 2 * abs(c["scale"]) * float(q.norm(dim=-1).max()) * float(turned.abs().max())
+            assert bool(((got - p @ v).abs() <= plain64.out_bound(c, p @ v, p @ v.abs(), 96) + 2 * s * (p @ v.abs())).all())
+            assert bool(((got_lse - z.logsumexp(-1)).abs() <= plain64.lse_bound(c, z.logsumexp(-1), 96) + s).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_repeats_and_streams(dtype):
     """The same bits again, on another stream too, with a workspace full of another call's data."""
     a = on_gpu(make([[3000, 20], [40, 700]], 9, 8, 2, 128, 64, 16, dtype, seed=9))
