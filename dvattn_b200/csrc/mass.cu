@@ -19,7 +19,13 @@ namespace dvb {
 // ---- prep: block (w, 16-row tile of a KV head, turn) -----------------------------------
 // The queries rotated for every turn, once for all the CTAs that read them; what each row and
 // every row sees of the turn; the spans.
+//
+// The tensor-core kernel takes a window that every counted row sees without a mask, so what a row
+// without weight adds there has to vanish by itself.  Zeros with an lse of infinity would not, next to
+// a key that is not finite (0 * inf).  Such a row takes the query of one that counts, its twin,
+// and the most negative lse: 2^(score - most) is 0 wherever the twin's weight is finite.
 constexpr int kPrepRows = 16;
+constexpr float kMostFloat = 3.402823466e38f;
 
 template <class T>
 __global__ void __launch_bounds__(128) mass_prep_kernel(MassParams p, int E) {
@@ -70,8 +76,17 @@ __global__ void __launch_bounds__(128) mass_prep_kernel(MassParams p, int E) {
         const int r = r0 + tid;
         const float x = row_lse(r);
         const size_t wh = (size_t)w * p.Hkv + h;
-        if (f == 0) p.nlse[wh * p.rows_pad + r] = x == neg_inf() ? neg_inf() : -x * kLog2e;
+        if (f == 0) p.nlse[wh * p.rows_pad + r] = x == neg_inf() ? -kMostFloat : -x * kLog2e;
         p.lim[fwh * p.rows_pad + r] = x == neg_inf() ? 0 : seen(r / p.G);
+    }
+    const unsigned dead = __ballot_sync(0xffffffffu, lane < kPrepRows && row_lse(r0 + lane) == neg_inf());
+    int twin = p.rows;  // the first row of the head that gives weight
+    for (int b = 0; dead && b < p.rows && twin == p.rows; b += 32 * 8) {
+        int first = p.rows;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (row_lse(b + 32 * u + lane) != neg_inf()) first = min(first, b + 32 * u + lane);
+        twin = __reduce_min_sync(0xffffffffu, first);
     }
     constexpr int AHEAD = 2;  // chunks a thread has in flight
     const int per = E * (int)sizeof(T) / 16, n = kPrepRows * per;
@@ -83,9 +98,9 @@ __global__ void __launch_bounds__(128) mass_prep_kernel(MassParams p, int E) {
             const int c = c0 + 128 * k;
             counts[k] = false;
             if (c >= n) break;
-            const int r = r0 + c / per, s = r / p.G, e0 = c % per * RotateChunk<T>::PER;
-            T* dst = static_cast<T*>(p.qr) + (fwh * p.rows_pad + r) * E;
-            counts[k] = row_lse(r) != neg_inf();
+            const int own = r0 + c / per, r = dead >> (own - r0) & 1u ? twin : own, s = r / p.G, e0 = c % per * RotateChunk<T>::PER;
+            T* dst = static_cast<T*>(p.qr) + (fwh * p.rows_pad + own) * E;
+            counts[k] = r < p.rows;
             if (counts[k])
                 ch[k].load(static_cast<const T*>(p.q) + (((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s) * E, dst,
                            p.cos + (fw * p.S + s) * p.R, p.sin + (fw * p.S + s) * p.R, e0, p.R, p.rot_vec);

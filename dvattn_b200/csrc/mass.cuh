@@ -22,8 +22,8 @@ struct MassParams : TurnSplit {
     const float* cos;
     const float* sin;
     const void* k;
-    // workspace; a row past `rows`, or whose lse is -inf, gives no weight: its query is zeros,
-    // its nlse -inf, its lim 0
+    // workspace; a row past `rows`, or whose lse is -inf, gives no weight: its query is that of a row
+    // that does (zeros where none does), its nlse the lowest number, its lim 0
     int* header;  // [3] error word (kErrorWordOffset)
     void* qr;     // [F][W][Hkv][rows_pad][E] T, queries rotated for the turn
     float* nlse;  // [W][Hkv][rows_pad] -lse in log2 units

@@ -98,6 +98,28 @@ def test_mass_masks(dtype):
     check(c, "few positions")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E", [64, 256])
+@pytest.mark.parametrize("S,G", [(3, 5), (40, 16)])
+def test_mass_of_keys_that_are_not_finite(dtype, E, S, G):
+    """Next to queries that give no weight (taken out, or the padding of a row tile): a key with -inf where every
+    counted query is positive weighs nothing, a key with NaN gets NaN, and no other key does."""
+    c = make([[700]], S, G, 1, E, 0, 16, dtype, seed=E + S)
+    c["q"][..., 1] = 0.5 + c["q"][..., 1].abs().clamp(max=2)
+    rows = c["bt"][0].long()
+    for p in (5, 300, 640):
+        c["kc"][rows[p // 16], p % 16, 0, 1] = -math.inf
+    finite = torch.ones(c["mass"].shape, dtype=torch.bool)
+    lse = torch.cat([s for _, s in plain64.scores(c, 0, 0)], -1).logsumexp(-1)
+    c["lse"] = lse.reshape(1, G, S).float()
+    c["lse"][:, :, 1] = -math.inf
+    check(c)
+    c["kc"][rows[20], 3, 0, 2] = math.nan
+    finite[:, :, 20 * 16 + 3] = False
+    got = add_mass(c).double().cpu()
+    assert torch.equal(torch.isfinite(got), finite) and bool(torch.isnan(got[~finite]).all())
+
+
 def test_mass_repeats_streams_and_c_abi():
     c = make([[3000, 20], [40, 700]], 9, 8, 2, 128, 64, 16, BF16, seed=9)
     a, b = add_mass(c), add_mass(c)
