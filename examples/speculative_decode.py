@@ -2,9 +2,9 @@
 
 A step verifies a tree of drafted tokens for every sequence in one pass over its cache
 (dvattn_tree_sdpa), appends the tokens that the model itself would have chosen
-(dvattn_tree_append), adds what attention they paid to the cached keys (dvattn_paged_mass) and,
-once a sequence holds more keys than its budget, lets each KV head drop its least attended ones
-(dvattn_paged_evict).  Nothing in a step waits for the host.
+(dvattn_tree_append), adds what attention they paid to the cached keys, their own ones among
+them (dvattn_paged_mass), and, once a sequence holds more keys than its budget, lets each KV head
+drop its least attended ones (dvattn_paged_evict).  Nothing in a step waits for the host.
 
 The model is a toy, one attention layer with random weights: its logits are those of the draft
 (a table by token) plus a projection of the attention output.
@@ -110,10 +110,11 @@ class Decoder:
             counts += going[:, 0]
         path = torch.cat(path, 1).int()
         dvattn_b200.dvattn_tree_append(self.k, self.v, k, v, cos, sin, self.tables, self.cached, path, counts)
-        # only accepted tokens count as queries of the cached keys
+        # only accepted tokens count as queries; their own keys are cached by now, one a level of the tree
         taken = torch.zeros(tokens.shape, dtype=torch.bool, device=m.device).scatter(1, path.long(), True)
         lse.masked_fill_(~taken[:, None], -float("inf"))
-        dvattn_b200.dvattn_paged_mass(self.mass, q, lse, loc, cos[None], sin[None], self.turns, self.k, self.tables, m.scale)
+        seen = (self.cached[:, None] + self.depth)[None].contiguous()
+        dvattn_b200.dvattn_paged_mass(self.mass, q, lse, seen, cos[None], sin[None], self.turns, self.k, self.tables, m.scale)
         self.cached += counts
         self.seen += counts
         gained = torch.where(torch.arange(LEVELS + 1, device=m.device) < counts[:, None], best.gather(1, path.long()), -1)

@@ -61,6 +61,19 @@ def test_speculative_steps_equal_greedy_decoding():
     assert bool((total > 0).all()) and bool((total <= queries * (1 + 1e-4)).all())
 
 
+def test_the_mass_holds_all_weight_of_the_accepted_tokens():
+    """Everything that an accepted token attended to is in the cache after its step, itself and the tokens
+    accepted before it included: a query head's weights add up to one."""
+    X = example()
+    model, d = setup(X, 5, 120)
+    gained = torch.stack([d.step() for _ in range(25)])
+    accepted = (gained >= 0).sum((0, 2)).double()
+    assert int((gained >= 0).sum(2).max()) > 1
+    want = (accepted * (model.Hq // model.Hkv))[:, None].expand(5, model.Hkv)
+    # scores and sums of both calls in 32 bits are within 1e-4 (the lse tolerance)
+    assert bool(((d.mass.sum(-1).double() - want).abs() <= 2e-4 * want).all())
+
+
 def test_speculative_steps_within_a_budget():
     X = example()
     _, d = setup(X, 5, 120)
