@@ -288,7 +288,7 @@ int mass_launch(const dvattn_mass_args* a, void* workspace, size_t wbytes, cudaS
     p.rot_vec = rotate_vec(a->R, a->cosines, a->sines);
     p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
     const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
-    p.cap = cap > 0x7fffffffLL ? 0x7fffffff : (int)cap;
+    p.cap = cap > kMostPositions ? kMostPositions : (int)cap;
     p.tail = 0; p.align = 1; p.kt = k.kt; p.nt = 1; p.groups = L.groups; p.least = 1;
     p.N = a->positions;
     p.scale_log2 = a->scale * kLog2e;

@@ -503,7 +503,7 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     p.rot_vec = rotate_vec(a->R, a->cosines, a->sines);
     p.tail = a->S; p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
     const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
-    p.cap = a->num_blocks <= 0 ? 0 : cap > 0x7fffffffLL ? 0x7fffffff : (int)cap;
+    p.cap = a->num_blocks <= 0 ? 0 : cap > kMostPositions ? kMostPositions : (int)cap;
     p.SW = L.sw; p.kt = k.kt; p.mi = k.mi; p.nt = L.nt; p.groups = L.groups; p.least = k.least;
     p.scale_log2 = a->scale * kLog2e;
     p.out = a->out; p.lse_out = a->lse_out; p.q = a->queries; p.cos = a->cosines; p.sin = a->sines;

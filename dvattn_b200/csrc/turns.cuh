@@ -15,8 +15,12 @@
 
 namespace dvb {
 
+// Positions of a sequence that are read at most: window arithmetic reaches up to two windows past the
+// last key, and stays within 32 bits.
+constexpr int kMostPositions = 0x7fffff00;
+
 struct TurnSplit {
-    int F, W, BS, maxb, cap, tail;
+    int F, W, BS, maxb, cap, tail;  // cap: positions of the block table, at most kMostPositions
     int kt, nt, groups;  // keys per window, row tiles per sequence, CTA groups
     int least;           // windows a group has at least, where there are that many
     int align;           // windows over the cache begin on logical positions that are multiples of it

@@ -182,7 +182,8 @@ typedef struct dvattn_rotary_args {
  * are not there either.  Token s sees the cached keys l <= locations[f,w,s] of every turn
  * (locations: the last cached key it sees, not its own position) and the drafted keys of its
  * ancestors and itself.  cosines/sines[f,w,s] rotate its query for turn f; those of the last
- * turn rotate its key as well.  A token that is not there gets zeros (lse: -inf).
+ * turn rotate its key as well.  A token that is not there gets zeros (lse: -inf).  Positions from
+ * 2^31 - 256 on are not read.
  */
 typedef struct dvattn_tree_args {
     int dtype;
@@ -238,7 +239,7 @@ typedef struct dvattn_tree_append_args {
  * Arguments of the accumulation of attention weight: mass[w,h,p] grows by the softmax weight
  * that the key at logical position p of sequence w and KV head h received from the queries
  * [W,Hq,S,E] of one attention call, whose lse is given.  A query whose lse is -inf adds
- * nothing.  Positions at and past `positions` are not accumulated.
+ * nothing.  Positions at and past `positions`, and from 2^31 - 256 on, are not accumulated.
  */
 typedef struct dvattn_mass_args {
     int dtype;

@@ -120,6 +120,24 @@ def test_mass_of_keys_that_are_not_finite(dtype, E, S, G):
     assert torch.equal(torch.isfinite(got), finite) and bool(torch.isnan(got[~finite]).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("BS", [65536, 65537])
+def test_mass_of_as_many_positions_as_there_are(dtype, BS):
+    """A turn of 2^31 - 1 keys, one page under all of them; the mass holds the first ones."""
+    n, E, N = 2 ** 31 - 1, 64, 70000
+    g = torch.Generator().manual_seed(17)
+    kc = torch.randn((1, BS, 1, E), generator=g).to(dtype)
+    q = torch.randn((1, 2, 1, E), generator=g).to(dtype)
+    none = torch.zeros((1, 1, 1, 0))
+    c = dict(q=q, loc=torch.full((1, 1, 1), n, dtype=torch.int32), cos=none, sin=none, L=torch.tensor([n], dtype=torch.int32), kc=kc,
+             bt=torch.zeros((1, 32769), dtype=torch.int32), scale=0.125, mass=torch.rand((1, 1, N), generator=g), lse=torch.full((1, 2, 1), 3.0))
+    got = add_mass(c).double().cpu()
+    add = (0.125 * q[0, :, 0].double() @ kc[0, :, 0].double().T - 3.0).exp().sum(0)
+    add = torch.cat([add, add])[:N][None, None]
+    ref = c["mass"].double() + add
+    assert bool(((got - ref).abs() <= plain64.mass_bound(c, ref, add)).all())
+
+
 def test_mass_repeats_streams_and_c_abi():
     c = make([[3000, 20], [40, 700]], 9, 8, 2, 128, 64, 16, BF16, seed=9)
     a, b = add_mass(c), add_mass(c)

@@ -246,6 +246,28 @@ def test_equal_to_a_causal_decode_of_the_appended_chain():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("BS", [65536, 65537])
+def test_as_many_positions_as_there_are(dtype, BS):
+    """A block table of more than 2^31 positions, one page under all of them: the first 2^31 - 256 are read."""
+    n, E, most = 2 ** 31 - 1, 64, 2 ** 31 - 256
+    g = torch.Generator().manual_seed(16)
+    kc, vc = (torch.randn((1, BS, 1, E), generator=g).to(dtype) for _ in range(2))
+    q, dk, dv = (torch.randn((1, h, 1, E), generator=g).to(dtype) for h in (2, 1, 1))
+    none = torch.zeros((1, 1, 1, 0))
+    c = dict(q=q, parents=torch.tensor([[-1]], dtype=torch.int32), loc=torch.full((1, 1, 1), n, dtype=torch.int32), cos=none, sin=none,
+             L=torch.tensor([n], dtype=torch.int32), kc=kc, vc=vc, bt=torch.zeros((1, 32769), dtype=torch.int32), scale=0.125, dk=dk, dv=dv)
+    out, lse = call(on_gpu(c))
+    times = torch.tensor([(most - p + BS - 1) // BS for p in range(BS)] + [1], dtype=torch.float64)
+    z = 0.125 * q[0, :, 0].double() @ torch.cat([kc[0, :, 0], dk[0, 0]]).double().T
+    w = z.exp() * times
+    v = torch.cat([vc[0, :, 0], dv[0, 0]]).double()
+    ref, mag = (w @ v / w.sum(1, keepdim=True))[None, :, None], (w @ v.abs() / w.sum(1, keepdim=True))[None, :, None]
+    assert bool(((out.double().cpu() - ref).abs() <= plain64.out_bound(c, ref, mag, most)).all())
+    want = w.sum(1).log()
+    assert bool(((lse.double().cpu()[0, :, 0] - want).abs() <= plain64.lse_bound(c, want, most)).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("R", [24, 64])
 def test_drafted_keys_are_those_that_the_append_writes(dtype, R):
     """cos/sin rows whose halves differ: a drafted key is turned by both, like the key that goes into the cache."""
