@@ -136,13 +136,14 @@ __global__ void __launch_bounds__(MassCfg<E, ROWS>::NT, 1) mass_tc_kernel(MassPa
             ++epoch;
             return true;
         };
-        if (!produce_windows<T, E, KT, C::PARTS>(p, src, C::K_STAGES, s0 + C::OFF_K + grp * C::K_STAGES * C::KTILE, k_full + 32 * grp, k_empty + 32 * grp,
+        Producer at{};
+        if (!produce_windows<T, E, KT, C::PARTS>(at, p, src, AsTheyAre{false}, C::K_STAGES, s0 + C::OFF_K + grp * C::K_STAGES * C::KTILE, k_full + 32 * grp, k_empty + 32 * grp,
                                                  take_run, wait, [&] { return *s_abort != 0; }, load_q)) {
             give_up(1);
             for (int y = max(0, epoch - C::Q_SETS); y < epoch; ++y) mbar_wait(q_full + 8 * (y % C::Q_SETS), (y / C::Q_SETS) & 1);
         }
     } else if (wid == C::WARP_WALK) {
-        if (!split_schedule(p, lane, g, runs, run_full, run_empty, [&] { return *s_abort != 0; }, p.passes)) give_up(1);
+        if (!split_schedule(p, lane, g, runs, run_full, run_empty, [&] { return *s_abort != 0; }, p.passes, [](int) {})) give_up(1);
     } else if (wid >= C::WARP_MMA) {
         // ============================ MMA of one group's windows ============================
         const int grp = wid - C::WARP_MMA;

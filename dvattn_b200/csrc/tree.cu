@@ -19,9 +19,10 @@ namespace dvb {
 // ---- prep ---------------------------------------------------------------------------
 // Block (w, 0) finds sequence w's ancestor sets, what each token sees of each turn and the
 // spans; the others rotate its queries for every turn and its drafted keys, once for all the
-// CTAs that read them.  Reads and writes (F + 1 parts of Hkv rows) a few percent of a call's
-// bytes, 6 us for one turn and one more per turn; done by the attention kernel's own threads, the
-// rotation stood between two pieces of its work for 5 us and more.
+// CTAs that read them, and copy its drafted values without infinities and NaN (tree_tc.cu).  Reads
+// and writes (F + 1 parts of Hkv rows) a few percent of a call's bytes, 6 us for one turn and one
+// more per turn; done by the attention kernel's own threads, the rotation stood between two pieces
+// of its work for 5 us and more.
 constexpr int kPrepChunks = 256;  // 16-byte chunks of a rotating block
 
 template <class T>
@@ -34,6 +35,7 @@ __global__ void __launch_bounds__(256, 4) tree_prep_kernel(TreeParams p, int E) 
         __shared__ int part[8];
         int* there = par + p.S;
         if (w == 0 && tid < 4) p.header[tid] = 0;
+        for (int j = tid; j < p.Hkv; j += 256) p.odd_any[w * p.Hkv + j] = 0;
         for (int j = tid; j < p.S; j += 256) par[j] = __ldg(p.parents + (size_t)w * p.S + j);
         __syncthreads();
         // a token is there if its line of parents, each before its child, ends at -1
@@ -60,16 +62,21 @@ __global__ void __launch_bounds__(256, 4) tree_prep_kernel(TreeParams p, int E) 
         for (int f = wid; f < p.F; f += 8) {
             for (; at < f; ++at) off += max(__ldg(p.L + at), 0);
             const int Lf = __ldg(p.L + f);
-            int v = 0;
+            int v = 0, least = 0x7fffffff;
             for (int s = lane; s < p.S; s += 32) {
                 const size_t x = ((size_t)f * p.W + w) * p.S + s;
                 const int n = there[s] ? turn_seen(Lf, __ldg(p.loc + x), off, p.cap) : 0;
                 p.lim[x] = n;
                 v = max(v, n);
+                if (there[s]) least = min(least, n);
             }
             v = __reduce_max_sync(0xffffffffu, v);
+            least = __reduce_min_sync(0xffffffffu, least);
             const int first = v > 0 ? (int)off : 0;  // below cap where a key is seen
-            if (lane == 0) p.span[(size_t)w * p.F + f] = make_int2(v, first);
+            if (lane == 0) {
+                p.span[(size_t)w * p.F + f] = make_int2(v, least < v ? first | (int)0x80000000 : first);
+                p.same[(size_t)w * p.F + f] = least;
+            }
             nw += turn_windows(p, v, first);
         }
         if (lane == 0) part[wid] = nw;
@@ -80,10 +87,24 @@ __global__ void __launch_bounds__(256, 4) tree_prep_kernel(TreeParams p, int E) 
         }
         return;
     }
-    // a chunk a thread: of the drafted keys [Hkv][S], for the last turn, or of the queries
-    // [Hkv][rows], for every turn
+    // a chunk a thread: of the drafted keys [Hkv][S], for the last turn, of the queries [Hkv][rows], for
+    // every turn, or of the drafted values
     const int keys = p.Hkv * p.S, per = E * (int)sizeof(T) / 16, all = (keys + p.Hkv * p.rows) * per;
-    const int c = (blockIdx.y - 1) * kPrepChunks + tid;
+    int c = (blockIdx.y - 1) * kPrepChunks + tid;
+    const int copies = (all + kPrepChunks - 1) / kPrepChunks;  // the first block with values
+    if (sizeof(T) == 2 && (int)blockIdx.y > copies) {
+        c -= copies * kPrepChunks;
+        if (c >= keys * per) return;
+        const size_t at = (size_t)w * keys * per + c;
+        uint4 v = __ldg(static_cast<const uint4*>(p.dv) + at);
+        if constexpr (sizeof(T) == 2) {  // a row's `per` lanes (8, 16 or 32) are neighbours
+            const unsigned group = per == 32 ? 0xffffffffu : ((1u << per) - 1) << (lane & ~(per - 1));
+            const unsigned any = __ballot_sync(group, make_finite<T>(v));
+            static_cast<uint4*>(p.dvr)[at] = v;
+            if (lane % per == 0) p.odd[at / per] = any != 0;
+        }
+        return;
+    }
     if (c >= all) return;
     const int x = c / per, e0 = (c - x * per) * RotateChunk<T>::PER;
     const bool key = x < keys;
@@ -228,12 +249,14 @@ template <int E> __global__ void __launch_bounds__(SimtCfg<E>::THREADS) tree_sim
                 }
             }
             const int key = win.k0 + lane;
+            uint32_t seen[4];  // the window's keys that a row sees
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
                 bool sees = false;
                 if (lane < win.n && (there >> a & 1u))
                     sees = win.f < p.F ? key < lim[a]
                                        : (__ldcg(p.anc + ((size_t)pc.w * p.S + tok[a]) * p.SW + (key >> 5)) >> (key & 31) & 1u) != 0;
+                seen[a] = __ballot_sync(0xffffffffu, sees);
                 const float x = sees ? sc[a] * p.scale_log2 : neg_inf();
                 float mx = x;
 #pragma unroll
@@ -261,10 +284,12 @@ template <int E> __global__ void __launch_bounds__(SimtCfg<E>::THREADS) tree_sim
                 for (int u = 0; u < 4; ++u) {
                     float vv[VC];
                     load_n(reinterpret_cast<const float*>(sV + (st * KT + k4 + u) * ROW) + lane * VC, vv);
+                    // a row that does not see the key takes nothing of it: 0 * NaN is NaN
 #pragma unroll
                     for (int a = 0; a < 4; ++a)
+                        if (seen[a] >> (k4 + u) & 1u)
 #pragma unroll
-                        for (int c = 0; c < VC; ++c) o[a][c] = fmaf(pr[a][u], vv[c], o[a][c]);
+                            for (int c = 0; c < VC; ++c) o[a][c] = fmaf(pr[a][u], vv[c], o[a][c]);
                 }
             }
             __syncthreads();
@@ -300,10 +325,21 @@ template <int E> __global__ void __launch_bounds__(SimtCfg<E>::THREADS) tree_sim
 // round trip.  Four at a time leave 48 registers and more resident blocks: 32 sequences 89 us, with
 // eight (66 registers) 94; one sequence in 33 parts 30 and 29.  A call whose error word is set gets
 // NaN in every output.
+//
+// 16-bit types: the attention kernel has taken infinities and NaN out of values that some tokens see and
+// others do not (tree_tc.cu).  Such an element decides its output whatever the rest is, so it is
+// added to the finished row of who sees it.
 constexpr int kMergeAhead = 4;
 
+template <class T> __device__ __forceinline__ void load_quad(const T* src, float (&v)[4]) {
+    const uint2 x = *reinterpret_cast<const uint2*>(src);
+    const T* y = reinterpret_cast<const T*>(&x);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = Elem<T>::to_f(y[c]);
+}
+
 template <class T, int E>
-__global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
+__global__ void __launch_bounds__(256, 5) tree_merge_kernel(TreeParams p) {
     constexpr int TPR = E / 4, RPB = 256 / TPR;  // threads per row, rows per block
     const int tid = threadIdx.x, lane = tid & 31;
     const int item = blockIdx.x, h = item % p.Hkv, t = item / p.Hkv % p.nt, w = item / p.Hkv / p.nt;
@@ -326,9 +362,12 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
     const int g0 = range.group_of(us), g1 = range.group_of(us + nw - 1);
     const int e = tid % TPR * 4;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const bool failed = __ldcg(p.header + 3) != 0;
-    if (g0 == g1 && !failed) return;
-    for (int i = blockIdx.y * RPB + tid / TPR; i < p.mi; i += gridDim.y * RPB) {
+    const int2 flags = __ldcg(reinterpret_cast<const int2*>(p.header + 2));
+    const bool failed = flags.y != 0;
+    // a value of the sequence and KV head has to be added
+    const bool odd = sizeof(T) == 2 && flags.x && __ldcg(p.odd_any + w * p.Hkv + h);
+    if (g0 == g1 && !failed && !odd) return;
+    for (int i = blockIdx.y * RPB + tid / TPR; i < p.mi && (g0 != g1 || failed); i += gridDim.y * RPB) {
         const int r = t * p.mi + i;
         if (r >= p.rows) break;
         const int s = r / p.G, hq = h * p.G + r - s * p.G;
@@ -381,6 +420,42 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
         store_quad<T>(op, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
         if (p.lse_out && e == 0) p.lse_out[orow] = den == 0.f ? neg_inf() : (m + log2f(den)) * kLn2;
     }
+    // ---- infinities and NaN, added to the finished rows ----
+    if constexpr (sizeof(T) == 2)
+        if (odd && !failed)
+#pragma unroll 1
+            for (int i = blockIdx.y * RPB + tid / TPR; i < p.mi && t * p.mi + i < p.rows; i += gridDim.y * RPB) {
+                const int r = t * p.mi + i, s = r / p.G;
+                T* op = static_cast<T*>(p.out) + (((size_t)w * p.Hq + h * p.G + r - s * p.G) * p.S + s) * E + e;
+                float a[4];
+                load_quad(op, a);
+                auto add = [&](const T* v) {
+                    float x[4];
+                    load_quad(v + e, x);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (!isfinite(x[c])) a[c] += x[c];
+                };
+                const size_t drafts = ((size_t)w * p.Hkv + h) * p.S;
+                const uint32_t* anc = p.anc + ((size_t)w * p.S + s) * p.SW;
+#pragma unroll 1
+                for (int j = 0; j <= s; ++j)
+                    if (__ldcg(p.odd + drafts + j) && (__ldcg(anc + (j >> 5)) >> (j & 31) & 1u)) add(static_cast<const T*>(p.dv) + (drafts + j) * E);
+#pragma unroll 1
+                for (int f = 0; f < p.F; ++f) {
+                    const int2 span = __ldcg(p.span + (size_t)w * p.F + f);
+                    if (span.y >= 0) continue;  // every token sees the same keys of the turn
+                    // those of the windows that were looked through, and a few before them: what the row
+                    // has already is the same when it counts twice
+                    const int first = span.y & 0x7fffffff, lim = __ldcg(p.lim + ((size_t)f * p.W + w) * p.S + s);
+#pragma unroll 1
+                    for (int l = max(0, __ldcg(p.same + (size_t)w * p.F + f) - p.kt); l < lim; ++l) {
+                        const int pos = first + l, page = __ldg(p.bt + (size_t)w * p.maxb + pos / p.BS);
+                        if (page >= 0 && page < p.NB) add(static_cast<const T*>(p.v) + (((size_t)page * p.BS + pos % p.BS) * p.Hkv + h) * E);
+                    }
+                }
+                store_quad<T>(op, a[0], a[1], a[2], a[3]);
+            }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -411,9 +486,11 @@ static int tree_stall_hook() {
     return t;
 }
 
-// 16-byte chunks of a sequence's drafted keys and of its queries.
-static long long tree_prep_chunks(const dvattn_tree_args* a) {
-    return ((long long)a->Hq + a->Hkv) * a->S * (a->E * (a->dtype == DVATTN_FLOAT32 ? 4 : 2) / 16);
+// Blocks of a sequence that rotate its drafted keys and its queries, and (16-bit types) copy its drafted values.
+static long long tree_prep_blocks(const dvattn_tree_args* a) {
+    const long long per = (long long)a->S * (a->E * (a->dtype == DVATTN_FLOAT32 ? 4 : 2) / 16);
+    const long long values = a->dtype == DVATTN_FLOAT32 ? 0 : a->Hkv * per;
+    return (((long long)a->Hq + a->Hkv) * per + kPrepChunks - 1) / kPrepChunks + (values + kPrepChunks - 1) / kPrepChunks;
 }
 
 static int tree_validate(const dvattn_tree_args* a) {
@@ -427,14 +504,14 @@ static int tree_validate(const dvattn_tree_args* a) {
     if (a->S > kTreeMaxTokens) return DVATTN_ERR_UNSUPPORTED;
     // grid limits: sequences are the prep grid's x, row blocks its y; items are the merge grid's x
     const long long rows = (long long)a->S * (a->Hq / a->Hkv);
-    if ((long long)a->F * a->W * a->Hq * a->S > 0x7fffffffLL || tree_prep_chunks(a) > 65534LL * kPrepChunks ||
+    if ((long long)a->F * a->W * a->Hq * a->S > 0x7fffffffLL || tree_prep_blocks(a) > 65534 ||
         (long long)a->W * a->Hkv * ((rows + 31) / 32) > 0x7fffffffLL)
         return DVATTN_ERR_UNSUPPORTED;
     return DVATTN_OK;
 }
 
 struct TreeLayout {
-    size_t nwin, span, anc, lim, dkr, qr, po, pl, total;
+    size_t nwin, span, anc, lim, same, odd, odd_any, dkr, dvr, qr, po, pl, total;
     int groups, sw, nt;
 };
 
@@ -460,8 +537,12 @@ static int tree_layout(const dvattn_tree_args* a, const TreeKernel& k, TreeLayou
     L.span = take(8 * (size_t)a->W * a->F);
     L.anc = take(4 * (size_t)a->W * a->S * L.sw);
     L.lim = take(4 * (size_t)a->F * a->W * a->S);
+    L.same = take(4 * (size_t)a->W * a->F);
+    L.odd = take((size_t)a->W * a->Hkv * a->S);
+    L.odd_any = take(4 * (size_t)a->W * a->Hkv);
     L.qr = take(esz * (size_t)a->F * a->W * a->Hq * a->S * a->E);
     L.dkr = take(esz * (size_t)a->W * a->Hkv * a->S * a->E);
+    L.dvr = take(esz == 2 ? esz * (size_t)a->W * a->Hkv * a->S * a->E : 0);
     L.po = take(4 * ctas * 2 * k.mi * a->E);
     L.pl = take(4 * ctas * 2 * k.mi);
     L.total = at;
@@ -515,9 +596,13 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     p.nwin = reinterpret_cast<int*>(ws + L.nwin);
     p.span = reinterpret_cast<int2*>(ws + L.span);
     p.lim = reinterpret_cast<int*>(ws + L.lim);
+    p.same = reinterpret_cast<int*>(ws + L.same);
+    p.odd = reinterpret_cast<uint8_t*>(ws + L.odd);
+    p.odd_any = reinterpret_cast<int*>(ws + L.odd_any);
     p.qr = ws + L.qr;
     p.anc = reinterpret_cast<uint32_t*>(ws + L.anc);
     p.dkr = ws + L.dkr;
+    p.dvr = ws + L.dvr;
     p.part_o = reinterpret_cast<float*>(ws + L.po);
     p.part_lse = reinterpret_cast<float*>(ws + L.pl);
 
@@ -530,7 +615,6 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
                         : a->dtype == DVATTN_FLOAT16 ? merge_fn<__half>(a->E) : merge_fn<__nv_bfloat16>(a->E);
     int E = a->E;
     void* pargs[] = {&p, &E};
-    const long long chunks = tree_prep_chunks(a);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -538,7 +622,7 @@ int tree_launch(const dvattn_tree_args* a, void* workspace, size_t wbytes, cudaS
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     cfg.stream = stream;
-    cfg.gridDim = dim3(a->W, 1 + (unsigned)((chunks + kPrepChunks - 1) / kPrepChunks));
+    cfg.gridDim = dim3(a->W, 1 + (unsigned)tree_prep_blocks(a));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 2 * sizeof(int) * (size_t)a->S;
     cudaError_t e = cudaLaunchKernelExC(&cfg, prep, pargs);

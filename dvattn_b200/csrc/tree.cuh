@@ -37,9 +37,14 @@ struct TreeParams : TurnSplit {
     const void* dk;
     const void* dv;
     // workspace
-    int* header;      // [3] error word (kErrorWordOffset)
+    int* header;      // [2] a value of the call is odd (below); [3] error word (kErrorWordOffset)
     uint32_t* anc;    // [W][S][SW] ancestor sets; a token that is not there has an empty one
     int* lim;         // [F][W][S] keys of the turn that the token sees; 0: it is not there
+    int* same;        // [W][F] keys of the turn that every token sees that is there
+    // values that are not finite (16-bit types: tree_merge_kernel)
+    uint8_t* odd;     // [W][Hkv][S] the drafted value is odd: it has an infinity or NaN
+    int* odd_any;     // [W][Hkv] so has one of them, or a cached value in the windows that are looked through
+    void* dvr;        // [W][Hkv][S][E] T, drafted values with zeros for such elements
     void* dkr;        // [W][Hkv][S][E] T, drafted keys rotated
     void* qr;         // [F][W][Hkv][rows][E] T, queries rotated for the turn
     float* part_o;    // [CTAs][2][mi][E] normalised partial outputs

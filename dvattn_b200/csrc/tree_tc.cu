@@ -14,7 +14,10 @@
 // swizzled rings with TMA boxes where pages and windows are whole numbers of boxes of 8 or more
 // rows (page sizes that are multiples of 8), else they gather rows with cp.async.  What lies in
 // rows that nobody sees never matters: their scores are masked, and their V rows are zeroed
-// before PV (0 * NaN is NaN).
+// before PV (0 * NaN is NaN).  An infinity or NaN of a value that some tokens see and others do not is
+// a zero for PV, too, and tree_merge_kernel adds it to who sees it: drafted values come from the prep
+// kernel's copy, and the V producer looks through the windows in which the tokens' locations differ (a call
+// in which they differ everywhere takes 1.3 to 1.5 times as long; one in which they do not, 1 to 2%).
 //
 // Measured with prep and merge: 32 sequences of two turns, 64/4 heads, 8 tokens, 337 MB: 89 us, 59%
 // of HBM's copy rate (203 with one CTA per SM, rows gathered and rotated by its own threads); the
@@ -72,6 +75,22 @@ __device__ __forceinline__ void store_sector(void* dst, const uint32_t* v) {
                  : "memory");
 }
 
+__device__ __forceinline__ void mark_odd(const TreeParams& p, int wh) {  // tells the merge
+    p.odd_any[wh] = 1;
+    p.header[2] = 1;
+}
+
+// The V producer's part in values that are not finite (windows.cuh).
+struct OddValues {
+    static constexpr bool always = false;
+    const TreeParams& p;
+    int h;
+    uint32_t raw;
+    __device__ __forceinline__ bool in(const SplitRun& run) const { return run.how & RUN_MIXED; }
+    __device__ __forceinline__ bool look(const SplitRun& run, int end) const { return __ldcg(p.same + (size_t)run.w * p.F + run.f) < end; }
+    __device__ __forceinline__ void found(const SplitRun& run) const { mark_odd(p, run.w * p.Hkv + h); }
+};
+
 template <class T, int E, bool TWO>
 __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_tc_kernel(TreeParams p, const __grid_constant__ TreeMaps maps) {
     using C = TcCfg<E, TWO>;
@@ -88,7 +107,7 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
     const uint32_t bar = s0 + C::OFF_BAR;
     const uint32_t k_full = bar, k_empty = bar + 32, v_full = bar + 64, v_empty = bar + 96;
     const uint32_t s_full = bar + 128, p_full = bar + 144, q_full = bar + 160, q_empty = bar + 176, o_done = bar + 192;
-    const uint32_t run_full = bar + 200, run_empty = run_full + 8 * RUN_RING;
+    const uint32_t run_full = bar + 200, run_empty = run_full + 8 * RUN_RING, v_raw = run_empty + 8 * RUN_RING;  // 45 in all
     SplitRun* runs = reinterpret_cast<SplitRun*>(smem + C::OFF_RUN);
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
     if (tid == 0) {
@@ -97,6 +116,7 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
             mbar_init(k_empty + 8 * s, 1);
             mbar_init(v_full + 8 * s, p.box ? 1 : 32);
             mbar_init(v_empty + 8 * s, 1);
+            mbar_init(v_raw + 8 * s, 1);
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(s_full + 8 * s, 1);
@@ -163,7 +183,7 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
     if (wid == C::WARP_K || wid == C::WARP_V) {
         const bool is_k = wid == C::WARP_K;
         WindowSource src;
-        src.cache = is_k ? p.k : p.v, src.tail = is_k ? p.dkr : p.dv;
+        src.cache = is_k ? p.k : p.v, src.tail = is_k ? p.dkr : p.dvr;
         src.map = is_k ? &maps.k : &maps.v, src.tail_map = is_k ? &maps.dk : &maps.dv;
         src.h = h, src.Hkv = p.Hkv, src.box = p.box, src.me = 0, src.of = 1, src.anc = p.anc, src.SW = p.SW;
         // keys and values that one row tile reads are read once: they leave L2 first, the partial
@@ -171,16 +191,28 @@ __global__ void __launch_bounds__(TcCfg<E, TWO>::NT, TcCfg<E, TWO>::CTAS) tree_t
         src.policy = p.nt == 1 ? l2_evict_first() : l2_evict_normal();
         src.stall = is_k && blockIdx.x == 0 ? p.stall_tile : -1;
         int epoch = 0;
-        const bool ok = produce_windows<T, E, KT, 1>(
-            p, src, is_k ? C::K_STAGES : VS, s0 + (is_k ? C::OFF_K : C::OFF_V), is_k ? k_full : v_full, is_k ? k_empty : v_empty, take_run, wait,
-            [&] { return *s_abort != 0; }, [&](const SplitRun& run) { return !is_k || !(run.how & RUN_Q_NEW) || load_q(run, epoch++); });
+        Producer at{};
+        auto stopped = [&] { return *s_abort != 0; };
+        auto opened = [&](const SplitRun& run) { return !is_k || !(run.how & RUN_Q_NEW) || load_q(run, epoch++); };
+        bool ok = produce_windows<T, E, KT, 1>(at, p, src, AsTheyAre{!is_k}, is_k ? C::K_STAGES : VS, s0 + (is_k ? C::OFF_K : C::OFF_V),
+                                               is_k ? k_full : v_full, is_k ? k_empty : v_empty, take_run, wait, stopped, opened);
+        // values from the first mixed run on: code of its own, which would cost every window 5% in the loop before
+        if (ok && at.left)
+            ok = produce_windows<T, E, KT, 1>(at, p, src, OddValues{p, h, v_raw}, VS, s0 + C::OFF_V, v_full, v_empty, take_run, wait, stopped,
+                                              [](const SplitRun&) { return true; });
         if (!ok) {
             give_up(1);
             if (is_k)  // what load_q requested lands before the CTA can exit, too
                 for (int y = max(0, epoch - C::Q_SETS); y < epoch; ++y) mbar_wait(q_full + 8 * (y % C::Q_SETS), (y / C::Q_SETS) & 1);
         }
     } else if (wid == C::WARP_WALK) {
-        if (!split_schedule(p, lane, g, runs, run_full, run_empty, [&] { return *s_abort != 0; })) give_up(1);
+        auto tail = [&](int w) {  // are there odd drafted values?
+            const int wh = w * p.Hkv + h;
+            for (int s = lane; s < p.S; s += 32)
+                if (__ldcg(p.odd + (size_t)wh * p.S + s)) mark_odd(p, wh);
+            __syncwarp();
+        };
+        if (!split_schedule(p, lane, g, runs, run_full, run_empty, [&] { return *s_abort != 0; }, 1, tail)) give_up(1);
     } else if (wid == C::WARP_MMA) {
         // =================================== MMA ===================================
         // (the whole warp converged: umma_warp)
@@ -489,7 +521,7 @@ bool tree_tc_maps(TreeParams& p, int dtype, int E, TreeMaps& m) {
     p.align = p.box ? p.box : 1;
     if (!p.box) return true;
     return encode_cache_map(&m.k, p.k, dtype, E, p.Hkv, tokens, p.box) && encode_cache_map(&m.v, p.v, dtype, E, p.Hkv, tokens, p.box) &&
-           encode_cache_map(&m.dk, p.dkr, dtype, E, 1, drafts, p.kt) && encode_cache_map(&m.dv, p.dv, dtype, E, 1, drafts, p.kt);
+           encode_cache_map(&m.dk, p.dkr, dtype, E, 1, drafts, p.kt) && encode_cache_map(&m.dv, p.dvr, dtype, E, 1, drafts, p.kt);
 }
 
 }  // namespace dvb

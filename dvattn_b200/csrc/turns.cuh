@@ -29,7 +29,9 @@ struct TurnSplit {
     const int* L;
     const int* bt;
     int* nwin;  // workspace: [W] windows of a sequence's row tile
-    int2* span;  // workspace: [W][F] {keys of the turn that some query of the sequence sees, its first position}
+    // workspace: [W][F] {keys of the turn that some query of the sequence sees, its first position}; the
+    // sign bit of the position: another query does not see them all (where the kernel asks for it)
+    int2* span;
 };
 
 // Keys of a turn that a query with location `loc` sees, the turn starting at logical
@@ -161,6 +163,7 @@ struct SplitWalk {
 // increasing order; `start` begins a sequence.
 struct SplitWin {
     int f, first, nf, sp, off, k0, n;  // turn, its first window, its windows, seen keys and first position
+    bool mixed;                        // some queries see keys of the turn that others do not
     int2 ahead;                        // the next turn's, loaded a turn early
     __device__ __forceinline__ int2 load(const TurnSplit& p, int w, int f_) const {
         return f_ < p.F ? __ldcg(p.span + (size_t)w * p.F + f_) : make_int2(p.tail, 0);
@@ -168,7 +171,8 @@ struct SplitWin {
     __device__ __forceinline__ void enter(const TurnSplit& p, int w, int2 x) {
         ahead = load(p, w, f + 1);
         sp = x.x;
-        off = x.y;
+        off = x.y & 0x7fffffff;
+        mixed = x.y < 0;
         nf = f < p.F ? turn_windows(p, sp, off) : 0x7fffffff - first;
     }
     __device__ __forceinline__ void start(const TurnSplit& p, int w) {
@@ -198,14 +202,15 @@ struct alignas(16) SplitRun {
 constexpr int RUN_FIRST = 1, RUN_LAST = 2;   // of its piece
 constexpr int RUN_WHOLE = 4, RUN_BEGIN = 8;  // the piece is a whole item; it begins one (SplitPiece::slot)
 constexpr int RUN_Q_NEW = 16, RUN_Q_END = 32;  // q rotated for another turn than before; the next run's will be
+constexpr int RUN_MIXED = 64;                  // of a turn that is mixed (SplitWin)
 constexpr int RUN_RING = 8;
 
 // The walking warp.  passes > 1: every run that many times, t = 0, 1, ..., each with its own q
 // (the split then has one row tile).  `full` and `empty` are RUN_RING mbarriers each (one arrival; one per
-// consumer).  false: a wait gave up.
-template <class Stop>
+// consumer).  `tail(w)` is called when the tail of sequence w has been handed out.  false: a wait gave up.
+template <class Stop, class Tail>
 __device__ __forceinline__ bool split_schedule(const TurnSplit& p, int lane, int g, SplitRun* ring, uint32_t full, uint32_t empty, Stop stopped,
-                                               int passes = 1) {
+                                               int passes, Tail tail) {
     SplitWalk walk;
     walk.place(p, lane, g);
     SplitPiece pc;
@@ -231,17 +236,33 @@ __device__ __forceinline__ bool split_schedule(const TurnSplit& p, int lane, int
             SplitRun r;
             r.w = pc.w, r.t = pc.t, r.f = win.f, r.off = win.off, r.k0 = win.k0, r.sp = win.sp, r.n = nx;
             r.how = (i == pc.i0 ? RUN_FIRST : 0) | (i + nx == pc.i1 ? RUN_LAST : 0) | (pc.whole() ? RUN_WHOLE : 0) | (pc.slot() ? RUN_BEGIN : 0) |
-                    (qt != turn ? RUN_Q_NEW : 0) | (i + nx == pc.i1 || qt != p.F - 1 ? RUN_Q_END : 0);
+                    (qt != turn ? RUN_Q_NEW : 0) | (i + nx == pc.i1 || qt != p.F - 1 ? RUN_Q_END : 0) | (win.mixed ? RUN_MIXED : 0);
             for (int pass = 0; pass < passes; ++pass) {
                 if (passes > 1) r.t = pass, r.how |= RUN_Q_NEW | RUN_Q_END;
                 if (!push(r)) return false;
             }
+            if (win.f == p.F) tail(pc.w);
             turn = qt;
             i += nx;
         }
     }
     SplitRun end{};
     return push(end);
+}
+
+// v, eight 16-bit elements, with zeros for infinities and NaN; true: there was one.
+template <class T> __device__ __forceinline__ bool make_finite(uint4& v) {
+    constexpr uint32_t top = Elem<T>::dtype == DVATTN_BFLOAT16 ? 0x7f80u : 0x7c00u;
+    bool any = false;
+    uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const bool lo = (x[u] & top) == top, hi = (x[u] >> 16 & top) == top;
+        if (lo) x[u] &= 0xffff0000u;
+        if (hi) x[u] &= 0xffffu;
+        any |= lo || hi;
+    }
+    return any;
 }
 
 // A 16-byte chunk (elements e0...) of a row rotated by apply_rotary_pos_emb: o[e] = x[e] c[e] -

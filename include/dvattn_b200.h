@@ -182,7 +182,8 @@ typedef struct dvattn_rotary_args {
  * are not there either.  Token s sees the cached keys l <= locations[f,w,s] of every turn
  * (locations: the last cached key it sees, not its own position) and the drafted keys of its
  * ancestors and itself.  cosines/sines[f,w,s] rotate its query for turn f; those of the last
- * turn rotate its key as well.  A token that is not there gets zeros (lse: -inf).  Positions from
+ * turn rotate its key as well.  A token that is not there gets zeros (lse: -inf).  What lies in a key
+ * or value reaches the tokens that see it and no other, infinities and NaN too.  Positions from
  * 2^31 - 256 on are not read.
  */
 typedef struct dvattn_tree_args {

@@ -245,6 +245,73 @@ def test_equal_to_a_causal_decode_of_the_appended_chain():
     assert bool(((lse - lse2).double().abs().cpu() <= 2 * plain64.lse_bound(c, exact_lse, 105)).all())
 
 
+def visible(c):
+    """[W, S, keys] which cached key of each turn, then which drafted key, a token sees."""
+    W, S = c["parents"].shape
+    cap = c["bt"].size(1) * c["kc"].size(1)
+    anc = torch.stack([plain64.ancestors(p) for p in c["parents"].tolist()])
+    there = anc.any(-1)
+    parts = [(torch.arange(n) <= c["loc"][f][..., None]) & there[..., None] for f, (_, n) in enumerate(plain64.turns(c["L"].tolist(), cap))]
+    return torch.cat(parts + [anc], -1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E,S,G,BS", [(64, 7, 2, 16), (64, 70, 4, 16), (128, 7, 2, 16), (128, 1, 16, 16), (128, 7, 2, 6), (128, 70, 4, 16),
+                                      (128, 70, 4, 6), (128, 300, 1, 16), (256, 7, 2, 16), (256, 40, 4, 5)])
+def test_values_that_are_not_finite_reach_who_sees_them(dtype, E, S, G, BS):
+    """Infinities and NaN in values of drafted tokens and of cached keys that some tokens see: an element of
+    who sees one is not finite, everything else has the bits of the same call with zeros in these places."""
+    c = make([[500, 130], [90, 61]], S, 2 * G, 2, E, 32, BS, dtype, seed=E + S, parents=None if S > 1 else [[-1], [-1]])
+    rs = np.random.RandomState(E + S + BS)
+    if S > 1:
+        c["parents"][1, S - 1] = -2
+        # locations by token: past the end, inside a window, in front of the turn
+        c["loc"][0, 0] = torch.from_numpy(rs.choice([499, 77, 430, -1], size=S).astype(np.int32))
+        c["loc"][1, 1] = torch.from_numpy(rs.choice([60, 40], size=S).astype(np.int32))
+        c["loc"][1, 0] = torch.from_numpy(rs.choice([129, 128], size=S).astype(np.int32))
+    # pages of every sequence's own
+    pages = c["bt"].size(1)
+    g = torch.Generator().manual_seed(18)
+    c["kc"], c["vc"] = (torch.randn((2 * pages, BS, 2, E), generator=g).to(dtype) for _ in range(2))
+    c["bt"] = torch.from_numpy(rs.permutation(2 * pages).reshape(2, pages).astype(np.int32))
+    spans = plain64.turns(c["L"].tolist(), pages * BS)
+    where = torch.cat([torch.arange(first, first + n) for first, n in spans])
+    cached = where.numel()
+    clean = {**c, "vc": c["vc"].clone(), "dv": c["dv"].clone()}
+    bad = torch.zeros((2, 2, cached + S, E))  # what lies there, 0: a finite value
+    special = [math.inf, -math.inf, math.nan]
+    spots = [(0, 70), (0, 80), (0, 429), (0, 431), (0, 499), (1, 499 + 41), (1, 499 + 62), (0, 500 + 129)]
+    spots += [(int(w), cached + int(j)) for w, j in zip(rs.randint(0, 2, 8), rs.randint(0, S, 8))]
+    for x, (w, key) in enumerate(spots):
+        if key >= bad.size(2):
+            continue
+        bad[w, x % 2, key, rs.randint(0, E, 3)] = special[x % 3]
+    for w in range(2):
+        for h in range(2):
+            for key in bad[w, h].ne(0).any(-1).nonzero()[:, 0].tolist():
+                b = bad[w, h, key]
+                row = lambda t: t["vc"][int(t["bt"][w, where[key] // BS]), where[key] % BS, h] if key < cached else t["dv"][w, h, key - cached]  # noqa: E731
+                row(clean)[:] = torch.where(b != 0, torch.zeros((), dtype=dtype), row(clean))
+                row(c)[:] = torch.where(b != 0, b.to(dtype), row(c))
+    want, want_lse = call(on_gpu(clean))
+    out, lse = call(on_gpu(c))
+    assert bool(torch.isfinite(want).all())
+    sees = visible(c).float()  # [W, S, keys]
+    hit = bad != 0
+    # per output: how many of each it sees
+    n = {v: torch.einsum("wsk,whke->whse", sees, (bad.isnan() if v != v else bad == v).float()) for v in special}
+    nan = (n[special[2]] > 0) | ((n[math.inf] > 0) & (n[-math.inf] > 0))
+    expect = want.cpu().view(2, 2, G, S, E).float()
+    for v in (math.inf, -math.inf):
+        expect = torch.where((n[v] > 0)[:, :, None], torch.tensor(v), expect)
+    expect = torch.where(nan[:, :, None], torch.tensor(math.nan), expect)
+    got = out.cpu().view(2, 2, G, S, E).float()
+    assert bool(hit.any()) and not bool(torch.isfinite(got).all())
+    assert torch.equal(got.isnan(), expect.isnan())
+    assert torch.equal(got.nan_to_num(nan=0.0), expect.nan_to_num(nan=0.0))
+    assert torch.equal(lse, want_lse)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("BS", [65536, 65537])
 def test_as_many_positions_as_there_are(dtype, BS):
