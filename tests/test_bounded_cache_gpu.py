@@ -296,6 +296,50 @@ def test_evict_repeats_and_c_abi():
         assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
 
 
+def test_append_mass_and_eviction_replayed_from_a_graph():
+    """Captured once, replayed over changed inputs: what the calls themselves give."""
+    W, Hkv, S, E, BS, n = 3, 2, 4, 64, 16, 300
+    kc, vc, bt, g = pool(W, n + 20, Hkv, E, BS, BF16, seed=10)
+    N = bt.size(1) * BS
+    kc, vc, bt = (t.to(DEV) for t in (kc, vc, bt))
+    dk, dv = (torch.randn((W, Hkv, S, E), generator=g).to(BF16).to(DEV) for _ in range(2))
+    q = torch.randn((W, 4 * Hkv, S, E), generator=g).to(BF16).to(DEV)
+    angles = torch.rand((1, W, S, 32), generator=g).to(DEV)
+    lse = torch.full((W, 4 * Hkv, S), 6.0, device=DEV)
+    mass = torch.rand((W, Hkv, N), generator=g).to(DEV)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    pos, acc, cnt, L = ints([n, n - 9, 17]), ints([[0, 1, 3]] * W), ints([3, 2, 1]), ints([N])
+    zero, source = ints([0] * W), torch.zeros((W, Hkv, N), dtype=torch.int32, device=DEV)
+    state = [kc, vc, mass, source]
+    start = [t.clone() for t in state]
+
+    def step():
+        dvattn_b200.dvattn_tree_append(kc, vc, dk, dv, angles[0], angles[0], bt, pos, acc, cnt)
+        seen = (pos + cnt)[None, :, None].expand(1, W, S).contiguous() - 1
+        dvattn_b200.dvattn_paged_mass(mass, q, lse, seen, angles, angles, L, kc, bt, 0.125)
+        dvattn_b200.dvattn_paged_evict(kc, vc, mass, bt, zero, pos + cnt, (pos + cnt).clamp(max=256), sink=2, recent=8, source=source)
+
+    def run(call, positions):
+        for t, x in zip(state, start):
+            t.copy_(x)
+        pos.copy_(positions)
+        call()
+        torch.cuda.synchronize()
+        return [t.clone() for t in state]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for positions in ([n, n - 9, 17], [280, 3, 255], [n, n, n]):
+        want = run(step, ints(positions))
+        for _ in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(run(graph.replay, ints(positions)), want))
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------
 def test_refusals():
     c = make([[10, 4], [3, 3]], 3, 4, 2, 64, 32, 16, F16, seed=14)
