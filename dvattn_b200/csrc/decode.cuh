@@ -27,7 +27,7 @@ int varlen_rope_attn_launch(const dvattn_varlen_args* a, const dvattn_rotary_arg
                             cudaStream_t stream);
 // paged KV append with fused K rotation (append.cu)
 int paged_append_launch(const dvattn_append_args* a, cudaStream_t stream);
-// the accepted tokens of a drafted tree appended (append.cu)
+// the accepted tokens of a drafted tree appended (tree_append.cu)
 int tree_append_launch(const dvattn_tree_append_args* a, cudaStream_t stream);
 // attention of a drafted tree (tree.cu)
 size_t tree_workspace_size(const dvattn_tree_args* a);

@@ -19,11 +19,11 @@
 // kernel's copy, and the V producer looks through the windows in which the tokens' locations differ (a call
 // in which they differ everywhere takes 1.3 to 1.5 times as long; one in which they do not, 1 to 2%).
 //
-// Measured with prep and merge: 32 sequences of two turns, 64/4 heads, 8 tokens, 337 MB: 89 us, 59%
-// of HBM's copy rate (203 with one CTA per SM, rows gathered and rotated by its own threads); the
+// Measured with prep and merge: 32 sequences of two turns, 64/4 heads, 8 tokens, 337 MB: 88 to 92 us
+// by the box, 57 to 59% of HBM's copy rate (203 with one CTA per SM, rows gathered and rotated by its own threads); the
 // stream alone reaches 89% with 128 rows, 98% with 32.  4 sequences of up to 131072 keys, 128/8
-// heads, 16 tokens (two tiles): 572 us, 671 TFLOP/s, 4325 cycles per 128-key window at the 1.5 GHz
-// that the power limit leaves; tensor core and SFU are each busy for a third of the time.
+// heads, 16 tokens (two tiles): 557 to 590 us, 688 to 650 TFLOP/s, 4325 cycles per 128-key window at
+// the 1.5 GHz that the power limit leaves; tensor core and SFU are each busy for a third of the time.
 //
 // Every wait is bounded; one that gives up sets the call's error word, ends the CTA with
 // nothing in flight, and tree_merge_kernel writes NaN to all outputs of the call.
@@ -44,8 +44,9 @@ template <int E, bool TWO> struct TcCfg {
     static constexpr int WARP_MMA = 4 * NG, WARP_K = 4 * NG + 1, WARP_V = 4 * NG + 2, WARP_WALK = 4 * NG + 3;
     // Registers of a softmax thread and of the others, out of an even share of 168 (two tiles,
     // 384 threads) or 128 (256 threads, two CTAs): 256 * 208 + 128 * 88 = 384 * 168 and
-    // 128 * 168 + 128 * 88 = 256 * 128.  A row of 128 scores does not fit in 168 (the batched
-    // decode took half as long again when it spilled).  0: every thread may have 255.
+    // 128 * 168 + 128 * 88 = 256 * 128.  A row of 64 scores fits in 168 (the batched decode took half as
+    // long again with 128 of them, which spilled); with 128 scores 208 still spill 108 bytes a thread.
+    // 0: every thread may have 255.
     static constexpr int REGS = TWO ? 208 : E == 256 ? 0 : 168;
     // Shared memory: sets of Q tiles (a second one lets the next turn's or piece's arrive while
     // the last one is in use), the K ring, the V ring.
@@ -56,6 +57,10 @@ template <int E, bool TWO> struct TcCfg {
     static constexpr int OFF_RUN = OFF_MISC + 32;
     static constexpr int SMEM = OFF_RUN + RUN_RING * (int)sizeof(SplitRun);
     static_assert(SMEM <= (CTAS == 2 ? 115712 : 232448), "more shared memory than a CTA may use");
+    // The softmax warps wait for v_full and v_empty in some phases only.  They cannot take the phase before
+    // for the one they wait for: a job's S is complete after the PV of two jobs before, which used V's
+    // stage for the last time before this window if the stages are two or more.
+    static_assert(VS >= 2, "a phase of v_full or v_empty could be taken for another");
     // TMEM columns: scores (P over them) at 0 and KT, O
     static constexpr int COLS = CTAS == 2 ? 256 : 512, TM_O = CTAS == 2 ? 128 : 256;
 };

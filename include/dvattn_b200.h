@@ -266,7 +266,8 @@ typedef struct dvattn_mass_args {
  * positions starts[w] + i, every KV head keeps keep[w] of its own: the first `sink`, the last
  * `recent`, then those of largest mass (NaN after everything else; equal ones by position).
  * Survivors in front of keep[w] stay in place, the i-th freed position there is filled by the
- * i-th survivor behind it.  The range's pages belong to sequence w alone.
+ * i-th survivor behind it.  The range's pages belong to sequence w alone.  W * Hkv is at most
+ * 65535, max_blocks_per_seq * block_size below 2^31 (DVATTN_ERR_UNSUPPORTED otherwise).
  */
 typedef struct dvattn_evict_args {
     int dtype;
