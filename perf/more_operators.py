@@ -23,7 +23,7 @@ TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 SIZE = {"f32": 4, "f16": 2, "bf16": 2}
 F8 = torch.float8_e4m3fn
 TOP = 448.0  # the largest e4m3 value
-LEAST = 2.0 ** -100  # the smallest scale that the append sets
+LEAST = 2.0 ** -60  # the smallest scale that the append sets
 
 
 # ------------------------------------------------------------------------------------------------------------
@@ -316,7 +316,7 @@ def _plain_append(s):
         x = x.transpose(1, 2)[live].float()  # [tokens, Hkv, E]
         amax = torch.zeros((NB, Hkv), device=x.device).scatter_reduce_(0, page[:, None].expand(-1, Hkv), x.abs().amax(-1), "amax")
         m, e = torch.frexp(amax)  # amax = m 2^e, 0.5 <= m < 1; 448 = 0.875 2^9
-        e = torch.where(amax == 0, -100, e - 9 + (m > 0.875)).clamp(min=-100)
+        e = torch.where(amax == 0, -60, e - 9 + (m > 0.875)).clamp(min=-60)
         need = ((e + 127).int() << 23).view(torch.float32)  # 2^e, LEAST or more
         new = torch.where((began == 0)[:, None], need, torch.maximum(scales, need))
         new = torch.where(touched[:, None], new, scales)
