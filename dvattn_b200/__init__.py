@@ -32,19 +32,24 @@ _load()
 
 from .api import (  # noqa: E402
     apply_rotary_pos_emb,
+    dvattn_assign_pages,
     dvattn_build_views,
     dvattn_fused,
     dvattn_lse_merge,
     dvattn_paged_append,
+    dvattn_paged_append_q8,
     dvattn_paged_evict,
     dvattn_paged_mass,
     dvattn_paged_sdpa,
+    dvattn_paged_sdpa_q8,
     dvattn_paged_sdpa_rope,
+    dvattn_release_pages,
     dvattn_rope,
     dvattn_sdpa,
     dvattn_tree_append,
     dvattn_tree_sdpa,
     dvattn_varlen_paged_sdpa,
+    dvattn_varlen_paged_sdpa_q8,
     dvattn_varlen_paged_sdpa_rope,
     dvattn_varlen_rope,
     rotate_half,
@@ -52,19 +57,24 @@ from .api import (  # noqa: E402
 
 __all__ = [
     "apply_rotary_pos_emb",
+    "dvattn_assign_pages",
     "dvattn_build_views",
     "dvattn_fused",
     "dvattn_lse_merge",
     "dvattn_paged_append",
+    "dvattn_paged_append_q8",
     "dvattn_paged_evict",
     "dvattn_paged_mass",
     "dvattn_paged_sdpa",
+    "dvattn_paged_sdpa_q8",
     "dvattn_paged_sdpa_rope",
+    "dvattn_release_pages",
     "dvattn_rope",
     "dvattn_sdpa",
     "dvattn_tree_append",
     "dvattn_tree_sdpa",
     "dvattn_varlen_paged_sdpa",
+    "dvattn_varlen_paged_sdpa_q8",
     "dvattn_varlen_paged_sdpa_rope",
     "dvattn_varlen_rope",
     "rotate_half",

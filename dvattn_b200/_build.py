@@ -23,8 +23,9 @@ CAPI_SO = os.path.join(HERE, "libdvattn_b200.so")
 TORCH_SO = os.path.join(HERE, "dvatt.abi3.so")
 
 CU_SOURCES = ["decode.cu", "rope.cu", "merge.cu", "capi.cu", "noalloc.cu", "peer.cu", "prefill.cu", "append.cu", "tree_append.cu", "views.cu",
-              "rope_tables.cu", "tree.cu", "tree_tc.cu", "mass.cu", "mass_tc.cu", "evict.cu"]
-HEADERS = ["common.cuh", "schedule.cuh", "decode.cuh", "tma_host.cuh", "turns.cuh", "tree.cuh", "tcgen05.cuh", "windows.cuh", "mass.cuh"]
+              "rope_tables.cu", "tree.cu", "tree_tc.cu", "mass.cu", "mass_tc.cu", "evict.cu",
+              "decode_q8.cu", "varlen_q8.cu", "append_q8.cu", "pages.cu"]
+HEADERS = ["common.cuh", "schedule.cuh", "decode.cuh", "tma_host.cuh", "turns.cuh", "tree.cuh", "tcgen05.cuh", "windows.cuh", "mass.cuh", "q8.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -214,6 +214,77 @@ def dvattn_paged_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch
     return mass_out
 
 
+def dvattn_paged_sdpa_q8(queries: torch.Tensor, locations: torch.Tensor, cosines: torch.Tensor, sines: torch.Tensor,
+                         fragment_lengths: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         k_scales: torch.Tensor, v_scales: torch.Tensor, block_tables: torch.Tensor, scale: float,
+                         out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                         out_f32: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dvattn_paged_sdpa`` over a cache held in 8 bits: k/v cache [NB,BS,Hkv,E] float8_e4m3fn,
+    each element standing for itself times the scale of its page and KV head (k_scales /
+    v_scales [NB,Hkv] f32, as ``dvattn_paged_append_q8`` sets them).  Queries and output are
+    f32, f16 or bf16."""
+    if out is None:
+        out = torch.empty(queries.shape[:3] + (v_cache.size(3),), dtype=queries.dtype, device=queries.device)
+    _ops.dvattn_paged_sdpa_q8(out, lse, out_f32, scale, locations, queries, cosines, sines, fragment_lengths, k_cache,
+                              v_cache, k_scales, v_scales, block_tables)
+    return out
+
+
+def dvattn_varlen_paged_sdpa_q8(queries: torch.Tensor, locations: torch.Tensor, cosines: torch.Tensor,
+                                sines: torch.Tensor, fragment_lengths: torch.Tensor, k_cache: torch.Tensor,
+                                v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                                block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                                cu_seqlens_k: Optional[torch.Tensor], scale: float, out: Optional[torch.Tensor] = None,
+                                lse: Optional[torch.Tensor] = None,
+                                out_f32: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dvattn_varlen_paged_sdpa`` over a cache held in 8 bits (``dvattn_paged_sdpa_q8``).  The
+    pages that the tokens see are widened to the queries' dtype in a workspace of up to
+    min(NB, W * max_blocks) pages of both caches; a batch of single tokens is better off with
+    ``dvattn_paged_sdpa_q8``."""
+    if out is None:
+        out = torch.empty((queries.size(0), queries.size(1), v_cache.size(3)), dtype=queries.dtype,
+                          device=queries.device)
+    _ops.dvattn_varlen_paged_sdpa_q8(out, lse, out_f32, scale, locations, queries, cosines, sines, fragment_lengths,
+                                     k_cache, v_cache, k_scales, v_scales, block_tables, cu_seqlens_q,
+                                     cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k)
+    return out
+
+
+def dvattn_paged_append_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                           v_scales: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, cosines: torch.Tensor,
+                           sines: torch.Tensor, block_tables: torch.Tensor, positions: torch.Tensor,
+                           counts: Optional[torch.Tensor] = None) -> None:
+    """``dvattn_paged_append`` into a cache held in 8 bits (float8_e4m3fn, scales [NB,Hkv] f32, both
+    updated).  A page's scale is the least power of two (2^-60 or more) that brings its largest element to 448
+    or less; it grows with the page's tokens, and those that were there are stored again when it does.
+    Infinities become NaN.  Pages must not be shared; what lies behind a page's last new token is lost."""
+    _ops.dvattn_paged_append_q8(k_cache, v_cache, k_scales, v_scales, keys, values, cosines, sines, block_tables,
+                                positions, counts)
+
+
+def dvattn_assign_pages(block_tables: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                        starts: torch.Tensor, counts: torch.Tensor, block_size: int,
+                        granted: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Pages for the new tokens at logical positions starts[w] + i, i < counts[w] (i32 [W] each): entries of
+    ``block_tables`` [W,max_blocks] i32 that they fall on and that are negative take one from the free list,
+    a stack of free_count [1] i32 page numbers in free_pages [N] i32.  Sequences are served in order; one whose
+    pages, with those of all before it, are not there gets none.  Returns ``granted`` [W] i32: counts[w], or 0
+    for a sequence that was not served (what ``positions`` and ``counts`` of an append take).  ``slots``
+    ([W,n] int64, optional) gets page * block_size + offset of token i < granted[w], -1 elsewhere."""
+    if granted is None:
+        granted = torch.empty_like(counts)
+    _ops.dvattn_assign_pages(block_tables, free_pages, free_count, granted, slots, starts, counts, block_size)
+    return granted
+
+
+def dvattn_release_pages(block_tables: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                         keep: torch.Tensor, block_size: int) -> None:
+    """Give back the pages of sequence w that lie wholly at or behind logical position keep[w] (i32 [W]; 0: all of
+    them): their entries of ``block_tables`` become -1, the pages go on the free list in the order of
+    (w, entry), as far as it has room.  The pages must not be shared."""
+    _ops.dvattn_release_pages(block_tables, free_pages, free_count, keep, block_size)
+
+
 def dvattn_rope(queries: torch.Tensor, cosines: torch.Tensor, sines: torch.Tensor, out=None) -> torch.Tensor:
     """Same signature as python/dvattn/attention.py:68-72: out [F,W,Hq,S,E]."""
     if out is None:

@@ -72,6 +72,13 @@ EXPORTS = [
     "dvattn_paged_mass",
     "dvattn_paged_evict_workspace_size",
     "dvattn_paged_evict",
+    "dvattn_paged_sdpa_q8_workspace_size",
+    "dvattn_paged_sdpa_q8",
+    "dvattn_varlen_paged_sdpa_q8_workspace_size",
+    "dvattn_varlen_paged_sdpa_q8",
+    "dvattn_paged_append_q8",
+    "dvattn_assign_pages",
+    "dvattn_release_pages",
 ]
 
 _vp = ctypes.c_void_p
@@ -151,6 +158,21 @@ class EvictArgs(ctypes.Structure):
                 ("source", _vp), ("block_tables", _vp), ("starts", _vp), ("lengths", _vp), ("keep", _vp)]
 
 
+class Q8Scales(ctypes.Structure):
+    _fields_ = [("k_scales", _vp), ("v_scales", _vp)]
+
+
+class AssignArgs(ctypes.Structure):
+    _fields_ = [("W", _i), ("block_size", _i), ("max_blocks_per_seq", _i), ("free_size", _i), ("n", _i),
+                ("block_tables", _vp), ("free_pages", _vp), ("free_count", _vp), ("starts", _vp), ("counts", _vp),
+                ("granted", _vp), ("slots", _vp)]
+
+
+class ReleaseArgs(ctypes.Structure):
+    _fields_ = [("W", _i), ("block_size", _i), ("max_blocks_per_seq", _i), ("free_size", _i), ("block_tables", _vp),
+                ("free_pages", _vp), ("free_count", _vp), ("keep", _vp)]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -226,6 +248,15 @@ def lib() -> ctypes.CDLL:
             size, call = getattr(L, name + "_workspace_size"), getattr(L, name)
             size.restype, size.argtypes = ctypes.c_size_t, [ctypes.POINTER(args)]
             call.restype, call.argtypes = _i, [ctypes.POINTER(args), _vp, ctypes.c_size_t, _vp]
+        for name, args in (("dvattn_paged_sdpa_q8", PagedArgs), ("dvattn_varlen_paged_sdpa_q8", VarlenArgs)):
+            size, call = getattr(L, name + "_workspace_size"), getattr(L, name)
+            size.restype, size.argtypes = ctypes.c_size_t, [ctypes.POINTER(args)]
+            call.restype = _i
+            call.argtypes = [ctypes.POINTER(args), ctypes.POINTER(Q8Scales), _vp, ctypes.c_size_t, _vp]
+        L.dvattn_paged_append_q8.restype = _i
+        L.dvattn_paged_append_q8.argtypes = [ctypes.POINTER(AppendArgs), ctypes.POINTER(Q8Scales), _vp]
+        for name, args in (("dvattn_assign_pages", AssignArgs), ("dvattn_release_pages", ReleaseArgs)):
+            getattr(L, name).restype, getattr(L, name).argtypes = _i, [ctypes.POINTER(args), _vp]
         L.dvattn_tree_append.restype = _i
         L.dvattn_tree_append.argtypes = [ctypes.POINTER(TreeAppendArgs), _vp]
         _lib = L
@@ -657,3 +688,63 @@ def paged_evict(k_cache, v_cache, mass, block_tables, starts, lengths, keep, sin
                   mass.data_ptr(), (mass if mass_out is None else mass_out).data_ptr(), _ptr(source),
                   block_tables.data_ptr(), starts.data_ptr(), lengths.data_ptr(), keep.data_ptr())
     return _with_workspace("dvattn_paged_evict", a, mass.device, workspace)
+
+
+def _scales(k_scales, v_scales) -> Q8Scales:
+    return Q8Scales(_ptr(k_scales), _ptr(v_scales))
+
+
+def _with_scales(name, args, scales, device, workspace=None):
+    if workspace is None:
+        n = getattr(lib(), name + "_workspace_size")(ctypes.byref(args))
+        workspace = torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+    st = getattr(lib(), name)(ctypes.byref(args), ctypes.byref(scales), workspace.data_ptr(), workspace.numel(), _stream(None))
+    if st != DVATTN_OK:
+        raise DvattnError(st, name)
+    return workspace
+
+
+def paged_sdpa_q8(out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, k_scales, v_scales,
+                  block_tables, lse=None, out_f32=None, workspace=None):
+    """dvattn_paged_sdpa_q8 through the C ABI; returns the workspace."""
+    a = paged_args(out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, block_tables, lse,
+                   out_f32)
+    return _with_scales("dvattn_paged_sdpa_q8", a, _scales(k_scales, v_scales), out.device, workspace)
+
+
+def varlen_paged_sdpa_q8(out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, k_scales,
+                         v_scales, block_tables, cu_seqlens_q, lse=None, out_f32=None, workspace=None):
+    """dvattn_varlen_paged_sdpa_q8 through the C ABI; returns the workspace."""
+    a = varlen_args(out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, block_tables,
+                    cu_seqlens_q, lse, out_f32)
+    return _with_scales("dvattn_varlen_paged_sdpa_q8", a, _scales(k_scales, v_scales), out.device, workspace)
+
+
+def paged_append_q8(k_cache, v_cache, k_scales, v_scales, keys, values, cosines, sines, block_tables, positions, counts=None):
+    """dvattn_paged_append_q8 through the C ABI."""
+    W, Hkv, n, E = keys.shape
+    a = AppendArgs(_DTYPE.get(keys.dtype, -1), W, Hkv, E, values.size(3), n, cosines.size(2), k_cache.size(1),
+                   block_tables.size(1), k_cache.size(0), k_cache.data_ptr(), v_cache.data_ptr(), keys.data_ptr(),
+                   values.data_ptr(), _ptr(cosines), _ptr(sines), block_tables.data_ptr(), positions.data_ptr(), _ptr(counts))
+    st = lib().dvattn_paged_append_q8(ctypes.byref(a), ctypes.byref(_scales(k_scales, v_scales)), _stream(None))
+    if st != DVATTN_OK:
+        raise DvattnError(st, "dvattn_paged_append_q8")
+
+
+def assign_pages(block_tables, free_pages, free_count, starts, counts, block_size, granted, slots=None):
+    """dvattn_assign_pages through the C ABI."""
+    a = AssignArgs(block_tables.size(0), block_size, block_tables.size(1), free_pages.numel(), 0 if slots is None else slots.size(1),
+                   block_tables.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), starts.data_ptr(), counts.data_ptr(),
+                   granted.data_ptr(), _ptr(slots))
+    st = lib().dvattn_assign_pages(ctypes.byref(a), _stream(None))
+    if st != DVATTN_OK:
+        raise DvattnError(st, "dvattn_assign_pages")
+
+
+def release_pages(block_tables, free_pages, free_count, keep, block_size):
+    """dvattn_release_pages through the C ABI."""
+    a = ReleaseArgs(block_tables.size(0), block_size, block_tables.size(1), free_pages.numel(), block_tables.data_ptr(),
+                    free_pages.data_ptr(), free_count.data_ptr(), keep.data_ptr())
+    st = lib().dvattn_release_pages(ctypes.byref(a), _stream(None))
+    if st != DVATTN_OK:
+        raise DvattnError(st, "dvattn_release_pages")

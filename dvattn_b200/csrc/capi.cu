@@ -100,6 +100,32 @@ int dvattn_paged_evict(const dvattn_evict_args* args, void* workspace, size_t wo
     return dvb::evict_launch(args, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
+size_t dvattn_paged_sdpa_q8_workspace_size(const dvattn_paged_args* args) { return dvb::decode_q8_workspace_size(args); }
+
+int dvattn_paged_sdpa_q8(const dvattn_paged_args* args, const dvattn_q8_scales* scales, void* workspace, size_t workspace_bytes,
+                         dvattn_stream_t stream) {
+    return dvb::decode_q8_launch(args, scales, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t dvattn_varlen_paged_sdpa_q8_workspace_size(const dvattn_varlen_args* args) { return dvb::varlen_q8_workspace_size(args); }
+
+int dvattn_varlen_paged_sdpa_q8(const dvattn_varlen_args* args, const dvattn_q8_scales* scales, void* workspace,
+                                size_t workspace_bytes, dvattn_stream_t stream) {
+    return dvb::varlen_q8_launch(args, scales, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int dvattn_paged_append_q8(const dvattn_append_args* args, const dvattn_q8_scales* scales, dvattn_stream_t stream) {
+    return dvb::append_q8_launch(args, scales, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int dvattn_assign_pages(const dvattn_assign_args* args, dvattn_stream_t stream) {
+    return dvb::assign_pages_launch(args, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int dvattn_release_pages(const dvattn_release_args* args, dvattn_stream_t stream) {
+    return dvb::release_pages_launch(args, reinterpret_cast<cudaStream_t>(stream));
+}
+
 size_t dvattn_sdpa_workspace_size(const dvattn_sdpa_args* args) { return dvb::sdpa_workspace_size(args); }
 
 int dvattn_sdpa(const dvattn_sdpa_args* args, void* workspace, size_t workspace_bytes, dvattn_stream_t stream) {

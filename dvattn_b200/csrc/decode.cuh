@@ -37,6 +37,15 @@ size_t mass_workspace_size(const dvattn_mass_args* a);
 int mass_launch(const dvattn_mass_args* a, void* workspace, size_t wbytes, cudaStream_t stream);
 size_t evict_workspace_size(const dvattn_evict_args* a);
 int evict_launch(const dvattn_evict_args* a, void* workspace, size_t wbytes, cudaStream_t stream);
+// the cache held in 8 bits: decode attention (decode_q8.cu), varlen attention (varlen_q8.cu), append (append_q8.cu)
+size_t decode_q8_workspace_size(const dvattn_paged_args* a);
+int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream);
+size_t varlen_q8_workspace_size(const dvattn_varlen_args* a);
+int varlen_q8_launch(const dvattn_varlen_args* a, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream);
+int append_q8_launch(const dvattn_append_args* a, const dvattn_q8_scales* sc, cudaStream_t stream);
+// pages from a free list and back (pages.cu)
+int assign_pages_launch(const dvattn_assign_args* a, cudaStream_t stream);
+int release_pages_launch(const dvattn_release_args* a, cudaStream_t stream);
 // contiguous fragments (the dvattn_sdpa op)
 size_t sdpa_workspace_size(const dvattn_sdpa_args* a);
 int sdpa_launch(const dvattn_sdpa_args* a, void* workspace, size_t wbytes, cudaStream_t stream);

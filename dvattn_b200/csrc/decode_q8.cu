@@ -1,0 +1,1212 @@
+// Paged multi-turn decode attention over a cache held in 8 bits (q8.cuh): for token s of sequence w and
+// its query head h of KV head k,
+//
+//   out = sum_l softmax_l(scale * rot_f(q) . (K8_l sk)) (V8_l sv)
+//
+// over the keys l that (w, s) sees in every turn f, the query rotated for the turn and rounded to its
+// type, sk and sv the scales of the key's page and head.  Two launches: the attention and the merge of
+// the items that more than one CTA worked on; each is a programmatic dependent of the one before it.
+//
+// Numerics.  e4m3 is exact in f16, so K and V are widened to f16 in registers and multiplied on
+// mma.sync with 32-bit accumulation; the scales never touch them.  q's row is multiplied by a power of
+// two that brings its largest element to 2^13 .. 2^14 and written as one f16 value (f16 and bf16 queries:
+// exact, but for elements under 2^-27 of the row's largest) or two (f32: hi + lo, 2^-24 of an
+// element), undone in the scores.  With sv = 2^e m (1 <= m < 2), z = log2-score + e is what the running
+// maximum r is taken over: P = 2^(z - r + 7), the numerator adds (P m) V8, the denominator P 2^-e, both in
+// units of 2^r, so pages of any scales meet in one accumulator.  P m is rounded to f16 (f32: to a hi
+// + lo pair) next to V; the denominator adds the unrounded P.  The 7 powers of two keep weights down to
+// 2^-21 of the largest at full precision and drop those under 2^-32.  r moves when the maximum has grown by
+// more than 6 (P stays below 2^14), so that the accumulators are rarely rescaled.
+//
+// Bound: HBM, a byte per cached element.  A CTA reads a page's rows of up to four KV heads together (contiguous
+// in HBM) by TMA, a warp works on 32 keys (head dim 256: 16) of one head.
+#include "decode.cuh"
+#include "q8.cuh"
+#include "tma_host.cuh"
+#include "turns.cuh"
+
+#include <cstdio>
+#include <cstdlib>
+
+namespace dvb {
+
+struct Q8Params : TurnSplit {
+    // of TurnSplit: F, BS, maxb, cap, NB, kt, nt, align, loc, L, bt; W: sequences of this launch
+    int w0;                 // its first sequence
+    int Hq, Hkv, G, S, R, rows;
+    int hc, hs;             // KV heads a CTA reads together, groups of them (hc * hs = Hkv)
+    int pairs;              // W * nt (sequence, row tile) pairs
+    int box, box_shift;     // rows of a TMA box (gathered: rows of the stage), its log2
+    int gather;             // pages are no whole boxes: rows are copied one by one
+    int sc_shift;           // log2 of the keys that share an entry of the stage's scales
+    long long tokens;       // all sequences' (a turn's stride in loc and cos / sin)
+    int stall_tile;         // test hook (DVATTN_TEST_STALL_TILE), -1: off
+    float scale_log2;
+    void* out;
+    float* lse_out;
+    float* out_f32;
+    const void* q;
+    const float* cos;
+    const float* sin;
+    const uint8_t* k;
+    const uint8_t* v;
+    const float* ks;
+    const float* vs;
+    // workspace
+    int* header;            // [3] error word (kErrorWordOffset)
+    long long* P;           // [pairs + 1] windows in front of a pair (of one head group)
+    float* part_o;          // [CTAs][2][hc][rows of a tile][E]
+    float* part_lse;        // [CTAs][2][hc][rows of a tile] log2 sums, -inf: nothing seen
+};
+
+constexpr int kQ8Warps = 4;
+constexpr int kQ8MaxPairs = 4096;  // their prefix sums lie in the stages at first
+
+// E: head dim, MT: 16-row tiles of a KV head's query rows, TERMS: f16 values per query element and weight.
+template <int E, int MT, int TERMS> struct Q8Cfg {
+    static constexpr int KPW = E == 256 ? 16 : 32;      // keys of a warp in a window
+    static constexpr int KROWS = kQ8Warps * KPW;        // (key, head) rows of a stage
+    static constexpr int TENSOR = KROWS * E;            // bytes of K (or V) in a stage
+    static constexpr int NT = KPW / 8;                  // 8-key tiles
+    static constexpr int KS = E / 16;                   // 16-deep steps of q . k
+    static constexpr int NJ = E / 8;                    // 8-column tiles of the output
+    static constexpr bool QREG = KS * MT * TERMS <= 8;  // q fragments in registers, else a lane keeps its own in shared memory
+    static constexpr int QBYTES = QREG ? 0 : kQ8Warps * KS * MT * TERMS * 512;
+    static constexpr int ROWS = 16 * MT;
+    static constexpr int CTAS = QBYTES + 4 * TENSOR > 100 * 1024 ? 1 : 2;  // per SM
+    static constexpr int ROOM = (CTAS == 2 ? 113 : 226) * 1024 - QBYTES - 6 * 1024;
+    static constexpr int STAGES = ROOM / (2 * TENSOR) > 6 ? 6 : ROOM / (2 * TENSOR);
+    static constexpr size_t OFF_Q = (size_t)STAGES * 2 * TENSOR;
+    static constexpr size_t OFF_SC = OFF_Q + QBYTES;                   // [STAGES][2][KROWS] scales
+    static constexpr size_t OFF_ML = OFF_SC + STAGES * 2 * KROWS * 4;  // [warps][ROWS][2]
+    static constexpr size_t OFF_DESC = OFF_ML + kQ8Warps * ROWS * 2 * 4;
+    static constexpr size_t OFF_BAR = OFF_DESC + STAGES * 48;
+    static constexpr size_t OFF_FLAG = OFF_BAR + STAGES * 16;
+    static constexpr size_t SMEM = OFF_FLAG + 16;
+    static_assert(STAGES >= 2 && OFF_Q >= (kQ8MaxPairs + 40) * 8, "the prefix sums fit in the stages");
+    static_assert(SMEM <= (CTAS == 2 ? 113 : 227) * 1024, "shared memory");
+    static_assert(2 * TENSOR >= 2 * ROWS * E * 4, "two heads' rows are combined in a stage");
+};
+
+// ---- the windows of a (sequence, row tile) pair ------------------------------------------
+__device__ __forceinline__ void tile_tokens(const Q8Params& p, int rows, int t, int& s0, int& s1) {
+    s0 = t * rows / p.G;
+    s1 = (min((t + 1) * rows, p.rows) - 1) / p.G;
+}
+// by one thread
+__device__ __forceinline__ int pair_windows(const Q8Params& p, int rows, int pair) {
+    const int w = p.w0 + pair / p.nt, t = pair % p.nt;
+    int s0, s1, nw = 0;
+    tile_tokens(p, rows, t, s0, s1);
+    long long off = 0;
+    for (int f = 0; f < p.F; ++f) {
+        const int L = __ldg(p.L + f);
+        int sp = 0;
+        for (int s = s0; s <= s1; ++s) sp = max(sp, turn_seen(L, __ldg(p.loc + f * p.tokens + (size_t)w * p.S + s), off, p.cap));
+        nw += turn_windows(p, sp, sp > 0 ? (int)off : 0);
+        off += max(L, 0);
+    }
+    return nw;
+}
+
+// CTA c's units [begin(c), begin(c + 1)): windows of all pairs and head groups, evenly split.
+struct Q8Split {
+    long long q, r;
+    int n;
+    __device__ __forceinline__ Q8Split(long long total, const Q8Params& p, int ctas) {
+        const long long most = total / p.least;
+        n = most < ctas ? (most > 0 ? (int)most : 1) : ctas;
+        q = total / n;
+        r = total % n;
+    }
+    __device__ __forceinline__ long long begin(int c) const {
+        if (c > n) c = n;
+        return c * q + (c < r ? c : r);
+    }
+    __device__ __forceinline__ int cta_of(long long u) const {
+        const long long more = r * (q + 1);
+        return (int)(u < more ? u / (q + 1) : r + (u - more) / q);
+    }
+};
+
+// What a stage holds: window [k0, k0 + kt) of turn f for head group hg of pair (w, t).
+struct alignas(16) Q8Stage {
+    int w, t, hg, f;
+    int off, k0, sp, how;  // the turn's first position, first key, seen keys; Q8_* bits, -1: the end
+    int pad[4];
+};
+constexpr int Q8_ITEM = 1, Q8_TURN = 2, Q8_LAST = 4, Q8_WHOLE = 8, Q8_BEGIN = 16;
+
+// Walks units [u, u1) by a whole warp; every lane holds the same values.
+struct Q8Walk {
+    long long rem;
+    int pair, hg, f, wi, left;  // wi: window of the turn, left: windows of the turn that are left
+    int sp, off;
+    long long off64;
+    bool item, turn;  // the next window begins an item's piece, a turn
+    bool begin;       // the piece begins its item
+
+    __device__ __forceinline__ void enter(const Q8Params& p, int rows, int lane) {  // turn f
+        const int w = p.w0 + pair / p.nt, t = pair % p.nt, L = __ldg(p.L + f);
+        int s0, s1, v = 0;
+        tile_tokens(p, rows, t, s0, s1);
+        for (int s = s0 + lane; s <= s1; s += 32) v = max(v, turn_seen(L, __ldg(p.loc + f * p.tokens + (size_t)w * p.S + s), off64, p.cap));
+        sp = __reduce_max_sync(0xffffffffu, v);
+        off = sp > 0 ? (int)off64 : 0;
+        off64 += max(L, 0);
+        left = turn_windows(p, sp, off);
+        wi = 0;
+        turn = true;
+    }
+    __device__ __forceinline__ void start(const Q8Params& p, int rows, int lane, int pair_, int hg_, int i, long long n) {
+        pair = pair_, hg = hg_, rem = n, begin = i == 0, item = true;
+        f = 0, off64 = 0;
+        enter(p, rows, lane);
+        while (i >= left) {
+            i -= left;
+            ++f;
+            enter(p, rows, lane);
+        }
+        wi = i;
+        left -= i;
+    }
+    // The next window; false: none.  `ended`: the windows handed out before end their item.
+    __device__ __forceinline__ bool next(const Q8Params& p, int rows, int lane, Q8Stage& d, bool& ended) {
+        ended = false;
+        while (left == 0) {
+            if (f + 1 < p.F) {
+                ++f;
+            } else {
+                ended = item = begin = true;
+                if (rem == 0) return false;
+                f = 0, off64 = 0;
+                if (++hg == p.hs) {
+                    hg = 0;
+                    if (++pair >= p.pairs) {
+                        rem = 0;
+                        return false;
+                    }
+                }
+            }
+            enter(p, rows, lane);
+        }
+        if (rem == 0) return false;
+        d.w = p.w0 + pair / p.nt, d.t = pair % p.nt, d.hg = hg, d.f = f, d.off = off, d.sp = sp;
+        d.k0 = wi * p.kt - (off & (p.align - 1));
+        d.how = (item ? Q8_ITEM : 0) | (turn ? Q8_TURN : 0) | (begin ? Q8_BEGIN : 0);
+        item = turn = false;
+        ++wi, --left, --rem;
+        return true;
+    }
+};
+
+// ---- small helpers ------------------------------------------------------------------------
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {  // when this thread's copies so far have landed
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) { return Elem<__half>::pack2(a, b); }
+
+// v = 2^e m of a scale (file comment), e at least -60; what is not finite or not positive comes out in m.
+struct Scale {
+    float e, m, inv;  // inv = 2^-e
+    __device__ __forceinline__ Scale(float v) {
+        const int b = __float_as_int(v), x = b & 0x7f800000;
+        const bool low = b < (67 << 23), odd = x == 0x7f800000;
+        e = low ? -60.f : __int_as_float((b >> 23) + 0x4b000000) - (8388608.f + 127.f);
+        m = low ? v * 0x1p60f : odd ? v : __int_as_float((b & 0x7fffff) | 0x3f800000);
+        inv = low ? 0x1p60f : odd ? 0x1p-128f : __int_as_float(0x7f000000 - x);
+    }
+};
+__device__ const float kOne = 1.f;
+
+// ---- the attention kernel ---------------------------------------------------------------------
+// Warps 0 .. 3 compute, warp 4 requests the windows.  Warp w works on head w % hc of the group and keys
+// [KPW (w / hc), + KPW) of the window; thread (n, t) = (lane / 4, lane % 4).
+//
+// Fragments.  The order of the elements in q . k and of the keys in P V is free as long as both operands
+// share it, so every fragment comes from whole 16-byte words of a stage:
+// * K: 8-key tile x, column n is key 8x + k(n), k(n) = n / 2 + 4 (n % 2); step 4i + u takes bytes 4u .. 4u + 3
+//   of 16-byte chunk t + 4i.  Neighbouring n lie 4 rows apart, which the 128-byte swizzle puts in different banks.
+// * the scores a thread then holds of a tile are those of keys 8x + t and 8x + t + 4: the rows whose V words it
+//   loads.  V: column n of output tile j of a 128-byte panel is element 16 c(n) + j, c(n) = k(n); the bytes of
+//   two rows are interleaved and widened in pairs.  A thread ends with 16 neighbouring elements twice.
+// * head dim 64: rows of 64 bytes; V words of 8 bytes, tile j of column n is element 8 c(n) + j with
+//   c(n) = n % 2 + 4 (n / 2 % 2) + 2 (n / 4).
+template <class T, int E, int MT>
+__global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1>::CTAS))
+    decode_q8_kernel(const __grid_constant__ Q8Params p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
+    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+    using C = Q8Cfg<E, MT, TERMS>;
+    constexpr int KPW = C::KPW, NT = C::NT, KS = C::KS, NJ = C::NJ, STAGES = C::STAGES, ROWS = C::ROWS;
+    constexpr int RB = E < 128 ? E : 128;  // bytes of a swizzled row
+    constexpr int NP = E / RB;             // panels
+    constexpr int NTH = (kQ8Warps + 1) * 32;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t s0 = smem_u32(smem);
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    const uint32_t bar_full = s0 + (uint32_t)C::OFF_BAR, bar_empty = bar_full + STAGES * 8;
+    volatile int* stop = reinterpret_cast<volatile int*>(smem + C::OFF_FLAG);
+    Q8Stage* desc = reinterpret_cast<Q8Stage*>(smem + C::OFF_DESC);
+    if (tid == 0) {
+        for (int st = 0; st < STAGES; ++st) {
+            mbar_init(bar_full + st * 8, 33);  // the request and the loading lanes' copies
+            mbar_init(bar_empty + st * 8, kQ8Warps);
+        }
+        *stop = 0;
+        fence_mbar_init();
+    }
+    // a programmatic dependent of whatever is before it: nothing is read or written earlier
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int c = blockIdx.x;
+    const bool aligned = (s0 & 1023) == 0;  // as the swizzle needs the stages
+    // cleared once per call: a bounded wait that gives up sets its bit long after
+    if (c == 0 && tid == 0 && (p.w0 == 0 || !aligned)) p.header[3] = aligned ? 0 : 4;
+    if (!aligned) return;
+
+    // ---- the split: every CTA adds up the windows of all pairs and finds its own range ----
+    long long* sP = reinterpret_cast<long long*>(smem);  // [pairs + 1], in the stages
+    long long* scratch = sP + p.pairs + 1;
+    long long carry = 0;
+    for (int base = 0; base < p.pairs; base += NTH) {
+        const int pair = base + tid;
+        const long long own = pair < p.pairs ? pair_windows(p, ROWS, pair) : 0;
+        long long x = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) scratch[wid] = x;
+        __syncthreads();
+        long long before = carry;
+        for (int y = 0; y < NTH / 32; ++y) {
+            if (y < wid) before += scratch[y];
+            carry += scratch[y];
+        }
+        if (pair < p.pairs) sP[pair] = before + x - own;
+        __syncthreads();
+    }
+    if (tid == 0) sP[p.pairs] = carry;
+    __syncthreads();
+    for (int i = c * NTH + tid; i <= p.pairs; i += gridDim.x * NTH) p.P[i] = sP[i];  // for the merge
+    const Q8Split split(carry * p.hs, p, gridDim.x);
+    const long long u0 = split.begin(c), u1 = split.begin(c + 1);
+    if (u0 >= u1) return;
+    int pair0 = 0;
+    {
+        int hi = p.pairs - 1;
+        while (pair0 < hi) {  // the last pair that begins at or before u0; those without windows begin with the next
+            const int mid = (pair0 + hi + 1) >> 1;
+            if (sP[mid] * p.hs <= u0) pair0 = mid; else hi = mid - 1;
+        }
+    }
+    const long long local = u0 - sP[pair0] * p.hs;
+    const int nw0 = (int)(sP[pair0 + 1] - sP[pair0]);
+    const int hg0 = (int)(local / nw0), i0 = (int)(local - (long long)hg0 * nw0);
+    fence_proxy_async_smem();  // TMA writes where the sums lay
+    __syncthreads();
+
+    if (wid == kQ8Warps) {
+        // ======================= the requesting warp =======================
+        const int boxes = p.kt >> p.box_shift;
+        if (lane == 0 && !p.gather) {
+            prefetch_tmap(&mk);
+            prefetch_tmap(&mv);
+        }
+        Q8Walk walk;
+        walk.start(p, ROWS, lane, pair0, hg0, i0, u1 - u0);
+        Q8Stage cur, nxt;
+        int page[4] = {-1, -1, -1, -1};  // of the next window: lane's box, or (gathered) keys lane + 32 x; -1: none
+        bool have, ended;
+        auto find = [&] {
+            have = walk.next(p, ROWS, lane, nxt, ended);
+            if (!have) return;
+            const int n = p.gather ? p.kt : boxes, step = p.gather ? 1 : p.box;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int i = lane + 32 * x, l = nxt.k0 + i * step;
+                page[x] = -1;
+                if (i < n && l + step > 0 && l < nxt.sp) {
+                    const int g = __ldg(p.bt + (size_t)nxt.w * p.maxb + (nxt.off + l) / p.BS);
+                    if (g >= 0 && g < p.NB) page[x] = g;
+                }
+                if (!p.gather) break;
+            }
+        };
+        find();
+        bool ok = true;
+        int i = 0;
+        for (;; ++i) {
+            const int st = i % STAGES;
+            if (i >= STAGES && (__any_sync(0xffffffffu, *stop != 0) || !__all_sync(0xffffffffu, mbar_wait(bar_empty + st * 8, (i / STAGES - 1) & 1)))) {
+                ok = false;
+                break;
+            }
+            if (!have) {
+                if (lane == 0) {
+                    desc[st].how = -1;
+                    mbar_arrive(bar_full + st * 8);
+                }
+                mbar_arrive(bar_full + st * 8);
+                break;
+            }
+            cur = nxt;
+            int pg[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) pg[x] = page[x];
+            find();  // a window ahead: its table entries are under way while this one waits
+            // the item's piece ends here where the next window begins another or there is none
+            if (!have || (nxt.how & Q8_ITEM)) cur.how |= Q8_LAST | (ended && (cur.how & Q8_BEGIN) ? Q8_WHOLE : 0);
+            if (i == p.stall_tile && c == 0) continue;  // test hook: this stage is never filled
+            const uint32_t dk = s0 + (uint32_t)(st * 2 * C::TENSOR), dv = dk + C::TENSOR, full = bar_full + st * 8;
+            if (lane == 0) {
+                desc[st] = cur;
+                if (p.gather) mbar_arrive(full);
+                else mbar_expect_tx(full, 2u * C::TENSOR);
+            }
+            __syncwarp();
+            const uint32_t sc = s0 + (uint32_t)C::OFF_SC + (uint32_t)(st * 2 * C::KROWS * 4);
+            if (!p.gather) {
+                if (lane < boxes) {
+                    const int pos = cur.off + cur.k0 + lane * p.box;
+                    const int z = pg[0] >= 0 ? pg[0] * p.BS + pos % p.BS : -2 * p.box;  // rows outside: zeros
+                    const uint32_t at = (uint32_t)(lane * p.box * p.hc * E);
+                    tma_load_4d(dk + at, &mk, 0, z, 0, cur.hg * p.hc, full);
+                    tma_load_4d(dv + at, &mv, 0, z, 0, cur.hg * p.hc, full);
+                }
+                // scales of groups of 8 keys, [group][head]: K's, then V's
+                const int per = p.kt / 8 * p.hc;
+                for (int x = lane; x < ((2 * per + 31) & ~31); x += 32) {
+                    const int y = x < per ? x : x - per, g = y / p.hc;
+                    const int b = __shfl_sync(0xffffffffu, pg[0], (g * 8) >> p.box_shift & 31);
+                    if (x < 2 * per)
+                        cp_async4(sc + 4 * (y + (x < per ? 0 : C::KROWS)),
+                                  b >= 0 ? (x < per ? p.ks : p.vs) + (size_t)b * p.Hkv + cur.hg * p.hc + y % p.hc : &kOne);
+                }
+            } else {
+                // 16-byte chunk ch of row (head, key): [head][panel][KT keys][RB bytes], swizzled as TMA writes it
+                constexpr int CH = E / 16;
+                for (int x = lane; x < C::KROWS * CH; x += 32) {
+                    const int row = x / CH, ch = x % CH, hh = row / p.kt, key = row - hh * p.kt;
+                    const int k32 = key >> 5;
+                    const int p0 = __shfl_sync(0xffffffffu, pg[0], key & 31), p1 = __shfl_sync(0xffffffffu, pg[1], key & 31);
+                    const int p2 = __shfl_sync(0xffffffffu, pg[2], key & 31), p3 = __shfl_sync(0xffffffffu, pg[3], key & 31);
+                    const int b = k32 == 0 ? p0 : k32 == 1 ? p1 : k32 == 2 ? p2 : p3;
+                    const int pos = cur.off + cur.k0 + key;
+                    const size_t at = b >= 0 ? (((size_t)b * p.BS + pos % p.BS) * p.Hkv + cur.hg * p.hc + hh) * E + ch * 16 : 0;
+                    const uint32_t panel = (uint32_t)((hh * NP + ch / (RB / 16)) * p.kt + key) * RB;
+                    const uint32_t to = panel + (uint32_t)((RB == 128 ? (ch & 7) ^ (key & 7) : ch ^ (key >> 1 & 3)) << 4);
+                    cp_async16_zfill(dk + to, p.k + at, b >= 0 ? 16 : 0);
+                    cp_async16_zfill(dv + to, p.v + at, b >= 0 ? 16 : 0);
+                }
+                for (int x = lane; x < C::KROWS; x += 32) {  // scales, [key][head]
+                    const int key = x / p.hc, k32 = key >> 5;
+                    const int p0 = __shfl_sync(0xffffffffu, pg[0], key & 31), p1 = __shfl_sync(0xffffffffu, pg[1], key & 31);
+                    const int p2 = __shfl_sync(0xffffffffu, pg[2], key & 31), p3 = __shfl_sync(0xffffffffu, pg[3], key & 31);
+                    const int b = k32 == 0 ? p0 : k32 == 1 ? p1 : k32 == 2 ? p2 : p3;
+                    const size_t at = (size_t)b * p.Hkv + cur.hg * p.hc + x % p.hc;
+                    cp_async4(sc + 4 * x, b >= 0 ? p.ks + at : &kOne);
+                    cp_async4(sc + 4 * (x + C::KROWS), b >= 0 ? p.vs + at : &kOne);
+                }
+            }
+            cp_async_arrive(full);
+        }
+        if (!ok) {
+            if (lane == 0) {
+                *stop = 1;
+                atomicOr(p.header + 3, 1);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            for (int j = max(0, i - STAGES); j < i; ++j)  // what was requested lands first (bounded)
+                if (j != p.stall_tile || c != 0) mbar_wait(bar_full + (j % STAGES) * 8, (j / STAGES) & 1);
+        }
+        return;
+    }
+
+    // =========================== computing warps ===========================
+    const int n = lane >> 2, t = lane & 3;
+    const int hh = wid % p.hc, grp = wid / p.hc, wph = kQ8Warps / p.hc;  // head of the group, warps per head
+    const int kw = grp * KPW;                                            // first key of the window
+    const int kn = (n >> 1) | ((n & 1) << 2);
+    // 8-key tile x: its rows' place in a stage's K (V), a panel further: + panel
+    uint32_t tile[NT];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        const int key = kw + 8 * x, b = key >> p.box_shift;
+        tile[x] = (uint32_t)(((b * p.hc + hh) * NP * p.box + (key & (p.box - 1))) * RB);
+    }
+    const uint32_t panel = (uint32_t)(p.box * RB);
+    uint32_t kofs[E < 128 ? 1 : 2], vofs[2];  // a thread's chunks in a tile
+    if constexpr (E >= 128) {
+        kofs[0] = (uint32_t)(kn * 128 + ((t ^ kn) << 4));
+        kofs[1] = (uint32_t)(kn * 128 + (((t + 4) ^ kn) << 4));
+        vofs[0] = (uint32_t)(t * 128 + ((kn ^ t) << 4));
+        vofs[1] = (uint32_t)((t + 4) * 128 + ((kn ^ (t + 4)) << 4));
+    } else {
+        const int cn = (n & 1) | ((n & 2) << 1) | ((n & 4) >> 1);
+        kofs[0] = (uint32_t)(kn * 64 + ((t ^ (kn >> 1 & 3)) << 4));
+        vofs[0] = (uint32_t)(t * 64 + (((cn >> 1) ^ (t >> 1)) << 4) + ((cn & 1) << 3));
+        vofs[1] = (uint32_t)((t + 4) * 64 + (((cn >> 1) ^ ((t + 4) >> 1 & 3)) << 4) + ((cn & 1) << 3));
+    }
+    const uint32_t sQ = s0 + (uint32_t)C::OFF_Q + (uint32_t)(wid * KS * MT * TERMS * 512 + lane * 16);
+    float* sML = reinterpret_cast<float*>(smem + C::OFF_ML);
+    const bool vec = p.R % 16 == 0 && !((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15);
+
+    uint32_t qf[C::QREG ? MT * TERMS * KS : 1][4];
+    float fr[MT][2];   // log2(e) * scale / (the row's power of two)
+    int lim[MT][2];    // keys of the turn that the row sees
+    int least = 0;     // that every row of the warp sees
+    float o[MT][NJ][4], r[MT][2], l[MT][2];
+
+    auto load_q = [&](const Q8Stage& d) {
+        const int h = d.hg * p.hc + hh;
+        const int L = __ldg(p.L + d.f);
+        least = 0x7fffffff;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = d.t * ROWS + mt * 16 + half * 8 + n;
+                const bool there = row < p.rows;
+                const int s = there ? row / p.G : 0, g = there ? row - s * p.G : 0;
+                const size_t tk = (size_t)d.w * p.S + s;
+                const T* x = static_cast<const T*>(p.q) + (((size_t)d.w * p.Hq + h * p.G + g) * p.S + s) * E;
+                const float* cr = p.cos + (d.f * p.tokens + tk) * p.R;
+                const float* sr = p.sin + (d.f * p.tokens + tk) * p.R;
+                lim[mt][half] = there ? turn_seen(L, __ldg(p.loc + d.f * p.tokens + tk), d.off, p.cap) : d.sp;
+                least = min(least, lim[mt][half]);
+                uint32_t raw[TERMS == 1 ? KS * 2 : 1];  // T pairs
+                float val[TERMS == 1 ? 1 : KS * 4];
+                float top = 0.f;
+#pragma unroll
+                for (int e8 = 0; e8 < KS / 2; ++e8) {  // 8 elements: chunk t + 4 (e8 / 2), half e8 % 2
+                    float v[8];
+                    rotated8<T, false>(x, cr, sr, 16 * (t + 4 * (e8 >> 1)) + 8 * (e8 & 1), p.R, vec, v);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        if (!there) v[u] = 0.f;
+                        top = fmaxf(top, fabsf(v[u]));
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        if constexpr (TERMS == 1) {
+                            raw[e8 * 4 + u] = Elem<T>::pack2(v[2 * u], v[2 * u + 1]);
+                        } else {
+                            val[e8 * 8 + 2 * u] = v[2 * u];
+                            val[e8 * 8 + 2 * u + 1] = v[2 * u + 1];
+                        }
+                    }
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int shift = min(140 - (__float_as_int(top) >> 23), 126);
+                const float mul = __int_as_float((127 + shift) << 23);
+                fr[mt][half] = p.scale_log2 * __int_as_float((127 - shift) << 23);
+                // step ks = 4i + u: a[half] = elements 4u, 4u + 1 of the chunk, a[2 + half] = 4u + 2, 4u + 3
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    float v[4];
+                    if constexpr (TERMS == 1) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) v[u] = Elem<T>::to_f(reinterpret_cast<const T*>(&raw[ks * 2 + (u >> 1)])[u & 1]) * mul;
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) v[u] = val[ks * 4 + u] * mul;
+                    }
+#pragma unroll
+                    for (int term = 0; term < TERMS; ++term) {
+                        const uint32_t lo = pack_f16(v[0], v[1]), hi = pack_f16(v[2], v[3]);
+                        const int at = (mt * TERMS + term) * KS + ks;
+                        if constexpr (C::QREG) {
+                            qf[at][half] = lo;
+                            qf[at][2 + half] = hi;
+                        } else {
+                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(sQ + at * 512 + half * 4), "r"(lo) : "memory");
+                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(sQ + at * 512 + 8 + half * 4), "r"(hi) : "memory");
+                        }
+                        const __half2 a = *reinterpret_cast<const __half2*>(&lo), b = *reinterpret_cast<const __half2*>(&hi);
+                        v[0] -= __low2float(a), v[1] -= __high2float(a), v[2] -= __low2float(b), v[3] -= __high2float(b);
+                    }
+                }
+            }
+        }
+        least = __reduce_min_sync(0xffffffffu, least);
+    };
+
+    for (int i = 0;; ++i) {
+        const int st = i % STAGES;
+        if (wph > 1 ? named_bar_or(1, kQ8Warps * 32, *stop != 0) : __any_sync(0xffffffffu, *stop != 0)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar_full + st * 8, (i / STAGES) & 1))) {
+            if (lane == 0) {
+                *stop = 1;
+                atomicOr(p.header + 3, 2);
+            }
+            __syncwarp();
+            continue;
+        }
+        const Q8Stage d = desc[st];
+        if (d.how < 0) break;
+        if (d.how & Q8_ITEM)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                r[mt][0] = r[mt][1] = neg_inf();
+                l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
+            }
+        if (d.how & (Q8_ITEM | Q8_TURN)) load_q(d);
+
+        const int first = d.k0 + kw;  // key of the warp's first column
+        if (first < d.sp && first + KPW > 0) {
+            const uint32_t kb = s0 + (uint32_t)(st * 2 * C::TENSOR), vb = kb + C::TENSOR;
+            const uint32_t sc = s0 + (uint32_t)C::OFF_SC + (uint32_t)(st * 2 * C::KROWS * 4);
+            const bool edge = first < 0 || first + KPW > least;
+            // ---- scores ----
+            float z[MT][NT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int x = 0; x < NT; ++x) z[mt][x][0] = z[mt][x][1] = z[mt][x][2] = z[mt][x][3] = 0.f;
+#pragma unroll
+            for (int ci = 0; ci < E / 64; ++ci) {
+                uint4 kf[NT];
+#pragma unroll
+                for (int x = 0; x < NT; ++x) kf[x] = lds128(kb + tile[x] + (ci >> 1) * panel + kofs[E < 128 ? 0 : ci & 1]);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int ks = 4 * ci + u;
+                    uint32_t a[MT * TERMS][4];
+#pragma unroll
+                    for (int y = 0; y < MT * TERMS; ++y) {
+                        if constexpr (C::QREG) {
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) a[y][v] = qf[y * KS + ks][v];
+                        } else {
+                            const uint4 v = lds128(sQ + (uint32_t)((y * KS + ks) * 512));
+                            a[y][0] = v.x, a[y][1] = v.y, a[y][2] = v.z, a[y][3] = v.w;
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                        const uint32_t word = u == 0 ? kf[x].x : u == 1 ? kf[x].y : u == 2 ? kf[x].z : kf[x].w;
+                        const uint32_t b0 = e4m3x2_to_f16x2(word), b1 = e4m3x2_hi_to_f16x2(word);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int term = TERMS - 1; term >= 0; --term) mma_f16(z[mt][x], a[mt * TERMS + term], b0, b1);
+                    }
+                }
+            }
+            // ---- weights ----
+            float vscale[NT][2];
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const int key = kw + 8 * x + t + 4 * y, at = (key >> p.sc_shift) * p.hc + hh;
+                    const float ks = lds_f32(sc + 4 * at);
+                    vscale[x][y] = lds_f32(sc + 4 * (at + C::KROWS));
+                    const float e = Scale(vscale[x][y]).e;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        z[mt][x][y] = fmaf(z[mt][x][y], ks * fr[mt][0], e);
+                        z[mt][x][2 + y] = fmaf(z[mt][x][2 + y], ks * fr[mt][1], e);
+                    }
+                    if (edge) {
+                        const int key_l = first + 8 * x + t + 4 * y;
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            if (key_l < 0 || key_l >= lim[mt][0]) z[mt][x][y] = neg_inf();
+                            if (key_l < 0 || key_l >= lim[mt][1]) z[mt][x][2 + y] = neg_inf();
+                        }
+                    }
+                }
+            bool moves = false;
+            float top[MT][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    float m = neg_inf();
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) m = fmaxf(m, fmaxf(z[mt][x][2 * y], z[mt][x][2 * y + 1]));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    top[mt][y] = m;
+                    moves |= m > r[mt][y] + 6.f;
+                }
+            if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+                        if (top[mt][y] > r[mt][y] + 6.f) {
+                            const float alpha = fast_exp2(r[mt][y] - top[mt][y]);
+                            r[mt][y] = top[mt][y];
+                            l[mt][y] *= alpha;
+#pragma unroll
+                            for (int j = 0; j < NJ; ++j) o[mt][j][2 * y] *= alpha, o[mt][j][2 * y + 1] *= alpha;
+                        }
+            }
+            uint32_t pa[MT][TERMS][NT / 2][4];
+            uint32_t unseen = 0;  // columns (x, y) that nobody sees
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float ref0 = r[mt][0] == neg_inf() ? 0.f : r[mt][0] - 7.f, ref1 = r[mt][1] == neg_inf() ? 0.f : r[mt][1] - 7.f;
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    float w0[2], w1[2];
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const Scale s(vscale[x][y]);
+                        const float a = fast_exp2(z[mt][x][y] - ref0), b = fast_exp2(z[mt][x][2 + y] - ref1);
+                        if (edge) {  // what a masked key's scales are does not matter
+                            const int key_l = first + 8 * x + t + 4 * y;
+                            const bool s0_ = key_l >= 0 && key_l < lim[mt][0], s1_ = key_l >= 0 && key_l < lim[mt][1];
+                            w0[y] = s0_ ? a * s.m : 0.f;
+                            w1[y] = s1_ ? b * s.m : 0.f;
+                            if (s0_) l[mt][0] = fmaf(a, s.inv, l[mt][0]);
+                            if (s1_) l[mt][1] = fmaf(b, s.inv, l[mt][1]);
+                            if (key_l < 0 || key_l >= d.sp) unseen |= 1u << (2 * x + y);
+                        } else {
+                            w0[y] = a * s.m;
+                            w1[y] = b * s.m;
+                            l[mt][0] = fmaf(a, s.inv, l[mt][0]);
+                            l[mt][1] = fmaf(b, s.inv, l[mt][1]);
+                        }
+                    }
+#pragma unroll
+                    for (int term = 0; term < TERMS; ++term) {
+                        const uint32_t a = pack_f16(w0[0], w0[1]), b = pack_f16(w1[0], w1[1]);
+                        pa[mt][term][x >> 1][(x & 1) * 2] = a;
+                        pa[mt][term][x >> 1][(x & 1) * 2 + 1] = b;
+                        if (TERMS > 1) {
+                            const __half2 ah = *reinterpret_cast<const __half2*>(&a), bh = *reinterpret_cast<const __half2*>(&b);
+                            w0[0] -= __low2float(ah), w0[1] -= __high2float(ah), w1[0] -= __low2float(bh), w1[1] -= __high2float(bh);
+                        }
+                    }
+                }
+            }
+            // ---- P V: a word of 4 elements of each of a thread's rows at a time ----
+            constexpr int VW = E < 128 ? 2 : 4;  // words a thread loads of a row of a panel
+#pragma unroll
+            for (int pn = 0; pn < NP; ++pn) {
+                uint32_t vw[NT][2][VW];
+#pragma unroll
+                for (int x = 0; x < NT; ++x)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const uint32_t at = vb + tile[x] + pn * panel + vofs[y];
+                        if constexpr (E < 128) {
+                            const uint2 v = lds64(at);
+                            vw[x][y][0] = v.x, vw[x][y][1] = v.y;
+                        } else {
+                            const uint4 v = lds128(at);
+                            vw[x][y][0] = v.x, vw[x][y][1] = v.y, vw[x][y][2] = v.z, vw[x][y][3] = v.w;
+                        }
+                    }
+                if (edge) {
+                    // keys that nobody sees: zeros.  A NaN in the value of a key that some rows see and others do not
+                    // (0 * NaN is NaN) becomes a zero here and is added to the rows that see it.
+                    bool odd = false;
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+#pragma unroll
+                            for (int u = 0; u < VW; ++u) {
+                                if (unseen >> (2 * x + y) & 1u) vw[x][y][u] = 0u;
+                                odd |= e4m3_nan(vw[x][y][u]) != 0;
+                            }
+                    if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+                        for (int mt = 0; mt < MT; ++mt) {
+                            uint32_t ind[NT / 2][4];  // 1 where the row sees the key
+#pragma unroll
+                            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                                for (int y = 0; y < 2; ++y) {
+                                    const int key_l = first + 8 * x + t;
+                                    const int lm = mt == 0 ? lim[0][y] : lim[MT - 1][y];
+                                    ind[x >> 1][(x & 1) * 2 + y] = (key_l >= 0 && key_l < lm ? 0x3c00u : 0u) | (key_l + 4 >= 0 && key_l + 4 < lm ? 0x3c000000u : 0u);
+                                }
+#pragma unroll
+                            for (int j = 0; j < 4 * VW; ++j) {
+                                float cnt[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                for (int g = 0; g < NT / 2; ++g) {
+                                    uint32_t b[2];
+#pragma unroll
+                                    for (int y = 0; y < 2; ++y) {
+                                        const uint32_t fa = e4m3_nan(vw[2 * g + y][0][j >> 2]) >> (8 * (j & 3)), fb = e4m3_nan(vw[2 * g + y][1][j >> 2]) >> (8 * (j & 3));
+                                        b[y] = (fa & 0x80u ? 0x3c00u : 0u) | (fb & 0x80u ? 0x3c000000u : 0u);
+                                    }
+                                    mma_f16(cnt, ind[g], b[0], b[1]);
+                                }
+#pragma unroll
+                                for (int y = 0; y < 4; ++y)
+                                    if (cnt[y] > 0.f) {
+                                        const float nan = __int_as_float(0x7fc00000);
+                                        if (mt == 0) o[0][pn * 4 * VW + j][y] = nan;
+                                        else o[MT - 1][pn * 4 * VW + j][y] = nan;
+                                    }
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < NT; ++x)
+#pragma unroll
+                            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                                for (int u = 0; u < VW; ++u) vw[x][y][u] = clear_bytes(vw[x][y][u], e4m3_nan(vw[x][y][u]));
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < VW; ++u) {
+                    float part[TERMS > 1 ? 4 : 1][4];  // f32: a window's sum by itself, added with one rounding
+                    if constexpr (TERMS > 1)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.f;
+#pragma unroll
+                    for (int g = 0; g < NT / 2; ++g) {
+                        // bytes of two rows side by side: (0, 1) and (2, 3) of each
+                        const uint32_t a0 = __byte_perm(vw[2 * g][0][u], vw[2 * g][1][u], 0x5140), a1 = __byte_perm(vw[2 * g][0][u], vw[2 * g][1][u], 0x7362);
+                        const uint32_t c0 = __byte_perm(vw[2 * g + 1][0][u], vw[2 * g + 1][1][u], 0x5140),
+                                       c1 = __byte_perm(vw[2 * g + 1][0][u], vw[2 * g + 1][1][u], 0x7362);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t b0 = j == 0 ? e4m3x2_to_f16x2(a0) : j == 1 ? e4m3x2_hi_to_f16x2(a0) : j == 2 ? e4m3x2_to_f16x2(a1) : e4m3x2_hi_to_f16x2(a1);
+                            const uint32_t b1 = j == 0 ? e4m3x2_to_f16x2(c0) : j == 1 ? e4m3x2_hi_to_f16x2(c0) : j == 2 ? e4m3x2_to_f16x2(c1) : e4m3x2_hi_to_f16x2(c1);
+                            if constexpr (TERMS > 1) {
+#pragma unroll
+                                for (int term = TERMS - 1; term >= 0; --term) mma_f16(part[j], pa[0][term][g], b0, b1);
+                            } else {
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][pn * 4 * VW + 4 * u + j], pa[mt][0][g], b0, b1);
+                            }
+                        }
+                    }
+                    if constexpr (TERMS > 1)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) o[0][pn * 4 * VW + 4 * u + j][y] += part[j][y];
+                }
+            }
+        }
+
+        if (!(d.how & Q8_LAST)) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_empty + st * 8);
+            continue;
+        }
+        // ---- the piece's result ----
+        const bool whole = (d.how & Q8_WHOLE) != 0;
+        const size_t slot = ((size_t)c * 2 + (d.how & Q8_BEGIN ? 1 : 0)) * p.hc;
+        auto out_row = [&](int head, int row) {  // of `out`; row < p.rows
+            const int s = row / p.G;
+            return ((size_t)d.w * p.Hq + (d.hg * p.hc + head) * p.G + row - s * p.G) * p.S + s;
+        };
+        float f[MT][2], lse2[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                float sum = l[mt][y];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                f[mt][y] = sum;
+                if (wph > 1 && t == 0) {
+                    const int row = mt * 16 + y * 8 + n;
+                    sML[(wid * ROWS + row) * 2] = r[mt][y];
+                    sML[(wid * ROWS + row) * 2 + 1] = sum;
+                }
+            }
+        if (wph > 1) named_bar_sync(2, kQ8Warps * 32);  // and every warp is done with the stage
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                float m = r[mt][y], sum = f[mt][y];
+                if (wph > 1) {
+                    const int row = mt * 16 + y * 8 + n;
+                    m = neg_inf();
+                    for (int g = 0; g < wph; ++g) m = fmaxf(m, sML[((g * p.hc + hh) * ROWS + row) * 2]);
+                    sum = 0.f;
+                    for (int g = 0; g < wph; ++g) {
+                        const float2 x = *reinterpret_cast<const float2*>(sML + ((g * p.hc + hh) * ROWS + row) * 2);
+                        // a warp that saw nothing adds nothing; one whose reference is infinite has a NaN sum
+                        sum += x.x == neg_inf() ? x.y : x.y * fast_exp2(x.x - m);
+                    }
+                }
+                // a sum that is 0: nothing seen (or only NaN scores' zero weights, which make it NaN)
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                f[mt][y] = r[mt][y] == neg_inf() && sum == sum ? 0.f : (wph > 1 && r[mt][y] != neg_inf() ? fast_exp2(r[mt][y] - m) * inv : inv);
+                // the sums are in units of 2^(r - 7)
+                lse2[mt][y] = sum == 0.f ? neg_inf() : (m == neg_inf() ? 0.f : m - 7.f) + log2f(sum);
+            }
+        if (wph == 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_empty + st * 8);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const int i16 = mt * 16 + y * 8 + n, row = d.t * ROWS + i16;
+                    if (row >= p.rows) continue;
+                    const size_t orow = whole ? out_row(hh, row) : (slot + hh) * ROWS + i16;
+#pragma unroll
+                    for (int pn = 0; pn < NP; ++pn)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {  // 16 (8) neighbouring elements
+                            const int e = E < 128 ? ((t & 1) << 5) + ((t & 2) << 3) + 8 * b : pn * 128 + 16 * t + 64 * b;
+                            constexpr int W16 = E < 128 ? 8 : 16;
+#pragma unroll
+                            for (int j = 0; j < W16; j += 4) {
+                                float x[4];
+#pragma unroll
+                                for (int v = 0; v < 4; ++v) x[v] = o[mt][pn * W16 + j + v][2 * y + b] * f[mt][y];
+                                if (whole) {
+                                    store_quad<T>(static_cast<T*>(p.out) + orow * E + e + j, x[0], x[1], x[2], x[3]);
+                                    if (p.out_f32) *reinterpret_cast<float4*>(p.out_f32 + orow * E + e + j) = make_float4(x[0], x[1], x[2], x[3]);
+                                } else {
+                                    *reinterpret_cast<float4*>(p.part_o + orow * E + e + j) = make_float4(x[0], x[1], x[2], x[3]);
+                                }
+                            }
+                        }
+                    if (t == 0) {
+                        if (!whole) p.part_lse[orow] = lse2[mt][y];
+                        else if (p.lse_out) p.lse_out[orow] = lse2[mt][y] * kLn2;
+                    }
+                }
+            continue;
+        }
+        // several warps per head: their outputs are added up, in order, where the stage's K and V lay
+        float* sO = reinterpret_cast<float*>(smem + (size_t)st * 2 * C::TENSOR);  // [hc][ROWS][E]
+#pragma unroll 1
+        for (int g = 0; g < wph; ++g) {
+            if (grp == g) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        float* dst = sO + ((size_t)hh * ROWS + mt * 16 + y * 8 + n) * E;
+#pragma unroll
+                        for (int pn = 0; pn < NP; ++pn)
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+                                const int e = E < 128 ? ((t & 1) << 5) + ((t & 2) << 3) + 8 * b : pn * 128 + 16 * t + 64 * b;
+                                constexpr int W16 = E < 128 ? 8 : 16;
+#pragma unroll
+                                for (int j = 0; j < W16; j += 4) {
+                                    float4* at = reinterpret_cast<float4*>(dst + e + j);
+                                    float4 x = g ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                                    x.x += o[mt][pn * W16 + j][2 * y + b] * f[mt][y];
+                                    x.y += o[mt][pn * W16 + j + 1][2 * y + b] * f[mt][y];
+                                    x.z += o[mt][pn * W16 + j + 2][2 * y + b] * f[mt][y];
+                                    x.w += o[mt][pn * W16 + j + 3][2 * y + b] * f[mt][y];
+                                    *at = x;
+                                }
+                            }
+                        if (g == 0 && t == 0) sML[(wid * ROWS + mt * 16 + y * 8 + n) * 2] = lse2[mt][y];  // wid = hh
+                    }
+            }
+            named_bar_sync(2, kQ8Warps * 32);
+        }
+        for (int x = tid * 4; x < p.hc * ROWS * E; x += kQ8Warps * 32 * 4) {
+            const int i16 = x / E % ROWS, head = x / E / ROWS, e = x % E, row = d.t * ROWS + i16;
+            if (row >= p.rows) continue;
+            const float4 v = *reinterpret_cast<const float4*>(sO + x);
+            const float ls = sML[(head * ROWS + i16) * 2];
+            if (whole) {
+                const size_t orow = out_row(head, row);
+                store_quad<T>(static_cast<T*>(p.out) + orow * E + e, v.x, v.y, v.z, v.w);
+                if (p.out_f32) *reinterpret_cast<float4*>(p.out_f32 + orow * E + e) = v;
+                if (p.lse_out && e == 0) p.lse_out[orow] = ls * kLn2;
+            } else {
+                const size_t at = (slot + head) * ROWS + i16;
+                *reinterpret_cast<float4*>(p.part_o + at * E + e) = v;
+                if (e == 0) p.part_lse[at] = ls;
+            }
+        }
+        fence_proxy_async_smem();  // the next window is written here by TMA
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_empty + st * 8);
+    }
+}
+
+// ---- merge ----------------------------------------------------------------------------------
+// Rows of items that more than one CTA worked on: the log-sum-exp combination of their partials, in CTA
+// order; zeros for pairs without a seen key; NaN in every output where the call's error word is set.
+constexpr int kQ8Ahead = 4;
+
+template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_kernel(const __grid_constant__ Q8Params p, int rows, int ctas) {
+    constexpr int TPR = E / 4, RPB = 256 / TPR;  // threads per row, rows per block
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int tid = threadIdx.x, h = blockIdx.x % p.Hkv, pair = blockIdx.x / p.Hkv;
+    const int w = p.w0 + pair / p.nt, t = pair % p.nt, hg = h / p.hc, hh = h - hg * p.hc;
+    const float nan = __int_as_float(0x7fc00000);
+    const long long P0 = __ldcg(p.P + pair), nw = __ldcg(p.P + pair + 1) - P0, total = __ldcg(p.P + p.pairs);
+    const bool failed = __ldcg(p.header + 3) != 0;
+    int c0 = 0, c1 = -1;  // CTAs of the item
+    if (nw > 0 && !failed) {
+        const Q8Split split(total * p.hs, p, ctas);
+        const long long us = P0 * p.hs + hg * nw;
+        c0 = split.cta_of(us), c1 = split.cta_of(us + nw - 1);
+        if (c0 == c1) return;
+    }
+    const int e = tid % TPR * 4;
+    for (int i = blockIdx.y * RPB + tid / TPR; i < rows && t * rows + i < p.rows; i += gridDim.y * RPB) {
+        const int row = t * rows + i, s = row / p.G;
+        const size_t orow = ((size_t)w * p.Hq + h * p.G + row - s * p.G) * p.S + s;
+        float m = neg_inf(), den = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c = c0; c <= c1; c += kQ8Ahead) {
+            float x[kQ8Ahead];
+            float4 v[kQ8Ahead];
+#pragma unroll
+            for (int k = 0; k < kQ8Ahead; ++k) {
+                const size_t at = (((size_t)(c + k) * 2 + (c + k == c0 ? 1 : 0)) * p.hc + hh) * rows + i;
+                x[k] = neg_inf();
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (c + k <= c1) {
+                    x[k] = __ldcg(p.part_lse + at);
+                    v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * E + e));
+                }
+            }
+            float mx = m;
+            bool bad = false;  // fmaxf drops a NaN, the result must not
+#pragma unroll
+            for (int k = 0; k < kQ8Ahead; ++k) {
+                mx = fmaxf(mx, x[k]);
+                bad |= x[k] != x[k];
+            }
+            const float mu = mx == neg_inf() ? 0.f : mx, alpha = fast_exp2(m - mu);
+            m = mx;
+            den = bad ? nan : den * alpha;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[k] *= alpha;
+#pragma unroll
+            for (int k = 0; k < kQ8Ahead; ++k) {
+                if (x[k] == neg_inf()) continue;  // an empty part adds nothing
+                const float f = fast_exp2(x[k] - mu);
+                den += f;
+                a[0] = fmaf(f, v[k].x, a[0]);
+                a[1] = fmaf(f, v[k].y, a[1]);
+                a[2] = fmaf(f, v[k].z, a[2]);
+                a[3] = fmaf(f, v[k].w, a[3]);
+            }
+        }
+        const float inv = failed ? nan : den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a[k] *= inv;
+        store_quad<T>(static_cast<T*>(p.out) + orow * E + e, a[0], a[1], a[2], a[3]);
+        if (p.out_f32) *reinterpret_cast<float4*>(p.out_f32 + orow * E + e) = make_float4(a[0], a[1], a[2], a[3]);
+        if (p.lse_out && e == 0) p.lse_out[orow] = failed ? nan : den == 0.f ? neg_inf() : (m + log2f(den)) * kLn2;
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------
+namespace {
+
+struct Q8Kernel {
+    const void* fn;
+    const void* merge;
+    int krows, rows, ctas;  // CTAs per SM
+    size_t smem;
+};
+template <class T, int E, int MT> Q8Kernel q8_kernel() {
+    using C = Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1>;
+    return {(const void*)&decode_q8_kernel<T, E, MT>, (const void*)&merge_q8_kernel<T, E>, C::KROWS, C::ROWS, C::CTAS, C::SMEM};
+}
+// One 16-row tile, or two where a KV head has more query rows (then the cache is read half as often); two
+// tiles do not fit in the registers with 32-bit queries or head dim 256.
+template <class T> Q8Kernel q8_pick_t(int E, int rows) {
+    if constexpr (sizeof(T) == 2)
+        if (rows > 16 && E <= 128) return E == 64 ? q8_kernel<T, 64, 2>() : q8_kernel<T, 128, 2>();
+    return E == 64 ? q8_kernel<T, 64, 1>() : E == 128 ? q8_kernel<T, 128, 1>() : q8_kernel<T, 256, 1>();
+}
+Q8Kernel q8_pick(int dtype, int E, int rows) {
+    return dtype == DVATTN_FLOAT32   ? q8_pick_t<float>(E, rows)
+           : dtype == DVATTN_FLOAT16 ? q8_pick_t<__half>(E, rows) : q8_pick_t<__nv_bfloat16>(E, rows);
+}
+
+struct Q8Layout {
+    size_t P, po, pl, total;
+    int ctas, hc, nt, slice;  // slice: sequences of a launch
+};
+int q8_layout(const dvattn_paged_args* a, const Q8Kernel& k, Q8Layout& L) {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return DVATTN_ERR_CUDA;
+    L.ctas = sms * k.ctas;
+    L.hc = a->Hkv % 4 == 0 ? 4 : a->Hkv % 2 == 0 ? 2 : 1;
+    L.nt = (a->S * (a->Hq / a->Hkv) + k.rows - 1) / k.rows;
+    L.slice = kQ8MaxPairs / L.nt;
+    if (L.slice > a->W) L.slice = a->W;
+    size_t at = 256;
+    auto take = [&](size_t bytes) {
+        const size_t r = at;
+        at += (bytes + 255) / 256 * 256;
+        return r;
+    };
+    L.P = take(8 * ((size_t)L.slice * L.nt + 1));
+    L.po = take(4 * (size_t)L.ctas * 2 * L.hc * k.rows * a->E);
+    L.pl = take(4 * (size_t)L.ctas * 2 * L.hc * k.rows);
+    L.total = at;
+    return DVATTN_OK;
+}
+
+int q8_validate(const dvattn_paged_args* a) {
+    const int st = decode_validate(a);
+    if (st != DVATTN_OK) return st;
+    const long long rows = (long long)a->S * (a->Hq / a->Hkv);
+    if (a->num_blocks < 0) return DVATTN_ERR_INVALID_ARGUMENT;
+    // a sequence's row tiles are one launch's
+    if (rows > 16LL * kQ8MaxPairs || (long long)a->F * a->W * a->S > 0x7fffffffLL || (long long)kQ8MaxPairs * a->Hkv > 0x7fffffffLL)
+        return DVATTN_ERR_UNSUPPORTED;
+    return DVATTN_OK;
+}
+
+// [tokens][Hkv][E] bytes as a 4-D map {128 (64) bytes, tokens, panels, heads} whose box is `box` tokens of hc heads,
+// landing as [head][panel][token][128 (64) bytes], swizzled.
+bool q8_map(CUtensorMap* m, const void* base, int E, int Hkv, int hc, long long tokens, int box) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return false;
+    const cuuint32_t rb = E < 128 ? 64 : 128;
+    cuuint64_t dims[4] = {rb, (cuuint64_t)tokens, (cuuint64_t)(E / rb), (cuuint64_t)Hkv};
+    cuuint64_t strides[3] = {(cuuint64_t)Hkv * E, rb, (cuuint64_t)E};
+    cuuint32_t b[4] = {rb, (cuuint32_t)box, (cuuint32_t)(E / rb), (cuuint32_t)hc};
+    cuuint32_t es[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              rb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// DVATTN_TEST_STALL_TILE=<i>: tests only (see the decode launcher); read once per process.
+int q8_stall_hook() {
+    static const int t = [] {
+        const char* e = getenv("DVATTN_TEST_STALL_TILE");
+        return e && *e ? atoi(e) : -1;
+    }();
+    return t;
+}
+
+}  // namespace
+
+size_t decode_q8_workspace_size(const dvattn_paged_args* a) {
+    if (q8_validate(a) != DVATTN_OK || (long long)a->W * a->S == 0 || a->Hq == 0) return 0;
+    Q8Layout L;
+    return q8_layout(a, q8_pick(a->dtype, a->E, a->S * (a->Hq / a->Hkv)), L) == DVATTN_OK ? L.total : 0;
+}
+
+int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream) {
+    int st = q8_validate(a);
+    if (st != DVATTN_OK) return st;
+    if (!sc) return DVATTN_ERR_INVALID_ARGUMENT;
+    if ((long long)a->W * a->S == 0 || a->Hq == 0) return DVATTN_OK;
+    const bool cached = a->max_blocks_per_seq > 0 && a->num_blocks > 0;
+    if (!a->out || !a->queries || (a->F > 0 && (!a->locations || !a->fragment_lengths)) || (a->F > 0 && a->R > 0 && (!a->cosines || !a->sines)) ||
+        (cached && (!a->k_cache || !a->v_cache || !a->block_tables || !sc->k_scales || !sc->v_scales)))
+        return DVATTN_ERR_INVALID_ARGUMENT;
+    for (const void* x : {a->queries, a->k_cache, a->v_cache, (const void*)a->out, (const void*)a->out_f32})
+        if (reinterpret_cast<uintptr_t>(x) & 15) return DVATTN_ERR_INVALID_ARGUMENT;
+    const Q8Kernel k = q8_pick(a->dtype, a->E, a->S * (a->Hq / a->Hkv));
+    Q8Layout L;
+    if ((st = q8_layout(a, k, L)) != DVATTN_OK) return st;
+    if (!workspace || wbytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return DVATTN_ERR_WORKSPACE;
+    if (cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem) != cudaSuccess ||
+        cudaFuncSetAttribute(k.fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+        return DVATTN_ERR_CUDA;
+    char* ws = static_cast<char*>(workspace);
+    Q8Params p{};
+    p.F = a->F; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.S = a->S; p.R = a->R;
+    p.rows = p.S * p.G;
+    p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
+    const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
+    p.cap = a->num_blocks <= 0 ? 0 : cap > kMostPositions ? kMostPositions : (int)cap;
+    p.hc = L.hc; p.hs = a->Hkv / L.hc; p.nt = L.nt; p.groups = L.ctas;
+    p.kt = k.krows / L.hc;
+    p.least = 1;
+    p.tokens = (long long)a->W * a->S;
+    p.scale_log2 = a->scale * kLog2e;
+    p.out = a->out; p.lse_out = a->lse_out; p.out_f32 = a->out_f32;
+    p.q = a->queries; p.cos = a->cosines; p.sin = a->sines; p.loc = a->locations; p.L = a->fragment_lengths;
+    p.k = static_cast<const uint8_t*>(a->k_cache); p.v = static_cast<const uint8_t*>(a->v_cache);
+    p.ks = sc->k_scales; p.vs = sc->v_scales; p.bt = a->block_tables;
+    p.stall_tile = q8_stall_hook();
+    p.header = reinterpret_cast<int*>(ws);
+    p.P = reinterpret_cast<long long*>(ws + L.P);
+    p.part_o = reinterpret_cast<float*>(ws + L.po);
+    p.part_lse = reinterpret_cast<float*>(ws + L.pl);
+    // pages that are whole numbers of boxes of 8 rows or more come by TMA, others row by row
+    int box = p.kt;
+    while (p.BS % box) box >>= 1;
+    alignas(64) CUtensorMap mk{}, mv{};
+    p.gather = box < 8 || !cached || a->num_blocks * a->block_size > 0x7fffffffLL - 2 * box;
+    if (p.gather) box = p.kt;
+    else if (!q8_map(&mk, a->k_cache, a->E, a->Hkv, L.hc, a->num_blocks * a->block_size, box) ||
+             !q8_map(&mv, a->v_cache, a->E, a->Hkv, L.hc, a->num_blocks * a->block_size, box))
+        return DVATTN_ERR_CUDA;
+    p.box = box;
+    while (1 << p.box_shift < box) ++p.box_shift;
+    p.align = p.gather ? 1 : box;
+    p.sc_shift = p.gather ? 0 : 3;
+
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.stream = stream;
+    cudaError_t e = cudaSuccess;
+    for (int w = 0; w < a->W && e == cudaSuccess; w += L.slice) {
+        p.w0 = w;
+        p.W = a->W - w < L.slice ? a->W - w : L.slice;
+        p.pairs = p.W * p.nt;
+        int rows = k.rows, ctas = L.ctas;
+        void* args[] = {&p, &mk, &mv};
+        cfg.gridDim = dim3((unsigned)L.ctas);
+        cfg.blockDim = dim3((kQ8Warps + 1) * 32);
+        cfg.dynamicSmemBytes = k.smem;
+        e = cudaLaunchKernelExC(&cfg, k.fn, args);
+        if (e != cudaSuccess) break;
+        void* margs[] = {&p, &rows, &ctas};
+        const int rpb = 256 / (a->E / 4);
+        cfg.gridDim = dim3((unsigned)(p.pairs * a->Hkv), (unsigned)((rows + rpb - 1) / rpb));
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        e = cudaLaunchKernelExC(&cfg, k.merge, margs);
+    }
+    if (e != cudaSuccess) {
+        if (getenv("DVATTN_DEBUG")) fprintf(stderr, "dvattn q8 launch: %s\n", cudaGetErrorString(e));
+        return DVATTN_ERR_CUDA;
+    }
+    return cudaGetLastError() == cudaSuccess ? DVATTN_OK : DVATTN_ERR_CUDA;
+}
+
+}  // namespace dvb

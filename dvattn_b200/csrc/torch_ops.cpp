@@ -93,19 +93,52 @@ dvattn_rotary_args rotary_args(const RotaryOpt& r, const at::Tensor& out, int ro
     return ra;
 }
 
+// The scales of a cache held in 8 bits (the *_q8 ops).
+struct ScalesOpt {
+    const at::Tensor* k;
+    const at::Tensor* v;
+};
+
+void check_q8(const ScalesOpt& s, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& out, const char* name) {
+    TORCH_CHECK(k_cache.scalar_type() == at::kFloat8_e4m3fn && v_cache.scalar_type() == at::kFloat8_e4m3fn, name,
+                ": k_cache/v_cache must be float8_e4m3fn");
+    check_all(out, {Named{s.k, "k_scales"}, Named{s.v, "v_scales"}});
+    for (const at::Tensor* t : {s.k, s.v})
+        TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == k_cache.size(0) && t->size(1) == k_cache.size(2), name,
+                    ": k_scales/v_scales must be f32 [NB, Hkv]");
+}
+
+template <class Args>
+void run_q8(const at::Tensor& out, const Args& a, const ScalesOpt& s, size_t (*size)(const Args*),
+            int (*call)(const Args*, const dvattn_q8_scales*, void*, size_t, dvattn_stream_t), const char* name) {
+    const dvattn_q8_scales sc{s.k->data_ptr<float>(), s.v->data_ptr<float>()};
+    int st = call(&a, &sc, nullptr, 0, cur_stream(out));  // validation only when nothing to do
+    if (st == DVATTN_ERR_WORKSPACE) {
+        const size_t wsb = size(&a);
+        TORCH_CHECK(wsb > 0, name, ": could not size the workspace");
+        at::Tensor ws = at::empty({(int64_t)wsb}, out.options().dtype(at::kByte));
+        st = call(&a, &sc, ws.data_ptr(), wsb, cur_stream(out));
+        check_status(st, name);
+        check_call_status(ws, cur_stream(out), name);
+    }
+    check_status(st, name);
+}
+
 void paged_impl(at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
                 const at::Tensor& cosines, const at::Tensor& sines, const at::Tensor& fragment_lengths,
                 const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_tables,
                 const c10::optional<at::Tensor>& lse, const c10::optional<at::Tensor>& out_f32,
-                const RotaryOpt* rot = nullptr) {
+                const RotaryOpt* rot = nullptr, const ScalesOpt* q8 = nullptr) {
     const c10::cuda::CUDAGuard guard(out.device());
     const int dt = dtype_code(out);
     TORCH_CHECK(out.dim() == 4, "dvattn_paged_sdpa: output must be [W, Hq, S, Ev]");
     TORCH_CHECK(queries.dim() == 4 && locations.dim() == 3 && (rot || (cosines.dim() == 4 && sines.dim() == 4)) &&
                     k_cache.dim() == 4 && v_cache.dim() == 4 && block_tables.dim() == 2 && fragment_lengths.dim() == 1,
                 "dvattn_paged_sdpa: wrong tensor ranks");
+    if (q8) check_q8(*q8, k_cache, v_cache, out, "dvattn_paged_sdpa_q8");
     for (auto* pr : {&queries, &k_cache, &v_cache})
-        TORCH_CHECK(pr->scalar_type() == out.scalar_type(), "dvattn_paged_sdpa: queries/k_cache/v_cache must have the output dtype");
+        TORCH_CHECK(pr->scalar_type() == out.scalar_type() || (q8 && pr != &queries),
+                    "dvattn_paged_sdpa: queries/k_cache/v_cache must have the output dtype");
     TORCH_CHECK(rot || (cosines.scalar_type() == at::kFloat && sines.scalar_type() == at::kFloat),
                 "dvattn_paged_sdpa: cosines/sines must be float32");
     check_i32(locations, "locations");
@@ -177,6 +210,10 @@ void paged_impl(at::Tensor& out, double scale, const at::Tensor& locations, cons
         check_call_status(ws, cur_stream(out), "dvattn_paged_sdpa_rope");
         return;
     }
+    if (q8) {
+        run_q8(out, a, *q8, dvattn_paged_sdpa_q8_workspace_size, dvattn_paged_sdpa_q8, "dvattn_paged_sdpa_q8");
+        return;
+    }
     int st = dvattn_paged_sdpa(&a, nullptr, 0, cur_stream(out));  // validation only when nothing to do
     if (st == DVATTN_ERR_WORKSPACE) {
         const size_t wsb = dvattn_paged_sdpa_workspace_size(&a);
@@ -212,14 +249,20 @@ void varlen_impl(at::Tensor& out, double scale, const at::Tensor& locations, con
                  const at::Tensor& cosines, const at::Tensor& sines, const at::Tensor& fragment_lengths,
                  const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_tables,
                  const at::Tensor& cu_seqlens_q, const at::Tensor& cu_seqlens_k, const c10::optional<at::Tensor>& lse,
-                 const c10::optional<at::Tensor>& out_f32, const RotaryOpt* rot = nullptr) {
+                 const c10::optional<at::Tensor>& out_f32, const RotaryOpt* rot = nullptr, const ScalesOpt* q8 = nullptr) {
     const c10::cuda::CUDAGuard guard(out.device());
     const int dt = dtype_code(out);
     TORCH_CHECK(queries.dim() == 3 && out.dim() == 3 && locations.dim() == 2 && (rot || (cosines.dim() == 3 && sines.dim() == 3)) &&
                     k_cache.dim() == 4 && v_cache.dim() == 4 && block_tables.dim() == 2 && cu_seqlens_q.dim() == 1,
                 "dvattn_varlen_paged_sdpa: wrong tensor ranks");
+    if (q8) {
+        check_q8(*q8, k_cache, v_cache, out, "dvattn_varlen_paged_sdpa_q8");
+        TORCH_CHECK(fragment_lengths.dim() == 1 && block_tables.size(0) == cu_seqlens_q.size(0) - 1,
+                    "dvattn_varlen_paged_sdpa_q8: block_tables must be [W, max_blocks], cu_seqlens_q [W + 1]");
+    }
     for (auto* pr : {&queries, &k_cache, &v_cache})
-        TORCH_CHECK(pr->scalar_type() == out.scalar_type(), "dvattn_varlen_paged_sdpa: queries/k_cache/v_cache must have the output dtype");
+        TORCH_CHECK(pr->scalar_type() == out.scalar_type() || (q8 && pr != &queries),
+                    "dvattn_varlen_paged_sdpa: queries/k_cache/v_cache must have the output dtype");
     TORCH_CHECK(rot || (cosines.scalar_type() == at::kFloat && sines.scalar_type() == at::kFloat),
                 "dvattn_varlen_paged_sdpa: cosines/sines must be float32");
     check_i32(locations, "locations");
@@ -286,6 +329,10 @@ void varlen_impl(at::Tensor& out, double scale, const at::Tensor& locations, con
         check_status(dvattn_varlen_paged_sdpa_rope(&a, &ra, ws.data_ptr(), wsb, cur_stream(out)),
                      "dvattn_varlen_paged_sdpa_rope");
         check_call_status(ws, cur_stream(out), "dvattn_varlen_paged_sdpa_rope");
+        return;
+    }
+    if (q8) {
+        run_q8(out, a, *q8, dvattn_varlen_paged_sdpa_q8_workspace_size, dvattn_varlen_paged_sdpa_q8, "dvattn_varlen_paged_sdpa_q8");
         return;
     }
     int st = dvattn_varlen_paged_sdpa(&a, nullptr, 0, cur_stream(out));
@@ -748,6 +795,131 @@ void dvattn_paged_evict_op(at::Tensor& k_cache, at::Tensor& v_cache, const at::T
 }
 
 // ---------------------------------------------------------------------------------
+// The paged cache held in 8 bits and the pages behind it (B200 additions)
+// ---------------------------------------------------------------------------------
+void dvattn_paged_sdpa_q8_op(at::Tensor& out, const c10::optional<at::Tensor>& lse, const c10::optional<at::Tensor>& out_f32,
+                             double scale, const at::Tensor& locations, const at::Tensor& queries, const at::Tensor& cosines,
+                             const at::Tensor& sines, const at::Tensor& fragment_lengths, const at::Tensor& k_cache,
+                             const at::Tensor& v_cache, const at::Tensor& k_scales, const at::Tensor& v_scales,
+                             const at::Tensor& block_tables) {
+    const ScalesOpt q8{&k_scales, &v_scales};
+    paged_impl(out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, block_tables, lse, out_f32,
+               nullptr, &q8);
+}
+
+void dvattn_varlen_paged_sdpa_q8_op(at::Tensor& out, const c10::optional<at::Tensor>& lse, const c10::optional<at::Tensor>& out_f32,
+                                    double scale, const at::Tensor& locations, const at::Tensor& queries, const at::Tensor& cosines,
+                                    const at::Tensor& sines, const at::Tensor& fragment_lengths, const at::Tensor& k_cache,
+                                    const at::Tensor& v_cache, const at::Tensor& k_scales, const at::Tensor& v_scales,
+                                    const at::Tensor& block_tables, const at::Tensor& cu_seqlens_q, const at::Tensor& cu_seqlens_k) {
+    const ScalesOpt q8{&k_scales, &v_scales};
+    varlen_impl(out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, block_tables, cu_seqlens_q,
+                cu_seqlens_k, lse, out_f32, nullptr, &q8);
+}
+
+void dvattn_paged_append_q8_op(at::Tensor& k_cache, at::Tensor& v_cache, at::Tensor& k_scales, at::Tensor& v_scales,
+                               const at::Tensor& keys, const at::Tensor& values, const at::Tensor& cosines, const at::Tensor& sines,
+                               const at::Tensor& block_tables, const at::Tensor& positions, const c10::optional<at::Tensor>& counts) {
+    const c10::cuda::CUDAGuard guard(k_cache.device());
+    const int dt = dtype_code(keys);
+    TORCH_CHECK(k_cache.dim() == 4 && v_cache.dim() == 4 && keys.dim() == 4 && values.dim() == 4 && cosines.dim() == 3 &&
+                    sines.dim() == 3 && block_tables.dim() == 2 && positions.dim() == 1,
+                "dvattn_paged_append_q8: wrong tensor ranks");
+    TORCH_CHECK(values.scalar_type() == keys.scalar_type(), "dvattn_paged_append_q8: keys and values must share the dtype");
+    TORCH_CHECK(cosines.scalar_type() == at::kFloat && sines.scalar_type() == at::kFloat,
+                "dvattn_paged_append_q8: cosines/sines must be float32");
+    check_i32(block_tables, "block_tables");
+    check_i32(positions, "positions");
+    check_all(k_cache, {Named{&k_cache, "k_cache"}, Named{&v_cache, "v_cache"}, Named{&keys, "keys"}, Named{&values, "values"},
+                        Named{&cosines, "cosines"}, Named{&sines, "sines"}, Named{&block_tables, "block_tables"},
+                        Named{&positions, "positions"}});
+    check_q8(ScalesOpt{&k_scales, &v_scales}, k_cache, v_cache, k_cache, "dvattn_paged_append_q8");
+    const int W = keys.size(0), Hkv = keys.size(1), n = keys.size(2), E = keys.size(3), Ev = values.size(3), R = cosines.size(2);
+    TORCH_CHECK(values.size(0) == W && values.size(1) == Hkv && values.size(2) == n,
+                "dvattn_paged_append_q8: values must be [W, Hkv, n, Ev]");
+    TORCH_CHECK(k_cache.size(2) == Hkv && k_cache.size(3) == E, "dvattn_paged_append_q8: k_cache must be [NB, BS, Hkv, E]");
+    TORCH_CHECK(v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1) && v_cache.size(2) == Hkv && v_cache.size(3) == Ev,
+                "dvattn_paged_append_q8: v_cache must be [NB, BS, Hkv, Ev]");
+    TORCH_CHECK(cosines.size(0) == W && cosines.size(1) == n && sines.sizes() == cosines.sizes(),
+                "dvattn_paged_append_q8: cosines/sines must be [W, n, R]");
+    TORCH_CHECK(block_tables.size(0) == W && positions.size(0) == W, "dvattn_paged_append_q8: block_tables [W, max_blocks], positions [W]");
+    dvattn_append_args a{};
+    a.dtype = dt;
+    a.W = W; a.Hkv = Hkv; a.E = E; a.Ev = Ev; a.n = n; a.R = R;
+    a.block_size = k_cache.size(1);
+    a.max_blocks_per_seq = block_tables.size(1);
+    a.num_blocks = k_cache.size(0);
+    a.k_cache = k_cache.data_ptr();
+    a.v_cache = v_cache.data_ptr();
+    a.keys = keys.const_data_ptr();
+    a.values = values.const_data_ptr();
+    a.cosines = cosines.const_data_ptr<float>();
+    a.sines = sines.const_data_ptr<float>();
+    a.block_tables = block_tables.const_data_ptr<int>();
+    a.positions = positions.const_data_ptr<int>();
+    if (counts.has_value()) {
+        check_cuda_tensor(*counts, "counts", k_cache);
+        check_i32(*counts, "counts");
+        TORCH_CHECK(counts->numel() == W, "dvattn_paged_append_q8: counts must be [W]");
+        a.counts = counts->const_data_ptr<int>();
+    }
+    const dvattn_q8_scales sc{k_scales.data_ptr<float>(), v_scales.data_ptr<float>()};
+    check_status(dvattn_paged_append_q8(&a, &sc, cur_stream(k_cache)), "dvattn_paged_append_q8");
+}
+
+void check_pages(const at::Tensor& block_tables, const at::Tensor& free_pages, const at::Tensor& free_count,
+                 std::initializer_list<Named> per_seq, const char* name) {
+    TORCH_CHECK(block_tables.dim() == 2 && free_pages.dim() == 1 && free_count.numel() == 1, name,
+                ": block_tables must be [W, max_blocks], free_pages [N], free_count [1]");
+    check_all(block_tables, {Named{&block_tables, "block_tables"}, Named{&free_pages, "free_pages"}, Named{&free_count, "free_count"}});
+    check_all(block_tables, per_seq);
+    check_i32(block_tables, "block_tables");
+    check_i32(free_pages, "free_pages");
+    check_i32(free_count, "free_count");
+    for (const Named& n : per_seq) {
+        check_i32(*n.first, n.second);
+        TORCH_CHECK(n.first->dim() == 1 && n.first->size(0) == block_tables.size(0), name, ": ", n.second, " must be [W]");
+    }
+}
+
+void dvattn_assign_pages_op(at::Tensor& block_tables, const at::Tensor& free_pages, at::Tensor& free_count, at::Tensor& granted,
+                            const c10::optional<at::Tensor>& slots, const at::Tensor& starts, const at::Tensor& counts, int64_t block_size) {
+    const c10::cuda::CUDAGuard guard(block_tables.device());
+    check_pages(block_tables, free_pages, free_count, {Named{&starts, "starts"}, Named{&counts, "counts"}, Named{&granted, "granted"}},
+                "dvattn_assign_pages");
+    TORCH_CHECK(block_size > 0 && block_size <= INT32_MAX && free_pages.size(0) <= INT32_MAX, "dvattn_assign_pages: block_size must be positive");
+    dvattn_assign_args a{};
+    a.W = block_tables.size(0); a.max_blocks_per_seq = block_tables.size(1); a.block_size = block_size; a.free_size = free_pages.size(0);
+    a.block_tables = block_tables.data_ptr<int>();
+    a.free_pages = free_pages.const_data_ptr<int>();
+    a.free_count = free_count.data_ptr<int>();
+    a.starts = starts.const_data_ptr<int>();
+    a.counts = counts.const_data_ptr<int>();
+    a.granted = granted.data_ptr<int>();
+    if (slots.has_value()) {
+        check_cuda_tensor(*slots, "slots", block_tables);
+        TORCH_CHECK(slots->scalar_type() == at::kLong && slots->dim() == 2 && slots->size(0) == a.W && slots->size(1) <= INT32_MAX,
+                    "dvattn_assign_pages: slots must be int64 [W, n]");
+        a.n = slots->size(1);
+        a.slots = reinterpret_cast<long long*>(slots->data_ptr<int64_t>());
+    }
+    check_status(dvattn_assign_pages(&a, cur_stream(block_tables)), "dvattn_assign_pages");
+}
+
+void dvattn_release_pages_op(at::Tensor& block_tables, at::Tensor& free_pages, at::Tensor& free_count, const at::Tensor& keep, int64_t block_size) {
+    const c10::cuda::CUDAGuard guard(block_tables.device());
+    check_pages(block_tables, free_pages, free_count, {Named{&keep, "keep"}}, "dvattn_release_pages");
+    TORCH_CHECK(block_size > 0 && block_size <= INT32_MAX && free_pages.size(0) <= INT32_MAX, "dvattn_release_pages: block_size must be positive");
+    dvattn_release_args a{};
+    a.W = block_tables.size(0); a.max_blocks_per_seq = block_tables.size(1); a.block_size = block_size; a.free_size = free_pages.size(0);
+    a.block_tables = block_tables.data_ptr<int>();
+    a.free_pages = free_pages.data_ptr<int>();
+    a.free_count = free_count.data_ptr<int>();
+    a.keep = keep.const_data_ptr<int>();
+    check_status(dvattn_release_pages(&a, cur_stream(block_tables)), "dvattn_release_pages");
+}
+
+// ---------------------------------------------------------------------------------
 // dvattn_sdpa / dvattn_fused: contiguous per-turn fragments (src/binding.cu:79-149,
 // 356-372).  key_fragments[f] is [Hkv, L_f, E] or [B, Hkv, L_f, E] with B = 1 (one
 // fragment shared by the W workers) or B = W; queries are [F, W, Hq, S, E], rotated.
@@ -884,6 +1056,20 @@ TORCH_LIBRARY(libdvatt, m) {
     m.def("dvattn_paged_evict(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor mass, Tensor(c!) mass_out, "
           "Tensor(d!)? source, Tensor block_tables, Tensor starts, Tensor lengths, Tensor keep, int sink, int recent) -> ()",
           tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("dvattn_paged_sdpa_q8(Tensor(a!) output, Tensor(b!)? lse, Tensor(c!)? out_f32, float scale, Tensor locations, "
+          "Tensor queries, Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor v_cache, "
+          "Tensor k_scales, Tensor v_scales, Tensor block_tables) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("dvattn_varlen_paged_sdpa_q8(Tensor(a!) output, Tensor(b!)? lse, Tensor(c!)? out_f32, float scale, Tensor locations, "
+          "Tensor queries, Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor v_cache, "
+          "Tensor k_scales, Tensor v_scales, Tensor block_tables, Tensor cu_seqlens_q, Tensor cu_seqlens_k) -> ()",
+          tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("dvattn_paged_append_q8(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scales, Tensor(d!) v_scales, Tensor keys, "
+          "Tensor values, Tensor cosines, Tensor sines, Tensor block_tables, Tensor positions, Tensor? counts) -> ()",
+          tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("dvattn_assign_pages(Tensor(a!) block_tables, Tensor free_pages, Tensor(b!) free_count, Tensor(c!) granted, "
+          "Tensor(d!)? slots, Tensor starts, Tensor counts, int block_size) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("dvattn_release_pages(Tensor(a!) block_tables, Tensor(b!) free_pages, Tensor(c!) free_count, Tensor keep, "
+          "int block_size) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
 }
 
 TORCH_LIBRARY_IMPL(libdvatt, CUDA, m) {
@@ -904,4 +1090,9 @@ TORCH_LIBRARY_IMPL(libdvatt, CUDA, m) {
     m.impl("dvattn_tree_append", dvattn_tree_append_op);
     m.impl("dvattn_paged_mass", dvattn_paged_mass_op);
     m.impl("dvattn_paged_evict", dvattn_paged_evict_op);
+    m.impl("dvattn_paged_sdpa_q8", dvattn_paged_sdpa_q8_op);
+    m.impl("dvattn_varlen_paged_sdpa_q8", dvattn_varlen_paged_sdpa_q8_op);
+    m.impl("dvattn_paged_append_q8", dvattn_paged_append_q8_op);
+    m.impl("dvattn_assign_pages", dvattn_assign_pages_op);
+    m.impl("dvattn_release_pages", dvattn_release_pages_op);
 }

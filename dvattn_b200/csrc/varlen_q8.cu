@@ -1,0 +1,216 @@
+// Packed chunked prefill over a paged cache held in 8 bits (q8.cuh): the pages that the call's tokens see are
+// widened to the queries' type in the workspace (value x scale, rounded once: exact in bf16, and in f16 within
+// its range, for the scales that the append sets; f16 values past the range saturate), then
+// the 16-bit (32-bit) varlen attention runs over them.
+//
+// A prefill is bound by its products, 4 E flops for every (query head, key) pair; widening a key costs
+// 2 E (1 + sizeof T) bytes once per KV head, the time of a few tokens' products.  The same widening inside the
+// attention kernel, per window and work item, would be done again for every 16 tokens.
+#include "decode.cuh"
+#include "q8.cuh"
+#include "turns.cuh"
+
+namespace dvb {
+
+namespace {
+
+struct WidenParams {
+    int F, W, T, BS, maxb, cap, own_table;  // own_table: page (w, j) of the widened caches is w * maxb + j
+    long long NB, chunks;                   // 16-byte chunks of a page of one 8-bit cache
+    int row16;                              // chunks of a (token, head) row
+    int Hkv;
+    const int* loc;
+    const int* L;
+    const int* cu;
+    const int* bt;
+    const uint8_t* k;
+    const uint8_t* v;
+    const float* ks;
+    const float* vs;
+    int* span;   // [W][F] keys of the turn that a token of the sequence sees
+    int* table;  // [W][maxb]
+    void* wk;
+    void* wv;
+};
+
+// A thread per (turn, token): the sequence of token t is the first w with t < cu[w + 1], else 0, as in the
+// varlen attention.
+__global__ void __launch_bounds__(256) widen_span_kernel(WidenParams p) {
+    const int f = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x;
+    int lo = 0, hi = p.W;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (t < __ldg(p.cu + mid + 1)) hi = mid; else lo = mid + 1;
+    }
+    const int w = lo < p.W ? lo : 0;
+    long long off = 0;
+    for (int g = 0; g < f; ++g) off += max(__ldg(p.L + g), 0);
+    const int v = t < p.T ? turn_seen(__ldg(p.L + f), __ldg(p.loc + (size_t)f * p.T + t), off, p.cap) : 0;
+    const unsigned peers = __match_any_sync(0xffffffffu, w);  // a warp's lanes have one sequence or a few
+    const int top = __reduce_max_sync(peers, v);
+    if (top > 0 && (threadIdx.x & 31) == __ffs(peers) - 1) atomicMax(p.span + (size_t)w * p.F + f, top);
+}
+
+template <class T> __device__ __forceinline__ T widened(float x) {
+    if constexpr (Elem<T>::dtype == DVATTN_FLOAT16) x = x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x;
+    return Elem<T>::from_f(x);
+}
+
+// Lane k of a warp looks at page warp + k * warps of the table; then the warp widens those that are seen.
+template <class T> __global__ void __launch_bounds__(256) widen_kernel(WidenParams p) {
+    const int lane = threadIdx.x & 31;
+    const long long warps = (long long)gridDim.x * 8, me = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), all = (long long)p.W * p.maxb;
+    for (long long base = 0; base < all; base += 32 * warps) {
+        const long long i = base + me + lane * warps;
+        int page = -1;
+        if (i < all) {
+            const int w = (int)(i / p.maxb), j = (int)(i - (long long)w * p.maxb);
+            const long long a = (long long)j * p.BS;
+            long long off = 0;
+            bool seen = false;
+            for (int f = 0; f < p.F; ++f) {
+                const int n = __ldcg(p.span + (size_t)w * p.F + f);
+                seen |= n > 0 && off < a + p.BS && off + n > a;
+                off += max(__ldg(p.L + f), 0);
+            }
+            if (seen) {
+                const int g = __ldg(p.bt + i);
+                if (g >= 0 && g < p.NB) page = g;
+            }
+            if (p.own_table) p.table[i] = page >= 0 ? (int)i : -1;
+        }
+        for (unsigned todo = __ballot_sync(0xffffffffu, page >= 0); todo; todo &= todo - 1) {
+            const int src = __ffs(todo) - 1;
+            const long long from = __shfl_sync(0xffffffffu, page, src), to = p.own_table ? base + me + src * warps : from;
+#pragma unroll 1
+            for (int tensor = 0; tensor < 2; ++tensor) {
+                const uint4* in = reinterpret_cast<const uint4*>(tensor ? p.v : p.k) + from * p.chunks;
+                uint4* out = static_cast<uint4*>(tensor ? p.wv : p.wk) + to * p.chunks * sizeof(T);
+                const float* sc = (tensor ? p.vs : p.ks) + from * p.Hkv;
+                constexpr int U = 4;
+                for (long long c0 = lane; c0 < p.chunks; c0 += 32 * U) {
+                    uint4 x[U];
+                    float s[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const long long c = c0 + 32 * u;
+                        if (c < p.chunks) {
+                            x[u] = __ldg(in + c);
+                            s[u] = __ldg(sc + (int)(c / p.row16 % p.Hkv));
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const long long c = c0 + 32 * u;
+                        if (c >= p.chunks) break;
+                        alignas(16) T y[16];
+                        const uint32_t word[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) {
+                            const uint32_t f = b & 1 ? e4m3x2_hi_to_f16x2(word[b >> 1]) : e4m3x2_to_f16x2(word[b >> 1]);
+                            const __half2 h = *reinterpret_cast<const __half2*>(&f);
+                            y[2 * b] = widened<T>(__low2float(h) * s[u]);
+                            y[2 * b + 1] = widened<T>(__high2float(h) * s[u]);
+                        }
+#pragma unroll
+                        for (int b = 0; b < (int)sizeof(T); ++b) out[c * sizeof(T) + b] = reinterpret_cast<const uint4*>(y)[b];
+                    }
+                }
+            }
+        }
+    }
+}
+
+size_t up(size_t x) { return (x + 255) / 256 * 256; }
+
+struct WidenLayout {
+    size_t own, span, table, wk, wv, total;
+    long long pages;
+    bool own_table;
+    dvattn_varlen_args wide;  // the call over the widened caches
+};
+bool widen_layout(const dvattn_varlen_args* a, WidenLayout& L) {
+    const long long mine = (long long)a->W * a->max_blocks_per_seq;
+    L.own_table = mine < a->num_blocks;
+    L.pages = L.own_table ? mine : a->num_blocks;
+    L.wide = *a;
+    L.wide.num_blocks = L.pages;
+    L.own = varlen_workspace_size(&L.wide);
+    if (L.own == 0) return false;
+    const size_t cache = (size_t)L.pages * a->block_size * a->Hkv * a->E * (a->dtype == DVATTN_FLOAT32 ? 4 : 2);
+    L.span = up(L.own);
+    L.table = L.span + up(4 * (size_t)a->W * a->F);
+    L.wk = L.table + (L.own_table ? up(4 * (size_t)mine) : 0);
+    L.wv = L.wk + up(cache);
+    L.total = L.wv + up(cache);
+    return true;
+}
+int widen_validate(const dvattn_varlen_args* a) {
+    if (!a || a->W < 0 || a->T < 0 || a->num_blocks < 0) return DVATTN_ERR_INVALID_ARGUMENT;
+    dvattn_paged_args v{};
+    v.dtype = a->dtype; v.F = a->F; v.W = a->T; v.Hq = a->Hq; v.Hkv = a->Hkv; v.E = a->E; v.Ev = a->Ev; v.S = 1; v.R = a->R;
+    v.block_size = a->block_size; v.max_blocks_per_seq = a->max_blocks_per_seq; v.num_blocks = a->num_blocks;
+    const int st = decode_validate(&v);
+    if (st != DVATTN_OK) return st;
+    // tables are indexed in 32 bits where they are the workspace's; turns are a grid's y
+    return (long long)a->W * a->max_blocks_per_seq > 0x7fffffffLL || a->F > 65535 ? DVATTN_ERR_UNSUPPORTED : DVATTN_OK;
+}
+
+}  // namespace
+
+size_t varlen_q8_workspace_size(const dvattn_varlen_args* a) {
+    WidenLayout L;
+    return widen_validate(a) == DVATTN_OK && a->T > 0 && a->Hq > 0 && widen_layout(a, L) ? L.total : 0;
+}
+
+int varlen_q8_launch(const dvattn_varlen_args* a, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream) {
+    int st = widen_validate(a);
+    if (st != DVATTN_OK) return st;
+    if (!sc) return DVATTN_ERR_INVALID_ARGUMENT;
+    if (a->T == 0 || a->Hq == 0) return DVATTN_OK;
+    const bool cached = a->W > 0 && a->max_blocks_per_seq > 0 && a->num_blocks > 0;
+    if (!a->out || !a->queries || !a->cu_seqlens_q || !a->k_cache || !a->v_cache || !a->block_tables ||
+        (a->F > 0 && (!a->locations || !a->fragment_lengths)) || (a->R > 0 && (!a->cosines || !a->sines)) ||
+        (cached && (!sc->k_scales || !sc->v_scales)))
+        return DVATTN_ERR_INVALID_ARGUMENT;
+    for (const void* x : {a->queries, a->k_cache, a->v_cache, (const void*)a->out, (const void*)a->out_f32})
+        if (reinterpret_cast<uintptr_t>(x) & 15) return DVATTN_ERR_INVALID_ARGUMENT;
+    WidenLayout L;
+    if (!widen_layout(a, L)) return DVATTN_ERR_UNSUPPORTED;
+    if (!workspace || wbytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return DVATTN_ERR_WORKSPACE;
+    char* ws = static_cast<char*>(workspace);
+    L.wide.k_cache = ws + L.wk;
+    L.wide.v_cache = ws + L.wv;
+    if (L.own_table) L.wide.block_tables = reinterpret_cast<int*>(ws + L.table);
+    if (cached && a->F > 0) {
+        WidenParams p{};
+        p.F = a->F; p.W = a->W; p.T = a->T; p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks; p.Hkv = a->Hkv;
+        const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
+        p.cap = cap > 0x7fffffffLL ? 0x7fffffff : (int)cap;
+        p.own_table = L.own_table;
+        p.row16 = a->E / 16;
+        p.chunks = (long long)a->block_size * a->Hkv * p.row16;
+        p.loc = a->locations; p.L = a->fragment_lengths; p.cu = a->cu_seqlens_q; p.bt = a->block_tables;
+        p.k = static_cast<const uint8_t*>(a->k_cache); p.v = static_cast<const uint8_t*>(a->v_cache);
+        p.ks = sc->k_scales; p.vs = sc->v_scales;
+        p.span = reinterpret_cast<int*>(ws + L.span);
+        p.table = reinterpret_cast<int*>(ws + L.table);
+        p.wk = ws + L.wk; p.wv = ws + L.wv;
+        int dev = 0, sms = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+            cudaMemsetAsync(p.span, 0, 4 * (size_t)a->W * a->F, stream) != cudaSuccess)
+            return DVATTN_ERR_CUDA;
+        widen_span_kernel<<<dim3((unsigned)((a->T + 255) / 256), (unsigned)a->F), 256, 0, stream>>>(p);
+        const long long want = ((long long)a->W * a->max_blocks_per_seq + 7) / 8;
+        const unsigned grid = (unsigned)(want < 4LL * sms ? want : 4LL * sms);
+        switch (a->dtype) {
+            case DVATTN_FLOAT16: widen_kernel<__half><<<grid, 256, 0, stream>>>(p); break;
+            case DVATTN_BFLOAT16: widen_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p); break;
+            default: widen_kernel<float><<<grid, 256, 0, stream>>>(p); break;
+        }
+        if (cudaGetLastError() != cudaSuccess) return DVATTN_ERR_CUDA;
+    }
+    return varlen_launch(&L.wide, workspace, L.own, stream, DVATTN_PHASE_ALL);
+}
+
+}  // namespace dvb

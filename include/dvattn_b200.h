@@ -290,6 +290,60 @@ typedef struct dvattn_evict_args {
     const int* keep;              /* [W] i32                                             */
 } dvattn_evict_args;
 
+/*
+ * The scales of a cache held in 8 bits.  In the *_q8 calls k_cache [NB,BS,Hkv,E] and v_cache
+ * [NB,BS,Hkv,Ev] hold one byte per element, an e4m3 value (OCP FP8: largest 448, 0x7f / 0xff NaN, no
+ * infinities) that stands for itself times the scale of its page and KV head.  Scales of pages that
+ * hold keys are positive; between 2^-60 and 2^126 they are taken as they are, smaller ones may lose bits
+ * of small weights.  The append writes powers of two.
+ */
+typedef struct dvattn_q8_scales {
+    float* k_scales;              /* [NB,Hkv] f32; only the append writes them            */
+    float* v_scales;              /* [NB,Hkv] f32                                         */
+} dvattn_q8_scales;
+
+/*
+ * Arguments of the page assignment (dvattn_assign_pages).  Sequence w is to hold new tokens at
+ * logical positions starts[w] + i, i < counts[w]: entries of its block-table row that these
+ * positions fall on and that are negative (no page) get one from the free list, a stack of
+ * free_count[0] page numbers.  Sequences are served in order: one whose entries, with those of all
+ * sequences before it, need more pages than there are gets none (granted[w] = 0; one that needs
+ * none is granted all the same), and so does one whose start is negative or whose positions pass
+ * the table.  The pages taken are the topmost ones of the stack, the lowest of them first.
+ */
+typedef struct dvattn_assign_args {
+    int W;
+    int block_size;
+    int max_blocks_per_seq;
+    int free_size;                /* capacity of free_pages                               */
+    int n;                        /* slots per sequence in `slots`                        */
+    int* block_tables;            /* [W,max_blocks] i32, updated                          */
+    const int* free_pages;        /* [free_size] i32                                      */
+    int* free_count;              /* [1] i32, updated                                     */
+    const int* starts;            /* [W] i32                                              */
+    const int* counts;            /* [W] i32                                              */
+    int* granted;                 /* [W] i32: counts[w], or 0                             */
+    long long* slots;             /* optional [W,n] i64: page * block_size + offset of granted
+                                     token i < granted[w], -1 behind them and without a page */
+} dvattn_assign_args;
+
+/*
+ * Arguments of the pages' return (dvattn_release_pages): entries of sequence w's block-table row
+ * that lie wholly at or behind logical position keep[w] (negative: none stays) and hold a page
+ * become -1, and their pages are pushed on the free list, in the order of (w, entry).  Pages that
+ * find no room in the list stay where they are.
+ */
+typedef struct dvattn_release_args {
+    int W;
+    int block_size;
+    int max_blocks_per_seq;
+    int free_size;
+    int* block_tables;            /* [W,max_blocks] i32, updated                          */
+    int* free_pages;              /* [free_size] i32, updated                             */
+    int* free_count;              /* [1] i32, updated                                     */
+    const int* keep;              /* [W] i32                                              */
+} dvattn_release_args;
+
 /* ABI version of this header (bumped on any layout change of the structs above). */
 int dvattn_abi_version(void);
 
@@ -349,7 +403,7 @@ int dvattn_paged_sdpa_noalloc(const dvattn_paged_args* args, dvattn_stream_t str
 
 /*
  * Error word of the last attention call that used `workspace` (dvattn_paged_sdpa,
- * dvattn_varlen_paged_sdpa, dvattn_sdpa and their *_rope / *_phase forms, dvattn_tree_sdpa,
+ * dvattn_varlen_paged_sdpa, dvattn_sdpa and their *_rope / *_phase / *_q8 forms, dvattn_tree_sdpa,
  * dvattn_paged_mass), or, with workspace == NULL, of the last dvattn_paged_sdpa_noalloc call
  * on the current device.  Waits for `stream` (call it after the attention call, before the next call on the same
  * workspace).  *error_word == 0: the call completed.  Nonzero: a bounded wait inside a
@@ -443,6 +497,43 @@ size_t dvattn_paged_mass_workspace_size(const dvattn_mass_args* args);
 int dvattn_paged_mass(const dvattn_mass_args* args, void* workspace, size_t workspace_bytes, dvattn_stream_t stream);
 size_t dvattn_paged_evict_workspace_size(const dvattn_evict_args* args);
 int dvattn_paged_evict(const dvattn_evict_args* args, void* workspace, size_t workspace_bytes, dvattn_stream_t stream);
+
+/*
+ * The paged cache in 8 bits (dvattn_q8_scales): half the bytes of a 16-bit cache, which is what a
+ * decode step is bound by.  No counterpart in the reference.
+ *
+ * dvattn_paged_sdpa_q8: dvattn_paged_sdpa over such a cache (dtype is the queries' and the
+ * output's); the S tokens of a sequence share the reading of its keys.  Workspace and status as
+ * there.  What lies in a key or value reaches the tokens that see it and no other, NaN too.
+ *
+ * dvattn_varlen_paged_sdpa_q8: dvattn_varlen_paged_sdpa over such a cache.  The pages that the
+ * tokens see are first widened to dtype in the workspace (min(num_blocks, W * max_blocks) pages of both
+ * caches), so the products run as in the 16-bit prefill; tokens and cu_seqlens are treated as there.
+ * A page that several sequences share is meant the same to all of them.
+ *
+ * dvattn_paged_append_q8: dvattn_paged_append into such a cache.  Keys (rotated, rounded to dtype) and
+ * values x of a page and head are stored as e4m3(x / s), to nearest even, with s the page's scale: the
+ * least power of two (2^-60 or more) for which the largest finite |x| new to the page is at most 448 s,
+ * or, in a page that held tokens in front of them, the page's own scale where that is larger;
+ * where it is smaller, the tokens in front are stored again as e4m3(q * s_old / s).  Infinities become
+ * NaN.  A page must not be shared, nor appended to by two sequences of a call; whatever lies behind the
+ * last new token of a page is lost.
+ */
+size_t dvattn_paged_sdpa_q8_workspace_size(const dvattn_paged_args* args);
+int dvattn_paged_sdpa_q8(const dvattn_paged_args* args, const dvattn_q8_scales* scales, void* workspace, size_t workspace_bytes,
+                         dvattn_stream_t stream);
+size_t dvattn_varlen_paged_sdpa_q8_workspace_size(const dvattn_varlen_args* args);
+int dvattn_varlen_paged_sdpa_q8(const dvattn_varlen_args* args, const dvattn_q8_scales* scales, void* workspace,
+                                size_t workspace_bytes, dvattn_stream_t stream);
+int dvattn_paged_append_q8(const dvattn_append_args* args, const dvattn_q8_scales* scales, dvattn_stream_t stream);
+
+/*
+ * Block tables and slot maps on the GPU, from request lengths and a free list: pages for a step's new
+ * tokens, and pages back.  Both are one launch and may be captured in a graph.  No counterpart in the
+ * reference, whose callers keep their tables on the host.
+ */
+int dvattn_assign_pages(const dvattn_assign_args* args, dvattn_stream_t stream);
+int dvattn_release_pages(const dvattn_release_args* args, dvattn_stream_t stream);
 
 /*
  * Standalone query rotation, schema `dvattn_rope` (src/binding.cu:41-77, src/rope.cuh:2-65):
