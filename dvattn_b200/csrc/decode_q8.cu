@@ -27,6 +27,7 @@
 
 #include <cstdio>
 #include <cstdlib>
+#include <type_traits>
 
 namespace dvb {
 
@@ -37,8 +38,6 @@ struct Q8Params : TurnSplit {
     int hc, hs;             // KV heads a CTA reads together, groups of them (hc * hs = Hkv)
     int pairs;              // W * nt (sequence, row tile) pairs
     int box, box_shift;     // rows of a TMA box (gathered: rows of the stage), its log2
-    int gather;             // pages are no whole boxes: rows are copied one by one
-    int sc_shift;           // log2 of the keys that share an entry of the stage's scales
     long long tokens;       // all sequences' (a turn's stride in loc and cos / sin)
     int stall_tile;         // test hook (DVATTN_TEST_STALL_TILE), -1: off
     float scale_log2;
@@ -59,33 +58,50 @@ struct Q8Params : TurnSplit {
     float* part_lse;        // [CTAs][2][hc][rows of a tile] log2 sums, -inf: nothing seen
 };
 
-constexpr int kQ8Warps = 4;
+constexpr int kQ8Warps = 4, kQ8Threads = 256;
 constexpr int kQ8MaxPairs = 4096;  // their prefix sums lie in the stages at first
 
 // E: head dim, MT: 16-row tiles of a KV head's query rows, TERMS: f16 values per query element and weight.
-template <int E, int MT, int TERMS> struct Q8Cfg {
+template <int E, int MT, int TERMS, bool GATHER> struct Q8Cfg {
     static constexpr int KPW = E == 256 ? 16 : 32;      // keys of a warp in a window
     static constexpr int KROWS = kQ8Warps * KPW;        // (key, head) rows of a stage
     static constexpr int TENSOR = KROWS * E;            // bytes of K (or V) in a stage
     static constexpr int NT = KPW / 8;                  // 8-key tiles
     static constexpr int KS = E / 16;                   // 16-deep steps of q . k
     static constexpr int NJ = E / 8;                    // 8-column tiles of the output
-    static constexpr bool QREG = KS * MT * TERMS <= 8;  // q fragments in registers, else a lane keeps its own in shared memory
-    static constexpr int QBYTES = QREG ? 0 : kQ8Warps * KS * MT * TERMS * 512;
     static constexpr int ROWS = 16 * MT;
+    // A head's query fragments: in registers once read, else read for every window, from one of two buffers.
+    static constexpr int QHEAD = KS * MT * TERMS * 512;
+    static constexpr bool QREG = QHEAD <= 4096;
+    static constexpr int QBUFS = QREG ? 1 : 2, HEADS = QREG ? 4 : 2;  // buffers, KV heads of a CTA at most
+    static constexpr int QBYTES = QBUFS * HEADS * QHEAD;
     static constexpr int CTAS = QBYTES + 4 * TENSOR > 100 * 1024 ? 1 : 2;  // per SM
-    static constexpr int ROOM = (CTAS == 2 ? 113 : 226) * 1024 - QBYTES - 6 * 1024;
-    static constexpr int STAGES = ROOM / (2 * TENSOR) > 6 ? 6 : ROOM / (2 * TENSOR);
+    static constexpr int LIMIT = CTAS == 2 ? 115712 : 232448;              // shared memory of each
+    // Two CTAs of an SM have 128 registers a thread at their launch; the computing warpgroup takes what the other one
+    // gives up.
+    static constexpr int REGS = QREG ? 168 : 208, FEW = 2 * 128 - REGS;
+    static constexpr int SCALES = GATHER ? KROWS : KROWS / 8;  // of a tensor in a stage: of each row, or of 8 neighbours
+    // a row's factor, what it sees; [QBUFS][HEADS][ROWS], [QBUFS][ROWS], [QBUFS] the least of them
+    static constexpr int ROWINFO = QBUFS * (HEADS * ROWS + ROWS + 1) * 4;
+    // [warps][ROWS][2] maxima and sums, where several warps share a head (two heads at most: a single
+    // query buffer's second half is free)
+    static constexpr int ML = QREG ? 0 : kQ8Warps * ROWS * 8;
+    static constexpr int STAGE = 2 * TENSOR + 2 * SCALES * 4 + 32 + 16;  // tiles, scales, description, barriers
+    static constexpr int FIT = (LIMIT - QBYTES - ROWINFO - ML - 16 * QBUFS - 64) / STAGE;
+    static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr size_t OFF_Q = (size_t)STAGES * 2 * TENSOR;
-    static constexpr size_t OFF_SC = OFF_Q + QBYTES;                   // [STAGES][2][KROWS] scales
-    static constexpr size_t OFF_ML = OFF_SC + STAGES * 2 * KROWS * 4;  // [warps][ROWS][2]
-    static constexpr size_t OFF_DESC = OFF_ML + kQ8Warps * ROWS * 2 * 4;
-    static constexpr size_t OFF_BAR = OFF_DESC + STAGES * 48;
-    static constexpr size_t OFF_FLAG = OFF_BAR + STAGES * 16;
-    static constexpr size_t SMEM = OFF_FLAG + 16;
+    static constexpr size_t OFF_ML = QREG ? OFF_Q + 2 * QHEAD : OFF_Q + QBYTES;
+    static constexpr size_t OFF_SC = OFF_Q + QBYTES + ML;               // [STAGES][2][SCALES]
+    static constexpr size_t OFF_DESC = OFF_SC + STAGES * 2 * SCALES * 4;
+    static constexpr size_t OFF_BAR = OFF_DESC + STAGES * 32;           // full, empty, then q's
+    static constexpr size_t OFF_FR = OFF_BAR + STAGES * 16 + QBUFS * 16;
+    static constexpr size_t OFF_LIM = OFF_FR + QBUFS * HEADS * ROWS * 4;
+    static constexpr size_t OFF_FLAG = OFF_LIM + QBUFS * (ROWS + 1) * 4;
+    static constexpr size_t SMEM = OFF_FLAG + 4;
     static_assert(STAGES >= 2 && OFF_Q >= (kQ8MaxPairs + 40) * 8, "the prefix sums fit in the stages");
-    static_assert(SMEM <= (CTAS == 2 ? 113 : 227) * 1024, "shared memory");
+    static_assert(SMEM <= LIMIT && OFF_BAR % 16 == 0, "shared memory");
     static_assert(2 * TENSOR >= 2 * ROWS * E * 4, "two heads' rows are combined in a stage");
+    static_assert(!QREG || 2 * QHEAD >= kQ8Warps * ROWS * 8, "maxima and sums");
 };
 
 // ---- the windows of a (sequence, row tile) pair ------------------------------------------
@@ -99,12 +115,23 @@ __device__ __forceinline__ int pair_windows(const Q8Params& p, int rows, int pai
     int s0, s1, nw = 0;
     tile_tokens(p, rows, t, s0, s1);
     long long off = 0;
-    for (int f = 0; f < p.F; ++f) {
-        const int L = __ldg(p.L + f);
-        int sp = 0;
-        for (int s = s0; s <= s1; ++s) sp = max(sp, turn_seen(L, __ldg(p.loc + f * p.tokens + (size_t)w * p.S + s), off, p.cap));
-        nw += turn_windows(p, sp, sp > 0 ? (int)off : 0);
-        off += max(L, 0);
+    constexpr int AHEAD = 4;  // turns whose lengths and first locations are loaded together
+    for (int f0 = 0; f0 < p.F; f0 += AHEAD) {
+        int L[AHEAD], at[AHEAD];
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x)
+            if (f0 + x < p.F) {
+                L[x] = __ldg(p.L + f0 + x);
+                at[x] = __ldg(p.loc + (f0 + x) * p.tokens + (size_t)w * p.S + s0);
+            }
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x)
+            if (f0 + x < p.F) {
+                int sp = turn_seen(L[x], at[x], off, p.cap);
+                for (int s = s0 + 1; s <= s1; ++s) sp = max(sp, turn_seen(L[x], __ldg(p.loc + (f0 + x) * p.tokens + (size_t)w * p.S + s), off, p.cap));
+                nw += turn_windows(p, sp, sp > 0 ? (int)off : 0);
+                off += max(L[x], 0);
+            }
     }
     return nw;
 }
@@ -133,8 +160,8 @@ struct Q8Split {
 struct alignas(16) Q8Stage {
     int w, t, hg, f;
     int off, k0, sp, how;  // the turn's first position, first key, seen keys; Q8_* bits, -1: the end
-    int pad[4];
 };
+static_assert(sizeof(Q8Stage) == 32, "OFF_DESC");
 constexpr int Q8_ITEM = 1, Q8_TURN = 2, Q8_LAST = 4, Q8_WHOLE = 8, Q8_BEGIN = 16;
 
 // Walks units [u, u1) by a whole warp; every lane holds the same values.
@@ -169,6 +196,10 @@ struct Q8Walk {
         }
         wi = i;
         left -= i;
+    }
+    __device__ __forceinline__ void skip_turn() {  // its windows that have not been handed out
+        const int k = left < rem ? left : (int)rem;
+        left -= k, rem -= k, wi += k;
     }
     // The next window; false: none.  `ended`: the windows handed out before end their item.
     __device__ __forceinline__ bool next(const Q8Params& p, int rows, int lane, Q8Stage& d, bool& ended) {
@@ -255,25 +286,31 @@ __device__ const float kOne = 1.f;
 //   two rows are interleaved and widened in pairs.  A thread ends with 16 neighbouring elements twice.
 // * head dim 64: rows of 64 bytes; V words of 8 bytes, tile j of column n is element 8 c(n) + j with
 //   c(n) = n % 2 + 4 (n / 2 % 2) + 2 (n / 4).
-template <class T, int E, int MT>
-__global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1>::CTAS))
+template <class T, int E, int MT, bool GATHER>
+__global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1, GATHER>::CTAS))
     decode_q8_kernel(const __grid_constant__ Q8Params p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-    using C = Q8Cfg<E, MT, TERMS>;
+    using C = Q8Cfg<E, MT, TERMS, GATHER>;
     constexpr int KPW = C::KPW, NT = C::NT, KS = C::KS, NJ = C::NJ, STAGES = C::STAGES, ROWS = C::ROWS;
     constexpr int RB = E < 128 ? E : 128;  // bytes of a swizzled row
     constexpr int NP = E / RB;             // panels
-    constexpr int NTH = (kQ8Warps + 1) * 32;
+    constexpr int NTH = kQ8Threads;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t s0 = smem_u32(smem);
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    const uint32_t bar_full = s0 + (uint32_t)C::OFF_BAR, bar_empty = bar_full + STAGES * 8;
+    const uint32_t bar_full = s0 + (uint32_t)C::OFF_BAR, bar_empty = bar_full + STAGES * 8, bar_q = bar_empty + STAGES * 8;
+    float* sFr = reinterpret_cast<float*>(smem + C::OFF_FR);
+    int* sLim = reinterpret_cast<int*>(smem + C::OFF_LIM);
     volatile int* stop = reinterpret_cast<volatile int*>(smem + C::OFF_FLAG);
     Q8Stage* desc = reinterpret_cast<Q8Stage*>(smem + C::OFF_DESC);
     if (tid == 0) {
         for (int st = 0; st < STAGES; ++st) {
             mbar_init(bar_full + st * 8, 33);  // the request and the loading lanes' copies
             mbar_init(bar_empty + st * 8, kQ8Warps);
+        }
+        for (int x = 0; x < C::QBUFS; ++x) {
+            mbar_init(bar_q + x * 16, 3);             // the rotating warps
+            mbar_init(bar_q + x * 16 + 8, kQ8Warps);  // free again
         }
         *stop = 0;
         fence_mbar_init();
@@ -330,10 +367,86 @@ __global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) =
     fence_proxy_async_smem();  // TMA writes where the sums lay
     __syncthreads();
 
-    if (wid == kQ8Warps) {
+    if (wid >= kQ8Warps) {
+        if constexpr (C::CTAS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEW));
+        if (wid > kQ8Warps) {
+            // =================== the rotating warps ===================
+            // A turn ahead of the computing warps: the query rows rotated, scaled and split into fragments.  E / 16 lanes
+            // per row, 16 elements (a K word's columns) each.
+            constexpr int CPR = E / 16, RPW = 32 / CPR;
+            const bool vec = p.R % 16 == 0 && !((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15);
+            const int ch = lane % CPR;
+            Q8Walk walk;
+            walk.start(p, ROWS, lane, pair0, hg0, i0, u1 - u0);
+            Q8Stage d;
+            bool ended;
+            for (int n = 0; walk.next(p, ROWS, lane, d, ended); ++n) {
+                walk.skip_turn();
+                const int buf = n % C::QBUFS;
+                if (n >= C::QBUFS && (__any_sync(0xffffffffu, *stop != 0) || !__all_sync(0xffffffffu, mbar_wait(bar_q + buf * 16 + 8, (n / C::QBUFS - 1) & 1)))) {
+                    if (lane == 0) {
+                        *stop = 1;
+                        atomicOr(p.header + 3, 1);
+                    }
+                    return;
+                }
+                if (wid == kQ8Warps + 1) {  // what the rows see
+                    const int row = d.t * ROWS + lane;
+                    int v = d.sp;
+                    if (lane < ROWS && row < p.rows)
+                        v = turn_seen(__ldg(p.L + d.f), __ldg(p.loc + d.f * p.tokens + (size_t)d.w * p.S + row / p.G), d.off, p.cap);
+                    if (lane < ROWS) sLim[buf * (ROWS + 1) + lane] = v;
+                    v = __reduce_min_sync(0xffffffffu, v);
+                    if (lane == 0) sLim[buf * (ROWS + 1) + ROWS] = v;
+                }
+                uint8_t* sQ = smem + C::OFF_Q + (size_t)buf * C::HEADS * C::QHEAD;
+#pragma unroll 1
+                for (int r0 = (wid - kQ8Warps - 1) * RPW; r0 < p.hc * ROWS; r0 += 3 * RPW) {
+                    const int row_h = r0 + lane / CPR, hh = row_h / ROWS, i16 = row_h % ROWS, row = d.t * ROWS + i16;
+                    const bool there = row < p.rows;  // RPW divides hc * ROWS
+                    const int s = there ? row / p.G : 0, g = there ? row - s * p.G : 0, h = d.hg * p.hc + hh;
+                    const size_t tk = (size_t)d.w * p.S + s, angle = (d.f * p.tokens + tk) * p.R;
+                    const T* x = static_cast<const T*>(p.q) + (((size_t)d.w * p.Hq + h * p.G + g) * p.S + s) * E;
+                    float v[2][8];
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) rotated8<T, false>(x, p.cos + angle, p.sin + angle, 16 * ch + 8 * y, p.R, vec, v[y]);
+                    float top = 0.f;
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) {
+                        float& e = v[y >> 3][y & 7];
+                        if (!there) e = 0.f;
+                        top = fmaxf(top, fabsf(e));
+                    }
+#pragma unroll
+                    for (int o = CPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const int shift = min(140 - (__float_as_int(top) >> 23), 126);
+                    const float mul = __int_as_float((127 + shift) << 23);
+                    if (ch == 0) sFr[(buf * C::HEADS + hh) * ROWS + i16] = p.scale_log2 * __int_as_float((127 - shift) << 23);
+                    // chunk t + 4i of row n + 8 half of tile mt: step 4i + u, a[half] = its elements 4u, 4u + 1, a[2 + half] the next two
+                    uint8_t* dst = sQ + (size_t)hh * C::QHEAD + ((i16 >> 4) * TERMS * KS + 4 * (ch >> 2)) * 512 + ((i16 & 7) * 4 + (ch & 3)) * 16 + (i16 >> 3 & 1) * 4;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        float w[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) w[y] = v[u >> 1][(u & 1) * 4 + y] * mul;
+#pragma unroll
+                        for (int term = 0; term < TERMS; ++term) {
+                            const uint32_t lo = pack_f16(w[0], w[1]), hi = pack_f16(w[2], w[3]);
+                            *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512) = lo;
+                            *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512 + 8) = hi;
+                            const __half2 a = *reinterpret_cast<const __half2*>(&lo), b = *reinterpret_cast<const __half2*>(&hi);
+                            w[0] -= __low2float(a), w[1] -= __high2float(a), w[2] -= __low2float(b), w[3] -= __high2float(b);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_q + buf * 16);
+            }
+            return;
+        }
         // ======================= the requesting warp =======================
         const int boxes = p.kt >> p.box_shift;
-        if (lane == 0 && !p.gather) {
+        if (lane == 0 && !GATHER) {
             prefetch_tmap(&mk);
             prefetch_tmap(&mv);
         }
@@ -345,16 +458,12 @@ __global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) =
         auto find = [&] {
             have = walk.next(p, ROWS, lane, nxt, ended);
             if (!have) return;
-            const int n = p.gather ? p.kt : boxes, step = p.gather ? 1 : p.box;
+            const int n = GATHER ? p.kt : boxes, step = GATHER ? 1 : p.box;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
+            for (int x = 0; x < (GATHER ? 4 : 1); ++x) {
                 const int i = lane + 32 * x, l = nxt.k0 + i * step;
                 page[x] = -1;
-                if (i < n && l + step > 0 && l < nxt.sp) {
-                    const int g = __ldg(p.bt + (size_t)nxt.w * p.maxb + (nxt.off + l) / p.BS);
-                    if (g >= 0 && g < p.NB) page[x] = g;
-                }
-                if (!p.gather) break;
+                if (i < n && l + step > 0 && l < nxt.sp) page[x] = __ldg(p.bt + (size_t)nxt.w * p.maxb + (nxt.off + l) / p.BS);
             }
         };
         find();
@@ -377,7 +486,7 @@ __global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) =
             cur = nxt;
             int pg[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) pg[x] = page[x];
+            for (int x = 0; x < 4; ++x) pg[x] = page[x] < p.NB ? page[x] : -1;
             find();  // a window ahead: its table entries are under way while this one waits
             // the item's piece ends here where the next window begins another or there is none
             if (!have || (nxt.how & Q8_ITEM)) cur.how |= Q8_LAST | (ended && (cur.how & Q8_BEGIN) ? Q8_WHOLE : 0);
@@ -385,12 +494,12 @@ __global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) =
             const uint32_t dk = s0 + (uint32_t)(st * 2 * C::TENSOR), dv = dk + C::TENSOR, full = bar_full + st * 8;
             if (lane == 0) {
                 desc[st] = cur;
-                if (p.gather) mbar_arrive(full);
+                if (GATHER) mbar_arrive(full);
                 else mbar_expect_tx(full, 2u * C::TENSOR);
             }
             __syncwarp();
-            const uint32_t sc = s0 + (uint32_t)C::OFF_SC + (uint32_t)(st * 2 * C::KROWS * 4);
-            if (!p.gather) {
+            const uint32_t sc = s0 + (uint32_t)C::OFF_SC + (uint32_t)(st * 2 * C::SCALES * 4);
+            if constexpr (!GATHER) {
                 if (lane < boxes) {
                     const int pos = cur.off + cur.k0 + lane * p.box;
                     const int z = pg[0] >= 0 ? pg[0] * p.BS + pos % p.BS : -2 * p.box;  // rows outside: zeros
@@ -404,7 +513,7 @@ __global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) =
                     const int y = x < per ? x : x - per, g = y / p.hc;
                     const int b = __shfl_sync(0xffffffffu, pg[0], (g * 8) >> p.box_shift & 31);
                     if (x < 2 * per)
-                        cp_async4(sc + 4 * (y + (x < per ? 0 : C::KROWS)),
+                        cp_async4(sc + 4 * (y + (x < per ? 0 : C::SCALES)),
                                   b >= 0 ? (x < per ? p.ks : p.vs) + (size_t)b * p.Hkv + cur.hg * p.hc + y % p.hc : &kOne);
                 }
             } else {
@@ -430,7 +539,7 @@ __global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) =
                     const int b = k32 == 0 ? p0 : k32 == 1 ? p1 : k32 == 2 ? p2 : p3;
                     const size_t at = (size_t)b * p.Hkv + cur.hg * p.hc + x % p.hc;
                     cp_async4(sc + 4 * x, b >= 0 ? p.ks + at : &kOne);
-                    cp_async4(sc + 4 * (x + C::KROWS), b >= 0 ? p.vs + at : &kOne);
+                    cp_async4(sc + 4 * (x + C::SCALES), b >= 0 ? p.vs + at : &kOne);
                 }
             }
             cp_async_arrive(full);
@@ -449,6 +558,7 @@ __global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) =
     }
 
     // =========================== computing warps ===========================
+    if constexpr (C::CTAS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS));
     const int n = lane >> 2, t = lane & 3;
     const int hh = wid % p.hc, grp = wid / p.hc, wph = kQ8Warps / p.hc;  // head of the group, warps per head
     const int kw = grp * KPW;                                            // first key of the window
@@ -473,9 +583,9 @@ __global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) =
         vofs[0] = (uint32_t)(t * 64 + (((cn >> 1) ^ (t >> 1)) << 4) + ((cn & 1) << 3));
         vofs[1] = (uint32_t)((t + 4) * 64 + (((cn >> 1) ^ ((t + 4) >> 1 & 3)) << 4) + ((cn & 1) << 3));
     }
-    const uint32_t sQ = s0 + (uint32_t)C::OFF_Q + (uint32_t)(wid * KS * MT * TERMS * 512 + lane * 16);
+    uint32_t sQ = 0;  // this lane's fragments of the turn's buffer
+    int nq = 0;       // turns so far
     float* sML = reinterpret_cast<float*>(smem + C::OFF_ML);
-    const bool vec = p.R % 16 == 0 && !((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15);
 
     uint32_t qf[C::QREG ? MT * TERMS * KS : 1][4];
     float fr[MT][2];   // log2(e) * scale / (the row's power of two)
@@ -483,79 +593,276 @@ __global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) =
     int least = 0;     // that every row of the warp sees
     float o[MT][NJ][4], r[MT][2], l[MT][2];
 
-    auto load_q = [&](const Q8Stage& d) {
-        const int h = d.hg * p.hc + hh;
-        const int L = __ldg(p.L + d.f);
-        least = 0x7fffffff;
+    // The next turn's fragments and row values; false: a wait gave up.
+    auto take_q = [&] {
+        const int buf = nq % C::QBUFS;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar_q + buf * 16, (nq / C::QBUFS) & 1))) return false;
+        sQ = s0 + (uint32_t)C::OFF_Q + (uint32_t)((buf * C::HEADS + hh) * C::QHEAD + lane * 16);
+        if constexpr (C::QREG) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+            for (int x = 0; x < MT * TERMS * KS; ++x) {
+                const uint4 v = lds128(sQ + x * 512);
+                qf[x][0] = v.x, qf[x][1] = v.y, qf[x][2] = v.z, qf[x][3] = v.w;
+            }
+        }
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int row = d.t * ROWS + mt * 16 + half * 8 + n;
-                const bool there = row < p.rows;
-                const int s = there ? row / p.G : 0, g = there ? row - s * p.G : 0;
-                const size_t tk = (size_t)d.w * p.S + s;
-                const T* x = static_cast<const T*>(p.q) + (((size_t)d.w * p.Hq + h * p.G + g) * p.S + s) * E;
-                const float* cr = p.cos + (d.f * p.tokens + tk) * p.R;
-                const float* sr = p.sin + (d.f * p.tokens + tk) * p.R;
-                lim[mt][half] = there ? turn_seen(L, __ldg(p.loc + d.f * p.tokens + tk), d.off, p.cap) : d.sp;
-                least = min(least, lim[mt][half]);
-                uint32_t raw[TERMS == 1 ? KS * 2 : 1];  // T pairs
-                float val[TERMS == 1 ? 1 : KS * 4];
-                float top = 0.f;
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int e8 = 0; e8 < KS / 2; ++e8) {  // 8 elements: chunk t + 4 (e8 / 2), half e8 % 2
-                    float v[8];
-                    rotated8<T, false>(x, cr, sr, 16 * (t + 4 * (e8 >> 1)) + 8 * (e8 & 1), p.R, vec, v);
+            for (int y = 0; y < 2; ++y) {
+                fr[mt][y] = lds_f32(s0 + (uint32_t)C::OFF_FR + 4 * ((buf * C::HEADS + hh) * ROWS + mt * 16 + y * 8 + n));
+                lim[mt][y] = __float_as_int(lds_f32(s0 + (uint32_t)C::OFF_LIM + 4 * (buf * (ROWS + 1) + mt * 16 + y * 8 + n)));
+            }
+        least = __float_as_int(lds_f32(s0 + (uint32_t)C::OFF_LIM + 4 * (buf * (ROWS + 1) + ROWS)));
+        // the buffer that is free now: this one, or (fragments are read for every window) the one before
+        __syncwarp();
+        if (lane == 0 && (C::QREG || nq > 0)) mbar_arrive(bar_q + (C::QREG ? buf : buf ^ 1) * 16 + 8);
+        ++nq;
+        return true;
+    };
+
+    // One window's keys [first, first + KPW) of this warp.  EDGE: some row does not see them all.
+    auto window = [&](auto edge, const Q8Stage& d, int first, uint32_t kb, uint32_t sc) {
+        constexpr bool EDGE = decltype(edge)::value;
+        constexpr int NS = GATHER ? 2 : 1;  // scales of an 8-key tile that a thread needs: its keys' own, or the one page's
+        const uint32_t vb = kb + C::TENSOR;
+        // ---- scores ----
+        float z[MT][NT][4];
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        if (!there) v[u] = 0.f;
-                        top = fmaxf(top, fabsf(v[u]));
-                    }
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        if constexpr (TERMS == 1) {
-                            raw[e8 * 4 + u] = Elem<T>::pack2(v[2 * u], v[2 * u + 1]);
-                        } else {
-                            val[e8 * 8 + 2 * u] = v[2 * u];
-                            val[e8 * 8 + 2 * u + 1] = v[2 * u + 1];
-                        }
+            for (int x = 0; x < NT; ++x) z[mt][x][0] = z[mt][x][1] = z[mt][x][2] = z[mt][x][3] = 0.f;
+#pragma unroll
+        for (int ci = 0; ci < E / 64; ++ci) {
+            uint4 kf[NT];
+#pragma unroll
+            for (int x = 0; x < NT; ++x) kf[x] = lds128(kb + tile[x] + (ci >> 1) * panel + kofs[E < 128 ? 0 : ci & 1]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int ks = 4 * ci + u;
+                uint32_t a[MT * TERMS][4];
+#pragma unroll
+                for (int y = 0; y < MT * TERMS; ++y) {
+                    if constexpr (C::QREG) {
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) a[y][v] = qf[y * KS + ks][v];
+                    } else {
+                        const uint4 v = lds128(sQ + (uint32_t)((y * KS + ks) * 512));
+                        a[y][0] = v.x, a[y][1] = v.y, a[y][2] = v.z, a[y][3] = v.w;
                     }
                 }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int shift = min(140 - (__float_as_int(top) >> 23), 126);
-                const float mul = __int_as_float((127 + shift) << 23);
-                fr[mt][half] = p.scale_log2 * __int_as_float((127 - shift) << 23);
-                // step ks = 4i + u: a[half] = elements 4u, 4u + 1 of the chunk, a[2 + half] = 4u + 2, 4u + 3
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    float v[4];
-                    if constexpr (TERMS == 1) {
+                for (int x = 0; x < NT; ++x) {
+                    const uint32_t word = u == 0 ? kf[x].x : u == 1 ? kf[x].y : u == 2 ? kf[x].z : kf[x].w;
+                    const uint32_t b0 = e4m3x2_to_f16x2(word), b1 = e4m3x2_hi_to_f16x2(word);
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) v[u] = Elem<T>::to_f(reinterpret_cast<const T*>(&raw[ks * 2 + (u >> 1)])[u & 1]) * mul;
-                    } else {
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) v[u] = val[ks * 4 + u] * mul;
-                    }
+                        for (int term = TERMS - 1; term >= 0; --term) mma_f16(z[mt][x], a[mt * TERMS + term], b0, b1);
+                }
+            }
+        }
+        // ---- weights ----
+        float vscale[NT][NS];
 #pragma unroll
-                    for (int term = 0; term < TERMS; ++term) {
-                        const uint32_t lo = pack_f16(v[0], v[1]), hi = pack_f16(v[2], v[3]);
-                        const int at = (mt * TERMS + term) * KS + ks;
-                        if constexpr (C::QREG) {
-                            qf[at][half] = lo;
-                            qf[at][2 + half] = hi;
-                        } else {
-                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(sQ + at * 512 + half * 4), "r"(lo) : "memory");
-                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(sQ + at * 512 + 8 + half * 4), "r"(hi) : "memory");
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int at = GATHER ? (kw + 8 * x + t + 4 * y) * p.hc + hh : (kw / 8 + x) * p.hc + hh;
+                float ks, e;
+                if (GATHER || y == 0) {
+                    ks = lds_f32(sc + 4 * at);
+                    vscale[x][GATHER ? y : 0] = lds_f32(sc + 4 * (at + C::SCALES));
+                    e = Scale(vscale[x][GATHER ? y : 0]).e;
+#pragma unroll
+                    for (int y2 = y; y2 < (GATHER ? y + 1 : 2); ++y2)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            z[mt][x][y2] = fmaf(z[mt][x][y2], ks * fr[mt][0], e);
+                            z[mt][x][2 + y2] = fmaf(z[mt][x][2 + y2], ks * fr[mt][1], e);
                         }
-                        const __half2 a = *reinterpret_cast<const __half2*>(&lo), b = *reinterpret_cast<const __half2*>(&hi);
-                        v[0] -= __low2float(a), v[1] -= __high2float(a), v[2] -= __low2float(b), v[3] -= __high2float(b);
+                }
+                if constexpr (EDGE) {
+                    const int key_l = first + 8 * x + t + 4 * y;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        if (key_l < 0 || key_l >= lim[mt][0]) z[mt][x][y] = neg_inf();
+                        if (key_l < 0 || key_l >= lim[mt][1]) z[mt][x][2 + y] = neg_inf();
+                    }
+                }
+            }
+        bool moves = false;
+        float top[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                float m = neg_inf();
+#pragma unroll
+                for (int x = 0; x < NT; ++x) m = fmaxf(m, fmaxf(z[mt][x][2 * y], z[mt][x][2 * y + 1]));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                top[mt][y] = m;
+                moves |= m > r[mt][y] + 6.f;
+            }
+        if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const bool up = top[mt][y] > r[mt][y] + 6.f;
+                    const float alpha = up ? fast_exp2(r[mt][y] - top[mt][y]) : 1.f;
+                    if (up) r[mt][y] = top[mt][y];
+                    l[mt][y] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) o[mt][j][2 * y] *= alpha, o[mt][j][2 * y + 1] *= alpha;
+                }
+        }
+        uint32_t pa[MT][TERMS][NT / 2][4];
+        uint32_t unseen = 0;  // columns (x, y) that nobody sees
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const float ref0 = r[mt][0] == neg_inf() ? 0.f : r[mt][0] - 7.f, ref1 = r[mt][1] == neg_inf() ? 0.f : r[mt][1] - 7.f;
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                float w0[2], w1[2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const Scale s(vscale[x][GATHER ? y : 0]);
+                    const float a = fast_exp2(z[mt][x][y] - ref0), b = fast_exp2(z[mt][x][2 + y] - ref1);
+                    if constexpr (EDGE) {  // what a masked key's scales are does not matter
+                        const int key_l = first + 8 * x + t + 4 * y;
+                        const bool s0_ = key_l >= 0 && key_l < lim[mt][0], s1_ = key_l >= 0 && key_l < lim[mt][1];
+                        w0[y] = s0_ ? a * s.m : 0.f;
+                        w1[y] = s1_ ? b * s.m : 0.f;
+                        if (s0_) l[mt][0] = fmaf(a, s.inv, l[mt][0]);
+                        if (s1_) l[mt][1] = fmaf(b, s.inv, l[mt][1]);
+                        if (key_l < 0 || key_l >= d.sp) unseen |= 1u << (2 * x + y);
+                    } else {
+                        w0[y] = a * s.m;
+                        w1[y] = b * s.m;
+                        l[mt][0] = fmaf(a, s.inv, l[mt][0]);
+                        l[mt][1] = fmaf(b, s.inv, l[mt][1]);
+                    }
+                }
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term) {
+                    const uint32_t a = pack_f16(w0[0], w0[1]), b = pack_f16(w1[0], w1[1]);
+                    pa[mt][term][x >> 1][(x & 1) * 2] = a;
+                    pa[mt][term][x >> 1][(x & 1) * 2 + 1] = b;
+                    if (TERMS > 1) {
+                        const __half2 ah = *reinterpret_cast<const __half2*>(&a), bh = *reinterpret_cast<const __half2*>(&b);
+                        w0[0] -= __low2float(ah), w0[1] -= __high2float(ah), w1[0] -= __low2float(bh), w1[1] -= __high2float(bh);
                     }
                 }
             }
         }
-        least = __reduce_min_sync(0xffffffffu, least);
+        // ---- P V: a word of 4 elements of each of a thread's rows at a time ----
+        constexpr int VW = E < 128 ? 2 : 4;  // words a thread loads of a row of a panel
+#pragma unroll
+        for (int pn = 0; pn < NP; ++pn) {
+            uint32_t vw[NT][2][VW];
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const uint32_t at = vb + tile[x] + pn * panel + vofs[y];
+                    if constexpr (E < 128) {
+                        const uint2 v = lds64(at);
+                        vw[x][y][0] = v.x, vw[x][y][1] = v.y;
+                    } else {
+                        const uint4 v = lds128(at);
+                        vw[x][y][0] = v.x, vw[x][y][1] = v.y, vw[x][y][2] = v.z, vw[x][y][3] = v.w;
+                    }
+                }
+            if constexpr (EDGE) {
+                // keys that nobody sees: zeros.  A NaN in the value of a key that some rows see and others do not
+                // (0 * NaN is NaN) becomes a zero here and is added to the rows that see it.
+                bool odd = false;
+#pragma unroll
+                for (int x = 0; x < NT; ++x)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int u = 0; u < VW; ++u) {
+                            if (unseen >> (2 * x + y) & 1u) vw[x][y][u] = 0u;
+                            odd |= e4m3_nan(vw[x][y][u]) != 0;
+                        }
+                if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+                    for (int mt = 0; mt < MT; ++mt) {
+                        uint32_t ind[NT / 2][4];  // 1 where the row sees the key
+#pragma unroll
+                        for (int x = 0; x < NT; ++x)
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const int key_l = first + 8 * x + t;
+                                const int lm = mt == 0 ? lim[0][y] : lim[MT - 1][y];
+                                ind[x >> 1][(x & 1) * 2 + y] = (key_l >= 0 && key_l < lm ? 0x3c00u : 0u) | (key_l + 4 >= 0 && key_l + 4 < lm ? 0x3c000000u : 0u);
+                            }
+#pragma unroll
+                        for (int j = 0; j < 4 * VW; ++j) {
+                            float cnt[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int g = 0; g < NT / 2; ++g) {
+                                uint32_t b[2];
+#pragma unroll
+                                for (int y = 0; y < 2; ++y) {
+                                    const uint32_t fa = e4m3_nan(vw[2 * g + y][0][j >> 2]) >> (8 * (j & 3)), fb = e4m3_nan(vw[2 * g + y][1][j >> 2]) >> (8 * (j & 3));
+                                    b[y] = (fa & 0x80u ? 0x3c00u : 0u) | (fb & 0x80u ? 0x3c000000u : 0u);
+                                }
+                                mma_f16(cnt, ind[g], b[0], b[1]);
+                            }
+#pragma unroll
+                            for (int y = 0; y < 4; ++y)
+                                if (cnt[y] > 0.f) {
+                                    const float nan = __int_as_float(0x7fc00000);
+                                    if (mt == 0) o[0][pn * 4 * VW + j][y] = nan;
+                                    else o[MT - 1][pn * 4 * VW + j][y] = nan;
+                                }
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+#pragma unroll
+                            for (int u = 0; u < VW; ++u) vw[x][y][u] = clear_bytes(vw[x][y][u], e4m3_nan(vw[x][y][u]));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < VW; ++u) {
+                [[maybe_unused]] float part[TERMS > 1 ? 4 : 1][4];  // f32: a window's sum by itself, added with one rounding
+                if constexpr (TERMS > 1) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.f;
+                }
+#pragma unroll
+                for (int g = 0; g < NT / 2; ++g) {
+                    // bytes of two rows side by side: (0, 1) and (2, 3) of each
+                    const uint32_t a0 = __byte_perm(vw[2 * g][0][u], vw[2 * g][1][u], 0x5140), a1 = __byte_perm(vw[2 * g][0][u], vw[2 * g][1][u], 0x7362);
+                    const uint32_t c0 = __byte_perm(vw[2 * g + 1][0][u], vw[2 * g + 1][1][u], 0x5140),
+                                   c1 = __byte_perm(vw[2 * g + 1][0][u], vw[2 * g + 1][1][u], 0x7362);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t b0 = j == 0 ? e4m3x2_to_f16x2(a0) : j == 1 ? e4m3x2_hi_to_f16x2(a0) : j == 2 ? e4m3x2_to_f16x2(a1) : e4m3x2_hi_to_f16x2(a1);
+                        const uint32_t b1 = j == 0 ? e4m3x2_to_f16x2(c0) : j == 1 ? e4m3x2_hi_to_f16x2(c0) : j == 2 ? e4m3x2_to_f16x2(c1) : e4m3x2_hi_to_f16x2(c1);
+                        if constexpr (TERMS > 1) {
+#pragma unroll
+                            for (int term = TERMS - 1; term >= 0; --term) mma_f16(part[j], pa[0][term][g], b0, b1);
+                        } else {
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][pn * 4 * VW + 4 * u + j], pa[mt][0][g], b0, b1);
+                        }
+                    }
+                }
+                if constexpr (TERMS > 1) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) o[0][pn * 4 * VW + 4 * u + j][y] += part[j][y];
+                }
+            }
+        }
     };
 
     for (int i = 0;; ++i) {
@@ -579,244 +886,20 @@ __global__ void __launch_bounds__((kQ8Warps + 1) * 32, (Q8Cfg<E, MT, sizeof(T) =
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
             }
-        if (d.how & (Q8_ITEM | Q8_TURN)) load_q(d);
+        if ((d.how & Q8_TURN) && !take_q()) {
+            if (lane == 0) {
+                *stop = 1;
+                atomicOr(p.header + 3, 2);
+            }
+            __syncwarp();
+            continue;
+        }
 
         const int first = d.k0 + kw;  // key of the warp's first column
         if (first < d.sp && first + KPW > 0) {
-            const uint32_t kb = s0 + (uint32_t)(st * 2 * C::TENSOR), vb = kb + C::TENSOR;
-            const uint32_t sc = s0 + (uint32_t)C::OFF_SC + (uint32_t)(st * 2 * C::KROWS * 4);
-            const bool edge = first < 0 || first + KPW > least;
-            // ---- scores ----
-            float z[MT][NT][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int x = 0; x < NT; ++x) z[mt][x][0] = z[mt][x][1] = z[mt][x][2] = z[mt][x][3] = 0.f;
-#pragma unroll
-            for (int ci = 0; ci < E / 64; ++ci) {
-                uint4 kf[NT];
-#pragma unroll
-                for (int x = 0; x < NT; ++x) kf[x] = lds128(kb + tile[x] + (ci >> 1) * panel + kofs[E < 128 ? 0 : ci & 1]);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int ks = 4 * ci + u;
-                    uint32_t a[MT * TERMS][4];
-#pragma unroll
-                    for (int y = 0; y < MT * TERMS; ++y) {
-                        if constexpr (C::QREG) {
-#pragma unroll
-                            for (int v = 0; v < 4; ++v) a[y][v] = qf[y * KS + ks][v];
-                        } else {
-                            const uint4 v = lds128(sQ + (uint32_t)((y * KS + ks) * 512));
-                            a[y][0] = v.x, a[y][1] = v.y, a[y][2] = v.z, a[y][3] = v.w;
-                        }
-                    }
-#pragma unroll
-                    for (int x = 0; x < NT; ++x) {
-                        const uint32_t word = u == 0 ? kf[x].x : u == 1 ? kf[x].y : u == 2 ? kf[x].z : kf[x].w;
-                        const uint32_t b0 = e4m3x2_to_f16x2(word), b1 = e4m3x2_hi_to_f16x2(word);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                            for (int term = TERMS - 1; term >= 0; --term) mma_f16(z[mt][x], a[mt * TERMS + term], b0, b1);
-                    }
-                }
-            }
-            // ---- weights ----
-            float vscale[NT][2];
-#pragma unroll
-            for (int x = 0; x < NT; ++x)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const int key = kw + 8 * x + t + 4 * y, at = (key >> p.sc_shift) * p.hc + hh;
-                    const float ks = lds_f32(sc + 4 * at);
-                    vscale[x][y] = lds_f32(sc + 4 * (at + C::KROWS));
-                    const float e = Scale(vscale[x][y]).e;
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        z[mt][x][y] = fmaf(z[mt][x][y], ks * fr[mt][0], e);
-                        z[mt][x][2 + y] = fmaf(z[mt][x][2 + y], ks * fr[mt][1], e);
-                    }
-                    if (edge) {
-                        const int key_l = first + 8 * x + t + 4 * y;
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            if (key_l < 0 || key_l >= lim[mt][0]) z[mt][x][y] = neg_inf();
-                            if (key_l < 0 || key_l >= lim[mt][1]) z[mt][x][2 + y] = neg_inf();
-                        }
-                    }
-                }
-            bool moves = false;
-            float top[MT][2];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    float m = neg_inf();
-#pragma unroll
-                    for (int x = 0; x < NT; ++x) m = fmaxf(m, fmaxf(z[mt][x][2 * y], z[mt][x][2 * y + 1]));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                    top[mt][y] = m;
-                    moves |= m > r[mt][y] + 6.f;
-                }
-            if (__any_sync(0xffffffffu, moves)) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int y = 0; y < 2; ++y)
-                        if (top[mt][y] > r[mt][y] + 6.f) {
-                            const float alpha = fast_exp2(r[mt][y] - top[mt][y]);
-                            r[mt][y] = top[mt][y];
-                            l[mt][y] *= alpha;
-#pragma unroll
-                            for (int j = 0; j < NJ; ++j) o[mt][j][2 * y] *= alpha, o[mt][j][2 * y + 1] *= alpha;
-                        }
-            }
-            uint32_t pa[MT][TERMS][NT / 2][4];
-            uint32_t unseen = 0;  // columns (x, y) that nobody sees
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const float ref0 = r[mt][0] == neg_inf() ? 0.f : r[mt][0] - 7.f, ref1 = r[mt][1] == neg_inf() ? 0.f : r[mt][1] - 7.f;
-#pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                    float w0[2], w1[2];
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const Scale s(vscale[x][y]);
-                        const float a = fast_exp2(z[mt][x][y] - ref0), b = fast_exp2(z[mt][x][2 + y] - ref1);
-                        if (edge) {  // what a masked key's scales are does not matter
-                            const int key_l = first + 8 * x + t + 4 * y;
-                            const bool s0_ = key_l >= 0 && key_l < lim[mt][0], s1_ = key_l >= 0 && key_l < lim[mt][1];
-                            w0[y] = s0_ ? a * s.m : 0.f;
-                            w1[y] = s1_ ? b * s.m : 0.f;
-                            if (s0_) l[mt][0] = fmaf(a, s.inv, l[mt][0]);
-                            if (s1_) l[mt][1] = fmaf(b, s.inv, l[mt][1]);
-                            if (key_l < 0 || key_l >= d.sp) unseen |= 1u << (2 * x + y);
-                        } else {
-                            w0[y] = a * s.m;
-                            w1[y] = b * s.m;
-                            l[mt][0] = fmaf(a, s.inv, l[mt][0]);
-                            l[mt][1] = fmaf(b, s.inv, l[mt][1]);
-                        }
-                    }
-#pragma unroll
-                    for (int term = 0; term < TERMS; ++term) {
-                        const uint32_t a = pack_f16(w0[0], w0[1]), b = pack_f16(w1[0], w1[1]);
-                        pa[mt][term][x >> 1][(x & 1) * 2] = a;
-                        pa[mt][term][x >> 1][(x & 1) * 2 + 1] = b;
-                        if (TERMS > 1) {
-                            const __half2 ah = *reinterpret_cast<const __half2*>(&a), bh = *reinterpret_cast<const __half2*>(&b);
-                            w0[0] -= __low2float(ah), w0[1] -= __high2float(ah), w1[0] -= __low2float(bh), w1[1] -= __high2float(bh);
-                        }
-                    }
-                }
-            }
-            // ---- P V: a word of 4 elements of each of a thread's rows at a time ----
-            constexpr int VW = E < 128 ? 2 : 4;  // words a thread loads of a row of a panel
-#pragma unroll
-            for (int pn = 0; pn < NP; ++pn) {
-                uint32_t vw[NT][2][VW];
-#pragma unroll
-                for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const uint32_t at = vb + tile[x] + pn * panel + vofs[y];
-                        if constexpr (E < 128) {
-                            const uint2 v = lds64(at);
-                            vw[x][y][0] = v.x, vw[x][y][1] = v.y;
-                        } else {
-                            const uint4 v = lds128(at);
-                            vw[x][y][0] = v.x, vw[x][y][1] = v.y, vw[x][y][2] = v.z, vw[x][y][3] = v.w;
-                        }
-                    }
-                if (edge) {
-                    // keys that nobody sees: zeros.  A NaN in the value of a key that some rows see and others do not
-                    // (0 * NaN is NaN) becomes a zero here and is added to the rows that see it.
-                    bool odd = false;
-#pragma unroll
-                    for (int x = 0; x < NT; ++x)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y)
-#pragma unroll
-                            for (int u = 0; u < VW; ++u) {
-                                if (unseen >> (2 * x + y) & 1u) vw[x][y][u] = 0u;
-                                odd |= e4m3_nan(vw[x][y][u]) != 0;
-                            }
-                    if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll 1
-                        for (int mt = 0; mt < MT; ++mt) {
-                            uint32_t ind[NT / 2][4];  // 1 where the row sees the key
-#pragma unroll
-                            for (int x = 0; x < NT; ++x)
-#pragma unroll
-                                for (int y = 0; y < 2; ++y) {
-                                    const int key_l = first + 8 * x + t;
-                                    const int lm = mt == 0 ? lim[0][y] : lim[MT - 1][y];
-                                    ind[x >> 1][(x & 1) * 2 + y] = (key_l >= 0 && key_l < lm ? 0x3c00u : 0u) | (key_l + 4 >= 0 && key_l + 4 < lm ? 0x3c000000u : 0u);
-                                }
-#pragma unroll
-                            for (int j = 0; j < 4 * VW; ++j) {
-                                float cnt[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                                for (int g = 0; g < NT / 2; ++g) {
-                                    uint32_t b[2];
-#pragma unroll
-                                    for (int y = 0; y < 2; ++y) {
-                                        const uint32_t fa = e4m3_nan(vw[2 * g + y][0][j >> 2]) >> (8 * (j & 3)), fb = e4m3_nan(vw[2 * g + y][1][j >> 2]) >> (8 * (j & 3));
-                                        b[y] = (fa & 0x80u ? 0x3c00u : 0u) | (fb & 0x80u ? 0x3c000000u : 0u);
-                                    }
-                                    mma_f16(cnt, ind[g], b[0], b[1]);
-                                }
-#pragma unroll
-                                for (int y = 0; y < 4; ++y)
-                                    if (cnt[y] > 0.f) {
-                                        const float nan = __int_as_float(0x7fc00000);
-                                        if (mt == 0) o[0][pn * 4 * VW + j][y] = nan;
-                                        else o[MT - 1][pn * 4 * VW + j][y] = nan;
-                                    }
-                            }
-                        }
-#pragma unroll
-                        for (int x = 0; x < NT; ++x)
-#pragma unroll
-                            for (int y = 0; y < 2; ++y)
-#pragma unroll
-                                for (int u = 0; u < VW; ++u) vw[x][y][u] = clear_bytes(vw[x][y][u], e4m3_nan(vw[x][y][u]));
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < VW; ++u) {
-                    float part[TERMS > 1 ? 4 : 1][4];  // f32: a window's sum by itself, added with one rounding
-                    if constexpr (TERMS > 1)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.f;
-#pragma unroll
-                    for (int g = 0; g < NT / 2; ++g) {
-                        // bytes of two rows side by side: (0, 1) and (2, 3) of each
-                        const uint32_t a0 = __byte_perm(vw[2 * g][0][u], vw[2 * g][1][u], 0x5140), a1 = __byte_perm(vw[2 * g][0][u], vw[2 * g][1][u], 0x7362);
-                        const uint32_t c0 = __byte_perm(vw[2 * g + 1][0][u], vw[2 * g + 1][1][u], 0x5140),
-                                       c1 = __byte_perm(vw[2 * g + 1][0][u], vw[2 * g + 1][1][u], 0x7362);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t b0 = j == 0 ? e4m3x2_to_f16x2(a0) : j == 1 ? e4m3x2_hi_to_f16x2(a0) : j == 2 ? e4m3x2_to_f16x2(a1) : e4m3x2_hi_to_f16x2(a1);
-                            const uint32_t b1 = j == 0 ? e4m3x2_to_f16x2(c0) : j == 1 ? e4m3x2_hi_to_f16x2(c0) : j == 2 ? e4m3x2_to_f16x2(c1) : e4m3x2_hi_to_f16x2(c1);
-                            if constexpr (TERMS > 1) {
-#pragma unroll
-                                for (int term = TERMS - 1; term >= 0; --term) mma_f16(part[j], pa[0][term][g], b0, b1);
-                            } else {
-#pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][pn * 4 * VW + 4 * u + j], pa[mt][0][g], b0, b1);
-                            }
-                        }
-                    }
-                    if constexpr (TERMS > 1)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) o[0][pn * 4 * VW + 4 * u + j][y] += part[j][y];
-                }
-            }
+            const uint32_t kb = s0 + (uint32_t)(st * 2 * C::TENSOR), sc = s0 + (uint32_t)C::OFF_SC + (uint32_t)(st * 2 * C::SCALES * 4);
+            if (first < 0 || first + KPW > least) window(std::true_type(), d, first, kb, sc);
+            else window(std::false_type(), d, first, kb, sc);
         }
 
         if (!(d.how & Q8_LAST)) {
@@ -1033,14 +1116,16 @@ template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_ker
 namespace {
 
 struct Q8Kernel {
-    const void* fn;
+    const void* fn[2];  // pages that come by TMA, row by row
     const void* merge;
-    int krows, rows, ctas;  // CTAs per SM
-    size_t smem;
+    int krows, rows, ctas, heads;  // CTAs per SM, KV heads of one at most
+    size_t smem[2];
 };
 template <class T, int E, int MT> Q8Kernel q8_kernel() {
-    using C = Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1>;
-    return {(const void*)&decode_q8_kernel<T, E, MT>, (const void*)&merge_q8_kernel<T, E>, C::KROWS, C::ROWS, C::CTAS, C::SMEM};
+    using C = Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1, false>;
+    using G = Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1, true>;
+    static_assert(C::KROWS == G::KROWS && C::CTAS == G::CTAS && C::HEADS == G::HEADS, "one layout");
+    return {{(const void*)&decode_q8_kernel<T, E, MT, false>, (const void*)&decode_q8_kernel<T, E, MT, true>}, (const void*)&merge_q8_kernel<T, E>, C::KROWS, C::ROWS, C::CTAS, C::HEADS, {C::SMEM, G::SMEM}};
 }
 // One 16-row tile, or two where a KV head has more query rows (then the cache is read half as often); two
 // tiles do not fit in the registers with 32-bit queries or head dim 256.
@@ -1063,7 +1148,7 @@ int q8_layout(const dvattn_paged_args* a, const Q8Kernel& k, Q8Layout& L) {
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return DVATTN_ERR_CUDA;
     L.ctas = sms * k.ctas;
-    L.hc = a->Hkv % 4 == 0 ? 4 : a->Hkv % 2 == 0 ? 2 : 1;
+    L.hc = a->Hkv % 4 == 0 && k.heads == 4 ? 4 : a->Hkv % 2 == 0 ? 2 : 1;
     L.nt = (a->S * (a->Hq / a->Hkv) + k.rows - 1) / k.rows;
     L.slice = kQ8MaxPairs / L.nt;
     if (L.slice > a->W) L.slice = a->W;
@@ -1138,9 +1223,6 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
     Q8Layout L;
     if ((st = q8_layout(a, k, L)) != DVATTN_OK) return st;
     if (!workspace || wbytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return DVATTN_ERR_WORKSPACE;
-    if (cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem) != cudaSuccess ||
-        cudaFuncSetAttribute(k.fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
-        return DVATTN_ERR_CUDA;
     char* ws = static_cast<char*>(workspace);
     Q8Params p{};
     p.F = a->F; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.S = a->S; p.R = a->R;
@@ -1166,16 +1248,19 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
     int box = p.kt;
     while (p.BS % box) box >>= 1;
     alignas(64) CUtensorMap mk{}, mv{};
-    p.gather = box < 8 || !cached || a->num_blocks * a->block_size > 0x7fffffffLL - 2 * box;
-    if (p.gather) box = p.kt;
+    const bool gather = box < 8 || !cached || a->num_blocks * a->block_size > 0x7fffffffLL - 2 * box;
+    if (gather) box = p.kt;
     else if (!q8_map(&mk, a->k_cache, a->E, a->Hkv, L.hc, a->num_blocks * a->block_size, box) ||
              !q8_map(&mv, a->v_cache, a->E, a->Hkv, L.hc, a->num_blocks * a->block_size, box))
         return DVATTN_ERR_CUDA;
     p.box = box;
     while (1 << p.box_shift < box) ++p.box_shift;
-    p.align = p.gather ? 1 : box;
-    p.sc_shift = p.gather ? 0 : 3;
+    p.align = gather ? 1 : box;
 
+    const void* fn = k.fn[gather];
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem[gather]) != cudaSuccess ||
+        cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+        return DVATTN_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1191,9 +1276,9 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
         int rows = k.rows, ctas = L.ctas;
         void* args[] = {&p, &mk, &mv};
         cfg.gridDim = dim3((unsigned)L.ctas);
-        cfg.blockDim = dim3((kQ8Warps + 1) * 32);
-        cfg.dynamicSmemBytes = k.smem;
-        e = cudaLaunchKernelExC(&cfg, k.fn, args);
+        cfg.blockDim = dim3(kQ8Threads);
+        cfg.dynamicSmemBytes = k.smem[gather];
+        e = cudaLaunchKernelExC(&cfg, fn, args);
         if (e != cudaSuccess) break;
         void* margs[] = {&p, &rows, &ctas};
         const int rpb = 256 / (a->E / 4);
