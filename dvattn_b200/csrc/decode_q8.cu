@@ -53,6 +53,8 @@ struct Q8Params : TurnSplit {
     const float* vs;
     // workspace
     int* header;            // [3] error word (kErrorWordOffset)
+    const uint8_t* qf;      // [F][pairs][Hkv] {fragments, [rows] factors} of the rotated queries
+    const uint8_t* ql;      // [F][pairs] {[rows] keys of the turn that the row sees, the least of them, unused}
     long long* P;           // [pairs + 1] windows in front of a pair (of one head group)
     float* part_o;          // [CTAs][2][hc][rows of a tile][E]
     float* part_lse;        // [CTAs][2][hc][rows of a tile] log2 sums, -inf: nothing seen
@@ -71,37 +73,34 @@ template <int E, int MT, int TERMS, bool GATHER> struct Q8Cfg {
     static constexpr int NJ = E / 8;                    // 8-column tiles of the output
     static constexpr int ROWS = 16 * MT;
     // A head's query fragments: in registers once read, else read for every window, from one of two buffers.
-    static constexpr int QHEAD = KS * MT * TERMS * 512;
-    static constexpr bool QREG = QHEAD <= 4096;
+    static constexpr int QFRAG = KS * MT * TERMS * 512, QHEAD = QFRAG + ROWS * 4;  // ... and the rows' factors
+    static constexpr bool QREG = QFRAG <= 4096;
     static constexpr int QBUFS = QREG ? 1 : 2, HEADS = QREG ? 4 : 2;  // buffers, KV heads of a CTA at most
-    static constexpr int QBYTES = QBUFS * HEADS * QHEAD;
-    static constexpr int CTAS = QBYTES + 4 * TENSOR > 100 * 1024 ? 1 : 2;  // per SM
+    static constexpr int LIMS = (ROWS + 4) * 4;                       // what the rows of a tile see, and the least of it
+    static constexpr int QBUF = HEADS * QHEAD + LIMS, QBYTES = QBUFS * QBUF;
+    static constexpr int CTAS = QBYTES + 4 * TENSOR > 101 * 1024 ? 1 : 2;  // per SM
     static constexpr int LIMIT = CTAS == 2 ? 115712 : 232448;              // shared memory of each
     // Two CTAs of an SM have 128 registers a thread at their launch; the computing warpgroup takes what the other one
     // gives up.
-    static constexpr int REGS = QREG ? 168 : 208, FEW = 2 * 128 - REGS;
+    static constexpr int REGS = QREG ? 200 : 208, FEW = 2 * 128 - REGS;
     static constexpr int SCALES = GATHER ? KROWS : KROWS / 8;  // of a tensor in a stage: of each row, or of 8 neighbours
-    // a row's factor, what it sees; [QBUFS][HEADS][ROWS], [QBUFS][ROWS], [QBUFS] the least of them
-    static constexpr int ROWINFO = QBUFS * (HEADS * ROWS + ROWS + 1) * 4;
     // [warps][ROWS][2] maxima and sums, where several warps share a head (two heads at most: a single
     // query buffer's second half is free)
     static constexpr int ML = QREG ? 0 : kQ8Warps * ROWS * 8;
+    static_assert(!QREG || 2 * QHEAD >= kQ8Warps * ROWS * 8, "maxima and sums");
     static constexpr int STAGE = 2 * TENSOR + 2 * SCALES * 4 + 32 + 16;  // tiles, scales, description, barriers
-    static constexpr int FIT = (LIMIT - QBYTES - ROWINFO - ML - 16 * QBUFS - 64) / STAGE;
+    static constexpr int FIT = (LIMIT - QBYTES - ML - 16 * QBUFS - 4) / STAGE;
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr size_t OFF_Q = (size_t)STAGES * 2 * TENSOR;
-    static constexpr size_t OFF_ML = QREG ? OFF_Q + 2 * QHEAD : OFF_Q + QBYTES;
+    static constexpr size_t OFF_ML = QREG ? OFF_Q + 2 * QHEAD + LIMS : OFF_Q + QBYTES;
     static constexpr size_t OFF_SC = OFF_Q + QBYTES + ML;               // [STAGES][2][SCALES]
     static constexpr size_t OFF_DESC = OFF_SC + STAGES * 2 * SCALES * 4;
     static constexpr size_t OFF_BAR = OFF_DESC + STAGES * 32;           // full, empty, then q's
-    static constexpr size_t OFF_FR = OFF_BAR + STAGES * 16 + QBUFS * 16;
-    static constexpr size_t OFF_LIM = OFF_FR + QBUFS * HEADS * ROWS * 4;
-    static constexpr size_t OFF_FLAG = OFF_LIM + QBUFS * (ROWS + 1) * 4;
+    static constexpr size_t OFF_FLAG = OFF_BAR + STAGES * 16 + QBUFS * 16;
     static constexpr size_t SMEM = OFF_FLAG + 4;
     static_assert(STAGES >= 2 && OFF_Q >= (kQ8MaxPairs + 40) * 8, "the prefix sums fit in the stages");
     static_assert(SMEM <= LIMIT && OFF_BAR % 16 == 0, "shared memory");
     static_assert(2 * TENSOR >= 2 * ROWS * E * 4, "two heads' rows are combined in a stage");
-    static_assert(!QREG || 2 * QHEAD >= kQ8Warps * ROWS * 8, "maxima and sums");
 };
 
 // ---- the windows of a (sequence, row tile) pair ------------------------------------------
@@ -140,11 +139,13 @@ __device__ __forceinline__ int pair_windows(const Q8Params& p, int rows, int pai
 struct Q8Split {
     long long q, r;
     int n;
-    __device__ __forceinline__ Q8Split(long long total, const Q8Params& p, int ctas) {
-        const long long most = total / p.least;
-        n = most < ctas ? (most > 0 ? (int)most : 1) : ctas;
-        q = total / n;
-        r = total % n;
+    __device__ __forceinline__ Q8Split(long long total, int ctas) {
+        n = total < ctas ? (total > 0 ? (int)total : 1) : ctas;
+        q = over(total, n);
+        r = total - q * n;
+    }
+    static __device__ __forceinline__ long long over(long long a, long long b) {  // in 32 bits where both allow
+        return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
     }
     __device__ __forceinline__ long long begin(int c) const {
         if (c > n) c = n;
@@ -152,7 +153,7 @@ struct Q8Split {
     }
     __device__ __forceinline__ int cta_of(long long u) const {
         const long long more = r * (q + 1);
-        return (int)(u < more ? u / (q + 1) : r + (u - more) / q);
+        return (int)(u < more ? over(u, q + 1) : r + over(u - more, q));
     }
 };
 
@@ -273,6 +274,81 @@ struct Scale {
 };
 __device__ const float kOne = 1.f;
 
+// ---- the rotation ----------------------------------------------------------------------------
+// Block (f, pair, h): the tile's query rows of KV head h rotated for turn f, scaled and split into the fragments that
+// the attention kernel reads (below), E / 8 lanes per row.  It runs while the attention kernel finds its split and requests
+// its first windows.  By the attention kernel's own warps, a turn took 4 to 10 us, in rounds of loads that few
+// registers allow.
+template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_q8_kernel(const __grid_constant__ Q8Params p, uint8_t* qf, uint8_t* ql) {
+    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+    using C = Q8Cfg<E, MT, TERMS, false>;
+    constexpr int ROWS = C::ROWS, KS = C::KS, LPR = E / 8, STEP = 128 / LPR;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int h = blockIdx.x % p.Hkv, fp = blockIdx.x / p.Hkv, f = fp / p.pairs, pair = fp - f * p.pairs;
+    const int w = p.w0 + pair / p.nt, t = pair % p.nt, tid = threadIdx.x;
+    long long off = 0;
+    for (int x = 0; x < f; ++x) off += max(__ldg(p.L + x), 0);
+    const int L = __ldg(p.L + f);
+    int s0, s1, sp = 0;
+    tile_tokens(p, ROWS, t, s0, s1);
+    const int* loc = p.loc + f * p.tokens + (size_t)w * p.S;
+    const bool vec = p.R % 16 == 0 && !((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15);
+    const int ch = tid % LPR;
+    float v[ROWS / STEP][8];
+#pragma unroll
+    for (int i = 0; i < ROWS / STEP; ++i) {
+        const int row = t * ROWS + i * STEP + tid / LPR;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[i][u] = 0.f;
+        if (row < p.rows) {
+            const int s = row / p.G;
+            const size_t angle = (f * p.tokens + (size_t)w * p.S + s) * p.R;
+            rotated8<T, false>(static_cast<const T*>(p.q) + (((size_t)w * p.Hq + h * p.G + row - s * p.G) * p.S + s) * E, p.cos + angle, p.sin + angle, 8 * ch,
+                               p.R, vec, v[i]);
+        }
+    }
+    for (int s = s0; s <= s1; ++s) sp = max(sp, turn_seen(L, __ldg(loc + s), off, p.cap));
+    if (sp == 0) return;  // nobody reads the turn
+    if (h == 0 && tid < 32) {
+        const int row = t * ROWS + tid, see = tid < ROWS && row < p.rows ? turn_seen(L, __ldg(loc + row / p.G), off, p.cap) : sp;
+        int* dst = reinterpret_cast<int*>(ql + (size_t)fp * C::LIMS);
+        if (tid < ROWS) dst[tid] = see;
+        const int least = __reduce_min_sync(0xffffffffu, see);
+        if (tid == 0) dst[ROWS] = least;
+    }
+    uint8_t* head = qf + (size_t)blockIdx.x * C::QHEAD;
+#pragma unroll
+    for (int i = 0; i < ROWS / STEP; ++i) {
+        const int i16 = i * STEP + tid / LPR;
+        float top = 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(v[i][u]));
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int shift = min(140 - (__float_as_int(top) >> 23), 126);
+        const float mul = __int_as_float((127 + shift) << 23);
+        if (ch == 0) reinterpret_cast<float*>(head + C::QFRAG)[i16] = p.scale_log2 * __int_as_float((127 - shift) << 23);
+        // 16-byte chunk t + 4j of row n + 8 half of tile mt: step 4j + u, a[half] = its elements 4u, 4u + 1, a[2 + half] the next two
+        const int c16 = ch >> 1;
+        uint8_t* dst = head + ((i16 >> 4) * TERMS * KS + 4 * (c16 >> 2) + 2 * (ch & 1)) * 512 + ((i16 & 7) * 4 + (c16 & 3)) * 16 + (i16 >> 3 & 1) * 4;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float x[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) x[y] = v[i][u * 4 + y] * mul;
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) {
+                const uint32_t lo = pack_f16(x[0], x[1]), hi = pack_f16(x[2], x[3]);
+                *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512) = lo;
+                *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512 + 8) = hi;
+                const __half2 a = *reinterpret_cast<const __half2*>(&lo), b = *reinterpret_cast<const __half2*>(&hi);
+                x[0] -= __low2float(a), x[1] -= __high2float(a), x[2] -= __low2float(b), x[3] -= __high2float(b);
+            }
+        }
+    }
+}
+
 // ---- the attention kernel ---------------------------------------------------------------------
 // Warps 0 .. 3 compute, warp 4 requests the windows.  Warp w works on head w % hc of the group and keys
 // [KPW (w / hc), + KPW) of the window; thread (n, t) = (lane / 4, lane % 4).
@@ -299,8 +375,6 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
     const uint32_t s0 = smem_u32(smem);
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const uint32_t bar_full = s0 + (uint32_t)C::OFF_BAR, bar_empty = bar_full + STAGES * 8, bar_q = bar_empty + STAGES * 8;
-    float* sFr = reinterpret_cast<float*>(smem + C::OFF_FR);
-    int* sLim = reinterpret_cast<int*>(smem + C::OFF_LIM);
     volatile int* stop = reinterpret_cast<volatile int*>(smem + C::OFF_FLAG);
     Q8Stage* desc = reinterpret_cast<Q8Stage*>(smem + C::OFF_DESC);
     if (tid == 0) {
@@ -309,21 +383,20 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
             mbar_init(bar_empty + st * 8, kQ8Warps);
         }
         for (int x = 0; x < C::QBUFS; ++x) {
-            mbar_init(bar_q + x * 16, 3);             // the rotating warps
+            mbar_init(bar_q + x * 16, 1);
             mbar_init(bar_q + x * 16 + 8, kQ8Warps);  // free again
         }
         *stop = 0;
         fence_mbar_init();
     }
-    // a programmatic dependent of whatever is before it: nothing is read or written earlier
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // A programmatic dependent of the rotation, whose blocks let this grid begin once whatever is before them has ended: the
+    // call's inputs and outputs are free.  What the rotation writes is waited for where it is read.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int c = blockIdx.x;
     const bool aligned = (s0 & 1023) == 0;  // as the swizzle needs the stages
     // cleared once per call: a bounded wait that gives up sets its bit long after
     if (c == 0 && tid == 0 && (p.w0 == 0 || !aligned)) p.header[3] = aligned ? 0 : 4;
     if (!aligned) return;
-
     // ---- the split: every CTA adds up the windows of all pairs and finds its own range ----
     long long* sP = reinterpret_cast<long long*>(smem);  // [pairs + 1], in the stages
     long long* scratch = sP + p.pairs + 1;
@@ -350,7 +423,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
     if (tid == 0) sP[p.pairs] = carry;
     __syncthreads();
     for (int i = c * NTH + tid; i <= p.pairs; i += gridDim.x * NTH) p.P[i] = sP[i];  // for the merge
-    const Q8Split split(carry * p.hs, p, gridDim.x);
+    const Q8Split split(carry * p.hs, gridDim.x);
     const long long u0 = split.begin(c), u1 = split.begin(c + 1);
     if (u0 >= u1) return;
     int pair0 = 0;
@@ -363,19 +436,17 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
     }
     const long long local = u0 - sP[pair0] * p.hs;
     const int nw0 = (int)(sP[pair0 + 1] - sP[pair0]);
-    const int hg0 = (int)(local / nw0), i0 = (int)(local - (long long)hg0 * nw0);
+    const int hg0 = (int)Q8Split::over(local, nw0), i0 = (int)(local - (long long)hg0 * nw0);
     fence_proxy_async_smem();  // TMA writes where the sums lay
     __syncthreads();
 
     if (wid >= kQ8Warps) {
         if constexpr (C::CTAS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEW));
-        if (wid > kQ8Warps) {
-            // =================== the rotating warps ===================
-            // A turn ahead of the computing warps: the query rows rotated, scaled and split into fragments.  E / 16 lanes
-            // per row, 16 elements (a K word's columns) each.
-            constexpr int CPR = E / 16, RPW = 32 / CPR;
-            const bool vec = p.R % 16 == 0 && !((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15);
-            const int ch = lane % CPR;
+        if (wid > kQ8Warps + 1) return;
+        if (wid == kQ8Warps + 1) {
+            // =================== requests the turns' fragments ===================
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            asm volatile("fence.proxy.async;" ::: "memory");  // written with ordinary stores, read by bulk copies
             Q8Walk walk;
             walk.start(p, ROWS, lane, pair0, hg0, i0, u1 - u0);
             Q8Stage d;
@@ -388,59 +459,16 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
                         *stop = 1;
                         atomicOr(p.header + 3, 1);
                     }
-                    return;
+                    break;
                 }
-                if (wid == kQ8Warps + 1) {  // what the rows see
-                    const int row = d.t * ROWS + lane;
-                    int v = d.sp;
-                    if (lane < ROWS && row < p.rows)
-                        v = turn_seen(__ldg(p.L + d.f), __ldg(p.loc + d.f * p.tokens + (size_t)d.w * p.S + row / p.G), d.off, p.cap);
-                    if (lane < ROWS) sLim[buf * (ROWS + 1) + lane] = v;
-                    v = __reduce_min_sync(0xffffffffu, v);
-                    if (lane == 0) sLim[buf * (ROWS + 1) + ROWS] = v;
-                }
-                uint8_t* sQ = smem + C::OFF_Q + (size_t)buf * C::HEADS * C::QHEAD;
-#pragma unroll 1
-                for (int r0 = (wid - kQ8Warps - 1) * RPW; r0 < p.hc * ROWS; r0 += 3 * RPW) {
-                    const int row_h = r0 + lane / CPR, hh = row_h / ROWS, i16 = row_h % ROWS, row = d.t * ROWS + i16;
-                    const bool there = row < p.rows;  // RPW divides hc * ROWS
-                    const int s = there ? row / p.G : 0, g = there ? row - s * p.G : 0, h = d.hg * p.hc + hh;
-                    const size_t tk = (size_t)d.w * p.S + s, angle = (d.f * p.tokens + tk) * p.R;
-                    const T* x = static_cast<const T*>(p.q) + (((size_t)d.w * p.Hq + h * p.G + g) * p.S + s) * E;
-                    float v[2][8];
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) rotated8<T, false>(x, p.cos + angle, p.sin + angle, 16 * ch + 8 * y, p.R, vec, v[y]);
-                    float top = 0.f;
-#pragma unroll
-                    for (int y = 0; y < 16; ++y) {
-                        float& e = v[y >> 3][y & 7];
-                        if (!there) e = 0.f;
-                        top = fmaxf(top, fabsf(e));
-                    }
-#pragma unroll
-                    for (int o = CPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    const int shift = min(140 - (__float_as_int(top) >> 23), 126);
-                    const float mul = __int_as_float((127 + shift) << 23);
-                    if (ch == 0) sFr[(buf * C::HEADS + hh) * ROWS + i16] = p.scale_log2 * __int_as_float((127 - shift) << 23);
-                    // chunk t + 4i of row n + 8 half of tile mt: step 4i + u, a[half] = its elements 4u, 4u + 1, a[2 + half] the next two
-                    uint8_t* dst = sQ + (size_t)hh * C::QHEAD + ((i16 >> 4) * TERMS * KS + 4 * (ch >> 2)) * 512 + ((i16 & 7) * 4 + (ch & 3)) * 16 + (i16 >> 3 & 1) * 4;
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        float w[4];
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) w[y] = v[u >> 1][(u & 1) * 4 + y] * mul;
-#pragma unroll
-                        for (int term = 0; term < TERMS; ++term) {
-                            const uint32_t lo = pack_f16(w[0], w[1]), hi = pack_f16(w[2], w[3]);
-                            *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512) = lo;
-                            *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512 + 8) = hi;
-                            const __half2 a = *reinterpret_cast<const __half2*>(&lo), b = *reinterpret_cast<const __half2*>(&hi);
-                            w[0] -= __low2float(a), w[1] -= __high2float(a), w[2] -= __low2float(b), w[3] -= __high2float(b);
-                        }
-                    }
+                if (lane == 0) {
+                    const uint32_t dst = s0 + (uint32_t)(C::OFF_Q + (size_t)buf * C::QBUF);
+                    const size_t at = (size_t)d.f * p.pairs + (size_t)(d.w - p.w0) * p.nt + d.t;
+                    mbar_expect_tx(bar_q + buf * 16, (uint32_t)(p.hc * C::QHEAD + C::LIMS));
+                    bulk_load(dst, p.qf + (at * p.Hkv + (size_t)d.hg * p.hc) * C::QHEAD, p.hc * C::QHEAD, bar_q + buf * 16);
+                    bulk_load(dst + (uint32_t)(p.hc * C::QHEAD), p.ql + at * C::LIMS, C::LIMS, bar_q + buf * 16);
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_q + buf * 16);
             }
             return;
         }
@@ -597,7 +625,9 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
     auto take_q = [&] {
         const int buf = nq % C::QBUFS;
         if (!__all_sync(0xffffffffu, mbar_wait(bar_q + buf * 16, (nq / C::QBUFS) & 1))) return false;
-        sQ = s0 + (uint32_t)C::OFF_Q + (uint32_t)((buf * C::HEADS + hh) * C::QHEAD + lane * 16);
+        const uint32_t base = s0 + (uint32_t)(C::OFF_Q + (size_t)buf * C::QBUF), head = base + (uint32_t)(hh * C::QHEAD);
+        const uint32_t limits = base + (uint32_t)(p.hc * C::QHEAD);
+        sQ = head + lane * 16;
         if constexpr (C::QREG) {
 #pragma unroll
             for (int x = 0; x < MT * TERMS * KS; ++x) {
@@ -609,10 +639,10 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                fr[mt][y] = lds_f32(s0 + (uint32_t)C::OFF_FR + 4 * ((buf * C::HEADS + hh) * ROWS + mt * 16 + y * 8 + n));
-                lim[mt][y] = __float_as_int(lds_f32(s0 + (uint32_t)C::OFF_LIM + 4 * (buf * (ROWS + 1) + mt * 16 + y * 8 + n)));
+                fr[mt][y] = lds_f32(head + C::QFRAG + 4 * (mt * 16 + y * 8 + n));
+                lim[mt][y] = __float_as_int(lds_f32(limits + 4 * (mt * 16 + y * 8 + n)));
             }
-        least = __float_as_int(lds_f32(s0 + (uint32_t)C::OFF_LIM + 4 * (buf * (ROWS + 1) + ROWS)));
+        least = __float_as_int(lds_f32(limits + 4 * ROWS));
         // the buffer that is free now: this one, or (fragments are read for every window) the one before
         __syncwarp();
         if (lane == 0 && (C::QREG || nq > 0)) mbar_arrive(bar_q + (C::QREG ? buf : buf ^ 1) * 16 + 8);
@@ -1057,7 +1087,7 @@ template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_ker
     const bool failed = __ldcg(p.header + 3) != 0;
     int c0 = 0, c1 = -1;  // CTAs of the item
     if (nw > 0 && !failed) {
-        const Q8Split split(total * p.hs, p, ctas);
+        const Q8Split split(total * p.hs, ctas);
         const long long us = P0 * p.hs + hg * nw;
         c0 = split.cta_of(us), c1 = split.cta_of(us + nw - 1);
         if (c0 == c1) return;
@@ -1117,7 +1147,9 @@ namespace {
 
 struct Q8Kernel {
     const void* fn[2];  // pages that come by TMA, row by row
+    const void* rotate;
     const void* merge;
+    int qhead, lims;        // bytes of a head's fragments and factors, of a tile's limits
     int krows, rows, ctas, heads;  // CTAs per SM, KV heads of one at most
     size_t smem[2];
 };
@@ -1125,7 +1157,8 @@ template <class T, int E, int MT> Q8Kernel q8_kernel() {
     using C = Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1, false>;
     using G = Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1, true>;
     static_assert(C::KROWS == G::KROWS && C::CTAS == G::CTAS && C::HEADS == G::HEADS, "one layout");
-    return {{(const void*)&decode_q8_kernel<T, E, MT, false>, (const void*)&decode_q8_kernel<T, E, MT, true>}, (const void*)&merge_q8_kernel<T, E>, C::KROWS, C::ROWS, C::CTAS, C::HEADS, {C::SMEM, G::SMEM}};
+    return {{(const void*)&decode_q8_kernel<T, E, MT, false>, (const void*)&decode_q8_kernel<T, E, MT, true>}, (const void*)&rotate_q8_kernel<T, E, MT>,
+            (const void*)&merge_q8_kernel<T, E>, C::QHEAD, C::LIMS, C::KROWS, C::ROWS, C::CTAS, C::HEADS, {C::SMEM, G::SMEM}};
 }
 // One 16-row tile, or two where a KV head has more query rows (then the cache is read half as often); two
 // tiles do not fit in the registers with 32-bit queries or head dim 256.
@@ -1140,7 +1173,7 @@ Q8Kernel q8_pick(int dtype, int E, int rows) {
 }
 
 struct Q8Layout {
-    size_t P, po, pl, total;
+    size_t P, qf, ql, po, pl, total;
     int ctas, hc, nt, slice;  // slice: sequences of a launch
 };
 int q8_layout(const dvattn_paged_args* a, const Q8Kernel& k, Q8Layout& L) {
@@ -1159,6 +1192,8 @@ int q8_layout(const dvattn_paged_args* a, const Q8Kernel& k, Q8Layout& L) {
         return r;
     };
     L.P = take(8 * ((size_t)L.slice * L.nt + 1));
+    L.qf = take((size_t)a->F * L.slice * L.nt * a->Hkv * k.qhead);
+    L.ql = take((size_t)a->F * L.slice * L.nt * k.lims);
     L.po = take(4 * (size_t)L.ctas * 2 * L.hc * k.rows * a->E);
     L.pl = take(4 * (size_t)L.ctas * 2 * L.hc * k.rows);
     L.total = at;
@@ -1171,7 +1206,7 @@ int q8_validate(const dvattn_paged_args* a) {
     const long long rows = (long long)a->S * (a->Hq / a->Hkv);
     if (a->num_blocks < 0) return DVATTN_ERR_INVALID_ARGUMENT;
     // a sequence's row tiles are one launch's
-    if (rows > 16LL * kQ8MaxPairs || (long long)a->F * a->W * a->S > 0x7fffffffLL || (long long)kQ8MaxPairs * a->Hkv > 0x7fffffffLL)
+    if (rows > 16LL * kQ8MaxPairs || (long long)a->F * a->W * a->S > 0x7fffffffLL || (long long)kQ8MaxPairs * a->Hkv * (a->F > 0 ? a->F : 1) > 0x7fffffffLL)
         return DVATTN_ERR_UNSUPPORTED;
     return DVATTN_OK;
 }
@@ -1232,7 +1267,6 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
     p.cap = a->num_blocks <= 0 ? 0 : cap > kMostPositions ? kMostPositions : (int)cap;
     p.hc = L.hc; p.hs = a->Hkv / L.hc; p.nt = L.nt; p.groups = L.ctas;
     p.kt = k.krows / L.hc;
-    p.least = 1;
     p.tokens = (long long)a->W * a->S;
     p.scale_log2 = a->scale * kLog2e;
     p.out = a->out; p.lse_out = a->lse_out; p.out_f32 = a->out_f32;
@@ -1241,6 +1275,10 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
     p.ks = sc->k_scales; p.vs = sc->v_scales; p.bt = a->block_tables;
     p.stall_tile = q8_stall_hook();
     p.header = reinterpret_cast<int*>(ws);
+    uint8_t* qf = reinterpret_cast<uint8_t*>(ws + L.qf);
+    uint8_t* ql = reinterpret_cast<uint8_t*>(ws + L.ql);
+    p.qf = qf;
+    p.ql = ql;
     p.P = reinterpret_cast<long long*>(ws + L.P);
     p.part_o = reinterpret_cast<float*>(ws + L.po);
     p.part_lse = reinterpret_cast<float*>(ws + L.pl);
@@ -1274,11 +1312,19 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
         p.W = a->W - w < L.slice ? a->W - w : L.slice;
         p.pairs = p.W * p.nt;
         int rows = k.rows, ctas = L.ctas;
+        void* rargs[] = {&p, &qf, &ql};
+        cfg.gridDim = dim3((unsigned)((long long)a->F * p.pairs * a->Hkv));
+        cfg.blockDim = dim3(128);
+        cfg.dynamicSmemBytes = 0;
+        if (a->F > 0) e = cudaLaunchKernelExC(&cfg, k.rotate, rargs);
+        if (e != cudaSuccess) break;
         void* args[] = {&p, &mk, &mv};
         cfg.gridDim = dim3((unsigned)L.ctas);
         cfg.blockDim = dim3(kQ8Threads);
         cfg.dynamicSmemBytes = k.smem[gather];
+        cfg.numAttrs = a->F > 0 ? 1 : 0;  // it waits for nothing itself: the rotation has
         e = cudaLaunchKernelExC(&cfg, fn, args);
+        cfg.numAttrs = 1;
         if (e != cudaSuccess) break;
         void* margs[] = {&p, &rows, &ctas};
         const int rpb = 256 / (a->E / 4);
