@@ -63,18 +63,23 @@ struct Q8Params : TurnSplit {
 constexpr int kQ8Warps = 4, kQ8Threads = 256;
 constexpr int kQ8MaxPairs = 4096;  // their prefix sums lie in the stages at first
 
-// E: head dim, MT: 16-row tiles of a KV head's query rows, TERMS: f16 values per query element and weight.
-template <int E, int MT, int TERMS, bool GATHER> struct Q8Cfg {
+// T: the queries' type, E: head dim, MT: 16-row tiles of a KV head's query rows.
+template <class T, int E, int MT, bool GATHER> struct Q8Cfg {
     static constexpr int KPW = E == 256 ? 16 : 32;      // keys of a warp in a window
     static constexpr int KROWS = kQ8Warps * KPW;        // (key, head) rows of a stage
     static constexpr int TENSOR = KROWS * E;            // bytes of K (or V) in a stage
     static constexpr int NT = KPW / 8;                  // 8-key tiles
-    static constexpr int KS = E / 16;                   // 16-deep steps of q . k
     static constexpr int NJ = E / 8;                    // 8-column tiles of the output
     static constexpr int ROWS = 16 * MT;
+    // Queries as sums of e4m3 values next to K as it is (bf16: 2, f16: 3), or of f16 values next to K widened (f16 where
+    // three do not fit in the registers: 1, f32: 2).
+    static constexpr bool BF = Elem<T>::dtype == DVATTN_BFLOAT16;
+    static constexpr bool NARROW = BF || (Elem<T>::dtype == DVATTN_FLOAT16 && E * MT <= 128);
+    static constexpr int QT = NARROW ? (BF ? 2 : 3) : sizeof(T) == 4 ? 2 : 1, PT = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int KS = NARROW ? E / 32 : E / 16;  // steps of q . k
     // A head's query fragments: in registers once read, else read for every window, from one of two buffers.
-    static constexpr int QFRAG = KS * MT * TERMS * 512, QHEAD = QFRAG + ROWS * 4;  // ... and the rows' factors
-    static constexpr bool QREG = QFRAG <= 4096;
+    static constexpr int QFRAG = KS * MT * QT * 512, QHEAD = QFRAG + ROWS * 4;  // ... and the rows' factors
+    static constexpr bool QREG = QFRAG <= 6144;
     static constexpr int QBUFS = QREG ? 1 : 2, HEADS = QREG ? 4 : 2;  // buffers, KV heads of a CTA at most
     static constexpr int LIMS = (ROWS + 4) * 4;                       // what the rows of a tile see, and the least of it
     static constexpr int QBUF = HEADS * QHEAD + LIMS, QBYTES = QBUFS * QBUF;
@@ -259,6 +264,28 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two 16 x 16 matrices of bytes, rows at the lanes' addresses (0 .. 15 and 16 .. 31): v[0], v[1] get rows 4 (lane % 4) .. + 3 of
+// columns lane / 4 and 8 + lane / 4 of the first, v[2], v[3] of the second.
+__device__ __forceinline__ void ldsm_b8_t(uint32_t addr, uint32_t (&v)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+template <class T> __device__ __forceinline__ void store_pair(T* dst, float2 x) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(dst) = x;
+    else *reinterpret_cast<uint32_t*>(dst) = Elem<T>::pack2(x.x, x.y);
+}
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) { return Elem<__half>::pack2(a, b); }
 
 // v = 2^e m of a scale (file comment), e at least -60; what is not finite or not positive comes out in m.
@@ -280,8 +307,7 @@ __device__ const float kOne = 1.f;
 // its first windows.  By the attention kernel's own warps, a turn took 4 to 10 us, in rounds of loads that few
 // registers allow.
 template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_q8_kernel(const __grid_constant__ Q8Params p, uint8_t* qf, uint8_t* ql) {
-    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-    using C = Q8Cfg<E, MT, TERMS, false>;
+    using C = Q8Cfg<T, E, MT, false>;
     constexpr int ROWS = C::ROWS, KS = C::KS, LPR = E / 8, STEP = 128 / LPR;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -326,25 +352,52 @@ template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_
         for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(v[i][u]));
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int shift = min(140 - (__float_as_int(top) >> 23), 126);
+        // the row's largest element to 2^7 .. 2^8 (e4m3) or 2^13 .. 2^14 (f16)
+        const int shift = min((C::NARROW ? 134 : 140) - (__float_as_int(top) >> 23), 126);
         const float mul = __int_as_float((127 + shift) << 23);
         if (ch == 0) reinterpret_cast<float*>(head + C::QFRAG)[i16] = p.scale_log2 * __int_as_float((127 - shift) << 23);
-        // 16-byte chunk t + 4j of row n + 8 half of tile mt: step 4j + u, a[half] = its elements 4u, 4u + 1, a[2 + half] the next two
-        const int c16 = ch >> 1;
-        uint8_t* dst = head + ((i16 >> 4) * TERMS * KS + 4 * (c16 >> 2) + 2 * (ch & 1)) * 512 + ((i16 & 7) * 4 + (c16 & 3)) * 16 + (i16 >> 3 & 1) * 4;
+        // elements 8 y .. 8 y + 7 of 16-byte K chunk t + 4j, row n + 8 half of tile mt; lane (n, t)'s fragment
+        const int c16 = ch >> 1, y = ch & 1;
+        uint8_t* dst = head + (i16 >> 4) * C::QT * KS * 512 + ((i16 & 7) * 4 + (c16 & 3)) * 16 + (i16 >> 3 & 1) * 4;
+        float x[8];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float x[4];
+        for (int u = 0; u < 8; ++u) x[u] = v[i][u] * mul;
+        if constexpr (C::NARROW) {  // step 2j + y: a[half] = the first four elements, a[2 + half] the others
+            dst += (2 * (c16 >> 2) + y) * 512;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) x[y] = v[i][u * 4 + y] * mul;
+            for (int term = 0; term < C::QT; ++term) {
+                uint32_t word[4];
 #pragma unroll
-            for (int term = 0; term < TERMS; ++term) {
-                const uint32_t lo = pack_f16(x[0], x[1]), hi = pack_f16(x[2], x[3]);
-                *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512) = lo;
-                *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512 + 8) = hi;
-                const __half2 a = *reinterpret_cast<const __half2*>(&lo), b = *reinterpret_cast<const __half2*>(&hi);
-                x[0] -= __low2float(a), x[1] -= __high2float(a), x[2] -= __low2float(b), x[3] -= __high2float(b);
+                for (int u = 0; u < 4; ++u) {
+                    const float nan = __int_as_float(0x7fc00000);  // e4m3 has no infinities
+                    float e0 = x[2 * u], e1 = x[2 * u + 1];
+                    if (term == 0) {
+                        if (fabsf(e0) > 448.f) e0 = nan;
+                        if (fabsf(e1) > 448.f) e1 = nan;
+                    }
+                    word[u] = f32x2_to_e4m3x2(e0, e1);
+                    const uint32_t f = e4m3x2_to_f16x2(word[u]);
+                    const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
+                    // the second and third are 16 times theirs
+                    x[2 * u] = (e0 - __low2float(f2)) * (term == 0 ? 16.f : 1.f);
+                    x[2 * u + 1] = (e1 - __high2float(f2)) * (term == 0 ? 16.f : 1.f);
+                }
+                *reinterpret_cast<uint32_t*>(dst + term * KS * 512) = word[0] | word[1] << 16;
+                *reinterpret_cast<uint32_t*>(dst + term * KS * 512 + 8) = word[2] | word[3] << 16;
             }
+        } else {  // step 4j + 2y + u: a[half] = elements 4u, 4u + 1, a[2 + half] the next two
+            dst += (4 * (c16 >> 2) + 2 * y) * 512;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int term = 0; term < C::QT; ++term) {
+                    float* e = x + 4 * u;
+                    const uint32_t lo = pack_f16(e[0], e[1]), hi = pack_f16(e[2], e[3]);
+                    *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512) = lo;
+                    *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512 + 8) = hi;
+                    const __half2 a = *reinterpret_cast<const __half2*>(&lo), b = *reinterpret_cast<const __half2*>(&hi);
+                    e[0] -= __low2float(a), e[1] -= __high2float(a), e[2] -= __low2float(b), e[3] -= __high2float(b);
+                }
         }
     }
 }
@@ -354,19 +407,20 @@ template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_
 // [KPW (w / hc), + KPW) of the window; thread (n, t) = (lane / 4, lane % 4).
 //
 // Fragments.  The order of the elements in q . k and of the keys in P V is free as long as both operands
-// share it, so every fragment comes from whole 16-byte words of a stage:
-// * K: 8-key tile x, column n is key 8x + k(n), k(n) = n / 2 + 4 (n % 2); step 4i + u takes bytes 4u .. 4u + 3
-//   of 16-byte chunk t + 4i.  Neighbouring n lie 4 rows apart, which the 128-byte swizzle puts in different banks.
-// * the scores a thread then holds of a tile are those of keys 8x + t and 8x + t + 4: the rows whose V words it
-//   loads.  V: column n of output tile j of a 128-byte panel is element 16 c(n) + j, c(n) = k(n); the bytes of
-//   two rows are interleaved and widened in pairs.  A thread ends with 16 neighbouring elements twice.
-// * head dim 64: rows of 64 bytes; V words of 8 bytes, tile j of column n is element 8 c(n) + j with
-//   c(n) = n % 2 + 4 (n / 2 % 2) + 2 (n / 4).
+// share it:
+// * K comes in 16-byte words: thread (n, t) takes chunks t + 4i of the rows of its columns n.  Next to e4m3 queries, two
+//   32-bit words of a chunk are a fragment (16 x 8 x 32) as they are; next to f16 ones, each word is widened to one
+//   (16 x 8 x 16).
+// * V comes by transposing 8-bit matrix loads: thread (n, t) gets, of column n, the keys of rows 4t .. 4t + 3, and
+//   widens them in pairs to a fragment.  So the scores that a thread holds have to be those of these four keys: of 16 keys,
+//   key(t, j) = 8 (t / 2) + 2 (t % 2) + j / 2 + 4 (j % 2) for tile j / 2, column 2t + j % 2.  Neighbouring columns lie four rows
+//   apart and eight rows in a row differ, which the 128-byte swizzle puts in different banks, and a thread's
+//   four keys lie in 8 neighbouring rows: one page, one scale.
 template <class T, int E, int MT, bool GATHER>
-__global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1, GATHER>::CTAS))
+__global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
     decode_q8_kernel(const __grid_constant__ Q8Params p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
-    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-    using C = Q8Cfg<E, MT, TERMS, GATHER>;
+    using C = Q8Cfg<T, E, MT, GATHER>;
+    constexpr int QT = C::QT, PT = C::PT;
     constexpr int KPW = C::KPW, NT = C::NT, KS = C::KS, NJ = C::NJ, STAGES = C::STAGES, ROWS = C::ROWS;
     constexpr int RB = E < 128 ? E : 128;  // bytes of a swizzled row
     constexpr int NP = E / RB;             // panels
@@ -590,36 +644,40 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
     const int n = lane >> 2, t = lane & 3;
     const int hh = wid % p.hc, grp = wid / p.hc, wph = kQ8Warps / p.hc;  // head of the group, warps per head
     const int kw = grp * KPW;                                            // first key of the window
-    const int kn = (n >> 1) | ((n & 1) << 2);
-    // 8-key tile x: its rows' place in a stage's K (V), a panel further: + panel
-    uint32_t tile[NT];
-#pragma unroll
-    for (int x = 0; x < NT; ++x) {
+    // 8 neighbouring keys x: their rows' place in a stage's K (V), a panel further: + panel
+    auto rows8 = [&](int x) {
         const int key = kw + 8 * x, b = key >> p.box_shift;
-        tile[x] = (uint32_t)(((b * p.hc + hh) * NP * p.box + (key & (p.box - 1))) * RB);
-    }
+        return (uint32_t)(((b * p.hc + hh) * NP * p.box + (key & (p.box - 1))) * RB);
+    };
+    auto swizzle = [](int row) { return (uint32_t)(RB == 128 ? row & 7 : row >> 1 & 3); };  // of a row's 16-byte chunks
     const uint32_t panel = (uint32_t)(p.box * RB);
-    uint32_t kofs[E < 128 ? 1 : 2], vofs[2];  // a thread's chunks in a tile
-    if constexpr (E >= 128) {
-        kofs[0] = (uint32_t)(kn * 128 + ((t ^ kn) << 4));
-        kofs[1] = (uint32_t)(kn * 128 + (((t + 4) ^ kn) << 4));
-        vofs[0] = (uint32_t)(t * 128 + ((kn ^ t) << 4));
-        vofs[1] = (uint32_t)((t + 4) * 128 + ((kn ^ (t + 4)) << 4));
-    } else {
-        const int cn = (n & 1) | ((n & 2) << 1) | ((n & 4) >> 1);
-        kofs[0] = (uint32_t)(kn * 64 + ((t ^ (kn >> 1 & 3)) << 4));
-        vofs[0] = (uint32_t)(t * 64 + (((cn >> 1) ^ (t >> 1)) << 4) + ((cn & 1) << 3));
-        vofs[1] = (uint32_t)((t + 4) * 64 + (((cn >> 1) ^ ((t + 4) >> 1 & 3)) << 4) + ((cn & 1) << 3));
+    constexpr int NG = NT / 2;  // 16-key groups
+    uint32_t kbase[NG], kofs[2][E < 128 ? 1 : 2];  // K rows of column n: its group's, by tile and chunk t or t + 4
+#pragma unroll
+    for (int g = 0; g < NG; ++g) kbase[g] = rows8(2 * g + (n >> 2));
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int row = (n >> 1 & 1) * 2 + x + 4 * (n & 1);
+#pragma unroll
+        for (int y = 0; y < (E < 128 ? 1 : 2); ++y) kofs[x][y] = (uint32_t)(row * RB) + (((t + 4 * y) ^ swizzle(row)) << 4);
     }
+    // V rows of a matrix load: lanes 0 .. 15 the first 16 keys, 16 .. 31 the next (head dim 256: the next 16 columns)
+    uint32_t vrow;
+    {
+        const int t4 = lane >> 2 & 3, j = lane & 3, key = (t4 >> 1) * 8 + (t4 & 1) * 2 + (j >> 1) + 4 * (j & 1), half = lane >> 4;
+        vrow = rows8((NG == 2 ? 2 * half : 0) + (key >> 3)) + (uint32_t)((key & 7) * RB) + ((swizzle(key & 7) ^ (uint32_t)(NG == 2 ? 0 : half)) << 4);
+    }
+    const int mykey = (t >> 1) * 8 + (t & 1) * 2;  // key(t, 0)
     uint32_t sQ = 0;  // this lane's fragments of the turn's buffer
     int nq = 0;       // turns so far
     float* sML = reinterpret_cast<float*>(smem + C::OFF_ML);
 
-    uint32_t qf[C::QREG ? MT * TERMS * KS : 1][4];
+    uint32_t qf[C::QREG ? MT * QT * KS : 1][4];
     float fr[MT][2];   // log2(e) * scale / (the row's power of two)
     int lim[MT][2];    // keys of the turn that the row sees
     int least = 0;     // that every row of the warp sees
-    float o[MT][NJ][4], r[MT][2], l[MT][2];
+    float o[MT][NJ][4], r[MT][2];
+    uint64_t l[MT][2];  // two sums each
 
     // The next turn's fragments and row values; false: a wait gave up.
     auto take_q = [&] {
@@ -630,7 +688,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
         sQ = head + lane * 16;
         if constexpr (C::QREG) {
 #pragma unroll
-            for (int x = 0; x < MT * TERMS * KS; ++x) {
+            for (int x = 0; x < MT * QT * KS; ++x) {
                 const uint4 v = lds128(sQ + x * 512);
                 qf[x][0] = v.x, qf[x][1] = v.y, qf[x][2] = v.z, qf[x][3] = v.w;
             }
@@ -653,25 +711,35 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
     // One window's keys [first, first + KPW) of this warp.  EDGE: some row does not see them all.
     auto window = [&](auto edge, const Q8Stage& d, int first, uint32_t kb, uint32_t sc) {
         constexpr bool EDGE = decltype(edge)::value;
-        constexpr int NS = GATHER ? 2 : 1;  // scales of an 8-key tile that a thread needs: its keys' own, or the one page's
         const uint32_t vb = kb + C::TENSOR;
+        auto key_of = [&](int x, int y) { return 16 * (x >> 1) + mykey + (x & 1) + 4 * y; };  // of tile x, this thread's column y
+        auto sees = [&](int x, int y, int mt, int half) {
+            const int key = first + key_of(x, y);
+            return key >= 0 && key < lim[mt][half];
+        };
         // ---- scores ----
         float z[MT][NT][4];
+        [[maybe_unused]] float z2[C::NARROW ? MT : 1][C::NARROW ? NT : 1][4];  // a score is z + z2 / 16
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int x = 0; x < NT; ++x) z[mt][x][0] = z[mt][x][1] = z[mt][x][2] = z[mt][x][3] = 0.f;
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    z[mt][x][y] = 0.f;
+                    if constexpr (C::NARROW) z2[mt][x][y] = 0.f;
+                }
 #pragma unroll
         for (int ci = 0; ci < E / 64; ++ci) {
             uint4 kf[NT];
 #pragma unroll
-            for (int x = 0; x < NT; ++x) kf[x] = lds128(kb + tile[x] + (ci >> 1) * panel + kofs[E < 128 ? 0 : ci & 1]);
+            for (int x = 0; x < NT; ++x) kf[x] = lds128(kb + kbase[x >> 1] + (ci >> 1) * panel + kofs[x & 1][E < 128 ? 0 : ci & 1]);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int ks = 4 * ci + u;
-                uint32_t a[MT * TERMS][4];
+            for (int u = 0; u < (C::NARROW ? 2 : 4); ++u) {
+                const int ks = (C::NARROW ? 2 : 4) * ci + u;
+                uint32_t a[MT * QT][4];
 #pragma unroll
-                for (int y = 0; y < MT * TERMS; ++y) {
+                for (int y = 0; y < MT * QT; ++y) {
                     if constexpr (C::QREG) {
 #pragma unroll
                         for (int v = 0; v < 4; ++v) a[y][v] = qf[y * KS + ks][v];
@@ -682,53 +750,75 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
                 }
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
-                    const uint32_t word = u == 0 ? kf[x].x : u == 1 ? kf[x].y : u == 2 ? kf[x].z : kf[x].w;
-                    const uint32_t b0 = e4m3x2_to_f16x2(word), b1 = e4m3x2_hi_to_f16x2(word);
+                    if constexpr (C::NARROW) {
+                        const uint32_t b0 = u == 0 ? kf[x].x : kf[x].z, b1 = u == 0 ? kf[x].y : kf[x].w;
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                        for (int mt = 0; mt < MT; ++mt) {
+                            mma_e4m3(z[mt][x], a[mt * QT], b0, b1);
 #pragma unroll
-                        for (int term = TERMS - 1; term >= 0; --term) mma_f16(z[mt][x], a[mt * TERMS + term], b0, b1);
+                            for (int term = 1; term < QT; ++term) mma_e4m3(z2[mt][x], a[mt * QT + term], b0, b1);
+                        }
+                    } else {
+                        const uint32_t word = u == 0 ? kf[x].x : u == 1 ? kf[x].y : u == 2 ? kf[x].z : kf[x].w;
+                        const uint32_t b0 = e4m3x2_to_f16x2(word), b1 = e4m3x2_hi_to_f16x2(word);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int term = QT - 1; term >= 0; --term) mma_f16(z[mt][x], a[mt * QT + term], b0, b1);
+                    }
                 }
             }
         }
         // ---- weights ----
-        float vscale[NT][NS];
+        // scales of a 16-key group: the one page's of this thread's keys, or each key's own
+        constexpr int NS = GATHER ? 4 : 1;
+        float vscale[NG][NS];
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const int at = GATHER ? (kw + 8 * x + t + 4 * y) * p.hc + hh : (kw / 8 + x) * p.hc + hh;
-                float ks, e;
-                if (GATHER || y == 0) {
-                    ks = lds_f32(sc + 4 * at);
-                    vscale[x][GATHER ? y : 0] = lds_f32(sc + 4 * (at + C::SCALES));
-                    e = Scale(vscale[x][GATHER ? y : 0]).e;
+            for (int k = 0; k < NS; ++k) {  // key(t, k): tile 2g + k / 2, column k % 2
+                const int at = (GATHER ? kw + key_of(2 * g + (k >> 1), k & 1) : (kw >> 3) + 2 * g + (t >> 1)) * p.hc + hh;
+                const float ks = lds_f32(sc + 4 * at);
+                vscale[g][k] = lds_f32(sc + 4 * (at + C::SCALES));
+                const float e = Scale(vscale[g][k]).e;
 #pragma unroll
-                    for (int y2 = y; y2 < (GATHER ? y + 1 : 2); ++y2)
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            z[mt][x][y2] = fmaf(z[mt][x][y2], ks * fr[mt][0], e);
-                            z[mt][x][2 + y2] = fmaf(z[mt][x][2 + y2], ks * fr[mt][1], e);
+                    for (int half = 0; half < 2; ++half) {
+                        const float f = ks * fr[mt][half];
+                        if constexpr (GATHER) {
+                            float& x = z[mt][2 * g + (k >> 1)][2 * half + (k & 1)];
+                            if constexpr (C::NARROW) x = fmaf(z2[mt][2 * g + (k >> 1)][2 * half + (k & 1)], 0.0625f, x);
+                            x = fmaf(x, f, e);
+                        } else {
+#pragma unroll
+                            for (int x = 2 * g; x < 2 * g + 2; ++x) {
+                                float* y = z[mt][x] + 2 * half;
+                                uint64_t v = f2u(y[0], y[1]);
+                                if constexpr (C::NARROW) v = ffma2(f2u(z2[mt][x][2 * half], z2[mt][x][2 * half + 1]), f2u(0.0625f, 0.0625f), v);
+                                u2f(ffma2(v, f2u(f, f), f2u(e, e)), y[0], y[1]);
+                            }
                         }
-                }
-                if constexpr (EDGE) {
-                    const int key_l = first + 8 * x + t + 4 * y;
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        if (key_l < 0 || key_l >= lim[mt][0]) z[mt][x][y] = neg_inf();
-                        if (key_l < 0 || key_l >= lim[mt][1]) z[mt][x][2 + y] = neg_inf();
                     }
-                }
             }
+        if constexpr (EDGE) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int x = 0; x < NT; ++x)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        if (!sees(x, y & 1, mt, y >> 1)) z[mt][x][y] = neg_inf();
+        }
         bool moves = false;
         float top[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                float m = neg_inf();
+                float m = fmaxf(z[mt][0][2 * y], z[mt][0][2 * y + 1]);
 #pragma unroll
-                for (int x = 0; x < NT; ++x) m = fmaxf(m, fmaxf(z[mt][x][2 * y], z[mt][x][2 * y + 1]));
+                for (int x = 1; x < NT; ++x) m = fmax3(m, z[mt][x][2 * y], z[mt][x][2 * y + 1]);
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 top[mt][y] = m;
@@ -742,154 +832,119 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
                     const bool up = top[mt][y] > r[mt][y] + 6.f;
                     const float alpha = up ? fast_exp2(r[mt][y] - top[mt][y]) : 1.f;
                     if (up) r[mt][y] = top[mt][y];
-                    l[mt][y] *= alpha;
+                    l[mt][y] = fmul2(l[mt][y], f2u(alpha, alpha));
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) o[mt][j][2 * y] *= alpha, o[mt][j][2 * y + 1] *= alpha;
                 }
         }
-        uint32_t pa[MT][TERMS][NT / 2][4];
-        uint32_t unseen = 0;  // columns (x, y) that nobody sees
+        uint32_t pa[MT][PT][NG][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const float ref0 = r[mt][0] == neg_inf() ? 0.f : r[mt][0] - 7.f, ref1 = r[mt][1] == neg_inf() ? 0.f : r[mt][1] - 7.f;
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                float w0[2], w1[2];
+            for (int half = 0; half < 2; ++half) {
+                const float ref = r[mt][half] == neg_inf() ? 0.f : r[mt][half] - 7.f;
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const Scale s(vscale[x][GATHER ? y : 0]);
-                    const float a = fast_exp2(z[mt][x][y] - ref0), b = fast_exp2(z[mt][x][2 + y] - ref1);
+                for (int x = 0; x < NT; ++x) {
+                    float w[2];
+                    u2f(fadd2(f2u(z[mt][x][2 * half], z[mt][x][2 * half + 1]), f2u(-ref, -ref)), w[0], w[1]);
+                    w[0] = fast_exp2(w[0]), w[1] = fast_exp2(w[1]);
+                    const Scale s0(vscale[x >> 1][GATHER ? 2 * (x & 1) : 0]), s1(vscale[x >> 1][GATHER ? 2 * (x & 1) + 1 : 0]);
                     if constexpr (EDGE) {  // what a masked key's scales are does not matter
-                        const int key_l = first + 8 * x + t + 4 * y;
-                        const bool s0_ = key_l >= 0 && key_l < lim[mt][0], s1_ = key_l >= 0 && key_l < lim[mt][1];
-                        w0[y] = s0_ ? a * s.m : 0.f;
-                        w1[y] = s1_ ? b * s.m : 0.f;
-                        if (s0_) l[mt][0] = fmaf(a, s.inv, l[mt][0]);
-                        if (s1_) l[mt][1] = fmaf(b, s.inv, l[mt][1]);
-                        if (key_l < 0 || key_l >= d.sp) unseen |= 1u << (2 * x + y);
+                        float a, b;
+                        u2f(l[mt][half], a, b);
+                        const bool see0 = sees(x, 0, mt, half), see1 = sees(x, 1, mt, half);
+                        if (see0) a = fmaf(w[0], s0.inv, a);
+                        if (see1) b = fmaf(w[1], s1.inv, b);
+                        l[mt][half] = f2u(a, b);
+                        w[0] = see0 ? w[0] * s0.m : 0.f;
+                        w[1] = see1 ? w[1] * s1.m : 0.f;
                     } else {
-                        w0[y] = a * s.m;
-                        w1[y] = b * s.m;
-                        l[mt][0] = fmaf(a, s.inv, l[mt][0]);
-                        l[mt][1] = fmaf(b, s.inv, l[mt][1]);
+                        l[mt][half] = ffma2(f2u(w[0], w[1]), f2u(s0.inv, s1.inv), l[mt][half]);
+                        u2f(fmul2(f2u(w[0], w[1]), f2u(s0.m, s1.m)), w[0], w[1]);
+                    }
+#pragma unroll
+                    for (int term = 0; term < PT; ++term) {
+                        const uint32_t a = pack_f16(w[0], w[1]);
+                        pa[mt][term][x >> 1][(x & 1) * 2 + half] = a;
+                        if constexpr (PT > 1) {
+                            const __half2 h2 = *reinterpret_cast<const __half2*>(&a);
+                            w[0] -= __low2float(h2), w[1] -= __high2float(h2);
+                        }
                     }
                 }
+            }
+        // ---- P V, a matrix load (2 or 4 output tiles) at a time ----
+        uint32_t keep[NG];  // the bytes of this thread's keys that anybody sees
+        if constexpr (EDGE) {
 #pragma unroll
-                for (int term = 0; term < TERMS; ++term) {
-                    const uint32_t a = pack_f16(w0[0], w0[1]), b = pack_f16(w1[0], w1[1]);
-                    pa[mt][term][x >> 1][(x & 1) * 2] = a;
-                    pa[mt][term][x >> 1][(x & 1) * 2 + 1] = b;
-                    if (TERMS > 1) {
-                        const __half2 ah = *reinterpret_cast<const __half2*>(&a), bh = *reinterpret_cast<const __half2*>(&b);
-                        w0[0] -= __low2float(ah), w0[1] -= __high2float(ah), w1[0] -= __low2float(bh), w1[1] -= __high2float(bh);
-                    }
+            for (int g = 0; g < NG; ++g) {
+                keep[g] = 0u;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int key = first + key_of(2 * g + (k >> 1), k & 1);
+                    if (key >= 0 && key < d.sp) keep[g] |= 0xffu << (8 * k);
                 }
             }
         }
-        // ---- P V: a word of 4 elements of each of a thread's rows at a time ----
-        constexpr int VW = E < 128 ? 2 : 4;  // words a thread loads of a row of a panel
+        constexpr int TJ = NG == 2 ? 2 : 4;  // output tiles of a load
 #pragma unroll
-        for (int pn = 0; pn < NP; ++pn) {
-            uint32_t vw[NT][2][VW];
-#pragma unroll
-            for (int x = 0; x < NT; ++x)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const uint32_t at = vb + tile[x] + pn * panel + vofs[y];
-                    if constexpr (E < 128) {
-                        const uint2 v = lds64(at);
-                        vw[x][y][0] = v.x, vw[x][y][1] = v.y;
-                    } else {
-                        const uint4 v = lds128(at);
-                        vw[x][y][0] = v.x, vw[x][y][1] = v.y, vw[x][y][2] = v.z, vw[x][y][3] = v.w;
-                    }
-                }
+        for (int j0 = 0; j0 < NJ; j0 += TJ) {
+            const int cb = j0 >> 1;  // 16-column block
+            uint32_t v[4];           // NG == 2: group g, tile j: v[2g + j]; else tile j: v[j]
+            ldsm_b8_t(((vb + (cb >> 3) * panel) + vrow) ^ (uint32_t)((cb & 7) << 4), v);
             if constexpr (EDGE) {
-                // keys that nobody sees: zeros.  A NaN in the value of a key that some rows see and others do not
-                // (0 * NaN is NaN) becomes a zero here and is added to the rows that see it.
+                // keys that nobody sees: zeros.  A NaN in the value of a key that some rows see and others do not (0 * NaN
+                // is NaN) becomes a zero here and is added to the rows that see it.
                 bool odd = false;
 #pragma unroll
-                for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int y = 0; y < 2; ++y)
-#pragma unroll
-                        for (int u = 0; u < VW; ++u) {
-                            if (unseen >> (2 * x + y) & 1u) vw[x][y][u] = 0u;
-                            odd |= e4m3_nan(vw[x][y][u]) != 0;
-                        }
+                for (int i = 0; i < 4; ++i) {
+                    v[i] &= keep[NG == 2 ? i >> 1 : 0];
+                    odd |= e4m3_nan(v[i]) != 0;
+                }
                 if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll 1
+#pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        uint32_t ind[NT / 2][4];  // 1 where the row sees the key
+                        uint32_t ind[NG][4];  // 1 where the row sees the key
 #pragma unroll
                         for (int x = 0; x < NT; ++x)
 #pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                const int key_l = first + 8 * x + t;
-                                const int lm = mt == 0 ? lim[0][y] : lim[MT - 1][y];
-                                ind[x >> 1][(x & 1) * 2 + y] = (key_l >= 0 && key_l < lm ? 0x3c00u : 0u) | (key_l + 4 >= 0 && key_l + 4 < lm ? 0x3c000000u : 0u);
-                            }
+                            for (int half = 0; half < 2; ++half)
+                                ind[x >> 1][(x & 1) * 2 + half] = (sees(x, 0, mt, half) ? 0x3c00u : 0u) | (sees(x, 1, mt, half) ? 0x3c000000u : 0u);
 #pragma unroll
-                        for (int j = 0; j < 4 * VW; ++j) {
+                        for (int j = 0; j < TJ; ++j) {
                             float cnt[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                            for (int g = 0; g < NT / 2; ++g) {
-                                uint32_t b[2];
-#pragma unroll
-                                for (int y = 0; y < 2; ++y) {
-                                    const uint32_t fa = e4m3_nan(vw[2 * g + y][0][j >> 2]) >> (8 * (j & 3)), fb = e4m3_nan(vw[2 * g + y][1][j >> 2]) >> (8 * (j & 3));
-                                    b[y] = (fa & 0x80u ? 0x3c00u : 0u) | (fb & 0x80u ? 0x3c000000u : 0u);
-                                }
-                                mma_f16(cnt, ind[g], b[0], b[1]);
+                            for (int g = 0; g < NG; ++g) {
+                                const uint32_t nan = e4m3_nan(v[NG == 2 ? 2 * g + j : j]);
+                                mma_f16(cnt, ind[g], (nan & 0x80u ? 0x3c00u : 0u) | (nan & 0x8000u ? 0x3c000000u : 0u),
+                                        (nan & 0x800000u ? 0x3c00u : 0u) | (nan & 0x80000000u ? 0x3c000000u : 0u));
                             }
 #pragma unroll
                             for (int y = 0; y < 4; ++y)
-                                if (cnt[y] > 0.f) {
-                                    const float nan = __int_as_float(0x7fc00000);
-                                    if (mt == 0) o[0][pn * 4 * VW + j][y] = nan;
-                                    else o[MT - 1][pn * 4 * VW + j][y] = nan;
-                                }
+                                if (cnt[y] > 0.f) o[mt][j0 + j][y] = __int_as_float(0x7fc00000);
                         }
                     }
 #pragma unroll
-                    for (int x = 0; x < NT; ++x)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y)
-#pragma unroll
-                            for (int u = 0; u < VW; ++u) vw[x][y][u] = clear_bytes(vw[x][y][u], e4m3_nan(vw[x][y][u]));
+                    for (int i = 0; i < 4; ++i) v[i] = clear_bytes(v[i], e4m3_nan(v[i]));
                 }
             }
 #pragma unroll
-            for (int u = 0; u < VW; ++u) {
-                [[maybe_unused]] float part[TERMS > 1 ? 4 : 1][4];  // f32: a window's sum by itself, added with one rounding
-                if constexpr (TERMS > 1) {
+            for (int j = 0; j < TJ; ++j) {
+                [[maybe_unused]] float part[4] = {0.f, 0.f, 0.f, 0.f};  // f32: a window's sum by itself, added with one rounding
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.f;
-                }
+                for (int g = 0; g < NG; ++g) {
+                    const uint32_t word = v[NG == 2 ? 2 * g + j : j], b0 = e4m3x2_to_f16x2(word), b1 = e4m3x2_hi_to_f16x2(word);
+                    if constexpr (PT > 1) {
 #pragma unroll
-                for (int g = 0; g < NT / 2; ++g) {
-                    // bytes of two rows side by side: (0, 1) and (2, 3) of each
-                    const uint32_t a0 = __byte_perm(vw[2 * g][0][u], vw[2 * g][1][u], 0x5140), a1 = __byte_perm(vw[2 * g][0][u], vw[2 * g][1][u], 0x7362);
-                    const uint32_t c0 = __byte_perm(vw[2 * g + 1][0][u], vw[2 * g + 1][1][u], 0x5140),
-                                   c1 = __byte_perm(vw[2 * g + 1][0][u], vw[2 * g + 1][1][u], 0x7362);
+                        for (int term = PT - 1; term >= 0; --term) mma_f16(part, pa[0][term][g], b0, b1);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t b0 = j == 0 ? e4m3x2_to_f16x2(a0) : j == 1 ? e4m3x2_hi_to_f16x2(a0) : j == 2 ? e4m3x2_to_f16x2(a1) : e4m3x2_hi_to_f16x2(a1);
-                        const uint32_t b1 = j == 0 ? e4m3x2_to_f16x2(c0) : j == 1 ? e4m3x2_hi_to_f16x2(c0) : j == 2 ? e4m3x2_to_f16x2(c1) : e4m3x2_hi_to_f16x2(c1);
-                        if constexpr (TERMS > 1) {
-#pragma unroll
-                            for (int term = TERMS - 1; term >= 0; --term) mma_f16(part[j], pa[0][term][g], b0, b1);
-                        } else {
-#pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][pn * 4 * VW + 4 * u + j], pa[mt][0][g], b0, b1);
-                        }
+                        for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][j0 + j], pa[mt][0][g], b0, b1);
                     }
                 }
-                if constexpr (TERMS > 1) {
+                if constexpr (PT > 1) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) o[0][pn * 4 * VW + 4 * u + j][y] += part[j][y];
+                    for (int y = 0; y < 4; ++y) o[0][j0 + j][y] += part[y];
                 }
             }
         }
@@ -912,7 +967,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 r[mt][0] = r[mt][1] = neg_inf();
-                l[mt][0] = l[mt][1] = 0.f;
+                l[mt][0] = l[mt][1] = f2u(0.f, 0.f);
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
             }
@@ -949,7 +1004,9 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                float sum = l[mt][y];
+                float sum, other;
+                u2f(l[mt][y], sum, other);
+                sum += other;
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                 f[mt][y] = sum;
@@ -993,24 +1050,16 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
                     if (row >= p.rows) continue;
                     const size_t orow = whole ? out_row(hh, row) : (slot + hh) * ROWS + i16;
 #pragma unroll
-                    for (int pn = 0; pn < NP; ++pn)
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {  // 16 (8) neighbouring elements
-                            const int e = E < 128 ? ((t & 1) << 5) + ((t & 2) << 3) + 8 * b : pn * 128 + 16 * t + 64 * b;
-                            constexpr int W16 = E < 128 ? 8 : 16;
-#pragma unroll
-                            for (int j = 0; j < W16; j += 4) {
-                                float x[4];
-#pragma unroll
-                                for (int v = 0; v < 4; ++v) x[v] = o[mt][pn * W16 + j + v][2 * y + b] * f[mt][y];
-                                if (whole) {
-                                    store_quad<T>(static_cast<T*>(p.out) + orow * E + e + j, x[0], x[1], x[2], x[3]);
-                                    if (p.out_f32) *reinterpret_cast<float4*>(p.out_f32 + orow * E + e + j) = make_float4(x[0], x[1], x[2], x[3]);
-                                } else {
-                                    *reinterpret_cast<float4*>(p.part_o + orow * E + e + j) = make_float4(x[0], x[1], x[2], x[3]);
-                                }
-                            }
+                    for (int j = 0; j < NJ; ++j) {
+                        const float2 x = make_float2(o[mt][j][2 * y] * f[mt][y], o[mt][j][2 * y + 1] * f[mt][y]);
+                        const size_t at = orow * E + 8 * j + 2 * t;
+                        if (whole) {
+                            store_pair<T>(static_cast<T*>(p.out) + at, x);
+                            if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + at) = x;
+                        } else {
+                            *reinterpret_cast<float2*>(p.part_o + at) = x;
                         }
+                    }
                     if (t == 0) {
                         if (!whole) p.part_lse[orow] = lse2[mt][y];
                         else if (p.lse_out) p.lse_out[orow] = lse2[mt][y] * kLn2;
@@ -1029,22 +1078,13 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<E, MT, sizeof(T) == 4 ? 2 :
                     for (int y = 0; y < 2; ++y) {
                         float* dst = sO + ((size_t)hh * ROWS + mt * 16 + y * 8 + n) * E;
 #pragma unroll
-                        for (int pn = 0; pn < NP; ++pn)
-#pragma unroll
-                            for (int b = 0; b < 2; ++b) {
-                                const int e = E < 128 ? ((t & 1) << 5) + ((t & 2) << 3) + 8 * b : pn * 128 + 16 * t + 64 * b;
-                                constexpr int W16 = E < 128 ? 8 : 16;
-#pragma unroll
-                                for (int j = 0; j < W16; j += 4) {
-                                    float4* at = reinterpret_cast<float4*>(dst + e + j);
-                                    float4 x = g ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
-                                    x.x += o[mt][pn * W16 + j][2 * y + b] * f[mt][y];
-                                    x.y += o[mt][pn * W16 + j + 1][2 * y + b] * f[mt][y];
-                                    x.z += o[mt][pn * W16 + j + 2][2 * y + b] * f[mt][y];
-                                    x.w += o[mt][pn * W16 + j + 3][2 * y + b] * f[mt][y];
-                                    *at = x;
-                                }
-                            }
+                        for (int j = 0; j < NJ; ++j) {
+                            float2* at = reinterpret_cast<float2*>(dst + 8 * j + 2 * t);
+                            float2 x = g ? *at : make_float2(0.f, 0.f);
+                            x.x += o[mt][j][2 * y] * f[mt][y];
+                            x.y += o[mt][j][2 * y + 1] * f[mt][y];
+                            *at = x;
+                        }
                         if (g == 0 && t == 0) sML[(wid * ROWS + mt * 16 + y * 8 + n) * 2] = lse2[mt][y];  // wid = hh
                     }
             }
@@ -1154,8 +1194,8 @@ struct Q8Kernel {
     size_t smem[2];
 };
 template <class T, int E, int MT> Q8Kernel q8_kernel() {
-    using C = Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1, false>;
-    using G = Q8Cfg<E, MT, sizeof(T) == 4 ? 2 : 1, true>;
+    using C = Q8Cfg<T, E, MT, false>;
+    using G = Q8Cfg<T, E, MT, true>;
     static_assert(C::KROWS == G::KROWS && C::CTAS == G::CTAS && C::HEADS == G::HEADS, "one layout");
     return {{(const void*)&decode_q8_kernel<T, E, MT, false>, (const void*)&decode_q8_kernel<T, E, MT, true>}, (const void*)&rotate_q8_kernel<T, E, MT>,
             (const void*)&merge_q8_kernel<T, E>, C::QHEAD, C::LIMS, C::KROWS, C::ROWS, C::CTAS, C::HEADS, {C::SMEM, G::SMEM}};
