@@ -38,6 +38,7 @@ struct Q8Params : TurnSplit {
     int hc, hs;             // KV heads a CTA reads together, groups of them (hc * hs = Hkv)
     int pairs;              // W * nt (sequence, row tile) pairs
     int box, box_shift;     // rows of a TMA box (gathered: rows of the stage), its log2
+    int bs_shift;           // log2 of the page size, -1: it is no power of two
     long long tokens;       // all sequences' (a turn's stride in loc and cos / sin)
     int stall_tile;         // test hook (DVATTN_TEST_STALL_TILE), -1: off
     float scale_log2;
@@ -60,26 +61,22 @@ struct Q8Params : TurnSplit {
     float* part_lse;        // [CTAs][2][hc][rows of a tile] log2 sums, -inf: nothing seen
 };
 
-constexpr int kQ8Warps = 4, kQ8Threads = 256;
+constexpr int kQ8Warps = 4, kQ8Threads = 256, kQ8Ahead8 = 4;
 constexpr int kQ8MaxPairs = 4096;  // their prefix sums lie in the stages at first
 
 // T: the queries' type, E: head dim, MT: 16-row tiles of a KV head's query rows.
 template <class T, int E, int MT, bool GATHER> struct Q8Cfg {
-    static constexpr int KPW = E == 256 ? 16 : 32;      // keys of a warp in a window
+    static constexpr int KPW = E * MT >= 256 ? 16 : 32;    // keys of a warp in a window
     static constexpr int KROWS = kQ8Warps * KPW;        // (key, head) rows of a stage
     static constexpr int TENSOR = KROWS * E;            // bytes of K (or V) in a stage
     static constexpr int NT = KPW / 8;                  // 8-key tiles
     static constexpr int NJ = E / 8;                    // 8-column tiles of the output
     static constexpr int ROWS = 16 * MT;
-    // Queries as sums of e4m3 values next to K as it is (bf16: 2, f16: 3), or of f16 values next to K widened (f16 where
-    // three do not fit in the registers: 1, f32: 2).
-    static constexpr bool BF = Elem<T>::dtype == DVATTN_BFLOAT16;
-    static constexpr bool NARROW = BF || (Elem<T>::dtype == DVATTN_FLOAT16 && E * MT <= 128);
-    static constexpr int QT = NARROW ? (BF ? 2 : 3) : sizeof(T) == 4 ? 2 : 1, PT = sizeof(T) == 4 ? 2 : 1;
-    static constexpr int KS = NARROW ? E / 32 : E / 16;  // steps of q . k
+    static constexpr int QT = sizeof(T) == 4 ? 2 : 1, PT = QT;  // f16 values of a query element, of a weight
+    static constexpr int KS = E / 16;                           // steps of q . k
     // A head's query fragments: in registers once read, else read for every window, from one of two buffers.
     static constexpr int QFRAG = KS * MT * QT * 512, QHEAD = QFRAG + ROWS * 4;  // ... and the rows' factors
-    static constexpr bool QREG = QFRAG <= 6144;
+    static constexpr bool QREG = QFRAG <= 4096;
     static constexpr int QBUFS = QREG ? 1 : 2, HEADS = QREG ? 4 : 2;  // buffers, KV heads of a CTA at most
     static constexpr int LIMS = (ROWS + 4) * 4;                       // what the rows of a tile see, and the least of it
     static constexpr int QBUF = HEADS * QHEAD + LIMS, QBYTES = QBUFS * QBUF;
@@ -93,19 +90,19 @@ template <class T, int E, int MT, bool GATHER> struct Q8Cfg {
     // query buffer's second half is free)
     static constexpr int ML = QREG ? 0 : kQ8Warps * ROWS * 8;
     static_assert(!QREG || 2 * QHEAD >= kQ8Warps * ROWS * 8, "maxima and sums");
-    static constexpr int STAGE = 2 * TENSOR + 2 * SCALES * 4 + 32 + 16;  // tiles, scales, description, barriers
+    static constexpr int STAGE = 2 * TENSOR + 2 * SCALES * 4 + 64 + 16;  // tiles, scales, two descriptions (the next window's is written early), barriers
     static constexpr int FIT = (LIMIT - QBYTES - ML - 16 * QBUFS - 4) / STAGE;
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr size_t OFF_Q = (size_t)STAGES * 2 * TENSOR;
     static constexpr size_t OFF_ML = QREG ? OFF_Q + 2 * QHEAD + LIMS : OFF_Q + QBYTES;
     static constexpr size_t OFF_SC = OFF_Q + QBYTES + ML;               // [STAGES][2][SCALES]
     static constexpr size_t OFF_DESC = OFF_SC + STAGES * 2 * SCALES * 4;
-    static constexpr size_t OFF_BAR = OFF_DESC + STAGES * 32;           // full, empty, then q's
+    static constexpr size_t OFF_BAR = OFF_DESC + STAGES * 64;           // full, empty, then q's
     static constexpr size_t OFF_FLAG = OFF_BAR + STAGES * 16 + QBUFS * 16;
     static constexpr size_t SMEM = OFF_FLAG + 4;
     static_assert(STAGES >= 2 && OFF_Q >= (kQ8MaxPairs + 40) * 8, "the prefix sums fit in the stages");
     static_assert(SMEM <= LIMIT && OFF_BAR % 16 == 0, "shared memory");
-    static_assert(2 * TENSOR >= 2 * ROWS * E * 4, "two heads' rows are combined in a stage");
+    static_assert(2 * TENSOR >= 2 * 16 * E * 4, "two heads' rows are combined in a stage");
 };
 
 // ---- the windows of a (sequence, row tile) pair ------------------------------------------
@@ -173,14 +170,15 @@ constexpr int Q8_ITEM = 1, Q8_TURN = 2, Q8_LAST = 4, Q8_WHOLE = 8, Q8_BEGIN = 16
 // Walks units [u, u1) by a whole warp; every lane holds the same values.
 struct Q8Walk {
     long long rem;
-    int pair, hg, f, wi, left;  // wi: window of the turn, left: windows of the turn that are left
-    int sp, off;
+    int pair, hg, f, left;  // left: windows of the turn that are left
+    int w, t;               // the pair's
+    int sp, off, k0;        // the turn's seen keys and first position, the next window's first key
     long long off64;
     bool item, turn;  // the next window begins an item's piece, a turn
     bool begin;       // the piece begins its item
 
     __device__ __forceinline__ void enter(const Q8Params& p, int rows, int lane) {  // turn f
-        const int w = p.w0 + pair / p.nt, t = pair % p.nt, L = __ldg(p.L + f);
+        const int L = __ldg(p.L + f);
         int s0, s1, v = 0;
         tile_tokens(p, rows, t, s0, s1);
         for (int s = s0 + lane; s <= s1; s += 32) v = max(v, turn_seen(L, __ldg(p.loc + f * p.tokens + (size_t)w * p.S + s), off64, p.cap));
@@ -188,11 +186,12 @@ struct Q8Walk {
         off = sp > 0 ? (int)off64 : 0;
         off64 += max(L, 0);
         left = turn_windows(p, sp, off);
-        wi = 0;
+        k0 = -(off & (p.align - 1));
         turn = true;
     }
     __device__ __forceinline__ void start(const Q8Params& p, int rows, int lane, int pair_, int hg_, int i, long long n) {
         pair = pair_, hg = hg_, rem = n, begin = i == 0, item = true;
+        w = p.w0 + pair / p.nt, t = pair % p.nt;
         f = 0, off64 = 0;
         enter(p, rows, lane);
         while (i >= left) {
@@ -200,15 +199,15 @@ struct Q8Walk {
             ++f;
             enter(p, rows, lane);
         }
-        wi = i;
+        k0 += i * p.kt;
         left -= i;
     }
-    __device__ __forceinline__ void skip_turn() {  // its windows that have not been handed out
+    __device__ __forceinline__ void skip_turn(const Q8Params& p) {  // its windows that have not been handed out
         const int k = left < rem ? left : (int)rem;
-        left -= k, rem -= k, wi += k;
+        left -= k, rem -= k, k0 += k * p.kt;
     }
-    // The next window; false: none.  `ended`: the windows handed out before end their item.
-    __device__ __forceinline__ bool next(const Q8Params& p, int rows, int lane, Q8Stage& d, bool& ended) {
+    // To the next window, which begins at key k0; false: none.  `ended`: the windows before end their item.
+    __device__ __forceinline__ bool seek(const Q8Params& p, int rows, int lane, bool& ended) {
         ended = false;
         while (left == 0) {
             if (f + 1 < p.F) {
@@ -223,23 +222,26 @@ struct Q8Walk {
                         rem = 0;
                         return false;
                     }
+                    w = p.w0 + pair / p.nt, t = pair % p.nt;
                 }
             }
             enter(p, rows, lane);
         }
-        if (rem == 0) return false;
-        d.w = p.w0 + pair / p.nt, d.t = pair % p.nt, d.hg = hg, d.f = f, d.off = off, d.sp = sp;
-        d.k0 = wi * p.kt - (off & (p.align - 1));
-        d.how = (item ? Q8_ITEM : 0) | (turn ? Q8_TURN : 0) | (begin ? Q8_BEGIN : 0);
+        return rem != 0;
+    }
+    __device__ __forceinline__ int how() const { return (item ? Q8_ITEM : 0) | (turn ? Q8_TURN : 0) | (begin ? Q8_BEGIN : 0); }
+    __device__ __forceinline__ void take(const Q8Params& p) {  // past the window
         item = turn = false;
-        ++wi, --left, --rem;
-        return true;
+        k0 += p.kt, --left, --rem;
     }
 };
 
 // ---- small helpers ------------------------------------------------------------------------
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {  // without an arrival
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {  // when this thread's copies so far have landed
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
@@ -261,11 +263,6 @@ __device__ __forceinline__ float lds_f32(uint32_t a) {
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -352,52 +349,25 @@ template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_
         for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(v[i][u]));
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // the row's largest element to 2^7 .. 2^8 (e4m3) or 2^13 .. 2^14 (f16)
-        const int shift = min((C::NARROW ? 134 : 140) - (__float_as_int(top) >> 23), 126);
+        const int shift = min(140 - (__float_as_int(top) >> 23), 126);
         const float mul = __int_as_float((127 + shift) << 23);
         if (ch == 0) reinterpret_cast<float*>(head + C::QFRAG)[i16] = p.scale_log2 * __int_as_float((127 - shift) << 23);
-        // elements 8 y .. 8 y + 7 of 16-byte K chunk t + 4j, row n + 8 half of tile mt; lane (n, t)'s fragment
-        const int c16 = ch >> 1, y = ch & 1;
-        uint8_t* dst = head + (i16 >> 4) * C::QT * KS * 512 + ((i16 & 7) * 4 + (c16 & 3)) * 16 + (i16 >> 3 & 1) * 4;
-        float x[8];
+        // chunk t + 4j of row n + 8 half of tile mt, lane (n, t)'s: step 4j + u, a[half] = elements 4u, 4u + 1, a[2 + half] the next two
+        const int c16 = ch >> 1;
+        uint8_t* dst = head + ((i16 >> 4) * C::QT * KS + 4 * (c16 >> 2) + 2 * (ch & 1)) * 512 + ((i16 & 7) * 4 + (c16 & 3)) * 16 + (i16 >> 3 & 1) * 4;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = v[i][u] * mul;
-        if constexpr (C::NARROW) {  // step 2j + y: a[half] = the first four elements, a[2 + half] the others
-            dst += (2 * (c16 >> 2) + y) * 512;
+        for (int u = 0; u < 2; ++u) {
+            float x[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) x[y] = v[i][u * 4 + y] * mul;
 #pragma unroll
             for (int term = 0; term < C::QT; ++term) {
-                uint32_t word[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const float nan = __int_as_float(0x7fc00000);  // e4m3 has no infinities
-                    float e0 = x[2 * u], e1 = x[2 * u + 1];
-                    if (term == 0) {
-                        if (fabsf(e0) > 448.f) e0 = nan;
-                        if (fabsf(e1) > 448.f) e1 = nan;
-                    }
-                    word[u] = f32x2_to_e4m3x2(e0, e1);
-                    const uint32_t f = e4m3x2_to_f16x2(word[u]);
-                    const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
-                    // the second and third are 16 times theirs
-                    x[2 * u] = (e0 - __low2float(f2)) * (term == 0 ? 16.f : 1.f);
-                    x[2 * u + 1] = (e1 - __high2float(f2)) * (term == 0 ? 16.f : 1.f);
-                }
-                *reinterpret_cast<uint32_t*>(dst + term * KS * 512) = word[0] | word[1] << 16;
-                *reinterpret_cast<uint32_t*>(dst + term * KS * 512 + 8) = word[2] | word[3] << 16;
+                const uint32_t lo = pack_f16(x[0], x[1]), hi = pack_f16(x[2], x[3]);
+                *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512) = lo;
+                *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512 + 8) = hi;
+                const __half2 a = *reinterpret_cast<const __half2*>(&lo), b = *reinterpret_cast<const __half2*>(&hi);
+                x[0] -= __low2float(a), x[1] -= __high2float(a), x[2] -= __low2float(b), x[3] -= __high2float(b);
             }
-        } else {  // step 4j + 2y + u: a[half] = elements 4u, 4u + 1, a[2 + half] the next two
-            dst += (4 * (c16 >> 2) + 2 * y) * 512;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int term = 0; term < C::QT; ++term) {
-                    float* e = x + 4 * u;
-                    const uint32_t lo = pack_f16(e[0], e[1]), hi = pack_f16(e[2], e[3]);
-                    *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512) = lo;
-                    *reinterpret_cast<uint32_t*>(dst + (term * KS + u) * 512 + 8) = hi;
-                    const __half2 a = *reinterpret_cast<const __half2*>(&lo), b = *reinterpret_cast<const __half2*>(&hi);
-                    e[0] -= __low2float(a), e[1] -= __high2float(a), e[2] -= __low2float(b), e[3] -= __high2float(b);
-                }
         }
     }
 }
@@ -408,9 +378,9 @@ template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_
 //
 // Fragments.  The order of the elements in q . k and of the keys in P V is free as long as both operands
 // share it:
-// * K comes in 16-byte words: thread (n, t) takes chunks t + 4i of the rows of its columns n.  Next to e4m3 queries, two
-//   32-bit words of a chunk are a fragment (16 x 8 x 32) as they are; next to f16 ones, each word is widened to one
-//   (16 x 8 x 16).
+// * K comes in 16-byte words: thread (n, t) takes chunks t + 4i of the rows of its columns n and widens each 32-bit word to a
+//   fragment.  (8-bit products would take K as it is, but mma.sync of e4m3 takes 22 cycles an instruction here, more than the
+//   f16 ones and the widening.)
 // * V comes by transposing 8-bit matrix loads: thread (n, t) gets, of column n, the keys of rows 4t .. 4t + 3, and
 //   widens them in pairs to a fragment.  So the scores that a thread holds have to be those of these four keys: of 16 keys,
 //   key(t, j) = 8 (t / 2) + 2 (t % 2) + j / 2 + 4 (j % 2) for tile j / 2, column 2t + j % 2.  Neighbouring columns lie four rows
@@ -433,7 +403,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
     Q8Stage* desc = reinterpret_cast<Q8Stage*>(smem + C::OFF_DESC);
     if (tid == 0) {
         for (int st = 0; st < STAGES; ++st) {
-            mbar_init(bar_full + st * 8, 33);  // the request and the loading lanes' copies
+            mbar_init(bar_full + st * 8, 33);  // the description and the loading lanes' copies
             mbar_init(bar_empty + st * 8, kQ8Warps);
         }
         for (int x = 0; x < C::QBUFS; ++x) {
@@ -503,10 +473,8 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
             asm volatile("fence.proxy.async;" ::: "memory");  // written with ordinary stores, read by bulk copies
             Q8Walk walk;
             walk.start(p, ROWS, lane, pair0, hg0, i0, u1 - u0);
-            Q8Stage d;
             bool ended;
-            for (int n = 0; walk.next(p, ROWS, lane, d, ended); ++n) {
-                walk.skip_turn();
+            for (int n = 0; walk.seek(p, ROWS, lane, ended); ++n) {
                 const int buf = n % C::QBUFS;
                 if (n >= C::QBUFS && (__any_sync(0xffffffffu, *stop != 0) || !__all_sync(0xffffffffu, mbar_wait(bar_q + buf * 16 + 8, (n / C::QBUFS - 1) & 1)))) {
                     if (lane == 0) {
@@ -517,109 +485,128 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                 }
                 if (lane == 0) {
                     const uint32_t dst = s0 + (uint32_t)(C::OFF_Q + (size_t)buf * C::QBUF);
-                    const size_t at = (size_t)d.f * p.pairs + (size_t)(d.w - p.w0) * p.nt + d.t;
+                    const size_t at = (size_t)walk.f * p.pairs + walk.pair;
                     mbar_expect_tx(bar_q + buf * 16, (uint32_t)(p.hc * C::QHEAD + C::LIMS));
-                    bulk_load(dst, p.qf + (at * p.Hkv + (size_t)d.hg * p.hc) * C::QHEAD, p.hc * C::QHEAD, bar_q + buf * 16);
+                    bulk_load(dst, p.qf + (at * p.Hkv + (size_t)walk.hg * p.hc) * C::QHEAD, p.hc * C::QHEAD, bar_q + buf * 16);
                     bulk_load(dst + (uint32_t)(p.hc * C::QHEAD), p.ql + at * C::LIMS, C::LIMS, bar_q + buf * 16);
                 }
                 __syncwarp();
+                walk.skip_turn(p);
             }
             return;
         }
         // ======================= the requesting warp =======================
-        const int boxes = p.kt >> p.box_shift;
+        // A window ahead of its requests: where its pages are has been looked up by then.  What does not change from window to
+        // window is worked out once: a window's turn came to 1.7 us otherwise, as long as HBM takes to bring it.
+        const int boxes = p.kt >> p.box_shift, hc_shift = p.hc >> 1;  // 1, 2, 4
         if (lane == 0 && !GATHER) {
             prefetch_tmap(&mk);
             prefetch_tmap(&mv);
         }
+        const uint32_t box_at = (uint32_t)(lane * p.box * p.hc * E);  // of this lane's box in a tile
+        // this lane's scale (pages that are whole boxes): of head y % hc, keys 8 (y / hc) .. + 7 of K's or V's tile
+        const int per = p.kt / 8 * p.hc, sy = lane < per ? lane : lane - per;
+        const bool scales = lane < 2 * per;
+        const float* sbase = (lane < per ? p.ks : p.vs) + (sy & (p.hc - 1));
+        const uint32_t sat = s0 + (uint32_t)(C::OFF_SC + 4 * (sy + (lane < per ? 0 : C::SCALES)));
+        const int sbox = (sy >> hc_shift) * 8 >> p.box_shift & 31;
         Q8Walk walk;
         walk.start(p, ROWS, lane, pair0, hg0, i0, u1 - u0);
-        Q8Stage cur, nxt;
-        int page[4] = {-1, -1, -1, -1};  // of the next window: lane's box, or (gathered) keys lane + 32 x; -1: none
+        // of the next window: lane's box, or (gathered) keys lane + 32 x: its page (-1: none) and row there
+        constexpr int NX = GATHER ? 4 : 1;
+        int page[NX], inpage[NX], how = 0, hg = 0;
         bool have, ended;
-        auto find = [&] {
-            have = walk.next(p, ROWS, lane, nxt, ended);
+        auto find = [&](int i) {
+            have = walk.seek(p, ROWS, lane, ended);
             if (!have) return;
             const int n = GATHER ? p.kt : boxes, step = GATHER ? 1 : p.box;
 #pragma unroll
-            for (int x = 0; x < (GATHER ? 4 : 1); ++x) {
-                const int i = lane + 32 * x, l = nxt.k0 + i * step;
+            for (int x = 0; x < NX; ++x) {
+                const int k = lane + 32 * x, l = walk.k0 + k * step, pos = walk.off + l;
                 page[x] = -1;
-                if (i < n && l + step > 0 && l < nxt.sp) page[x] = __ldg(p.bt + (size_t)nxt.w * p.maxb + (nxt.off + l) / p.BS);
+                if (k < n && l + step > 0 && l < walk.sp) {
+                    const int at = p.bs_shift >= 0 ? pos >> p.bs_shift : pos / p.BS;
+                    inpage[x] = pos - at * p.BS;
+                    page[x] = __ldg(p.bt + (size_t)walk.w * p.maxb + at);
+                }
             }
+            how = walk.how();
+            hg = walk.hg;
+            if (lane == 0) {
+                Q8Stage& d = desc[i % (2 * STAGES)];
+                d.w = walk.w, d.t = walk.t, d.hg = hg, d.f = walk.f;
+                d.off = walk.off, d.k0 = walk.k0, d.sp = walk.sp;
+            }
+            walk.take(p);
         };
-        find();
+        find(0);
         bool ok = true;
         int i = 0;
         for (;; ++i) {
             const int st = i % STAGES;
+            const uint32_t full = bar_full + st * 8;
             if (i >= STAGES && (__any_sync(0xffffffffu, *stop != 0) || !__all_sync(0xffffffffu, mbar_wait(bar_empty + st * 8, (i / STAGES - 1) & 1)))) {
                 ok = false;
                 break;
             }
             if (!have) {
                 if (lane == 0) {
-                    desc[st].how = -1;
-                    mbar_arrive(bar_full + st * 8);
+                    desc[i % (2 * STAGES)].how = -1;
+                    mbar_arrive(full);
                 }
-                mbar_arrive(bar_full + st * 8);
+                mbar_arrive(full);
                 break;
             }
-            cur = nxt;
-            int pg[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) pg[x] = page[x] < p.NB ? page[x] : -1;
-            find();  // a window ahead: its table entries are under way while this one waits
-            // the item's piece ends here where the next window begins another or there is none
-            if (!have || (nxt.how & Q8_ITEM)) cur.how |= Q8_LAST | (ended && (cur.how & Q8_BEGIN) ? Q8_WHOLE : 0);
-            if (i == p.stall_tile && c == 0) continue;  // test hook: this stage is never filled
-            const uint32_t dk = s0 + (uint32_t)(st * 2 * C::TENSOR), dv = dk + C::TENSOR, full = bar_full + st * 8;
-            if (lane == 0) {
-                desc[st] = cur;
-                if (GATHER) mbar_arrive(full);
-                else mbar_expect_tx(full, 2u * C::TENSOR);
-            }
-            __syncwarp();
-            const uint32_t sc = s0 + (uint32_t)C::OFF_SC + (uint32_t)(st * 2 * C::SCALES * 4);
+            int pg[NX], row[NX], what = how;
+            const int heads = hg * p.hc;  // the first head
             if constexpr (!GATHER) {
-                if (lane < boxes) {
-                    const int pos = cur.off + cur.k0 + lane * p.box;
-                    const int z = pg[0] >= 0 ? pg[0] * p.BS + pos % p.BS : -2 * p.box;  // rows outside: zeros
-                    const uint32_t at = (uint32_t)(lane * p.box * p.hc * E);
-                    tma_load_4d(dk + at, &mk, 0, z, 0, cur.hg * p.hc, full);
-                    tma_load_4d(dv + at, &mv, 0, z, 0, cur.hg * p.hc, full);
-                }
-                // scales of groups of 8 keys, [group][head]: K's, then V's
-                const int per = p.kt / 8 * p.hc;
-                for (int x = lane; x < ((2 * per + 31) & ~31); x += 32) {
-                    const int y = x < per ? x : x - per, g = y / p.hc;
-                    const int b = __shfl_sync(0xffffffffu, pg[0], (g * 8) >> p.box_shift & 31);
-                    if (x < 2 * per)
-                        cp_async4(sc + 4 * (y + (x < per ? 0 : C::SCALES)),
-                                  b >= 0 ? (x < per ? p.ks : p.vs) + (size_t)b * p.Hkv + cur.hg * p.hc + y % p.hc : &kOne);
+                if (i != p.stall_tile || c != 0) {  // test hook: that stage is never filled
+                    if (lane == 0) mbar_expect(full, 2u * C::TENSOR);
+                    __syncwarp();
+                    const int b = page[0] < p.NB ? page[0] : -1;
+                    if (lane < boxes) {
+                        const int z = b >= 0 ? b * p.BS + inpage[0] : -2 * p.box;  // rows outside: zeros
+                        const uint32_t dk = s0 + (uint32_t)(st * 2 * C::TENSOR) + box_at;
+                        tma_load_4d(dk, &mk, 0, z, 0, heads, full);
+                        tma_load_4d(dk + C::TENSOR, &mv, 0, z, 0, heads, full);
+                    }
+                    const int sb = __shfl_sync(0xffffffffu, b, sbox);
+                    if (scales) cp_async4(sat + (uint32_t)(st * 2 * C::SCALES * 4), sb >= 0 ? sbase + (size_t)sb * p.Hkv + heads : &kOne);
                 }
             } else {
+#pragma unroll
+                for (int x = 0; x < NX; ++x) pg[x] = page[x] < p.NB ? page[x] : -1, row[x] = inpage[x];
+            }
+            find(i + 1);
+            // the item's piece ends here where the next window begins another or there is none
+            if (!have || (how & Q8_ITEM)) what |= Q8_LAST | (ended && (what & Q8_BEGIN) ? Q8_WHOLE : 0);
+            if (i == p.stall_tile && c == 0) continue;
+            if (lane == 0) {
+                desc[i % (2 * STAGES)].how = what;
+                mbar_arrive(full);  // the description is there
+            }
+            if constexpr (GATHER) {
                 // 16-byte chunk ch of row (head, key): [head][panel][KT keys][RB bytes], swizzled as TMA writes it
+                const uint32_t dk = s0 + (uint32_t)(st * 2 * C::TENSOR), dv = dk + C::TENSOR;
+                const uint32_t sc = s0 + (uint32_t)C::OFF_SC + (uint32_t)(st * 2 * C::SCALES * 4);
+                auto of_key = [&](const int (&v)[NX], int key) {
+                    const int v0 = __shfl_sync(0xffffffffu, v[0], key & 31), v1 = __shfl_sync(0xffffffffu, v[1], key & 31);
+                    const int v2 = __shfl_sync(0xffffffffu, v[2], key & 31), v3 = __shfl_sync(0xffffffffu, v[3], key & 31);
+                    return key < 32 ? v0 : key < 64 ? v1 : key < 96 ? v2 : v3;
+                };
                 constexpr int CH = E / 16;
                 for (int x = lane; x < C::KROWS * CH; x += 32) {
-                    const int row = x / CH, ch = x % CH, hh = row / p.kt, key = row - hh * p.kt;
-                    const int k32 = key >> 5;
-                    const int p0 = __shfl_sync(0xffffffffu, pg[0], key & 31), p1 = __shfl_sync(0xffffffffu, pg[1], key & 31);
-                    const int p2 = __shfl_sync(0xffffffffu, pg[2], key & 31), p3 = __shfl_sync(0xffffffffu, pg[3], key & 31);
-                    const int b = k32 == 0 ? p0 : k32 == 1 ? p1 : k32 == 2 ? p2 : p3;
-                    const int pos = cur.off + cur.k0 + key;
-                    const size_t at = b >= 0 ? (((size_t)b * p.BS + pos % p.BS) * p.Hkv + cur.hg * p.hc + hh) * E + ch * 16 : 0;
+                    const int r = x / CH, ch = x % CH, hh = r / p.kt, key = r - hh * p.kt;
+                    const int b = of_key(pg, key), in = of_key(row, key);
+                    const size_t at = b >= 0 ? (((size_t)b * p.BS + in) * p.Hkv + heads + hh) * E + ch * 16 : 0;
                     const uint32_t panel = (uint32_t)((hh * NP + ch / (RB / 16)) * p.kt + key) * RB;
                     const uint32_t to = panel + (uint32_t)((RB == 128 ? (ch & 7) ^ (key & 7) : ch ^ (key >> 1 & 3)) << 4);
                     cp_async16_zfill(dk + to, p.k + at, b >= 0 ? 16 : 0);
                     cp_async16_zfill(dv + to, p.v + at, b >= 0 ? 16 : 0);
                 }
                 for (int x = lane; x < C::KROWS; x += 32) {  // scales, [key][head]
-                    const int key = x / p.hc, k32 = key >> 5;
-                    const int p0 = __shfl_sync(0xffffffffu, pg[0], key & 31), p1 = __shfl_sync(0xffffffffu, pg[1], key & 31);
-                    const int p2 = __shfl_sync(0xffffffffu, pg[2], key & 31), p3 = __shfl_sync(0xffffffffu, pg[3], key & 31);
-                    const int b = k32 == 0 ? p0 : k32 == 1 ? p1 : k32 == 2 ? p2 : p3;
-                    const size_t at = (size_t)b * p.Hkv + cur.hg * p.hc + x % p.hc;
+                    const int b = of_key(pg, x >> hc_shift);
+                    const size_t at = (size_t)b * p.Hkv + heads + (x & (p.hc - 1));
                     cp_async4(sc + 4 * x, b >= 0 ? p.ks + at : &kOne);
                     cp_async4(sc + 4 * (x + C::SCALES), b >= 0 ? p.vs + at : &kOne);
                 }
@@ -719,24 +706,18 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
         };
         // ---- scores ----
         float z[MT][NT][4];
-        [[maybe_unused]] float z2[C::NARROW ? MT : 1][C::NARROW ? NT : 1][4];  // a score is z + z2 / 16
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int x = 0; x < NT; ++x)
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    z[mt][x][y] = 0.f;
-                    if constexpr (C::NARROW) z2[mt][x][y] = 0.f;
-                }
+            for (int x = 0; x < NT; ++x) z[mt][x][0] = z[mt][x][1] = z[mt][x][2] = z[mt][x][3] = 0.f;
 #pragma unroll
         for (int ci = 0; ci < E / 64; ++ci) {
             uint4 kf[NT];
 #pragma unroll
             for (int x = 0; x < NT; ++x) kf[x] = lds128(kb + kbase[x >> 1] + (ci >> 1) * panel + kofs[x & 1][E < 128 ? 0 : ci & 1]);
 #pragma unroll
-            for (int u = 0; u < (C::NARROW ? 2 : 4); ++u) {
-                const int ks = (C::NARROW ? 2 : 4) * ci + u;
+            for (int u = 0; u < 4; ++u) {
+                const int ks = 4 * ci + u;
                 uint32_t a[MT * QT][4];
 #pragma unroll
                 for (int y = 0; y < MT * QT; ++y) {
@@ -750,25 +731,23 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                 }
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
-                    if constexpr (C::NARROW) {
-                        const uint32_t b0 = u == 0 ? kf[x].x : kf[x].z, b1 = u == 0 ? kf[x].y : kf[x].w;
+                    const uint32_t word = u == 0 ? kf[x].x : u == 1 ? kf[x].y : u == 2 ? kf[x].z : kf[x].w;
+                    const uint32_t b0 = e4m3x2_to_f16x2(word), b1 = e4m3x2_hi_to_f16x2(word);
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            mma_e4m3(z[mt][x], a[mt * QT], b0, b1);
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                            for (int term = 1; term < QT; ++term) mma_e4m3(z2[mt][x], a[mt * QT + term], b0, b1);
-                        }
-                    } else {
-                        const uint32_t word = u == 0 ? kf[x].x : u == 1 ? kf[x].y : u == 2 ? kf[x].z : kf[x].w;
-                        const uint32_t b0 = e4m3x2_to_f16x2(word), b1 = e4m3x2_hi_to_f16x2(word);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                            for (int term = QT - 1; term >= 0; --term) mma_f16(z[mt][x], a[mt * QT + term], b0, b1);
-                    }
+                        for (int term = QT - 1; term >= 0; --term) mma_f16(z[mt][x], a[mt * QT + term], b0, b1);
                 }
             }
         }
+        constexpr int TJ = NG == 2 ? 2 : 4, AHEAD = kQ8Ahead8;  // output tiles of a load of V; loads under way
+        uint32_t vals[AHEAD][4];                  // NG == 2: group g, tile j: [2g + j]; else tile j: [j]
+        auto load_v = [&](int j0) {
+            const int cb = j0 >> 1;  // 16-column block
+            ldsm_b8_t(((vb + (cb >> 3) * panel) + vrow) ^ (uint32_t)((cb & 7) << 4), vals[j0 / TJ % AHEAD]);
+        };
+#pragma unroll
+        for (int j0 = 0; j0 < AHEAD * TJ && j0 < NJ; j0 += TJ) load_v(j0);
         // ---- weights ----
         // scales of a 16-key group: the one page's of this thread's keys, or each key's own
         constexpr int NS = GATHER ? 4 : 1;
@@ -788,15 +767,12 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                         const float f = ks * fr[mt][half];
                         if constexpr (GATHER) {
                             float& x = z[mt][2 * g + (k >> 1)][2 * half + (k & 1)];
-                            if constexpr (C::NARROW) x = fmaf(z2[mt][2 * g + (k >> 1)][2 * half + (k & 1)], 0.0625f, x);
                             x = fmaf(x, f, e);
                         } else {
 #pragma unroll
                             for (int x = 2 * g; x < 2 * g + 2; ++x) {
                                 float* y = z[mt][x] + 2 * half;
-                                uint64_t v = f2u(y[0], y[1]);
-                                if constexpr (C::NARROW) v = ffma2(f2u(z2[mt][x][2 * half], z2[mt][x][2 * half + 1]), f2u(0.0625f, 0.0625f), v);
-                                u2f(ffma2(v, f2u(f, f), f2u(e, e)), y[0], y[1]);
+                                u2f(ffma2(f2u(y[0], y[1]), f2u(f, f), f2u(e, e)), y[0], y[1]);
                             }
                         }
                     }
@@ -873,7 +849,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                     }
                 }
             }
-        // ---- P V, a matrix load (2 or 4 output tiles) at a time ----
+        // ---- P V, a matrix load (2 or 4 output tiles) at a time, AHEAD of them under way ----
         uint32_t keep[NG];  // the bytes of this thread's keys that anybody sees
         if constexpr (EDGE) {
 #pragma unroll
@@ -886,12 +862,9 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                 }
             }
         }
-        constexpr int TJ = NG == 2 ? 2 : 4;  // output tiles of a load
 #pragma unroll
         for (int j0 = 0; j0 < NJ; j0 += TJ) {
-            const int cb = j0 >> 1;  // 16-column block
-            uint32_t v[4];           // NG == 2: group g, tile j: v[2g + j]; else tile j: v[j]
-            ldsm_b8_t(((vb + (cb >> 3) * panel) + vrow) ^ (uint32_t)((cb & 7) << 4), v);
+            uint32_t(&v)[4] = vals[j0 / TJ % AHEAD];
             if constexpr (EDGE) {
                 // keys that nobody sees: zeros.  A NaN in the value of a key that some rows see and others do not (0 * NaN
                 // is NaN) becomes a zero here and is added to the rows that see it.
@@ -947,6 +920,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                     for (int y = 0; y < 4; ++y) o[0][j0 + j][y] += part[y];
                 }
             }
+            if (j0 + AHEAD * TJ < NJ) load_v(j0 + AHEAD * TJ);
         }
     };
 
@@ -961,7 +935,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
             __syncwarp();
             continue;
         }
-        const Q8Stage d = desc[st];
+        const Q8Stage d = desc[i % (2 * STAGES)];
         if (d.how < 0) break;
         if (d.how & Q8_ITEM)
 #pragma unroll
@@ -1067,16 +1041,16 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                 }
             continue;
         }
-        // several warps per head: their outputs are added up, in order, where the stage's K and V lay
-        float* sO = reinterpret_cast<float*>(smem + (size_t)st * 2 * C::TENSOR);  // [hc][ROWS][E]
-#pragma unroll 1
-        for (int g = 0; g < wph; ++g) {
-            if (grp == g) {
+        // several warps per head: their outputs are added up, in order, where the stage's K and V lay, 16 rows at a time
+        float* sO = reinterpret_cast<float*>(smem + (size_t)st * 2 * C::TENSOR);  // [hc][16][E]
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll 1
+            for (int g = 0; g < wph; ++g) {
+                if (grp == g)
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        float* dst = sO + ((size_t)hh * ROWS + mt * 16 + y * 8 + n) * E;
+                        float* dst = sO + ((size_t)hh * 16 + y * 8 + n) * E;
 #pragma unroll
                         for (int j = 0; j < NJ; ++j) {
                             float2* at = reinterpret_cast<float2*>(dst + 8 * j + 2 * t);
@@ -1087,24 +1061,25 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                         }
                         if (g == 0 && t == 0) sML[(wid * ROWS + mt * 16 + y * 8 + n) * 2] = lse2[mt][y];  // wid = hh
                     }
+                named_bar_sync(2, kQ8Warps * 32);
             }
-            named_bar_sync(2, kQ8Warps * 32);
-        }
-        for (int x = tid * 4; x < p.hc * ROWS * E; x += kQ8Warps * 32 * 4) {
-            const int i16 = x / E % ROWS, head = x / E / ROWS, e = x % E, row = d.t * ROWS + i16;
-            if (row >= p.rows) continue;
-            const float4 v = *reinterpret_cast<const float4*>(sO + x);
-            const float ls = sML[(head * ROWS + i16) * 2];
-            if (whole) {
-                const size_t orow = out_row(head, row);
-                store_quad<T>(static_cast<T*>(p.out) + orow * E + e, v.x, v.y, v.z, v.w);
-                if (p.out_f32) *reinterpret_cast<float4*>(p.out_f32 + orow * E + e) = v;
-                if (p.lse_out && e == 0) p.lse_out[orow] = ls * kLn2;
-            } else {
-                const size_t at = (slot + head) * ROWS + i16;
-                *reinterpret_cast<float4*>(p.part_o + at * E + e) = v;
-                if (e == 0) p.part_lse[at] = ls;
+            for (int x = tid * 4; x < p.hc * 16 * E; x += kQ8Warps * 32 * 4) {
+                const int i16 = mt * 16 + x / E % 16, head = x / E / 16, e = x % E, row = d.t * ROWS + i16;
+                if (row >= p.rows) continue;
+                const float4 v = *reinterpret_cast<const float4*>(sO + x);
+                const float ls = sML[(head * ROWS + i16) * 2];
+                if (whole) {
+                    const size_t orow = out_row(head, row);
+                    store_quad<T>(static_cast<T*>(p.out) + orow * E + e, v.x, v.y, v.z, v.w);
+                    if (p.out_f32) *reinterpret_cast<float4*>(p.out_f32 + orow * E + e) = v;
+                    if (p.lse_out && e == 0) p.lse_out[orow] = ls * kLn2;
+                } else {
+                    const size_t at = (slot + head) * ROWS + i16;
+                    *reinterpret_cast<float4*>(p.part_o + at * E + e) = v;
+                    if (e == 0) p.part_lse[at] = ls;
+                }
             }
+            if (mt + 1 < MT) named_bar_sync(2, kQ8Warps * 32);
         }
         fence_proxy_async_smem();  // the next window is written here by TMA
         __syncwarp();
@@ -1334,6 +1309,8 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
     p.box = box;
     while (1 << p.box_shift < box) ++p.box_shift;
     p.align = gather ? 1 : box;
+    p.bs_shift = (p.BS & (p.BS - 1)) == 0 ? 0 : -1;
+    while (p.bs_shift >= 0 && 1 << p.bs_shift < p.BS) ++p.bs_shift;
 
     const void* fn = k.fn[gather];
     if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem[gather]) != cudaSuccess ||

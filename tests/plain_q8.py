@@ -88,13 +88,12 @@ def varlen(c):
 
 
 def score_error(c):
-    """Of a scaled score: the dot product of E terms in 32 bits, at most |q| |k| scale in magnitude.  An element of a 16-bit query is
-    held as a sum of e4m3 values, exact but for the last one's smallest step: 2^-10 / 16 next to a row's largest element of 2^7 or
-    more, 2^-21 of it, so the dot product is off by up to 2^-21 sqrt(E) |q| |k| (32-bit queries: a pair of f16, 2^-24 of an element)."""
+    """Of a scaled score: the dot product of E terms in 32 bits, at most |q| |k| scale in magnitude; q's elements under 2^-27 of the
+    row's largest keep 2^-39 of it, less than the sum's own rounding."""
     k = values(c["kc"], c["ks"])
     top = float(torch.nan_to_num(k).norm(dim=-1).max()) if k.numel() else 0.0
     b = abs(c["scale"]) * float(torch.nan_to_num(c["q"].float()).norm(dim=-1).max()) * top
-    return (plain64.U32 * (8 * math.sqrt(c["q"].size(-1)) + 4) + 2.0 ** -21 * math.sqrt(c["q"].size(-1))) * b
+    return plain64.U32 * (8 * math.sqrt(c["q"].size(-1)) + 4) * b
 
 
 def out_bound(c, out, mag, top, keys, wide=False):
