@@ -57,19 +57,22 @@ struct Q8Params : TurnSplit {
     const uint8_t* qf;      // [F][pairs][Hkv] {fragments, [rows] factors} of the rotated queries
     const uint8_t* ql;      // [F][pairs] {[rows] keys of the turn that the row sees, the least of them, unused}
     long long* P;           // [pairs + 1] windows in front of a pair (of one head group)
+    long long* cstart;      // [CTAs + 1] windows in front of a CTA's
     float* part_o;          // [CTAs][2][hc][rows of a tile][E]
     float* part_lse;        // [CTAs][2][hc][rows of a tile] log2 sums, -inf: nothing seen
 };
 
-constexpr int kQ8Warps = 4, kQ8Threads = 256, kQ8Ahead8 = 4;
-constexpr int kQ8MaxPairs = 4096;  // their prefix sums lie in the stages at first
+constexpr int kQ8Warps = 4, kQ8Threads = 256;
+constexpr int kQ8MaxPairs = 2048;  // their prefix sums lie in the stages at first
+// A turn's start (a partial window, its rotated queries, the look-up of its keys) and a piece's end cost about as much as this
+// many windows: the split counts them.  TODO
+constexpr int kQ8TurnCost = 4;
 
 // T: the queries' type, E: head dim, MT: 16-row tiles of a KV head's query rows.
 template <class T, int E, int MT, bool GATHER> struct Q8Cfg {
-    static constexpr int KPW = E * MT >= 256 ? 16 : 32;    // keys of a warp in a window
+    static constexpr int KPW = 16;                      // keys of a warp in a window
     static constexpr int KROWS = kQ8Warps * KPW;        // (key, head) rows of a stage
     static constexpr int TENSOR = KROWS * E;            // bytes of K (or V) in a stage
-    static constexpr int NT = KPW / 8;                  // 8-key tiles
     static constexpr int NJ = E / 8;                    // 8-column tiles of the output
     static constexpr int ROWS = 16 * MT;
     static constexpr int QT = sizeof(T) == 4 ? 2 : 1, PT = QT;  // f16 values of a query element, of a weight
@@ -91,16 +94,16 @@ template <class T, int E, int MT, bool GATHER> struct Q8Cfg {
     static constexpr int ML = QREG ? 0 : kQ8Warps * ROWS * 8;
     static_assert(!QREG || 2 * QHEAD >= kQ8Warps * ROWS * 8, "maxima and sums");
     static constexpr int STAGE = 2 * TENSOR + 2 * SCALES * 4 + 64 + 16;  // tiles, scales, two descriptions (the next window's is written early), barriers
-    static constexpr int FIT = (LIMIT - QBYTES - ML - 16 * QBUFS - 4) / STAGE;
+    static constexpr int FIT = (LIMIT - QBYTES - ML - 16 * QBUFS - 12) / STAGE;
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr size_t OFF_Q = (size_t)STAGES * 2 * TENSOR;
     static constexpr size_t OFF_ML = QREG ? OFF_Q + 2 * QHEAD + LIMS : OFF_Q + QBYTES;
     static constexpr size_t OFF_SC = OFF_Q + QBYTES + ML;               // [STAGES][2][SCALES]
     static constexpr size_t OFF_DESC = OFF_SC + STAGES * 2 * SCALES * 4;
     static constexpr size_t OFF_BAR = OFF_DESC + STAGES * 64;           // full, empty, then q's
-    static constexpr size_t OFF_FLAG = OFF_BAR + STAGES * 16 + QBUFS * 16;
+    static constexpr size_t OFF_SYNC = OFF_BAR + STAGES * 16 + QBUFS * 16, OFF_FLAG = OFF_SYNC + 8;
     static constexpr size_t SMEM = OFF_FLAG + 4;
-    static_assert(STAGES >= 2 && OFF_Q >= (kQ8MaxPairs + 40) * 8, "the prefix sums fit in the stages");
+    static_assert(STAGES >= 2 && OFF_Q >= (2 * kQ8MaxPairs + 40) * 8, "the prefix sums fit in the stages");
     static_assert(SMEM <= LIMIT && OFF_BAR % 16 == 0, "shared memory");
     static_assert(2 * TENSOR >= 2 * 16 * E * 4, "two heads' rows are combined in a stage");
 };
@@ -110,10 +113,10 @@ __device__ __forceinline__ void tile_tokens(const Q8Params& p, int rows, int t, 
     s0 = t * rows / p.G;
     s1 = (min((t + 1) * rows, p.rows) - 1) / p.G;
 }
-// by one thread
-__device__ __forceinline__ int pair_windows(const Q8Params& p, int rows, int pair) {
+// by one thread: {windows, turns that have any}
+__device__ __forceinline__ int2 pair_windows(const Q8Params& p, int rows, int pair) {
     const int w = p.w0 + pair / p.nt, t = pair % p.nt;
-    int s0, s1, nw = 0;
+    int s0, s1, nw = 0, turns = 0;
     tile_tokens(p, rows, t, s0, s1);
     long long off = 0;
     constexpr int AHEAD = 4;  // turns whose lengths and first locations are loaded together
@@ -131,13 +134,14 @@ __device__ __forceinline__ int pair_windows(const Q8Params& p, int rows, int pai
                 int sp = turn_seen(L[x], at[x], off, p.cap);
                 for (int s = s0 + 1; s <= s1; ++s) sp = max(sp, turn_seen(L[x], __ldg(p.loc + (f0 + x) * p.tokens + (size_t)w * p.S + s), off, p.cap));
                 nw += turn_windows(p, sp, sp > 0 ? (int)off : 0);
+                turns += sp > 0;
                 off += max(L[x], 0);
             }
     }
-    return nw;
+    return make_int2(nw, turns);
 }
 
-// CTA c's units [begin(c), begin(c + 1)): windows of all pairs and head groups, evenly split.
+// CTA c's units [begin(c), begin(c + 1)): windows and turn starts (kQ8TurnCost each) of all pairs and head groups, evenly split.
 struct Q8Split {
     long long q, r;
     int n;
@@ -153,21 +157,72 @@ struct Q8Split {
         if (c > n) c = n;
         return c * q + (c < r ? c : r);
     }
-    __device__ __forceinline__ int cta_of(long long u) const {
-        const long long more = r * (q + 1);
-        return (int)(u < more ? over(u, q + 1) : r + over(u - more, q));
-    }
 };
 
-// What a stage holds: window [k0, k0 + kt) of turn f for head group hg of pair (w, t).
+// What a stage holds: keys [k0, k0 + kt) of a turn of which sp are seen, for head group hg of pair (w, t).
 struct alignas(16) Q8Stage {
-    int w, t, hg, f;
-    int off, k0, sp, how;  // the turn's first position, first key, seen keys; Q8_* bits, -1: the end
+    int k0, sp, how, pad0;  // how: Q8_* bits, -1: the end
+    int w, t, hg, pad1;
 };
 static_assert(sizeof(Q8Stage) == 32, "OFF_DESC");
 constexpr int Q8_ITEM = 1, Q8_TURN = 2, Q8_LAST = 4, Q8_WHOLE = 8, Q8_BEGIN = 16;
 
-// Walks units [u, u1) by a whole warp; every lane holds the same values.
+// Window i of turn f of an item; off: the turn's first position, begin: nothing of the item lies in front, before: windows
+// in front, of all.
+struct alignas(16) Q8Place {
+    int pair, hg, f, i;
+    long long off, before;
+    int begin, pad[3];
+};
+// Unit `rest` of a pair, by a whole warp, a turn per lane: fills in f, i, off and begin; returns the windows in front.
+__device__ __forceinline__ int find_unit(const Q8Params& p, int rows, int lane, int pair, long long rest, Q8Place& at) {
+    const int w = p.w0 + pair / p.nt, t = pair % p.nt;
+    int s0, s1, windows = 0;
+    tile_tokens(p, rows, t, s0, s1);
+    long long off = 0;
+    for (int f0 = 0;; f0 += 32) {
+        const bool there = f0 + lane < p.F;
+        const int L = there ? __ldg(p.L + f0 + lane) : 0;
+        long long sum = max(L, 0);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const long long mine = off + sum - max(L, 0);
+        int sp = 0;
+        if (there)
+            for (int s = s0; s <= s1; ++s) sp = max(sp, turn_seen(L, __ldg(p.loc + (f0 + lane) * p.tokens + (size_t)w * p.S + s), mine, p.cap));
+        const int nw = there ? turn_windows(p, sp, sp > 0 ? (int)mine : 0) : 0;
+        int upto = nw;
+        long long units = nw > 0 ? nw + kQ8TurnCost : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            const long long y = __shfl_up_sync(0xffffffffu, units, o);
+            if (lane >= o) upto += x, units += y;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, units > rest);
+        if (past) {
+            const int k = __ffs(past) - 1;
+            const int own = __shfl_sync(0xffffffffu, nw, k), front = windows + __shfl_sync(0xffffffffu, upto, k) - own;
+            const long long in = rest - (__shfl_sync(0xffffffffu, units, k) - own - kQ8TurnCost) - kQ8TurnCost;
+            at.f = f0 + k, at.i = in > 0 ? (int)in : 0;
+            at.off = __shfl_sync(0xffffffffu, mine, k);
+            at.begin = front + at.i == 0;
+            return front + at.i;
+        }
+        rest -= __shfl_sync(0xffffffffu, units, 31);
+        windows += __shfl_sync(0xffffffffu, upto, 31);
+        off += __shfl_sync(0xffffffffu, sum, 31);
+        if (f0 + 32 >= p.F) {  // not reached: rest lies below the pair's units
+            at.f = at.i = at.begin = 0, at.off = 0;
+            return 0;
+        }
+    }
+}
+
+// Walks the windows of a range by a whole warp; every lane holds the same values.
 struct Q8Walk {
     long long rem;
     int pair, hg, f, left;  // left: windows of the turn that are left
@@ -189,18 +244,14 @@ struct Q8Walk {
         k0 = -(off & (p.align - 1));
         turn = true;
     }
-    __device__ __forceinline__ void start(const Q8Params& p, int rows, int lane, int pair_, int hg_, int i, long long n) {
-        pair = pair_, hg = hg_, rem = n, begin = i == 0, item = true;
+    // at `at`, for n windows
+    __device__ __forceinline__ void start(const Q8Params& p, int rows, int lane, const Q8Place& at, long long n) {
+        pair = at.pair, hg = at.hg, rem = n, begin = at.begin != 0, item = true;
         w = p.w0 + pair / p.nt, t = pair % p.nt;
-        f = 0, off64 = 0;
+        f = at.f, off64 = at.off;
         enter(p, rows, lane);
-        while (i >= left) {
-            i -= left;
-            ++f;
-            enter(p, rows, lane);
-        }
-        k0 += i * p.kt;
-        left -= i;
+        k0 += at.i * p.kt;
+        left -= at.i;
     }
     __device__ __forceinline__ void skip_turn(const Q8Params& p) {  // its windows that have not been handed out
         const int k = left < rem ? left : (int)rem;
@@ -391,7 +442,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
     decode_q8_kernel(const __grid_constant__ Q8Params p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
     using C = Q8Cfg<T, E, MT, GATHER>;
     constexpr int QT = C::QT, PT = C::PT;
-    constexpr int KPW = C::KPW, NT = C::NT, KS = C::KS, NJ = C::NJ, STAGES = C::STAGES, ROWS = C::ROWS;
+    constexpr int KPW = C::KPW, KS = C::KS, NJ = C::NJ, STAGES = C::STAGES, ROWS = C::ROWS;
     constexpr int RB = E < 128 ? E : 128;  // bytes of a swizzled row
     constexpr int NP = E / RB;             // panels
     constexpr int NTH = kQ8Threads;
@@ -410,6 +461,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
             mbar_init(bar_q + x * 16, 1);
             mbar_init(bar_q + x * 16 + 8, kQ8Warps);  // free again
         }
+        mbar_init(s0 + (uint32_t)C::OFF_SYNC, kQ8Warps);
         *stop = 0;
         fence_mbar_init();
     }
@@ -421,48 +473,63 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
     // cleared once per call: a bounded wait that gives up sets its bit long after
     if (c == 0 && tid == 0 && (p.w0 == 0 || !aligned)) p.header[3] = aligned ? 0 : 4;
     if (!aligned) return;
-    // ---- the split: every CTA adds up the windows of all pairs and finds its own range ----
-    long long* sP = reinterpret_cast<long long*>(smem);  // [pairs + 1], in the stages
-    long long* scratch = sP + p.pairs + 1;
-    long long carry = 0;
+    // ---- the split: every CTA adds up the windows and units of all pairs and finds its own range ----
+    long long* sP = reinterpret_cast<long long*>(smem);  // [pairs + 1] windows in front of a pair, in the stages
+    long long* sU = sP + p.pairs + 1;                    // [pairs + 1] units
+    long long* scratch = sU + p.pairs + 1;
+    long long carry = 0, carry_u = 0;
     for (int base = 0; base < p.pairs; base += NTH) {
         const int pair = base + tid;
-        const long long own = pair < p.pairs ? pair_windows(p, ROWS, pair) : 0;
-        long long x = own;
+        const int2 own = pair < p.pairs ? pair_windows(p, ROWS, pair) : make_int2(0, 0);
+        const long long own_u = own.x + (long long)kQ8TurnCost * own.y;
+        long long x = own.x, u = own_u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+            const long long y = __shfl_up_sync(0xffffffffu, x, o), yu = __shfl_up_sync(0xffffffffu, u, o);
+            if (lane >= o) x += y, u += yu;
         }
-        if (lane == 31) scratch[wid] = x;
+        if (lane == 31) scratch[wid] = x, scratch[8 + wid] = u;
         __syncthreads();
-        long long before = carry;
+        long long before = carry, before_u = carry_u;
         for (int y = 0; y < NTH / 32; ++y) {
-            if (y < wid) before += scratch[y];
-            carry += scratch[y];
+            if (y < wid) before += scratch[y], before_u += scratch[8 + y];
+            carry += scratch[y], carry_u += scratch[8 + y];
         }
-        if (pair < p.pairs) sP[pair] = before + x - own;
+        if (pair < p.pairs) sP[pair] = before + x - own.x, sU[pair] = before_u + u - own_u;
         __syncthreads();
     }
-    if (tid == 0) sP[p.pairs] = carry;
+    if (tid == 0) sP[p.pairs] = carry, sU[p.pairs] = carry_u;
     __syncthreads();
     for (int i = c * NTH + tid; i <= p.pairs; i += gridDim.x * NTH) p.P[i] = sP[i];  // for the merge
-    const Q8Split split(carry * p.hs, gridDim.x);
-    const long long u0 = split.begin(c), u1 = split.begin(c + 1);
-    if (u0 >= u1) return;
-    int pair0 = 0;
-    {
-        int hi = p.pairs - 1;
-        while (pair0 < hi) {  // the last pair that begins at or before u0; those without windows begin with the next
-            const int mid = (pair0 + hi + 1) >> 1;
-            if (sP[mid] * p.hs <= u0) pair0 = mid; else hi = mid - 1;
+    Q8Place* place = reinterpret_cast<Q8Place*>(scratch);                            // of the range's two ends
+    if (wid < 2) {
+        const Q8Split split(carry_u * p.hs, gridDim.x);
+        const long long u = split.begin(c + wid);
+        Q8Place at{};
+        at.pair = p.pairs, at.before = carry * p.hs;
+        if (u < carry_u * p.hs) {
+            int pair = 0, hi = p.pairs - 1;
+            while (pair < hi) {  // the last pair that begins at or before u; those without windows begin with the next
+                const int mid = (pair + hi + 1) >> 1;
+                if (sU[mid] * p.hs <= u) pair = mid; else hi = mid - 1;
+            }
+            const long long local = u - sU[pair] * p.hs, units = sU[pair + 1] - sU[pair];
+            at.pair = pair, at.hg = (int)Q8Split::over(local, units);
+            at.before = sP[pair] * p.hs + at.hg * (sP[pair + 1] - sP[pair]);
+            at.before += find_unit(p, ROWS, lane, pair, local - at.hg * units, at);
+        }
+        if (lane == 0) {
+            place[wid] = at;
+            if (wid == 0) p.cstart[c] = at.before;
+            else if (c == (int)gridDim.x - 1) p.cstart[c + 1] = at.before;
         }
     }
-    const long long local = u0 - sP[pair0] * p.hs;
-    const int nw0 = (int)(sP[pair0 + 1] - sP[pair0]);
-    const int hg0 = (int)Q8Split::over(local, nw0), i0 = (int)(local - (long long)hg0 * nw0);
     fence_proxy_async_smem();  // TMA writes where the sums lay
     __syncthreads();
+    const Q8Place from = place[0];
+    const long long count = place[1].before - from.before;
+    __syncthreads();
+    if (count <= 0) return;
 
     if (wid >= kQ8Warps) {
         if constexpr (C::CTAS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEW));
@@ -472,7 +539,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
             asm volatile("griddepcontrol.wait;" ::: "memory");
             asm volatile("fence.proxy.async;" ::: "memory");  // written with ordinary stores, read by bulk copies
             Q8Walk walk;
-            walk.start(p, ROWS, lane, pair0, hg0, i0, u1 - u0);
+            walk.start(p, ROWS, lane, from, count);
             bool ended;
             for (int n = 0; walk.seek(p, ROWS, lane, ended); ++n) {
                 const int buf = n % C::QBUFS;
@@ -511,7 +578,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
         const uint32_t sat = s0 + (uint32_t)(C::OFF_SC + 4 * (sy + (lane < per ? 0 : C::SCALES)));
         const int sbox = (sy >> hc_shift) * 8 >> p.box_shift & 31;
         Q8Walk walk;
-        walk.start(p, ROWS, lane, pair0, hg0, i0, u1 - u0);
+        walk.start(p, ROWS, lane, from, count);
         // of the next window: lane's box, or (gathered) keys lane + 32 x: its page (-1: none) and row there
         constexpr int NX = GATHER ? 4 : 1;
         int page[NX], inpage[NX], how = 0, hg = 0;
@@ -534,8 +601,8 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
             hg = walk.hg;
             if (lane == 0) {
                 Q8Stage& d = desc[i % (2 * STAGES)];
-                d.w = walk.w, d.t = walk.t, d.hg = hg, d.f = walk.f;
-                d.off = walk.off, d.k0 = walk.k0, d.sp = walk.sp;
+                d.k0 = walk.k0, d.sp = walk.sp;
+                d.w = walk.w, d.t = walk.t, d.hg = hg;
             }
             walk.take(p);
         };
@@ -638,21 +705,19 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
     };
     auto swizzle = [](int row) { return (uint32_t)(RB == 128 ? row & 7 : row >> 1 & 3); };  // of a row's 16-byte chunks
     const uint32_t panel = (uint32_t)(p.box * RB);
-    constexpr int NG = NT / 2;  // 16-key groups
-    uint32_t kbase[NG], kofs[2][E < 128 ? 1 : 2];  // K rows of column n: its group's, by tile and chunk t or t + 4
-#pragma unroll
-    for (int g = 0; g < NG; ++g) kbase[g] = rows8(2 * g + (n >> 2));
+    constexpr int NT = KPW / 8;              // 8-key tiles
+    uint32_t kofs[2][E < 128 ? 1 : 2];       // K rows of column n, by tile and chunk t or t + 4
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int row = (n >> 1 & 1) * 2 + x + 4 * (n & 1);
 #pragma unroll
-        for (int y = 0; y < (E < 128 ? 1 : 2); ++y) kofs[x][y] = (uint32_t)(row * RB) + (((t + 4 * y) ^ swizzle(row)) << 4);
+        for (int y = 0; y < (E < 128 ? 1 : 2); ++y) kofs[x][y] = rows8(n >> 2) + (uint32_t)(row * RB) + (((t + 4 * y) ^ swizzle(row)) << 4);
     }
-    // V rows of a matrix load: lanes 0 .. 15 the first 16 keys, 16 .. 31 the next (head dim 256: the next 16 columns)
+    // V rows of a matrix load: lanes 0 .. 15 the keys' 16 bytes of a block of columns, 16 .. 31 of the next one
     uint32_t vrow;
     {
         const int t4 = lane >> 2 & 3, j = lane & 3, key = (t4 >> 1) * 8 + (t4 & 1) * 2 + (j >> 1) + 4 * (j & 1), half = lane >> 4;
-        vrow = rows8((NG == 2 ? 2 * half : 0) + (key >> 3)) + (uint32_t)((key & 7) * RB) + ((swizzle(key & 7) ^ (uint32_t)(NG == 2 ? 0 : half)) << 4);
+        vrow = rows8(key >> 3) + (uint32_t)((key & 7) * RB) + ((swizzle(key & 7) ^ (uint32_t)half) << 4);
     }
     const int mykey = (t >> 1) * 8 + (t & 1) * 2;  // key(t, 0)
     uint32_t sQ = 0;  // this lane's fragments of the turn's buffer
@@ -696,10 +761,10 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
     };
 
     // One window's keys [first, first + KPW) of this warp.  EDGE: some row does not see them all.
-    auto window = [&](auto edge, const Q8Stage& d, int first, uint32_t kb, uint32_t sc) {
+    auto window = [&](auto edge, int sp, int first, uint32_t kb, uint32_t sc) {
         constexpr bool EDGE = decltype(edge)::value;
         const uint32_t vb = kb + C::TENSOR;
-        auto key_of = [&](int x, int y) { return 16 * (x >> 1) + mykey + (x & 1) + 4 * y; };  // of tile x, this thread's column y
+        auto key_of = [&](int x, int y) { return mykey + x + 4 * y; };  // of tile x, this thread's column y
         auto sees = [&](int x, int y, int mt, int half) {
             const int key = first + key_of(x, y);
             return key >= 0 && key < lim[mt][half];
@@ -714,7 +779,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
         for (int ci = 0; ci < E / 64; ++ci) {
             uint4 kf[NT];
 #pragma unroll
-            for (int x = 0; x < NT; ++x) kf[x] = lds128(kb + kbase[x >> 1] + (ci >> 1) * panel + kofs[x & 1][E < 128 ? 0 : ci & 1]);
+            for (int x = 0; x < NT; ++x) kf[x] = lds128(kb + (ci >> 1) * panel + kofs[x][E < 128 ? 0 : ci & 1]);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int ks = 4 * ci + u;
@@ -740,8 +805,8 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                 }
             }
         }
-        constexpr int TJ = NG == 2 ? 2 : 4, AHEAD = kQ8Ahead8;  // output tiles of a load of V; loads under way
-        uint32_t vals[AHEAD][4];                  // NG == 2: group g, tile j: [2g + j]; else tile j: [j]
+        constexpr int TJ = 4, AHEAD = 4;  // output tiles of a load of V; loads under way
+        uint32_t vals[AHEAD][4];
         auto load_v = [&](int j0) {
             const int cb = j0 >> 1;  // 16-column block
             ldsm_b8_t(((vb + (cb >> 3) * panel) + vrow) ^ (uint32_t)((cb & 7) << 4), vals[j0 / TJ % AHEAD]);
@@ -749,34 +814,32 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
 #pragma unroll
         for (int j0 = 0; j0 < AHEAD * TJ && j0 < NJ; j0 += TJ) load_v(j0);
         // ---- weights ----
-        // scales of a 16-key group: the one page's of this thread's keys, or each key's own
+        // scales of this thread's keys: their one page's, or each key's own
         constexpr int NS = GATHER ? 4 : 1;
-        float vscale[NG][NS];
+        float vscale[NS];
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int k = 0; k < NS; ++k) {  // key(t, k): tile k / 2, column k % 2
+            const int at = (GATHER ? kw + key_of(k >> 1, k & 1) : (kw >> 3) + (t >> 1)) * p.hc + hh;
+            const float ks = lds_f32(sc + 4 * at);
+            vscale[k] = lds_f32(sc + 4 * (at + C::SCALES));
+            const float e = Scale(vscale[k]).e;
 #pragma unroll
-            for (int k = 0; k < NS; ++k) {  // key(t, k): tile 2g + k / 2, column k % 2
-                const int at = (GATHER ? kw + key_of(2 * g + (k >> 1), k & 1) : (kw >> 3) + 2 * g + (t >> 1)) * p.hc + hh;
-                const float ks = lds_f32(sc + 4 * at);
-                vscale[g][k] = lds_f32(sc + 4 * (at + C::SCALES));
-                const float e = Scale(vscale[g][k]).e;
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int half = 0; half < 2; ++half) {
+                    const float f = ks * fr[mt][half];
+                    if constexpr (GATHER) {
+                        float& x = z[mt][k >> 1][2 * half + (k & 1)];
+                        x = fmaf(x, f, e);
+                    } else {
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float f = ks * fr[mt][half];
-                        if constexpr (GATHER) {
-                            float& x = z[mt][2 * g + (k >> 1)][2 * half + (k & 1)];
-                            x = fmaf(x, f, e);
-                        } else {
-#pragma unroll
-                            for (int x = 2 * g; x < 2 * g + 2; ++x) {
-                                float* y = z[mt][x] + 2 * half;
-                                u2f(ffma2(f2u(y[0], y[1]), f2u(f, f), f2u(e, e)), y[0], y[1]);
-                            }
+                        for (int x = 0; x < NT; ++x) {
+                            float* y = z[mt][x] + 2 * half;
+                            u2f(ffma2(f2u(y[0], y[1]), f2u(f, f), f2u(e, e)), y[0], y[1]);
                         }
                     }
-            }
+                }
+        }
         if constexpr (EDGE) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
@@ -792,9 +855,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                float m = fmaxf(z[mt][0][2 * y], z[mt][0][2 * y + 1]);
-#pragma unroll
-                for (int x = 1; x < NT; ++x) m = fmax3(m, z[mt][x][2 * y], z[mt][x][2 * y + 1]);
+                float m = fmax3(fmaxf(z[mt][0][2 * y], z[mt][0][2 * y + 1]), z[mt][1][2 * y], z[mt][1][2 * y + 1]);
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 top[mt][y] = m;
@@ -813,7 +874,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                     for (int j = 0; j < NJ; ++j) o[mt][j][2 * y] *= alpha, o[mt][j][2 * y + 1] *= alpha;
                 }
         }
-        uint32_t pa[MT][PT][NG][4];
+        uint32_t pa[MT][PT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -824,7 +885,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                     float w[2];
                     u2f(fadd2(f2u(z[mt][x][2 * half], z[mt][x][2 * half + 1]), f2u(-ref, -ref)), w[0], w[1]);
                     w[0] = fast_exp2(w[0]), w[1] = fast_exp2(w[1]);
-                    const Scale s0(vscale[x >> 1][GATHER ? 2 * (x & 1) : 0]), s1(vscale[x >> 1][GATHER ? 2 * (x & 1) + 1 : 0]);
+                    const Scale s0(vscale[GATHER ? 2 * x : 0]), s1(vscale[GATHER ? 2 * x + 1 : 0]);
                     if constexpr (EDGE) {  // what a masked key's scales are does not matter
                         float a, b;
                         u2f(l[mt][half], a, b);
@@ -841,7 +902,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
 #pragma unroll
                     for (int term = 0; term < PT; ++term) {
                         const uint32_t a = pack_f16(w[0], w[1]);
-                        pa[mt][term][x >> 1][(x & 1) * 2 + half] = a;
+                        pa[mt][term][x * 2 + half] = a;
                         if constexpr (PT > 1) {
                             const __half2 h2 = *reinterpret_cast<const __half2*>(&a);
                             w[0] -= __low2float(h2), w[1] -= __high2float(h2);
@@ -849,17 +910,13 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                     }
                 }
             }
-        // ---- P V, a matrix load (2 or 4 output tiles) at a time, AHEAD of them under way ----
-        uint32_t keep[NG];  // the bytes of this thread's keys that anybody sees
+        // ---- P V, a matrix load (4 output tiles) at a time, AHEAD of them under way ----
+        [[maybe_unused]] uint32_t seen = 0u;  // the bytes of this thread's keys that anybody sees
         if constexpr (EDGE) {
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                keep[g] = 0u;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int key = first + key_of(2 * g + (k >> 1), k & 1);
-                    if (key >= 0 && key < d.sp) keep[g] |= 0xffu << (8 * k);
-                }
+            for (int k = 0; k < 4; ++k) {
+                const int key = first + key_of(k >> 1, k & 1);
+                if (key >= 0 && key < sp) seen |= 0xffu << (8 * k);
             }
         }
 #pragma unroll
@@ -871,27 +928,24 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                 bool odd = false;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    v[i] &= keep[NG == 2 ? i >> 1 : 0];
+                    v[i] &= seen;
                     odd |= e4m3_nan(v[i]) != 0;
                 }
                 if (__any_sync(0xffffffffu, odd)) {
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        uint32_t ind[NG][4];  // 1 where the row sees the key
+                        uint32_t ind[4];  // 1 where the row sees the key
 #pragma unroll
                         for (int x = 0; x < NT; ++x)
 #pragma unroll
                             for (int half = 0; half < 2; ++half)
-                                ind[x >> 1][(x & 1) * 2 + half] = (sees(x, 0, mt, half) ? 0x3c00u : 0u) | (sees(x, 1, mt, half) ? 0x3c000000u : 0u);
+                                ind[x * 2 + half] = (sees(x, 0, mt, half) ? 0x3c00u : 0u) | (sees(x, 1, mt, half) ? 0x3c000000u : 0u);
 #pragma unroll
                         for (int j = 0; j < TJ; ++j) {
                             float cnt[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                            for (int g = 0; g < NG; ++g) {
-                                const uint32_t nan = e4m3_nan(v[NG == 2 ? 2 * g + j : j]);
-                                mma_f16(cnt, ind[g], (nan & 0x80u ? 0x3c00u : 0u) | (nan & 0x8000u ? 0x3c000000u : 0u),
-                                        (nan & 0x800000u ? 0x3c00u : 0u) | (nan & 0x80000000u ? 0x3c000000u : 0u));
-                            }
+                            const uint32_t nan = e4m3_nan(v[j]);
+                            mma_f16(cnt, ind, (nan & 0x80u ? 0x3c00u : 0u) | (nan & 0x8000u ? 0x3c000000u : 0u),
+                                    (nan & 0x800000u ? 0x3c00u : 0u) | (nan & 0x80000000u ? 0x3c000000u : 0u));
 #pragma unroll
                             for (int y = 0; y < 4; ++y)
                                 if (cnt[y] > 0.f) o[mt][j0 + j][y] = __int_as_float(0x7fc00000);
@@ -903,41 +957,38 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
             }
 #pragma unroll
             for (int j = 0; j < TJ; ++j) {
-                [[maybe_unused]] float part[4] = {0.f, 0.f, 0.f, 0.f};  // f32: a window's sum by itself, added with one rounding
+                const uint32_t b0 = e4m3x2_to_f16x2(v[j]), b1 = e4m3x2_hi_to_f16x2(v[j]);
+                if constexpr (PT > 1) {  // f32: a window's sum by itself, added with one rounding
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const uint32_t word = v[NG == 2 ? 2 * g + j : j], b0 = e4m3x2_to_f16x2(word), b1 = e4m3x2_hi_to_f16x2(word);
-                    if constexpr (PT > 1) {
-#pragma unroll
-                        for (int term = PT - 1; term >= 0; --term) mma_f16(part, pa[0][term][g], b0, b1);
-                    } else {
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][j0 + j], pa[mt][0][g], b0, b1);
-                    }
-                }
-                if constexpr (PT > 1) {
+                    for (int term = PT - 1; term >= 0; --term) mma_f16(part, pa[0][term], b0, b1);
 #pragma unroll
                     for (int y = 0; y < 4; ++y) o[0][j0 + j][y] += part[y];
+                } else {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][j0 + j], pa[mt][0], b0, b1);
                 }
             }
             if (j0 + AHEAD * TJ < NJ) load_v(j0 + AHEAD * TJ);
         }
     };
 
-    for (int i = 0;; ++i) {
-        const int st = i % STAGES;
-        if (wph > 1 ? named_bar_or(1, kQ8Warps * 32, *stop != 0) : __any_sync(0xffffffffu, *stop != 0)) break;
-        if (!__all_sync(0xffffffffu, mbar_wait(bar_full + st * 8, (i / STAGES) & 1))) {
-            if (lane == 0) {
-                *stop = 1;
-                atomicOr(p.header + 3, 2);
-            }
-            __syncwarp();
-            continue;
-        }
-        const Q8Stage d = desc[i % (2 * STAGES)];
-        if (d.how < 0) break;
-        if (d.how & Q8_ITEM)
+    // Several warps per head meet at the end of a piece, at a barrier whose waits are bounded, too.  false: a wait gave up.
+    uint32_t met = 0;
+    auto meet = [&] {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s0 + (uint32_t)C::OFF_SYNC);
+        return __all_sync(0xffffffffu, mbar_wait(s0 + (uint32_t)C::OFF_SYNC, met++ & 1)) != 0;
+    };
+
+    bool ok = true;
+    for (int st = 0, at = 0, phase = 0;; st = st + 1 == STAGES ? 0 : st + 1, at = at + 1 == 2 * STAGES ? 0 : at + 1, phase ^= st == 0) {
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar_full + st * 8, phase)) != 0)) break;
+        const Q8Stage* d = desc + at;
+        const int4 what = *reinterpret_cast<const int4*>(d);
+        const int k0 = what.x, sp = what.y, how = what.z;
+        if (how < 0) break;
+        if (how & Q8_ITEM)
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 r[mt][0] = r[mt][1] = neg_inf();
@@ -945,33 +996,28 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
             }
-        if ((d.how & Q8_TURN) && !take_q()) {
-            if (lane == 0) {
-                *stop = 1;
-                atomicOr(p.header + 3, 2);
-            }
-            __syncwarp();
-            continue;
-        }
+        if ((how & Q8_TURN) && !(ok = take_q())) break;
 
-        const int first = d.k0 + kw;  // key of the warp's first column
-        if (first < d.sp && first + KPW > 0) {
+        const int first = k0 + kw;  // key of the warp's first column
+        if (first < sp && first + KPW > 0) {
             const uint32_t kb = s0 + (uint32_t)(st * 2 * C::TENSOR), sc = s0 + (uint32_t)C::OFF_SC + (uint32_t)(st * 2 * C::SCALES * 4);
-            if (first < 0 || first + KPW > least) window(std::true_type(), d, first, kb, sc);
-            else window(std::false_type(), d, first, kb, sc);
+            if (first < 0 || first + KPW > least) window(std::true_type(), sp, first, kb, sc);
+            else window(std::false_type(), sp, first, kb, sc);
         }
 
-        if (!(d.how & Q8_LAST)) {
+        if (!(how & Q8_LAST)) {
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_empty + st * 8);
             continue;
         }
         // ---- the piece's result ----
-        const bool whole = (d.how & Q8_WHOLE) != 0;
-        const size_t slot = ((size_t)c * 2 + (d.how & Q8_BEGIN ? 1 : 0)) * p.hc;
+        const int4 item = *reinterpret_cast<const int4*>(&d->w);
+        const int w = item.x, tile0 = item.y * ROWS, h0 = item.z * p.hc;  // its first row, the group's first head
+        const bool whole = (how & Q8_WHOLE) != 0;
+        const size_t slot = ((size_t)c * 2 + (how & Q8_BEGIN ? 1 : 0)) * p.hc;
         auto out_row = [&](int head, int row) {  // of `out`; row < p.rows
             const int s = row / p.G;
-            return ((size_t)d.w * p.Hq + (d.hg * p.hc + head) * p.G + row - s * p.G) * p.S + s;
+            return ((size_t)w * p.Hq + (h0 + head) * p.G + row - s * p.G) * p.S + s;
         };
         float f[MT][2], lse2[MT][2];
 #pragma unroll
@@ -990,7 +1036,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                     sML[(wid * ROWS + row) * 2 + 1] = sum;
                 }
             }
-        if (wph > 1) named_bar_sync(2, kQ8Warps * 32);  // and every warp is done with the stage
+        if (wph > 1 && !(ok = meet())) break;  // and every warp is done with the stage
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -1013,84 +1059,78 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                 // the sums are in units of 2^(r - 7)
                 lse2[mt][y] = sum == 0.f ? neg_inf() : (m == neg_inf() ? 0.f : m - 7.f) + log2f(sum);
             }
-        if (wph == 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_empty + st * 8);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) o[mt][j][y] *= f[mt][y >> 1];
+        if (wph > 1) {
+            // the warps of a head add up their outputs where the stage's K and V lay, half of them to the other half, a tile at a
+            // time; a row's 8-column pieces are shuffled so that rows lie in different banks
+            float* sO = reinterpret_cast<float*>(smem + (size_t)st * 2 * C::TENSOR);  // [hc][wph / 2][16][E]
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
+                for (int half = wph >> 1; half > 0 && ok; half >>= 1) {
+                    float* part = sO + ((size_t)(hh * (wph >> 1) + (grp & (half - 1))) * 16 + n) * E + 2 * t;
+                    if (grp >= half && grp < 2 * half)
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const int i16 = mt * 16 + y * 8 + n, row = d.t * ROWS + i16;
-                    if (row >= p.rows) continue;
-                    const size_t orow = whole ? out_row(hh, row) : (slot + hh) * ROWS + i16;
+                        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        const float2 x = make_float2(o[mt][j][2 * y] * f[mt][y], o[mt][j][2 * y + 1] * f[mt][y]);
-                        const size_t at = orow * E + 8 * j + 2 * t;
-                        if (whole) {
-                            store_pair<T>(static_cast<T*>(p.out) + at, x);
-                            if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + at) = x;
-                        } else {
-                            *reinterpret_cast<float2*>(p.part_o + at) = x;
-                        }
-                    }
-                    if (t == 0) {
-                        if (!whole) p.part_lse[orow] = lse2[mt][y];
-                        else if (p.lse_out) p.lse_out[orow] = lse2[mt][y] * kLn2;
-                    }
+                            for (int y = 0; y < 2; ++y)
+                                *reinterpret_cast<float2*>(part + 8 * y * E + 8 * (j ^ n)) = make_float2(o[mt][j][2 * y], o[mt][j][2 * y + 1]);
+                    ok = meet();
+                    if (grp < half)
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const float2 x = *reinterpret_cast<const float2*>(part + 8 * y * E + 8 * (j ^ n));
+                                o[mt][j][2 * y] += x.x;
+                                o[mt][j][2 * y + 1] += x.y;
+                            }
+                    if (half > 1 || mt + 1 < MT) ok = ok && meet();  // before they are written again
                 }
-            continue;
+            if (!ok) break;
+            fence_proxy_async_smem();  // the next window is written here by TMA
         }
-        // several warps per head: their outputs are added up, in order, where the stage's K and V lay, 16 rows at a time
-        float* sO = reinterpret_cast<float*>(smem + (size_t)st * 2 * C::TENSOR);  // [hc][16][E]
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll 1
-            for (int g = 0; g < wph; ++g) {
-                if (grp == g)
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        float* dst = sO + ((size_t)hh * 16 + y * 8 + n) * E;
-#pragma unroll
-                        for (int j = 0; j < NJ; ++j) {
-                            float2* at = reinterpret_cast<float2*>(dst + 8 * j + 2 * t);
-                            float2 x = g ? *at : make_float2(0.f, 0.f);
-                            x.x += o[mt][j][2 * y] * f[mt][y];
-                            x.y += o[mt][j][2 * y + 1] * f[mt][y];
-                            *at = x;
-                        }
-                        if (g == 0 && t == 0) sML[(wid * ROWS + mt * 16 + y * 8 + n) * 2] = lse2[mt][y];  // wid = hh
-                    }
-                named_bar_sync(2, kQ8Warps * 32);
-            }
-            for (int x = tid * 4; x < p.hc * 16 * E; x += kQ8Warps * 32 * 4) {
-                const int i16 = mt * 16 + x / E % 16, head = x / E / 16, e = x % E, row = d.t * ROWS + i16;
-                if (row >= p.rows) continue;
-                const float4 v = *reinterpret_cast<const float4*>(sO + x);
-                const float ls = sML[(head * ROWS + i16) * 2];
-                if (whole) {
-                    const size_t orow = out_row(head, row);
-                    store_quad<T>(static_cast<T*>(p.out) + orow * E + e, v.x, v.y, v.z, v.w);
-                    if (p.out_f32) *reinterpret_cast<float4*>(p.out_f32 + orow * E + e) = v;
-                    if (p.lse_out && e == 0) p.lse_out[orow] = ls * kLn2;
-                } else {
-                    const size_t at = (slot + head) * ROWS + i16;
-                    *reinterpret_cast<float4*>(p.part_o + at * E + e) = v;
-                    if (e == 0) p.part_lse[at] = ls;
-                }
-            }
-            if (mt + 1 < MT) named_bar_sync(2, kQ8Warps * 32);
-        }
-        fence_proxy_async_smem();  // the next window is written here by TMA
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_empty + st * 8);
+        if (grp > 0) continue;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int i16 = mt * 16 + y * 8 + n, row = tile0 + i16;
+                if (row >= p.rows) continue;
+                const size_t orow = whole ? out_row(hh, row) : (slot + hh) * ROWS + i16;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const float2 x = make_float2(o[mt][j][2 * y], o[mt][j][2 * y + 1]);
+                    const size_t e = orow * E + 8 * j + 2 * t;
+                    if (whole) {
+                        store_pair<T>(static_cast<T*>(p.out) + e, x);
+                        if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + e) = x;
+                    } else {
+                        *reinterpret_cast<float2*>(p.part_o + e) = x;
+                    }
+                }
+                if (t == 0) {
+                    if (!whole) p.part_lse[orow] = lse2[mt][y];
+                    else if (p.lse_out) p.lse_out[orow] = lse2[mt][y] * kLn2;
+                }
+            }
+    }
+    if (!ok && lane == 0) {  // a wait gave up
+        *stop = 1;
+        atomicOr(p.header + 3, 2);
     }
 }
 
 // ---- merge ----------------------------------------------------------------------------------
 // Rows of items that more than one CTA worked on: the log-sum-exp combination of their partials, in CTA
 // order; zeros for pairs without a seen key; NaN in every output where the call's error word is set.
-constexpr int kQ8Ahead = 4;
+constexpr int kQ8Ahead = 4, kQ8MaxCtas = 1023;
 
 template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_kernel(const __grid_constant__ Q8Params p, int rows, int ctas) {
     constexpr int TPR = E / 4, RPB = 256 / TPR;  // threads per row, rows per block
@@ -1098,14 +1138,26 @@ template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_ker
     const int tid = threadIdx.x, h = blockIdx.x % p.Hkv, pair = blockIdx.x / p.Hkv;
     const int w = p.w0 + pair / p.nt, t = pair % p.nt, hg = h / p.hc, hh = h - hg * p.hc;
     const float nan = __int_as_float(0x7fc00000);
-    const long long P0 = __ldcg(p.P + pair), nw = __ldcg(p.P + pair + 1) - P0, total = __ldcg(p.P + p.pairs);
+    const long long P0 = __ldcg(p.P + pair), nw = __ldcg(p.P + pair + 1) - P0, first = P0 * p.hs + hg * nw;
     const bool failed = __ldcg(p.header + 3) != 0;
-    int c0 = 0, c1 = -1;  // CTAs of the item
-    if (nw > 0 && !failed) {
-        const Q8Split split(total * p.hs, ctas);
-        const long long us = P0 * p.hs + hg * nw;
-        c0 = split.cta_of(us), c1 = split.cta_of(us + nw - 1);
-        if (c0 == c1) return;
+    int c0 = 0, c1 = -1;  // CTAs of the item: the last that begin at or before its first and last windows
+    __shared__ long long starts[kQ8MaxCtas + 1];
+    {
+        long long at[(kQ8MaxCtas + 256) / 256];
+#pragma unroll
+        for (int x = 0; x < (kQ8MaxCtas + 256) / 256; ++x) at[x] = x * 256 + tid <= ctas ? __ldcg(p.cstart + x * 256 + tid) : 0;
+#pragma unroll
+        for (int x = 0; x < (kQ8MaxCtas + 256) / 256; ++x)
+            if (x * 256 + tid <= ctas) starts[x * 256 + tid] = at[x];
+        __syncthreads();
+        auto last = [&](long long window) {  // CTA that begins at or before it, by a whole warp
+            const int lane = tid & 31, g = 32 * (__popc(__ballot_sync(0xffffffffu, 32 * lane < ctas && starts[32 * lane & 1023] <= window)) - 1);
+            return g + __popc(__ballot_sync(0xffffffffu, g + lane < ctas && starts[g + lane & 1023] <= window)) - 1;
+        };
+        if (nw > 0 && !failed) {
+            c0 = last(first), c1 = last(first + nw - 1);
+            if (c0 == c1) return;
+        }
     }
     const int e = tid % TPR * 4;
     for (int i = blockIdx.y * RPB + tid / TPR; i < rows && t * rows + i < p.rows; i += gridDim.y * RPB) {
@@ -1120,7 +1172,7 @@ template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_ker
                 const size_t at = (((size_t)(c + k) * 2 + (c + k == c0 ? 1 : 0)) * p.hc + hh) * rows + i;
                 x[k] = neg_inf();
                 v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (c + k <= c1) {
+                if (c + k <= c1 && starts[c + k] < starts[c + k + 1]) {  // a CTA may have no windows
                     x[k] = __ldcg(p.part_lse + at);
                     v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * E + e));
                 }
@@ -1188,14 +1240,14 @@ Q8Kernel q8_pick(int dtype, int E, int rows) {
 }
 
 struct Q8Layout {
-    size_t P, qf, ql, po, pl, total;
+    size_t P, cstart, qf, ql, po, pl, total;
     int ctas, hc, nt, slice;  // slice: sequences of a launch
 };
 int q8_layout(const dvattn_paged_args* a, const Q8Kernel& k, Q8Layout& L) {
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return DVATTN_ERR_CUDA;
-    L.ctas = sms * k.ctas;
+    L.ctas = sms * k.ctas < kQ8MaxCtas ? sms * k.ctas : kQ8MaxCtas;
     L.hc = a->Hkv % 4 == 0 && k.heads == 4 ? 4 : a->Hkv % 2 == 0 ? 2 : 1;
     L.nt = (a->S * (a->Hq / a->Hkv) + k.rows - 1) / k.rows;
     L.slice = kQ8MaxPairs / L.nt;
@@ -1207,6 +1259,7 @@ int q8_layout(const dvattn_paged_args* a, const Q8Kernel& k, Q8Layout& L) {
         return r;
     };
     L.P = take(8 * ((size_t)L.slice * L.nt + 1));
+    L.cstart = take(8 * ((size_t)L.ctas + 1));
     L.qf = take((size_t)a->F * L.slice * L.nt * a->Hkv * k.qhead);
     L.ql = take((size_t)a->F * L.slice * L.nt * k.lims);
     L.po = take(4 * (size_t)L.ctas * 2 * L.hc * k.rows * a->E);
@@ -1295,6 +1348,7 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
     p.qf = qf;
     p.ql = ql;
     p.P = reinterpret_cast<long long*>(ws + L.P);
+    p.cstart = reinterpret_cast<long long*>(ws + L.cstart);
     p.part_o = reinterpret_cast<float*>(ws + L.po);
     p.part_lse = reinterpret_cast<float*>(ws + L.pl);
     // pages that are whole numbers of boxes of 8 rows or more come by TMA, others row by row
