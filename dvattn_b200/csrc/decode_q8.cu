@@ -325,11 +325,6 @@ __device__ __forceinline__ void ldsm_b8_t(uint32_t addr, uint32_t (&v)[4]) {
                  : "r"(addr)
                  : "memory");
 }
-__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 template <class T> __device__ __forceinline__ void store_pair(T* dst, float2 x) {
     if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(dst) = x;
     else *reinterpret_cast<uint32_t*>(dst) = Elem<T>::pack2(x.x, x.y);
