@@ -58,8 +58,8 @@ struct Q8Params : TurnSplit {
     const uint8_t* ql;      // [F][pairs] {[rows] keys of the turn that the row sees, the least of them, unused}
     long long* P;           // [pairs + 1] windows in front of a pair (of one head group)
     long long* cstart;      // [CTAs + 1] windows in front of a CTA's
-    float* part_o;          // [CTAs][2][hc][rows of a tile][E]
-    float* part_lse;        // [CTAs][2][hc][rows of a tile] log2 sums, -inf: nothing seen
+    float* part_o;          // [CTAs][2][hc][rows of a tile][E] sums of weight x value
+    float2* part_ml;        // [CTAs][2][hc][rows of a tile] reference m of the weights 2^(score - m + 7), and their sum
 };
 
 constexpr int kQ8Warps = 4, kQ8Threads = 256;
@@ -418,6 +418,11 @@ template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_
     }
 }
 
+// Natural logarithm of weights 2^(score - m + 7) that add up to `sum`; m = -inf: none are seen, or their sum is NaN.
+__device__ __forceinline__ float log_sum(float m, float sum) {
+    return sum == 0.f ? neg_inf() : ((m == neg_inf() ? 0.f : m - 7.f) + log2f(sum)) * kLn2;
+}
+
 // ---- the attention kernel ---------------------------------------------------------------------
 // Warps 0 .. 3 compute, warp 4 requests the windows.  Warp w works on head w % hc of the group and keys
 // [KPW (w / hc), + KPW) of the window; thread (n, t) = (lane / 4, lane % 4).
@@ -772,6 +777,8 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
             for (int x = 0; x < NT; ++x) z[mt][x][0] = z[mt][x][1] = z[mt][x][2] = z[mt][x][3] = 0.f;
 #pragma unroll
         for (int ci = 0; ci < E / 64; ++ci) {
+            // f32: the sum of 64 elements by itself, added with one rounding (a tensor core's sum cuts at every step)
+            [[maybe_unused]] float part[NT][4] = {};
             uint4 kf[NT];
 #pragma unroll
             for (int x = 0; x < NT; ++x) kf[x] = lds128(kb + (ci >> 1) * panel + kofs[x][E < 128 ? 0 : ci & 1]);
@@ -796,8 +803,14 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int term = QT - 1; term >= 0; --term) mma_f16(z[mt][x], a[mt * QT + term], b0, b1);
+                        for (int term = QT - 1; term >= 0; --term) mma_f16(QT > 1 && term == 0 ? part[x] : z[mt][x], a[mt * QT + term], b0, b1);
                 }
+            }
+            if constexpr (QT > 1) {
+#pragma unroll
+                for (int x = 0; x < NT; ++x)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) z[0][x][y] += part[x][y];
             }
         }
         constexpr int TJ = 4, AHEAD = 4;  // output tiles of a load of V; loads under way
@@ -1014,7 +1027,8 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
             const int s = row / p.G;
             return ((size_t)w * p.Hq + (h0 + head) * p.G + row - s * p.G) * p.S + s;
         };
-        float f[MT][2], lse2[MT][2];
+        float f[MT][2];
+        float2 ml[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -1049,10 +1063,9 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                     }
                 }
                 // a sum that is 0: nothing seen (or only NaN scores' zero weights, which make it NaN)
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                const float inv = sum == 0.f ? 0.f : whole ? 1.f / sum : 1.f;
                 f[mt][y] = r[mt][y] == neg_inf() && sum == sum ? 0.f : (wph > 1 && r[mt][y] != neg_inf() ? fast_exp2(r[mt][y] - m) * inv : inv);
-                // the sums are in units of 2^(r - 7)
-                lse2[mt][y] = sum == 0.f ? neg_inf() : (m == neg_inf() ? 0.f : m - 7.f) + log2f(sum);
+                ml[mt][y] = make_float2(m, sum);
             }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -1111,8 +1124,8 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                     }
                 }
                 if (t == 0) {
-                    if (!whole) p.part_lse[orow] = lse2[mt][y];
-                    else if (p.lse_out) p.lse_out[orow] = lse2[mt][y] * kLn2;
+                    if (!whole) p.part_ml[orow] = ml[mt][y];
+                    else if (p.lse_out) p.lse_out[orow] = log_sum(ml[mt][y].x, ml[mt][y].y);
                 }
             }
     }
@@ -1123,9 +1136,12 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
 }
 
 // ---- merge ----------------------------------------------------------------------------------
-// Rows of items that more than one CTA worked on: the log-sum-exp combination of their partials, in CTA
+// Rows of items that more than one CTA worked on: their partials' sums, brought to one reference, in CTA
 // order; zeros for pairs without a seen key; NaN in every output where the call's error word is set.
 constexpr int kQ8Ahead = 4, kQ8MaxCtas = 1023;
+
+// 2^x of a part's weight: ex2.approx is 2 ulp off, which shows in 32 bits.
+template <class T> __device__ __forceinline__ float weight(float x) { return sizeof(T) == 4 ? exp2f(x) : fast_exp2(x); }
 
 template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_kernel(const __grid_constant__ Q8Params p, int rows, int ctas) {
     constexpr int TPR = E / 4, RPB = 256 / TPR;  // threads per row, rows per block
@@ -1160,35 +1176,32 @@ template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_ker
         const size_t orow = ((size_t)w * p.Hq + h * p.G + row - s * p.G) * p.S + s;
         float m = neg_inf(), den = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
         for (int c = c0; c <= c1; c += kQ8Ahead) {
-            float x[kQ8Ahead];
+            float2 x[kQ8Ahead];
             float4 v[kQ8Ahead];
 #pragma unroll
             for (int k = 0; k < kQ8Ahead; ++k) {
                 const size_t at = (((size_t)(c + k) * 2 + (c + k == c0 ? 1 : 0)) * p.hc + hh) * rows + i;
-                x[k] = neg_inf();
+                x[k] = make_float2(neg_inf(), 0.f);
                 v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (c + k <= c1 && starts[c + k] < starts[c + k + 1]) {  // a CTA may have no windows
-                    x[k] = __ldcg(p.part_lse + at);
+                    x[k] = __ldcg(p.part_ml + at);
                     v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * E + e));
                 }
             }
             float mx = m;
-            bool bad = false;  // fmaxf drops a NaN, the result must not
 #pragma unroll
-            for (int k = 0; k < kQ8Ahead; ++k) {
-                mx = fmaxf(mx, x[k]);
-                bad |= x[k] != x[k];
-            }
-            const float mu = mx == neg_inf() ? 0.f : mx, alpha = fast_exp2(m - mu);
+            for (int k = 0; k < kQ8Ahead; ++k) mx = fmaxf(mx, x[k].x);
+            const float mu = mx == neg_inf() ? 0.f : mx, alpha = weight<T>(m - mu);
             m = mx;
-            den = bad ? nan : den * alpha;
+            den *= alpha;
 #pragma unroll
             for (int k = 0; k < 4; ++k) a[k] *= alpha;
 #pragma unroll
             for (int k = 0; k < kQ8Ahead; ++k) {
-                if (x[k] == neg_inf()) continue;  // an empty part adds nothing
-                const float f = fast_exp2(x[k] - mu);
-                den += f;
+                if (x[k].y == 0.f) continue;  // an empty part adds nothing
+                // a NaN sum: a NaN score (of a reference that is infinite, or of a row's only keys) reaches every element
+                const float f = x[k].y != x[k].y ? x[k].y : weight<T>(x[k].x - mu);
+                den = fmaf(f, x[k].y, den);
                 a[0] = fmaf(f, v[k].x, a[0]);
                 a[1] = fmaf(f, v[k].y, a[1]);
                 a[2] = fmaf(f, v[k].z, a[2]);
@@ -1200,7 +1213,7 @@ template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_ker
         for (int k = 0; k < 4; ++k) a[k] *= inv;
         store_quad<T>(static_cast<T*>(p.out) + orow * E + e, a[0], a[1], a[2], a[3]);
         if (p.out_f32) *reinterpret_cast<float4*>(p.out_f32 + orow * E + e) = make_float4(a[0], a[1], a[2], a[3]);
-        if (p.lse_out && e == 0) p.lse_out[orow] = failed ? nan : den == 0.f ? neg_inf() : (m + log2f(den)) * kLn2;
+        if (p.lse_out && e == 0) p.lse_out[orow] = failed ? nan : log_sum(m, den);
     }
 }
 
@@ -1258,7 +1271,7 @@ int q8_layout(const dvattn_paged_args* a, const Q8Kernel& k, Q8Layout& L) {
     L.qf = take((size_t)a->F * L.slice * L.nt * a->Hkv * k.qhead);
     L.ql = take((size_t)a->F * L.slice * L.nt * k.lims);
     L.po = take(4 * (size_t)L.ctas * 2 * L.hc * k.rows * a->E);
-    L.pl = take(4 * (size_t)L.ctas * 2 * L.hc * k.rows);
+    L.pl = take(8 * (size_t)L.ctas * 2 * L.hc * k.rows);
     L.total = at;
     return DVATTN_OK;
 }
@@ -1345,7 +1358,7 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
     p.P = reinterpret_cast<long long*>(ws + L.P);
     p.cstart = reinterpret_cast<long long*>(ws + L.cstart);
     p.part_o = reinterpret_cast<float*>(ws + L.po);
-    p.part_lse = reinterpret_cast<float*>(ws + L.pl);
+    p.part_ml = reinterpret_cast<float2*>(ws + L.pl);
     // pages that are whole numbers of boxes of 8 rows or more come by TMA, others row by row
     int box = p.kt;
     while (p.BS % box) box >>= 1;
