@@ -4,8 +4,9 @@
 //   out = sum_l softmax_l(scale * rot_f(q) . (K8_l sk)) (V8_l sv)
 //
 // over the keys l that (w, s) sees in every turn f, the query rotated for the turn and rounded to its
-// type, sk and sv the scales of the key's page and head.  Two launches: the attention and the merge of
-// the items that more than one CTA worked on; each is a programmatic dependent of the one before it.
+// type, sk and sv the scales of the key's page and head.  Three launches, each a programmatic dependent of the one before
+// it: the rotation of every turn's queries into matrix fragments, the attention, and the merge of the items that more than
+// one CTA worked on.
 //
 // Numerics.  e4m3 is exact in f16, so K and V are widened to f16 in registers and multiplied on
 // mma.sync with 32-bit accumulation; the scales never touch them.  q's row is multiplied by a power of
@@ -18,8 +19,15 @@
 // 2^-21 of the largest at full precision and drop those under 2^-32.  r moves when the maximum has grown by
 // more than 6 (P stays below 2^14), so that the accumulators are rarely rescaled.
 //
-// Bound: HBM, a byte per cached element.  A CTA reads a page's rows of up to four KV heads together (contiguous
-// in HBM) by TMA, a warp works on 32 keys (head dim 256: 16) of one head.
+// Bound: HBM has a byte per cached element to bring, but a byte is also a conversion and products of tensor cores that take
+// K and V in 16 bits: 128 heads over 8 x 128k keys run at 69% of the copy bandwidth (843 MB in 187 us) with the issue slots
+// 37% and the tensor cores 28% busy; eight computing warps per SM, one dependent step after the other, are what
+// is left (the registers hold no more of them).  8-bit products would need no conversion, but mma.sync of e4m3 takes 22
+// cycles an instruction here against 8 of f16.
+// A CTA reads a page's rows of up to four KV heads together (contiguous in HBM) by TMA; a warp works on 16 keys of one head.
+// With 32 keys a warp waits less often but needs more registers, and a range ends further from its share: 32 sequences of
+// 64 / 4 heads, bf16, 64.2 us against 57.5; head dim 64, chunks of 5 tokens 82 against 61; the long case 186.6 against 190.
+// Rotating the queries in this kernel instead of in a launch of its own cost 4 to 10 us at each turn's start.
 #include "decode.cuh"
 #include "q8.cuh"
 #include "tma_host.cuh"
@@ -65,7 +73,8 @@ struct Q8Params : TurnSplit {
 constexpr int kQ8Warps = 4, kQ8Threads = 256;
 constexpr int kQ8MaxPairs = 2048;  // their prefix sums lie in the stages at first
 // A turn's start (a partial window, its rotated queries, the look-up of its keys) and a piece's end cost about as much as this
-// many windows: the split counts them.  TODO
+// many windows: the split counts them.  96 sequences of 1 to 4 turns, head dim 256: 97.4 us, counted as nothing 107; 32
+// sequences of two turns 57.3, counted as two windows 57.8, as six 57.2.
 constexpr int kQ8TurnCost = 4;
 
 // T: the queries' type, E: head dim, MT: 16-row tiles of a KV head's query rows.

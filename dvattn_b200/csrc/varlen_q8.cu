@@ -5,7 +5,8 @@
 //
 // A prefill is bound by its products, 4 E flops for every (query head, key) pair; widening a key costs
 // 2 E (1 + sizeof T) bytes once per KV head, the time of a few tokens' products.  The same widening inside the
-// attention kernel, per window and work item, would be done again for every 16 tokens.
+// attention kernel, per window and work item, would be done again for every 16 tokens.  Eight chunks of up to 777 tokens
+// behind up to 8192 keys, 32 / 2 heads of 128, bf16: 19 us of 309 (span 3.5, widening 15.5, of which HBM needs 7.5).
 #include "decode.cuh"
 #include "q8.cuh"
 #include "turns.cuh"
@@ -16,8 +17,8 @@ namespace {
 
 struct WidenParams {
     int F, W, T, BS, maxb, cap, own_table;  // own_table: page (w, j) of the widened caches is w * maxb + j
-    long long NB, chunks;                   // 16-byte chunks of a page of one 8-bit cache
-    int row16;                              // chunks of a (token, head) row
+    long long NB, chunks;                   // groups of 8 elements of a page of one cache
+    int row8;                               // ... of a (token, head) row: 8, 16 or 32
     int Hkv;
     const int* loc;
     const int* L;
@@ -82,40 +83,42 @@ template <class T> __global__ void __launch_bounds__(256) widen_kernel(WidenPara
         for (unsigned todo = __ballot_sync(0xffffffffu, page >= 0); todo; todo &= todo - 1) {
             const int src = __ffs(todo) - 1;
             const long long from = __shfl_sync(0xffffffffu, page, src), to = p.own_table ? base + me + src * warps : from;
-#pragma unroll 1
-            for (int tensor = 0; tensor < 2; ++tensor) {
-                const uint4* in = reinterpret_cast<const uint4*>(tensor ? p.v : p.k) + from * p.chunks;
-                uint4* out = static_cast<uint4*>(tensor ? p.wv : p.wk) + to * p.chunks * sizeof(T);
-                const float* sc = (tensor ? p.vs : p.ks) + from * p.Hkv;
-                constexpr int U = 4;
-                for (long long c0 = lane; c0 < p.chunks; c0 += 32 * U) {
-                    uint4 x[U];
-                    float s[U];
+            // A lane's groups lie 32 apart, whole rows: their heads go round by as many.
+            constexpr int U = 4;
+            const int step = 32 / p.row8 % p.Hkv;
+            int head = lane / p.row8 % p.Hkv;
+            const uint2* in[2] = {reinterpret_cast<const uint2*>(p.k) + from * p.chunks, reinterpret_cast<const uint2*>(p.v) + from * p.chunks};
+            uint4* out[2] = {static_cast<uint4*>(p.wk) + to * p.chunks * (sizeof(T) / 2), static_cast<uint4*>(p.wv) + to * p.chunks * (sizeof(T) / 2)};
+            const float* sc[2] = {p.ks + from * p.Hkv, p.vs + from * p.Hkv};
+            for (long long c0 = lane; c0 < p.chunks; c0 += 32 * U) {
+                uint2 x[2][U];
+                float s[2][U];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const long long c = c0 + 32 * u;
-                        if (c < p.chunks) {
-                            x[u] = __ldg(in + c);
-                            s[u] = __ldg(sc + (int)(c / p.row16 % p.Hkv));
+                for (int u = 0; u < U; ++u, head = head + step < p.Hkv ? head + step : head + step - p.Hkv)
+#pragma unroll
+                    for (int tensor = 0; tensor < 2; ++tensor)
+                        if (c0 + 32 * u < p.chunks) {
+                            x[tensor][u] = __ldg(in[tensor] + c0 + 32 * u);
+                            s[tensor][u] = __ldg(sc[tensor] + head);
                         }
-                    }
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int tensor = 0; tensor < 2; ++tensor) {
                         const long long c = c0 + 32 * u;
-                        if (c >= p.chunks) break;
-                        alignas(16) T y[16];
-                        const uint32_t word[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+                        if (c >= p.chunks) continue;
+                        alignas(16) T y[8];
 #pragma unroll
-                        for (int b = 0; b < 8; ++b) {
-                            const uint32_t f = b & 1 ? e4m3x2_hi_to_f16x2(word[b >> 1]) : e4m3x2_to_f16x2(word[b >> 1]);
+                        for (int b = 0; b < 4; ++b) {
+                            const uint32_t word = b < 2 ? x[tensor][u].x : x[tensor][u].y;
+                            const uint32_t f = b & 1 ? e4m3x2_hi_to_f16x2(word) : e4m3x2_to_f16x2(word);
                             const __half2 h = *reinterpret_cast<const __half2*>(&f);
-                            y[2 * b] = widened<T>(__low2float(h) * s[u]);
-                            y[2 * b + 1] = widened<T>(__high2float(h) * s[u]);
+                            y[2 * b] = widened<T>(__low2float(h) * s[tensor][u]);
+                            y[2 * b + 1] = widened<T>(__high2float(h) * s[tensor][u]);
                         }
 #pragma unroll
-                        for (int b = 0; b < (int)sizeof(T); ++b) out[c * sizeof(T) + b] = reinterpret_cast<const uint4*>(y)[b];
+                        for (int b = 0; b < (int)sizeof(T) / 2; ++b) out[tensor][c * (sizeof(T) / 2) + b] = reinterpret_cast<const uint4*>(y)[b];
                     }
-                }
             }
         }
     }
@@ -188,8 +191,8 @@ int varlen_q8_launch(const dvattn_varlen_args* a, const dvattn_q8_scales* sc, vo
         const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
         p.cap = cap > 0x7fffffffLL ? 0x7fffffff : (int)cap;
         p.own_table = L.own_table;
-        p.row16 = a->E / 16;
-        p.chunks = (long long)a->block_size * a->Hkv * p.row16;
+        p.row8 = a->E / 8;
+        p.chunks = (long long)a->block_size * a->Hkv * p.row8;
         p.loc = a->locations; p.L = a->fragment_lengths; p.cu = a->cu_seqlens_q; p.bt = a->block_tables;
         p.k = static_cast<const uint8_t*>(a->k_cache); p.v = static_cast<const uint8_t*>(a->v_cache);
         p.ks = sc->k_scales; p.vs = sc->v_scales;
