@@ -1,0 +1,155 @@
+"""The 8-bit paged cache at its edges: pools past 4 GB, refusals of the torch ops, replayed appends, calls on several streams at
+once, page tables that sequences share."""
+import pytest
+import torch
+
+import dvattn_b200
+import plain_q8
+import test_q8_gpu as q8
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+F8 = torch.float8_e4m3fn
+
+
+def high(c, pages):
+    """The call with its cache's pages moved to the top of a pool of `pages`, the bytes below NaN."""
+    NB = c["kc"].size(0)
+    out = dict(c, bt=torch.where(c["bt"] >= 0, c["bt"] + (pages - NB), c["bt"]))
+    for name in ("kc", "vc"):
+        big = torch.full((pages,) + c[name].shape[1:], 0x7f, dtype=torch.uint8, device=DEV)
+        big[pages - NB:] = c[name].view(torch.uint8)
+        out[name] = big.view(F8)
+    for name in ("ks", "vs"):
+        big = torch.full((pages, c[name].size(1)), float("nan"), device=DEV)
+        big[pages - NB:] = c[name]
+        out[name] = big
+    return out
+
+
+@pytest.mark.parametrize("BS", [16, 6])  # pages by TMA, row by row
+def test_offsets_past_32_bits(BS):
+    """Bitwise what the same pages give in a small pool: decode, packed prefill and append at byte offsets above 2^32."""
+    Hkv, E = 2, 128
+    pages = (1 << 32) // (BS * Hkv * E) + 500
+    c = q8.on_gpu(q8.make([[200, 77], [40, 500]], 2, 8, Hkv, E, 64, BS, BF16))
+    v = q8.on_gpu(q8.make_varlen([[50, 9], [120, 40]], [3, 20], 8, Hkv, E, 32, BS, BF16))
+    for data, call in ((c, q8.call), (v, q8.call_varlen)):
+        small = call(data)
+        big = high(data, pages)
+        for x, y in zip(small, call(big)):
+            assert torch.equal(x, y)
+        del big
+    g = torch.Generator(device=DEV).manual_seed(0)
+    new = torch.randn((2, Hkv, 9, E), generator=g, device=DEV, dtype=BF16)
+    ang = torch.rand((2, 9, 64), generator=g, device=DEV)
+    at = torch.tensor([270, 533], dtype=torch.int32, device=DEV)
+    big = high(c, pages)
+    for d in (c, big):
+        dvattn_b200.dvattn_paged_append_q8(d["kc"], d["vc"], d["ks"], d["vs"], new, -new, ang, ang, d["bt"], at)
+    NB = c["kc"].size(0)
+    for name in ("kc", "vc"):
+        assert torch.equal(big[name][pages - NB:].view(torch.uint8), c[name].view(torch.uint8))
+        assert bool((big[name][:pages - NB].view(torch.uint8) == 0x7f).all())
+    for name in ("ks", "vs"):
+        assert torch.equal(big[name][pages - NB:], c[name]) and bool(torch.isnan(big[name][:pages - NB]).all())
+
+
+def test_refusals_of_the_ops():
+    c = q8.on_gpu(q8.make([[20, 7]], 1, 4, 2, 64, 32, 16, F16))
+    good = [c["q"], c["loc"], c["cos"], c["sin"], c["L"], c["kc"], c["vc"], c["ks"], c["vs"], c["bt"]]
+    dvattn_b200.dvattn_paged_sdpa_q8(*good, c["scale"])
+    bad = {0: [c["q"].double(), c["q"][0], c["q"].expand(2, -1, -1, -1)], 1: [c["loc"].long(), c["loc"][:1]], 2: [c["cos"].half(), c["cos"][..., :20]],
+           4: [c["L"].long(), c["L"][:1], c["L"].cpu()], 5: [c["kc"].view(torch.uint8), c["kc"].float(), c["kc"].to(torch.float8_e5m2), c["kc"][..., :32]],
+           6: [c["vc"].view(torch.uint8), c["vc"][:, :8], c["vc"].transpose(1, 2)],
+           7: [c["ks"].double(), c["ks"][:, :1], c["ks"][:1], c["ks"][:, 0], c["ks"].t().contiguous().t(), c["ks"].cpu()], 8: [c["vs"].half(), c["vs"][..., None]],
+           9: [c["bt"].long(), c["bt"][0], c["bt"].expand(3, -1)]}
+    for i, values in bad.items():
+        for x in values:
+            args = list(good)
+            args[i] = x
+            with pytest.raises(Exception):
+                dvattn_b200.dvattn_paged_sdpa_q8(*args, c["scale"])
+    i32 = dict(dtype=torch.int32, device=DEV)
+    new, ang, at = torch.zeros((1, 2, 3, 64), dtype=F16, device=DEV), torch.zeros((1, 3, 32), device=DEV), torch.zeros(1, **i32)
+    put = [c["kc"], c["vc"], c["ks"], c["vs"], new, new, ang, ang, c["bt"], at]
+    for i, values in {0: [c["kc"].view(torch.uint8), c["kc"].half()], 2: [c["ks"][:1], c["ks"].half()], 4: [new.float(), new[:, :1], new.transpose(1, 2)],
+                      6: [ang[..., :16], ang.half(), ang[:, :2]], 8: [c["bt"].long(), c["bt"].expand(2, -1)], 9: [at.long(), at[:0]]}.items():
+        for x in values:
+            args = list(put)
+            args[i] = x
+            with pytest.raises(Exception):
+                dvattn_b200.dvattn_paged_append_q8(*args)
+    bt, free, count = torch.full((2, 4), -1, **i32), torch.arange(8, **i32), torch.tensor([8], **i32)
+    two = torch.ones(2, **i32)
+    for args in ([bt.long(), free, count, two, two], [bt, free.long(), count, two, two], [bt, free, count.long(), two, two], [bt, free, count, two[:1], two],
+                 [bt, free, count, two, two.long()], [bt.t(), free, count, two, two], [bt, free[None], count, two, two], [bt.cpu(), free, count, two, two],
+                 [bt, free, torch.zeros(2, **i32), two, two]):
+        with pytest.raises(Exception):
+            dvattn_b200.dvattn_assign_pages(*args, 16)
+        with pytest.raises(Exception):
+            dvattn_b200.dvattn_release_pages(*args[:4 if args[4] is two else 3], *([] if args[4] is two else [two.long()]), 16)
+    for size in (0, -1, 1 << 32):
+        with pytest.raises(Exception):
+            dvattn_b200.dvattn_assign_pages(bt, free, count, two, two, size)
+    for slots in (torch.zeros((2, 3), **i32), torch.zeros((1, 3), dtype=torch.int64, device=DEV), torch.zeros(6, dtype=torch.int64, device=DEV)):
+        with pytest.raises(Exception):
+            dvattn_b200.dvattn_assign_pages(bt, free, count, two, two, 16, slots=slots)
+    assert int(count) == 8 and bool((bt == -1).all())
+
+
+def test_append_replayed_at_other_positions():
+    """One captured append, its inputs written anew between replays; the same as calls of their own."""
+    c = q8.make_append(3, 2, 2, 64, 32, 16, BF16, [0, 7, 30], 4)
+    d = {k: x.to(DEV) if torch.is_tensor(x) else x for k, x in c.items()}
+    names = ("kc", "vc", "ks", "vs")
+    start = {n: d[n].clone() for n in names}
+
+    def put(x):
+        dvattn_b200.dvattn_paged_append_q8(x["kc"], x["vc"], x["ks"], x["vs"], x["k"], x["v"], x["cos"], x["sin"], x["bt"], x["positions"])
+
+    put(d)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        put(d)
+    own = {**d, **{n: start[n].clone() for n in names}, "k": d["k"].clone(), "v": d["v"].clone(), "positions": d["positions"].clone()}
+    for n in names:
+        d[n].copy_(start[n])
+    for step in range(5):
+        graph.replay()
+        put(own)
+        for x in (d, own):
+            x["positions"] += 2
+            x["k"] *= 1.7
+            x["v"] *= -1.3
+    torch.cuda.synchronize()
+    for n in names:
+        assert torch.equal(d[n].view(torch.uint8), own[n].view(torch.uint8)), n
+
+
+def test_two_streams_at_once():
+    """Two calls that overlap, each with a workspace of its own: each result is that of the call alone."""
+    cs = [q8.on_gpu(q8.make([[3000, 500 * i], [40, 2000]], 1, 16, 2, 128, 64, 16, BF16, seed=i)) for i in (1, 2)]
+    alone = [q8.call(c) for c in cs]
+    streams = [torch.cuda.Stream() for _ in cs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, (c, s) in enumerate(zip(cs, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(q8.call(c))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for x in got[i]:
+            assert torch.equal(x[0], alone[i][0]) and torch.equal(x[1], alone[i][1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sequences_that_share_pages(dtype):
+    """A prompt's pages in three sequences' tables, and a page twice in one table."""
+    c = q8.make([[64, 20], [64, 33], [64, 5]], 1, 8, 2, 64, 32, 16, dtype)
+    c["bt"][1:, :4] = c["bt"][0, :4]
+    c["bt"][2, 1] = c["bt"][2, 0]
+    q8.check(c)
