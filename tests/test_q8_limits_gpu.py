@@ -153,3 +153,27 @@ def test_sequences_that_share_pages(dtype):
     c["bt"][1:, :4] = c["bt"][0, :4]
     c["bt"][2, 1] = c["bt"][2, 0]
     q8.check(c)
+
+
+@pytest.mark.parametrize("W,BS,maxb,longest", [(9000, 4, 4, 16), (9000, 4, 4, 1), (200, 16, 300, 4800), (100, 2, 200, 400), (2, 16, 5000, 80000),
+                                               (128, 16, 33, 500), (129, 16, 33, 500), (256, 8, 64, 3), (257, 8, 64, 512), (85, 16, 1, 16)])
+@pytest.mark.parametrize("spare", [7, 0, -1, -300])
+def test_pages_by_rows_and_by_parts(W, BS, maxb, longest, spare):
+    """Several chunks of sequences to a warp, several warps to a sequence, long rows, and too few pages with each."""
+    q8.test_pages(W, BS, maxb, longest, spare)
+
+
+def test_append_tiles_at_the_border_of_a_warp():
+    """Pages whose tile one warp can just hold, cannot, and that four warps cannot hold either; each type."""
+    for dtype, E, sizes in ((BF16, 128, (16, 17, 64, 65, 200)), (F16, 64, (32, 33, 130)), (F32, 128, (8, 9, 33, 70)), (BF16, 256, (8, 9, 33))):
+        for BS in sizes:
+            for R in (0, E // 2, E):
+                q8.check_append(q8.make_append(2, 2, 2 * BS + 3, E, R, BS, dtype, [0, BS // 2], 4, seed=BS, magnitude=1.0))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_ranges_of_the_split(dtype):
+    """Windows in numbers around the CTAs', turns of one key, and turns that are empty for some sequences."""
+    for turns in ([[1] * 6] * 9, [[1, 0, 33, 0, 0, 1], [0, 0, 0, 0, 0, 0], [0, 700, 0, 1, 0, 0]], [[5000, 1, 1, 4000]], [[64 * 148]], [[64 * 297, 1]],
+                  [[1, 64 * 300], [0, 1]]):
+        q8.check(q8.make(turns, 1, 8, 1, 64, 32, 16, dtype))
