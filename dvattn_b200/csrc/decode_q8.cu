@@ -20,13 +20,13 @@
 // more than 6 (P stays below 2^14), so that the accumulators are rarely rescaled.
 //
 // Bound: HBM has a byte per cached element to bring, but a byte is also a conversion and products of tensor cores that take
-// K and V in 16 bits: 128 heads over 8 x 128k keys run at 69% of the copy bandwidth (843 MB in 187 us) with the issue slots
-// 37% and the tensor cores 28% busy; eight computing warps per SM, one dependent step after the other, are what
-// is left (the registers hold no more of them).  8-bit products would need no conversion, but mma.sync of e4m3 takes 22
-// cycles an instruction here against 8 of f16.
-// A CTA reads a page's rows of up to four KV heads together (contiguous in HBM) by TMA; a warp works on 16 keys of one head.
-// With 32 keys a warp waits less often but needs more registers, and a range ends further from its share: 32 sequences of
-// 64 / 4 heads, bf16, 64.2 us against 57.5; head dim 64, chunks of 5 tokens 82 against 61; the long case 186.6 against 190.
+// K and V in 16 bits: 128 heads over 4 x 65k to 131k keys (843 MB) take 170 us, 76% of the copy bandwidth.  With eight
+// computing warps an SM (190 us) the issue slots were 37% and the tensor cores 28% busy, a warp waiting 7 cycles from
+// instruction to instruction: twelve is what the registers hold.  8-bit products would need no conversion, but mma.sync of
+// e4m3 takes 22 cycles an instruction here against 8 of f16.
+// A CTA reads a page's rows of two or four KV heads together (contiguous in HBM) by TMA; a warp works on 16 keys of one
+// head.  With 32 keys a warp waits less often but needs more registers, and a range ends further from its share: 32 sequences of
+// 64 / 4 heads, bf16, 64.2 us against 57.5; head dim 64, chunks of 5 tokens 82 against 61 (both with two CTAs an SM).
 // Rotating the queries in this kernel instead of in a launch of its own cost 4 to 10 us at each turn's start.
 #include "decode.cuh"
 #include "q8.cuh"
@@ -70,12 +70,12 @@ struct Q8Params : TurnSplit {
     float2* part_ml;        // [CTAs][2][hc][rows of a tile] reference m of the weights 2^(score - m + 7), and their sum
 };
 
-constexpr int kQ8Warps = 4, kQ8Threads = 256;
+constexpr int kQ8Warps = 4;
 constexpr int kQ8MaxPairs = 2048;  // their prefix sums lie in the stages at first
 // A turn's start (a partial window, its rotated queries, the look-up of its keys) and a piece's end cost about as much as this
-// many windows: the split counts them.  96 sequences of 1 to 4 turns, head dim 256: 97.4 us, counted as nothing 107; 32
-// sequences of two turns 57.3, counted as two windows 57.8, as six 57.2.
-constexpr int kQ8TurnCost = 4;
+// many windows: the split counts them.  96 sequences of 1 to 4 turns, head dim 256: 95.8 us (counted as nothing 107, as eight
+// windows 98.2 to 99.4); 32 sequences of two turns 53.4 (four windows 54.5, twelve 54.2).
+constexpr int kQ8TurnCost = 6;
 
 // T: the queries' type, E: head dim, MT: 16-row tiles of a KV head's query rows.
 template <class T, int E, int MT, bool GATHER> struct Q8Cfg {
@@ -86,14 +86,20 @@ template <class T, int E, int MT, bool GATHER> struct Q8Cfg {
     static constexpr int ROWS = 16 * MT;
     static constexpr int QT = sizeof(T) == 4 ? 2 : 1, PT = QT;  // f16 values of a query element, of a weight
     static constexpr int KS = E / 16;                           // steps of q . k
-    // A head's query fragments: in registers once read, else read for every window, from one of two buffers.
+    // A head's query fragments: in registers once read, or read for every window, from one of two buffers.
     static constexpr int QFRAG = KS * MT * QT * 512, QHEAD = QFRAG + ROWS * 4;  // ... and the rows' factors
-    static constexpr bool QREG = QFRAG <= 4096;
+    // Three CTAs of an SM where a warp's sums and one window fit in 128 registers a thread: four computing warps and one that
+    // requests all.  Else two (f32 of head dim 256: one) of two warpgroups, registers split between them, with a warp of its own
+    // for the queries.  128 heads over 4 x 65k to 131k keys, f16: 170 us against 190; 32 sequences of 64 / 4 heads, bf16, 53.4
+    // against 57.5; two row tiles (head dim 64) would spill, 67.9 against 61.5.
+    static constexpr bool THREE = QT == 1 && MT == 1 && E <= 128;
+    static constexpr bool QREG = !THREE && QFRAG <= 4096;
     static constexpr int QBUFS = QREG ? 1 : 2, HEADS = QREG ? 4 : 2;  // buffers, KV heads of a CTA at most
     static constexpr int LIMS = (ROWS + 4) * 4;                       // what the rows of a tile see, and the least of it
     static constexpr int QBUF = HEADS * QHEAD + LIMS, QBYTES = QBUFS * QBUF;
-    static constexpr int CTAS = QBYTES + 4 * TENSOR > 101 * 1024 ? 1 : 2;  // per SM
-    static constexpr int LIMIT = CTAS == 2 ? 115712 : 232448;              // shared memory of each
+    static constexpr int CTAS = THREE ? 3 : QBYTES + 4 * TENSOR > 101 * 1024 ? 1 : 2;  // per SM
+    static constexpr int LIMIT = CTAS == 3 ? 76800 : CTAS == 2 ? 115712 : 232448;
+    static constexpr int THREADS = THREE ? 160 : 256;              // shared memory of each
     // Two CTAs of an SM have 128 registers a thread at their launch; the computing warpgroup takes what the other one
     // gives up.
     static constexpr int REGS = QREG ? 200 : 208, FEW = 2 * 128 - REGS;
@@ -447,14 +453,14 @@ __device__ __forceinline__ float log_sum(float m, float sum) {
 //   apart and eight rows in a row differ, which the 128-byte swizzle puts in different banks, and a thread's
 //   four keys lie in 8 neighbouring rows: one page, one scale.
 template <class T, int E, int MT, bool GATHER>
-__global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
+__global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, E, MT, GATHER>::CTAS))
     decode_q8_kernel(const __grid_constant__ Q8Params p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
     using C = Q8Cfg<T, E, MT, GATHER>;
     constexpr int QT = C::QT, PT = C::PT;
     constexpr int KPW = C::KPW, KS = C::KS, NJ = C::NJ, STAGES = C::STAGES, ROWS = C::ROWS;
     constexpr int RB = E < 128 ? E : 128;  // bytes of a swizzled row
     constexpr int NP = E / RB;             // panels
-    constexpr int NTH = kQ8Threads;
+    constexpr int NTH = C::THREADS;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t s0 = smem_u32(smem);
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -543,30 +549,36 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
     if (wid >= kQ8Warps) {
         if constexpr (C::CTAS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEW));
         if (wid > kQ8Warps + 1) return;
-        if (wid == kQ8Warps + 1) {
-            // =================== requests the turns' fragments ===================
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            asm volatile("fence.proxy.async;" ::: "memory");  // written with ordinary stores, read by bulk copies
+        // Requests the fragments of turn f of head group hg of a pair, the n-th of this CTA; false: a wait gave up.
+        auto request_q = [&](int n, int f, int pair, int hg) {
+            if (n == 0) {
+                asm volatile("griddepcontrol.wait;" ::: "memory");
+                asm volatile("fence.proxy.async;" ::: "memory");  // written with ordinary stores, read by bulk copies
+            }
+            const int buf = n % C::QBUFS;
+            if (n >= C::QBUFS && (__any_sync(0xffffffffu, *stop != 0) || !__all_sync(0xffffffffu, mbar_wait(bar_q + buf * 16 + 8, (n / C::QBUFS - 1) & 1)))) return false;
+            if (lane == 0) {
+                const uint32_t dst = s0 + (uint32_t)(C::OFF_Q + (size_t)buf * C::QBUF);
+                const size_t at = (size_t)f * p.pairs + pair;
+                mbar_expect_tx(bar_q + buf * 16, (uint32_t)(p.hc * C::QHEAD + C::LIMS));
+                bulk_load(dst, p.qf + (at * p.Hkv + (size_t)hg * p.hc) * C::QHEAD, p.hc * C::QHEAD, bar_q + buf * 16);
+                bulk_load(dst + (uint32_t)(p.hc * C::QHEAD), p.ql + at * C::LIMS, C::LIMS, bar_q + buf * 16);
+            }
+            __syncwarp();
+            return true;
+        };
+        if (!C::THREE && wid == kQ8Warps + 1) {  // a warp of its own for them
             Q8Walk walk;
             walk.start(p, ROWS, lane, from, count);
             bool ended;
             for (int n = 0; walk.seek(p, ROWS, lane, ended); ++n) {
-                const int buf = n % C::QBUFS;
-                if (n >= C::QBUFS && (__any_sync(0xffffffffu, *stop != 0) || !__all_sync(0xffffffffu, mbar_wait(bar_q + buf * 16 + 8, (n / C::QBUFS - 1) & 1)))) {
+                if (!request_q(n, walk.f, walk.pair, walk.hg)) {
                     if (lane == 0) {
                         *stop = 1;
                         atomicOr(p.header + 3, 1);
                     }
                     break;
                 }
-                if (lane == 0) {
-                    const uint32_t dst = s0 + (uint32_t)(C::OFF_Q + (size_t)buf * C::QBUF);
-                    const size_t at = (size_t)walk.f * p.pairs + walk.pair;
-                    mbar_expect_tx(bar_q + buf * 16, (uint32_t)(p.hc * C::QHEAD + C::LIMS));
-                    bulk_load(dst, p.qf + (at * p.Hkv + (size_t)walk.hg * p.hc) * C::QHEAD, p.hc * C::QHEAD, bar_q + buf * 16);
-                    bulk_load(dst + (uint32_t)(p.hc * C::QHEAD), p.ql + at * C::LIMS, C::LIMS, bar_q + buf * 16);
-                }
-                __syncwarp();
                 walk.skip_turn(p);
             }
             return;
@@ -618,6 +630,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
         find(0);
         bool ok = true;
         int i = 0;
+        [[maybe_unused]] int turns = 0;
         for (;; ++i) {
             const int st = i % STAGES;
             const uint32_t full = bar_full + st * 8;
@@ -652,6 +665,11 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
             } else {
 #pragma unroll
                 for (int x = 0; x < NX; ++x) pg[x] = page[x] < p.NB ? page[x] : -1, row[x] = inpage[x];
+            }
+            if (C::THREE && (what & Q8_TURN) && !request_q(turns++, walk.f, walk.pair, hg)) {
+                ok = false;
+                ++i;
+                break;
             }
             find(i + 1);
             // the item's piece ends here where the next window begins another or there is none
@@ -822,7 +840,7 @@ __global__ void __launch_bounds__(kQ8Threads, (Q8Cfg<T, E, MT, GATHER>::CTAS))
                     for (int y = 0; y < 4; ++y) z[0][x][y] += part[x][y];
             }
         }
-        constexpr int TJ = 4, AHEAD = 4;  // output tiles of a load of V; loads under way
+        constexpr int TJ = 4, AHEAD = 2;  // output tiles of a load of V; loads under way
         uint32_t vals[AHEAD][4];
         auto load_v = [&](int j0) {
             const int cb = j0 >> 1;  // 16-column block
@@ -1234,7 +1252,7 @@ struct Q8Kernel {
     const void* rotate;
     const void* merge;
     int qhead, lims;        // bytes of a head's fragments and factors, of a tile's limits
-    int krows, rows, ctas, heads;  // CTAs per SM, KV heads of one at most
+    int krows, rows, ctas, heads, threads;  // CTAs per SM, KV heads of one at most
     size_t smem[2];
 };
 template <class T, int E, int MT> Q8Kernel q8_kernel() {
@@ -1242,7 +1260,7 @@ template <class T, int E, int MT> Q8Kernel q8_kernel() {
     using G = Q8Cfg<T, E, MT, true>;
     static_assert(C::KROWS == G::KROWS && C::CTAS == G::CTAS && C::HEADS == G::HEADS, "one layout");
     return {{(const void*)&decode_q8_kernel<T, E, MT, false>, (const void*)&decode_q8_kernel<T, E, MT, true>}, (const void*)&rotate_q8_kernel<T, E, MT>,
-            (const void*)&merge_q8_kernel<T, E>, C::QHEAD, C::LIMS, C::KROWS, C::ROWS, C::CTAS, C::HEADS, {C::SMEM, G::SMEM}};
+            (const void*)&merge_q8_kernel<T, E>, C::QHEAD, C::LIMS, C::KROWS, C::ROWS, C::CTAS, C::HEADS, C::THREADS, {C::SMEM, G::SMEM}};
 }
 // One 16-row tile, or two where a KV head has more query rows (then the cache is read half as often); two
 // tiles do not fit in the registers with 32-bit queries or head dim 256.
@@ -1408,7 +1426,7 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
         if (e != cudaSuccess) break;
         void* args[] = {&p, &mk, &mv};
         cfg.gridDim = dim3((unsigned)L.ctas);
-        cfg.blockDim = dim3(kQ8Threads);
+        cfg.blockDim = dim3(k.threads);
         cfg.dynamicSmemBytes = k.smem[gather];
         cfg.numAttrs = a->F > 0 ? 1 : 0;  // it waits for nothing itself: the rotation has
         e = cudaLaunchKernelExC(&cfg, fn, args);

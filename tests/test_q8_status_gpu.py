@@ -25,7 +25,7 @@ import dvattn_b200
 import test_q8_gpu as q8
 from dvattn_b200 import capi
 what, S, BS = sys.argv[2], int(sys.argv[3]), int(sys.argv[4])
-c = q8.on_gpu(q8.make([[30000, 77], [40, 40000]], S, 16, 2, 128, 64, BS, torch.bfloat16))
+c = q8.on_gpu(q8.make([[60000, 77], [40, 80000]], S, 32, 4, 128, 64, BS, torch.bfloat16))
 out, lse = torch.zeros_like(c["q"]), torch.zeros(c["q"].shape[:3], device="cuda:0")
 if what == "capi":
     ws = capi.paged_sdpa_q8(out, c["scale"], c["loc"], c["q"], c["cos"], c["sin"], c["L"], c["kc"], c["vc"], c["ks"], c["vs"], c["bt"], lse=lse)
