@@ -40,6 +40,10 @@ int evict_launch(const dvattn_evict_args* a, void* workspace, size_t wbytes, cud
 // the cache held in 8 bits: decode attention (decode_q8.cu), varlen attention (varlen_q8.cu), append (append_q8.cu)
 size_t decode_q8_workspace_size(const dvattn_paged_args* a);
 int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream);
+// over packed tokens, a call of one token for each `sequence` of `tokens` (cos / sin rows of R / 2); cu: where the nseq sequences begin
+size_t packed_q8_workspace_size(const dvattn_paged_args* tokens, const int* cu, int nseq);
+int packed_q8_launch(const dvattn_paged_args* tokens, const int* cu, int nseq, const dvattn_q8_scales* sc, void* workspace, size_t wbytes,
+                     cudaStream_t stream);
 size_t varlen_q8_workspace_size(const dvattn_varlen_args* a);
 int varlen_q8_launch(const dvattn_varlen_args* a, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream);
 int append_q8_launch(const dvattn_append_args* a, const dvattn_q8_scales* sc, cudaStream_t stream);

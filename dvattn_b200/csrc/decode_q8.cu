@@ -41,10 +41,14 @@ namespace dvb {
 
 struct Q8Params : TurnSplit {
     // of TurnSplit: F, BS, maxb, cap, NB, kt, nt, align, loc, L, bt; W: sequences of this launch
-    int w0;                 // its first sequence
+    int w0;                 // its first sequence (packed tokens: its first tile)
     int Hq, Hkv, G, S, R, rows;
+    int sh, ss;             // row of `out` of head h, token s of a sequence: (its first token) Hq + h sh + s ss
+    int angles;             // entries of a row of cos / sin
+    const int* cu;          // packed tokens: where the sequences begin, [nseq + 1]; null: S tokens of each
+    int nseq;
     int hc, hs;             // KV heads a CTA reads together, groups of them (hc * hs = Hkv)
-    int pairs;              // W * nt (sequence, row tile) pairs
+    int pairs;              // (sequence, row tile) pairs: W * nt, packed tokens: tiles, some of them empty
     int box, box_shift;     // rows of a TMA box (gathered: rows of the stage), its log2
     int bs_shift;           // log2 of the page size, -1: it is no power of two
     long long tokens;       // all sequences' (a turn's stride in loc and cos / sin)
@@ -124,15 +128,41 @@ template <class T, int E, int MT, bool GATHER> struct Q8Cfg {
 };
 
 // ---- the windows of a (sequence, row tile) pair ------------------------------------------
-__device__ __forceinline__ void tile_tokens(const Q8Params& p, int rows, int t, int& s0, int& s1) {
-    s0 = t * rows / p.G;
-    s1 = (min((t + 1) * rows, p.rows) - 1) / p.G;
+struct Q8Tile {
+    int table, t, tok0, rows;  // row of the block tables, tile of the sequence, its first token, its rows
+    // tokens s0 .. s1 of the sequence (none: s0 > s1)
+    __device__ __forceinline__ void tokens(const Q8Params& p, int size, int& s0, int& s1) const {
+        s0 = t * size / p.G;
+        s1 = t * size < rows ? (min((t + 1) * size, rows) - 1) / p.G : s0 - 1;
+    }
+};
+// Where sequence w of packed tokens begins: as the 16-bit attention reads them, tokens before the first sequence and those
+// behind the last one (a sequence `nseq` here) have the first one's table.
+__device__ __forceinline__ int packed_start(const Q8Params& p, int w) {
+    return w <= 0 ? 0 : w > p.nseq ? (int)p.tokens : min(max(__ldg(p.cu + w), 0), (int)p.tokens);
 }
+// Packed: sequence w's tiles are those from floor(first row / size) + w on, which leaves room for them all.
+__device__ __forceinline__ Q8Tile tile_of(const Q8Params& p, int size, int pair) {
+    if (p.cu == nullptr) {
+        const int w = p.w0 + pair / p.nt;
+        return {w, pair % p.nt, w * p.S, p.rows};
+    }
+    const int x = p.w0 + pair;
+    int w = 0, hi = p.nseq;
+    while (w < hi) {
+        const int mid = (w + hi + 1) >> 1;
+        if ((int)((long long)packed_start(p, mid) * p.G / size) + mid <= x) w = mid; else hi = mid - 1;
+    }
+    const int tok0 = packed_start(p, w), rows = (packed_start(p, w + 1) - tok0) * p.G;
+    return {w < p.nseq ? w : 0, x - ((int)((long long)tok0 * p.G / size) + w), tok0, rows};
+}
+__device__ __forceinline__ size_t out_row(const Q8Params& p, int tok0, int head, int s) { return (size_t)tok0 * p.Hq + (size_t)head * p.sh + (size_t)s * p.ss; }
 // by one thread: {windows, turns that have any}
 __device__ __forceinline__ int2 pair_windows(const Q8Params& p, int rows, int pair) {
-    const int w = p.w0 + pair / p.nt, t = pair % p.nt;
+    const Q8Tile tile = tile_of(p, rows, pair);
     int s0, s1, nw = 0, turns = 0;
-    tile_tokens(p, rows, t, s0, s1);
+    tile.tokens(p, rows, s0, s1);
+    if (s0 > s1) return make_int2(0, 0);
     long long off = 0;
     constexpr int AHEAD = 4;  // turns whose lengths and first locations are loaded together
     for (int f0 = 0; f0 < p.F; f0 += AHEAD) {
@@ -141,13 +171,13 @@ __device__ __forceinline__ int2 pair_windows(const Q8Params& p, int rows, int pa
         for (int x = 0; x < AHEAD; ++x)
             if (f0 + x < p.F) {
                 L[x] = __ldg(p.L + f0 + x);
-                at[x] = __ldg(p.loc + (f0 + x) * p.tokens + (size_t)w * p.S + s0);
+                at[x] = __ldg(p.loc + (f0 + x) * p.tokens + tile.tok0 + s0);
             }
 #pragma unroll
         for (int x = 0; x < AHEAD; ++x)
             if (f0 + x < p.F) {
                 int sp = turn_seen(L[x], at[x], off, p.cap);
-                for (int s = s0 + 1; s <= s1; ++s) sp = max(sp, turn_seen(L[x], __ldg(p.loc + (f0 + x) * p.tokens + (size_t)w * p.S + s), off, p.cap));
+                for (int s = s0 + 1; s <= s1; ++s) sp = max(sp, turn_seen(L[x], __ldg(p.loc + (f0 + x) * p.tokens + tile.tok0 + s), off, p.cap));
                 nw += turn_windows(p, sp, sp > 0 ? (int)off : 0);
                 turns += sp > 0;
                 off += max(L[x], 0);
@@ -174,10 +204,10 @@ struct Q8Split {
     }
 };
 
-// What a stage holds: keys [k0, k0 + kt) of a turn of which sp are seen, for head group hg of pair (w, t).
+// What a stage holds: keys [k0, k0 + kt) of a turn of which sp are seen.
 struct alignas(16) Q8Stage {
     int k0, sp, how, pad0;  // how: Q8_* bits, -1: the end
-    int w, t, hg, pad1;
+    int tok0, t, hg, rows;  // of the pair, its head group
 };
 static_assert(sizeof(Q8Stage) == 32, "OFF_DESC");
 constexpr int Q8_ITEM = 1, Q8_TURN = 2, Q8_LAST = 4, Q8_WHOLE = 8, Q8_BEGIN = 16;
@@ -191,9 +221,9 @@ struct alignas(16) Q8Place {
 };
 // Unit `rest` of a pair, by a whole warp, a turn per lane: fills in f, i, off and begin; returns the windows in front.
 __device__ __forceinline__ int find_unit(const Q8Params& p, int rows, int lane, int pair, long long rest, Q8Place& at) {
-    const int w = p.w0 + pair / p.nt, t = pair % p.nt;
+    const Q8Tile tile = tile_of(p, rows, pair);
     int s0, s1, windows = 0;
-    tile_tokens(p, rows, t, s0, s1);
+    tile.tokens(p, rows, s0, s1);
     long long off = 0;
     for (int f0 = 0;; f0 += 32) {
         const bool there = f0 + lane < p.F;
@@ -207,7 +237,7 @@ __device__ __forceinline__ int find_unit(const Q8Params& p, int rows, int lane, 
         const long long mine = off + sum - max(L, 0);
         int sp = 0;
         if (there)
-            for (int s = s0; s <= s1; ++s) sp = max(sp, turn_seen(L, __ldg(p.loc + (f0 + lane) * p.tokens + (size_t)w * p.S + s), mine, p.cap));
+            for (int s = s0; s <= s1; ++s) sp = max(sp, turn_seen(L, __ldg(p.loc + (f0 + lane) * p.tokens + tile.tok0 + s), mine, p.cap));
         const int nw = there ? turn_windows(p, sp, sp > 0 ? (int)mine : 0) : 0;
         int upto = nw;
         long long units = nw > 0 ? nw + kQ8TurnCost : 0;
@@ -241,7 +271,7 @@ __device__ __forceinline__ int find_unit(const Q8Params& p, int rows, int lane, 
 struct Q8Walk {
     long long rem;
     int pair, hg, f, left;  // left: windows of the turn that are left
-    int w, t;               // the pair's
+    Q8Tile tile;            // the pair's
     int sp, off, k0;        // the turn's seen keys and first position, the next window's first key
     long long off64;
     bool item, turn;  // the next window begins an item's piece, a turn
@@ -250,8 +280,8 @@ struct Q8Walk {
     __device__ __forceinline__ void enter(const Q8Params& p, int rows, int lane) {  // turn f
         const int L = __ldg(p.L + f);
         int s0, s1, v = 0;
-        tile_tokens(p, rows, t, s0, s1);
-        for (int s = s0 + lane; s <= s1; s += 32) v = max(v, turn_seen(L, __ldg(p.loc + f * p.tokens + (size_t)w * p.S + s), off64, p.cap));
+        tile.tokens(p, rows, s0, s1);
+        for (int s = s0 + lane; s <= s1; s += 32) v = max(v, turn_seen(L, __ldg(p.loc + f * p.tokens + tile.tok0 + s), off64, p.cap));
         sp = __reduce_max_sync(0xffffffffu, v);
         off = sp > 0 ? (int)off64 : 0;
         off64 += max(L, 0);
@@ -262,7 +292,7 @@ struct Q8Walk {
     // at `at`, for n windows
     __device__ __forceinline__ void start(const Q8Params& p, int rows, int lane, const Q8Place& at, long long n) {
         pair = at.pair, hg = at.hg, rem = n, begin = at.begin != 0, item = true;
-        w = p.w0 + pair / p.nt, t = pair % p.nt;
+        tile = tile_of(p, rows, pair);
         f = at.f, off64 = at.off;
         enter(p, rows, lane);
         k0 += at.i * p.kt;
@@ -288,7 +318,7 @@ struct Q8Walk {
                         rem = 0;
                         return false;
                     }
-                    w = p.w0 + pair / p.nt, t = pair % p.nt;
+                    tile = tile_of(p, rows, pair);
                 }
             }
             enter(p, rows, lane);
@@ -370,13 +400,16 @@ template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int h = blockIdx.x % p.Hkv, fp = blockIdx.x / p.Hkv, f = fp / p.pairs, pair = fp - f * p.pairs;
-    const int w = p.w0 + pair / p.nt, t = pair % p.nt, tid = threadIdx.x;
+    const int tid = threadIdx.x;
+    const Q8Tile tile = tile_of(p, ROWS, pair);
+    const int t = tile.t;
     long long off = 0;
     for (int x = 0; x < f; ++x) off += max(__ldg(p.L + x), 0);
     const int L = __ldg(p.L + f);
     int s0, s1, sp = 0;
-    tile_tokens(p, ROWS, t, s0, s1);
-    const int* loc = p.loc + f * p.tokens + (size_t)w * p.S;
+    tile.tokens(p, ROWS, s0, s1);
+    if (s0 > s1) return;
+    const int* loc = p.loc + f * p.tokens + tile.tok0;
     const bool vec = p.R % 16 == 0 && !((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15);
     const int ch = tid % LPR;
     float v[ROWS / STEP][8];
@@ -385,17 +418,17 @@ template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_
         const int row = t * ROWS + i * STEP + tid / LPR;
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[i][u] = 0.f;
-        if (row < p.rows) {
+        if (row < tile.rows) {
             const int s = row / p.G;
-            const size_t angle = (f * p.tokens + (size_t)w * p.S + s) * p.R;
-            rotated8<T, false>(static_cast<const T*>(p.q) + (((size_t)w * p.Hq + h * p.G + row - s * p.G) * p.S + s) * E, p.cos + angle, p.sin + angle, 8 * ch,
-                               p.R, vec, v[i]);
+            const size_t angle = (f * p.tokens + tile.tok0 + s) * p.angles;
+            rotated8<T, false>(static_cast<const T*>(p.q) + out_row(p, tile.tok0, h * p.G + row - s * p.G, s) * E, p.cos + angle, p.sin + angle, 8 * ch, p.R, vec,
+                               v[i]);
         }
     }
     for (int s = s0; s <= s1; ++s) sp = max(sp, turn_seen(L, __ldg(loc + s), off, p.cap));
     if (sp == 0) return;  // nobody reads the turn
     if (h == 0 && tid < 32) {
-        const int row = t * ROWS + tid, see = tid < ROWS && row < p.rows ? turn_seen(L, __ldg(loc + row / p.G), off, p.cap) : sp;
+        const int row = t * ROWS + tid, see = tid < ROWS && row < tile.rows ? turn_seen(L, __ldg(loc + row / p.G), off, p.cap) : sp;
         int* dst = reinterpret_cast<int*>(ql + (size_t)fp * C::LIMS);
         if (tid < ROWS) dst[tid] = see;
         const int least = __reduce_min_sync(0xffffffffu, see);
@@ -615,7 +648,7 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
                 if (k < n && l + step > 0 && l < walk.sp) {
                     const int at = p.bs_shift >= 0 ? pos >> p.bs_shift : pos / p.BS;
                     inpage[x] = pos - at * p.BS;
-                    page[x] = __ldg(p.bt + (size_t)walk.w * p.maxb + at);
+                    page[x] = __ldg(p.bt + (size_t)walk.tile.table * p.maxb + at);
                 }
             }
             how = walk.how();
@@ -623,7 +656,7 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
             if (lane == 0) {
                 Q8Stage& d = desc[i % (2 * STAGES)];
                 d.k0 = walk.k0, d.sp = walk.sp;
-                d.w = walk.w, d.t = walk.t, d.hg = hg;
+                d.tok0 = walk.tile.tok0, d.t = walk.tile.t, d.hg = hg, d.rows = walk.tile.rows;
             }
             walk.take(p);
         };
@@ -1046,14 +1079,10 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
             continue;
         }
         // ---- the piece's result ----
-        const int4 item = *reinterpret_cast<const int4*>(&d->w);
-        const int w = item.x, tile0 = item.y * ROWS, h0 = item.z * p.hc;  // its first row, the group's first head
+        const int4 item = *reinterpret_cast<const int4*>(&d->tok0);
+        const int tile0 = item.y * ROWS, h0 = item.z * p.hc;  // its first row, the group's first head
         const bool whole = (how & Q8_WHOLE) != 0;
         const size_t slot = ((size_t)c * 2 + (how & Q8_BEGIN ? 1 : 0)) * p.hc;
-        auto out_row = [&](int head, int row) {  // of `out`; row < p.rows
-            const int s = row / p.G;
-            return ((size_t)w * p.Hq + (h0 + head) * p.G + row - s * p.G) * p.S + s;
-        };
         float f[MT][2];
         float2 ml[MT][2];
 #pragma unroll
@@ -1137,8 +1166,9 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
                 const int i16 = mt * 16 + y * 8 + n, row = tile0 + i16;
-                if (row >= p.rows) continue;
-                const size_t orow = whole ? out_row(hh, row) : (slot + hh) * ROWS + i16;
+                if (row >= item.w) continue;
+                const int tok = row / p.G;
+                const size_t orow = whole ? out_row(p, item.x, (h0 + hh) * p.G + row - tok * p.G, tok) : (slot + hh) * ROWS + i16;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     const float2 x = make_float2(o[mt][j][2 * y], o[mt][j][2 * y + 1]);
@@ -1174,7 +1204,8 @@ template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_ker
     constexpr int TPR = E / 4, RPB = 256 / TPR;  // threads per row, rows per block
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, h = blockIdx.x % p.Hkv, pair = blockIdx.x / p.Hkv;
-    const int w = p.w0 + pair / p.nt, t = pair % p.nt, hg = h / p.hc, hh = h - hg * p.hc;
+    const Q8Tile tile = tile_of(p, rows, pair);
+    const int t = tile.t, hg = h / p.hc, hh = h - hg * p.hc;
     const float nan = __int_as_float(0x7fc00000);
     const long long P0 = __ldcg(p.P + pair), nw = __ldcg(p.P + pair + 1) - P0, first = P0 * p.hs + hg * nw;
     const bool failed = __ldcg(p.header + 3) != 0;
@@ -1198,9 +1229,9 @@ template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_ker
         }
     }
     const int e = tid % TPR * 4;
-    for (int i = blockIdx.y * RPB + tid / TPR; i < rows && t * rows + i < p.rows; i += gridDim.y * RPB) {
+    for (int i = blockIdx.y * RPB + tid / TPR; i < rows && t * rows + i < tile.rows; i += gridDim.y * RPB) {
         const int row = t * rows + i, s = row / p.G;
-        const size_t orow = ((size_t)w * p.Hq + h * p.G + row - s * p.G) * p.S + s;
+        const size_t orow = out_row(p, tile.tok0, h * p.G + row - s * p.G, s);
         float m = neg_inf(), den = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
         for (int c = c0; c <= c1; c += kQ8Ahead) {
             float2 x[kQ8Ahead];
@@ -1276,17 +1307,32 @@ Q8Kernel q8_pick(int dtype, int E, int rows) {
 
 struct Q8Layout {
     size_t P, cstart, qf, ql, po, pl, total;
-    int ctas, hc, nt, slice;  // slice: sequences of a launch
+    int ctas, hc, nt, slice;  // slice: sequences of a launch (packed: tiles)
+    int items;                // sequences (packed: tiles) of all
 };
-int q8_layout(const dvattn_paged_args* a, const Q8Kernel& k, Q8Layout& L) {
+// Packed tokens: nseq sequences that begin at cu; `a` is the call with a token for a sequence.
+struct Q8Packed {
+    const int* cu;
+    int nseq;
+};
+int q8_rows(const dvattn_paged_args* a, const Q8Packed* pk) {  // query rows of a KV head in a sequence, at most
+    const long long n = (long long)(pk ? a->W : a->S) * (a->Hq / a->Hkv);
+    return (int)(n < 1 << 20 ? n : 1 << 20);
+}
+int q8_layout(const dvattn_paged_args* a, const Q8Packed* pk, const Q8Kernel& k, Q8Layout& L) {
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return DVATTN_ERR_CUDA;
     L.ctas = sms * k.ctas < kQ8MaxCtas ? sms * k.ctas : kQ8MaxCtas;
     L.hc = a->Hkv % 4 == 0 && k.heads == 4 ? 4 : a->Hkv % 2 == 0 ? 2 : 1;
-    L.nt = (a->S * (a->Hq / a->Hkv) + k.rows - 1) / k.rows;
+    L.nt = pk ? 1 : (a->S * (a->Hq / a->Hkv) + k.rows - 1) / k.rows;
+    L.items = pk ? (int)((long long)a->W * (a->Hq / a->Hkv) / k.rows) + pk->nseq + 1 : a->W;
     L.slice = kQ8MaxPairs / L.nt;
-    if (L.slice > a->W) L.slice = a->W;
+    if (pk) {  // 256 MB of fragments are enough to keep the GPU busy
+        const long long fit = (256LL << 20) / ((long long)(a->F > 0 ? a->F : 1) * a->Hkv * k.qhead);
+        if (L.slice > fit) L.slice = fit > 64 ? (int)fit : 64;
+    }
+    if (L.slice > L.items) L.slice = L.items;
     size_t at = 256;
     auto take = [&](size_t bytes) {
         const size_t r = at;
@@ -1306,7 +1352,7 @@ int q8_layout(const dvattn_paged_args* a, const Q8Kernel& k, Q8Layout& L) {
 int q8_validate(const dvattn_paged_args* a) {
     const int st = decode_validate(a);
     if (st != DVATTN_OK) return st;
-    const long long rows = (long long)a->S * (a->Hq / a->Hkv);
+    const long long rows = (long long)a->S * (a->Hq / a->Hkv);  // packed: of a token
     if (a->num_blocks < 0) return DVATTN_ERR_INVALID_ARGUMENT;
     // a sequence's row tiles are one launch's
     if (rows > 16LL * kQ8MaxPairs || (long long)a->F * a->W * a->S > 0x7fffffffLL || (long long)kQ8MaxPairs * a->Hkv * (a->F > 0 ? a->F : 1) > 0x7fffffffLL)
@@ -1340,13 +1386,13 @@ int q8_stall_hook() {
 
 }  // namespace
 
-size_t decode_q8_workspace_size(const dvattn_paged_args* a) {
+static size_t q8_size(const dvattn_paged_args* a, const Q8Packed* pk) {
     if (q8_validate(a) != DVATTN_OK || (long long)a->W * a->S == 0 || a->Hq == 0) return 0;
     Q8Layout L;
-    return q8_layout(a, q8_pick(a->dtype, a->E, a->S * (a->Hq / a->Hkv)), L) == DVATTN_OK ? L.total : 0;
+    return q8_layout(a, pk, q8_pick(a->dtype, a->E, q8_rows(a, pk)), L) == DVATTN_OK ? L.total : 0;
 }
 
-int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream) {
+static int q8_launch(const dvattn_paged_args* a, const Q8Packed* pk, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream) {
     int st = q8_validate(a);
     if (st != DVATTN_OK) return st;
     if (!sc) return DVATTN_ERR_INVALID_ARGUMENT;
@@ -1357,17 +1403,20 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
         return DVATTN_ERR_INVALID_ARGUMENT;
     for (const void* x : {a->queries, a->k_cache, a->v_cache, (const void*)a->out, (const void*)a->out_f32})
         if (reinterpret_cast<uintptr_t>(x) & 15) return DVATTN_ERR_INVALID_ARGUMENT;
-    const Q8Kernel k = q8_pick(a->dtype, a->E, a->S * (a->Hq / a->Hkv));
+    const Q8Kernel k = q8_pick(a->dtype, a->E, q8_rows(a, pk));
     Q8Layout L;
-    if ((st = q8_layout(a, k, L)) != DVATTN_OK) return st;
+    if ((st = q8_layout(a, pk, k, L)) != DVATTN_OK) return st;
     if (!workspace || wbytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return DVATTN_ERR_WORKSPACE;
     char* ws = static_cast<char*>(workspace);
     Q8Params p{};
     p.F = a->F; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.S = a->S; p.R = a->R;
     p.rows = p.S * p.G;
+    p.sh = pk ? 1 : a->S, p.ss = pk ? a->Hq : 1;
+    p.angles = pk ? a->R / 2 : a->R;
+    p.cu = pk ? pk->cu : nullptr, p.nseq = pk ? pk->nseq : 0;
     p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
     const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
-    p.cap = a->num_blocks <= 0 ? 0 : cap > kMostPositions ? kMostPositions : (int)cap;
+    p.cap = a->num_blocks <= 0 || (pk && pk->nseq == 0) ? 0 : cap > kMostPositions ? kMostPositions : (int)cap;
     p.hc = L.hc; p.hs = a->Hkv / L.hc; p.nt = L.nt; p.groups = L.ctas;
     p.kt = k.krows / L.hc;
     p.tokens = (long long)a->W * a->S;
@@ -1413,9 +1462,9 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
     cfg.numAttrs = 1;
     cfg.stream = stream;
     cudaError_t e = cudaSuccess;
-    for (int w = 0; w < a->W && e == cudaSuccess; w += L.slice) {
+    for (int w = 0; w < L.items && e == cudaSuccess; w += L.slice) {
         p.w0 = w;
-        p.W = a->W - w < L.slice ? a->W - w : L.slice;
+        p.W = L.items - w < L.slice ? L.items - w : L.slice;
         p.pairs = p.W * p.nt;
         int rows = k.rows, ctas = L.ctas;
         void* rargs[] = {&p, &qf, &ql};
@@ -1444,6 +1493,20 @@ int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, voi
         return DVATTN_ERR_CUDA;
     }
     return cudaGetLastError() == cudaSuccess ? DVATTN_OK : DVATTN_ERR_CUDA;
+}
+
+size_t decode_q8_workspace_size(const dvattn_paged_args* a) { return q8_size(a, nullptr); }
+int decode_q8_launch(const dvattn_paged_args* a, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream) {
+    return q8_launch(a, nullptr, sc, workspace, wbytes, stream);
+}
+size_t packed_q8_workspace_size(const dvattn_paged_args* tokens, const int* cu, int nseq) {
+    const Q8Packed pk{cu, nseq};
+    return q8_size(tokens, &pk);
+}
+int packed_q8_launch(const dvattn_paged_args* tokens, const int* cu, int nseq, const dvattn_q8_scales* sc, void* workspace, size_t wbytes,
+                     cudaStream_t stream) {
+    const Q8Packed pk{cu, nseq};
+    return q8_launch(tokens, &pk, sc, workspace, wbytes, stream);
 }
 
 }  // namespace dvb

@@ -1,12 +1,15 @@
-// Packed chunked prefill over a paged cache held in 8 bits (q8.cuh): the pages that the call's tokens see are
-// widened to the queries' type in the workspace (value x scale, rounded once: exact in bf16, and in f16 within
-// its range, for the scales that the append sets; f16 values past the range saturate), then
-// the 16-bit (32-bit) varlen attention runs over them.
+// Packed chunked prefill over a paged cache held in 8 bits (q8.cuh).
 //
-// A prefill is bound by its products, 4 E flops for every (query head, key) pair; widening a key costs
+// Calls that the 16-bit attention gives to its tensor-core prefill: the pages that the call's tokens see are
+// widened to the queries' type in the workspace (value x scale, rounded once: exact in bf16, and in f16 within
+// its range, for the scales that the append sets; f16 values past the range saturate), then it runs over them.
+// Such a prefill is bound by its products, 4 E flops for every (query head, key) pair; widening a key costs
 // 2 E (1 + sizeof T) bytes once per KV head, the time of a few tokens' products.  The same widening inside the
 // attention kernel, per window and work item, would be done again for every 16 tokens.  Eight chunks of up to 777 tokens
 // behind up to 8192 keys, 32 / 2 heads of 128, bf16: 19 us of 309 (span 3.5, widening 15.5, of which HBM needs 7.5).
+//
+// All others (32-bit queries, head dims 64 and 256, odd pages, few tokens): the decode attention over the cache as it is, its row
+// tiles cut from the packed tokens.  TODO
 #include "decode.cuh"
 #include "q8.cuh"
 #include "turns.cuh"
@@ -132,15 +135,16 @@ struct WidenLayout {
     bool own_table;
     dvattn_varlen_args wide;  // the call over the widened caches
 };
+// false: not a call for the tensor-core prefill
 bool widen_layout(const dvattn_varlen_args* a, WidenLayout& L) {
     const long long mine = (long long)a->W * a->max_blocks_per_seq;
     L.own_table = mine < a->num_blocks;
     L.pages = L.own_table ? mine : a->num_blocks;
     L.wide = *a;
     L.wide.num_blocks = L.pages;
-    L.own = varlen_workspace_size(&L.wide);
-    if (L.own == 0) return false;
-    const size_t cache = (size_t)L.pages * a->block_size * a->Hkv * a->E * (a->dtype == DVATTN_FLOAT32 ? 4 : 2);
+    if (!prefill_eligible(&L.wide)) return false;
+    L.own = prefill_workspace_size(&L.wide);
+    const size_t cache = (size_t)L.pages * a->block_size * a->Hkv * a->E * 2;
     L.span = up(L.own);
     L.table = L.span + up(4 * (size_t)a->W * a->F);
     L.wk = L.table + (L.own_table ? up(4 * (size_t)mine) : 0);
@@ -148,22 +152,35 @@ bool widen_layout(const dvattn_varlen_args* a, WidenLayout& L) {
     L.total = L.wv + up(cache);
     return true;
 }
-int widen_validate(const dvattn_varlen_args* a) {
-    if (!a || a->W < 0 || a->T < 0 || a->num_blocks < 0) return DVATTN_ERR_INVALID_ARGUMENT;
+// A call of one token for each sequence.
+dvattn_paged_args tokens_of(const dvattn_varlen_args* a) {
     dvattn_paged_args v{};
     v.dtype = a->dtype; v.F = a->F; v.W = a->T; v.Hq = a->Hq; v.Hkv = a->Hkv; v.E = a->E; v.Ev = a->Ev; v.S = 1; v.R = a->R;
-    v.block_size = a->block_size; v.max_blocks_per_seq = a->max_blocks_per_seq; v.num_blocks = a->num_blocks;
+    v.block_size = a->block_size; v.max_blocks_per_seq = a->max_blocks_per_seq; v.num_blocks = a->num_blocks; v.scale = a->scale;
+    v.out = a->out; v.queries = a->queries; v.cosines = a->cosines; v.sines = a->sines; v.locations = a->locations;
+    v.fragment_lengths = a->fragment_lengths; v.k_cache = a->k_cache; v.v_cache = a->v_cache; v.block_tables = a->block_tables;
+    v.lse_out = a->lse_out; v.out_f32 = a->out_f32;
+    return v;
+}
+int widen_validate(const dvattn_varlen_args* a) {
+    if (!a || a->W < 0 || a->T < 0 || a->num_blocks < 0) return DVATTN_ERR_INVALID_ARGUMENT;
+    const dvattn_paged_args v = tokens_of(a);
     const int st = decode_validate(&v);
     if (st != DVATTN_OK) return st;
     // tables are indexed in 32 bits where they are the workspace's; turns are a grid's y
-    return (long long)a->W * a->max_blocks_per_seq > 0x7fffffffLL || a->F > 65535 ? DVATTN_ERR_UNSUPPORTED : DVATTN_OK;
+    return (long long)a->W * a->max_blocks_per_seq > 0x7fffffffLL || a->F > 65535 ||
+                   (long long)a->T * (a->Hq / a->Hkv) > 0x7fffff00LL
+               ? DVATTN_ERR_UNSUPPORTED : DVATTN_OK;
 }
 
 }  // namespace
 
 size_t varlen_q8_workspace_size(const dvattn_varlen_args* a) {
+    if (widen_validate(a) != DVATTN_OK || a->T == 0 || a->Hq == 0) return 0;
     WidenLayout L;
-    return widen_validate(a) == DVATTN_OK && a->T > 0 && a->Hq > 0 && widen_layout(a, L) ? L.total : 0;
+    if (widen_layout(a, L)) return L.total;
+    const dvattn_paged_args v = tokens_of(a);
+    return packed_q8_workspace_size(&v, a->cu_seqlens_q, a->W);
 }
 
 int varlen_q8_launch(const dvattn_varlen_args* a, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream) {
@@ -179,7 +196,10 @@ int varlen_q8_launch(const dvattn_varlen_args* a, const dvattn_q8_scales* sc, vo
     for (const void* x : {a->queries, a->k_cache, a->v_cache, (const void*)a->out, (const void*)a->out_f32})
         if (reinterpret_cast<uintptr_t>(x) & 15) return DVATTN_ERR_INVALID_ARGUMENT;
     WidenLayout L;
-    if (!widen_layout(a, L)) return DVATTN_ERR_UNSUPPORTED;
+    if (!widen_layout(a, L)) {
+        const dvattn_paged_args v = tokens_of(a);
+        return packed_q8_launch(&v, a->cu_seqlens_q, a->W, sc, workspace, wbytes, stream);
+    }
     if (!workspace || wbytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return DVATTN_ERR_WORKSPACE;
     char* ws = static_cast<char*>(workspace);
     L.wide.k_cache = ws + L.wk;
@@ -206,11 +226,8 @@ int varlen_q8_launch(const dvattn_varlen_args* a, const dvattn_q8_scales* sc, vo
         widen_span_kernel<<<dim3((unsigned)((a->T + 255) / 256), (unsigned)a->F), 256, 0, stream>>>(p);
         const long long want = ((long long)a->W * a->max_blocks_per_seq + 7) / 8;
         const unsigned grid = (unsigned)(want < 4LL * sms ? want : 4LL * sms);
-        switch (a->dtype) {
-            case DVATTN_FLOAT16: widen_kernel<__half><<<grid, 256, 0, stream>>>(p); break;
-            case DVATTN_BFLOAT16: widen_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p); break;
-            default: widen_kernel<float><<<grid, 256, 0, stream>>>(p); break;
-        }
+        if (a->dtype == DVATTN_FLOAT16) widen_kernel<__half><<<grid, 256, 0, stream>>>(p);
+        else widen_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
         if (cudaGetLastError() != cudaSuccess) return DVATTN_ERR_CUDA;
     }
     return varlen_launch(&L.wide, workspace, L.own, stream, DVATTN_PHASE_ALL);
