@@ -177,3 +177,43 @@ def test_ranges_of_the_split(dtype):
     for turns in ([[1] * 6] * 9, [[1, 0, 33, 0, 0, 1], [0, 0, 0, 0, 0, 0], [0, 700, 0, 1, 0, 0]], [[5000, 1, 1, 4000]], [[64 * 148]], [[64 * 297, 1]],
                   [[1, 64 * 300], [0, 1]]):
         q8.check(q8.make(turns, 1, 8, 1, 64, 32, 16, dtype))
+
+
+@pytest.mark.parametrize("dtype,E,Hq,Hkv", [(F32, 64, 6, 2), (F32, 256, 5, 1), (F16, 64, 48, 3), (BF16, 256, 8, 2), (BF16, 128, 3, 3)])
+@pytest.mark.parametrize("BS", [16, 6])
+def test_packed_row_tiles(dtype, E, Hq, Hkv, BS):
+    """Row tiles of packed tokens: groups that do not divide a tile, sequences of no, one and many tokens, several turns."""
+    q8.check_varlen(q8.make_varlen([[50, 9], [0, 0], [0, 0], [120, 40], [3, 3], [1, 300]], [5, 1, 0, 37, 2, 64], Hq, Hkv, E, E // 2, BS, dtype, seed=E + BS))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_packed_in_several_launches(dtype):
+    """More row tiles than a launch takes; the same as each sequence in a call of its own."""
+    c = q8.on_gpu(q8.make_varlen([[40], [17], [300]], [3000, 3, 1400], 16, 1, 64, 32, 16, dtype))
+    out, lse = q8.call_varlen(c)
+    assert c["q"].size(0) * 16 // 32 > 2048 and bool(torch.isfinite(out.float()).all())
+    cu = c["cu"].tolist()
+    for w in range(3):
+        at = slice(cu[w], cu[w + 1])
+        one = dict(c, q=c["q"][at].contiguous(), loc=c["loc"][:, at].contiguous(), cos=c["cos"][:, at].contiguous(), sin=c["sin"][:, at].contiguous(),
+                   bt=c["bt"][w:w + 1].contiguous(), cu=torch.tensor([0, cu[w + 1] - cu[w]], dtype=torch.int32, device=DEV))
+        o, l = q8.call_varlen(one)
+        # the split of the keys differs: both are within the bounds of the definition
+        ref = plain_q8.varlen({k: x.cpu() if torch.is_tensor(x) else x for k, x in dict(one, q=one["q"][:40], loc=one["loc"][:, :40], cos=one["cos"][:, :40],
+                                                                                        sin=one["sin"][:, :40], cu=one["cu"].clamp(max=40)).items()})
+        q8.close(one, o[:40], l[:40], *ref)
+        q8.close(one, out[at][:40], lse[at][:40], *ref)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_packed_tokens_outside_the_sequences(dtype):
+    """cu that begins behind the first token or ends before the last one: those tokens have the first sequence's table, in the 16-bit
+    attention as here; cu of no order reads nothing outside."""
+    c = q8.make_varlen([[60], [33]], [20, 12], 8, 2, 64, 32, 16, dtype)
+    for cu in ([3, 20, 30], [0, 0, 0], [0, 32, 32], [9, 9, 40]):
+        q8.check_varlen(dict(c, cu=torch.tensor(cu, dtype=torch.int32)))
+    for cu in ([5, -3, 1000], [32, 16, 0], [-7, 1 << 30, 4]):
+        q8.call_varlen(q8.on_gpu(dict(c, cu=torch.tensor(cu, dtype=torch.int32))))
+    torch.cuda.synchronize()
+    with pytest.raises(Exception):  # tokens and no sequence: the tables are empty, a null pointer, as in the 16-bit attention
+        q8.call_varlen(q8.on_gpu(dict(c, bt=c["bt"][:0], cu=torch.zeros(1, dtype=torch.int32))))
