@@ -43,7 +43,6 @@ struct Q8Params : TurnSplit {
     // of TurnSplit: F, BS, maxb, cap, NB, kt, nt, align, loc, L, bt; W: sequences of this launch
     int w0;                 // its first sequence (packed tokens: its first tile)
     int Hq, Hkv, G, S, R, rows;
-    int sh, ss;             // row of `out` of head h, token s of a sequence: (its first token) Hq + h sh + s ss
     int angles;             // entries of a row of cos / sin
     const int* cu;          // packed tokens: where the sequences begin, [nseq + 1]; null: S tokens of each
     int nseq;
@@ -142,8 +141,9 @@ __device__ __forceinline__ int packed_start(const Q8Params& p, int w) {
     return w <= 0 ? 0 : w > p.nseq ? (int)p.tokens : min(max(__ldg(p.cu + w), 0), (int)p.tokens);
 }
 // Packed: sequence w's tiles are those from floor(first row / size) + w on, which leaves room for them all.
-__device__ __forceinline__ Q8Tile tile_of(const Q8Params& p, int size, int pair) {
-    if (p.cu == nullptr) {
+// PACKED: a template argument throughout, since the search below in every kernel's start costs a call of the other kind 1 to 3 us.
+template <bool PACKED> __device__ __forceinline__ Q8Tile tile_of(const Q8Params& p, int size, int pair) {
+    if constexpr (!PACKED) {
         const int w = p.w0 + pair / p.nt;
         return {w, pair % p.nt, w * p.S, p.rows};
     }
@@ -156,10 +156,13 @@ __device__ __forceinline__ Q8Tile tile_of(const Q8Params& p, int size, int pair)
     const int tok0 = packed_start(p, w), rows = (packed_start(p, w + 1) - tok0) * p.G;
     return {w < p.nseq ? w : 0, x - ((int)((long long)tok0 * p.G / size) + w), tok0, rows};
 }
-__device__ __forceinline__ size_t out_row(const Q8Params& p, int tok0, int head, int s) { return (size_t)tok0 * p.Hq + (size_t)head * p.sh + (size_t)s * p.ss; }
+// of `out`, and of the queries: [token][head] or [sequence][head][token]
+template <bool PACKED> __device__ __forceinline__ size_t out_row(const Q8Params& p, int tok0, int head, int s) {
+    return PACKED ? (size_t)(tok0 + s) * p.Hq + head : (size_t)tok0 * p.Hq + (size_t)head * p.S + s;
+}
 // by one thread: {windows, turns that have any}
-__device__ __forceinline__ int2 pair_windows(const Q8Params& p, int rows, int pair) {
-    const Q8Tile tile = tile_of(p, rows, pair);
+template <bool PACKED> __device__ __forceinline__ int2 pair_windows(const Q8Params& p, int rows, int pair) {
+    const Q8Tile tile = tile_of<PACKED>(p, rows, pair);
     int s0, s1, nw = 0, turns = 0;
     tile.tokens(p, rows, s0, s1);
     if (s0 > s1) return make_int2(0, 0);
@@ -207,7 +210,7 @@ struct Q8Split {
 // What a stage holds: keys [k0, k0 + kt) of a turn of which sp are seen.
 struct alignas(16) Q8Stage {
     int k0, sp, how, pad0;  // how: Q8_* bits, -1: the end
-    int tok0, t, hg, rows;  // of the pair, its head group
+    int pair, hg, pad1, pad2;
 };
 static_assert(sizeof(Q8Stage) == 32, "OFF_DESC");
 constexpr int Q8_ITEM = 1, Q8_TURN = 2, Q8_LAST = 4, Q8_WHOLE = 8, Q8_BEGIN = 16;
@@ -220,8 +223,8 @@ struct alignas(16) Q8Place {
     int begin, pad[3];
 };
 // Unit `rest` of a pair, by a whole warp, a turn per lane: fills in f, i, off and begin; returns the windows in front.
-__device__ __forceinline__ int find_unit(const Q8Params& p, int rows, int lane, int pair, long long rest, Q8Place& at) {
-    const Q8Tile tile = tile_of(p, rows, pair);
+template <bool PACKED> __device__ __forceinline__ int find_unit(const Q8Params& p, int rows, int lane, int pair, long long rest, Q8Place& at) {
+    const Q8Tile tile = tile_of<PACKED>(p, rows, pair);
     int s0, s1, windows = 0;
     tile.tokens(p, rows, s0, s1);
     long long off = 0;
@@ -268,10 +271,10 @@ __device__ __forceinline__ int find_unit(const Q8Params& p, int rows, int lane, 
 }
 
 // Walks the windows of a range by a whole warp; every lane holds the same values.
-struct Q8Walk {
+template <bool PACKED> struct Q8Walk {
     long long rem;
     int pair, hg, f, left;  // left: windows of the turn that are left
-    Q8Tile tile;            // the pair's
+    int table;              // the pair's
     int sp, off, k0;        // the turn's seen keys and first position, the next window's first key
     long long off64;
     bool item, turn;  // the next window begins an item's piece, a turn
@@ -279,7 +282,9 @@ struct Q8Walk {
 
     __device__ __forceinline__ void enter(const Q8Params& p, int rows, int lane) {  // turn f
         const int L = __ldg(p.L + f);
+        const Q8Tile tile = tile_of<PACKED>(p, rows, pair);
         int s0, s1, v = 0;
+        table = tile.table;
         tile.tokens(p, rows, s0, s1);
         for (int s = s0 + lane; s <= s1; s += 32) v = max(v, turn_seen(L, __ldg(p.loc + f * p.tokens + tile.tok0 + s), off64, p.cap));
         sp = __reduce_max_sync(0xffffffffu, v);
@@ -292,7 +297,6 @@ struct Q8Walk {
     // at `at`, for n windows
     __device__ __forceinline__ void start(const Q8Params& p, int rows, int lane, const Q8Place& at, long long n) {
         pair = at.pair, hg = at.hg, rem = n, begin = at.begin != 0, item = true;
-        tile = tile_of(p, rows, pair);
         f = at.f, off64 = at.off;
         enter(p, rows, lane);
         k0 += at.i * p.kt;
@@ -318,7 +322,6 @@ struct Q8Walk {
                         rem = 0;
                         return false;
                     }
-                    tile = tile_of(p, rows, pair);
                 }
             }
             enter(p, rows, lane);
@@ -394,14 +397,14 @@ __device__ const float kOne = 1.f;
 // the attention kernel reads (below), E / 8 lanes per row.  It runs while the attention kernel finds its split and requests
 // its first windows.  By the attention kernel's own warps, a turn took 4 to 10 us, in rounds of loads that few
 // registers allow.
-template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_q8_kernel(const __grid_constant__ Q8Params p, uint8_t* qf, uint8_t* ql) {
+template <class T, int E, int MT, bool PACKED> __global__ void __launch_bounds__(128) rotate_q8_kernel(const __grid_constant__ Q8Params p, uint8_t* qf, uint8_t* ql) {
     using C = Q8Cfg<T, E, MT, false>;
     constexpr int ROWS = C::ROWS, KS = C::KS, LPR = E / 8, STEP = 128 / LPR;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int h = blockIdx.x % p.Hkv, fp = blockIdx.x / p.Hkv, f = fp / p.pairs, pair = fp - f * p.pairs;
     const int tid = threadIdx.x;
-    const Q8Tile tile = tile_of(p, ROWS, pair);
+    const Q8Tile tile = tile_of<PACKED>(p, ROWS, pair);
     const int t = tile.t;
     long long off = 0;
     for (int x = 0; x < f; ++x) off += max(__ldg(p.L + x), 0);
@@ -421,7 +424,7 @@ template <class T, int E, int MT> __global__ void __launch_bounds__(128) rotate_
         if (row < tile.rows) {
             const int s = row / p.G;
             const size_t angle = (f * p.tokens + tile.tok0 + s) * p.angles;
-            rotated8<T, false>(static_cast<const T*>(p.q) + out_row(p, tile.tok0, h * p.G + row - s * p.G, s) * E, p.cos + angle, p.sin + angle, 8 * ch, p.R, vec,
+            rotated8<T, false>(static_cast<const T*>(p.q) + out_row<PACKED>(p, tile.tok0, h * p.G + row - s * p.G, s) * E, p.cos + angle, p.sin + angle, 8 * ch, p.R, vec,
                                v[i]);
         }
     }
@@ -485,7 +488,7 @@ __device__ __forceinline__ float log_sum(float m, float sum) {
 //   key(t, j) = 8 (t / 2) + 2 (t % 2) + j / 2 + 4 (j % 2) for tile j / 2, column 2t + j % 2.  Neighbouring columns lie four rows
 //   apart and eight rows in a row differ, which the 128-byte swizzle puts in different banks, and a thread's
 //   four keys lie in 8 neighbouring rows: one page, one scale.
-template <class T, int E, int MT, bool GATHER>
+template <class T, int E, int MT, bool GATHER, bool PACKED>
 __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, E, MT, GATHER>::CTAS))
     decode_q8_kernel(const __grid_constant__ Q8Params p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
     using C = Q8Cfg<T, E, MT, GATHER>;
@@ -528,7 +531,7 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
     long long carry = 0, carry_u = 0;
     for (int base = 0; base < p.pairs; base += NTH) {
         const int pair = base + tid;
-        const int2 own = pair < p.pairs ? pair_windows(p, ROWS, pair) : make_int2(0, 0);
+        const int2 own = pair < p.pairs ? pair_windows<PACKED>(p, ROWS, pair) : make_int2(0, 0);
         const long long own_u = own.x + (long long)kQ8TurnCost * own.y;
         long long x = own.x, u = own_u;
 #pragma unroll
@@ -564,7 +567,7 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
             const long long local = u - sU[pair] * p.hs, units = sU[pair + 1] - sU[pair];
             at.pair = pair, at.hg = (int)Q8Split::over(local, units);
             at.before = sP[pair] * p.hs + at.hg * (sP[pair + 1] - sP[pair]);
-            at.before += find_unit(p, ROWS, lane, pair, local - at.hg * units, at);
+            at.before += find_unit<PACKED>(p, ROWS, lane, pair, local - at.hg * units, at);
         }
         if (lane == 0) {
             place[wid] = at;
@@ -601,7 +604,7 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
             return true;
         };
         if (!C::THREE && wid == kQ8Warps + 1) {  // a warp of its own for them
-            Q8Walk walk;
+            Q8Walk<PACKED> walk;
             walk.start(p, ROWS, lane, from, count);
             bool ended;
             for (int n = 0; walk.seek(p, ROWS, lane, ended); ++n) {
@@ -631,7 +634,7 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
         const float* sbase = (lane < per ? p.ks : p.vs) + (sy & (p.hc - 1));
         const uint32_t sat = s0 + (uint32_t)(C::OFF_SC + 4 * (sy + (lane < per ? 0 : C::SCALES)));
         const int sbox = (sy >> hc_shift) * 8 >> p.box_shift & 31;
-        Q8Walk walk;
+        Q8Walk<PACKED> walk;
         walk.start(p, ROWS, lane, from, count);
         // of the next window: lane's box, or (gathered) keys lane + 32 x: its page (-1: none) and row there
         constexpr int NX = GATHER ? 4 : 1;
@@ -648,7 +651,7 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
                 if (k < n && l + step > 0 && l < walk.sp) {
                     const int at = p.bs_shift >= 0 ? pos >> p.bs_shift : pos / p.BS;
                     inpage[x] = pos - at * p.BS;
-                    page[x] = __ldg(p.bt + (size_t)walk.tile.table * p.maxb + at);
+                    page[x] = __ldg(p.bt + (size_t)walk.table * p.maxb + at);
                 }
             }
             how = walk.how();
@@ -656,7 +659,7 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
             if (lane == 0) {
                 Q8Stage& d = desc[i % (2 * STAGES)];
                 d.k0 = walk.k0, d.sp = walk.sp;
-                d.tok0 = walk.tile.tok0, d.t = walk.tile.t, d.hg = hg, d.rows = walk.tile.rows;
+                d.pair = walk.pair, d.hg = hg;
             }
             walk.take(p);
         };
@@ -1079,8 +1082,9 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
             continue;
         }
         // ---- the piece's result ----
-        const int4 item = *reinterpret_cast<const int4*>(&d->tok0);
-        const int tile0 = item.y * ROWS, h0 = item.z * p.hc;  // its first row, the group's first head
+        const int2 item = *reinterpret_cast<const int2*>(&d->pair);
+        const Q8Tile tile = tile_of<PACKED>(p, ROWS, item.x);
+        const int tile0 = tile.t * ROWS, h0 = item.y * p.hc;  // its first row, the group's first head
         const bool whole = (how & Q8_WHOLE) != 0;
         const size_t slot = ((size_t)c * 2 + (how & Q8_BEGIN ? 1 : 0)) * p.hc;
         float f[MT][2];
@@ -1166,9 +1170,9 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
                 const int i16 = mt * 16 + y * 8 + n, row = tile0 + i16;
-                if (row >= item.w) continue;
+                if (row >= tile.rows) continue;
                 const int tok = row / p.G;
-                const size_t orow = whole ? out_row(p, item.x, (h0 + hh) * p.G + row - tok * p.G, tok) : (slot + hh) * ROWS + i16;
+                const size_t orow = whole ? out_row<PACKED>(p, tile.tok0, (h0 + hh) * p.G + row - tok * p.G, tok) : (slot + hh) * ROWS + i16;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     const float2 x = make_float2(o[mt][j][2 * y], o[mt][j][2 * y + 1]);
@@ -1200,11 +1204,11 @@ constexpr int kQ8Ahead = 4, kQ8MaxCtas = 1023;
 // 2^x of a part's weight: ex2.approx is 2 ulp off, which shows in 32 bits.
 template <class T> __device__ __forceinline__ float weight(float x) { return sizeof(T) == 4 ? exp2f(x) : fast_exp2(x); }
 
-template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_kernel(const __grid_constant__ Q8Params p, int rows, int ctas) {
+template <class T, int E, bool PACKED> __global__ void __launch_bounds__(256, 4) merge_q8_kernel(const __grid_constant__ Q8Params p, int rows, int ctas) {
     constexpr int TPR = E / 4, RPB = 256 / TPR;  // threads per row, rows per block
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, h = blockIdx.x % p.Hkv, pair = blockIdx.x / p.Hkv;
-    const Q8Tile tile = tile_of(p, rows, pair);
+    const Q8Tile tile = tile_of<PACKED>(p, rows, pair);
     const int t = tile.t, hg = h / p.hc, hh = h - hg * p.hc;
     const float nan = __int_as_float(0x7fc00000);
     const long long P0 = __ldcg(p.P + pair), nw = __ldcg(p.P + pair + 1) - P0, first = P0 * p.hs + hg * nw;
@@ -1231,7 +1235,7 @@ template <class T, int E> __global__ void __launch_bounds__(256, 4) merge_q8_ker
     const int e = tid % TPR * 4;
     for (int i = blockIdx.y * RPB + tid / TPR; i < rows && t * rows + i < tile.rows; i += gridDim.y * RPB) {
         const int row = t * rows + i, s = row / p.G;
-        const size_t orow = out_row(p, tile.tok0, h * p.G + row - s * p.G, s);
+        const size_t orow = out_row<PACKED>(p, tile.tok0, h * p.G + row - s * p.G, s);
         float m = neg_inf(), den = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
         for (int c = c0; c <= c1; c += kQ8Ahead) {
             float2 x[kQ8Ahead];
@@ -1286,23 +1290,24 @@ struct Q8Kernel {
     int krows, rows, ctas, heads, threads;  // CTAs per SM, KV heads of one at most
     size_t smem[2];
 };
-template <class T, int E, int MT> Q8Kernel q8_kernel() {
+template <class T, int E, int MT, bool PACKED> Q8Kernel q8_kernel() {
     using C = Q8Cfg<T, E, MT, false>;
     using G = Q8Cfg<T, E, MT, true>;
     static_assert(C::KROWS == G::KROWS && C::CTAS == G::CTAS && C::HEADS == G::HEADS, "one layout");
-    return {{(const void*)&decode_q8_kernel<T, E, MT, false>, (const void*)&decode_q8_kernel<T, E, MT, true>}, (const void*)&rotate_q8_kernel<T, E, MT>,
-            (const void*)&merge_q8_kernel<T, E>, C::QHEAD, C::LIMS, C::KROWS, C::ROWS, C::CTAS, C::HEADS, C::THREADS, {C::SMEM, G::SMEM}};
+    return {{(const void*)&decode_q8_kernel<T, E, MT, false, PACKED>, (const void*)&decode_q8_kernel<T, E, MT, true, PACKED>},
+            (const void*)&rotate_q8_kernel<T, E, MT, PACKED>, (const void*)&merge_q8_kernel<T, E, PACKED>,
+            C::QHEAD, C::LIMS, C::KROWS, C::ROWS, C::CTAS, C::HEADS, C::THREADS, {C::SMEM, G::SMEM}};
 }
 // One 16-row tile, or two where a KV head has more query rows (then the cache is read half as often); two
 // tiles do not fit in the registers with 32-bit queries or head dim 256.
-template <class T> Q8Kernel q8_pick_t(int E, int rows) {
+template <class T, bool PACKED> Q8Kernel q8_pick_t(int E, int rows) {
     if constexpr (sizeof(T) == 2)
-        if (rows > 16 && E <= 128) return E == 64 ? q8_kernel<T, 64, 2>() : q8_kernel<T, 128, 2>();
-    return E == 64 ? q8_kernel<T, 64, 1>() : E == 128 ? q8_kernel<T, 128, 1>() : q8_kernel<T, 256, 1>();
+        if (rows > 16 && E <= 128) return E == 64 ? q8_kernel<T, 64, 2, PACKED>() : q8_kernel<T, 128, 2, PACKED>();
+    return E == 64 ? q8_kernel<T, 64, 1, PACKED>() : E == 128 ? q8_kernel<T, 128, 1, PACKED>() : q8_kernel<T, 256, 1, PACKED>();
 }
-Q8Kernel q8_pick(int dtype, int E, int rows) {
-    return dtype == DVATTN_FLOAT32   ? q8_pick_t<float>(E, rows)
-           : dtype == DVATTN_FLOAT16 ? q8_pick_t<__half>(E, rows) : q8_pick_t<__nv_bfloat16>(E, rows);
+template <bool PACKED> Q8Kernel q8_pick(int dtype, int E, int rows) {
+    return dtype == DVATTN_FLOAT32   ? q8_pick_t<float, PACKED>(E, rows)
+           : dtype == DVATTN_FLOAT16 ? q8_pick_t<__half, PACKED>(E, rows) : q8_pick_t<__nv_bfloat16, PACKED>(E, rows);
 }
 
 struct Q8Layout {
@@ -1315,9 +1320,10 @@ struct Q8Packed {
     const int* cu;
     int nseq;
 };
-int q8_rows(const dvattn_paged_args* a, const Q8Packed* pk) {  // query rows of a KV head in a sequence, at most
+Q8Kernel q8_of(const dvattn_paged_args* a, const Q8Packed* pk) {  // by the query rows of a KV head in a sequence, at most
     const long long n = (long long)(pk ? a->W : a->S) * (a->Hq / a->Hkv);
-    return (int)(n < 1 << 20 ? n : 1 << 20);
+    const int rows = (int)(n < 1 << 20 ? n : 1 << 20);
+    return pk ? q8_pick<true>(a->dtype, a->E, rows) : q8_pick<false>(a->dtype, a->E, rows);
 }
 int q8_layout(const dvattn_paged_args* a, const Q8Packed* pk, const Q8Kernel& k, Q8Layout& L) {
     int dev = 0, sms = 0;
@@ -1389,7 +1395,7 @@ int q8_stall_hook() {
 static size_t q8_size(const dvattn_paged_args* a, const Q8Packed* pk) {
     if (q8_validate(a) != DVATTN_OK || (long long)a->W * a->S == 0 || a->Hq == 0) return 0;
     Q8Layout L;
-    return q8_layout(a, pk, q8_pick(a->dtype, a->E, q8_rows(a, pk)), L) == DVATTN_OK ? L.total : 0;
+    return q8_layout(a, pk, q8_of(a, pk), L) == DVATTN_OK ? L.total : 0;
 }
 
 static int q8_launch(const dvattn_paged_args* a, const Q8Packed* pk, const dvattn_q8_scales* sc, void* workspace, size_t wbytes, cudaStream_t stream) {
@@ -1403,7 +1409,7 @@ static int q8_launch(const dvattn_paged_args* a, const Q8Packed* pk, const dvatt
         return DVATTN_ERR_INVALID_ARGUMENT;
     for (const void* x : {a->queries, a->k_cache, a->v_cache, (const void*)a->out, (const void*)a->out_f32})
         if (reinterpret_cast<uintptr_t>(x) & 15) return DVATTN_ERR_INVALID_ARGUMENT;
-    const Q8Kernel k = q8_pick(a->dtype, a->E, q8_rows(a, pk));
+    const Q8Kernel k = q8_of(a, pk);
     Q8Layout L;
     if ((st = q8_layout(a, pk, k, L)) != DVATTN_OK) return st;
     if (!workspace || wbytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return DVATTN_ERR_WORKSPACE;
@@ -1411,7 +1417,6 @@ static int q8_launch(const dvattn_paged_args* a, const Q8Packed* pk, const dvatt
     Q8Params p{};
     p.F = a->F; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.S = a->S; p.R = a->R;
     p.rows = p.S * p.G;
-    p.sh = pk ? 1 : a->S, p.ss = pk ? a->Hq : 1;
     p.angles = pk ? a->R / 2 : a->R;
     p.cu = pk ? pk->cu : nullptr, p.nseq = pk ? pk->nseq : 0;
     p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
