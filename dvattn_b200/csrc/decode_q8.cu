@@ -101,8 +101,8 @@ template <class T, int E, int MT, bool GATHER> struct Q8Cfg {
     static constexpr int LIMS = (ROWS + 4) * 4;                       // what the rows of a tile see, and the least of it
     static constexpr int QBUF = HEADS * QHEAD + LIMS, QBYTES = QBUFS * QBUF;
     static constexpr int CTAS = THREE ? 3 : QBYTES + 4 * TENSOR > 101 * 1024 ? 1 : 2;  // per SM
-    static constexpr int LIMIT = CTAS == 3 ? 76800 : CTAS == 2 ? 115712 : 232448;
-    static constexpr int THREADS = THREE ? 160 : 256;              // shared memory of each
+    static constexpr int LIMIT = CTAS == 3 ? 76800 : CTAS == 2 ? 115712 : 232448;     // shared memory of each
+    static constexpr int THREADS = THREE ? 160 : 256;
     // Two CTAs of an SM have 128 registers a thread at their launch; the computing warpgroup takes what the other one
     // gives up.
     static constexpr int REGS = QREG ? 200 : 208, FEW = 2 * 128 - REGS;
@@ -210,7 +210,7 @@ struct Q8Split {
 // What a stage holds: keys [k0, k0 + kt) of a turn of which sp are seen.
 struct alignas(16) Q8Stage {
     int k0, sp, how, pad0;  // how: Q8_* bits, -1: the end
-    int pair, hg, pad1, pad2;
+    int pair, hg, pad1, pad2;  // what its rows are of
 };
 static_assert(sizeof(Q8Stage) == 32, "OFF_DESC");
 constexpr int Q8_ITEM = 1, Q8_TURN = 2, Q8_LAST = 4, Q8_WHOLE = 8, Q8_BEGIN = 16;
@@ -475,7 +475,7 @@ __device__ __forceinline__ float log_sum(float m, float sum) {
 }
 
 // ---- the attention kernel ---------------------------------------------------------------------
-// Warps 0 .. 3 compute, warp 4 requests the windows.  Warp w works on head w % hc of the group and keys
+// Warps 0 .. 3 compute, warp 4 requests the windows and, with 160 threads, the rotated queries (else warp 5).  Warp w works on head w % hc of the group and keys
 // [KPW (w / hc), + KPW) of the window; thread (n, t) = (lane / 4, lane % 4).
 //
 // Fragments.  The order of the elements in q . k and of the keys in P V is free as long as both operands

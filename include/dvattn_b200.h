@@ -506,10 +506,12 @@ int dvattn_paged_evict(const dvattn_evict_args* args, void* workspace, size_t wo
  * output's); the S tokens of a sequence share the reading of its keys.  Workspace and status as
  * there.  What lies in a key or value reaches the tokens that see it and no other, NaN too.
  *
- * dvattn_varlen_paged_sdpa_q8: dvattn_varlen_paged_sdpa over such a cache.  The pages that the
- * tokens see are first widened to dtype in the workspace (min(num_blocks, W * max_blocks) pages of both
- * caches), so the products run as in the 16-bit prefill; tokens and cu_seqlens are treated as there.
- * A page that several sequences share is meant the same to all of them.
+ * dvattn_varlen_paged_sdpa_q8: dvattn_varlen_paged_sdpa over such a cache; tokens and cu_seqlens_q (in
+ * order) are treated as there.  Where the 16-bit call would take its tensor-core prefill, the pages that the
+ * tokens see are widened to dtype in the workspace (min(num_blocks, W * max_blocks) pages of both caches)
+ * and it runs over them; then a NaN or infinity in a page may reach other tokens of its sequence, as in
+ * that prefill.  Other calls read the cache as it is, in row tiles of the packed tokens (workspace: at most
+ * about 256 MB of rotated queries).
  *
  * dvattn_paged_append_q8: dvattn_paged_append into such a cache.  Keys (rotated, rounded to dtype) and
  * values x of a page and head are stored as e4m3(x / s), to nearest even, with s the page's scale: the
