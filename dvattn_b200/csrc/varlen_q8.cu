@@ -170,9 +170,10 @@ int widen_validate(const dvattn_varlen_args* a) {
     const dvattn_paged_args v = tokens_of(a);
     const int st = decode_validate(&v);
     if (st != DVATTN_OK) return st;
-    // tables are indexed in 32 bits where they are the workspace's; turns are a grid's y
+    // tables are indexed in 32 bits where they are the workspace's; turns are a grid's y; row tiles, and one more for every
+    // sequence, are counted in 32 bits
     return (long long)a->W * a->max_blocks_per_seq > 0x7fffffffLL || a->F > 65535 ||
-                   (long long)a->T * (a->Hq / a->Hkv) > 0x7fffff00LL
+                   (long long)a->T * (a->Hq / a->Hkv) > 0x7fffff00LL || a->W > 1 << 30
                ? DVATTN_ERR_UNSUPPORTED : DVATTN_OK;
 }
 

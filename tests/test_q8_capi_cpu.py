@@ -49,9 +49,9 @@ COMMON = [(dict(dtype=7), UNSUPPORTED), (dict(dtype=-1), UNSUPPORTED), (dict(E=9
 
 
 @pytest.mark.parametrize("name,make,kw,status",
-                         [("dvattn_paged_sdpa_q8", paged, kw, st) for kw, st in COMMON + [(dict(S=-1), INVALID)]] +
+                         [("dvattn_paged_sdpa_q8", paged, kw, st) for kw, st in COMMON + [(dict(S=-1), INVALID), (dict(S=2049), UNSUPPORTED), (dict(F=1 << 20, S=1 << 11), UNSUPPORTED)]] +
                          [("dvattn_varlen_paged_sdpa_q8", varlen, kw, st) for kw, st in COMMON + [
-                             (dict(T=-1), INVALID), (dict(F=65536), UNSUPPORTED),
+                             (dict(T=-1), INVALID), (dict(F=65536), UNSUPPORTED), (dict(T=1 << 28), UNSUPPORTED), (dict(W=(1 << 30) + 1, max_blocks_per_seq=1), UNSUPPORTED),
                              (dict(W=1 << 16, max_blocks_per_seq=1 << 16), UNSUPPORTED)]])
 def test_attention(name, make, kw, status):
     """dict(): sizes in order, but null pointers."""

@@ -217,3 +217,9 @@ def test_packed_tokens_outside_the_sequences(dtype):
     torch.cuda.synchronize()
     with pytest.raises(Exception):  # tokens and no sequence: the tables are empty, a null pointer, as in the 16-bit attention
         q8.call_varlen(q8.on_gpu(dict(c, bt=c["bt"][:0], cu=torch.zeros(1, dtype=torch.int32))))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_most_rows_of_a_sequence(dtype):
+    """2048 tokens of 16 query heads to a KV head: as many row tiles as a launch takes, a sequence a launch."""
+    q8.check(q8.make([[2100], [2060]], 2048, 16, 1, 64, 32, 16, dtype))
