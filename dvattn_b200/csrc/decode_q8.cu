@@ -350,11 +350,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-    return v;
-}
 __device__ __forceinline__ float lds_f32(uint32_t a) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
@@ -1422,7 +1417,7 @@ static int q8_launch(const dvattn_paged_args* a, const Q8Packed* pk, const dvatt
     p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.NB = a->num_blocks;
     const long long cap = (long long)a->max_blocks_per_seq * a->block_size;
     p.cap = a->num_blocks <= 0 || (pk && pk->nseq == 0) ? 0 : cap > kMostPositions ? kMostPositions : (int)cap;
-    p.hc = L.hc; p.hs = a->Hkv / L.hc; p.nt = L.nt; p.groups = L.ctas;
+    p.hc = L.hc; p.hs = a->Hkv / L.hc; p.nt = L.nt;
     p.kt = k.krows / L.hc;
     p.tokens = (long long)a->W * a->S;
     p.scale_log2 = a->scale * kLog2e;
