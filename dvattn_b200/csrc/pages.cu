@@ -136,6 +136,7 @@ __device__ __forceinline__ int own_part(const Chunk& c, unsigned mask, int base)
 
 template <bool ASSIGN> __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) pages_kernel(PageParams p) {
     cg::cluster_group cluster = cg::this_cluster();
+    cluster.barrier_arrive();  // every block arrives once it runs: others write into its shared memory only after that
     __shared__ int warp_sum[kWarps];
     __shared__ int block_sum[2][kBlocks], block_used[kBlocks];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, rank = (int)cluster.block_rank(), me = rank * kWarps + wid;
@@ -167,6 +168,7 @@ template <bool ASSIGN> __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_
             if (i < wid) before += warp_sum[i];
             sum += warp_sum[i];
         }
+        if (buffer == 0) cluster.barrier_wait();  // all blocks run (the first use of their shared memory)
         if (threadIdx.x < kBlocks) *cluster.map_shared_rank(&block_sum[buffer][rank], threadIdx.x) = sum;
         cluster.sync();
         for (int i = 0; i < kBlocks; ++i) {

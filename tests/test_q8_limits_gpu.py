@@ -223,3 +223,23 @@ def test_packed_tokens_outside_the_sequences(dtype):
 def test_most_rows_of_a_sequence(dtype):
     """2048 tokens of 16 query heads to a KV head: as many row tiles as a launch takes, a sequence a launch."""
     q8.check(q8.make([[2100], [2060]], 2048, 16, 1, 64, 32, 16, dtype))
+
+
+@pytest.mark.parametrize("W", [1, 2, 129, 160, 200, 255])
+def test_pages_of_blocks_without_sequences(W):
+    """Whole blocks of the page kernels' cluster without a sequence, which reach the exchange of counts before the others have walked
+    theirs (or begun): every one of many calls gives what the first does, and the pages come back as they were."""
+    BS, maxb = 16, 60
+    i32 = dict(dtype=torch.int32, device=DEV)
+    starts = torch.arange(W, **i32) % 7 * 13
+    counts = torch.arange(W, **i32) % 5 * 101 + 1
+    bt, count = torch.full((W, maxb), -1, **i32), torch.tensor([W * maxb], **i32)
+    free = torch.arange(W * maxb, **i32)
+    ref = plain_q8.assign(bt.cpu(), free.cpu(), W * maxb, starts.cpu(), counts.cpu(), BS)
+    before = bt.clone(), free.clone(), count.clone()
+    zero = torch.zeros_like(starts)
+    for _ in range(300):
+        granted = dvattn_b200.dvattn_assign_pages(bt, free, count, starts, counts, BS)
+        assert torch.equal(bt.cpu(), ref[0]) and int(count) == ref[1] and torch.equal(granted.cpu(), ref[2])
+        dvattn_b200.dvattn_release_pages(bt, free, count, zero, BS)
+        assert torch.equal(bt, before[0]) and torch.equal(count, before[2]) and torch.equal(free, before[1])
