@@ -269,8 +269,8 @@ __global__ void __launch_bounds__(256) slots_kernel(PageParams p) {
 
 int pages_check(int W, int BS, int maxb, int size) {
     if (W < 0 || BS <= 0 || maxb < 0 || size < 0) return DVATTN_ERR_INVALID_ARGUMENT;
-    // entries and positions are counted in 32 bits
-    if ((long long)W * maxb > 0x7fffffffLL || (long long)maxb * BS > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
+    // entries and positions are counted in 32 bits, entries by walks that step past the last one by up to 32 * kRowAhead
+    if ((long long)W * maxb > 0x7fffffffLL - 2 * 32 * kRowAhead || (long long)maxb * BS > 0x7fffffffLL) return DVATTN_ERR_UNSUPPORTED;
     return DVATTN_OK;
 }
 

@@ -142,3 +142,11 @@ def test_the_python_calls_want_gpu_tensors():
     for call in calls:
         with pytest.raises(Exception):
             call()
+
+
+@pytest.mark.parametrize("name,make", [("dvattn_assign_pages", assign), ("dvattn_release_pages", release)])
+def test_tables_that_a_walk_would_step_past_32_bits(name, make):
+    """A walk's step behind the last of 2^31 - 1 entries does not fit in 32 bits; 1024 entries fewer do (null pointers: refused next)."""
+    for W, most in ((1, 0x7fffffff), (7, 0x7fffffff // 7), (1, 0x7fffffff - 1023)):
+        assert getattr(LIB, name)(ctypes.byref(make(W=W, max_blocks_per_seq=most, block_size=1)), None) == UNSUPPORTED
+    assert getattr(LIB, name)(ctypes.byref(make(W=1, max_blocks_per_seq=0x7fffffff - 1024, block_size=1)), None) == INVALID
