@@ -269,8 +269,9 @@ def dvattn_assign_pages(block_tables: torch.Tensor, free_pages: torch.Tensor, fr
     ``block_tables`` [W,max_blocks] i32 that they fall on and that are negative take one from the free list,
     a stack of free_count [1] i32 page numbers in free_pages [N] i32.  Sequences are served in order; one whose
     pages, with those of all before it, are not there gets none.  Returns ``granted`` [W] i32: counts[w], or 0
-    for a sequence that was not served (what ``positions`` and ``counts`` of an append take).  ``slots``
-    ([W,n] int64, optional) gets page * block_size + offset of token i < granted[w], -1 elsewhere."""
+    for a sequence that was not served (what ``positions`` and ``counts`` of an append take); it must not be ``starts``
+    or ``counts`` itself.  ``slots`` ([W,n] int64, optional) gets page * block_size + offset of token i < granted[w],
+    -1 elsewhere."""
     if granted is None:
         granted = torch.empty_like(counts)
     _ops.dvattn_assign_pages(block_tables, free_pages, free_count, granted, slots, starts, counts, block_size)

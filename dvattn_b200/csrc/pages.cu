@@ -284,6 +284,9 @@ int assign_pages_launch(const dvattn_assign_args* a, cudaStream_t stream) {
     if (a->W == 0) return DVATTN_OK;
     if (!a->free_count || !a->starts || !a->counts || !a->granted || (a->max_blocks_per_seq > 0 && !a->block_tables) || (a->free_size > 0 && !a->free_pages))
         return DVATTN_ERR_INVALID_ARGUMENT;
+    // several warps read a sequence's start and count while one writes what it is granted
+    for (const int* in : {a->starts, a->counts})
+        if (a->granted < in + a->W && in < a->granted + a->W) return DVATTN_ERR_INVALID_ARGUMENT;
     PageParams p{};
     p.W = a->W; p.BS = a->block_size; p.maxb = a->max_blocks_per_seq; p.size = a->free_size; p.n = a->n;
     p.per = (a->W + kBlocks * kWarps - 1) / (kBlocks * kWarps);

@@ -322,7 +322,7 @@ typedef struct dvattn_assign_args {
     int* free_count;              /* [1] i32, updated                                     */
     const int* starts;            /* [W] i32                                              */
     const int* counts;            /* [W] i32                                              */
-    int* granted;                 /* [W] i32: counts[w], or 0                             */
+    int* granted;                 /* [W] i32: counts[w], or 0; not over starts or counts  */
     long long* slots;             /* optional [W,n] i64: page * block_size + offset of granted
                                      token i < granted[w], -1 behind them and without a page */
 } dvattn_assign_args;

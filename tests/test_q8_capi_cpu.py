@@ -150,3 +150,11 @@ def test_tables_that_a_walk_would_step_past_32_bits(name, make):
     for W, most in ((1, 0x7fffffff), (7, 0x7fffffff // 7), (1, 0x7fffffff - 1023)):
         assert getattr(LIB, name)(ctypes.byref(make(W=W, max_blocks_per_seq=most, block_size=1)), None) == UNSUPPORTED
     assert getattr(LIB, name)(ctypes.byref(make(W=1, max_blocks_per_seq=0x7fffffff - 1024, block_size=1)), None) == INVALID
+
+
+@pytest.mark.parametrize("at", [256, 260, 252])
+@pytest.mark.parametrize("name", ["starts", "counts"])
+def test_granted_counts_over_the_requests(name, at):
+    """Granted counts written where starts or counts are still read (a free list without pages: nothing else would be refused)."""
+    ok = dict(block_tables=4096, free_pages=4096, free_count=4096, starts=1024, counts=2048, granted=256)
+    assert LIB.dvattn_assign_pages(ctypes.byref(assign(**{**ok, name: at})), None) == INVALID
