@@ -87,6 +87,9 @@ __device__ __forceinline__ int turn_vis_pf(int L, int loc, int off, int cap) {
     v = min(v, cap - off);
     return v > 0 ? v : 0;
 }
+// The first position of the turn behind one of length L at `off`: lengths below zero are empty (positions never step back in front of
+// the table), and positions end at the table's end, where nothing is visible (their sum stays within 32 bits).
+__device__ __forceinline__ int turn_next(int off, int L, int cap) { return L <= 0 ? off : L < cap - off ? off + L : cap; }
 
 // ---- work list ---------------------------------------------------------------------
 // Token t belongs to the first sequence w with t < cu_q[w+1], else to sequence 0
@@ -124,7 +127,7 @@ __global__ void __launch_bounds__(1024) prefill_prep_kernel(Params p) {
             int off = 0;
             for (int f = 0; f < p.F; ++f) {
                 c += turn_vis_pf(p.L[f], p.loc[(size_t)f * p.T + last], off, p.cap);
-                off += p.L[f];
+                off = turn_next(off, p.L[f], p.cap);
             }
         }
         cost[s] = c;
@@ -185,7 +188,7 @@ struct TileSeq {
                 valid = true;
                 return;
             }
-            off += __ldg(p.L + f);
+            off = turn_next(off, __ldg(p.L + f), p.cap);
         }
         valid = false;
     }
@@ -199,7 +202,7 @@ struct TileSeq {
             win += KT;
             return;
         }
-        off += __ldg(p.L + f);
+        off = turn_next(off, __ldg(p.L + f), p.cap);
         ++f;
         seek(p, it, lane);
     }

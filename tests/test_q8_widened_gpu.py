@@ -1,0 +1,51 @@
+"""The packed prefill over an 8-bit cache on its widening path: the pages that the tokens see widened in the workspace and given to the
+tensor-core prefill.  Small calls are sent there with DVATTN_PREFILL=1, and the workspace's size shows that they went."""
+import pytest
+import torch
+
+import plain_q8
+import test_q8_gpu as q8
+from dvattn_b200 import capi
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def workspace(c):
+    """Bytes that the call asks for, and those of the widened pages of both caches."""
+    a = capi.varlen_args(c["q"], c["scale"], c["loc"], c["q"], c["cos"], c["sin"], c["L"], c["kc"], c["vc"], c["bt"], c["cu"])
+    NB, BS, Hkv, E = c["kc"].shape
+    return capi.lib().dvattn_varlen_paged_sdpa_q8_workspace_size(a), 2 * 2 * min(NB, c["bt"].numel()) * BS * Hkv * E
+
+
+def check(c):
+    """Against the definition, on the widening path."""
+    d = q8.on_gpu(c)
+    size, pages = workspace(d)
+    assert pages <= size < pages + (1 << 20)
+    out, lse = q8.call_varlen(d)
+    torch.cuda.synchronize()
+    q8.close(c, out, lse, *plain_q8.varlen(c), wide=True)
+    return out, lse
+
+
+@pytest.fixture
+def widened(monkeypatch):
+    monkeypatch.setenv("DVATTN_PREFILL", "1")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("extra_pages", [0, 90])
+def test_fragment_lengths_below_zero_and_past_the_table(widened, dtype, extra_pages):
+    """A turn of a length below zero is empty, and a sum of lengths past 2^31 ends at the table's end: the same bits as with lengths that
+    say so plainly."""
+    c = q8.make_varlen([[60, 0, 45], [33, 0, 20]], [9, 30], 8, 2, 128, 32, 16, dtype, extra_pages=extra_pages)
+    positions = c["bt"].size(1) * 16
+    for odd, plain in (([64, -20, 75], [64, 0, 75]), ([-5, -2147483648, 75], [0, 0, 75]), ([2147483647, 2147483647, 64], [positions, 0, 0]),
+                       ([40, 2147483647, 2147483647], [40, positions, 0])):
+        ref = dict(c, L=torch.tensor(plain, dtype=torch.int32), loc=c["loc"].clone())
+        ref["loc"][1] = ref["loc"][2] - 3  # the turn in the middle has keys, where it has a length
+        want = check(ref)
+        got = q8.call_varlen(q8.on_gpu(dict(ref, L=torch.tensor(odd, dtype=torch.int32))))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
