@@ -83,7 +83,7 @@ struct Params {
 };
 
 __device__ __forceinline__ int turn_vis_pf(int L, int loc, int off, int cap) {
-    int v = min(L, loc + 1);
+    int v = loc < L ? loc + 1 : L;  // loc may be the largest number of its type
     v = min(v, cap - off);
     return v > 0 ? v : 0;
 }

@@ -49,3 +49,13 @@ def test_fragment_lengths_below_zero_and_past_the_table(widened, dtype, extra_pa
         want = check(ref)
         got = q8.call_varlen(q8.on_gpu(dict(ref, L=torch.tensor(odd, dtype=torch.int32))))
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_locations(widened, dtype):
+    """Locations of any order and sign, beyond the turn (the largest of all among them), and tokens that see nothing."""
+    c = q8.make_varlen([[60, 45], [33, 20]], [9, 30], 8, 2, 128, 32, 16, dtype)
+    c["loc"][0, ::3], c["loc"][0, 1::4], c["loc"][1, ::5] = 2147483647, -7, 500
+    c["loc"][:, 4], c["loc"][:, 20] = -1, torch.tensor([-2147483648, 2147483647], dtype=torch.int32)
+    out, lse = check(c)
+    assert not out[4].any() and bool((lse[4] == -torch.inf).all())
