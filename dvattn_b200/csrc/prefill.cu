@@ -92,6 +92,9 @@ __device__ __forceinline__ int turn_vis_pf(int L, int loc, int off, int cap) {
 __device__ __forceinline__ int turn_next(int off, int L, int cap) { return L <= 0 ? off : L < cap - off ? off + L : cap; }
 
 // ---- work list ---------------------------------------------------------------------
+// Bytes of shared memory for a segment (a sequence, and the tokens behind the last one), and the sequences for which 48 KB suffice.
+constexpr int SEG_BYTES = sizeof(long long) + 4 * sizeof(int);
+constexpr int MAX_W = 48 * 1024 / SEG_BYTES - 1;
 // Token t belongs to the first sequence w with t < cu_q[w+1], else to sequence 0
 // (varlen_paged_kernel_v21.cuh:40-47).  With a non-decreasing cu_q that gives W + 1
 // contiguous segments: segment w = [w ? cu[w] : 0, cu[w+1]) of sequence w, and segment W
@@ -666,6 +669,7 @@ bool prefill_eligible(const dvattn_varlen_args* v) {
     if (v->R % 16 || v->R > v->E) return false;
     const int BS = v->block_size;
     if (!(BS == 8 || BS == 16 || BS == 32 || BS == 64 || BS == 128)) return false;
+    if (v->W > pf::MAX_W) return false;  // the work list is sorted in one block's shared memory
     if (v->num_blocks <= 0 || v->num_blocks * (long long)BS > 0x7fffffffLL) return false;
     // enough items to fill the GPU; short prefills go through the split-KV decode schedule
     return mode == 1 || (long long)v->T * v->Hkv >= 148LL * prefill_tokens_per_item(v);
@@ -707,8 +711,7 @@ int prefill_launch(const dvattn_varlen_args* v, void* workspace, size_t wbytes, 
     p.max_items = prefill_max_items(v);
     p.stall_tile = prefill_stall_hook();
 
-    const size_t prep_smem = (sizeof(long long) + 4 * sizeof(int)) * ((size_t)p.W + 1);
-    if (prep_smem > 48 * 1024) return DVATTN_ERR_UNSUPPORTED;
+    const size_t prep_smem = pf::SEG_BYTES * ((size_t)p.W + 1);
     if (phase == DVATTN_PHASE_ALL || phase == DVATTN_PHASE_SCHEDULE) pf::prefill_prep_kernel<<<1, 1024, prep_smem, stream>>>(p);
     if (phase != DVATTN_PHASE_ALL && phase != DVATTN_PHASE_ATTEND) return cudaGetLastError() == cudaSuccess ? DVATTN_OK : DVATTN_ERR_CUDA;
 

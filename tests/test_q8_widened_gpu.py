@@ -3,6 +3,7 @@ tensor-core prefill.  Small calls are sent there with DVATTN_PREFILL=1, and the 
 import pytest
 import torch
 
+import dvattn_b200
 import plain_q8
 import test_q8_gpu as q8
 from dvattn_b200 import capi
@@ -59,3 +60,18 @@ def test_locations(widened, dtype):
     c["loc"][:, 4], c["loc"][:, 20] = -1, torch.tensor([-2147483648, 2147483647], dtype=torch.int32)
     out, lse = check(c)
     assert not out[4].any() and bool((lse[4] == -torch.inf).all())
+
+
+@pytest.mark.parametrize("W", [2047, 2048, 2100])
+def test_sequences_that_the_prefill_can_sort(widened, W):
+    """2047 sequences are sorted by the tensor-core prefill; with more the call runs without it, over a 16-bit cache, too."""
+    new = [0 if w % 3 == 1 else 2 + w % 2 for w in range(W)]
+    c = q8.make_varlen([[w % 40] for w in range(W)], new, 4, 1, 128, 32, 16, BF16)
+    d = q8.on_gpu(c)
+    size, pages = workspace(d)
+    assert (pages <= size < pages + (1 << 20)) == (W < 2048)
+    out, lse = q8.call_varlen(d)
+    q8.close(c, out, lse, *plain_q8.varlen(c), wide=W < 2048)
+    k, v = [plain_q8.values(c[x], c[y]).to(BF16).to(DEV) for x, y in (("kc", "ks"), ("vc", "vs"))]
+    wide = dvattn_b200.dvattn_varlen_paged_sdpa(d["q"], d["loc"], d["cos"], d["sin"], d["L"], k, v, d["bt"], d["cu"], None, d["scale"])
+    q8.close(c, wide, lse, *plain_q8.varlen(c), wide=True)
