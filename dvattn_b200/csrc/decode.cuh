@@ -55,6 +55,7 @@ size_t sdpa_workspace_size(const dvattn_sdpa_args* a);
 int sdpa_launch(const dvattn_sdpa_args* a, void* workspace, size_t wbytes, cudaStream_t stream);
 // tcgen05 varlen prefill (prefill.cu): used by varlen_launch when prefill_eligible()
 bool prefill_eligible(const dvattn_varlen_args* a);
+bool prefill_forced();  // wherever it can run (DVATTN_PREFILL=1)
 size_t prefill_workspace_size(const dvattn_varlen_args* a);
 int prefill_launch(const dvattn_varlen_args* a, void* workspace, size_t wbytes, cudaStream_t stream, int phase);
 

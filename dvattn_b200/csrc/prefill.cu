@@ -661,6 +661,8 @@ static int prefill_mode() {
     return e && e[0] == '0' ? 0 : e && e[0] == '1' ? 1 : 2;
 }
 
+bool prefill_forced() { return prefill_mode() == 1; }
+
 bool prefill_eligible(const dvattn_varlen_args* v) {
     const int mode = prefill_mode();
     if (mode == 0) return false;

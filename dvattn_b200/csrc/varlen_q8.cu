@@ -1,18 +1,24 @@
 // Packed chunked prefill over a paged cache held in 8 bits (q8.cuh).
 //
-// Calls that the 16-bit attention gives to its tensor-core prefill: the pages that the call's tokens see are
-// widened to the queries' type in the workspace (value x scale, rounded once: exact in bf16, and in f16 within
-// its range, for the scales that the append sets; f16 values past the range saturate), then it runs over them.
-// Such a prefill is bound by its products, 4 E flops for every (query head, key) pair; widening a key costs
-// 2 E (1 + sizeof T) bytes once per KV head, the time of a few tokens' products.  The same widening inside the
+// Calls that the 16-bit attention gives to its tensor-core prefill and whose sequences have many tokens: the pages that
+// the call's tokens see are widened to the queries' type in the workspace (value x scale, rounded once: exact in bf16, and in
+// f16 within its range, for the scales that the append sets; f16 values past the range saturate), then it runs over them.
+// Its products, 4 E flops for every (query head, key) pair, are what bounds it then; widening a key costs
+// 2 E (1 + sizeof T) bytes once per KV head, and reading it again.  The same widening inside the
 // attention kernel, per window and work item, would be done again for every 16 tokens.  Eight chunks of up to 777 tokens
 // behind up to 8192 keys, 32 / 2 heads of 128, bf16: 19 us of 309 (span 3.5, widening 15.5, of which HBM needs 7.5).
 //
 // All others (32-bit queries, head dims 64 and 256, odd pages, few tokens): the decode attention over the cache as it is
 // (decode_q8.cu), its row tiles of 16 or 32 query rows cut from the packed tokens.  1624 tokens of four sequences behind up to 2000
-// keys, 32 / 4 heads: 433 us in f32 (head dim 128), 181 in bf16 with head dim 64.  Where both can run, the tensor cores' tiles of
-// 128 rows win: 114 us against 269 with head dim 128 in bf16, 312 against 1327 in the case above; with too few tokens for them
-// (113) it is 56.
+// keys, 32 / 4 heads: 433 us in f32 (head dim 128), 181 in bf16 with head dim 64; 113 tokens of head dim 128 in bf16 56.
+//
+// Where both can run (kWidenRows): the tiles read a key's byte once for every 32 query rows of its sequence and KV head, the
+// widening five bytes whatever the rows, so the rows of a sequence decide.  The host knows their average.  bf16, head dim 128,
+// keys of 2000 positions in front, widened against row tiles: 592 sequences of one token with 64 / 8 heads 3037 us against 983,
+// 74 of 8 tokens (64 rows) 399 against 261, 37 of 16 (128 rows) 209 against 250, 10 of 64 137 against 269; 32 / 2 heads, 8 tokens
+// (128 rows) 224 against 265, 4 tokens 428 against 284; 8 / 8 heads, 128 tokens 226 against 277, 64 tokens 420 against 276.
+// Behind 8000 keys the two meet at 128 rows (721 and 755).  One sequence of many tokens among others of one (64 / 8 heads): 100
+// beside 1024 tokens (89 rows on average) 676 against 643, 64 beside 2048 (260 rows) 589 against 1189.
 #include "decode.cuh"
 #include "q8.cuh"
 #include "turns.cuh"
@@ -130,6 +136,8 @@ template <class T> __global__ void __launch_bounds__(256) widen_kernel(WidenPara
     }
 }
 
+constexpr int kWidenRows = 128;  // query rows of a sequence and KV head, on average, from which pages are widened (file comment)
+
 size_t up(size_t x) { return (x + 255) / 256 * 256; }
 
 struct WidenLayout {
@@ -140,6 +148,7 @@ struct WidenLayout {
 };
 // false: not a call for the tensor-core prefill
 bool widen_layout(const dvattn_varlen_args* a, WidenLayout& L) {
+    if (!prefill_forced() && (long long)a->T * (a->Hq / a->Hkv) < (long long)kWidenRows * a->W) return false;
     const long long mine = (long long)a->W * a->max_blocks_per_seq;
     L.own_table = mine < a->num_blocks;
     L.pages = L.own_table ? mine : a->num_blocks;

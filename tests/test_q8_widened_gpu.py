@@ -75,3 +75,16 @@ def test_sequences_that_the_prefill_can_sort(widened, W):
     k, v = [plain_q8.values(c[x], c[y]).to(BF16).to(DEV) for x, y in (("kc", "ks"), ("vc", "vs"))]
     wide = dvattn_b200.dvattn_varlen_paged_sdpa(d["q"], d["loc"], d["cos"], d["sin"], d["L"], k, v, d["bt"], d["cu"], None, d["scale"])
     q8.close(c, wide, lse, *plain_q8.varlen(c), wide=True)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new,widens", [([1] * 600, False), ([8] * 74, False), ([16] * 37, True), ([1] * 200 + [400], False), ([1] * 20 + [600], True)])
+def test_rows_of_a_sequence_decide(dtype, new, widens):
+    """64 / 8 heads, enough tokens in all for the tensor-core prefill: pages are widened from 128 query rows (16 tokens) of a KV head in a
+    sequence on average."""
+    c = q8.make_varlen([[w % 30] for w in range(len(new))], new, 64, 8, 128, 32, 16, dtype)
+    d = q8.on_gpu(c)
+    size, pages = workspace(d)
+    assert (pages <= size < pages + (1 << 20)) == widens
+    out, lse = q8.call_varlen(d)
+    q8.close(c, out, lse, *plain_q8.varlen(c), wide=widens)
