@@ -1315,8 +1315,13 @@ struct Q8Packed {
     const int* cu;
     int nseq;
 };
-Q8Kernel q8_of(const dvattn_paged_args* a, const Q8Packed* pk) {  // by the query rows of a KV head in a sequence, at most
-    const long long n = (long long)(pk ? a->W : a->S) * (a->Hq / a->Hkv);
+// By the query rows of a KV head in a sequence, of packed tokens on average (rounded up to whole tokens).  bf16, 64 / 8 heads of 128,
+// two tiles against one: 592 packed sequences of one token behind 2000 keys 983 us against 578, 64 of them 135 against 82, 500 and a chunk
+// of 256 tokens 944 against 602, 30 behind 8000 and a chunk of 28 222 against 149; head dim 64: 587 against 451, with a chunk 567
+// against 474.  By the call's tokens, as without packing, all of these would have two.
+Q8Kernel q8_of(const dvattn_paged_args* a, const Q8Packed* pk) {
+    const int nseq = pk && pk->nseq > 0 ? pk->nseq : 1;
+    const long long n = (pk ? ((long long)a->W + nseq - 1) / nseq : (long long)a->S) * (a->Hq / a->Hkv);
     const int rows = (int)(n < 1 << 20 ? n : 1 << 20);
     return pk ? q8_pick<true>(a->dtype, a->E, rows) : q8_pick<false>(a->dtype, a->E, rows);
 }

@@ -12,9 +12,9 @@
 // (decode_q8.cu), its row tiles of 16 or 32 query rows cut from the packed tokens.  1624 tokens of four sequences behind up to 2000
 // keys, 32 / 4 heads: 433 us in f32 (head dim 128), 181 in bf16 with head dim 64; 113 tokens of head dim 128 in bf16 56.
 //
-// Where both can run (kWidenRows): the tiles read a key's byte once for every 32 query rows of its sequence and KV head, the
+// Where both can run (kWidenRows): the tiles read a key's byte once for every 16 or 32 query rows of its sequence and KV head, the
 // widening five bytes whatever the rows, so the rows of a sequence decide.  The host knows their average.  bf16, head dim 128,
-// keys of 2000 positions in front, widened against row tiles: 592 sequences of one token with 64 / 8 heads 3037 us against 983,
+// keys of 2000 positions in front, widened against row tiles: 592 sequences of one token with 64 / 8 heads 3037 us against 578,
 // 74 of 8 tokens (64 rows) 399 against 261, 37 of 16 (128 rows) 209 against 250, 10 of 64 137 against 269; 32 / 2 heads, 8 tokens
 // (128 rows) 224 against 265, 4 tokens 428 against 284; 8 / 8 heads, 128 tokens 226 against 277, 64 tokens 420 against 276.
 // Behind 8000 keys the two meet at 128 rows (721 and 755).  One sequence of many tokens among others of one (64 / 8 heads): 100

@@ -1,5 +1,5 @@
-"""The packed prefill over an 8-bit cache on its widening path: the pages that the tokens see widened in the workspace and given to the
-tensor-core prefill.  Small calls are sent there with DVATTN_PREFILL=1, and the workspace's size shows that they went."""
+"""Which way the packed prefill over an 8-bit cache takes, and its widening path: the pages that the tokens see widened in the workspace
+and given to the tensor-core prefill.  Small calls are sent there with DVATTN_PREFILL=1, and the workspace's size shows that they went."""
 import pytest
 import torch
 
@@ -88,3 +88,13 @@ def test_rows_of_a_sequence_decide(dtype, new, widens):
     assert (pages <= size < pages + (1 << 20)) == widens
     out, lse = q8.call_varlen(d)
     q8.close(c, out, lse, *plain_q8.varlen(c), wide=widens)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("E,Hq,Hkv", [(64, 16, 2), (128, 16, 1), (128, 15, 3), (256, 8, 8)])
+@pytest.mark.parametrize("new", [[1] * 70, [0, 1, 0, 0, 1], [1] * 40 + [25], [2] * 9 + [1]])
+def test_few_rows_of_a_sequence(dtype, E, Hq, Hkv, new):
+    """Packed sequences of 16 query rows or fewer on average: tiles of 16 rows, a chunk's and a single token's."""
+    c = q8.make_varlen([[17 * w % 90, w % 3] for w in range(len(new))], new, Hq, Hkv, E, 32, 16, dtype, seed=E + len(new))
+    out, lse = q8.call_varlen(q8.on_gpu(c))
+    q8.close(c, out, lse, *plain_q8.varlen(c))
