@@ -138,6 +138,10 @@ template <class T> __global__ void __launch_bounds__(256) widen_kernel(WidenPara
 
 constexpr int kWidenRows = 128;  // query rows of a sequence and KV head, on average, from which pages are widened (file comment)
 
+// Bytes of widened pages that a call asks for at most: the pages of the pool, or of the batch's tables, take up to twice the pool's bytes,
+// seen or not, which a GPU that a large pool fills does not have.  Calls that would need more run on the row tiles, in 256 MB.
+constexpr size_t kMostWidened = 16ull << 30;
+
 size_t up(size_t x) { return (x + 255) / 256 * 256; }
 
 struct WidenLayout {
@@ -157,6 +161,7 @@ bool widen_layout(const dvattn_varlen_args* a, WidenLayout& L) {
     if (!prefill_eligible(&L.wide)) return false;
     L.own = prefill_workspace_size(&L.wide);
     const size_t cache = (size_t)L.pages * a->block_size * a->Hkv * a->E * 2;
+    if (2 * cache > kMostWidened) return false;
     L.span = up(L.own);
     L.table = L.span + up(4 * (size_t)a->W * a->F);
     L.wk = L.table + (L.own_table ? up(4 * (size_t)mine) : 0);

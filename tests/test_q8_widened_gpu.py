@@ -6,6 +6,7 @@ import torch
 import dvattn_b200
 import plain_q8
 import test_q8_gpu as q8
+import test_q8_limits_gpu as limits
 from dvattn_b200 import capi
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +99,37 @@ def test_few_rows_of_a_sequence(dtype, E, Hq, Hkv, new):
     c = q8.make_varlen([[17 * w % 90, w % 3] for w in range(len(new))], new, Hq, Hkv, E, 32, 16, dtype, seed=E + len(new))
     out, lse = q8.call_varlen(q8.on_gpu(c))
     q8.close(c, out, lse, *plain_q8.varlen(c))
+
+
+def far(c, pages, maxb):
+    """The call (two turns, of which the first is not seen) with its last turn at the end of tables of `maxb` entries, its pages at the
+    top of a pool of `pages`."""
+    h = limits.high(c, pages)
+    BS, W = c["kc"].size(1), c["bt"].size(0)
+    n = c["bt"].size(1)
+    maxb -= (maxb - n) * BS % 128 // BS  # windows begin at the same places
+    bt = torch.full((W, maxb), -1, dtype=torch.int32, device=DEV)
+    bt[:, maxb - n:] = h["bt"]
+    L = c["L"].clone()
+    L[0] += (maxb - n) * BS
+    return dict(h, bt=bt, L=L)
+
+
+def two_turns(dtype, seed=0):
+    """Two sequences of two turns, the first of them unseen."""
+    c = q8.make_varlen([[32, 45], [32, 120]], [9, 30], 8, 2, 128, 32, 16, dtype, seed=seed)
+    c["loc"][0] = -1
+    return c
+
+
+def test_most_bytes_of_widened_pages(widened, monkeypatch):
+    """A pool whose widened pages would take more than 16 GB: the call runs on the row tiles, in a small workspace."""
+    c = q8.on_gpu(two_turns(F16))
+    pages = (1 << 32) // (16 * 2 * 128) + 500
+    d = far(c, pages, pages)
+    size, widened_bytes = workspace(d)
+    assert size < 1 << 28 and widened_bytes > 16 << 30
+    got = q8.call_varlen(d)
+    monkeypatch.setenv("DVATTN_PREFILL", "0")
+    want = q8.call_varlen(c)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
