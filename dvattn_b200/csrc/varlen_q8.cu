@@ -159,6 +159,7 @@ bool widen_layout(const dvattn_varlen_args* a, WidenLayout& L) {
     L.wide = *a;
     L.wide.num_blocks = L.pages;
     if (!prefill_eligible(&L.wide)) return false;
+    if ((long long)a->max_blocks_per_seq * a->block_size > kMostPositions) return false;  // windows there pass 32 bits in the prefill
     L.own = prefill_workspace_size(&L.wide);
     const size_t cache = (size_t)L.pages * a->block_size * a->Hkv * a->E * 2;
     if (2 * cache > kMostWidened) return false;

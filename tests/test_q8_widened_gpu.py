@@ -133,3 +133,21 @@ def test_most_bytes_of_widened_pages(widened, monkeypatch):
     monkeypatch.setenv("DVATTN_PREFILL", "0")
     want = q8.call_varlen(c)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_last_positions_of_32_bits(widened, monkeypatch):
+    """A table of 2^31 positions: those up to 2^31 - 256 are seen, as in the other calls over such a cache."""
+    c = q8.make_varlen([[112, 144]], [5], 8, 2, 128, 32, 128, BF16)
+    c["loc"][0], c["loc"][1] = -1, torch.tensor([10, 143, 200, 299, 500], dtype=torch.int32)
+    c["bt"] = c["bt"][:, :2].contiguous()
+    c["L"][1] = 300
+    d = q8.on_gpu(c)
+    bt = torch.full((1, 1 << 24), -1, dtype=torch.int32, device=DEV)
+    bt[0, -4:-2] = d["bt"][0]
+    bt[0, -2:] = d["bt"][0]  # positions that are not seen
+    big = dict(d, bt=bt, L=d["L"] + torch.tensor([(1 << 31) - 512, 0], dtype=torch.int32, device=DEV))
+    got = q8.call_varlen(big)
+    q8.close(c, *got, *plain_q8.varlen(c))
+    monkeypatch.setenv("DVATTN_PREFILL", "0")
+    want = q8.call_varlen(big)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
