@@ -40,14 +40,14 @@
 namespace dvb {
 
 struct Q8Params : TurnSplit {
-    // of TurnSplit: F, BS, maxb, cap, NB, kt, nt, align, loc, L, bt; W: sequences of this launch
-    int w0;                 // its first sequence (packed tokens: its first tile)
+    // of TurnSplit: F, BS, maxb, cap, NB, kt, nt, align, loc, L, bt
+    int first;              // the launch's first pair of all
     int Hq, Hkv, G, S, R, rows;
     int angles;             // entries of a row of cos / sin
     const int* cu;          // packed tokens: where the sequences begin, [nseq + 1]; null: S tokens of each
     int nseq;
     int hc, hs;             // KV heads a CTA reads together, groups of them (hc * hs = Hkv)
-    int pairs;              // (sequence, row tile) pairs: W * nt, packed tokens: tiles, some of them empty
+    int pairs;              // (sequence, row tile) pairs of the launch, packed tokens: tiles, some of them empty
     int box, box_shift;     // rows of a TMA box (gathered: rows of the stage), its log2
     int bs_shift;           // log2 of the page size, -1: it is no power of two
     long long tokens;       // all sequences' (a turn's stride in loc and cos / sin)
@@ -74,7 +74,8 @@ struct Q8Params : TurnSplit {
 };
 
 constexpr int kQ8Warps = 4;
-constexpr int kQ8MaxPairs = 2048;  // their prefix sums lie in the stages at first
+constexpr int kQ8MaxPairs = 2048;  // of a launch: their prefix sums lie in the stages at first
+constexpr long long kQ8Fragments = 256LL << 20;  // bytes of rotated queries in the workspace, at most (q8_layout)
 // A turn's start (a partial window, its rotated queries, the look-up of its keys) and a piece's end cost about as much as this
 // many windows: the split counts them.  96 sequences of 1 to 4 turns, head dim 256: 95.8 us (counted as nothing 107, as eight
 // windows 98.2 to 99.4); 32 sequences of two turns 53.4 (four windows 54.5, twelve 54.2).
@@ -143,11 +144,11 @@ __device__ __forceinline__ int packed_start(const Q8Params& p, int w) {
 // Packed: sequence w's tiles are those from floor(first row / size) + w on, which leaves room for them all.
 // PACKED: a template argument throughout, since the search below in every kernel's start costs a call of the other kind 1 to 3 us.
 template <bool PACKED> __device__ __forceinline__ Q8Tile tile_of(const Q8Params& p, int size, int pair) {
+    const int x = p.first + pair;
     if constexpr (!PACKED) {
-        const int w = p.w0 + pair / p.nt;
-        return {w, pair % p.nt, w * p.S, p.rows};
+        const int w = x / p.nt;
+        return {w, x - w * p.nt, w * p.S, p.rows};
     }
-    const int x = p.w0 + pair;
     int w = 0, hi = p.nseq;
     while (w < hi) {
         const int mid = (w + hi + 1) >> 1;
@@ -517,7 +518,7 @@ __global__ void __launch_bounds__((Q8Cfg<T, E, MT, GATHER>::THREADS), (Q8Cfg<T, 
     const int c = blockIdx.x;
     const bool aligned = (s0 & 1023) == 0;  // as the swizzle needs the stages
     // cleared once per call: a bounded wait that gives up sets its bit long after
-    if (c == 0 && tid == 0 && (p.w0 == 0 || !aligned)) p.header[3] = aligned ? 0 : 4;
+    if (c == 0 && tid == 0 && (p.first == 0 || !aligned)) p.header[3] = aligned ? 0 : 4;
     if (!aligned) return;
     // ---- the split: every CTA adds up the windows and units of all pairs and finds its own range ----
     long long* sP = reinterpret_cast<long long*>(smem);  // [pairs + 1] windows in front of a pair, in the stages
@@ -1307,8 +1308,8 @@ template <bool PACKED> Q8Kernel q8_pick(int dtype, int E, int rows) {
 
 struct Q8Layout {
     size_t P, cstart, qf, ql, po, pl, total;
-    int ctas, hc, nt, slice;  // slice: sequences of a launch (packed: tiles)
-    int items;                // sequences (packed: tiles) of all
+    int ctas, hc, nt, slice;  // slice: (sequence, row tile) pairs of a launch
+    int items;                // of all
 };
 // Packed tokens: nseq sequences that begin at cu; `a` is the call with a token for a sequence.
 struct Q8Packed {
@@ -1332,12 +1333,11 @@ int q8_layout(const dvattn_paged_args* a, const Q8Packed* pk, const Q8Kernel& k,
     L.ctas = sms * k.ctas < kQ8MaxCtas ? sms * k.ctas : kQ8MaxCtas;
     L.hc = a->Hkv % 4 == 0 && k.heads == 4 ? 4 : a->Hkv % 2 == 0 ? 2 : 1;
     L.nt = pk ? 1 : (a->S * (a->Hq / a->Hkv) + k.rows - 1) / k.rows;
-    L.items = pk ? (int)((long long)a->W * (a->Hq / a->Hkv) / k.rows) + pk->nseq + 1 : a->W;
-    L.slice = kQ8MaxPairs / L.nt;
-    if (pk) {  // 256 MB of fragments are enough to keep the GPU busy
-        const long long fit = (256LL << 20) / ((long long)(a->F > 0 ? a->F : 1) * a->Hkv * k.qhead);
-        if (L.slice > fit) L.slice = fit > 64 ? (int)fit : 64;
-    }
+    L.items = pk ? (int)((long long)a->W * (a->Hq / a->Hkv) / k.rows) + pk->nseq + 1 : a->W * L.nt;
+    // 256 MB of fragments (one pair's, where that is more) keep the GPU busy: writing and reading them takes five times a launch's ends
+    const long long fit = kQ8Fragments / ((long long)(a->F > 0 ? a->F : 1) * (a->Hkv * (long long)k.qhead + k.lims));
+    L.slice = fit < 1 ? 1 : fit < kQ8MaxPairs ? (int)fit : kQ8MaxPairs;
+    if (L.slice > L.nt) L.slice -= L.slice % L.nt;
     if (L.slice > L.items) L.slice = L.items;
     size_t at = 256;
     auto take = [&](size_t bytes) {
@@ -1345,10 +1345,10 @@ int q8_layout(const dvattn_paged_args* a, const Q8Packed* pk, const Q8Kernel& k,
         at += (bytes + 255) / 256 * 256;
         return r;
     };
-    L.P = take(8 * ((size_t)L.slice * L.nt + 1));
+    L.P = take(8 * ((size_t)L.slice + 1));
     L.cstart = take(8 * ((size_t)L.ctas + 1));
-    L.qf = take((size_t)a->F * L.slice * L.nt * a->Hkv * k.qhead);
-    L.ql = take((size_t)a->F * L.slice * L.nt * k.lims);
+    L.qf = take((size_t)a->F * L.slice * a->Hkv * k.qhead);
+    L.ql = take((size_t)a->F * L.slice * k.lims);
     L.po = take(4 * (size_t)L.ctas * 2 * L.hc * k.rows * a->E);
     L.pl = take(8 * (size_t)L.ctas * 2 * L.hc * k.rows);
     L.total = at;
@@ -1360,8 +1360,8 @@ int q8_validate(const dvattn_paged_args* a) {
     if (st != DVATTN_OK) return st;
     const long long rows = (long long)a->S * (a->Hq / a->Hkv);  // packed: of a token
     if (a->num_blocks < 0) return DVATTN_ERR_INVALID_ARGUMENT;
-    // a sequence's row tiles are one launch's
-    if (rows > 16LL * kQ8MaxPairs || (long long)a->F * a->W * a->S > 0x7fffffffLL || (long long)kQ8MaxPairs * a->Hkv * (a->F > 0 ? a->F : 1) > 0x7fffffffLL)
+    // rows of a sequence; (turn, token)s, as many as row tiles or more; blocks of a launch
+    if (rows > 32768 || (long long)(a->F > 0 ? a->F : 1) * a->W * a->S > 0x7fffffffLL || (long long)kQ8MaxPairs * a->Hkv * (a->F > 0 ? a->F : 1) > 0x7fffffffLL)
         return DVATTN_ERR_UNSUPPORTED;
     return DVATTN_OK;
 }
@@ -1467,10 +1467,9 @@ static int q8_launch(const dvattn_paged_args* a, const Q8Packed* pk, const dvatt
     cfg.numAttrs = 1;
     cfg.stream = stream;
     cudaError_t e = cudaSuccess;
-    for (int w = 0; w < L.items && e == cudaSuccess; w += L.slice) {
-        p.w0 = w;
-        p.W = L.items - w < L.slice ? L.items - w : L.slice;
-        p.pairs = p.W * p.nt;
+    for (long long x = 0; x < L.items && e == cudaSuccess; x += L.slice) {
+        p.first = (int)x;
+        p.pairs = L.items - p.first < L.slice ? L.items - p.first : L.slice;
         int rows = k.rows, ctas = L.ctas;
         void* rargs[] = {&p, &qf, &ql};
         cfg.gridDim = dim3((unsigned)((long long)a->F * p.pairs * a->Hkv));

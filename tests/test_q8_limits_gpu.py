@@ -6,6 +6,7 @@ import torch
 import dvattn_b200
 import plain_q8
 import test_q8_gpu as q8
+from dvattn_b200 import capi
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -243,3 +244,36 @@ def test_pages_of_blocks_without_sequences(W):
         assert torch.equal(bt.cpu(), ref[0]) and int(count) == ref[1] and torch.equal(granted.cpu(), ref[2])
         dvattn_b200.dvattn_release_pages(bt, free, count, zero, BS)
         assert torch.equal(bt, before[0]) and torch.equal(count, before[2]) and torch.equal(free, before[1])
+
+
+def paged_workspace(c):
+    a = capi.paged_args(c["q"], c["scale"], c["loc"], c["q"], c["cos"], c["sin"], c["L"], c["kc"], c["vc"], c["bt"])
+    return capi.lib().dvattn_paged_sdpa_q8_workspace_size(a)
+
+
+def varlen_workspace(c):
+    a = capi.varlen_args(c["q"], c["scale"], c["loc"], c["q"], c["cos"], c["sin"], c["L"], c["kc"], c["vc"], c["bt"], c["cu"])
+    return capi.lib().dvattn_varlen_paged_sdpa_q8_workspace_size(a)
+
+
+def test_most_bytes_of_rotated_queries():
+    """256 MB of rotated queries and what else a workspace holds (partial results of all CTAs: under 64 MB), however large the call: a
+    sequence's row tiles, and the packed tokens', go to as many launches as that takes."""
+    c = q8.make([[40, 7, 0, 30], [3, 50, 20, 1]], 600, 128, 8, 256, 32, 16, F32)
+    d = q8.on_gpu(c)
+    assert 600 * 2 * 4 * 8 * 16448 > 512 << 20 and 256 << 20 < paged_workspace(d) < 320 << 20
+    out, lse = q8.call(d)
+    q8.close(c, out, lse, *plain_q8.paged(c))
+    turns = [[(w + f) % 4 for f in range(64)] for w in range(3)]
+    c = q8.make_varlen(turns, [300, 1, 400], 8, 8, 256, 32, 16, F32)
+    d = q8.on_gpu(c)
+    assert 256 << 20 < varlen_workspace(d) < 320 << 20
+    out, lse = q8.call_varlen(d)
+    q8.close(c, out, lse, *plain_q8.varlen(c))
+    # sizes that are not run: 2048 tokens of a sequence, 4 turns; one row tile of 4096 turns is more than 256 MB
+    a = capi.PagedArgs()
+    for k, v in dict(dtype=capi.DVATTN_FLOAT32, F=4, W=2, Hq=128, Hkv=8, E=256, Ev=256, S=2048, R=32, block_size=16, max_blocks_per_seq=8, num_blocks=8).items():
+        setattr(a, k, v)
+    assert 0 < capi.lib().dvattn_paged_sdpa_q8_workspace_size(a) < 320 << 20
+    a.F, a.S = 4096, 1
+    assert 4096 * 8 * 16448 < capi.lib().dvattn_paged_sdpa_q8_workspace_size(a) < 4096 * 8 * 16448 + (64 << 20)
