@@ -277,3 +277,14 @@ def test_most_bytes_of_rotated_queries():
     assert 0 < capi.lib().dvattn_paged_sdpa_q8_workspace_size(a) < 320 << 20
     a.F, a.S = 4096, 1
     assert 4096 * 8 * 16448 < capi.lib().dvattn_paged_sdpa_q8_workspace_size(a) < 4096 * 8 * 16448 + (64 << 20)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("E", [64, 128, 256])
+def test_value_scales_as_far_apart_as_they_may_be(dtype, E):
+    """Scales of V 2^100 apart in one sequence and head, the least that the append writes among them: the keys of every page count."""
+    c = q8.make([[300, 40], [5000, 3]], 2, 8, 2, E, 32, 16, dtype)
+    c["vs"][::2], c["vs"][1::2] = 2.0 ** -60, 2.0 ** 40
+    q8.check(c)
+    c["vs"][:], c["vs"][c["bt"][0, 3]] = 2.0 ** 26, 2.0 ** 126 / 448
+    q8.check(c)
