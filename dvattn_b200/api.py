@@ -238,9 +238,9 @@ def dvattn_varlen_paged_sdpa_q8(queries: torch.Tensor, locations: torch.Tensor, 
                                 lse: Optional[torch.Tensor] = None,
                                 out_f32: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``dvattn_varlen_paged_sdpa`` over a cache held in 8 bits (``dvattn_paged_sdpa_q8``).  Calls
-    for the tensor-core prefill (16-bit, E = 128, enough tokens) widen the pages that the tokens see
-    in a workspace of up to min(NB, W * max_blocks) pages of both caches; all others read the cache
-    as it is."""
+    for the tensor-core prefill (16-bit, E = 128, enough tokens in all and 128 query rows of a KV head
+    in a sequence on average) widen the pages that the tokens see in a workspace of up to
+    min(NB, W * max_blocks) pages of both caches, at most 16 GB; all others read the cache as it is."""
     if out is None:
         out = torch.empty((queries.size(0), queries.size(1), v_cache.size(3)), dtype=queries.dtype,
                           device=queries.device)

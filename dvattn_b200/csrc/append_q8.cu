@@ -9,13 +9,14 @@
 //
 // A warp per tile whose groups of 8 elements its lanes can hold (kHeld each, as they are in memory), a block of four warps for
 // larger ones; what a thread cannot hold it reads again (from L1) once the scale is known.  Prompts of up to 2048 tokens of 16
-// sequences in pages of 16 (256 groups a tile), bf16, 2 KV heads of 128: 12.9 us with a warp per tile, 25.6 with a block.
+// sequences in pages of 16 (256 groups a tile), bf16, 2 KV heads of 128: 12.9 us with a warp per tile, 25.6 with a block (replayed
+// from a graph; a call by itself takes 14.3).
 //
 // What bounds it is not HBM (27 MB take 4.2 us) but the length of a tile's chain, position -> page -> scale -> store, and the
 // instructions of the rotation: so a tile's rotating groups come first and its other groups after them, a warp does one or
 // the other, all loads of a thread are under way before the first is used, and maxima are taken of the bits, two elements an
 // operation (non-finite elements have a path of their own).  32 sequences of up to 501 tokens in pages of 64, f16, 8 KV
-// heads, all of 128 dims rotated: 29 us (63 MB), with every head reading the angles again from L2.
+// heads, all of 128 dims rotated: 29 us replayed, 33 by itself (63 MB), with every head reading the angles again from L2.
 #include "decode.cuh"
 #include "q8.cuh"
 #include "tcgen05.cuh"

@@ -11,19 +11,21 @@
 // Numerics.  e4m3 is exact in f16, so K and V are widened to f16 in registers and multiplied on
 // mma.sync with 32-bit accumulation; the scales never touch them.  q's row is multiplied by a power of
 // two that brings its largest element to 2^13 .. 2^14 and written as one f16 value (f16 and bf16 queries:
-// exact, but for elements under 2^-27 of the row's largest) or two (f32: hi + lo, 2^-24 of an
+// exact, but for elements under 2^-27 of the row's largest) or two (f32: hi + lo, within 2^-23 of an
 // element), undone in the scores.  With sv = 2^e m (1 <= m < 2), z = log2-score + e is what the running
 // maximum r is taken over: P = 2^(z - r + 7), the numerator adds (P m) V8, the denominator P 2^-e, both in
 // units of 2^r, so pages of any scales meet in one accumulator.  P m is rounded to f16 (f32: to a hi
 // + lo pair) next to V; the denominator adds the unrounded P.  The 7 powers of two keep weights down to
 // 2^-21 of the largest at full precision and drop those under 2^-32.  r moves when the maximum has grown by
-// more than 6 (P stays below 2^14), so that the accumulators are rarely rescaled.
+// more than 6 (P stays below 2^14), so that the accumulators are rarely rescaled.  Values' scales that a row sees have to lie within
+// 2^100 of one another: further below the largest, P of a key falls under the least 32-bit number, though P 2^-e would count.
 //
-// Bound: HBM has a byte per cached element to bring, but a byte is also a conversion and products of tensor cores that take
-// K and V in 16 bits: 128 heads over 4 x 65k to 131k keys (843 MB) take 170 us, 76% of the copy bandwidth.  With eight
-// computing warps an SM (190 us) the issue slots were 37% and the tensor cores 28% busy, a warp waiting 7 cycles from
-// instruction to instruction: twelve is what the registers hold.  8-bit products would need no conversion, but mma.sync of
-// e4m3 takes 22 cycles an instruction here against 8 of f16.
+// Bound (times of calls replayed from a graph): HBM has a byte per cached element to bring.  128 heads over 4 x 65k to 131k keys
+// (843 MB) take 162 us, 80% of the copy bandwidth (a call by itself, on inputs that are not in L2, 180); without any products,
+// only windows requested and handed back, it is 151.  The rest is that a byte is also a conversion and products of tensor cores that
+// take K and V in 16 bits.  With eight computing warps an SM (190 us) the issue slots were 37% and the tensor cores 28% busy, a warp
+// waiting 7 cycles from instruction to instruction: twelve is what the registers hold.  8-bit products would need no conversion, but a
+// query would be a sum of e4m3 terms, and one e4m3 mma.sync takes 22 cycles here, the two of f16 that are as deep 20.
 // A CTA reads a page's rows of two or four KV heads together (contiguous in HBM) by TMA; a warp works on 16 keys of one
 // head.  With 32 keys a warp waits less often but needs more registers, and a range ends further from its share: 32 sequences of
 // 64 / 4 heads, bf16, 64.2 us against 57.5; head dim 64, chunks of 5 tokens 82 against 61 (both with two CTAs an SM).
@@ -477,8 +479,7 @@ __device__ __forceinline__ float log_sum(float m, float sum) {
 // Fragments.  The order of the elements in q . k and of the keys in P V is free as long as both operands
 // share it:
 // * K comes in 16-byte words: thread (n, t) takes chunks t + 4i of the rows of its columns n and widens each 32-bit word to a
-//   fragment.  (8-bit products would take K as it is, but mma.sync of e4m3 takes 22 cycles an instruction here, more than the
-//   f16 ones and the widening.)
+//   fragment.  (8-bit products would take K as it is, at the file comment's cost.)
 // * V comes by transposing 8-bit matrix loads: thread (n, t) gets, of column n, the keys of rows 4t .. 4t + 3, and
 //   widens them in pairs to a fragment.  So the scores that a thread holds have to be those of these four keys: of 16 keys,
 //   key(t, j) = 8 (t / 2) + 2 (t % 2) + j / 2 + 4 (j % 2) for tile j / 2, column 2t + j % 2.  Neighbouring columns lie four rows

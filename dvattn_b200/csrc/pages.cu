@@ -10,9 +10,9 @@
 // Bound: the launch, the cluster's barriers, and the walks' instructions on 8 SMs.  So a walk over long rows (from 32
 // entries a sequence on average, or one sequence's) goes row by row, 32 entries a load, and only short rows are packed 32 to a
 // load with a search for each entry's owner; and the second walk ends behind the warp's last entry that moves.  Released
-// and assigned, B200: 256 sequences with tables of 2001 pages, one token each, 26.7 us (48.5 with the search alone, of which
-// the release's look at 512,256 entries took 39 and takes 11.6); 48 prompts of up to 32,000 tokens 34 us (91).  A cluster of
-// 16 blocks takes a tenth less but may not be launchable.
+// and assigned, B200, replayed from a graph: 256 sequences with tables of 2001 pages, one token each, 26.7 us (48.5 with the search
+// alone, of which the release's look at 512,256 entries took 39 and takes 11.6; calls by themselves 30.7); 48 prompts of up to 32,000
+// tokens 34 us (91; by themselves 41.0).  A cluster of 16 blocks takes a tenth less but may not be launchable.
 #include "decode.cuh"
 
 #include <cooperative_groups.h>

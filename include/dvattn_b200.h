@@ -295,7 +295,9 @@ typedef struct dvattn_evict_args {
  * [NB,BS,Hkv,Ev] hold one byte per element, an e4m3 value (OCP FP8: largest 448, 0x7f / 0xff NaN, no
  * infinities) that stands for itself times the scale of its page and KV head.  Scales of pages that
  * hold keys are positive; between 2^-60 and 2^126 they are taken as they are, smaller ones may lose bits
- * of small weights.  The append writes powers of two.
+ * of small weights.  The v_scales of a head that one token sees lie within 2^100 of one another (those that
+ * the append sets do for values up to 2^48): keys of the smallest may lose their weight otherwise.  The
+ * append writes powers of two.
  */
 typedef struct dvattn_q8_scales {
     float* k_scales;              /* [NB,Hkv] f32; only the append writes them            */
@@ -504,14 +506,17 @@ int dvattn_paged_evict(const dvattn_evict_args* args, void* workspace, size_t wo
  *
  * dvattn_paged_sdpa_q8: dvattn_paged_sdpa over such a cache (dtype is the queries' and the
  * output's); the S tokens of a sequence share the reading of its keys.  Workspace and status as
- * there.  What lies in a key or value reaches the tokens that see it and no other, NaN too.
+ * there (at most about 256 MB of rotated queries, or one row tile's: 16 or 32 rows of every turn).  What
+ * lies in a key or value reaches the tokens that see it and no other, NaN too.
  *
  * dvattn_varlen_paged_sdpa_q8: dvattn_varlen_paged_sdpa over such a cache; tokens and cu_seqlens_q (in
- * order) are treated as there.  Where the 16-bit call would take its tensor-core prefill, the pages that the
- * tokens see are widened to dtype in the workspace (min(num_blocks, W * max_blocks) pages of both caches)
- * and it runs over them; then a NaN or infinity in a page may reach other tokens of its sequence, as in
- * that prefill.  Other calls read the cache as it is, in row tiles of the packed tokens (workspace: at most
- * about 256 MB of rotated queries).
+ * order) are treated as there.  Where the 16-bit call would take its tensor-core prefill and a sequence has
+ * 128 query rows of a KV head or more on average (T * Hq / Hkv >= 128 W), the pages that the tokens see are
+ * widened to dtype in the workspace (min(num_blocks, W * max_blocks) pages of both caches, 16 GB at most) and it
+ * runs over them.  Then weights are rounded to dtype next to V; value * scale is rounded to dtype where the scale
+ * is no power of two, and in f16 taken for 65504 where it is larger; and a NaN or infinity in a page may reach
+ * other tokens of its sequence, as in that prefill.  Other calls read the cache as it is, in row tiles of the
+ * packed tokens (weights in f16, of f32 queries in a pair of them; workspace as above).
  *
  * dvattn_paged_append_q8: dvattn_paged_append into such a cache.  Keys (rotated, rounded to dtype) and
  * values x of a page and head are stored as e4m3(x / s), to nearest even, with s the page's scale: the
@@ -531,8 +536,9 @@ int dvattn_paged_append_q8(const dvattn_append_args* args, const dvattn_q8_scale
 
 /*
  * Block tables and slot maps on the GPU, from request lengths and a free list: pages for a step's new
- * tokens, and pages back.  Both are one launch and may be captured in a graph.  No counterpart in the
- * reference, whose callers keep their tables on the host.
+ * tokens, and pages back.  Both are one launch, but for slot maps of more than 32768 entries, which are
+ * written by a launch of their own (one for every 65535 sequences), and may be captured in a graph.  Tables have
+ * fewer than 2^31 - 1024 entries.  No counterpart in the reference, whose callers keep their tables on the host.
  */
 int dvattn_assign_pages(const dvattn_assign_args* args, dvattn_stream_t stream);
 int dvattn_release_pages(const dvattn_release_args* args, dvattn_stream_t stream);
